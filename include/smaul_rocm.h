@@ -481,6 +481,85 @@ int smaul_swiglu_backward(const void* dout, const void* g, const void* u, void* 
                           hipStream_t stream);
 
 /*
+ * Routing to experts from the router's logits (no counterpart in the reference,
+ * whose router is the softmax top-k of smaul_moe_router):
+ *   s = softmax(logits) or sigmoid(logits); c = s + bias (bias fp32 [E] or NULL);
+ *   a group's (E / groups consecutive experts) score is the sum of its group_best
+ *   (1 or 2) highest c, or its highest where it has one; of the top_groups best
+ *   groups the k experts with the highest c, descending; ties, of groups too, to
+ *   the lowest index.  Without a bias experts are ordered by their logits.
+ *   topw = s of the chosen (without the bias); renorm: over their sum (1 / n of the
+ *   n chosen where the sum is below 1e-6); times scale.
+ * An expert with a logit of -inf, or whose c is -inf or NaN, is not chosen; a slot
+ * that no expert fills has topi -1 and topw 0 (smaul_moe_dispatch drops it).
+ * logits: dtype [T, E]; prob fp32 [T, E] (s) or NULL; topi int64 [T, k]; topw fp32
+ * [T, k].  E <= 512, k <= 16, groups <= 64 (a divisor of E), and top_groups groups
+ * hold at least k experts.  The choice is that of scores in 64 bits.
+ */
+enum { SMAUL_SCORE_SOFTMAX = 0, SMAUL_SCORE_SIGMOID = 1 };
+int smaul_moe_route(const void* logits, int dtype, const float* bias, float* prob, int64_t* topi, float* topw,
+                    int64_t T, int64_t E, int64_t k, int score, int64_t groups, int64_t top_groups, int group_best,
+                    int renorm, float scale, hipStream_t stream);
+
+/*
+ * Gradient of smaul_moe_route in the logits, from those of topw (fp32 [T, k]) and of
+ * prob (fp32 [T, E] or NULL), with the choice topi as a constant.  A slot of -1
+ * gives nothing, whatever dtopw holds there; a row renormalised to 1 / n neither.
+ * dlogits is of the logits' dtype.
+ */
+int smaul_moe_route_backward(const float* dtopw, const void* logits, int dtype, const int64_t* topi,
+                             const float* dprob, void* dlogits, int64_t T, int64_t E, int64_t k, int score,
+                             int renorm, float scale, hipStream_t stream);
+
+/*
+ * Microscaled 4-bit floating point (no counterpart in the reference).  A row of K
+ * values is n = ceil(K / 32) blocks: codes uint8 [rows, 16 n], value 2 j of a block in
+ * the low half of its byte j, scales uint8 [rows, n].  A code is E2M1 ({0, .5, 1, 1.5,
+ * 2, 3, 4, 6} by its low 3 bits, bit 3 the sign), a scale E8M0 (2^(byte - 127), 255
+ * NaN).  Quantisation: 2^(floor(log2(largest magnitude)) - 2), at least 2^-127; values
+ * to nearest, ties to the even code, past 6 to 6; a block that holds an infinity or
+ * NaN is all NaN.  Values past K are code 0.  x and y: dtype (f32 or bf16) [rows, K];
+ * any K >= 1; codes 4-byte aligned.
+ */
+int smaul_mx4_quantize(const void* x, int dtype, uint8_t* codes, uint8_t* scales, int64_t rows, int64_t K,
+                       hipStream_t stream);
+int smaul_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* y, int dtype, int64_t rows, int64_t K,
+                         hipStream_t stream);
+
+/*
+ * y[rows, out_f] = x[rows, in_f] . decode(w, s)^T, w and s [out_f, in_f] in that format
+ * (w 16-byte aligned), x and y of dtype.  SMAUL_ACT_KEEP multiplies x as it is (fp32 as
+ * two bf16 terms, within 2^-17 of each value), SMAUL_ACT_MX4 rounds its rows to the
+ * format first, in the workspace; sums are fp32.
+ */
+enum { SMAUL_ACT_KEEP = 0, SMAUL_ACT_MX4 = 1 };
+int64_t smaul_mx4_linear_workspace_size(int64_t rows, int64_t in_f, int64_t out_f, int act);
+int smaul_mx4_linear(const void* x, int dtype, const uint8_t* w, const uint8_t* s, void* y, int64_t rows,
+                     int64_t in_f, int64_t out_f, int act, void* workspace, int64_t workspace_bytes,
+                     hipStream_t stream);
+
+/* dx[rows, in_f] = g[rows, out_f] . decode(w, s): its input gradient (x as it is), g and dx of dtype. */
+int smaul_mx4_backward_input(const void* g, int dtype, const uint8_t* w, const uint8_t* s, void* dx, int64_t rows,
+                             int64_t in_f, int64_t out_f, hipStream_t stream);
+
+/*
+ * The routed SwiGLU experts in that format: out[t] = sum over t's slots, ascending
+ * expert, of topw * (hdn . Wd^T), hdn = silu(x . Wg^T) * (x . Wu^T).  Weights of all
+ * experts one after the other: gate_w / up_w [E, h, d], down_w [E, d, h] (codes,
+ * 16-byte aligned) with their scales.  SMAUL_ACT_KEEP: hdn and the slots' outputs are
+ * rounded to dtype; SMAUL_ACT_MX4 (bf16 x): x and hdn (from fp32) are rounded to the
+ * format, the outputs to bf16.  Slots with topi outside [0, E) or topw not above 0 add
+ * nothing.  counts int32 [E] (rows of each expert).  d a multiple of 8, E <= 64,
+ * k <= min(E, 8); workspace 256-byte aligned.  T == 0 writes nothing.
+ */
+int64_t smaul_mx4_moe_workspace_size(int64_t T, int64_t d, int64_t h, int64_t E, int64_t k, int dtype, int act);
+int smaul_mx4_moe_forward(const void* x, int dtype, const int64_t* topi, const float* topw, const uint8_t* gate_w,
+                          const uint8_t* gate_s, const uint8_t* up_w, const uint8_t* up_s, const uint8_t* down_w,
+                          const uint8_t* down_s, void* out, int32_t* counts, int64_t T, int64_t d, int64_t h,
+                          int64_t E, int64_t k, int act, void* workspace, int64_t workspace_bytes,
+                          hipStream_t stream);
+
+/*
  * Measured ceilings for the roofline figures (bench.py --peaks); no
  * counterpart in the reference and not on the MoE path.
  * smaul_peak_mfma: `workgroups` x 4 waves, each issuing `iters` rounds of 8

@@ -22,6 +22,8 @@ DTYPE_BF16 = 1
 FLAG_CANONICAL_CODES = 1
 FLAG_ALIGNED_CODES = 2
 FLAG_TILED_LAYOUT = 4
+SCORES = {"softmax": 0, "sigmoid": 1}
+ACTS = {"keep": 0, "mx4": 1}
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -72,6 +74,15 @@ SIGNATURES = {
     "smaul_swiglu_backward": (_I, [_P, _P, _P, _P, _P, _I64, _I, _P]),
     "smaul_wait_timeouts": (_I, [_P, _I, _P]),
     "smaul_debug_tail_wait": (_I, [_I, _I]),
+    "smaul_moe_route": (_I, [_P, _I, _P, _P, _P, _P, _I64, _I64, _I64, _I, _I64, _I64, _I, _I, ctypes.c_float, _P]),
+    "smaul_moe_route_backward": (_I, [_P, _P, _I, _P, _P, _P, _I64, _I64, _I64, _I, _I, ctypes.c_float, _P]),
+    "smaul_mx4_quantize": (_I, [_P, _I, _P, _P, _I64, _I64, _P]),
+    "smaul_mx4_dequantize": (_I, [_P, _P, _P, _I, _I64, _I64, _P]),
+    "smaul_mx4_linear_workspace_size": (_I64, [_I64, _I64, _I64, _I]),
+    "smaul_mx4_linear": (_I, [_P, _I, _P, _P, _P, _I64, _I64, _I64, _I, _P, _I64, _P]),
+    "smaul_mx4_backward_input": (_I, [_P, _I, _P, _P, _P, _I64, _I64, _I64, _P]),
+    "smaul_mx4_moe_workspace_size": (_I64, [_I64, _I64, _I64, _I64, _I64, _I, _I]),
+    "smaul_mx4_moe_forward": (_I, [_P, _I] + [_P] * 10 + [_I64, _I64, _I64, _I64, _I64, _I, _P, _I64, _P]),
     "smaul_peak_mfma": (_I, [_P, _I, _I, _P]),
     "smaul_peak_stream": (_I, [_P, _I64, _P, _I, _P]),
     "smaul_peak_lds_dma": (_I, [_P, _I64, _P, _I, _I, _P]),

@@ -431,6 +431,226 @@ class RocmBackend:
     def sparse_grad_v(self, dout, x, cols, values, budget=1 << 22):
         raise NotImplementedError("rocm backend: sparse_grad_v is not implemented")
 
+    # ---- routing from logits, and the 4-bit format ---------------------------
+    def moe_route(self, logits, top_k, score="softmax", bias=None, groups=1, top_groups=None, group_best=2,
+                  renorm=True, scale=1.0, need_prob=True):
+        """Routing to experts: (prob [T, E] fp32 or None, topi [T, k] int64, topw [T, k] fp32).
+
+        logits [T, E] fp32 or bf16.  The scores are softmax(logits) or
+        sigmoid(logits) (``score``); the choice goes by score + ``bias`` ([E], for
+        balance): of the ``top_groups`` groups (of ``groups`` equal ones) whose
+        ``group_best`` (1 or 2) highest sum to the most, the ``top_k`` experts with
+        the highest, descending, ties to the lowest index.  ``topw`` is the chosen
+        scores without the bias, over their sum with ``renorm`` (1 / n where the sum
+        is below 1e-6), times ``scale``.  An expert whose logit is -inf is never
+        chosen, nor one whose score or bias is NaN; a slot that no expert fills is
+        -1 with weight 0, which the dispatch drops.  The choice is that of scores
+        in 64 bits.  ``prob`` is the scores, None unless ``need_prob``."""
+        lib = _lib.load()
+        _need_device("moe_route", logits, bias)
+        T, E, top_k = self._route_check("moe_route", logits, top_k, score)
+        groups = int(groups)
+        top_groups = groups if top_groups is None else int(top_groups)
+        if groups < 1 or E % groups or not 1 <= top_groups <= groups or top_groups * (E // groups) < top_k:
+            raise ValueError(f"moe_route: groups must divide the {E} experts and top_groups of them hold {top_k}, got "
+                             f"{groups} and {top_groups}")
+        if group_best not in (1, 2):
+            raise ValueError(f"moe_route: group_best must be 1 or 2, got {group_best!r}")
+        if bias is not None:
+            if bias.numel() != E:
+                raise RuntimeError(f"moe_route: bias must have {E} elements, got {bias.numel()}")
+            bias = bias.detach()
+            if not (bias.dtype == torch.float32 and bias.is_contiguous()):
+                bias = bias.float().contiguous()
+        z = logits if logits.is_contiguous() else logits.contiguous()
+        dev = z.device
+        prob = torch.empty(T, E, dtype=torch.float32, device=dev) if need_prob else None
+        topi = torch.empty(T, top_k, dtype=torch.int64, device=dev)
+        topw = torch.empty(T, top_k, dtype=torch.float32, device=dev)
+        with _device(dev):
+            rc = lib.smaul_moe_route(z.data_ptr(), _ACT[z.dtype], None if bias is None else bias.data_ptr(),
+                                     None if prob is None else prob.data_ptr(), topi.data_ptr(), topw.data_ptr(),
+                                     T, E, top_k, _lib.SCORES[score], groups, top_groups, group_best, int(bool(renorm)),
+                                     float(scale), _stream_handle(dev))
+        _lib.check(rc, "moe_route")
+        return prob, topi, topw
+
+    @staticmethod
+    def _route_check(name, logits, top_k, score):
+        if logits.dtype not in _ACT or logits.dim() != 2:
+            raise RuntimeError(f"{name}: logits must be 2-D float32 or bfloat16, got {logits.dtype} "
+                               f"{tuple(logits.shape)}")
+        if score not in _lib.SCORES:
+            raise ValueError(f"{name}: score must be one of {sorted(_lib.SCORES)}, got {score!r}")
+        T, E = logits.shape
+        if not 1 <= top_k <= E:
+            raise ValueError(f"{name}: top_k must be in [1, {E}], got {top_k}")
+        return T, E, int(top_k)
+
+    def moe_route_backward(self, dtopw, logits, topi, score="softmax", renorm=True, scale=1.0, dprob=None):
+        """The gradient of ``moe_route`` in its logits (their type), from that of topw
+        ([T, k] fp32) and, if given, of prob ([T, E] fp32); the choice ``topi`` is a
+        constant.  A slot of -1 gives none, whatever dtopw holds there."""
+        lib = _lib.load()
+        _need_device("moe_route_backward", logits, dtopw, topi, dprob)
+        T, E, k = self._route_check("moe_route_backward", logits, topi.shape[-1] if topi.dim() else 0, score)
+        for what, t, dtype, shape in (("dtopw", dtopw, torch.float32, (T, k)), ("topi", topi, torch.int64, (T, k)),
+                                      ("dprob", dprob, torch.float32, (T, E))):
+            if t is not None and (t.dtype != dtype or tuple(t.shape) != shape):
+                raise RuntimeError(f"moe_route_backward: {what} must be {dtype} {list(shape)}, got {t.dtype} "
+                                   f"{list(t.shape)}")
+        dtopw, z, topi = (t if t.is_contiguous() else t.contiguous() for t in (dtopw, logits, topi))
+        if dprob is not None and not dprob.is_contiguous():
+            dprob = dprob.contiguous()
+        dz = torch.empty_like(z)
+        with _device(z.device):
+            rc = lib.smaul_moe_route_backward(dtopw.data_ptr(), z.data_ptr(), _ACT[z.dtype], topi.data_ptr(),
+                                              None if dprob is None else dprob.data_ptr(), dz.data_ptr(), T, E, k,
+                                              _lib.SCORES[score], int(bool(renorm)), float(scale),
+                                              _stream_handle(z.device))
+        _lib.check(rc, "moe_route_backward")
+        return dz
+
+    def mx4_quantize(self, x):
+        """(codes uint8 [..., 16 n], scales uint8 [..., n]) of x [..., K] fp32 or bf16, n =
+        ceil(K / 32): blocks of 32 values in 4 bits (E2M1) with a shared power of two
+        (E8M0).  A block that holds an infinity or NaN is all NaN (scale 255)."""
+        lib = _lib.load()
+        _need_device("mx4_quantize", x)
+        if x.dtype not in _ACT or x.dim() < 1 or x.shape[-1] < 1:
+            raise RuntimeError(f"mx4_quantize: x must be float32 or bfloat16 rows, got {x.dtype} {tuple(x.shape)}")
+        K = x.shape[-1]
+        n = (K + 31) // 32
+        xc = x if x.is_contiguous() else x.contiguous()
+        codes = torch.empty(*x.shape[:-1], n * 16, dtype=torch.uint8, device=x.device)
+        scales = torch.empty(*x.shape[:-1], n, dtype=torch.uint8, device=x.device)
+        with _device(x.device):
+            rc = lib.smaul_mx4_quantize(xc.data_ptr(), _ACT[x.dtype], codes.data_ptr(), scales.data_ptr(),
+                                        xc.numel() // K, K, _stream_handle(x.device))
+        _lib.check(rc, "mx4_quantize")
+        return codes, scales
+
+    @staticmethod
+    def _mx4_check(name, codes, scales, lead, K):
+        """The codes and scales [*lead, 16 n] / [*lead, n] of rows of K values, contiguous."""
+        n = (K + 31) // 32
+        for what, t, last in (("codes", codes, n * 16), ("scales", scales, n)):
+            if t.dtype != torch.uint8 or tuple(t.shape) != (*lead, last):
+                raise RuntimeError(f"{name}: {what} must be uint8 {[*lead, last]}, got {t.dtype} {list(t.shape)}")
+        codes = codes if codes.is_contiguous() and codes.data_ptr() % 16 == 0 else codes.clone(
+            memory_format=torch.contiguous_format)
+        return codes, scales if scales.is_contiguous() else scales.contiguous()
+
+    def mx4_dequantize(self, codes, scales, in_f, dtype=torch.float32):
+        """The values [..., in_f] in ``dtype`` (fp32 or bf16, exact in both) that codes
+        [..., 16 n] and scales [..., n] stand for, n = ceil(in_f / 32)."""
+        lib = _lib.load()
+        _need_device("mx4_dequantize", codes, scales)
+        if dtype not in _ACT:
+            raise RuntimeError(f"mx4_dequantize: dtype must be float32 or bfloat16, got {dtype}")
+        if in_f < 1:
+            raise ValueError(f"mx4_dequantize: in_f must be positive, got {in_f}")
+        lead = tuple(codes.shape[:-1])
+        codes, scales = self._mx4_check("mx4_dequantize", codes, scales, lead, in_f)
+        y = torch.empty(*lead, in_f, dtype=dtype, device=codes.device)
+        with _device(codes.device):
+            rc = lib.smaul_mx4_dequantize(codes.data_ptr(), scales.data_ptr(), y.data_ptr(), _ACT[dtype],
+                                          y.numel() // in_f, in_f, _stream_handle(codes.device))
+        _lib.check(rc, "mx4_dequantize")
+        return y
+
+    def mx4_forward(self, x, w, s, in_f, out_f, act="keep"):
+        """y [rows, out_f] = x [rows, in_f] . W^T in x's type (fp32 or bf16), W the weight
+        that codes w [out_f, 16 n] and scales s [out_f, n] stand for (``mx4_quantize``).
+        ``act``: "keep" multiplies x as it is, "mx4" rounds its rows to the format
+        first.  Sums are fp32."""
+        lib = _lib.load()
+        _need_device("mx4_forward", x, w, s)
+        if act not in _lib.ACTS:
+            raise ValueError(f"mx4_forward: act must be one of {sorted(_lib.ACTS)}, got {act!r}")
+        x, w, s = self._mx4_product_check("mx4_forward", "x", x, w, s, in_f, out_f, in_f)
+        rows, a = x.shape[0], _lib.ACTS[act]
+        y = torch.empty(rows, out_f, dtype=x.dtype, device=x.device)
+        nws = lib.smaul_mx4_linear_workspace_size(rows, in_f, out_f, a)
+        ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws > 0 else None
+        with _device(x.device):
+            rc = lib.smaul_mx4_linear(x.data_ptr(), _ACT[x.dtype], w.data_ptr(), s.data_ptr(), y.data_ptr(), rows, in_f,
+                                      out_f, a, None if ws is None else ws.data_ptr(), nws, _stream_handle(x.device))
+        _lib.check(rc, "mx4_forward")
+        return y
+
+    def mx4_backward_input(self, g, w, s, in_f, out_f):
+        """dx [rows, in_f] = g [rows, out_f] . W in g's type (fp32 or bf16): the input
+        gradient of ``mx4_forward`` (act "keep")."""
+        lib = _lib.load()
+        _need_device("mx4_backward_input", g, w, s)
+        g, w, s = self._mx4_product_check("mx4_backward_input", "g", g, w, s, in_f, out_f, out_f)
+        dx = torch.empty(g.shape[0], in_f, dtype=g.dtype, device=g.device)
+        with _device(g.device):
+            rc = lib.smaul_mx4_backward_input(g.data_ptr(), _ACT[g.dtype], w.data_ptr(), s.data_ptr(), dx.data_ptr(),
+                                              g.shape[0], in_f, out_f, _stream_handle(g.device))
+        _lib.check(rc, "mx4_backward_input")
+        return dx
+
+    def _mx4_product_check(self, name, what, x, w, s, in_f, out_f, width):
+        if in_f < 1 or out_f < 1:
+            raise ValueError(f"{name}: in_f/out_f must be positive, got {in_f}/{out_f}")
+        if x.dtype not in _ACT:
+            raise RuntimeError(f"{name}: {what} must be float32 or bfloat16, got {x.dtype}")
+        if x.dim() != 2 or x.shape[1] != width:
+            raise RuntimeError(f"{name}: {what} must be [rows, {width}], got {tuple(x.shape)}")
+        w, s = self._mx4_check(name, w, s, (out_f,), in_f)
+        return x if x.is_contiguous() else x.contiguous(), w, s
+
+    def mx4_moe_forward(self, x, topi, topw, experts, act="keep"):
+        """The routed SwiGLU experts in the 4-bit format: (out [..., d] of x's type,
+        counts [E] int32 on the device).
+
+        x [..., d] fp32 or bf16; topi [..., k] int64 and topw [..., k] fp32 from
+        ``moe_route`` (or ``moe_router``), distinct experts a token; experts:
+        (gate_w, gate_s, up_w, up_s, down_w, down_s), the codes [E, h, 16 n] (gate,
+        up) and [E, d, 16 n] (down) and scales of all experts.  ``act`` "mx4" (bf16 x)
+        rounds the rows of x and the hidden rows to the format, "keep" the hidden
+        rows to x's type.  Slots with topi outside [0, E) or topw not above 0 add
+        nothing."""
+        lib = _lib.load()
+        _need_device("mx4_moe_forward", x, topi, topw, *experts)
+        if act not in _lib.ACTS:
+            raise ValueError(f"mx4_moe_forward: act must be one of {sorted(_lib.ACTS)}, got {act!r}")
+        if x.dtype not in _ACT or x.dim() < 2:
+            raise RuntimeError(f"mx4_moe_forward: x must be float32 or bfloat16 rows, got {x.dtype} {tuple(x.shape)}")
+        if len(experts) != 6 or experts[0].dim() != 3:
+            raise ValueError("mx4_moe_forward: experts is (gate_w, gate_s, up_w, up_s, down_w, down_s) of all experts")
+        d = x.shape[-1]
+        E, h = experts[0].shape[:2]
+        gw, gs = self._mx4_check("mx4_moe_forward: gate", experts[0], experts[1], (E, h), d)
+        uw, us = self._mx4_check("mx4_moe_forward: up", experts[2], experts[3], (E, h), d)
+        dw, dsc = self._mx4_check("mx4_moe_forward: down", experts[4], experts[5], (E, d), h)
+        k = topi.shape[-1]
+        lead = x.shape[:-1]
+        if topi.dtype != torch.int64 or topw.dtype != torch.float32 or tuple(topi.shape) != (*lead, k) or \
+                tuple(topw.shape) != (*lead, k):
+            raise RuntimeError(f"mx4_moe_forward: topi int64 and topw float32 {[*lead, 'k']} expected, got {topi.dtype} "
+                               f"{list(topi.shape)} / {topw.dtype} {list(topw.shape)}")
+        if not 1 <= k <= min(E, 8) or E > 64:
+            raise ValueError(f"mx4_moe_forward: need 1 <= k <= min(E, 8) and E <= 64, got k={k}, E={E}")
+        xc, topi, topw = (t if t.is_contiguous() else t.contiguous() for t in (x, topi, topw))
+        dev, a, dt = x.device, _lib.ACTS[act], _ACT[x.dtype]
+        T = xc.numel() // d
+        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        if T == 0:
+            return out, torch.zeros(E, dtype=torch.int32, device=dev)
+        counts = torch.empty(E, dtype=torch.int32, device=dev)
+        nws = lib.smaul_mx4_moe_workspace_size(T, d, h, E, k, dt, a)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        with _device(dev):
+            rc = lib.smaul_mx4_moe_forward(xc.data_ptr(), dt, topi.data_ptr(), topw.data_ptr(), gw.data_ptr(),
+                                           gs.data_ptr(), uw.data_ptr(), us.data_ptr(), dw.data_ptr(), dsc.data_ptr(),
+                                           out.data_ptr(), counts.data_ptr(), T, d, h, E, k, a, ws.data_ptr(), nws,
+                                           _stream_handle(dev))
+        _lib.check(rc, "mx4_moe_forward")
+        return out, counts
+
     # ---- MoE (model.py:557-585) -------------------------------------------
     def _expert_entry(self, experts: Sequence[Sequence[torch.Tensor]], device, d, h, tile):
         """The repack cache entry of a set of experts: ``table``, a device int64
