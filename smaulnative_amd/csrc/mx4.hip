@@ -8,6 +8,7 @@
 // A code and its scale are exact in bf16, so every product of the matrix cores is
 // exact for bf16 activations and for activations in the format itself, and its
 // sums are fp32; fp32 activations are two bf16 terms (hi + lo).
+#include "lds_dma.h"
 #include "mx4.h"
 
 using smaul::check_launch;
@@ -124,6 +125,7 @@ struct Mx4Args {
   void* y;                 // [rows][N] (O_MX4: codes)
   uint8_t* ys;             // O_MX4: scales
   int64_t R, K, N;
+  int64_t ldx, ldw, ldy;   // row strides of mx4_gemm_kernel: x and y in values (codes: blocks), W in blocks
   const int32_t* seg_off;  // null: dense, R rows of one expert
   const int32_t* tile_off;
   int E;
@@ -290,6 +292,360 @@ int launch_tiles(const Mx4Args& p, int64_t m_tiles, hipStream_t stream) {
   return check_launch("mx4_tile_kernel");
 }
 
+// The kernel of larger calls: K in stages, activations, codes and scales brought to
+// LDS by DMA, NSTAGE stages in flight, 4 waves of half the rows by half the columns.
+//
+// Roles: the weight's rows are the matrix instruction's rows and the activations its
+// columns, and row i of a 32 x 32 tile is given weight row 16 ((i / 4) % 2) + 4 (i / 8)
+// + i % 4, so that the 16 sums of a lane are 16 consecutive outputs of one activation
+// row: they leave as whole 16-byte stores, and a block of the format has its largest
+// value in 15 comparisons and one exchange.
+//
+// A_MX4 runs v_mfma_scale_f32_32x32x64_f8f6f4 on the codes as they are: lane i + 32 g
+// has block g of a 64-wide step of its row, one scale byte for the 32 values.  A stage
+// is 128 wide (64 bytes a row) with four scale bytes a row, a dword.  A_BF16 and A_F32
+// take stages of 64 (128 and 256 bytes a row); a lane's 16 bytes of codes are its block
+// g, decoded to bf16 with their scale (exact), and MFMA step q multiplies values
+// 32 g + 8 q and on.  fp32 activations are three bf16 terms, split after the LDS read.
+template <int AT, int BM, int BN, int NSTAGE>
+struct Mx4Cfg {
+  static constexpr int KS = AT == A_MX4 ? 128 : 64;
+  static constexpr int XROW = AT == A_MX4 ? 64 : AT == A_BF16 ? 128 : 256, WROW = KS / 2;
+  static constexpr int XB = BM * XROW, WB = BN * WROW;
+  static constexpr int SROWS = BN + (AT == A_MX4 ? BM : 0);
+  static constexpr int STAGE = XB + WB + SROWS * 4;
+  static constexpr int X_INS = XB / 4096, W_INS = WB / 4096, S_INS = SROWS / 64;  // DMA instructions: a wave's, all
+  static constexpr int DMA_MIN = X_INS + W_INS + S_INS / 4;
+  static constexpr int TT = BM / 64, WT = BN / 64;  // 32 x 32 tiles of a wave
+  static constexpr int LDS = NSTAGE * STAGE;
+  static_assert(XB % 4096 == 0 && WB % 4096 == 0 && SROWS % 64 == 0, "whole DMA instructions");
+  static_assert(DMA_MIN * (NSTAGE - 2) + 2 < 64 && LDS <= 160 * 1024, "pipeline depth");
+};
+
+// the weight row of row i of a 32-row tile
+__device__ __forceinline__ int mx4_perm(int i) { return ((i >> 2) & 1) * 16 + (i >> 3) * 4 + (i & 3); }
+
+// the chunk swizzle of 32-byte rows (as swz_a and swz_b of the longer ones)
+__device__ __forceinline__ int swz_c(int r) { return ((r >> 2) ^ (r >> 3)) & 1; }
+
+// columns that a product writes: past N zeros, up to the padded row
+template <int OT>
+__host__ __device__ __forceinline__ int64_t mx4_cols(const Mx4Args& p) {
+  const int64_t c = OT == O_MX4 ? p.ldy * MX4_BLOCK : p.ldy;
+  return c > p.N ? c : p.N;
+}
+
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ i32x8_t mx4_operand(uint4 c) {
+  i32x8_t r;  // 32 codes; the instruction reads no more of the eight registers
+  r[0] = (int)c.x; r[1] = (int)c.y; r[2] = (int)c.z; r[3] = (int)c.w;
+  r[4] = r[5] = r[6] = r[7] = 0;
+  return r;
+}
+
+// v = a + b + c in bf16 terms (24 bits)
+__device__ __forceinline__ void mx4_split3(const float (&v)[8], bf16x8_t (&t)[3]) {
+  float r[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = v[j];
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    uint32_t u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      u[j] = pack_bf16(r[2 * j], r[2 * j + 1]);
+      r[2 * j] = r[2 * j] - __uint_as_float(u[j] << 16);
+      r[2 * j + 1] = r[2 * j + 1] - __uint_as_float(u[j] & 0xffff0000u);
+    }
+    t[q] = __builtin_bit_cast(bf16x8_t, make_uint4(u[0], u[1], u[2], u[3]));
+  }
+}
+
+template <int AT, int OT, bool SWIGLU, int BM, int BN, int NSTAGE>
+__global__ void __launch_bounds__(256, 2) mx4_gemm_kernel(Mx4Args p) {
+  using C = Mx4Cfg<AT, BM, BN, NSTAGE>;
+  constexpr int TT = C::TT, WT = C::WT, BNO = SWIGLU ? BN / 2 : BN;
+  __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+
+  // a contiguous band of tiles for each XCD (workgroup b runs on XCD b % 8), in
+  // groups of GM row tiles by all column tiles
+  int mt, nt;
+  {
+    constexpr int GM = 8, NXCD = 8;
+    const int n_tiles = (int)((mx4_cols<OT>(p) + BNO - 1) / BNO), total = gridDim.x, m_tiles = total / n_tiles;
+    int lin = blockIdx.x;
+    const int full = total / NXCD * NXCD;
+    if (lin < full) lin = lin % NXCD * (full / NXCD) + lin / NXCD;
+    const int g = lin / (GM * n_tiles), within = lin - g * GM * n_tiles, gm = min(GM, m_tiles - g * GM);
+    mt = g * GM + within % gm;
+    nt = within / gm;
+  }
+  int e, rows;
+  int64_t row0;
+  if (!mx4_tile<BM>(p, mt, lane, e, row0, rows)) return;
+  const int64_t n0 = (int64_t)nt * BNO;
+  const int64_t ebytes = (int64_t)e * p.N * p.ldw;  // this expert's scales; its codes are 16 times that far
+  const uint8_t* W1 = p.w + ebytes * 16;
+  const uint8_t* S1 = p.s + ebytes;
+  const uint8_t* W2 = SWIGLU ? p.w2 + ebytes * 16 : W1;
+  const uint8_t* S2 = SWIGLU ? p.s2 + ebytes : S1;
+
+  // ---- DMA sources of this lane (32-bit offsets; the host checks the range) ----
+  // Rows past the end read the last one: their sums are not stored.
+  constexpr int XL = C::XROW / 16, XR = 64 / XL;  // lanes a row, rows an instruction
+  uint32_t x_off[C::X_INS];
+#pragma unroll
+  for (int a = 0; a < C::X_INS; ++a) {
+    const int r = (wave * C::X_INS + a) * XR + lane / XL;
+    const int c = AT == A_MX4 ? (lane & 3) ^ swz_b(r) : AT == A_BF16 ? (lane & 7) ^ swz_a(r) : (lane & 15) ^ (r & 15);
+    const int64_t lr = row0 + min(r, rows - 1);
+    const int64_t xr = p.row_idx ? (int64_t)p.row_idx[lr] : lr;
+    x_off[a] = (uint32_t)(xr * p.ldx * (AT == A_MX4 ? 16 : AT == A_BF16 ? 2 : 4) + c * 16);
+  }
+  // staged weight row q: tile q / 32 of the wave halves (gate's, then up's), permuted
+  auto w_row = [&](int q) -> uint32_t {
+    int t = q >> 5;
+    if (SWIGLU) t = t >= BN / 64 ? t - BN / 64 : t;
+    return (uint32_t)min<int64_t>(n0 + t * 32 + mx4_perm(q & 31), p.N - 1);
+  };
+  constexpr int WL = C::WROW / 16, WR = 64 / WL;
+  uint32_t w_off[C::W_INS];
+#pragma unroll
+  for (int b = 0; b < C::W_INS; ++b) {
+    const int q = (wave * C::W_INS + b) * WR + lane / WL;
+    const int c = AT == A_MX4 ? (lane & 3) ^ swz_b(q) : (lane & 1) ^ swz_c(q);
+    w_off[b] = (uint32_t)(w_row(q) * p.ldw * 16 + c * 16);
+  }
+  // scale instruction i stages rows 64 i + lane of the weight, then of x
+  constexpr int SI = (C::S_INS + 3) / 4;
+  uint32_t s_off[SI];
+#pragma unroll
+  for (int i = 0; i < SI; ++i) {
+    const int q = (wave + 4 * i) * 64 + lane;
+    if (q < BN) {
+      s_off[i] = (uint32_t)(w_row(q) * p.ldw);
+    } else {
+      const int64_t lr = row0 + min(q - BN, rows - 1);
+      s_off[i] = (uint32_t)((p.row_idx ? (int64_t)p.row_idx[lr] : lr) * p.ldx);
+    }
+  }
+
+  const uint32_t lds0 = lds_offset(&smem[0]);
+  auto dma_stage = [&](int kt, int buf) {
+    const uint32_t l = lds0 + (uint32_t)(buf * C::STAGE);
+    // 4 scale bytes a row: the stage's own (128 wide), or the two stages' that share them
+    const int64_t sk = AT == A_MX4 ? (int64_t)kt * 4 : (int64_t)(kt >> 1) * 4;
+#pragma unroll
+    for (int i = 0; i < SI; ++i) {
+      const int q = wave + 4 * i;
+      if (C::S_INS % 4 == 0 || q < C::S_INS) {
+        const uint8_t* src = q * 64 >= BN ? p.xs : (SWIGLU && q * 64 >= BN / 2 ? S2 : S1);
+        dma4(src + sk, s_off[i], l + C::XB + C::WB + q * 256);
+      }
+    }
+    const char* xk = (const char*)p.x + (int64_t)kt * C::XROW;
+#pragma unroll
+    for (int a = 0; a < C::X_INS; ++a) dma16(xk, x_off[a], l + (wave * C::X_INS + a) * 1024);
+#pragma unroll
+    for (int b = 0; b < C::W_INS; ++b) {
+      const int q = (wave * C::W_INS + b) * WR;
+      dma16((SWIGLU && q >= BN / 2 ? W2 : W1) + (int64_t)kt * C::WROW, w_off[b],
+            l + C::XB + (wave * C::W_INS + b) * 1024);
+    }
+  };
+
+  const int g = lane >> 5, l32 = lane & 31;
+  // staged row of weight tile j of this wave: with SwiGLU its gate tiles, then its up tiles
+  auto w_tile = [&](int j) -> int {
+    if constexpr (SWIGLU) return j < WT / 2 ? wn * (BN / 4) + j * 32 : BN / 2 + wn * (BN / 4) + (j - WT / 2) * 32;
+    else return wn * (BN / 2) + j * 32;
+  };
+  f32x16_t acc[WT][TT];
+#pragma unroll
+  for (int j = 0; j < WT; ++j)
+#pragma unroll
+    for (int i = 0; i < TT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[j][i][r] = 0.0f;
+
+  auto compute = [&](int buf, int kt) {
+    const char* xs_ = smem + buf * C::STAGE;
+    const char* ws_ = xs_ + C::XB;
+    const char* ss_ = ws_ + C::WB;
+    if constexpr (AT == A_MX4) {
+      int sw[WT], sx[TT];
+#pragma unroll
+      for (int j = 0; j < WT; ++j) sw[j] = (int)(*(const uint32_t*)(ss_ + (w_tile(j) + l32) * 4) >> (8 * g));
+#pragma unroll
+      for (int i = 0; i < TT; ++i)
+        sx[i] = (int)(*(const uint32_t*)(ss_ + (BN + wm * (BM / 2) + i * 32 + l32) * 4) >> (8 * g));
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        i32x8_t wf[WT], xf[TT];
+#pragma unroll
+        for (int j = 0; j < WT; ++j) {
+          const int r = w_tile(j) + l32;
+          wf[j] = mx4_operand(*(const uint4*)(ws_ + r * 64 + (((ks * 2 + g) ^ swz_b(r)) << 4)));
+        }
+#pragma unroll
+        for (int i = 0; i < TT; ++i) {
+          const int r = wm * (BM / 2) + i * 32 + l32;
+          xf[i] = mx4_operand(*(const uint4*)(xs_ + r * 64 + (((ks * 2 + g) ^ swz_b(r)) << 4)));
+        }
+#pragma unroll
+        for (int j = 0; j < WT; ++j)
+#pragma unroll
+          for (int i = 0; i < TT; ++i)
+            acc[j][i] = ks == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[j], xf[i], acc[j][i], 4, 4, 0,
+                                                                                 sw[j], 0, sx[i])
+                                : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[j], xf[i], acc[j][i], 4, 4, 2,
+                                                                                 sw[j], 2, sx[i]);
+      }
+    } else {
+      // codes of block g of each weight row, and its scale
+      uint4 wc[WT];
+      float sc[WT];
+#pragma unroll
+      for (int j = 0; j < WT; ++j) {
+        const int r = w_tile(j) + l32;
+        wc[j] = *(const uint4*)(ws_ + r * 32 + ((g ^ swz_c(r)) << 4));
+        sc[j] = mx4_scale((*(const uint32_t*)(ss_ + r * 4) >> (8 * g + 16 * (kt & 1))) & 255u);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        constexpr int NT = AT == A_F32 ? 3 : 1;
+        bf16x8_t xf[TT][NT];
+#pragma unroll
+        for (int i = 0; i < TT; ++i) {
+          const int r = wm * (BM / 2) + i * 32 + l32;
+          if constexpr (AT == A_BF16) {
+            xf[i][0] = *(const bf16x8_t*)(xs_ + r * 128 + (((g * 4 + q) ^ swz_a(r)) << 4));
+          } else {
+            const float4 a = *(const float4*)(xs_ + r * 256 + (((g * 8 + q * 2) ^ (r & 15)) << 4));
+            const float4 b = *(const float4*)(xs_ + r * 256 + (((g * 8 + q * 2 + 1) ^ (r & 15)) << 4));
+            const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            bf16x8_t t[3];
+            mx4_split3(v, t);
+#pragma unroll
+            for (int k = 0; k < NT; ++k) xf[i][k] = t[k];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < WT; ++j) {
+          const uint32_t c = q == 0 ? wc[j].x : q == 1 ? wc[j].y : q == 2 ? wc[j].z : wc[j].w;
+          const bf16x8_t wf = __builtin_bit_cast(bf16x8_t, mx4_decode8(c, sc[j]));
+#pragma unroll
+          for (int i = 0; i < TT; ++i)
+#pragma unroll
+            for (int k = 0; k < NT; ++k)
+              acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf, xf[i][k], acc[j][i], 0, 0, 0);
+        }
+      }
+    }
+  };
+
+  // Stage kt is complete when at most the loads of the later stages are outstanding;
+  // the barrier publishes it and frees the buffer of stage kt - 1.  Stages past the
+  // end load the last one again into a buffer nobody reads.
+  const int nk = (int)(p.K / C::KS);
+#pragma unroll
+  for (int s = 0; s + 1 < NSTAGE; ++s) dma_stage(s < nk ? s : nk - 1, s);
+  int buf = 0, nbuf = NSTAGE - 1;
+  for (int kt = 0; kt < nk; ++kt) {
+    wait_vm<C::DMA_MIN * (NSTAGE - 2)>();
+    __syncthreads();
+    const int ks = kt + NSTAGE - 1;
+    dma_stage(ks < nk ? ks : nk - 1, nbuf);
+    compute(buf, kt);
+    buf = buf + 1 == NSTAGE ? 0 : buf + 1;
+    nbuf = nbuf + 1 == NSTAGE ? 0 : nbuf + 1;
+  }
+  wait_vm<0>();
+
+  // ---- epilogue: 16 consecutive outputs of one row a lane -------------------------
+  constexpr int OTW = SWIGLU ? WT / 2 : WT;
+#pragma unroll
+  for (int i = 0; i < TT; ++i) {
+    const int lr = wm * (BM / 2) + i * 32 + l32;
+    const bool live = lr < rows;
+    const int64_t row = row0 + lr;
+#pragma unroll
+    for (int j = 0; j < OTW; ++j) {
+      const int64_t nb0 = n0 + wn * (BNO / 2) + j * 32, n = nb0 + g * 16;
+      float v[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        v[r] = SWIGLU ? mx4_swiglu(acc[j][i][r], acc[j + WT / 2 < WT ? j + WT / 2 : j][i][r]) : acc[j][i][r];
+        if (nb0 + 32 > p.N && n + r >= p.N) v[r] = 0.0f;  // padding
+      }
+      if constexpr (OT == O_MX4) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) m = max(m, __float_as_uint(v[r]) & 0x7fffffffu);
+        m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+        const uint32_t byte = mx4_scale_byte(m);
+        const float* v0 = v;
+        const uint32_t lo = mx4_encode8(v0, byte), hi = mx4_encode8(v0 + 8, byte);
+        const int64_t b = row * p.ldy + nb0 / MX4_BLOCK;
+        if (live && nb0 / MX4_BLOCK < p.ldy) {
+          *(uint2*)((uint8_t*)p.y + b * 16 + g * 8) = make_uint2(lo, hi);
+          if (g == 0) p.ys[b] = (uint8_t)byte;
+        }
+      } else if (live && n < p.ldy) {
+        const int64_t o = row * p.ldy + n;
+        const bool whole = n + 16 <= p.ldy && p.ldy % 8 == 0;
+        if constexpr (OT == O_BF16) {
+          uint32_t u[8];
+#pragma unroll
+          for (int r = 0; r < 8; ++r) u[r] = pack_bf16(v[2 * r], v[2 * r + 1]);
+          uint16_t* y = (uint16_t*)p.y + o;
+          if (whole) {
+            ((uint4*)y)[0] = make_uint4(u[0], u[1], u[2], u[3]);
+            ((uint4*)y)[1] = make_uint4(u[4], u[5], u[6], u[7]);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (n + r < p.ldy) y[r] = (uint16_t)(u[r / 2] >> (16 * (r & 1)));
+          }
+        } else {
+          float* y = (float*)p.y + o;
+          if (whole) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              ((float4*)y)[r] = make_float4(v[4 * r], v[4 * r + 1], v[4 * r + 2], v[4 * r + 3]);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (n + r < p.ldy) y[r] = v[r];
+          }
+        }
+      }
+    }
+  }
+}
+
+template <int AT, int OT, bool SWIGLU, int BM, int BN, int NSTAGE>
+int launch_gemm_cfg(const Mx4Args& p, int64_t m_tiles, hipStream_t stream) {
+  constexpr int BNO = SWIGLU ? BN / 2 : BN;
+  const int64_t n_tiles = (mx4_cols<OT>(p) + BNO - 1) / BNO;
+  if (m_tiles * n_tiles > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: too many tiles");
+  hipLaunchKernelGGL((mx4_gemm_kernel<AT, OT, SWIGLU, BM, BN, NSTAGE>), dim3((unsigned)(m_tiles * n_tiles)),
+                     dim3(256), 0, stream, p);
+  return check_launch("mx4_gemm_kernel");
+}
+
+// Whether mx4_gemm_kernel takes the call: whole 128-wide stages, 16-byte rows, and
+// 32-bit offsets from the activations' and an expert's codes.  xrows: rows of x.
+bool gemm_ok(const Mx4Args& p, int at, int64_t xrows) {
+  const int64_t xbytes = xrows * p.ldx * (at == A_MX4 ? 16 : at == A_BF16 ? 2 : 4);
+  return p.K % 128 == 0 && p.ldw % 4 == 0 && p.N * p.ldw * 16 < (1LL << 32) && xbytes < (1LL << 32) &&
+         ((uintptr_t)p.x & 15) == 0 && ((uintptr_t)p.w & 15) == 0 && ((uintptr_t)p.s & 3) == 0 &&
+         (!p.w2 || (((uintptr_t)p.w2 & 15) == 0 && ((uintptr_t)p.s2 & 3) == 0)) && ((uintptr_t)p.y & 15) == 0;
+}
+
 constexpr int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 bool aligned(const void* p, int to) { return ((uintptr_t)p & (to - 1)) == 0; }
 bool dtype_ok(int d) { return d == SMAUL_DTYPE_F32 || d == SMAUL_DTYPE_BF16; }
@@ -308,13 +664,24 @@ int launch_quantize(const void* x, int dtype, uint8_t* codes, uint8_t* scales, i
   return check_launch("mx4_quantize_kernel");
 }
 
+// row tiles of the two product kernels
+constexpr int64_t TILE_BM = 64;
+int64_t gemm_bm(int at) { return at == A_F32 ? 64 : 128; }
+
+template <int AT, int OT, bool SWIGLU>
+int launch_product(const Mx4Args& p, bool gemm, int64_t m_tiles, hipStream_t stream) {
+  if (!gemm) return launch_tiles<AT, OT, SWIGLU, false>(p, m_tiles, stream);
+  if constexpr (AT == A_F32) return launch_gemm_cfg<AT, OT, SWIGLU, 64, 256, 3>(p, m_tiles, stream);
+  else return launch_gemm_cfg<AT, OT, SWIGLU, 128, 256, 3>(p, m_tiles, stream);
+}
+
 // activations with a weight: y of `out` type
-int launch_linear(Mx4Args p, int at, int out, int64_t m_tiles, hipStream_t stream) {
+int launch_linear(const Mx4Args& p, int at, int out, bool gemm, int64_t m_tiles, hipStream_t stream) {
   if (at == A_MX4)
-    return out == O_BF16 ? launch_tiles<A_MX4, O_BF16, false, false>(p, m_tiles, stream)
-                         : launch_tiles<A_MX4, O_F32, false, false>(p, m_tiles, stream);
-  return at == A_BF16 ? launch_tiles<A_BF16, O_BF16, false, false>(p, m_tiles, stream)
-                      : launch_tiles<A_F32, O_F32, false, false>(p, m_tiles, stream);
+    return out == O_BF16 ? launch_product<A_MX4, O_BF16, false>(p, gemm, m_tiles, stream)
+                         : launch_product<A_MX4, O_F32, false>(p, gemm, m_tiles, stream);
+  return at == A_BF16 ? launch_product<A_BF16, O_BF16, false>(p, gemm, m_tiles, stream)
+                      : launch_product<A_F32, O_F32, false>(p, gemm, m_tiles, stream);
 }
 
 }  // namespace
@@ -386,7 +753,12 @@ int smaul_mx4_linear(const void* x, int dtype, const uint8_t* w, const uint8_t* 
     p.xs = scales;
     at = A_MX4;
   }
-  return launch_linear(p, at, bf16 ? O_BF16 : O_F32, (rows + 63) / 64, stream);
+  p.ldx = at == A_MX4 ? mx4_blocks(in_f) : in_f;
+  p.ldw = mx4_blocks(in_f);
+  p.ldy = out_f;
+  const bool gemm = rows > TILE_BM && gemm_ok(p, at, rows);
+  const int64_t bm = gemm ? gemm_bm(at) : TILE_BM;
+  return launch_linear(p, at, bf16 ? O_BF16 : O_F32, gemm, (rows + bm - 1) / bm, stream);
 }
 
 int smaul_mx4_backward_input(const void* g, int dtype, const uint8_t* w, const uint8_t* s, void* dx, int64_t rows,
@@ -475,14 +847,8 @@ int smaul_mx4_moe_forward(const void* x, int dtype, const int64_t* topi, const f
   int32_t* perm_row = (int32_t*)(ws + q.perm_row);
   int32_t* inv = (int32_t*)(ws + q.inv);
   const bool bf16 = dtype == SMAUL_DTYPE_BF16, mx4 = act == SMAUL_ACT_MX4;
-  const int64_t R = T * k, m_tiles = (R + 63) / 64 + E;
-  int rc = smaul_moe_dispatch(topi, topw, counts, seg_off, tile_off, perm_row, (float*)(ws + q.perm_w), inv, T, E, k,
-                              64, ws + q.scratch, q.scratch_bytes, stream);
-  if (rc) return rc;
-  if (mx4) {
-    rc = launch_quantize(x, dtype, (uint8_t*)ws + q.xc, (uint8_t*)ws + q.xs, T, d, stream);
-    if (rc) return rc;
-  }
+  const int at = mx4 ? A_MX4 : bf16 ? A_BF16 : A_F32;
+  const int64_t R = T * k;
   Mx4Args p{};
   p.x = mx4 ? ws + q.xc : x;
   p.xs = mx4 ? (uint8_t*)ws + q.xs : nullptr;
@@ -495,27 +861,42 @@ int smaul_mx4_moe_forward(const void* x, int dtype, const int64_t* topi, const f
   p.ys = mx4 ? (uint8_t*)ws + q.hs : nullptr;
   p.K = d;
   p.N = h;
+  p.ldx = mx4 ? mx4_blocks(d) : d;
+  p.ldw = mx4_blocks(d);
+  p.ldy = mx4 ? mx4_blocks(h) : h;
   p.seg_off = seg_off;
   p.tile_off = tile_off;
   p.E = (int)E;
   p.xvec = aligned(x, 16) && d % 8 == 0;
-  rc = mx4 ? launch_tiles<A_MX4, O_MX4, true, false>(p, m_tiles, stream)
-           : bf16 ? launch_tiles<A_BF16, O_BF16, true, false>(p, m_tiles, stream)
-                  : launch_tiles<A_F32, O_F32, true, false>(p, m_tiles, stream);
-  if (rc) return rc;
-  Mx4Args dn{};
-  dn.x = ws + q.hc;
+  Mx4Args dn = p;
+  dn.x = p.y;
   dn.xs = p.ys;
+  dn.row_idx = nullptr;
   dn.w = down_w;
   dn.s = down_s;
+  dn.w2 = dn.s2 = nullptr;
   dn.y = ws + q.y;
+  dn.ys = nullptr;
   dn.K = h;
   dn.N = d;
-  dn.seg_off = seg_off;
-  dn.tile_off = tile_off;
-  dn.E = (int)E;
+  dn.ldx = p.ldy;
+  dn.ldw = mx4_blocks(h);
+  dn.ldy = d;
   dn.xvec = h % (bf16 ? 8 : 4) == 0;
-  rc = launch_linear(dn, mx4 ? A_MX4 : bf16 ? A_BF16 : A_F32, bf16 ? O_BF16 : O_F32, m_tiles, stream);
+  const bool gemm = T > 64 && gemm_ok(p, at, T) && gemm_ok(dn, at, R);
+  const int64_t bm = gemm ? gemm_bm(at) : TILE_BM, m_tiles = (R + bm - 1) / bm + E;
+  int rc = smaul_moe_dispatch(topi, topw, counts, seg_off, tile_off, perm_row, (float*)(ws + q.perm_w), inv, T, E, k,
+                              bm, ws + q.scratch, q.scratch_bytes, stream);
+  if (rc) return rc;
+  if (mx4) {
+    rc = launch_quantize(x, dtype, (uint8_t*)ws + q.xc, (uint8_t*)ws + q.xs, T, d, stream);
+    if (rc) return rc;
+  }
+  rc = mx4 ? launch_product<A_MX4, O_MX4, true>(p, gemm, m_tiles, stream)
+           : bf16 ? launch_product<A_BF16, O_BF16, true>(p, gemm, m_tiles, stream)
+                  : launch_product<A_F32, O_F32, true>(p, gemm, m_tiles, stream);
+  if (rc) return rc;
+  rc = launch_linear(dn, at, bf16 ? O_BF16 : O_F32, gemm, m_tiles, stream);
   if (rc) return rc;
   return smaul_moe_combine(ws + q.y, dtype, topi, topw, inv, out, T, d, k, stream);
 }

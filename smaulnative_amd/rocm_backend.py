@@ -530,16 +530,21 @@ class RocmBackend:
         _lib.check(rc, "mx4_quantize")
         return codes, scales
 
-    @staticmethod
-    def _mx4_check(name, codes, scales, lead, K):
+    def _mx4_check(self, name, codes, scales, lead, K):
         """The codes and scales [*lead, 16 n] / [*lead, n] of rows of K values, contiguous."""
         n = (K + 31) // 32
         for what, t, last in (("codes", codes, n * 16), ("scales", scales, n)):
             if t.dtype != torch.uint8 or tuple(t.shape) != (*lead, last):
                 raise RuntimeError(f"{name}: {what} must be uint8 {[*lead, last]}, got {t.dtype} {list(t.shape)}")
-        codes = codes if codes.is_contiguous() and codes.data_ptr() % 16 == 0 else codes.clone(
-            memory_format=torch.contiguous_format)
-        return codes, scales if scales.is_contiguous() else scales.contiguous()
+        return self._aligned(codes), self._aligned(scales)
+
+    @staticmethod
+    def _aligned(t):
+        """t contiguous from a 16-byte boundary, copied where it is not: the products'
+        rows are read 16 bytes at a time."""
+        if t.is_contiguous() and t.data_ptr() % 16 == 0:
+            return t
+        return t.clone(memory_format=torch.contiguous_format)
 
     def mx4_dequantize(self, codes, scales, in_f, dtype=torch.float32):
         """The values [..., in_f] in ``dtype`` (fp32 or bf16, exact in both) that codes
@@ -600,7 +605,7 @@ class RocmBackend:
         if x.dim() != 2 or x.shape[1] != width:
             raise RuntimeError(f"{name}: {what} must be [rows, {width}], got {tuple(x.shape)}")
         w, s = self._mx4_check(name, w, s, (out_f,), in_f)
-        return x if x.is_contiguous() else x.contiguous(), w, s
+        return self._aligned(x), w, s
 
     def mx4_moe_forward(self, x, topi, topw, experts, act="keep"):
         """The routed SwiGLU experts in the 4-bit format: (out [..., d] of x's type,
@@ -634,7 +639,8 @@ class RocmBackend:
                                f"{list(topi.shape)} / {topw.dtype} {list(topw.shape)}")
         if not 1 <= k <= min(E, 8) or E > 64:
             raise ValueError(f"mx4_moe_forward: need 1 <= k <= min(E, 8) and E <= 64, got k={k}, E={E}")
-        xc, topi, topw = (t if t.is_contiguous() else t.contiguous() for t in (x, topi, topw))
+        topi, topw = (t if t.is_contiguous() else t.contiguous() for t in (topi, topw))
+        xc = self._aligned(x)
         dev, a, dt = x.device, _lib.ACTS[act], _ACT[x.dtype]
         T = xc.numel() // d
         out = torch.empty(x.shape, dtype=x.dtype, device=dev)
