@@ -528,12 +528,12 @@ int smaul_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* y, i
 
 /*
  * y[rows, out_f] = x[rows, in_f] . decode(w, s)^T, w and s [out_f, in_f] in that format
- * (w 16-byte aligned), x and y of dtype.  SMAUL_ACT_KEEP multiplies x as it is (fp32 as
- * two bf16 terms, within 2^-17 of each value), SMAUL_ACT_MX4 rounds its rows to the
- * format first, in the workspace; sums are fp32.
+ * (x, y and w 16-byte aligned, the workspace 256), x and y of dtype.  SMAUL_ACT_KEEP
+ * multiplies x as it is, SMAUL_ACT_MX4 rounds its rows to the format first, in the
+ * workspace; sums are fp32.
  */
 enum { SMAUL_ACT_KEEP = 0, SMAUL_ACT_MX4 = 1 };
-int64_t smaul_mx4_linear_workspace_size(int64_t rows, int64_t in_f, int64_t out_f, int act);
+int64_t smaul_mx4_linear_workspace_size(int64_t rows, int64_t in_f, int64_t out_f, int dtype, int act);
 int smaul_mx4_linear(const void* x, int dtype, const uint8_t* w, const uint8_t* s, void* y, int64_t rows,
                      int64_t in_f, int64_t out_f, int act, void* workspace, int64_t workspace_bytes,
                      hipStream_t stream);
@@ -546,9 +546,9 @@ int smaul_mx4_backward_input(const void* g, int dtype, const uint8_t* w, const u
  * The routed SwiGLU experts in that format: out[t] = sum over t's slots, ascending
  * expert, of topw * (hdn . Wd^T), hdn = silu(x . Wg^T) * (x . Wu^T).  Weights of all
  * experts one after the other: gate_w / up_w [E, h, d], down_w [E, d, h] (codes,
- * 16-byte aligned) with their scales.  SMAUL_ACT_KEEP: hdn and the slots' outputs are
- * rounded to dtype; SMAUL_ACT_MX4 (bf16 x): x and hdn (from fp32) are rounded to the
- * format, the outputs to bf16.  Slots with topi outside [0, E) or topw not above 0 add
+ * 16-byte aligned as x and out) with their scales.  SMAUL_ACT_KEEP: hdn is rounded to
+ * dtype; SMAUL_ACT_MX4 (bf16 x): x and hdn (from fp32) are rounded to the format, the
+ * slots' outputs to bf16.  Slots with topi outside [0, E) or topw not above 0 add
  * nothing.  counts int32 [E] (rows of each expert).  d a multiple of 8, E <= 64,
  * k <= min(E, 8); workspace 256-byte aligned.  T == 0 writes nothing.
  */

@@ -78,7 +78,7 @@ SIGNATURES = {
     "smaul_moe_route_backward": (_I, [_P, _P, _I, _P, _P, _P, _I64, _I64, _I64, _I, _I, ctypes.c_float, _P]),
     "smaul_mx4_quantize": (_I, [_P, _I, _P, _P, _I64, _I64, _P]),
     "smaul_mx4_dequantize": (_I, [_P, _P, _P, _I, _I64, _I64, _P]),
-    "smaul_mx4_linear_workspace_size": (_I64, [_I64, _I64, _I64, _I]),
+    "smaul_mx4_linear_workspace_size": (_I64, [_I64, _I64, _I64, _I, _I]),
     "smaul_mx4_linear": (_I, [_P, _I, _P, _P, _P, _I64, _I64, _I64, _I, _P, _I64, _P]),
     "smaul_mx4_backward_input": (_I, [_P, _I, _P, _P, _P, _I64, _I64, _I64, _P]),
     "smaul_mx4_moe_workspace_size": (_I64, [_I64, _I64, _I64, _I64, _I64, _I, _I]),

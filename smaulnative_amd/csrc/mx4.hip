@@ -53,49 +53,88 @@ __device__ __forceinline__ uint32_t mx4_amax8(const float (&v)[8]) {
   return m;
 }
 
+// the block's largest bits over its quad of lanes
+__device__ __forceinline__ uint32_t mx4_quad_max(uint32_t m) {
+  m = max(m, (uint32_t)__shfl_xor((int)m, 1, 4));
+  return max(m, (uint32_t)__shfl_xor((int)m, 2, 4));
+}
+
+// VEC: K is a multiple of 32, so that groups of 8 values, their codes and their
+// blocks are each one run over the whole matrix; a thread takes MX4_U groups, all
+// loaded first.  Otherwise a row's last block is padded and a thread takes one.
+constexpr int MX4_U = 4;
+
 template <bool BF16, bool VEC>
 __global__ void __launch_bounds__(256)
 mx4_quantize_kernel(const void* __restrict__ x, uint32_t* __restrict__ codes, uint8_t* __restrict__ scales,
                     int64_t rows, int64_t K) {
-  const int64_t nb = mx4_blocks(K);
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t blk = i >> 2;
-  if (blk >= rows * nb) return;  // whole quads
-  const int64_t row = blk / nb, b = blk - row * nb;
-  const int q = (int)(i & 3);
-  float v[8];
-  mx4_load8<BF16, VEC>(x, row, K, b * MX4_BLOCK + q * 8, v);
-  uint32_t m = mx4_amax8(v);
-  m = max(m, (uint32_t)__shfl_xor((int)m, 1, 4));
-  m = max(m, (uint32_t)__shfl_xor((int)m, 2, 4));
-  const uint32_t byte = mx4_scale_byte(m);
-  codes[i] = mx4_encode8(v, byte);
-  if (q == 0) scales[blk] = (uint8_t)byte;
+  const int64_t nb = mx4_blocks(K), groups = rows * nb * 4;
+  if constexpr (VEC) {
+    const int64_t i0 = (int64_t)blockIdx.x * (256 * MX4_U) + threadIdx.x;
+    float v[MX4_U][8];
+#pragma unroll
+    for (int u = 0; u < MX4_U; ++u)
+      if (i0 + u * 256 < groups) mx4_load8<BF16, true>(x, 0, 0, (i0 + u * 256) * 8, v[u]);
+#pragma unroll
+    for (int u = 0; u < MX4_U; ++u) {
+      const int64_t i = i0 + u * 256;
+      if (i < groups) {  // whole quads
+        const uint32_t byte = mx4_scale_byte(mx4_quad_max(mx4_amax8(v[u])));
+        codes[i] = mx4_encode8(v[u], byte);
+        if ((i & 3) == 0) scales[i >> 2] = (uint8_t)byte;
+      }
+    }
+  } else {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= groups) return;
+    const int64_t blk = i >> 2, row = blk / nb, b = blk - row * nb;
+    float v[8];
+    mx4_load8<BF16, false>(x, row, K, b * MX4_BLOCK + (i & 3) * 8, v);
+    const uint32_t byte = mx4_scale_byte(mx4_quad_max(mx4_amax8(v)));
+    codes[i] = mx4_encode8(v, byte);
+    if ((i & 3) == 0) scales[blk] = (uint8_t)byte;
+  }
+}
+
+// 8 decoded values to a row from its column c0, 16 bytes at a time
+template <bool BF16>
+__device__ __forceinline__ void mx4_store8(void* y, int64_t o, uint4 d) {
+  if constexpr (BF16) {
+    *(uint4*)((uint16_t*)y + o) = d;
+  } else {
+    const uint32_t u[4] = {d.x, d.y, d.z, d.w};
+    float4* p = (float4*)((float*)y + o);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      p[j] = make_float4(__uint_as_float(u[2 * j] << 16), __uint_as_float(u[2 * j] & 0xffff0000u),
+                         __uint_as_float(u[2 * j + 1] << 16), __uint_as_float(u[2 * j + 1] & 0xffff0000u));
+  }
 }
 
 template <bool BF16, bool VEC>
 __global__ void __launch_bounds__(256)
 mx4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, void* __restrict__ y,
                       int64_t rows, int64_t K) {
-  const int64_t nb = mx4_blocks(K);
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t blk = i >> 2;
-  if (blk >= rows * nb) return;
-  const int64_t row = blk / nb, c0 = (blk - row * nb) * MX4_BLOCK + (i & 3) * 8;
-  const uint4 d = mx4_decode8(codes[i], mx4_scale(scales[blk]));
-  const uint32_t u[4] = {d.x, d.y, d.z, d.w};
-  const int64_t o = row * K + c0;
+  const int64_t nb = mx4_blocks(K), groups = rows * nb * 4;
   if constexpr (VEC) {
-    if constexpr (BF16) {
-      *(uint4*)((uint16_t*)y + o) = d;
-    } else {
-      float4* p = (float4*)((float*)y + o);
+    const int64_t i0 = (int64_t)blockIdx.x * (256 * MX4_U) + threadIdx.x;
+    uint32_t c[MX4_U], s[MX4_U];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        p[j] = make_float4(__uint_as_float(u[2 * j] << 16), __uint_as_float(u[2 * j] & 0xffff0000u),
-                           __uint_as_float(u[2 * j + 1] << 16), __uint_as_float(u[2 * j + 1] & 0xffff0000u));
-    }
+    for (int u = 0; u < MX4_U; ++u)
+      if (i0 + u * 256 < groups) {
+        c[u] = codes[i0 + u * 256];
+        s[u] = scales[(i0 + u * 256) >> 2];
+      }
+#pragma unroll
+    for (int u = 0; u < MX4_U; ++u)
+      if (i0 + u * 256 < groups) mx4_store8<BF16>(y, (i0 + u * 256) * 8, mx4_decode8(c[u], mx4_scale(s[u])));
   } else {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= groups) return;
+    const int64_t blk = i >> 2, row = blk / nb, c0 = (blk - row * nb) * MX4_BLOCK + (i & 3) * 8;
+    const uint4 d = mx4_decode8(codes[i], mx4_scale(scales[blk]));
+    const uint32_t u[4] = {d.x, d.y, d.z, d.w};
+    const int64_t o = row * K + c0;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (c0 + j < K) {
@@ -103,6 +142,119 @@ mx4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restr
         if constexpr (BF16) ((uint16_t*)y)[o + j] = (uint16_t)b;
         else ((float*)y)[o + j] = __uint_as_float(b << 16);
       }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// operands of the GEMM (mx4_gemm_kernel), one launch for all of a call's
+// ---------------------------------------------------------------------------
+// Scales go to [group of 128 values][row] dwords (four blocks' bytes): a stage's
+// scales of consecutive rows are then whole cache lines (a dword from every row of
+// the stored layout costs the GEMM as many line requests as a stage's codes).
+// Activations are rounded to the format straight into that form, and rows whose
+// width is no whole number of stages are copied to padded ones: codes 0.
+// Widths are padded to whole stages of the widest kind, MX4_STAGE.
+constexpr int MX4_GROUP = 128, MX4_STAGE = 256;
+__host__ __device__ __forceinline__ int64_t mx4_groups(int64_t K) {
+  return (K + MX4_STAGE - 1) / MX4_STAGE * (MX4_STAGE / MX4_GROUP);
+}
+
+struct Mx4Weight {
+  const uint8_t* w;
+  const uint8_t* s;
+  uint32_t* st;    // [E][groups][N] dwords
+  uint4* wp;       // padded codes [E N][groups * 4], or null: used as they are
+  int64_t N, K;    // rows of an expert
+  int64_t blocks;  // workgroups that the matrix takes
+};
+enum { P_NONE = 0, P_ROUND = 1, P_PAD = 2 };  // activations: as they are, rounded, or copied to padded rows
+struct Mx4Prep {
+  Mx4Weight m[3];
+  const void* x;
+  void* xo;        // codes [T][groups * 4] of 16 bytes, or padded rows
+  uint32_t* xst;   // P_ROUND: scales [groups][T]
+  int64_t T, K;
+  int64_t xblocks;
+  int xmode, xvec;
+};
+
+// a workgroup: 16 rows by 4 groups, 16 lanes a row
+template <bool BF16>
+__device__ __forceinline__ void mx4_prep_rows(const Mx4Prep& p, int64_t block) {
+  const int64_t ng = mx4_groups(p.K), cb = (ng + 3) / 4;
+  const int64_t row = block / cb * 16 + (threadIdx.x >> 4), g0 = block % cb * 4;
+  const int c = threadIdx.x & 15;
+  if (row >= p.T) return;  // whole quads
+  float v[4][8];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int64_t c0 = (g0 + u) * MX4_GROUP + c * 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[u][j] = 0.0f;
+    if (c0 < p.K) {
+      if (p.xvec && c0 + 8 <= p.K) mx4_load8<BF16, true>(p.x, row, p.K, c0, v[u]);
+      else mx4_load8<BF16, false>(p.x, row, p.K, c0, v[u]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    if (g0 + u >= ng) break;
+    const int64_t at = row * ng * 16 + (g0 + u) * 16 + c;  // groups of 8 values
+    if (p.xmode == P_ROUND) {
+      uint32_t byte = mx4_scale_byte(mx4_quad_max(mx4_amax8(v[u])));
+      ((uint32_t*)p.xo)[at] = mx4_encode8(v[u], byte);
+      byte <<= 8 * (c >> 2);  // the group's four blocks to one dword
+      byte |= (uint32_t)__shfl_xor((int)byte, 4, 16);
+      byte |= (uint32_t)__shfl_xor((int)byte, 8, 16);
+      if (c == 0) p.xst[(g0 + u) * p.T + row] = byte;
+    } else if constexpr (BF16) {
+      ((uint4*)p.xo)[at] = make_uint4(pack_bf16(v[u][0], v[u][1]), pack_bf16(v[u][2], v[u][3]),
+                                      pack_bf16(v[u][4], v[u][5]), pack_bf16(v[u][6], v[u][7]));
+    } else {
+      ((float4*)p.xo)[at * 2] = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
+      ((float4*)p.xo)[at * 2 + 1] = make_float4(v[u][4], v[u][5], v[u][6], v[u][7]);
+    }
+  }
+}
+
+// a thread: the four blocks of one group of one row, rows fastest
+__device__ __forceinline__ void mx4_prep_weight(const Mx4Weight& m, int64_t E, int64_t block) {
+  const int64_t ng = mx4_groups(m.K), nb = mx4_blocks(m.K);
+  const int64_t i = block * 256 + threadIdx.x;
+  if (i >= E * ng * m.N) return;
+  const int64_t q = i / m.N, n = i - q * m.N, e = q / ng, g = q - e * ng, row = e * m.N + n;
+  const uint8_t* s = m.s + row * nb + g * 4;
+  uint32_t d = 0;
+  if (nb % 4 == 0 && ((uintptr_t)m.s & 3) == 0) {
+    d = *(const uint32_t*)s;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) d |= (g * 4 + j < nb ? (uint32_t)s[j] : 127u) << (8 * j);
+  }
+  m.st[i] = d;
+  if (m.wp) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      m.wp[(row * ng + g) * 4 + j] =
+          g * 4 + j < nb ? ((const uint4*)m.w)[row * nb + g * 4 + j] : make_uint4(0, 0, 0, 0);
+  }
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(256) mx4_prep_kernel(Mx4Prep p, int64_t E) {
+  int64_t b = blockIdx.x;
+  if (b < p.xblocks) {
+    mx4_prep_rows<BF16>(p, b);
+    return;
+  }
+  b -= p.xblocks;
+#pragma unroll
+  for (int j = 0; j < 3; ++j) {
+    if (b < p.m[j].blocks) {
+      mx4_prep_weight(p.m[j], E, b);
+      return;
+    }
+    b -= p.m[j].blocks;
   }
 }
 
@@ -125,7 +277,9 @@ struct Mx4Args {
   void* y;                 // [rows][N] (O_MX4: codes)
   uint8_t* ys;             // O_MX4: scales
   int64_t R, K, N;
-  int64_t ldx, ldw, ldy;   // row strides of mx4_gemm_kernel: x and y in values (codes: blocks), W in blocks
+  // mx4_gemm_kernel: scales are [group][row] dwords (w's of each expert, xs and ys over
+  // xrows and yrows rows); row strides of x and y in values (codes: blocks), of W in blocks
+  int64_t ldx, ldw, ldy, xrows, yrows;
   const int32_t* seg_off;  // null: dense, R rows of one expert
   const int32_t* tile_off;
   int E;
@@ -283,6 +437,10 @@ __global__ void __launch_bounds__(256) mx4_tile_kernel(Mx4Args p) {
   }
 }
 
+constexpr int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+bool aligned(const void* p, int to) { return ((uintptr_t)p & (to - 1)) == 0; }
+bool dtype_ok(int d) { return d == SMAUL_DTYPE_F32 || d == SMAUL_DTYPE_BF16; }
+
 template <int AT, int OT, bool SWIGLU, bool TRANS>
 int launch_tiles(const Mx4Args& p, int64_t m_tiles, hipStream_t stream) {
   const int64_t n_tiles = (p.N + 63) / 64;
@@ -292,41 +450,51 @@ int launch_tiles(const Mx4Args& p, int64_t m_tiles, hipStream_t stream) {
   return check_launch("mx4_tile_kernel");
 }
 
-// The kernel of larger calls: K in stages, activations, codes and scales brought to
-// LDS by DMA, NSTAGE stages in flight, 4 waves of half the rows by half the columns.
+// The kernel of larger calls: K in stages of KS, activations, codes and scales brought
+// to LDS by DMA, NSTAGE stages in flight, WM x WN waves over BM rows x BN columns.
 //
 // Roles: the weight's rows are the matrix instruction's rows and the activations its
 // columns, and row i of a 32 x 32 tile is given weight row 16 ((i / 4) % 2) + 4 (i / 8)
 // + i % 4, so that the 16 sums of a lane are 16 consecutive outputs of one activation
 // row: they leave as whole 16-byte stores, and a block of the format has its largest
-// value in 15 comparisons and one exchange.
+// value in 8 instructions and one exchange.
 //
 // A_MX4 runs v_mfma_scale_f32_32x32x64_f8f6f4 on the codes as they are: lane i + 32 g
-// has block g of a 64-wide step of its row, one scale byte for the 32 values.  A stage
-// is 128 wide (64 bytes a row) with four scale bytes a row, a dword.  A_BF16 and A_F32
-// take stages of 64 (128 and 256 bytes a row); a lane's 16 bytes of codes are its block
-// g, decoded to bf16 with their scale (exact), and MFMA step q multiplies values
-// 32 g + 8 q and on.  fp32 activations are three bf16 terms, split after the LDS read.
-template <int AT, int BM, int BN, int NSTAGE>
+// has block g of a 64-wide step of its row, one scale byte for the 32 values.  A_BF16
+// and A_F32 decode: a lane's 16 bytes of codes are its block g of the 64-wide step,
+// times their scale (exact), and MFMA q multiplies values 32 g + 8 q and on; fp32
+// activations are three bf16 terms, split after the LDS read.
+//
+// Stages are as wide as make their rows whole cache lines: what bounds the loop is the
+// number of L2 requests, and half a line costs as much as a whole one (16384 rows,
+// K 4096 -> 4096: 190 us with 64-byte rows of codes).
+template <int AT, int BM, int BN, int WM, int WN, int KS, int NSTAGE>
 struct Mx4Cfg {
-  static constexpr int KS = AT == A_MX4 ? 128 : 64;
-  static constexpr int XROW = AT == A_MX4 ? 64 : AT == A_BF16 ? 128 : 256, WROW = KS / 2;
+  static constexpr int NW = WM * WN;
+  static constexpr int XROW = AT == A_MX4 ? KS / 2 : AT == A_BF16 ? KS * 2 : KS * 4, WROW = KS / 2;
   static constexpr int XB = BM * XROW, WB = BN * WROW;
-  static constexpr int SROWS = BN + (AT == A_MX4 ? BM : 0);
-  static constexpr int STAGE = XB + WB + SROWS * 4;
-  static constexpr int X_INS = XB / 4096, W_INS = WB / 4096, S_INS = SROWS / 64;  // DMA instructions: a wave's, all
-  static constexpr int DMA_MIN = X_INS + W_INS + S_INS / 4;
-  static constexpr int TT = BM / 64, WT = BN / 64;  // 32 x 32 tiles of a wave
+  static constexpr int SROWS = BN + (AT == A_MX4 ? BM : 0), SG = KS < 128 ? 1 : KS / 128;  // scale rows, dwords a row
+  static constexpr int STAGE = XB + WB + SROWS * SG * 4;
+  // DMA instructions: a wave's of x and W, all of the scales
+  static constexpr int X_INS = XB / (1024 * NW), W_INS = WB / (1024 * NW), S_INS = SROWS * SG / 64;
+  static constexpr int DMA_MIN = X_INS + W_INS + S_INS / NW;
+  static constexpr int TT = BM / WM / 32, WT = BN / WN / 32;  // 32 x 32 tiles of a wave
   static constexpr int LDS = NSTAGE * STAGE;
-  static_assert(XB % 4096 == 0 && WB % 4096 == 0 && SROWS % 64 == 0, "whole DMA instructions");
-  static_assert(DMA_MIN * (NSTAGE - 2) + 2 < 64 && LDS <= 160 * 1024, "pipeline depth");
+  static_assert(XB % (1024 * NW) == 0 && WB % (1024 * NW) == 0 && SROWS % 64 == 0, "whole DMA instructions");
+  static_assert(DMA_MIN * (NSTAGE - 2) < 64 && LDS <= 160 * 1024, "pipeline depth");
 };
 
 // the weight row of row i of a 32-row tile
 __device__ __forceinline__ int mx4_perm(int i) { return ((i >> 2) & 1) * 16 + (i >> 3) * 4 + (i & 3); }
 
-// the chunk swizzle of 32-byte rows (as swz_a and swz_b of the longer ones)
-__device__ __forceinline__ int swz_c(int r) { return ((r >> 2) ^ (r >> 3)) & 1; }
+// the place of chunk c (16 bytes) of LDS row r, rows of ROW bytes (as swz_a and swz_b)
+template <int ROW>
+__device__ __forceinline__ int mx4_swz(int r, int c) {
+  if constexpr (ROW == 32) return c ^ (((r >> 2) ^ (r >> 3)) & 1);
+  else if constexpr (ROW == 64) return c ^ swz_b(r);
+  else if constexpr (ROW == 128) return c ^ swz_a(r);
+  else return c ^ (r & 15);
+}
 
 // columns that a product writes: past N zeros, up to the padded row
 template <int OT>
@@ -361,14 +529,14 @@ __device__ __forceinline__ void mx4_split3(const float (&v)[8], bf16x8_t (&t)[3]
   }
 }
 
-template <int AT, int OT, bool SWIGLU, int BM, int BN, int NSTAGE>
-__global__ void __launch_bounds__(256, 2) mx4_gemm_kernel(Mx4Args p) {
-  using C = Mx4Cfg<AT, BM, BN, NSTAGE>;
-  constexpr int TT = C::TT, WT = C::WT, BNO = SWIGLU ? BN / 2 : BN;
+template <int AT, int OT, bool SWIGLU, int BM, int BN, int WM, int WN, int KS, int NSTAGE>
+__global__ void __launch_bounds__(WM * WN * 64, 2) mx4_gemm_kernel(Mx4Args p) {
+  using C = Mx4Cfg<AT, BM, BN, WM, WN, KS, NSTAGE>;
+  constexpr int TT = C::TT, WT = C::WT, NW = C::NW, BNO = SWIGLU ? BN / 2 : BN, XROW = C::XROW, WROW = C::WROW;
   __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = wave / WN, wn = wave % WN;
 
   // a contiguous band of tiles for each XCD (workgroup b runs on XCD b % 8), in
   // groups of GM row tiles by all column tiles
@@ -387,72 +555,69 @@ __global__ void __launch_bounds__(256, 2) mx4_gemm_kernel(Mx4Args p) {
   int64_t row0;
   if (!mx4_tile<BM>(p, mt, lane, e, row0, rows)) return;
   const int64_t n0 = (int64_t)nt * BNO;
-  const int64_t ebytes = (int64_t)e * p.N * p.ldw;  // this expert's scales; its codes are 16 times that far
-  const uint8_t* W1 = p.w + ebytes * 16;
-  const uint8_t* S1 = p.s + ebytes;
-  const uint8_t* W2 = SWIGLU ? p.w2 + ebytes * 16 : W1;
-  const uint8_t* S2 = SWIGLU ? p.s2 + ebytes : S1;
+  const int64_t eblocks = (int64_t)e * p.N * p.ldw;  // ldw / 4 groups of N dwords: as many bytes as blocks
+  const uint8_t* W1 = p.w + eblocks * 16;
+  const uint8_t* S1 = p.s + eblocks;
+  const uint8_t* W2 = SWIGLU ? p.w2 + eblocks * 16 : W1;
+  const uint8_t* S2 = SWIGLU ? p.s2 + eblocks : S1;
 
   // ---- DMA sources of this lane (32-bit offsets; the host checks the range) ----
   // Rows past the end read the last one: their sums are not stored.
-  constexpr int XL = C::XROW / 16, XR = 64 / XL;  // lanes a row, rows an instruction
+  constexpr int XL = XROW / 16, XR = 64 / XL;  // lanes a row, rows an instruction
   uint32_t x_off[C::X_INS];
 #pragma unroll
   for (int a = 0; a < C::X_INS; ++a) {
     const int r = (wave * C::X_INS + a) * XR + lane / XL;
-    const int c = AT == A_MX4 ? (lane & 3) ^ swz_b(r) : AT == A_BF16 ? (lane & 7) ^ swz_a(r) : (lane & 15) ^ (r & 15);
     const int64_t lr = row0 + min(r, rows - 1);
     const int64_t xr = p.row_idx ? (int64_t)p.row_idx[lr] : lr;
-    x_off[a] = (uint32_t)(xr * p.ldx * (AT == A_MX4 ? 16 : AT == A_BF16 ? 2 : 4) + c * 16);
+    x_off[a] = (uint32_t)(xr * p.ldx * (AT == A_MX4 ? 16 : AT == A_BF16 ? 2 : 4) + mx4_swz<XROW>(r, lane % XL) * 16);
   }
-  // staged weight row q: tile q / 32 of the wave halves (gate's, then up's), permuted
+  // staged weight row q: tiles of 32 (gate's, then up's), permuted
   auto w_row = [&](int q) -> uint32_t {
     int t = q >> 5;
     if (SWIGLU) t = t >= BN / 64 ? t - BN / 64 : t;
     return (uint32_t)min<int64_t>(n0 + t * 32 + mx4_perm(q & 31), p.N - 1);
   };
-  constexpr int WL = C::WROW / 16, WR = 64 / WL;
+  constexpr int WL = WROW / 16, WR = 64 / WL;
   uint32_t w_off[C::W_INS];
 #pragma unroll
   for (int b = 0; b < C::W_INS; ++b) {
     const int q = (wave * C::W_INS + b) * WR + lane / WL;
-    const int c = AT == A_MX4 ? (lane & 3) ^ swz_b(q) : (lane & 1) ^ swz_c(q);
-    w_off[b] = (uint32_t)(w_row(q) * p.ldw * 16 + c * 16);
+    w_off[b] = (uint32_t)(w_row(q) * p.ldw * 16 + mx4_swz<WROW>(q, lane % WL) * 16);
   }
-  // scale instruction i stages rows 64 i + lane of the weight, then of x
-  constexpr int SI = (C::S_INS + 3) / 4;
+  // scale instruction i stages 64 rows of one group: of the weight's, then of x's
+  constexpr int SI = (C::S_INS + NW - 1) / NW, SP = C::SROWS / 64;
   uint32_t s_off[SI];
 #pragma unroll
   for (int i = 0; i < SI; ++i) {
-    const int q = (wave + 4 * i) * 64 + lane;
+    const int q = (wave + NW * i) % SP * 64 + lane;
     if (q < BN) {
-      s_off[i] = (uint32_t)(w_row(q) * p.ldw);
+      s_off[i] = w_row(q) * 4;
     } else {
       const int64_t lr = row0 + min(q - BN, rows - 1);
-      s_off[i] = (uint32_t)((p.row_idx ? (int64_t)p.row_idx[lr] : lr) * p.ldx);
+      s_off[i] = (uint32_t)((p.row_idx ? (int64_t)p.row_idx[lr] : lr) * 4);
     }
   }
 
   const uint32_t lds0 = lds_offset(&smem[0]);
   auto dma_stage = [&](int kt, int buf) {
     const uint32_t l = lds0 + (uint32_t)(buf * C::STAGE);
-    // 4 scale bytes a row: the stage's own (128 wide), or the two stages' that share them
-    const int64_t sk = AT == A_MX4 ? (int64_t)kt * 4 : (int64_t)(kt >> 1) * 4;
 #pragma unroll
     for (int i = 0; i < SI; ++i) {
-      const int q = wave + 4 * i;
-      if (C::S_INS % 4 == 0 || q < C::S_INS) {
-        const uint8_t* src = q * 64 >= BN ? p.xs : (SWIGLU && q * 64 >= BN / 2 ? S2 : S1);
-        dma4(src + sk, s_off[i], l + C::XB + C::WB + q * 256);
+      const int q = wave + NW * i, r = q % SP * 64;
+      if (C::S_INS % NW == 0 || q < C::S_INS) {
+        const int64_t grp = KS < 128 ? kt / (128 / KS) : (int64_t)kt * C::SG + q / SP;
+        const uint8_t* src = r >= BN ? p.xs + grp * p.xrows * 4 : (SWIGLU && r >= BN / 2 ? S2 : S1) + grp * p.N * 4;
+        dma4(src, s_off[i], l + C::XB + C::WB + q * 256);
       }
     }
-    const char* xk = (const char*)p.x + (int64_t)kt * C::XROW;
+    const char* xk = (const char*)p.x + (int64_t)kt * XROW;
 #pragma unroll
     for (int a = 0; a < C::X_INS; ++a) dma16(xk, x_off[a], l + (wave * C::X_INS + a) * 1024);
 #pragma unroll
     for (int b = 0; b < C::W_INS; ++b) {
       const int q = (wave * C::W_INS + b) * WR;
-      dma16((SWIGLU && q >= BN / 2 ? W2 : W1) + (int64_t)kt * C::WROW, w_off[b],
+      dma16((SWIGLU && q >= BN / 2 ? W2 : W1) + (int64_t)kt * WROW, w_off[b],
             l + C::XB + (wave * C::W_INS + b) * 1024);
     }
   };
@@ -460,8 +625,9 @@ __global__ void __launch_bounds__(256, 2) mx4_gemm_kernel(Mx4Args p) {
   const int g = lane >> 5, l32 = lane & 31;
   // staged row of weight tile j of this wave: with SwiGLU its gate tiles, then its up tiles
   auto w_tile = [&](int j) -> int {
-    if constexpr (SWIGLU) return j < WT / 2 ? wn * (BN / 4) + j * 32 : BN / 2 + wn * (BN / 4) + (j - WT / 2) * 32;
-    else return wn * (BN / 2) + j * 32;
+    if constexpr (SWIGLU)
+      return j < WT / 2 ? wn * (BN / WN / 2) + j * 32 : BN / 2 + wn * (BN / WN / 2) + (j - WT / 2) * 32;
+    else return wn * (BN / WN) + j * 32;
   };
   f32x16_t acc[WT][TT];
 #pragma unroll
@@ -471,132 +637,186 @@ __global__ void __launch_bounds__(256, 2) mx4_gemm_kernel(Mx4Args p) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[j][i][r] = 0.0f;
 
-  auto compute = [&](int buf, int kt) {
-    const char* xs_ = smem + buf * C::STAGE;
-    const char* ws_ = xs_ + C::XB;
-    const char* ss_ = ws_ + C::WB;
-    if constexpr (AT == A_MX4) {
-      int sw[WT], sx[TT];
+  const int nk = (int)(p.K / KS);
+  if constexpr (AT == A_MX4) {
+    // Steps of 64: the operands of a step are read from LDS while the step before is
+    // multiplied, the first of a stage during the last of the stage before.  By then
+    // every wave has the rest of its stage in registers, so that one barrier frees
+    // the buffer for the loads of the stage after the next.  (Left to itself the
+    // compiler reads each operand just before its use: 2.2 times the time of the
+    // instructions' own.)
+    constexpr int STEPS = KS / 64;
+    static_assert(STEPS == 2 || STEPS == 4, "the operands' double buffers repeat every 4 steps");
+    i32x8_t wf[2][WT], xf[2][TT];
+    uint32_t sw[2][WT], sx[2][TT];
+    const char* w_at[WT];  // fixed parts of the addresses
+    const char* x_at[TT];
 #pragma unroll
-      for (int j = 0; j < WT; ++j) sw[j] = (int)(*(const uint32_t*)(ss_ + (w_tile(j) + l32) * 4) >> (8 * g));
+    for (int j = 0; j < WT; ++j) w_at[j] = smem + C::XB + (w_tile(j) + l32) * WROW;
 #pragma unroll
-      for (int i = 0; i < TT; ++i)
-        sx[i] = (int)(*(const uint32_t*)(ss_ + (BN + wm * (BM / 2) + i * 32 + l32) * 4) >> (8 * g));
+    for (int i = 0; i < TT; ++i) x_at[i] = smem + (wm * (BM / WM) + i * 32 + l32) * XROW;
+    const char* s_at = smem + C::XB + C::WB + l32 * 4;
+    // step u (of 4) is step u % STEPS of a stage
+    auto read = [&](int buf, int u) {
+      const int st = u % STEPS, o = buf * C::STAGE, c = st * 2 + g, to = u & 1;
+      if (u % 2 == 0) {  // the scales of a group of 128
+        const int sb = st / 2;
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        i32x8_t wf[WT], xf[TT];
+        for (int j = 0; j < WT; ++j)
+          sw[u / 2][j] = *(const uint32_t*)(s_at + o + (sb * C::SROWS + w_tile(j)) * 4);
+#pragma unroll
+        for (int i = 0; i < TT; ++i)
+          sx[u / 2][i] = *(const uint32_t*)(s_at + o + (sb * C::SROWS + BN + wm * (BM / WM) + i * 32) * 4);
+      }
+      // tiles are 32 rows apart, which the swizzles do not see
+#pragma unroll
+      for (int i = 0; i < TT; ++i) xf[to][i] = mx4_operand(*(const uint4*)(x_at[i] + o + mx4_swz<XROW>(l32, c) * 16));
+#pragma unroll
+      for (int j = 0; j < WT; ++j) wf[to][j] = mx4_operand(*(const uint4*)(w_at[j] + o + mx4_swz<WROW>(l32, c) * 16));
+    };
+    auto multiply = [&](int u) {
+      if (u % 2 == 0) {  // this lane's blocks, g and g + 2 of the four, to bytes 0 and 2
+#pragma unroll
+        for (int j = 0; j < WT; ++j) sw[u / 2][j] >>= 8 * g;
+#pragma unroll
+        for (int i = 0; i < TT; ++i) sx[u / 2][i] >>= 8 * g;
+      }
+#pragma unroll
+      for (int j = 0; j < WT; ++j)
+#pragma unroll
+        for (int i = 0; i < TT; ++i)
+          acc[j][i] = u % 2 == 0
+              ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[0][j], xf[0][i], acc[j][i], 4, 4, 0,
+                                                                (int)sw[u / 2][j], 0, (int)sx[u / 2][i])
+              : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[1][j], xf[1][i], acc[j][i], 4, 4, 2,
+                                                                (int)sw[u / 2][j], 2, (int)sx[u / 2][i]);
+    };
+#pragma unroll
+    for (int s = 0; s < NSTAGE; ++s) dma_stage(s < nk ? s : nk - 1, s);
+    wait_vm<C::DMA_MIN * (NSTAGE - 1)>();
+    __syncthreads();
+    read(0, 0);
+    int buf = 0;
+    for (int kt = 0; kt < nk; kt += 4 / STEPS) {  // K is a multiple of 256
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if ((u + 1) % STEPS != 0) {
+          read(buf, u + 1);
+        } else {
+          const int next = buf + 1 == NSTAGE ? 0 : buf + 1, ks = kt + u / STEPS + NSTAGE;
+          wait_vm<C::DMA_MIN * (NSTAGE - 2)>();
+          __syncthreads();
+          dma_stage(ks < nk ? ks : nk - 1, buf);
+          read(next, (u + 1) & 3);
+          buf = next;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(u);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    wait_vm<0>();
+  } else {
+    auto compute = [&](int buf, int kt) {
+      const char* xs_ = smem + buf * C::STAGE;
+      const char* ws_ = xs_ + C::XB;
+      const char* ss_ = ws_ + C::WB;
+#pragma unroll
+      for (int h = 0; h < KS / 64; ++h) {
+        const int sh = 8 * g + 16 * (KS < 128 ? kt & 1 : h & 1);
+        uint4 wc[WT];  // codes of block g of each weight row, and its scale
+        float sc[WT];
 #pragma unroll
         for (int j = 0; j < WT; ++j) {
           const int r = w_tile(j) + l32;
-          wf[j] = mx4_operand(*(const uint4*)(ws_ + r * 64 + (((ks * 2 + g) ^ swz_b(r)) << 4)));
+          wc[j] = *(const uint4*)(ws_ + r * WROW + mx4_swz<WROW>(r, h * 2 + g) * 16);
+          sc[j] = mx4_scale((*(const uint32_t*)(ss_ + (h / 2 * C::SROWS + r) * 4) >> sh) & 255u);
         }
 #pragma unroll
-        for (int i = 0; i < TT; ++i) {
-          const int r = wm * (BM / 2) + i * 32 + l32;
-          xf[i] = mx4_operand(*(const uint4*)(xs_ + r * 64 + (((ks * 2 + g) ^ swz_b(r)) << 4)));
-        }
+        for (int q = 0; q < 4; ++q) {
+          constexpr int NT = AT == A_F32 ? 3 : 1;
+          bf16x8_t xf[TT][NT];
 #pragma unroll
-        for (int j = 0; j < WT; ++j)
+          for (int i = 0; i < TT; ++i) {
+            const int r = wm * (BM / WM) + i * 32 + l32;
+            if constexpr (AT == A_BF16) {
+              xf[i][0] = *(const bf16x8_t*)(xs_ + r * XROW + mx4_swz<XROW>(r, h * 8 + g * 4 + q) * 16);
+            } else {
+              const float4 a = *(const float4*)(xs_ + r * XROW + mx4_swz<XROW>(r, h * 16 + g * 8 + q * 2) * 16);
+              const float4 b = *(const float4*)(xs_ + r * XROW + mx4_swz<XROW>(r, h * 16 + g * 8 + q * 2 + 1) * 16);
+              const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+              bf16x8_t t[3];
+              mx4_split3(v, t);
 #pragma unroll
-          for (int i = 0; i < TT; ++i)
-            acc[j][i] = ks == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[j], xf[i], acc[j][i], 4, 4, 0,
-                                                                                 sw[j], 0, sx[i])
-                                : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[j], xf[i], acc[j][i], 4, 4, 2,
-                                                                                 sw[j], 2, sx[i]);
-      }
-    } else {
-      // codes of block g of each weight row, and its scale
-      uint4 wc[WT];
-      float sc[WT];
+              for (int k = 0; k < NT; ++k) xf[i][k] = t[k];
+            }
+          }
 #pragma unroll
-      for (int j = 0; j < WT; ++j) {
-        const int r = w_tile(j) + l32;
-        wc[j] = *(const uint4*)(ws_ + r * 32 + ((g ^ swz_c(r)) << 4));
-        sc[j] = mx4_scale((*(const uint32_t*)(ss_ + r * 4) >> (8 * g + 16 * (kt & 1))) & 255u);
-      }
+          for (int j = 0; j < WT; ++j) {
+            const uint32_t c = q == 0 ? wc[j].x : q == 1 ? wc[j].y : q == 2 ? wc[j].z : wc[j].w;
+            const bf16x8_t wf = __builtin_bit_cast(bf16x8_t, mx4_decode8(c, sc[j]));
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        constexpr int NT = AT == A_F32 ? 3 : 1;
-        bf16x8_t xf[TT][NT];
+            for (int i = 0; i < TT; ++i)
 #pragma unroll
-        for (int i = 0; i < TT; ++i) {
-          const int r = wm * (BM / 2) + i * 32 + l32;
-          if constexpr (AT == A_BF16) {
-            xf[i][0] = *(const bf16x8_t*)(xs_ + r * 128 + (((g * 4 + q) ^ swz_a(r)) << 4));
-          } else {
-            const float4 a = *(const float4*)(xs_ + r * 256 + (((g * 8 + q * 2) ^ (r & 15)) << 4));
-            const float4 b = *(const float4*)(xs_ + r * 256 + (((g * 8 + q * 2 + 1) ^ (r & 15)) << 4));
-            const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            bf16x8_t t[3];
-            mx4_split3(v, t);
-#pragma unroll
-            for (int k = 0; k < NT; ++k) xf[i][k] = t[k];
+              for (int k = 0; k < NT; ++k)
+                acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf, xf[i][k], acc[j][i], 0, 0, 0);
           }
         }
-#pragma unroll
-        for (int j = 0; j < WT; ++j) {
-          const uint32_t c = q == 0 ? wc[j].x : q == 1 ? wc[j].y : q == 2 ? wc[j].z : wc[j].w;
-          const bf16x8_t wf = __builtin_bit_cast(bf16x8_t, mx4_decode8(c, sc[j]));
-#pragma unroll
-          for (int i = 0; i < TT; ++i)
-#pragma unroll
-            for (int k = 0; k < NT; ++k)
-              acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf, xf[i][k], acc[j][i], 0, 0, 0);
-        }
       }
-    }
-  };
-
-  // Stage kt is complete when at most the loads of the later stages are outstanding;
-  // the barrier publishes it and frees the buffer of stage kt - 1.  Stages past the
-  // end load the last one again into a buffer nobody reads.
-  const int nk = (int)(p.K / C::KS);
+    };
+    // Stage kt is complete when at most the loads of the later stages are outstanding;
+    // the barrier publishes it and frees the buffer of stage kt - 1.  Stages past the
+    // end load the last one again into a buffer nobody reads.
 #pragma unroll
-  for (int s = 0; s + 1 < NSTAGE; ++s) dma_stage(s < nk ? s : nk - 1, s);
-  int buf = 0, nbuf = NSTAGE - 1;
-  for (int kt = 0; kt < nk; ++kt) {
-    wait_vm<C::DMA_MIN * (NSTAGE - 2)>();
-    __syncthreads();
-    const int ks = kt + NSTAGE - 1;
-    dma_stage(ks < nk ? ks : nk - 1, nbuf);
-    compute(buf, kt);
-    buf = buf + 1 == NSTAGE ? 0 : buf + 1;
-    nbuf = nbuf + 1 == NSTAGE ? 0 : nbuf + 1;
+    for (int s = 0; s + 1 < NSTAGE; ++s) dma_stage(s < nk ? s : nk - 1, s);
+    int buf = 0, nbuf = NSTAGE - 1;
+    for (int kt = 0; kt < nk; ++kt) {
+      wait_vm<C::DMA_MIN * (NSTAGE - 2)>();
+      __syncthreads();
+      const int ks = kt + NSTAGE - 1;
+      dma_stage(ks < nk ? ks : nk - 1, nbuf);
+      compute(buf, kt);
+      buf = buf + 1 == NSTAGE ? 0 : buf + 1;
+      nbuf = nbuf + 1 == NSTAGE ? 0 : nbuf + 1;
+    }
+    wait_vm<0>();
   }
-  wait_vm<0>();
 
   // ---- epilogue: 16 consecutive outputs of one row a lane -------------------------
   constexpr int OTW = SWIGLU ? WT / 2 : WT;
+  const bool inside = n0 + BNO <= p.N;  // of the whole workgroup: no column past N
+  const bool whole = OT != O_MX4 && n0 + BNO <= p.ldy && p.ldy % 8 == 0;
 #pragma unroll
   for (int i = 0; i < TT; ++i) {
-    const int lr = wm * (BM / 2) + i * 32 + l32;
+    const int lr = wm * (BM / WM) + i * 32 + l32;
     const bool live = lr < rows;
     const int64_t row = row0 + lr;
 #pragma unroll
     for (int j = 0; j < OTW; ++j) {
-      const int64_t nb0 = n0 + wn * (BNO / 2) + j * 32, n = nb0 + g * 16;
+      const int64_t nb0 = n0 + wn * (BNO / WN) + j * 32, n = nb0 + g * 16;
       float v[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
+      for (int r = 0; r < 16; ++r)
         v[r] = SWIGLU ? mx4_swiglu(acc[j][i][r], acc[j + WT / 2 < WT ? j + WT / 2 : j][i][r]) : acc[j][i][r];
-        if (nb0 + 32 > p.N && n + r >= p.N) v[r] = 0.0f;  // padding
+      if (!inside) {  // padding
+        const int left = (int)(p.N - n < 16 ? p.N - n : 16);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) v[r] = r < left ? v[r] : 0.0f;
       }
       if constexpr (OT == O_MX4) {
-        uint32_t m = 0;
+        float m = __builtin_fabsf(v[0]);  // NaN stays NaN
 #pragma unroll
-        for (int r = 0; r < 16; ++r) m = max(m, __float_as_uint(v[r]) & 0x7fffffffu);
-        m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
-        const uint32_t byte = mx4_scale_byte(m);
-        const float* v0 = v;
-        const uint32_t lo = mx4_encode8(v0, byte), hi = mx4_encode8(v0 + 8, byte);
+        for (int r = 1; r < 16; ++r) m = __builtin_elementwise_maximum(m, __builtin_fabsf(v[r]));
+        m = __builtin_elementwise_maximum(m, __shfl_xor(m, 32, 64));
+        const uint32_t byte = mx4_scale_byte(__float_as_uint(m) & 0x7fffffffu);
+        const uint32_t lo = mx4_encode8(v, byte), hi = mx4_encode8(v + 8, byte);
         const int64_t b = row * p.ldy + nb0 / MX4_BLOCK;
         if (live && nb0 / MX4_BLOCK < p.ldy) {
           *(uint2*)((uint8_t*)p.y + b * 16 + g * 8) = make_uint2(lo, hi);
-          if (g == 0) p.ys[b] = (uint8_t)byte;
+          if (g == 0) p.ys[(nb0 / MX4_GROUP * p.yrows + row) * 4 + nb0 % MX4_GROUP / MX4_BLOCK] = (uint8_t)byte;
         }
-      } else if (live && n < p.ldy) {
+      } else if (live) {
         const int64_t o = row * p.ldy + n;
-        const bool whole = n + 16 <= p.ldy && p.ldy % 8 == 0;
         if constexpr (OT == O_BF16) {
           uint32_t u[8];
 #pragma unroll
@@ -627,35 +847,109 @@ __global__ void __launch_bounds__(256, 2) mx4_gemm_kernel(Mx4Args p) {
   }
 }
 
-template <int AT, int OT, bool SWIGLU, int BM, int BN, int NSTAGE>
+template <int AT, int OT, bool SWIGLU, int BM, int BN, int WM, int WN, int KS, int NSTAGE>
 int launch_gemm_cfg(const Mx4Args& p, int64_t m_tiles, hipStream_t stream) {
   constexpr int BNO = SWIGLU ? BN / 2 : BN;
   const int64_t n_tiles = (mx4_cols<OT>(p) + BNO - 1) / BNO;
   if (m_tiles * n_tiles > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: too many tiles");
-  hipLaunchKernelGGL((mx4_gemm_kernel<AT, OT, SWIGLU, BM, BN, NSTAGE>), dim3((unsigned)(m_tiles * n_tiles)),
-                     dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((mx4_gemm_kernel<AT, OT, SWIGLU, BM, BN, WM, WN, KS, NSTAGE>),
+                     dim3((unsigned)(m_tiles * n_tiles)), dim3(WM * WN * 64), 0, stream, p);
   return check_launch("mx4_gemm_kernel");
 }
 
-// Whether mx4_gemm_kernel takes the call: whole 128-wide stages, 16-byte rows, and
-// 32-bit offsets from the activations' and an expert's codes.  xrows: rows of x.
-bool gemm_ok(const Mx4Args& p, int at, int64_t xrows) {
-  const int64_t xbytes = xrows * p.ldx * (at == A_MX4 ? 16 : at == A_BF16 ? 2 : 4);
-  return p.K % 128 == 0 && p.ldw % 4 == 0 && p.N * p.ldw * 16 < (1LL << 32) && xbytes < (1LL << 32) &&
-         ((uintptr_t)p.x & 15) == 0 && ((uintptr_t)p.w & 15) == 0 && ((uintptr_t)p.s & 3) == 0 &&
-         (!p.w2 || (((uintptr_t)p.w2 & 15) == 0 && ((uintptr_t)p.s2 & 3) == 0)) && ((uintptr_t)p.y & 15) == 0;
+// Whether mx4_gemm_kernel's 32-bit offsets reach the rows: `xrows` activations of K
+// values, an expert's N rows.
+bool gemm_fits(int at, int64_t xrows, int64_t K, int64_t N) {
+  const int64_t ng = mx4_groups(K);
+  return xrows * ng * (at == A_MX4 ? 64 : at == A_BF16 ? 256 : 512) < (1LL << 32) && N * ng * 64 < (1LL << 32);
 }
 
-constexpr int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
-bool aligned(const void* p, int to) { return ((uintptr_t)p & (to - 1)) == 0; }
-bool dtype_ok(int d) { return d == SMAUL_DTYPE_F32 || d == SMAUL_DTYPE_BF16; }
+// out[t] = the sum of its slots' rows times their weights, in ascending expert order
+// (fp32, product and sum rounded each, as smaul_moe_combine's), in x's type.  The
+// slots' rows stay fp32 where the hidden rows were rounded to bf16 already: one
+// rounding less between the experts and the sum.  A thread has 8 columns; every row
+// is read before the first is used.
+template <bool YF32, bool OBF16, int KM>
+__global__ void __launch_bounds__(256)
+mx4_combine_kernel(const void* __restrict__ y, const int64_t* __restrict__ topi, const float* __restrict__ topw,
+                   const int32_t* __restrict__ inv, void* __restrict__ out, int64_t T, int d, int k) {
+  const int cpt = d / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, t = i / cpt;
+  if (t >= T) return;
+  const int c = (int)(i - t * cpt) * 8;
+  int pos[KM], key[KM];
+  float w[KM];
+#pragma unroll
+  for (int j = 0; j < KM; ++j)
+    if (j < k) {
+      pos[j] = inv[t * k + j];
+      key[j] = (int)topi[t * k + j];
+      w[j] = topw[t * k + j];
+    }
+#pragma unroll
+  for (int j = 0; j < KM; ++j)
+    if (j >= k || pos[j] < 0) {
+      pos[j] = -1;
+      key[j] = 0x7fffffff;
+      w[j] = 0.0f;
+    }
+#pragma unroll
+  for (int pass = 0; pass < KM; ++pass)
+#pragma unroll
+    for (int j = pass & 1; j + 1 < KM; j += 2) {
+      const bool swap = key[j] > key[j + 1];
+      const int k0 = key[j], p0 = pos[j];
+      const float w0 = w[j];
+      key[j] = swap ? key[j + 1] : k0;
+      pos[j] = swap ? pos[j + 1] : p0;
+      w[j] = swap ? w[j + 1] : w0;
+      key[j + 1] = swap ? k0 : key[j + 1];
+      pos[j + 1] = swap ? p0 : pos[j + 1];
+      w[j + 1] = swap ? w0 : w[j + 1];
+    }
+  float v[KM][8];
+#pragma unroll
+  for (int j = 0; j < KM; ++j)
+    if (pos[j] >= 0) mx4_load8<!YF32, true>(y, pos[j], d, c, v[j]);
+  float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < KM; ++j)
+    if (pos[j] >= 0)
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float pr = v[j][q] * w[j];
+        acc[q] = acc[q] + pr;
+      }
+  const int64_t o = t * d + c;
+  if constexpr (OBF16) {
+    *(uint4*)((uint16_t*)out + o) = make_uint4(pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3]),
+                                               pack_bf16(acc[4], acc[5]), pack_bf16(acc[6], acc[7]));
+  } else {
+    ((float4*)((float*)out + o))[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    ((float4*)((float*)out + o))[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+  }
+}
+
+template <bool YF32, bool OBF16>
+int launch_combine(const void* y, const int64_t* topi, const float* topw, const int32_t* inv, void* out, int64_t T,
+                   int64_t d, int64_t k, hipStream_t stream) {
+  const dim3 grid((unsigned)((T * (d / 8) + 255) / 256)), block(256);
+#define SMAUL_C(KM) \
+  hipLaunchKernelGGL((mx4_combine_kernel<YF32, OBF16, KM>), grid, block, 0, stream, y, topi, topw, inv, out, T, (int)d, (int)k)
+  if (k <= 2) SMAUL_C(2);
+  else if (k <= 4) SMAUL_C(4);
+  else SMAUL_C(8);
+#undef SMAUL_C
+  return check_launch("mx4_combine_kernel");
+}
 
 int launch_quantize(const void* x, int dtype, uint8_t* codes, uint8_t* scales, int64_t rows, int64_t K,
                     hipStream_t stream) {
   const int64_t threads = rows * mx4_blocks(K) * 4;
   if (threads > 256LL * 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_quantize: too many values");
-  const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
   const bool vec = K % MX4_BLOCK == 0 && aligned(x, 16), bf16 = dtype == SMAUL_DTYPE_BF16;
+  const int64_t per = vec ? 256 * MX4_U : 256;
+  const dim3 grid((unsigned)((threads + per - 1) / per)), block(256);
 #define SMAUL_Q(B, V) \
   hipLaunchKernelGGL((mx4_quantize_kernel<B, V>), grid, block, 0, stream, x, (uint32_t*)codes, scales, rows, K)
   if (bf16) { if (vec) SMAUL_Q(true, true); else SMAUL_Q(true, false); }
@@ -666,13 +960,14 @@ int launch_quantize(const void* x, int dtype, uint8_t* codes, uint8_t* scales, i
 
 // row tiles of the two product kernels
 constexpr int64_t TILE_BM = 64;
-int64_t gemm_bm(int at) { return at == A_F32 ? 64 : 128; }
+int64_t gemm_bm(int at) { return at == A_F32 ? 64 : at == A_MX4 ? 256 : 128; }
 
 template <int AT, int OT, bool SWIGLU>
 int launch_product(const Mx4Args& p, bool gemm, int64_t m_tiles, hipStream_t stream) {
   if (!gemm) return launch_tiles<AT, OT, SWIGLU, false>(p, m_tiles, stream);
-  if constexpr (AT == A_F32) return launch_gemm_cfg<AT, OT, SWIGLU, 64, 256, 3>(p, m_tiles, stream);
-  else return launch_gemm_cfg<AT, OT, SWIGLU, 128, 256, 3>(p, m_tiles, stream);
+  if constexpr (AT == A_F32) return launch_gemm_cfg<AT, OT, SWIGLU, 64, 256, 2, 2, 64, 3>(p, m_tiles, stream);
+  else if constexpr (AT == A_BF16) return launch_gemm_cfg<AT, OT, SWIGLU, 128, 256, 2, 2, 64, 3>(p, m_tiles, stream);
+  else return launch_gemm_cfg<AT, OT, SWIGLU, 256, 256, 4, 2, 256, 2>(p, m_tiles, stream);
 }
 
 // activations with a weight: y of `out` type
@@ -680,8 +975,65 @@ int launch_linear(const Mx4Args& p, int at, int out, bool gemm, int64_t m_tiles,
   if (at == A_MX4)
     return out == O_BF16 ? launch_product<A_MX4, O_BF16, false>(p, gemm, m_tiles, stream)
                          : launch_product<A_MX4, O_F32, false>(p, gemm, m_tiles, stream);
-  return at == A_BF16 ? launch_product<A_BF16, O_BF16, false>(p, gemm, m_tiles, stream)
-                      : launch_product<A_F32, O_F32, false>(p, gemm, m_tiles, stream);
+  if (at == A_BF16)
+    return out == O_BF16 ? launch_product<A_BF16, O_BF16, false>(p, gemm, m_tiles, stream)
+                         : launch_product<A_BF16, O_F32, false>(p, gemm, m_tiles, stream);
+  return launch_product<A_F32, O_F32, false>(p, gemm, m_tiles, stream);
+}
+
+int launch_prep(Mx4Prep p, int dtype, int64_t E, hipStream_t stream) {
+  int64_t blocks = 0;
+  if (p.xmode != P_NONE) {
+    p.xblocks = (p.T + 15) / 16 * ((mx4_groups(p.K) + 3) / 4);
+    p.xvec = aligned(p.x, 16) && p.K % (dtype == SMAUL_DTYPE_BF16 ? 8 : 4) == 0;
+    blocks += p.xblocks;
+  }
+  for (auto& m : p.m) {
+    if (m.w) m.blocks = (E * mx4_groups(m.K) * m.N + 255) / 256;
+    blocks += m.blocks;
+  }
+  if (blocks > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: too many rows");
+  if (dtype == SMAUL_DTYPE_BF16) hipLaunchKernelGGL(mx4_prep_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, stream, p, E);
+  else hipLaunchKernelGGL(mx4_prep_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, stream, p, E);
+  return check_launch("mx4_prep_kernel");
+}
+
+// a workspace laid out part by part
+struct Parts {
+  int64_t at = 0;
+  int64_t take(int64_t bytes) {
+    const int64_t here = at;
+    at += align256(bytes);
+    return here;
+  }
+};
+
+// A linear's workspace: the activations rounded or in padded rows, and the weight's
+// scales (and padded codes) as the GEMM reads them.  Up to 64 rows the tile kernel
+// reads the stored weight.
+struct LinearParts {
+  bool gemm;
+  int64_t x, xs, st, wp, total;
+};
+LinearParts linear_parts(int64_t rows, int64_t K, int64_t N, int dtype, int act) {
+  const bool mx4 = act == SMAUL_ACT_MX4;
+  const int at = mx4 ? A_MX4 : dtype == SMAUL_DTYPE_BF16 ? A_BF16 : A_F32;
+  const int64_t ng = mx4_groups(K), nb = mx4_blocks(K);
+  const bool pad = K % MX4_STAGE != 0;
+  LinearParts q{};
+  Parts w;
+  q.gemm = rows > TILE_BM && gemm_fits(at, rows, K, N);
+  if (!q.gemm) {
+    q.x = w.take(mx4 ? rows * nb * 16 : 0);
+    q.xs = w.take(mx4 ? rows * nb : 0);
+  } else {
+    q.x = w.take(mx4 ? rows * ng * 64 : pad ? rows * ng * MX4_GROUP * (at == A_BF16 ? 2 : 4) : 0);
+    q.xs = w.take(mx4 ? rows * ng * 4 : 0);
+    q.st = w.take(N * ng * 4);
+    q.wp = w.take(pad ? N * ng * 64 : 0);
+  }
+  q.total = w.at;
+  return q;
 }
 
 }  // namespace
@@ -705,8 +1057,9 @@ int smaul_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* y, i
   if (!aligned(codes, 4)) return fail(SMAUL_ERR_INVALID, "mx4_dequantize: codes must be 4-byte aligned");
   const int64_t threads = rows * mx4_blocks(K) * 4;
   if (threads > 256LL * 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_dequantize: too many values");
-  const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
   const bool vec = K % MX4_BLOCK == 0 && aligned(y, 16), bf16 = dtype == SMAUL_DTYPE_BF16;
+  const int64_t per = vec ? 256 * MX4_U : 256;
+  const dim3 grid((unsigned)((threads + per - 1) / per)), block(256);
 #define SMAUL_D(B, V) \
   hipLaunchKernelGGL((mx4_dequantize_kernel<B, V>), grid, block, 0, stream, (const uint32_t*)codes, scales, y, rows, K)
   if (bf16) { if (vec) SMAUL_D(true, true); else SMAUL_D(true, false); }
@@ -715,9 +1068,9 @@ int smaul_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* y, i
   return check_launch("mx4_dequantize_kernel");
 }
 
-int64_t smaul_mx4_linear_workspace_size(int64_t rows, int64_t in_f, int64_t out_f, int act) {
-  if (rows < 0 || in_f <= 0 || out_f <= 0) return -1;
-  return act == SMAUL_ACT_MX4 ? align256(rows * mx4_blocks(in_f) * 16) + align256(rows * mx4_blocks(in_f)) : 0;
+int64_t smaul_mx4_linear_workspace_size(int64_t rows, int64_t in_f, int64_t out_f, int dtype, int act) {
+  if (rows < 0 || in_f <= 0 || out_f <= 0 || !dtype_ok(dtype)) return -1;
+  return linear_parts(rows, in_f, out_f, dtype, act).total;
 }
 
 int smaul_mx4_linear(const void* x, int dtype, const uint8_t* w, const uint8_t* s, void* y, int64_t rows,
@@ -727,13 +1080,18 @@ int smaul_mx4_linear(const void* x, int dtype, const uint8_t* w, const uint8_t* 
     return fail(SMAUL_ERR_INVALID, "mx4_linear: bad sizes, dtype or act");
   if (rows == 0) return SMAUL_OK;
   if (!x || !w || !s || !y) return fail(SMAUL_ERR_INVALID, "mx4_linear: null pointer");
-  if (!aligned(w, 16)) return fail(SMAUL_ERR_INVALID, "mx4_linear: codes must be 16-byte aligned");
-  const int64_t need = smaul_mx4_linear_workspace_size(rows, in_f, out_f, act);
-  if (workspace_bytes < need || (need > 0 && (!workspace || !aligned(workspace, 16))))
+  if (!aligned(x, 16) || !aligned(w, 16) || !aligned(y, 16))
+    return fail(SMAUL_ERR_INVALID, "mx4_linear: x, y and the codes must be 16-byte aligned");
+  const LinearParts q = linear_parts(rows, in_f, out_f, dtype, act);
+  if (workspace_bytes < q.total || (q.total > 0 && (!workspace || !aligned(workspace, 256))))
     return fail(SMAUL_ERR_INVALID, "mx4_linear: workspace %lld < %lld bytes, or unaligned", (long long)workspace_bytes,
-                (long long)need);
+                (long long)q.total);
+  const bool bf16 = dtype == SMAUL_DTYPE_BF16, mx4 = act == SMAUL_ACT_MX4, pad = in_f % MX4_STAGE != 0;
+  const int at = mx4 ? A_MX4 : bf16 ? A_BF16 : A_F32;
+  char* ws = (char*)workspace;
   Mx4Args p{};
-  p.x = x;
+  p.x = mx4 || (q.gemm && pad) ? ws + q.x : x;
+  p.xs = (uint8_t*)ws + q.xs;
   p.w = w;
   p.s = s;
   p.y = y;
@@ -741,24 +1099,32 @@ int smaul_mx4_linear(const void* x, int dtype, const uint8_t* w, const uint8_t* 
   p.K = in_f;
   p.N = out_f;
   p.E = 1;
-  const bool bf16 = dtype == SMAUL_DTYPE_BF16;
-  p.xvec = aligned(x, 16) && in_f % (bf16 ? 8 : 4) == 0;
-  int at = bf16 ? A_BF16 : A_F32;
-  if (act == SMAUL_ACT_MX4) {
-    uint8_t* codes = (uint8_t*)workspace;
-    uint8_t* scales = codes + align256(rows * mx4_blocks(in_f) * 16);
-    const int rc = launch_quantize(x, dtype, codes, scales, rows, in_f, stream);
-    if (rc) return rc;
-    p.x = codes;
-    p.xs = scales;
-    at = A_MX4;
+  p.xvec = in_f % (bf16 ? 8 : 4) == 0;
+  int rc = SMAUL_OK;
+  if (q.gemm) {
+    const int64_t ng = mx4_groups(in_f);
+    Mx4Prep f{};
+    f.m[0] = Mx4Weight{w, s, (uint32_t*)(ws + q.st), pad ? (uint4*)(ws + q.wp) : nullptr, out_f, in_f, 0};
+    f.x = x;
+    f.xo = ws + q.x;
+    f.xst = (uint32_t*)(ws + q.xs);
+    f.T = rows;
+    f.K = in_f;
+    f.xmode = mx4 ? P_ROUND : pad ? P_PAD : P_NONE;
+    rc = launch_prep(f, dtype, 1, stream);
+    p.s = (uint8_t*)ws + q.st;
+    if (pad) p.w = (uint8_t*)ws + q.wp;
+    p.K = ng * MX4_GROUP;
+    p.ldx = mx4 ? ng * 4 : p.K;
+    p.ldw = ng * 4;
+    p.ldy = out_f;
+    p.xrows = rows;
+  } else if (mx4) {
+    rc = launch_quantize(x, dtype, (uint8_t*)ws + q.x, (uint8_t*)ws + q.xs, rows, in_f, stream);
   }
-  p.ldx = at == A_MX4 ? mx4_blocks(in_f) : in_f;
-  p.ldw = mx4_blocks(in_f);
-  p.ldy = out_f;
-  const bool gemm = rows > TILE_BM && gemm_ok(p, at, rows);
-  const int64_t bm = gemm ? gemm_bm(at) : TILE_BM;
-  return launch_linear(p, at, bf16 ? O_BF16 : O_F32, gemm, (rows + bm - 1) / bm, stream);
+  if (rc) return rc;
+  const int64_t bm = q.gemm ? gemm_bm(at) : TILE_BM;
+  return launch_linear(p, at, bf16 ? O_BF16 : O_F32, q.gemm, (rows + bm - 1) / bm, stream);
 }
 
 int smaul_mx4_backward_input(const void* g, int dtype, const uint8_t* w, const uint8_t* s, void* dx, int64_t rows,
@@ -783,34 +1149,44 @@ int smaul_mx4_backward_input(const void* g, int dtype, const uint8_t* w, const u
               : launch_tiles<A_F32, O_F32, false, true>(p, (rows + 63) / 64, stream);
 }
 
-// The experts' workspace, each part 256-byte aligned: the dispatch's tables and
-// scratch, the rounded rows of x (act mx4), the hidden rows, the slots' outputs.
+// The experts' workspace: the dispatch's tables and scratch, x as the products read
+// it, the hidden rows, the weights' scales (and padded codes), the slots' outputs.
 struct Mx4MoeParts {
-  int64_t seg_off, tile_off, perm_row, perm_w, inv, scratch, scratch_bytes, xc, xs, hc, hs, y, total;
+  bool gemm;
+  int64_t seg_off, tile_off, perm_row, perm_w, inv, scratch, scratch_bytes, xc, xs, hc, hs, st[3], wp[3], y, total;
 };
 static Mx4MoeParts mx4_moe_parts(int64_t T, int64_t d, int64_t h, int64_t E, int64_t k, int dtype, int act) {
   Mx4MoeParts q{};
-  int64_t at = 0;
-  auto take = [&](int64_t bytes) {
-    const int64_t here = at;
-    at += align256(bytes);
-    return here;
-  };
-  const int64_t size = dtype == SMAUL_DTYPE_BF16 ? 2 : 4;
+  Parts w;
+  const int64_t size = dtype == SMAUL_DTYPE_BF16 ? 2 : 4, R = T * k, gd = mx4_groups(d), gh = mx4_groups(h);
   const bool mx4 = act == SMAUL_ACT_MX4;
-  q.seg_off = take((E + 1) * 4);
-  q.tile_off = take((E + 1) * 4);
-  q.perm_row = take(T * k * 4);
-  q.perm_w = take(T * k * 4);
-  q.inv = take(T * k * 4);
+  const int at = mx4 ? A_MX4 : size == 2 ? A_BF16 : A_F32;
+  q.gemm = T > TILE_BM && gemm_fits(at, T, d, h) && gemm_fits(at, R, h, d);
+  q.seg_off = w.take((E + 1) * 4);
+  q.tile_off = w.take((E + 1) * 4);
+  q.perm_row = w.take(R * 4);
+  q.perm_w = w.take(R * 4);
+  q.inv = w.take(R * 4);
   q.scratch_bytes = smaul_moe_dispatch_workspace_size(T, E);
-  q.scratch = take(q.scratch_bytes);
-  q.xc = take(mx4 ? T * mx4_blocks(d) * 16 : 0);
-  q.xs = take(mx4 ? T * mx4_blocks(d) : 0);
-  q.hc = take(mx4 ? T * k * mx4_blocks(h) * 16 : T * k * h * size);
-  q.hs = take(mx4 ? T * k * mx4_blocks(h) : 0);
-  q.y = take(T * k * d * size);
-  q.total = at;
+  q.scratch = w.take(q.scratch_bytes);
+  if (q.gemm) {
+    const bool pd = d % MX4_STAGE != 0, ph = h % MX4_STAGE != 0;
+    q.xc = w.take(mx4 ? T * gd * 64 : pd ? T * gd * MX4_GROUP * size : 0);
+    q.xs = w.take(mx4 ? T * gd * 4 : 0);
+    q.hc = w.take(mx4 ? R * gh * 64 : R * gh * MX4_GROUP * size);
+    q.hs = w.take(mx4 ? R * gh * 4 : 0);
+    for (int j = 0; j < 3; ++j) {
+      q.st[j] = w.take(E * (j < 2 ? h * gd : d * gh) * 4);
+      q.wp[j] = w.take(j < 2 ? (pd ? E * h * gd * 64 : 0) : (ph ? E * d * gh * 64 : 0));
+    }
+  } else {
+    q.xc = w.take(mx4 ? T * mx4_blocks(d) * 16 : 0);
+    q.xs = w.take(mx4 ? T * mx4_blocks(d) : 0);
+    q.hc = w.take(mx4 ? R * mx4_blocks(h) * 16 : R * h * size);
+    q.hs = w.take(mx4 ? R * mx4_blocks(h) : 0);
+  }
+  q.y = w.take(R * d * (mx4 ? 2 : 4));
+  q.total = w.at;
   return q;
 }
 
@@ -835,8 +1211,8 @@ int smaul_mx4_moe_forward(const void* x, int dtype, const int64_t* topi, const f
   if (T == 0) return SMAUL_OK;
   if (!x || !topi || !topw || !gate_w || !gate_s || !up_w || !up_s || !down_w || !down_s || !out || !counts)
     return fail(SMAUL_ERR_INVALID, "mx4_moe: null pointer");
-  if (!aligned(gate_w, 16) || !aligned(up_w, 16) || !aligned(down_w, 16) || !aligned(out, 16))
-    return fail(SMAUL_ERR_INVALID, "mx4_moe: codes and out must be 16-byte aligned");
+  if (!aligned(x, 16) || !aligned(gate_w, 16) || !aligned(up_w, 16) || !aligned(down_w, 16) || !aligned(out, 16))
+    return fail(SMAUL_ERR_INVALID, "mx4_moe: x, out and the codes must be 16-byte aligned");
   const Mx4MoeParts q = mx4_moe_parts(T, d, h, E, k, dtype, act);
   if (workspace_bytes < q.total || !workspace || !aligned(workspace, 256))
     return fail(SMAUL_ERR_INVALID, "mx4_moe: workspace %lld < %lld bytes, or unaligned", (long long)workspace_bytes,
@@ -848,57 +1224,88 @@ int smaul_mx4_moe_forward(const void* x, int dtype, const int64_t* topi, const f
   int32_t* inv = (int32_t*)(ws + q.inv);
   const bool bf16 = dtype == SMAUL_DTYPE_BF16, mx4 = act == SMAUL_ACT_MX4;
   const int at = mx4 ? A_MX4 : bf16 ? A_BF16 : A_F32;
-  const int64_t R = T * k;
+  const int64_t R = T * k, gd = mx4_groups(d), gh = mx4_groups(h);
+  const bool pd = d % MX4_STAGE != 0, ph = h % MX4_STAGE != 0;
+  const int64_t bm = q.gemm ? gemm_bm(at) : TILE_BM, m_tiles = (R + bm - 1) / bm + E;
+  int rc = smaul_moe_dispatch(topi, topw, counts, seg_off, tile_off, perm_row, (float*)(ws + q.perm_w), inv, T, E, k,
+                              bm, ws + q.scratch, q.scratch_bytes, stream);
+  if (rc) return rc;
   Mx4Args p{};
-  p.x = mx4 ? ws + q.xc : x;
-  p.xs = mx4 ? (uint8_t*)ws + q.xs : nullptr;
+  p.x = mx4 || (q.gemm && pd) ? ws + q.xc : x;
+  p.xs = (uint8_t*)ws + q.xs;
   p.row_idx = perm_row;
   p.w = gate_w;
   p.s = gate_s;
   p.w2 = up_w;
   p.s2 = up_s;
   p.y = ws + q.hc;
-  p.ys = mx4 ? (uint8_t*)ws + q.hs : nullptr;
+  p.ys = (uint8_t*)ws + q.hs;
   p.K = d;
   p.N = h;
-  p.ldx = mx4 ? mx4_blocks(d) : d;
-  p.ldw = mx4_blocks(d);
-  p.ldy = mx4 ? mx4_blocks(h) : h;
   p.seg_off = seg_off;
   p.tile_off = tile_off;
   p.E = (int)E;
-  p.xvec = aligned(x, 16) && d % 8 == 0;
+  p.xvec = d % 8 == 0;
   Mx4Args dn = p;
   dn.x = p.y;
   dn.xs = p.ys;
   dn.row_idx = nullptr;
   dn.w = down_w;
   dn.s = down_s;
-  dn.w2 = dn.s2 = nullptr;
   dn.y = ws + q.y;
-  dn.ys = nullptr;
   dn.K = h;
   dn.N = d;
-  dn.ldx = p.ldy;
-  dn.ldw = mx4_blocks(h);
-  dn.ldy = d;
   dn.xvec = h % (bf16 ? 8 : 4) == 0;
-  const bool gemm = T > 64 && gemm_ok(p, at, T) && gemm_ok(dn, at, R);
-  const int64_t bm = gemm ? gemm_bm(at) : TILE_BM, m_tiles = (R + bm - 1) / bm + E;
-  int rc = smaul_moe_dispatch(topi, topw, counts, seg_off, tile_off, perm_row, (float*)(ws + q.perm_w), inv, T, E, k,
-                              bm, ws + q.scratch, q.scratch_bytes, stream);
-  if (rc) return rc;
-  if (mx4) {
+  if (q.gemm) {
+    const uint8_t* w[3] = {gate_w, up_w, down_w};
+    const uint8_t* s[3] = {gate_s, up_s, down_s};
+    const uint8_t* at_w[3];
+    const uint8_t* at_s[3];
+    Mx4Prep f{};
+    for (int j = 0; j < 3; ++j) {
+      const bool pad = j < 2 ? pd : ph;
+      f.m[j] = Mx4Weight{w[j], s[j], (uint32_t*)(ws + q.st[j]), pad ? (uint4*)(ws + q.wp[j]) : nullptr,
+                         j < 2 ? h : d, j < 2 ? d : h, 0};
+      at_w[j] = pad ? (uint8_t*)ws + q.wp[j] : w[j];
+      at_s[j] = (uint8_t*)ws + q.st[j];
+    }
+    f.x = x;
+    f.xo = ws + q.xc;
+    f.xst = (uint32_t*)(ws + q.xs);
+    f.T = T;
+    f.K = d;
+    f.xmode = mx4 ? P_ROUND : pd ? P_PAD : P_NONE;
+    rc = launch_prep(f, dtype, E, stream);
+    p.w = at_w[0];
+    p.s = at_s[0];
+    p.w2 = at_w[1];
+    p.s2 = at_s[1];
+    p.K = gd * MX4_GROUP;
+    p.ldx = mx4 ? gd * 4 : p.K;
+    p.ldw = gd * 4;
+    p.ldy = mx4 ? gh * 4 : gh * MX4_GROUP;
+    p.xrows = T;
+    p.yrows = R;
+    dn.w = at_w[2];
+    dn.s = at_s[2];
+    dn.K = gh * MX4_GROUP;
+    dn.ldx = p.ldy;
+    dn.ldw = gh * 4;
+    dn.ldy = d;
+    dn.xrows = R;
+  } else if (mx4) {
     rc = launch_quantize(x, dtype, (uint8_t*)ws + q.xc, (uint8_t*)ws + q.xs, T, d, stream);
-    if (rc) return rc;
   }
-  rc = mx4 ? launch_product<A_MX4, O_MX4, true>(p, gemm, m_tiles, stream)
-           : bf16 ? launch_product<A_BF16, O_BF16, true>(p, gemm, m_tiles, stream)
-                  : launch_product<A_F32, O_F32, true>(p, gemm, m_tiles, stream);
   if (rc) return rc;
-  rc = launch_linear(dn, at, bf16 ? O_BF16 : O_F32, gemm, m_tiles, stream);
+  rc = mx4 ? launch_product<A_MX4, O_MX4, true>(p, q.gemm, m_tiles, stream)
+           : bf16 ? launch_product<A_BF16, O_BF16, true>(p, q.gemm, m_tiles, stream)
+                  : launch_product<A_F32, O_F32, true>(p, q.gemm, m_tiles, stream);
   if (rc) return rc;
-  return smaul_moe_combine(ws + q.y, dtype, topi, topw, inv, out, T, d, k, stream);
+  rc = launch_linear(dn, at, mx4 ? O_BF16 : O_F32, q.gemm, m_tiles, stream);
+  if (rc) return rc;
+  return mx4 ? launch_combine<false, true>(ws + q.y, topi, topw, inv, out, T, d, k, stream)
+             : bf16 ? launch_combine<true, true>(ws + q.y, topi, topw, inv, out, T, d, k, stream)
+                    : launch_combine<true, false>(ws + q.y, topi, topw, inv, out, T, d, k, stream);
 }
 
 }  // extern "C"

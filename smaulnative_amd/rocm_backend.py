@@ -576,7 +576,7 @@ class RocmBackend:
         x, w, s = self._mx4_product_check("mx4_forward", "x", x, w, s, in_f, out_f, in_f)
         rows, a = x.shape[0], _lib.ACTS[act]
         y = torch.empty(rows, out_f, dtype=x.dtype, device=x.device)
-        nws = lib.smaul_mx4_linear_workspace_size(rows, in_f, out_f, a)
+        nws = lib.smaul_mx4_linear_workspace_size(rows, in_f, out_f, _ACT[x.dtype], a)
         ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws > 0 else None
         with _device(x.device):
             rc = lib.smaul_mx4_linear(x.data_ptr(), _ACT[x.dtype], w.data_ptr(), s.data_ptr(), y.data_ptr(), rows, in_f,

@@ -50,14 +50,14 @@ def test_mx4_arguments():
     assert lib.smaul_mx4_dequantize(P, P, None, 0, 4, 32, None) == bad
     assert lib.smaul_mx4_dequantize(P + 1, P, P, 0, 4, 32, None) == bad
     for act in (0, 1):
-        need = lib.smaul_mx4_linear_workspace_size(100, 64, 32, act)
+        need = lib.smaul_mx4_linear_workspace_size(100, 64, 32, 1, act)
         assert need >= (100 * 2 * 17 if act else 0)
         assert lib.smaul_mx4_linear(P, 1, P, P, P, 100, 64, 32, act, None, max(need, 1) - 1, None) == bad or need == 0
         assert lib.smaul_mx4_linear(P, 1, P + 4, P, P, 100, 64, 32, act, P, need, None) == bad
         assert lib.smaul_mx4_linear(P, 1, P, P, P, 0, 64, 32, act, None, 0, None) == _lib.SMAUL_OK
     assert lib.smaul_mx4_linear(P, 1, P, P, P, 100, 64, 32, 2, P, 1 << 20, None) == bad
     assert lib.smaul_mx4_linear(P, 1, P, P, P, 100, 0, 32, 0, None, 0, None) == bad
-    assert lib.smaul_mx4_linear_workspace_size(-1, 64, 32, 1) == -1
+    assert lib.smaul_mx4_linear_workspace_size(-1, 64, 32, 1, 1) == -1
     assert lib.smaul_mx4_backward_input(P, 0, P, P, None, 4, 64, 32, None) == bad
     assert lib.smaul_mx4_backward_input(P, 0, P + 8, P, P, 4, 64, 32, None) == bad
     size = lib.smaul_mx4_moe_workspace_size(64, 128, 256, 8, 2, 1, 1)
