@@ -538,9 +538,14 @@ int smaul_mx4_linear(const void* x, int dtype, const uint8_t* w, const uint8_t* 
                      int64_t in_f, int64_t out_f, int act, void* workspace, int64_t workspace_bytes,
                      hipStream_t stream);
 
-/* dx[rows, in_f] = g[rows, out_f] . decode(w, s): its input gradient (x as it is), g and dx of dtype. */
+/*
+ * dx[rows, in_f] = g[rows, out_f] . decode(w, s): its input gradient (x as it is), g and
+ * dx of dtype; g, w and dx 16-byte aligned, the workspace 256.
+ */
+int64_t smaul_mx4_backward_input_workspace_size(int64_t rows, int64_t in_f, int64_t out_f, int dtype);
 int smaul_mx4_backward_input(const void* g, int dtype, const uint8_t* w, const uint8_t* s, void* dx, int64_t rows,
-                             int64_t in_f, int64_t out_f, hipStream_t stream);
+                             int64_t in_f, int64_t out_f, void* workspace, int64_t workspace_bytes,
+                             hipStream_t stream);
 
 /*
  * The routed SwiGLU experts in that format: out[t] = sum over t's slots, ascending

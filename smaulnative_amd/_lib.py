@@ -80,7 +80,8 @@ SIGNATURES = {
     "smaul_mx4_dequantize": (_I, [_P, _P, _P, _I, _I64, _I64, _P]),
     "smaul_mx4_linear_workspace_size": (_I64, [_I64, _I64, _I64, _I, _I]),
     "smaul_mx4_linear": (_I, [_P, _I, _P, _P, _P, _I64, _I64, _I64, _I, _P, _I64, _P]),
-    "smaul_mx4_backward_input": (_I, [_P, _I, _P, _P, _P, _I64, _I64, _I64, _P]),
+    "smaul_mx4_backward_input_workspace_size": (_I64, [_I64, _I64, _I64, _I]),
+    "smaul_mx4_backward_input": (_I, [_P, _I, _P, _P, _P, _I64, _I64, _I64, _P, _I64, _P]),
     "smaul_mx4_moe_workspace_size": (_I64, [_I64, _I64, _I64, _I64, _I64, _I, _I]),
     "smaul_mx4_moe_forward": (_I, [_P, _I] + [_P] * 10 + [_I64, _I64, _I64, _I64, _I64, _I, _P, _I64, _P]),
     "smaul_peak_mfma": (_I, [_P, _I, _I, _P]),

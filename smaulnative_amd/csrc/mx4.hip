@@ -7,7 +7,7 @@
 //
 // A code and its scale are exact in bf16, so every product of the matrix cores is
 // exact for bf16 activations and for activations in the format itself, and its
-// sums are fp32; fp32 activations are two bf16 terms (hi + lo).
+// sums are fp32; fp32 activations are three bf16 terms, all of their 24 bits.
 #include "lds_dma.h"
 #include "mx4.h"
 
@@ -258,11 +258,44 @@ __global__ void __launch_bounds__(256) mx4_prep_kernel(Mx4Prep p, int64_t E) {
   }
 }
 
+// The weight turned round, for the input gradient: wt[i][o] = W[o][i] in bf16, rows of
+// ldo values (zeros from O on).  A workgroup: 64 o by 64 i, through LDS.
+__global__ void __launch_bounds__(256)
+mx4_turn_kernel(const uint8_t* __restrict__ w, const uint8_t* __restrict__ s, uint16_t* __restrict__ wt, int64_t O,
+                int64_t I, int64_t ldo) {
+  constexpr int LD = 72;  // 16-byte rows of 64 o, off the banks' period
+  __shared__ __attribute__((aligned(16))) uint16_t sh[64 * LD];
+  const int64_t nb = mx4_blocks(I), ti = (I + 63) / 64;
+  const int64_t i0 = blockIdx.x % ti * 64, o0 = blockIdx.x / ti * 64;
+  {
+    const int o = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
+    const int64_t b = (i0 + c) / MX4_BLOCK;
+    uint2 codes = make_uint2(0, 0);
+    float sc = 1.0f;
+    if (o0 + o < O && b < nb) {
+      codes = *(const uint2*)(w + ((o0 + o) * nb + b) * 16 + (c & 16) / 2);
+      sc = mx4_scale(s[(o0 + o) * nb + b]);
+    }
+    const uint4 lo = mx4_decode8(codes.x, sc), hi = mx4_decode8(codes.y, sc);
+    const uint32_t u[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sh[(c + j) * LD + o] = (uint16_t)(u[j / 2] >> (16 * (j & 1)));
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int at = threadIdx.x + q * 256, i = at >> 3, c = (at & 7) * 8;
+    if (i0 + i < I) *(uint4*)(wt + (i0 + i) * ldo + o0 + c) = *(const uint4*)&sh[i * LD + c];
+  }
+}
+
 // ---------------------------------------------------------------------------
 // products
 // ---------------------------------------------------------------------------
-// Activations: A_BF16, A_F32 (hi + lo) or A_MX4 (codes and scales).
+// Activations: A_BF16, A_F32 (three bf16 terms) or A_MX4 (codes and scales).
 enum { A_BF16 = 0, A_F32 = 1, A_MX4 = 2 };
+// The weight: codes and scales, or (mx4_gemm_kernel) rows already decoded to bf16.
+enum { W_MX4 = 0, W_BF16 = 1 };
 // What a tile's sums become: rounded to bf16, fp32, or blocks of the format.
 enum { O_BF16 = 0, O_F32 = 1, O_MX4 = 2 };
 
@@ -312,14 +345,32 @@ __device__ __forceinline__ float mx4_swiglu(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-g * 1.4426950408889634f)) * u;
 }
 
+// v = a + b + c, each the next 8 significant bits: exact in bf16, and all 24 of fp32
+__device__ __forceinline__ void mx4_split3(const float (&v)[8], bf16x8_t (&t)[3]) {
+  uint32_t h[3][8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    h[0][j] = __float_as_uint(v[j]) & 0xffff0000u;
+    const float r = v[j] - __uint_as_float(h[0][j]);
+    h[1][j] = __float_as_uint(r) & 0xffff0000u;
+    h[2][j] = __float_as_uint(r - __uint_as_float(h[1][j]));
+  }
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    uint32_t u[4];  // the high halves of pairs
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u[j] = __builtin_amdgcn_perm(h[q][2 * j + 1], h[q][2 * j], 0x07060302u);
+    t[q] = __builtin_bit_cast(bf16x8_t, make_uint4(u[0], u[1], u[2], u[3]));
+  }
+}
+
 // The kernel for every shape: 64 x 64 outputs, K in steps of one block, operands
 // decoded to bf16 in LDS and multiplied by v_mfma_f32_32x32x16_bf16, a quarter of
-// the tile a wave.  TRANS: the sum runs over the weight's rows (the input
-// gradient), x is g and the outputs are the weight's columns.
-template <int AT, int OT, bool SWIGLU, bool TRANS>
+// the tile a wave.
+template <int AT, int OT, bool SWIGLU>
 __global__ void __launch_bounds__(256) mx4_tile_kernel(Mx4Args p) {
   constexpr int LD = MX4_BLOCK + 8;
-  constexpr int AP = AT == A_F32 ? 2 : 1, BP = SWIGLU ? 2 : 1;
+  constexpr int AP = AT == A_F32 ? 3 : 1, BP = SWIGLU ? 2 : 1;
   __shared__ __attribute__((aligned(16))) uint16_t sa[AP][64 * LD];
   __shared__ __attribute__((aligned(16))) uint16_t sb[BP][64 * LD];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -328,10 +379,9 @@ __global__ void __launch_bounds__(256) mx4_tile_kernel(Mx4Args p) {
   const int n_tiles = (int)((p.N + 63) / 64);
   if (!mx4_tile<64>(p, blockIdx.x / n_tiles, lane, e, row0, rows)) return;
   const int64_t n0 = (int64_t)(blockIdx.x % n_tiles) * 64;
-  // TRANS: the weight has p.K rows (the sum) of p.N columns
-  const int64_t nb = mx4_blocks(TRANS ? p.N : p.K), wrows = TRANS ? p.K : p.N;
-  const uint8_t* W[2] = {p.w + (int64_t)e * wrows * nb * 16, SWIGLU ? p.w2 + (int64_t)e * wrows * nb * 16 : nullptr};
-  const uint8_t* S[2] = {p.s + (int64_t)e * wrows * nb, SWIGLU ? p.s2 + (int64_t)e * wrows * nb : nullptr};
+  const int64_t nb = mx4_blocks(p.K);
+  const uint8_t* W[2] = {p.w + (int64_t)e * p.N * nb * 16, SWIGLU ? p.w2 + (int64_t)e * p.N * nb * 16 : nullptr};
+  const uint8_t* S[2] = {p.s + (int64_t)e * p.N * nb, SWIGLU ? p.s2 + (int64_t)e * p.N * nb : nullptr};
 
   const int ar = tid >> 2, ac = (tid & 3) * 8;  // this thread's row and columns of A (and of W)
   const bool arow = ar < rows;
@@ -360,39 +410,19 @@ __global__ void __launch_bounds__(256) mx4_tile_kernel(Mx4Args p) {
         if (p.xvec && c0 + 8 <= p.K) mx4_load8<AT == A_BF16, true>(p.x, xr, p.K, c0, v);
         else mx4_load8<AT == A_BF16, false>(p.x, xr, p.K, c0, v);
       }
-      uint4 hi = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-      *(uint4*)&sa[0][ar * LD + ac] = hi;
-      if constexpr (AT == A_F32) {
-        const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w};
-        uint32_t lo[4];
+      bf16x8_t t[3];  // bf16 values are the first term
+      mx4_split3(v, t);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          lo[j] = pack_bf16(v[2 * j] - __uint_as_float(h[j] << 16),
-                            v[2 * j + 1] - __uint_as_float(h[j] & 0xffff0000u));
-        *(uint4*)&sa[AP - 1][ar * LD + ac] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      }
+      for (int q = 0; q < AP; ++q) *(bf16x8_t*)&sa[q][ar * LD + ac] = t[q];
     }
 #pragma unroll
     for (int q = 0; q < BP; ++q) {
       uint4 d = zero;
-      if constexpr (TRANS) {
-        // 32 rows of the weight by 64 columns: 8 codes of a row, written column by column
-        const int o = tid >> 3, c = (tid & 7) * 8;
-        const int64_t wr = kb * MX4_BLOCK + o, wc = n0 + c;
-        if (wr < wrows && wc < nb * MX4_BLOCK) {
-          const int64_t b = wr * nb + wc / MX4_BLOCK;
-          d = mx4_decode8(*(const uint32_t*)(W[q] + b * 16 + (wc % MX4_BLOCK) / 2), mx4_scale(S[q][b]));
-        }
-        const uint32_t u[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sb[q][(c + j) * LD + o] = (uint16_t)(u[j / 2] >> (16 * (j & 1)));
-      } else {
-        if (n0 + ar < p.N) {
-          const int64_t b = (n0 + ar) * nb + kb;
-          d = mx4_decode8(*(const uint32_t*)(W[q] + b * 16 + ac / 2), mx4_scale(S[q][b]));
-        }
-        *(uint4*)&sb[q][ar * LD + ac] = d;
+      if (n0 + ar < p.N) {
+        const int64_t b = (n0 + ar) * nb + kb;
+        d = mx4_decode8(*(const uint32_t*)(W[q] + b * 16 + ac / 2), mx4_scale(S[q][b]));
       }
+      *(uint4*)&sb[q][ar * LD + ac] = d;
     }
     __syncthreads();
 #pragma unroll
@@ -441,11 +471,11 @@ constexpr int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 bool aligned(const void* p, int to) { return ((uintptr_t)p & (to - 1)) == 0; }
 bool dtype_ok(int d) { return d == SMAUL_DTYPE_F32 || d == SMAUL_DTYPE_BF16; }
 
-template <int AT, int OT, bool SWIGLU, bool TRANS>
+template <int AT, int OT, bool SWIGLU>
 int launch_tiles(const Mx4Args& p, int64_t m_tiles, hipStream_t stream) {
   const int64_t n_tiles = (p.N + 63) / 64;
   if (m_tiles * n_tiles > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: too many tiles");
-  hipLaunchKernelGGL((mx4_tile_kernel<AT, OT, SWIGLU, TRANS>), dim3((unsigned)(m_tiles * n_tiles)), dim3(256), 0,
+  hipLaunchKernelGGL((mx4_tile_kernel<AT, OT, SWIGLU>), dim3((unsigned)(m_tiles * n_tiles)), dim3(256), 0,
                      stream, p);
   return check_launch("mx4_tile_kernel");
 }
@@ -468,12 +498,13 @@ int launch_tiles(const Mx4Args& p, int64_t m_tiles, hipStream_t stream) {
 // Stages are as wide as make their rows whole cache lines: what bounds the loop is the
 // number of L2 requests, and half a line costs as much as a whole one (16384 rows,
 // K 4096 -> 4096: 190 us with 64-byte rows of codes).
-template <int AT, int BM, int BN, int WM, int WN, int KS, int NSTAGE>
+template <int AT, int WF, int BM, int BN, int WM, int WN, int KS, int NSTAGE>
 struct Mx4Cfg {
   static constexpr int NW = WM * WN;
-  static constexpr int XROW = AT == A_MX4 ? KS / 2 : AT == A_BF16 ? KS * 2 : KS * 4, WROW = KS / 2;
+  static constexpr int XROW = AT == A_MX4 ? KS / 2 : AT == A_BF16 ? KS * 2 : KS * 4;
+  static constexpr int WROW = WF == W_BF16 ? KS * 2 : KS / 2;
   static constexpr int XB = BM * XROW, WB = BN * WROW;
-  static constexpr int SROWS = BN + (AT == A_MX4 ? BM : 0), SG = KS < 128 ? 1 : KS / 128;  // scale rows, dwords a row
+  static constexpr int SROWS = WF == W_BF16 ? 0 : BN + (AT == A_MX4 ? BM : 0), SG = KS < 128 ? 1 : KS / 128;  // scale rows, dwords a row
   static constexpr int STAGE = XB + WB + SROWS * SG * 4;
   // DMA instructions: a wave's of x and W, all of the scales
   static constexpr int X_INS = XB / (1024 * NW), W_INS = WB / (1024 * NW), S_INS = SROWS * SG / 64;
@@ -511,27 +542,41 @@ __device__ __forceinline__ i32x8_t mx4_operand(uint4 c) {
   return r;
 }
 
-// v = a + b + c in bf16 terms (24 bits)
-__device__ __forceinline__ void mx4_split3(const float (&v)[8], bf16x8_t (&t)[3]) {
-  float r[8];
+// 16 consecutive sums of row `row` from column n, cast; columns from `ld` on are not
+// the row's.  whole (uniform): all of them are, and 16-byte aligned.
+template <bool BF16>
+__device__ __forceinline__ void mx4_store16(void* out, int64_t row, int64_t ld, int64_t n, bool whole,
+                                            const float (&v)[16]) {
+  const int64_t o = row * ld + n;
+  if constexpr (BF16) {
+    uint32_t u[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) r[j] = v[j];
+    for (int r = 0; r < 8; ++r) u[r] = pack_bf16(v[2 * r], v[2 * r + 1]);
+    uint16_t* y = (uint16_t*)out + o;
+    if (whole) {
+      ((uint4*)y)[0] = make_uint4(u[0], u[1], u[2], u[3]);
+      ((uint4*)y)[1] = make_uint4(u[4], u[5], u[6], u[7]);
+    } else {
 #pragma unroll
-  for (int q = 0; q < 3; ++q) {
-    uint32_t u[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      u[j] = pack_bf16(r[2 * j], r[2 * j + 1]);
-      r[2 * j] = r[2 * j] - __uint_as_float(u[j] << 16);
-      r[2 * j + 1] = r[2 * j + 1] - __uint_as_float(u[j] & 0xffff0000u);
+      for (int r = 0; r < 16; ++r)
+        if (n + r < ld) y[r] = (uint16_t)(u[r / 2] >> (16 * (r & 1)));
     }
-    t[q] = __builtin_bit_cast(bf16x8_t, make_uint4(u[0], u[1], u[2], u[3]));
+  } else {
+    float* y = (float*)out + o;
+    if (whole) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) ((float4*)y)[r] = make_float4(v[4 * r], v[4 * r + 1], v[4 * r + 2], v[4 * r + 3]);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (n + r < ld) y[r] = v[r];
+    }
   }
 }
 
-template <int AT, int OT, bool SWIGLU, int BM, int BN, int WM, int WN, int KS, int NSTAGE>
+template <int AT, int WF, int OT, bool SWIGLU, int BM, int BN, int WM, int WN, int KS, int NSTAGE>
 __global__ void __launch_bounds__(WM * WN * 64, 2) mx4_gemm_kernel(Mx4Args p) {
-  using C = Mx4Cfg<AT, BM, BN, WM, WN, KS, NSTAGE>;
+  using C = Mx4Cfg<AT, WF, BM, BN, WM, WN, KS, NSTAGE>;
   constexpr int TT = C::TT, WT = C::WT, NW = C::NW, BNO = SWIGLU ? BN / 2 : BN, XROW = C::XROW, WROW = C::WROW;
   __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -583,11 +628,11 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) mx4_gemm_kernel(Mx4Args p) {
 #pragma unroll
   for (int b = 0; b < C::W_INS; ++b) {
     const int q = (wave * C::W_INS + b) * WR + lane / WL;
-    w_off[b] = (uint32_t)(w_row(q) * p.ldw * 16 + mx4_swz<WROW>(q, lane % WL) * 16);
+    w_off[b] = (uint32_t)(w_row(q) * p.ldw * (WF == W_BF16 ? 2 : 16) + mx4_swz<WROW>(q, lane % WL) * 16);
   }
   // scale instruction i stages 64 rows of one group: of the weight's, then of x's
-  constexpr int SI = (C::S_INS + NW - 1) / NW, SP = C::SROWS / 64;
-  uint32_t s_off[SI];
+  constexpr int SI = (C::S_INS + NW - 1) / NW, SP = C::SROWS < 64 ? 1 : C::SROWS / 64;
+  uint32_t s_off[SI < 1 ? 1 : SI];
 #pragma unroll
   for (int i = 0; i < SI; ++i) {
     const int q = (wave + NW * i) % SP * 64 + lane;
@@ -727,7 +772,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) mx4_gemm_kernel(Mx4Args p) {
         uint4 wc[WT];  // codes of block g of each weight row, and its scale
         float sc[WT];
 #pragma unroll
-        for (int j = 0; j < WT; ++j) {
+        for (int j = 0; j < WT && WF == W_MX4; ++j) {
           const int r = w_tile(j) + l32;
           wc[j] = *(const uint4*)(ws_ + r * WROW + mx4_swz<WROW>(r, h * 2 + g) * 16);
           sc[j] = mx4_scale((*(const uint32_t*)(ss_ + (h / 2 * C::SROWS + r) * 4) >> sh) & 255u);
@@ -753,8 +798,14 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) mx4_gemm_kernel(Mx4Args p) {
           }
 #pragma unroll
           for (int j = 0; j < WT; ++j) {
-            const uint32_t c = q == 0 ? wc[j].x : q == 1 ? wc[j].y : q == 2 ? wc[j].z : wc[j].w;
-            const bf16x8_t wf = __builtin_bit_cast(bf16x8_t, mx4_decode8(c, sc[j]));
+            bf16x8_t wf;
+            if constexpr (WF == W_BF16) {
+              const int r = w_tile(j) + l32;
+              wf = *(const bf16x8_t*)(ws_ + r * WROW + mx4_swz<WROW>(r, h * 8 + g * 4 + q) * 16);
+            } else {
+              const uint32_t c = q == 0 ? wc[j].x : q == 1 ? wc[j].y : q == 2 ? wc[j].z : wc[j].w;
+              wf = __builtin_bit_cast(bf16x8_t, mx4_decode8(c, sc[j]));
+            }
 #pragma unroll
             for (int i = 0; i < TT; ++i)
 #pragma unroll
@@ -816,43 +867,18 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) mx4_gemm_kernel(Mx4Args p) {
           if (g == 0) p.ys[(nb0 / MX4_GROUP * p.yrows + row) * 4 + nb0 % MX4_GROUP / MX4_BLOCK] = (uint8_t)byte;
         }
       } else if (live) {
-        const int64_t o = row * p.ldy + n;
-        if constexpr (OT == O_BF16) {
-          uint32_t u[8];
-#pragma unroll
-          for (int r = 0; r < 8; ++r) u[r] = pack_bf16(v[2 * r], v[2 * r + 1]);
-          uint16_t* y = (uint16_t*)p.y + o;
-          if (whole) {
-            ((uint4*)y)[0] = make_uint4(u[0], u[1], u[2], u[3]);
-            ((uint4*)y)[1] = make_uint4(u[4], u[5], u[6], u[7]);
-          } else {
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (n + r < p.ldy) y[r] = (uint16_t)(u[r / 2] >> (16 * (r & 1)));
-          }
-        } else {
-          float* y = (float*)p.y + o;
-          if (whole) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              ((float4*)y)[r] = make_float4(v[4 * r], v[4 * r + 1], v[4 * r + 2], v[4 * r + 3]);
-          } else {
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (n + r < p.ldy) y[r] = v[r];
-          }
-        }
+        mx4_store16<OT == O_BF16>(p.y, row, p.ldy, n, whole, v);
       }
     }
   }
 }
 
-template <int AT, int OT, bool SWIGLU, int BM, int BN, int WM, int WN, int KS, int NSTAGE>
+template <int AT, int WF, int OT, bool SWIGLU, int BM, int BN, int WM, int WN, int KS, int NSTAGE>
 int launch_gemm_cfg(const Mx4Args& p, int64_t m_tiles, hipStream_t stream) {
   constexpr int BNO = SWIGLU ? BN / 2 : BN;
   const int64_t n_tiles = (mx4_cols<OT>(p) + BNO - 1) / BNO;
   if (m_tiles * n_tiles > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: too many tiles");
-  hipLaunchKernelGGL((mx4_gemm_kernel<AT, OT, SWIGLU, BM, BN, WM, WN, KS, NSTAGE>),
+  hipLaunchKernelGGL((mx4_gemm_kernel<AT, WF, OT, SWIGLU, BM, BN, WM, WN, KS, NSTAGE>),
                      dim3((unsigned)(m_tiles * n_tiles)), dim3(WM * WN * 64), 0, stream, p);
   return check_launch("mx4_gemm_kernel");
 }
@@ -964,10 +990,10 @@ int64_t gemm_bm(int at) { return at == A_F32 ? 64 : at == A_MX4 ? 256 : 128; }
 
 template <int AT, int OT, bool SWIGLU>
 int launch_product(const Mx4Args& p, bool gemm, int64_t m_tiles, hipStream_t stream) {
-  if (!gemm) return launch_tiles<AT, OT, SWIGLU, false>(p, m_tiles, stream);
-  if constexpr (AT == A_F32) return launch_gemm_cfg<AT, OT, SWIGLU, 64, 256, 2, 2, 64, 3>(p, m_tiles, stream);
-  else if constexpr (AT == A_BF16) return launch_gemm_cfg<AT, OT, SWIGLU, 128, 256, 2, 2, 64, 3>(p, m_tiles, stream);
-  else return launch_gemm_cfg<AT, OT, SWIGLU, 256, 256, 4, 2, 256, 2>(p, m_tiles, stream);
+  if (!gemm) return launch_tiles<AT, OT, SWIGLU>(p, m_tiles, stream);
+  if constexpr (AT == A_F32) return launch_gemm_cfg<AT, W_MX4, OT, SWIGLU, 64, 256, 2, 2, 64, 3>(p, m_tiles, stream);
+  else if constexpr (AT == A_BF16) return launch_gemm_cfg<AT, W_MX4, OT, SWIGLU, 128, 256, 2, 2, 64, 3>(p, m_tiles, stream);
+  else return launch_gemm_cfg<AT, W_MX4, OT, SWIGLU, 256, 256, 4, 2, 256, 2>(p, m_tiles, stream);
 }
 
 // activations with a weight: y of `out` type
@@ -1034,6 +1060,31 @@ LinearParts linear_parts(int64_t rows, int64_t K, int64_t N, int dtype, int act)
   }
   q.total = w.at;
   return q;
+}
+
+// The input gradient's workspace: the weight turned round and decoded, and g in padded
+// rows where its width is no whole number of stages.
+struct DxParts {
+  int64_t ldo, wt, g, total;
+  bool pad;
+};
+DxParts dx_parts(int64_t rows, int64_t I, int64_t O, int dtype) {
+  DxParts q{};
+  Parts w;
+  q.ldo = mx4_groups(O) * MX4_GROUP;
+  q.pad = O % 64 != 0;
+  q.wt = w.take(I * q.ldo * 2);
+  q.g = w.take(q.pad ? rows * q.ldo * (dtype == SMAUL_DTYPE_BF16 ? 2 : 4) : 0);
+  q.total = w.at;
+  return q;
+}
+
+template <int AT, int OT>
+int launch_dx(const Mx4Args& p, hipStream_t stream) {
+  // us, 4096 rows 2560 -> 1024 bf16: 33 of 8 waves, 35.5 of 4; 64 rows x 64 columns 44.
+  // fp32, 512 rows: 37 of 64 x 64, 41 of 64 x 128
+  if constexpr (AT == A_F32) return launch_gemm_cfg<AT, W_BF16, OT, false, 64, 64, 2, 2, 64, 3>(p, (p.R + 63) / 64, stream);
+  else return launch_gemm_cfg<AT, W_BF16, OT, false, 128, 128, 4, 2, 64, 4>(p, (p.R + 127) / 128, stream);
 }
 
 }  // namespace
@@ -1127,26 +1178,57 @@ int smaul_mx4_linear(const void* x, int dtype, const uint8_t* w, const uint8_t* 
   return launch_linear(p, at, bf16 ? O_BF16 : O_F32, q.gemm, (rows + bm - 1) / bm, stream);
 }
 
+int64_t smaul_mx4_backward_input_workspace_size(int64_t rows, int64_t in_f, int64_t out_f, int dtype) {
+  if (rows < 0 || in_f <= 0 || out_f <= 0 || !dtype_ok(dtype)) return -1;
+  return dx_parts(rows, in_f, out_f, dtype).total;
+}
+
 int smaul_mx4_backward_input(const void* g, int dtype, const uint8_t* w, const uint8_t* s, void* dx, int64_t rows,
-                             int64_t in_f, int64_t out_f, hipStream_t stream) {
+                             int64_t in_f, int64_t out_f, void* workspace, int64_t workspace_bytes,
+                             hipStream_t stream) {
   if (!dtype_ok(dtype) || rows < 0 || in_f <= 0 || out_f <= 0)
     return fail(SMAUL_ERR_INVALID, "mx4_backward_input: bad sizes or dtype");
   if (rows == 0) return SMAUL_OK;
   if (!g || !w || !s || !dx) return fail(SMAUL_ERR_INVALID, "mx4_backward_input: null pointer");
   if (!aligned(w, 16)) return fail(SMAUL_ERR_INVALID, "mx4_backward_input: codes must be 16-byte aligned");
+  if (!aligned(g, 16) || !aligned(dx, 16))
+    return fail(SMAUL_ERR_INVALID, "mx4_backward_input: g and dx must be 16-byte aligned");
+  const DxParts q = dx_parts(rows, in_f, out_f, dtype);
+  if (workspace_bytes < q.total || !workspace || !aligned(workspace, 256))
+    return fail(SMAUL_ERR_INVALID, "mx4_backward_input: workspace %lld < %lld bytes, or unaligned",
+                (long long)workspace_bytes, (long long)q.total);
+  const bool bf16 = dtype == SMAUL_DTYPE_BF16;
+  char* ws = (char*)workspace;
+  const int64_t turns = q.ldo / 64 * ((in_f + 63) / 64);
+  if (turns > 2147483647LL || !gemm_fits(bf16 ? A_BF16 : A_F32, rows, out_f, 1) || in_f * q.ldo * 2 >= (1LL << 32))
+    return fail(SMAUL_ERR_UNSUPPORTED, "mx4_backward_input: more than 4 GiB of g or of the decoded weight");
+  hipLaunchKernelGGL(mx4_turn_kernel, dim3((unsigned)turns), dim3(256), 0, stream, w, s, (uint16_t*)(ws + q.wt), out_f,
+                     in_f, q.ldo);
+  int rc = check_launch("mx4_turn_kernel");
+  if (rc) return rc;
   Mx4Args p{};
   p.x = g;
-  p.w = w;
-  p.s = s;
+  p.w = (uint8_t*)ws + q.wt;
   p.y = dx;
   p.R = rows;
-  p.K = out_f;
+  p.K = q.pad ? q.ldo : out_f;
   p.N = in_f;
+  p.ldx = p.K;
+  p.ldw = q.ldo;
+  p.ldy = in_f;
   p.E = 1;
-  const bool bf16 = dtype == SMAUL_DTYPE_BF16;
-  p.xvec = aligned(g, 16) && out_f % (bf16 ? 8 : 4) == 0;
-  return bf16 ? launch_tiles<A_BF16, O_BF16, false, true>(p, (rows + 63) / 64, stream)
-              : launch_tiles<A_F32, O_F32, false, true>(p, (rows + 63) / 64, stream);
+  if (q.pad) {
+    Mx4Prep f{};
+    f.x = g;
+    f.xo = ws + q.g;
+    f.T = rows;
+    f.K = out_f;
+    f.xmode = P_PAD;
+    rc = launch_prep(f, dtype, 1, stream);
+    if (rc) return rc;
+    p.x = ws + q.g;
+  }
+  return bf16 ? launch_dx<A_BF16, O_BF16>(p, stream) : launch_dx<A_F32, O_F32>(p, stream);
 }
 
 // The experts' workspace: the dispatch's tables and scratch, x as the products read

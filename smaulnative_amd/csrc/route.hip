@@ -60,12 +60,12 @@ __device__ __forceinline__ void wave_sync() {
 
 // One token by one wave, the scores and every comparison in 64 bits: two experts
 // next to each other are told apart whatever a rounding in 32 bits would say.
-// sh: E doubles of this wave.
+// NV: ceil(E / 64) or more; sh: E doubles of this wave.
+template <int NV>
 __device__ __forceinline__ void route_row64(const RouteArgs& p, int64_t t, int lane, double* sh) {
-  constexpr int NV = ROUTE_MAX_E / 64;
   const double inf = __builtin_huge_val();
   double s[NV], key[NV];
-  double m = -inf;
+  double m = -inf, sum = 1.0;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const int e = lane + 64 * v;
@@ -77,7 +77,7 @@ __device__ __forceinline__ void route_row64(const RouteArgs& p, int64_t t, int l
     for (int v = 0; v < NV; ++v) s[v] = 1.0 / (1.0 + exp(-key[v]));
   } else {
     m = wave_max_f(m);
-    double sum = 0.0;
+    sum = 0.0;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       s[v] = lane + 64 * v < p.E ? exp(key[v] - m) : 0.0;
@@ -87,29 +87,25 @@ __device__ __forceinline__ void route_row64(const RouteArgs& p, int64_t t, int l
 #pragma unroll
     for (int v = 0; v < NV; ++v) s[v] = s[v] / sum;
   }
-  if (p.prob) {
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-      if (lane + 64 * v < p.E) p.prob[t * p.E + lane + 64 * v] = (float)s[v];
-  }
   // the choice's c in LDS for the groups; key: what the experts are ordered by
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const int e = lane + 64 * v;
     if (e < p.E) {
+      if (p.prob) p.prob[t * p.E + e] = (float)s[v];
       const double c = p.bias ? s[v] + (double)p.bias[e] : s[v];
       const bool live = key[v] > -inf && c > -inf;
       sh[e] = live ? c : -inf;
       key[v] = live ? (p.bias ? c : key[v]) : -inf;
     }
   }
-  uint64_t in = ~0ull;
-  const int per = p.E / p.groups;
   if (p.top_groups < p.groups) {
     wave_sync();
+    const int per = p.E / p.groups;
     double score = -inf;
     if (lane < p.groups) {
       double b1 = -inf, b2 = -inf;
+#pragma unroll 8
       for (int j = 0; j < per; ++j) {
         const double c = sh[lane * per + j];
         b2 = c > b1 ? b1 : (c > b2 ? c : b2);
@@ -118,66 +114,317 @@ __device__ __forceinline__ void route_row64(const RouteArgs& p, int64_t t, int l
       score = p.group_best == 2 && b2 > -inf ? b1 + b2 : b1;
     }
     int ahead = 0;
+#pragma unroll 4
     for (int g = 0; g < p.groups; ++g) {
       const double o = __shfl(score, g, 64);
       ahead += o > score || (o == score && g < lane);
     }
-    in = __ballot(lane < p.groups && ahead < p.top_groups);
-  }
+    const uint64_t in = __ballot(lane < p.groups && ahead < p.top_groups);
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const int e = lane + 64 * v;
-    if (e < p.E && !((in >> (e / per)) & 1ull)) key[v] = -inf;
+    for (int v = 0; v < NV; ++v) {
+      const int e = lane + 64 * v;
+      if (e < p.E && !((in >> (e / per)) & 1ull)) key[v] = -inf;
+    }
   }
   // the highest left, k times over; lane j keeps slot j
   int mine = -1, n = 0;
-  double mys = 0.0, total = 0.0;
   for (int j = 0; j < p.k; ++j) {
-    double bk = -inf, bs = 0.0;
+    double bk = -inf;
     int be = 0x7fffffff;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
       if (key[v] > bk) {
         bk = key[v];
-        bs = s[v];
         be = lane + 64 * v;
       }
     for (int o = 32; o >= 1; o >>= 1) {
-      const double k2 = __shfl_xor(bk, o, 64), s2 = __shfl_xor(bs, o, 64);
+      const double k2 = __shfl_xor(bk, o, 64);
       const int e2 = __shfl_xor(be, o, 64);
       if (k2 > bk || (k2 == bk && e2 < be)) {
         bk = k2;
-        bs = s2;
         be = e2;
       }
     }
     if (!(bk > -inf)) break;  // uniform: nobody is left
-    if (lane == j) {
-      mine = be;
-      mys = bs;
-    }
+    if (lane == j) mine = be;
     ++n;
-    total += bs;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
       if (lane + 64 * v == be) key[v] = -inf;
   }
+  double w = 0.0;
+  if (mine >= 0) {
+    const double z = (double)route_load(p.z, t * p.E + mine, p.bf16);
+    w = p.sigmoid ? 1.0 / (1.0 + exp(-z)) : exp(z - m) / sum;
+  }
+  const double total = wave_sum_f(w);
   if (lane < p.k) {
-    double w = mys;
-    if (p.renorm && mine >= 0) w = total < (double)ROUTE_MIN_SUM ? 1.0 / n : mys / total;
+    if (p.renorm && mine >= 0) w = total < (double)ROUTE_MIN_SUM ? 1.0 / n : w / total;
     p.topi[t * p.k + lane] = mine;
     p.topw[t * p.k + lane] = (float)(w * p.scale);
   }
   wave_sync();
 }
 
-constexpr int ROUTE_WAVES = 4;
+// ---------------------------------------------------------------------------
+// forward: 16 lanes a token, expert 16 v + lane in register v
+// ---------------------------------------------------------------------------
+// The scores are fp32.  An expert's key is one word: its c (or logit) as an ordered
+// integer, the lowest bits replaced by V - 1 - v.  The highest key left is V / 2
+// three-way maxima and four lane exchanges; its low bits say which v, the lowest lane
+// that has it which expert: equal values come out in the order of their index.
+//
+// What the rounding of the scores or those lost bits could change is not decided in 32
+// bits: experts closer than the error bound are ordered by their c in 64 bits among
+// the few found, and where two groups (the last one in, the first one out) or the
+// scores of a softmax with a bias are that close, the token is done again by
+// route_row64.  In 64 bits throughout, one wave a token, 65536 tokens by 256 experts
+// took 225 us.
+constexpr int ROUTE_WAVES = 4, ROUTE_TOK = ROUTE_WAVES * 4;
 
+template <int CTRL>
+__device__ __forceinline__ uint32_t row_ror(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+// over the 16 lanes of a token, in every lane (rotations by 8, 4, 2, 1)
+#define SMAUL_ROW_REDUCE(v, op)      \
+  do {                               \
+    v = op(v, row_ror<0x128>(v));    \
+    v = op(v, row_ror<0x124>(v));    \
+    v = op(v, row_ror<0x122>(v));    \
+    v = op(v, row_ror<0x121>(v));    \
+  } while (0)
+__device__ __forceinline__ uint32_t op_umax(uint32_t a, uint32_t b) { return max(a, b); }
+__device__ __forceinline__ uint32_t op_fmax(uint32_t a, uint32_t b) {
+  return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+}
+__device__ __forceinline__ uint32_t op_fadd(uint32_t a, uint32_t b) {
+  return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+}
+__device__ __forceinline__ float row_max(float v) {
+  uint32_t u = __float_as_uint(v);
+  SMAUL_ROW_REDUCE(u, op_fmax);
+  return __uint_as_float(u);
+}
+__device__ __forceinline__ float row_sum(float v) {
+  uint32_t u = __float_as_uint(v);
+  SMAUL_ROW_REDUCE(u, op_fadd);
+  return __uint_as_float(u);
+}
+
+// exp, to |x| 2^-24 of its value and two units
+__device__ __forceinline__ float route_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+__device__ __forceinline__ float route_score(float z, int sigmoid, float m, float inv) {
+  return sigmoid ? __builtin_amdgcn_rcpf(1.0f + route_exp(-z)) : route_exp(z - m) * inv;
+}
+
+template <int V>
 __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
-  __shared__ double sh[ROUTE_WAVES][ROUTE_MAX_E];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t t = (int64_t)blockIdx.x * ROUTE_WAVES + wave;
-  if (t < p.T) route_row64(p, t, lane, sh[wave]);
+  constexpr uint32_t LOW = V - 1;
+  constexpr float INF = __builtin_huge_valf();
+  // route_row64's doubles, or the c of the wave's four tokens
+  constexpr int SH = 4 * (V * 16 + 8) / 2 > ROUTE_MAX_E ? 4 * (V * 16 + 8) / 2 : ROUTE_MAX_E;
+  __shared__ double sh64[ROUTE_WAVES][SH];
+  __shared__ float shg[ROUTE_TOK][ROUTE_MAX_G];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, tq = lane >> 4;
+  const int64_t t = (int64_t)blockIdx.x * ROUTE_TOK + threadIdx.x / 16;
+  const bool on = t < p.T;
+  const int64_t row = (on ? t : p.T - 1) * p.E;  // lanes past the end follow along, and store nothing
+  float z[V], s[V], b[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int e = v * 16 + l;
+    z[v] = e < p.E ? route_load(p.z, row + e, p.bf16) + 0.0f : -INF;  // -0 is 0: a tie
+    b[v] = p.bias && e < p.E ? p.bias[e] : 0.0f;
+  }
+  float m = -INF, inv = 1.0f;
+  if (!p.sigmoid) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) m = fmaxf(m, z[v]);
+    m = row_max(m);
+    float sum = 0.0f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      s[v] = v * 16 + l < p.E ? route_exp(z[v] - m) : 0.0f;
+      sum += s[v];
+    }
+    inv = 1.0f / row_sum(sum);
+#pragma unroll
+    for (int v = 0; v < V; ++v) s[v] = s[v] * inv;
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) s[v] = route_score(z[v], 1, 0.0f, 0.0f);
+  }
+  if (p.prob && on) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (v * 16 + l < p.E) p.prob[row + v * 16 + l] = s[v];
+  }
+  // Error of a c: the sum's V + 4 roundings and the exponential's, on scores of at
+  // most s_top (the row's highest), and the rounding of c itself.
+  const float s_err = (p.sigmoid ? 1.0f : inv) * (V + 16) * 0x1p-24f;
+  uint32_t key[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const float c = p.bias ? s[v] + b[v] : s[v];
+    const bool live = z[v] > -INF && c > -INF;
+    s[v] = live ? c : -INF;  // from here on: c
+    const uint32_t u = __float_as_uint(p.bias ? c : z[v]);
+    key[v] = live ? ((u ^ ((uint32_t)((int)u >> 31) | 0x80000000u)) & ~LOW) | (LOW - v) : 0u;
+  }
+  bool again = false;
+  if (p.top_groups < p.groups) {
+    // c to LDS, a group to a lane; the groups' scores to LDS, and each lane counts
+    // the groups ahead of its own
+    float* sc = (float*)sh64[wave] + tq * (V * 16 + 8);  // 8: the tokens' rows in other banks
+#pragma unroll
+    for (int v = 0; v < V; ++v) sc[v * 16 + l] = s[v];
+    wave_sync();
+    const int per = p.E / p.groups;
+    float* sg = shg[wave * 4 + tq];
+    float top = 0.0f;
+    for (int g = l; g < p.groups; g += 16) {
+      float b1 = -INF, b2 = -INF;
+      auto take = [&](float c) {
+        b2 = __builtin_amdgcn_fmed3f(b1, b2, c);
+        b1 = fmaxf(b1, c);
+      };
+      // each lane from another place on: other banks
+      if (per % 4 == 0) {
+        int i = 4 * l % per;
+#pragma unroll 2
+        for (int j = 0; j < per; j += 4) {
+          const float4 c = *(const float4*)(sc + g * per + i);
+          i = i + 4 == per ? 0 : i + 4;
+          take(c.x);
+          take(c.y);
+          take(c.z);
+          take(c.w);
+        }
+      } else {
+        int i = l % per;
+        for (int j = 0; j < per; ++j) {
+          take(sc[g * per + i]);
+          i = i + 1 == per ? 0 : i + 1;
+        }
+      }
+      const float score = p.group_best == 2 && b2 > -INF ? b1 + b2 : b1;
+      sg[g] = score;
+      if (b1 > -INF) top = fmaxf(top, fmaxf(fabsf(b1), fabsf(score)));
+    }
+    wave_sync();
+    uint64_t in = 0;
+    float lowest = INF, highest = -INF;  // of the groups in and out
+    for (int g0 = 0; g0 < p.groups; g0 += 16) {
+      const int g = g0 + l;
+      bool chosen = false;
+      if (g < p.groups) {
+        const float mine = sg[g];
+        int ahead = 0;
+        for (int o = 0; o < p.groups; ++o) {
+          const float other = sg[o];
+          ahead += other > mine || (other == mine && o < g);
+        }
+        chosen = ahead < p.top_groups;
+        if (chosen) lowest = fminf(lowest, mine);
+        else highest = fmaxf(highest, mine);
+      }
+      in |= (__ballot(chosen) >> (tq * 16) & 0xffffull) << g0;
+    }
+    lowest = -row_max(-lowest);
+    highest = row_max(highest);
+    top = row_max(top);
+    // groups without a live expert may change places
+    again = highest > -INF && lowest - highest <= 4.0f * s_err + 8.0f * 0x1p-24f * top;
+    const uint32_t magic = ((1u << 20) + per - 1) / per;  // e / per for e, per <= 512
+    const uint32_t in0 = (uint32_t)in, in1 = (uint32_t)(in >> 32);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const uint32_t g = (v * 16 + l) * magic >> 20;
+      const uint32_t word = p.groups > 32 && g >= 32 ? in1 : in0;
+      key[v] &= (uint32_t)__builtin_amdgcn_sbfe((int)word, g & 31, 1);
+    }
+  }
+  // Lane j gets the j-th highest.  The walk goes on past k while the next one is too
+  // near to the last to be left out.
+  int mine = -1, n = 0;
+  bool near = false, done = false;
+  uint32_t last = 0;
+  for (int j = 0; __ballot(!done); ++j) {
+    uint32_t best = key[0];
+#pragma unroll
+    for (int v = 1; v < V; ++v) best = max(best, key[v]);
+    const uint32_t own = best;
+    SMAUL_ROW_REDUCE(best, op_umax);
+    bool close = false;
+    if (j > 0 && best != 0u) {
+      const uint32_t ua = last & ~LOW, ub = best & ~LOW;
+      if (p.bias) {
+        const float fa = __uint_as_float(ua >> 31 ? ua ^ 0x80000000u : ~ua);
+        const float fb = __uint_as_float(ub >> 31 ? ub ^ 0x80000000u : ~ub);
+        // each c is off by s_err and half a unit, the second may gain V units by its low bits
+        close = !(fa - fb > 2.0f * s_err + (V + 2) * 0x1p-23f * fmaxf(fabsf(fa), fabsf(fb)));
+      } else {
+        close = !p.bf16 && ua == ub;  // logits that the low bits may tell apart
+      }
+    }
+    if (!done) {
+      done = best == 0u || (j >= p.k && !close);
+      if (!done && j == 16) done = again = true;  // more of them than lanes
+      if (!done) {
+        near |= close;
+        n = j + 1;
+      }
+    }
+    last = best;
+    // the lowest lane that has it
+    const uint32_t has = (uint32_t)(__ballot(own == best) >> (tq * 16)) & 0xffffu;
+    const int owner = __builtin_ctz(has);
+    if (!done && l == j) mine = (int)(LOW - (best & LOW)) * 16 + owner;
+    const uint32_t gone = l == owner ? best : 1u;  // 1: no key (a live one is over 2^22)
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = key[v] == gone ? 0u : key[v];
+  }
+  // Neighbours too near for 32 bits: the n found are ordered by what they are in 64
+  // (the sum of a softmax with a bias is left to route_row64).
+  if (p.bias && !p.sigmoid) again |= near;
+  if (__ballot(near && !again)) {
+    double x = -__builtin_huge_val();
+    if (mine >= 0) {
+      x = (double)route_load(p.z, row + mine, p.bf16);
+      if (p.bias) x = 1.0 / (1.0 + exp(-x)) + (double)p.bias[mine];
+    }
+    int ahead = 0;
+    for (int i = 0; i < 16; ++i) {
+      const double y = __shfl(x, i, 16);
+      const int e = __shfl(mine, i, 16);
+      ahead += y > x || (y == x && e < mine);
+    }
+    int sorted = -1;
+    for (int i = 0; i < 16; ++i) {
+      const int e = __shfl(mine, i, 16), at = __shfl(ahead, i, 16);
+      if (e >= 0 && at == l) sorted = e;
+    }
+    mine = sorted;
+  }
+  if (l >= p.k) mine = -1;
+  n = min(n, p.k);
+  float w = 0.0f;
+  if (mine >= 0) w = route_score(route_load(p.z, row + mine, p.bf16), p.sigmoid, m, inv);
+  const float total = row_sum(w);
+  if (p.renorm && mine >= 0) w = total < ROUTE_MIN_SUM ? 1.0f / n : w / total;
+  // a sum next to the guard's border is the 64-bit form's to judge
+  if (p.renorm) again |= fabsf(total - ROUTE_MIN_SUM) <= 64 * 0x1p-24f * ROUTE_MIN_SUM;
+  if (on && l < p.k) {
+    p.topi[t * p.k + l] = mine;
+    p.topw[t * p.k + l] = w * p.scale;
+  }
+  uint64_t redo = __ballot(again && on && l == 0);
+  while (redo) {  // uniform
+    const int q = __builtin_ctzll(redo) >> 4;
+    redo &= redo - 1;
+    route_row64<(V + 3) / 4>(p, (int64_t)blockIdx.x * ROUTE_TOK + wave * 4 + q, lane, sh64[wave]);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -303,8 +550,15 @@ int smaul_moe_route(const void* logits, int dtype, const float* bias, float* pro
   if (!logits || !topi || !topw) return fail(SMAUL_ERR_INVALID, "route: null pointer");
   const RouteArgs p{logits, bias, prob, topi, topw, T, (int)E, (int)k, dtype == SMAUL_DTYPE_BF16,
                     score == SMAUL_SCORE_SIGMOID, (int)groups, (int)top_groups, group_best, renorm != 0, scale};
-  hipLaunchKernelGGL(route_kernel, dim3((unsigned)((T + ROUTE_WAVES - 1) / ROUTE_WAVES)), dim3(ROUTE_WAVES * 64), 0,
-                     stream, p);
+  const dim3 grid((unsigned)((T + ROUTE_TOK - 1) / ROUTE_TOK)), block(ROUTE_WAVES * 64);
+#define SMAUL_R(V) hipLaunchKernelGGL((route_kernel<V>), grid, block, 0, stream, p)
+  if (E <= 16) SMAUL_R(1);
+  else if (E <= 32) SMAUL_R(2);
+  else if (E <= 64) SMAUL_R(4);
+  else if (E <= 128) SMAUL_R(8);
+  else if (E <= 256) SMAUL_R(16);
+  else SMAUL_R(32);
+#undef SMAUL_R
   return check_launch("route_kernel");
 }
 

@@ -591,9 +591,11 @@ class RocmBackend:
         _need_device("mx4_backward_input", g, w, s)
         g, w, s = self._mx4_product_check("mx4_backward_input", "g", g, w, s, in_f, out_f, out_f)
         dx = torch.empty(g.shape[0], in_f, dtype=g.dtype, device=g.device)
+        nws = lib.smaul_mx4_backward_input_workspace_size(g.shape[0], in_f, out_f, _ACT[g.dtype])
+        ws = torch.empty(nws, dtype=torch.uint8, device=g.device)
         with _device(g.device):
             rc = lib.smaul_mx4_backward_input(g.data_ptr(), _ACT[g.dtype], w.data_ptr(), s.data_ptr(), dx.data_ptr(),
-                                              g.shape[0], in_f, out_f, _stream_handle(g.device))
+                                              g.shape[0], in_f, out_f, ws.data_ptr(), nws, _stream_handle(g.device))
         _lib.check(rc, "mx4_backward_input")
         return dx
 
