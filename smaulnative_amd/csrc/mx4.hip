@@ -303,7 +303,7 @@ struct Mx4Args {
   const void* x;           // rows of K values (A_MX4: codes, 16 bytes a block)
   const uint8_t* xs;       // A_MX4: scales
   const int32_t* row_idx;  // logical row -> x row (null: the same)
-  const uint8_t* w;        // [E] [N][nb 16] codes
+  const uint8_t* w;        // [E] [N] rows of codes
   const uint8_t* s;        // [E] [N][nb] scales
   const uint8_t* w2;       // SwiGLU: up's (w, s are gate's)
   const uint8_t* s2;
@@ -316,7 +316,7 @@ struct Mx4Args {
   const int32_t* seg_off;  // null: dense, R rows of one expert
   const int32_t* tile_off;
   int E;
-  int xvec;                // x rows may be read 16 bytes at a time
+  int xvec;                // mx4_stream_kernel: x rows may be read 16 bytes at a time
 };
 
 // the rows of m-tile mt: its expert, first logical row and row count (uniform);
@@ -364,121 +364,9 @@ __device__ __forceinline__ void mx4_split3(const float (&v)[8], bf16x8_t (&t)[3]
   }
 }
 
-// The kernel for every shape: 64 x 64 outputs, K in steps of one block, operands
-// decoded to bf16 in LDS and multiplied by v_mfma_f32_32x32x16_bf16, a quarter of
-// the tile a wave.
-template <int AT, int OT, bool SWIGLU>
-__global__ void __launch_bounds__(256) mx4_tile_kernel(Mx4Args p) {
-  constexpr int LD = MX4_BLOCK + 8;
-  constexpr int AP = AT == A_F32 ? 3 : 1, BP = SWIGLU ? 2 : 1;
-  __shared__ __attribute__((aligned(16))) uint16_t sa[AP][64 * LD];
-  __shared__ __attribute__((aligned(16))) uint16_t sb[BP][64 * LD];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int e, rows;
-  int64_t row0;
-  const int n_tiles = (int)((p.N + 63) / 64);
-  if (!mx4_tile<64>(p, blockIdx.x / n_tiles, lane, e, row0, rows)) return;
-  const int64_t n0 = (int64_t)(blockIdx.x % n_tiles) * 64;
-  const int64_t nb = mx4_blocks(p.K);
-  const uint8_t* W[2] = {p.w + (int64_t)e * p.N * nb * 16, SWIGLU ? p.w2 + (int64_t)e * p.N * nb * 16 : nullptr};
-  const uint8_t* S[2] = {p.s + (int64_t)e * p.N * nb, SWIGLU ? p.s2 + (int64_t)e * p.N * nb : nullptr};
-
-  const int ar = tid >> 2, ac = (tid & 3) * 8;  // this thread's row and columns of A (and of W)
-  const bool arow = ar < rows;
-  const int64_t xr = arow ? (p.row_idx ? p.row_idx[row0 + ar] : row0 + ar) : 0;
-  const int wm = wave >> 1, wn = wave & 1;
-  f32x16_t acc[BP];
-#pragma unroll
-  for (int q = 0; q < BP; ++q)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[q][r] = 0.0f;
-
-  const int64_t steps = mx4_blocks(p.K);
-  for (int64_t kb = 0; kb < steps; ++kb) {
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    if constexpr (AT == A_MX4) {
-      uint4 d = zero;
-      if (arow) {
-        const int64_t b = xr * steps + kb;
-        d = mx4_decode8(((const uint32_t*)p.x)[b * 4 + (tid & 3)], mx4_scale(p.xs[b]));
-      }
-      *(uint4*)&sa[0][ar * LD + ac] = d;
-    } else {
-      float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      const int64_t c0 = kb * MX4_BLOCK + ac;
-      if (arow) {
-        if (p.xvec && c0 + 8 <= p.K) mx4_load8<AT == A_BF16, true>(p.x, xr, p.K, c0, v);
-        else mx4_load8<AT == A_BF16, false>(p.x, xr, p.K, c0, v);
-      }
-      bf16x8_t t[3];  // bf16 values are the first term
-      mx4_split3(v, t);
-#pragma unroll
-      for (int q = 0; q < AP; ++q) *(bf16x8_t*)&sa[q][ar * LD + ac] = t[q];
-    }
-#pragma unroll
-    for (int q = 0; q < BP; ++q) {
-      uint4 d = zero;
-      if (n0 + ar < p.N) {
-        const int64_t b = (n0 + ar) * nb + kb;
-        d = mx4_decode8(*(const uint32_t*)(W[q] + b * 16 + ac / 2), mx4_scale(S[q][b]));
-      }
-      *(uint4*)&sb[q][ar * LD + ac] = d;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const int k = ks * 16 + (lane >> 5) * 8;
-#pragma unroll
-      for (int a = 0; a < AP; ++a) {
-        const bf16x8_t af = *(const bf16x8_t*)&sa[a][(wm * 32 + (lane & 31)) * LD + k];
-#pragma unroll
-        for (int q = 0; q < BP; ++q)
-          acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              af, *(const bf16x8_t*)&sb[q][(wn * 32 + (lane & 31)) * LD + k], acc[q], 0, 0, 0);
-      }
-    }
-    __syncthreads();
-  }
-
-  // register r of lane: row 8 (r / 4) + 4 (lane / 32) + r % 4, column lane % 32
-  const int64_t n = n0 + wn * 32 + (lane & 31);
-  const int64_t onb = mx4_blocks(p.N);
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int row = wm * 32 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
-    const float v = SWIGLU ? mx4_swiglu(acc[0][r], acc[BP - 1][r]) : acc[0][r];
-    const int64_t o = (row0 + row) * p.N + n;
-    if constexpr (OT == O_MX4) {
-      // the 32 lanes of a half hold one row's block (columns past N are zeros)
-      uint32_t m = __float_as_uint(v) & 0x7fffffffu;
-      for (int d = 16; d >= 1; d >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d, 32));
-      const uint32_t byte = mx4_scale_byte(m);
-      uint32_t c = byte == 255 ? 0u : __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v, 0.0f, mx4_scale(byte), 0) & 15u;
-      c |= (uint32_t)__shfl_xor((int)c, 1, 64) << 4;  // even lanes: a byte of two codes
-      const int64_t b = (row0 + row) * onb + n / MX4_BLOCK;
-      if (row < rows && n / MX4_BLOCK < onb) {
-        if (!(lane & 1)) ((uint8_t*)p.y)[b * 16 + (lane & 31) / 2] = (uint8_t)c;
-        if ((lane & 31) == 0) p.ys[b] = (uint8_t)byte;
-      }
-    } else if (row < rows && n < p.N) {
-      if constexpr (OT == O_BF16) ((__bf16*)p.y)[o] = (__bf16)v;
-      else ((float*)p.y)[o] = v;
-    }
-  }
-}
-
 constexpr int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 bool aligned(const void* p, int to) { return ((uintptr_t)p & (to - 1)) == 0; }
 bool dtype_ok(int d) { return d == SMAUL_DTYPE_F32 || d == SMAUL_DTYPE_BF16; }
-
-template <int AT, int OT, bool SWIGLU>
-int launch_tiles(const Mx4Args& p, int64_t m_tiles, hipStream_t stream) {
-  const int64_t n_tiles = (p.N + 63) / 64;
-  if (m_tiles * n_tiles > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: too many tiles");
-  hipLaunchKernelGGL((mx4_tile_kernel<AT, OT, SWIGLU>), dim3((unsigned)(m_tiles * n_tiles)), dim3(256), 0,
-                     stream, p);
-  return check_launch("mx4_tile_kernel");
-}
 
 // The kernel of larger calls: K in stages of KS, activations, codes and scales brought
 // to LDS by DMA, NSTAGE stages in flight, WM x WN waves over BM rows x BN columns.
@@ -601,27 +489,33 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) mx4_gemm_kernel(Mx4Args p) {
   if (!mx4_tile<BM>(p, mt, lane, e, row0, rows)) return;
   const int64_t n0 = (int64_t)nt * BNO;
   const int64_t eblocks = (int64_t)e * p.N * p.ldw;  // ldw / 4 groups of N dwords: as many bytes as blocks
-  const uint8_t* W1 = p.w + eblocks * 16;
-  const uint8_t* S1 = p.s + eblocks;
-  const uint8_t* W2 = SWIGLU ? p.w2 + eblocks * 16 : W1;
-  const uint8_t* S2 = SWIGLU ? p.s2 + eblocks : S1;
+  const int64_t nw = min<int64_t>(n0, p.N - 1);  // the tile's first weight row; a tile of padding reads the last
+  const int64_t w0 = (eblocks + nw * p.ldw) * 16, s0 = eblocks + nw * 4;
+  const uint8_t* W1 = p.w + (WF == W_BF16 ? nw * p.ldw * 2 : w0);
+  const uint8_t* S1 = p.s + s0;
+  const uint8_t* W2 = SWIGLU ? p.w2 + w0 : W1;
+  const uint8_t* S2 = SWIGLU ? p.s2 + s0 : S1;
 
-  // ---- DMA sources of this lane (32-bit offsets; the host checks the range) ----
-  // Rows past the end read the last one: their sums are not stored.
+  // ---- DMA sources of this lane: 32-bit offsets from the tile's first rows (gathered
+  // ones from x's; the host checks its size).  Rows past the end read the last one: their
+  // sums are not stored.
+  constexpr int XS = AT == A_MX4 ? 16 : AT == A_BF16 ? 2 : 4;
+  const char* X = (const char*)p.x + (p.row_idx ? 0 : row0 * p.ldx * XS);
   constexpr int XL = XROW / 16, XR = 64 / XL;  // lanes a row, rows an instruction
   uint32_t x_off[C::X_INS];
 #pragma unroll
   for (int a = 0; a < C::X_INS; ++a) {
     const int r = (wave * C::X_INS + a) * XR + lane / XL;
-    const int64_t lr = row0 + min(r, rows - 1);
-    const int64_t xr = p.row_idx ? (int64_t)p.row_idx[lr] : lr;
-    x_off[a] = (uint32_t)(xr * p.ldx * (AT == A_MX4 ? 16 : AT == A_BF16 ? 2 : 4) + mx4_swz<XROW>(r, lane % XL) * 16);
+    const int lr = min(r, rows - 1);
+    const int64_t xr = p.row_idx ? (int64_t)p.row_idx[row0 + lr] : lr;
+    x_off[a] = (uint32_t)(xr * p.ldx * XS + mx4_swz<XROW>(r, lane % XL) * 16);
   }
-  // staged weight row q: tiles of 32 (gate's, then up's), permuted
-  auto w_row = [&](int q) -> uint32_t {
+  // staged weight row q, from the first: tiles of 32 (gate's, then up's), permuted
+  const int64_t left = p.N - 1 - nw;
+  auto w_row = [&](int q) -> int64_t {
     int t = q >> 5;
     if (SWIGLU) t = t >= BN / 64 ? t - BN / 64 : t;
-    return (uint32_t)min<int64_t>(n0 + t * 32 + mx4_perm(q & 31), p.N - 1);
+    return min<int64_t>(t * 32 + mx4_perm(q & 31), left);
   };
   constexpr int WL = WROW / 16, WR = 64 / WL;
   uint32_t w_off[C::W_INS];
@@ -637,7 +531,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) mx4_gemm_kernel(Mx4Args p) {
   for (int i = 0; i < SI; ++i) {
     const int q = (wave + NW * i) % SP * 64 + lane;
     if (q < BN) {
-      s_off[i] = w_row(q) * 4;
+      s_off[i] = (uint32_t)(w_row(q) * 4);
     } else {
       const int64_t lr = row0 + min(q - BN, rows - 1);
       s_off[i] = (uint32_t)((p.row_idx ? (int64_t)p.row_idx[lr] : lr) * 4);
@@ -656,7 +550,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) mx4_gemm_kernel(Mx4Args p) {
         dma4(src, s_off[i], l + C::XB + C::WB + q * 256);
       }
     }
-    const char* xk = (const char*)p.x + (int64_t)kt * XROW;
+    const char* xk = X + (int64_t)kt * XROW;
 #pragma unroll
     for (int a = 0; a < C::X_INS; ++a) dma16(xk, x_off[a], l + (wave * C::X_INS + a) * 1024);
 #pragma unroll
@@ -883,11 +777,237 @@ int launch_gemm_cfg(const Mx4Args& p, int64_t m_tiles, hipStream_t stream) {
   return check_launch("mx4_gemm_kernel");
 }
 
-// Whether mx4_gemm_kernel's 32-bit offsets reach the rows: `xrows` activations of K
-// values, an expert's N rows.
-bool gemm_fits(int at, int64_t xrows, int64_t K, int64_t N) {
-  const int64_t ng = mx4_groups(K);
-  return xrows * ng * (at == A_MX4 ? 64 : at == A_BF16 ? 256 : 512) < (1LL << 32) && N * ng * 64 < (1LL << 32);
+// The kernel of few rows (up to 64): a workgroup has 32 columns of one expert, its NW
+// waves a slice of K each, so that every byte of the weight is read once and all at
+// the same time; rows of x come from the caches, straight into registers.  The
+// waves' sums meet in LDS and are added in the order of the waves.
+//
+// The experts' rows are found here, without a dispatch: a workgroup looks through the
+// T k <= 512 slots for its expert's; the hidden rows and the outputs
+// stand at their slots.  Two launches less than a dispatch takes, and a layer of 64
+// tokens is launches and latency (84 us with the tile kernel behind a dispatch).
+struct Mx4Slots {
+  const int64_t* topi;  // null: dense, row r of x to row r of y
+  const float* topw;
+  int32_t* counts;      // by the first workgroup of each expert, or null
+  int T, k;
+  int by_token;         // x rows by token (else by slot)
+};
+constexpr int ST_ROWS = 64, ST_SLOTS = 512;
+
+// whether slot i of (token, expert) is one that the layer runs: an expert of the E, a
+// weight above 0, and the token's first slot with it (as smaul_moe_dispatch)
+__device__ __forceinline__ bool mx4_slot(const int64_t* topi, const float* topw, int64_t t, int j, int k, int E, int e) {
+  if (topi[t * k + j] != e || !(topw[t * k + j] > 0.0f) || e < 0 || e >= E) return false;
+  for (int i = 0; i < j; ++i)
+    if (topi[t * k + i] == e && topw[t * k + i] > 0.0f) return false;
+  return true;
+}
+
+template <int AT, int OT, bool SWIGLU, bool VEC, int NW>
+__global__ void __launch_bounds__(NW * 64) mx4_stream_kernel(Mx4Args p, Mx4Slots q) {
+  constexpr int SW = SWIGLU ? 2 : 1, U = (AT == A_F32 ? 2 : 4) / (AT == A_MX4 ? 1 : SW);  // steps read at once
+  constexpr int JS = 1024 + 64;  // bytes between the quarters of a wave's sums: other banks
+  __shared__ __attribute__((aligned(16))) char red[NW * 4 * JS];
+  constexpr int NC = ST_SLOTS / (NW * 64);  // slots a thread
+  __shared__ int s_row[ST_ROWS], s_cnt[NC * NW];
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n_tiles = (int)((p.N + 31) / 32);
+  const int e = blockIdx.x / n_tiles;
+  const int64_t n0 = (int64_t)(blockIdx.x % n_tiles) * 32;
+
+  int rows = (int)p.R;
+  if (q.topi) {
+    bool mine[NC];
+    uint64_t b[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int i = c * NW * 64 + tid;
+      mine[c] = i < q.T * q.k && mx4_slot(q.topi, q.topw, i / q.k, i % q.k, q.k, p.E, e);
+      b[c] = __ballot(mine[c]);
+      if (lane == 0) s_cnt[c * NW + wave] = __popcll(b[c]);
+    }
+    __syncthreads();
+    rows = 0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      int before = rows;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        before += w < wave ? s_cnt[c * NW + w] : 0;
+        rows += s_cnt[c * NW + w];
+      }
+      // at most one slot a token: rows <= T <= 64
+      if (mine[c]) s_row[before + __popcll(b[c] & ((1ull << lane) - 1))] = c * NW * 64 + tid;
+    }
+    if (q.counts && n0 == 0 && tid == 0) q.counts[e] = rows;
+    __syncthreads();
+  }
+
+  const int64_t nb = mx4_blocks(p.K);
+  const int64_t wrow = n0 + mx4_perm(l32) < p.N ? n0 + mx4_perm(l32) : p.N - 1;
+  const int64_t wblk = ((int64_t)e * p.N + wrow) * nb;
+  const int steps = (int)((nb + 1) / 2), per = (steps + NW - 1) / NW;
+  const int lo = min(wave * per, steps), hi = min(lo + per, steps);
+
+  for (int r0 = 0; r0 < rows; r0 += 32) {  // uniform
+    const int r = min(r0 + l32, rows - 1);
+    const int64_t slot = q.topi ? s_row[r] : r;
+    const int64_t xr = q.topi && q.by_token ? slot / q.k : slot;
+    f32x16_t acc[SW];
+#pragma unroll
+    for (int j = 0; j < SW; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[j][i] = 0.0f;
+
+    for (int s0 = lo; s0 < hi; s0 += U) {
+      uint4 wc[U][SW];
+      uint32_t ws[U][SW];
+      uint4 xv[U][AT == A_MX4 ? 1 : AT == A_BF16 ? 4 : 8];
+      uint32_t xsc[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t b = (int64_t)(s0 + u) * 2 + g;  // this lane's block of the step
+        const bool in = s0 + u < hi && b < nb;
+#pragma unroll
+        for (int j = 0; j < SW; ++j) {
+          wc[u][j] = in ? *(const uint4*)((j ? p.w2 : p.w) + (wblk + b) * 16) : make_uint4(0, 0, 0, 0);
+          ws[u][j] = in ? (j ? p.s2 : p.s)[wblk + b] : 0u;
+        }
+        if constexpr (AT == A_MX4) {
+          xv[u][0] = in ? *(const uint4*)((const uint8_t*)p.x + (xr * nb + b) * 16) : make_uint4(0, 0, 0, 0);
+          xsc[u] = in ? p.xs[xr * nb + b] : 0u;
+        } else if constexpr (VEC) {
+          constexpr int V16 = AT == A_BF16 ? 4 : 8, EL = AT == A_BF16 ? 8 : 4;
+#pragma unroll
+          for (int v = 0; v < V16; ++v) {
+            const int64_t c = b * MX4_BLOCK + v * EL;  // K is a multiple of EL
+            const char* src = (const char*)p.x + (xr * p.K + c) * (AT == A_BF16 ? 2 : 4);
+            xv[u][v] = s0 + u < hi && c < p.K ? *(const uint4*)src : make_uint4(0, 0, 0, 0);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (s0 + u >= hi) break;  // uniform
+        if constexpr (AT == A_MX4) {
+#pragma unroll
+          for (int j = 0; j < SW; ++j)
+            acc[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx4_operand(wc[u][j]), mx4_operand(xv[u][0]), acc[j],
+                                                                    4, 4, 0, (int)ws[u][j], 0, (int)xsc[u]);
+        } else {
+          const int64_t b = (int64_t)(s0 + u) * 2 + g;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            constexpr int NT = AT == A_F32 ? 3 : 1;
+            bf16x8_t t[3];
+            if constexpr (VEC && AT == A_BF16) {
+              t[0] = __builtin_bit_cast(bf16x8_t, xv[u][v]);
+            } else {
+              float f[8];
+              if constexpr (VEC) {
+                const uint4 a = xv[u][2 * v], c = xv[u][2 * v + 1];
+                f[0] = __uint_as_float(a.x); f[1] = __uint_as_float(a.y); f[2] = __uint_as_float(a.z); f[3] = __uint_as_float(a.w);
+                f[4] = __uint_as_float(c.x); f[5] = __uint_as_float(c.y); f[6] = __uint_as_float(c.z); f[7] = __uint_as_float(c.w);
+              } else {
+                mx4_load8<AT == A_BF16, false>(p.x, xr, p.K, b * MX4_BLOCK + v * 8, f);
+              }
+              mx4_split3(f, t);
+            }
+#pragma unroll
+            for (int j = 0; j < SW; ++j) {
+              const uint4 c = wc[u][j];
+              const bf16x8_t wf = __builtin_bit_cast(
+                  bf16x8_t, mx4_decode8(v == 0 ? c.x : v == 1 ? c.y : v == 2 ? c.z : c.w, mx4_scale(ws[u][j])));
+#pragma unroll
+              for (int k = 0; k < NT; ++k)
+                acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf, t[k], acc[j], 0, 0, 0);
+            }
+          }
+        }
+      }
+    }
+    // Register 4 i + 0..3 of a lane: quarter i of its 16 consecutive outputs.  Gate's
+    // sums and up's go through the same LDS, for twice the workgroups on a CU.
+    const int row = tid >> 3, h = (tid >> 2) & 1, i = tid & 3;  // 8 threads a row: quarter i of half h
+    float v[SW][4];
+#pragma unroll
+    for (int j = 0; j < SW; ++j) {
+      if (j) __syncthreads();
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        *(float4*)(red + (wave * 4 + c) * JS + lane * 16) =
+            make_float4(acc[j][4 * c], acc[j][4 * c + 1], acc[j][4 * c + 2], acc[j][4 * c + 3]);
+      __syncthreads();
+      if (tid < 256) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[j][c] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const float4 a = *(const float4*)(red + (w * 4 + i) * JS + (h * 32 + row) * 16);
+          v[j][0] += a.x;
+          v[j][1] += a.y;
+          v[j][2] += a.z;
+          v[j][3] += a.w;
+        }
+      }
+    }
+    if (tid < 256) {
+      const int64_t n = n0 + h * 16 + i * 4;
+      float o[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        o[c] = SWIGLU ? mx4_swiglu(v[0][c], v[SW - 1][c]) : v[0][c];
+        if (n + c >= p.N) o[c] = 0.0f;
+      }
+      const bool live = r0 + row < rows;
+      const int64_t yr = live ? (q.topi ? s_row[r0 + row] : r0 + row) : 0;
+      if constexpr (OT == O_MX4) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) m = max(m, __float_as_uint(o[c]) & 0x7fffffffu);
+        for (int d = 4; d >= 1; d >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d, 8));
+        const uint32_t byte = mx4_scale_byte(m);
+        const float e8[8] = {o[0], o[1], o[2], o[3], 0.0f, 0.0f, 0.0f, 0.0f};
+        const int64_t b = yr * mx4_blocks(p.N) + n0 / MX4_BLOCK;
+        if (live) {
+          *(uint16_t*)((uint8_t*)p.y + b * 16 + h * 8 + i * 2) = (uint16_t)mx4_encode8(e8, byte);
+          if ((tid & 7) == 0) p.ys[b] = (uint8_t)byte;
+        }
+      } else if (live) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (n + c < p.N) {
+            if constexpr (OT == O_BF16) ((__bf16*)p.y)[yr * p.N + n + c] = (__bf16)o[c];
+            else ((float*)p.y)[yr * p.N + n + c] = o[c];
+          }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <int AT, int OT, bool SWIGLU, int NW>
+int launch_stream_cfg(const Mx4Args& p, const Mx4Slots& q, int64_t groups, hipStream_t stream) {
+  const dim3 grid((unsigned)groups), block(NW * 64);
+  if constexpr (AT != A_MX4) {
+    if (!p.xvec) {
+      hipLaunchKernelGGL((mx4_stream_kernel<AT, OT, SWIGLU, false, NW>), grid, block, 0, stream, p, q);
+      return check_launch("mx4_stream_kernel");
+    }
+  }
+  hipLaunchKernelGGL((mx4_stream_kernel<AT, OT, SWIGLU, true, NW>), grid, block, 0, stream, p, q);
+  return check_launch("mx4_stream_kernel");
+}
+
+template <int AT, int OT, bool SWIGLU>
+int launch_stream(const Mx4Args& p, const Mx4Slots& q, hipStream_t stream) {
+  const int64_t groups = (p.N + 31) / 32 * p.E;
+  if (groups > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: too many columns");
+  // 4 waves where there are workgroups enough for that: then all of them run at once
+  if (groups > 2 * cu_count()) return launch_stream_cfg<AT, OT, SWIGLU, 4>(p, q, groups, stream);
+  return launch_stream_cfg<AT, OT, SWIGLU, 8>(p, q, groups, stream);
 }
 
 // out[t] = the sum of its slots' rows times their weights, in ascending expert order
@@ -898,7 +1018,7 @@ bool gemm_fits(int at, int64_t xrows, int64_t K, int64_t N) {
 template <bool YF32, bool OBF16, int KM>
 __global__ void __launch_bounds__(256)
 mx4_combine_kernel(const void* __restrict__ y, const int64_t* __restrict__ topi, const float* __restrict__ topw,
-                   const int32_t* __restrict__ inv, void* __restrict__ out, int64_t T, int d, int k) {
+                   const int32_t* __restrict__ inv, void* __restrict__ out, int64_t T, int d, int k, int E) {
   const int cpt = d / 8;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, t = i / cpt;
   if (t >= T) return;
@@ -908,10 +1028,19 @@ mx4_combine_kernel(const void* __restrict__ y, const int64_t* __restrict__ topi,
 #pragma unroll
   for (int j = 0; j < KM; ++j)
     if (j < k) {
-      pos[j] = inv[t * k + j];
-      key[j] = (int)topi[t * k + j];
+      const int64_t e = topi[t * k + j];
+      key[j] = (int)e;
       w[j] = topw[t * k + j];
+      // no dispatch's rows: the outputs stand at their slots
+      pos[j] = inv ? inv[t * k + j] : e >= 0 && e < E && w[j] > 0.0f ? (int)(t * k) + j : -1;
     }
+  if (!inv) {  // a second slot of one expert adds nothing
+#pragma unroll
+    for (int j = 1; j < KM; ++j)
+#pragma unroll
+      for (int i = 0; i < j; ++i)
+        if (j < k && pos[i] >= 0 && key[i] == key[j]) pos[j] = -1;
+  }
 #pragma unroll
   for (int j = 0; j < KM; ++j)
     if (j >= k || pos[j] < 0) {
@@ -958,10 +1087,11 @@ mx4_combine_kernel(const void* __restrict__ y, const int64_t* __restrict__ topi,
 
 template <bool YF32, bool OBF16>
 int launch_combine(const void* y, const int64_t* topi, const float* topw, const int32_t* inv, void* out, int64_t T,
-                   int64_t d, int64_t k, hipStream_t stream) {
+                   int64_t d, int64_t k, int64_t E, hipStream_t stream) {
   const dim3 grid((unsigned)((T * (d / 8) + 255) / 256)), block(256);
 #define SMAUL_C(KM) \
-  hipLaunchKernelGGL((mx4_combine_kernel<YF32, OBF16, KM>), grid, block, 0, stream, y, topi, topw, inv, out, T, (int)d, (int)k)
+  hipLaunchKernelGGL((mx4_combine_kernel<YF32, OBF16, KM>), grid, block, 0, stream, y, topi, topw, inv, out, T, \
+                     (int)d, (int)k, (int)E)
   if (k <= 2) SMAUL_C(2);
   else if (k <= 4) SMAUL_C(4);
   else SMAUL_C(8);
@@ -984,27 +1114,26 @@ int launch_quantize(const void* x, int dtype, uint8_t* codes, uint8_t* scales, i
   return check_launch("mx4_quantize_kernel");
 }
 
-// row tiles of the two product kernels
-constexpr int64_t TILE_BM = 64;
-int64_t gemm_bm(int at) { return at == A_F32 ? 64 : at == A_MX4 ? 256 : 128; }
+// up to this many rows (tokens of a layer) mx4_stream_kernel, past them mx4_gemm_kernel
+int64_t gemm_bm(int at) { return at == A_F32 ? 64 : at == A_MX4 ? 256 : 128; }  // its row tiles
 
 template <int AT, int OT, bool SWIGLU>
-int launch_product(const Mx4Args& p, bool gemm, int64_t m_tiles, hipStream_t stream) {
-  if (!gemm) return launch_tiles<AT, OT, SWIGLU>(p, m_tiles, stream);
+int launch_product(const Mx4Args& p, const Mx4Slots* few, int64_t m_tiles, hipStream_t stream) {
+  if (few) return launch_stream<AT, OT, SWIGLU>(p, *few, stream);
   if constexpr (AT == A_F32) return launch_gemm_cfg<AT, W_MX4, OT, SWIGLU, 64, 256, 2, 2, 64, 3>(p, m_tiles, stream);
   else if constexpr (AT == A_BF16) return launch_gemm_cfg<AT, W_MX4, OT, SWIGLU, 128, 256, 2, 2, 64, 3>(p, m_tiles, stream);
   else return launch_gemm_cfg<AT, W_MX4, OT, SWIGLU, 256, 256, 4, 2, 256, 2>(p, m_tiles, stream);
 }
 
 // activations with a weight: y of `out` type
-int launch_linear(const Mx4Args& p, int at, int out, bool gemm, int64_t m_tiles, hipStream_t stream) {
+int launch_linear(const Mx4Args& p, int at, int out, const Mx4Slots* few, int64_t m_tiles, hipStream_t stream) {
   if (at == A_MX4)
-    return out == O_BF16 ? launch_product<A_MX4, O_BF16, false>(p, gemm, m_tiles, stream)
-                         : launch_product<A_MX4, O_F32, false>(p, gemm, m_tiles, stream);
+    return out == O_BF16 ? launch_product<A_MX4, O_BF16, false>(p, few, m_tiles, stream)
+                         : launch_product<A_MX4, O_F32, false>(p, few, m_tiles, stream);
   if (at == A_BF16)
-    return out == O_BF16 ? launch_product<A_BF16, O_BF16, false>(p, gemm, m_tiles, stream)
-                         : launch_product<A_BF16, O_F32, false>(p, gemm, m_tiles, stream);
-  return launch_product<A_F32, O_F32, false>(p, gemm, m_tiles, stream);
+    return out == O_BF16 ? launch_product<A_BF16, O_BF16, false>(p, few, m_tiles, stream)
+                         : launch_product<A_BF16, O_F32, false>(p, few, m_tiles, stream);
+  return launch_product<A_F32, O_F32, false>(p, few, m_tiles, stream);
 }
 
 int launch_prep(Mx4Prep p, int dtype, int64_t E, hipStream_t stream) {
@@ -1035,25 +1164,24 @@ struct Parts {
 };
 
 // A linear's workspace: the activations rounded or in padded rows, and the weight's
-// scales (and padded codes) as the GEMM reads them.  Up to 64 rows the tile kernel
-// reads the stored weight.
+// scales (and padded codes) as the GEMM reads them.  Up to ST_ROWS rows the weight is
+// read as it is stored.
 struct LinearParts {
   bool gemm;
   int64_t x, xs, st, wp, total;
 };
 LinearParts linear_parts(int64_t rows, int64_t K, int64_t N, int dtype, int act) {
   const bool mx4 = act == SMAUL_ACT_MX4;
-  const int at = mx4 ? A_MX4 : dtype == SMAUL_DTYPE_BF16 ? A_BF16 : A_F32;
-  const int64_t ng = mx4_groups(K), nb = mx4_blocks(K);
+  const int64_t ng = mx4_groups(K), nb = mx4_blocks(K), size = dtype == SMAUL_DTYPE_BF16 ? 2 : 4;
   const bool pad = K % MX4_STAGE != 0;
   LinearParts q{};
   Parts w;
-  q.gemm = rows > TILE_BM && gemm_fits(at, rows, K, N);
+  q.gemm = rows > ST_ROWS;
   if (!q.gemm) {
     q.x = w.take(mx4 ? rows * nb * 16 : 0);
     q.xs = w.take(mx4 ? rows * nb : 0);
   } else {
-    q.x = w.take(mx4 ? rows * ng * 64 : pad ? rows * ng * MX4_GROUP * (at == A_BF16 ? 2 : 4) : 0);
+    q.x = w.take(mx4 ? rows * ng * 64 : pad ? rows * ng * MX4_GROUP * size : 0);
     q.xs = w.take(mx4 ? rows * ng * 4 : 0);
     q.st = w.take(N * ng * 4);
     q.wp = w.take(pad ? N * ng * 64 : 0);
@@ -1174,8 +1302,9 @@ int smaul_mx4_linear(const void* x, int dtype, const uint8_t* w, const uint8_t* 
     rc = launch_quantize(x, dtype, (uint8_t*)ws + q.x, (uint8_t*)ws + q.xs, rows, in_f, stream);
   }
   if (rc) return rc;
-  const int64_t bm = q.gemm ? gemm_bm(at) : TILE_BM;
-  return launch_linear(p, at, bf16 ? O_BF16 : O_F32, q.gemm, (rows + bm - 1) / bm, stream);
+  const Mx4Slots few{};
+  return launch_linear(p, at, bf16 ? O_BF16 : O_F32, q.gemm ? nullptr : &few, (rows + gemm_bm(at) - 1) / gemm_bm(at),
+                       stream);
 }
 
 int64_t smaul_mx4_backward_input_workspace_size(int64_t rows, int64_t in_f, int64_t out_f, int dtype) {
@@ -1200,8 +1329,7 @@ int smaul_mx4_backward_input(const void* g, int dtype, const uint8_t* w, const u
   const bool bf16 = dtype == SMAUL_DTYPE_BF16;
   char* ws = (char*)workspace;
   const int64_t turns = q.ldo / 64 * ((in_f + 63) / 64);
-  if (turns > 2147483647LL || !gemm_fits(bf16 ? A_BF16 : A_F32, rows, out_f, 1) || in_f * q.ldo * 2 >= (1LL << 32))
-    return fail(SMAUL_ERR_UNSUPPORTED, "mx4_backward_input: more than 4 GiB of g or of the decoded weight");
+  if (turns > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_backward_input: too large a weight");
   hipLaunchKernelGGL(mx4_turn_kernel, dim3((unsigned)turns), dim3(256), 0, stream, w, s, (uint16_t*)(ws + q.wt), out_f,
                      in_f, q.ldo);
   int rc = check_launch("mx4_turn_kernel");
@@ -1242,16 +1370,15 @@ static Mx4MoeParts mx4_moe_parts(int64_t T, int64_t d, int64_t h, int64_t E, int
   Parts w;
   const int64_t size = dtype == SMAUL_DTYPE_BF16 ? 2 : 4, R = T * k, gd = mx4_groups(d), gh = mx4_groups(h);
   const bool mx4 = act == SMAUL_ACT_MX4;
-  const int at = mx4 ? A_MX4 : size == 2 ? A_BF16 : A_F32;
-  q.gemm = T > TILE_BM && gemm_fits(at, T, d, h) && gemm_fits(at, R, h, d);
-  q.seg_off = w.take((E + 1) * 4);
-  q.tile_off = w.take((E + 1) * 4);
-  q.perm_row = w.take(R * 4);
-  q.perm_w = w.take(R * 4);
-  q.inv = w.take(R * 4);
-  q.scratch_bytes = smaul_moe_dispatch_workspace_size(T, E);
-  q.scratch = w.take(q.scratch_bytes);
+  q.gemm = T > ST_ROWS;
   if (q.gemm) {
+    q.seg_off = w.take((E + 1) * 4);
+    q.tile_off = w.take((E + 1) * 4);
+    q.perm_row = w.take(R * 4);
+    q.perm_w = w.take(R * 4);
+    q.inv = w.take(R * 4);
+    q.scratch_bytes = smaul_moe_dispatch_workspace_size(T, E);
+    q.scratch = w.take(q.scratch_bytes);
     const bool pd = d % MX4_STAGE != 0, ph = h % MX4_STAGE != 0;
     q.xc = w.take(mx4 ? T * gd * 64 : pd ? T * gd * MX4_GROUP * size : 0);
     q.xs = w.take(mx4 ? T * gd * 4 : 0);
@@ -1308,10 +1435,16 @@ int smaul_mx4_moe_forward(const void* x, int dtype, const int64_t* topi, const f
   const int at = mx4 ? A_MX4 : bf16 ? A_BF16 : A_F32;
   const int64_t R = T * k, gd = mx4_groups(d), gh = mx4_groups(h);
   const bool pd = d % MX4_STAGE != 0, ph = h % MX4_STAGE != 0;
-  const int64_t bm = q.gemm ? gemm_bm(at) : TILE_BM, m_tiles = (R + bm - 1) / bm + E;
-  int rc = smaul_moe_dispatch(topi, topw, counts, seg_off, tile_off, perm_row, (float*)(ws + q.perm_w), inv, T, E, k,
-                              bm, ws + q.scratch, q.scratch_bytes, stream);
-  if (rc) return rc;
+  const int64_t bm = gemm_bm(at), m_tiles = (R + bm - 1) / bm + E;
+  if (q.gemm && !(mx4 || T * (pd ? gd * MX4_GROUP : d) * (bf16 ? 2 : 4) < (1LL << 32)))
+    return fail(SMAUL_ERR_UNSUPPORTED, "mx4_moe: more than 4 GiB of x");
+  if (mx4 && T * gd * 64 >= (1LL << 32)) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_moe: more than 4 GiB of codes of x");
+  int rc = SMAUL_OK;
+  if (q.gemm) {
+    rc = smaul_moe_dispatch(topi, topw, counts, seg_off, tile_off, perm_row, (float*)(ws + q.perm_w), inv, T, E, k, bm,
+                            ws + q.scratch, q.scratch_bytes, stream);
+    if (rc) return rc;
+  }
   Mx4Args p{};
   p.x = mx4 || (q.gemm && pd) ? ws + q.xc : x;
   p.xs = (uint8_t*)ws + q.xs;
@@ -1379,15 +1512,19 @@ int smaul_mx4_moe_forward(const void* x, int dtype, const int64_t* topi, const f
     rc = launch_quantize(x, dtype, (uint8_t*)ws + q.xc, (uint8_t*)ws + q.xs, T, d, stream);
   }
   if (rc) return rc;
-  rc = mx4 ? launch_product<A_MX4, O_MX4, true>(p, q.gemm, m_tiles, stream)
-           : bf16 ? launch_product<A_BF16, O_BF16, true>(p, q.gemm, m_tiles, stream)
-                  : launch_product<A_F32, O_F32, true>(p, q.gemm, m_tiles, stream);
+  // up to ST_ROWS tokens the products find their rows by themselves
+  Mx4Slots up{topi, topw, counts, (int)T, (int)k, 1}, down{topi, topw, nullptr, (int)T, (int)k, 0};
+  const Mx4Slots* few = q.gemm ? nullptr : &up;
+  rc = mx4 ? launch_product<A_MX4, O_MX4, true>(p, few, m_tiles, stream)
+           : bf16 ? launch_product<A_BF16, O_BF16, true>(p, few, m_tiles, stream)
+                  : launch_product<A_F32, O_F32, true>(p, few, m_tiles, stream);
   if (rc) return rc;
-  rc = launch_linear(dn, at, mx4 ? O_BF16 : O_F32, q.gemm, m_tiles, stream);
+  rc = launch_linear(dn, at, mx4 ? O_BF16 : O_F32, q.gemm ? nullptr : &down, m_tiles, stream);
   if (rc) return rc;
-  return mx4 ? launch_combine<false, true>(ws + q.y, topi, topw, inv, out, T, d, k, stream)
-             : bf16 ? launch_combine<true, true>(ws + q.y, topi, topw, inv, out, T, d, k, stream)
-                    : launch_combine<true, false>(ws + q.y, topi, topw, inv, out, T, d, k, stream);
+  const int32_t* at_row = q.gemm ? inv : nullptr;
+  return mx4 ? launch_combine<false, true>(ws + q.y, topi, topw, at_row, out, T, d, k, E, stream)
+             : bf16 ? launch_combine<true, true>(ws + q.y, topi, topw, at_row, out, T, d, k, E, stream)
+                    : launch_combine<true, false>(ws + q.y, topi, topw, at_row, out, T, d, k, E, stream);
 }
 
 }  // extern "C"
