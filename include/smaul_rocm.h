@@ -266,6 +266,19 @@ int smaul_moe_forward(const void* x, int act_dtype, const float* gate_w, const f
                       int flags, hipStream_t stream);
 
 /*
+ * smaul_moe_forward on a routing that is given: topi [T, k] and topw [T, k] are INPUTS
+ * (smaul_moe_route's, or any other's), and no router runs; prob is not touched.  Slots
+ * with topi outside [0, E) or topw not above 0 add nothing.  gate_w is not read, but
+ * not NULL.
+ */
+int smaul_moe_forward_routed(const void* x, int act_dtype, const float* gate_w, const float* gate_b,
+                             const uint8_t* const* gate_w8, const float* const* gate_s, const uint8_t* const* up_w8,
+                             const float* const* up_s, const uint8_t* const* down_w8, const float* const* down_s,
+                             void* out, float* prob, int64_t* topi, float* topw, int32_t* counts, void* workspace,
+                             int64_t workspace_bytes, int64_t T, int64_t d, int64_t h, int64_t E, int64_t k,
+                             int64_t tile, int flags, hipStream_t stream);
+
+/*
  * smaul_moe_forward without a workspace argument: the layer's workspace is a
  * static device array inside the library (SMAUL_NOALLOC_SCRATCH_BYTES, one per
  * GPU, held until the process ends), so the call allocates nothing -- no

@@ -225,7 +225,7 @@ __device__ __forceinline__ void mx4_prep_weight(const Mx4Weight& m, int64_t E, i
   const int64_t q = i / m.N, n = i - q * m.N, e = q / ng, g = q - e * ng, row = e * m.N + n;
   const uint8_t* s = m.s + row * nb + g * 4;
   uint32_t d = 0;
-  if (nb % 4 == 0 && ((uintptr_t)m.s & 3) == 0) {
+  if (g * 4 + 4 <= nb && nb % 4 == 0 && ((uintptr_t)m.s & 3) == 0) {
     d = *(const uint32_t*)s;
   } else {
 #pragma unroll

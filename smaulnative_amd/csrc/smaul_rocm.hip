@@ -5372,6 +5372,18 @@ int smaul_moe_forward(const void* x, int act_dtype, const float* gate_w, const f
                           false, nullptr, stream);
 }
 
+int smaul_moe_forward_routed(const void* x, int act_dtype, const float* gate_w, const float* gate_b,
+                             const uint8_t* const* gate_w8, const float* const* gate_s, const uint8_t* const* up_w8,
+                             const float* const* up_s, const uint8_t* const* down_w8, const float* const* down_s,
+                             void* out, float* prob, int64_t* topi, float* topw, int32_t* counts, void* workspace,
+                             int64_t workspace_bytes, int64_t T, int64_t d, int64_t h, int64_t E, int64_t k,
+                             int64_t tile, int flags, hipStream_t stream) {
+  if (T > 0 && (!topi || !topw)) return fail(SMAUL_ERR_INVALID, "moe_forward_routed: needs topi and topw");
+  return moe_forward_impl(x, act_dtype, gate_w, gate_b, gate_w8, gate_s, up_w8, up_s, down_w8, down_s, out, prob, topi,
+                          topw, counts, workspace, workspace_bytes, T, d, h, E, k, tile, flags, nullptr, true, nullptr,
+                          stream);
+}
+
 int smaul_moe_forward_noalloc(const void* x, int act_dtype, const float* gate_w, const float* gate_b,
                               const uint8_t* const* gate_w8, const float* const* gate_s,
                               const uint8_t* const* up_w8, const float* const* up_s,

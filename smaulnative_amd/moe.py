@@ -17,6 +17,11 @@ a decode step does not force a device->host sync per layer.
 
 Only the plain architecture's dense SwiGLU experts are on this path; the rawr
 (sparse) experts are not (model.py:528-534).
+
+Beyond the reference, a config may ask for another router (``router_*``: sigmoid
+scores, groups, a balance bias, no renormalisation, a scale; the backend's
+``moe_route`` in place of its softmax router) and for experts in 4 bits
+(``precision="mx4"``, ``MX4Experts``).
 """
 from __future__ import annotations
 
@@ -41,8 +46,17 @@ class MoEConfig:
     tile: int = 64
     num_experts: int = 1
     num_experts_per_tok: int = 1
-    precision: str = "fp8"
+    precision: str = "fp8"  # "mx4": experts in microscaled 4-bit floating point
     architecture: str = "plain"
+    # the router (RocmBackend.moe_route); a config without these has the softmax top-k
+    router_score: str = "softmax"
+    router_groups: int = 1
+    router_top_groups: int | None = None
+    router_group_best: int = 2
+    router_renorm: bool = True
+    router_scale: float = 1.0
+    router_bias: bool = False  # a balance bias of the choice, moved by balance_step()
+    expert_act: str = "keep"  # mx4 experts: "mx4" rounds their activations too
 
     def __post_init__(self):
         for name in ("d_model", "tile", "num_experts", "num_experts_per_tok"):
@@ -123,6 +137,30 @@ class _GatherRows(torch.autograd.Function):
         return _sum_slots(dy, (ctx.saved_tensors[0], ctx.full)), None, None, None
 
 
+class _Route(torch.autograd.Function):
+    """(prob, topi, topw) of the backend's ``moe_route``, differentiable in the logits
+    through the scores and the chosen weights (the choice is a constant)."""
+
+    @staticmethod
+    def forward(ctx, logits, bias, top_k, args):
+        ctx.set_materialize_grads(False)
+        prob, topi, topw = get_backend().moe_route(logits, top_k, bias=bias, **args)
+        ctx.mark_non_differentiable(topi)
+        ctx.save_for_backward(logits, topi)
+        ctx.args = {n: args[n] for n in ("score", "renorm", "scale")}
+        return prob, topi, topw
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dprob, dtopi, dtopw):
+        logits, topi = ctx.saved_tensors
+        if dtopw is None:
+            if dprob is None:
+                return None, None, None, None
+            dtopw = torch.zeros(topi.shape, dtype=torch.float32, device=topi.device)
+        return get_backend().moe_route_backward(dtopw, logits, topi, dprob=dprob, **ctx.args), None, None, None
+
+
 class SwiFFN(nn.Module):
     """model.py:282-290: down((silu(gate(x).float()) * up(x).float()).to(x.dtype))."""
 
@@ -170,12 +208,55 @@ class SwiFFN_MoE(nn.Module):
         self.num_experts = cfg.num_experts
         self.architecture = "plain"
         self.tile = cfg.tile
-        self.experts = nn.ModuleList([SwiFFN(cfg) for _ in range(cfg.num_experts)])
+        if cfg.precision == "mx4":
+            from smaulnative_amd.mx4 import MX4Experts
+            self.experts = MX4Experts(cfg.num_experts, cfg.d_model, int(cfg.d_model * cfg.ffn_mult),
+                                      getattr(cfg, "expert_act", "keep"))
+        else:
+            self.experts = nn.ModuleList([SwiFFN(cfg) for _ in range(cfg.num_experts)])
         self.gate = nn.Linear(cfg.d_model, cfg.num_experts, bias=False)
+        self.route_args = self._route_config(cfg)
+        if getattr(cfg, "router_bias", False):
+            self.register_buffer("balance_bias", torch.zeros(cfg.num_experts))
+        else:
+            self.balance_bias = None
         self.last_prob = None
         self.last_topi = None
         self._counts_dev = None
         self._counts_host = [0] * cfg.num_experts
+
+    @staticmethod
+    def _route_config(cfg):
+        """moe_route's arguments from the config's ``router_*`` fields, or None for the
+        reference's router (softmax, top-k, renormalised)."""
+        E, k = cfg.num_experts, cfg.num_experts_per_tok
+        args = dict(score=getattr(cfg, "router_score", "softmax"), groups=getattr(cfg, "router_groups", 1),
+                    top_groups=getattr(cfg, "router_top_groups", None), group_best=getattr(cfg, "router_group_best", 2),
+                    renorm=getattr(cfg, "router_renorm", True), scale=getattr(cfg, "router_scale", 1.0))
+        if args["top_groups"] is None:
+            args["top_groups"] = args["groups"]
+        if args["score"] not in ("softmax", "sigmoid"):
+            raise ValueError(f"router_score must be 'softmax' or 'sigmoid', got {args['score']!r}")
+        if args["groups"] < 1 or E % args["groups"] or not 1 <= args["top_groups"] <= args["groups"] or \
+                args["top_groups"] * (E // args["groups"]) < k:
+            raise ValueError(f"router_groups ({args['groups']}) must divide the {E} experts and router_top_groups "
+                             f"({args['top_groups']}) of them hold {k}")
+        if args["group_best"] not in (1, 2):
+            raise ValueError(f"router_group_best must be 1 or 2, got {args['group_best']!r}")
+        plain = args["score"] == "softmax" and args["top_groups"] == args["groups"] and args["renorm"] and \
+            args["scale"] == 1.0 and not getattr(cfg, "router_bias", False)
+        return None if plain and cfg.precision != "mx4" else args
+
+    @torch.no_grad()
+    def balance_step(self, rate: float) -> None:
+        """Moves the balance bias by ``rate`` towards the experts that got fewer rows than
+        their share in the last forward, and away from the others."""
+        if self.balance_bias is None:
+            raise RuntimeError("balance_step: the layer has no balance bias (router_bias)")
+        counts = self._counts_dev
+        counts = torch.tensor(self._counts_host, device=self.balance_bias.device) if counts is None else counts
+        counts = counts.to(self.balance_bias.dtype)
+        self.balance_bias.add_(torch.sign(counts.mean() - counts), alpha=rate)
 
     # -- diagnostics (model.py:538-543,583-584,587-606), materialised lazily --
     @property
@@ -210,14 +291,35 @@ class SwiFFN_MoE(nn.Module):
             raise RuntimeError(f"compute backend {be.name!r} has no moe_forward entry")
         if _needs_grad(self, x):
             return self._forward_train(x)
-        experts = [ex.buffers6() for ex in self.experts]
-        out, prob, topi, counts = be.moe_forward(x, self.gate.weight, self.gate.bias, experts,
-                                                 self.top_k, self.tile)
+        if self.route_args is not None or not isinstance(self.experts, nn.ModuleList):
+            out, prob, topi, counts = self._forward_routed(be, x)
+        else:
+            experts = [ex.buffers6() for ex in self.experts]
+            out, prob, topi, counts = be.moe_forward(x, self.gate.weight, self.gate.bias, experts,
+                                                     self.top_k, self.tile)
         # plain attributes (or a subclass's properties), set past
         # nn.Module.__setattr__ (3 us each): none is a parameter, buffer or module
         for name, value in (("last_prob", prob), ("last_topi", topi), ("_counts_dev", counts)):
             object.__setattr__(self, name, value)
         return out
+
+    def _logits(self, xs):
+        return F.linear(xs.float(), self.gate.weight.float(), None if self.gate.bias is None else self.gate.bias.float())
+
+    def _forward_routed(self, be, x):
+        """(out, prob, topi, counts): the router's logits, ``moe_route``, and the experts on
+        that routing."""
+        lead, k = x.shape[:-1], self.top_k
+        xs = x.reshape(-1, x.shape[-1])
+        prob, topi, topw = be.moe_route(self._logits(xs), k, bias=self.balance_bias, **(self.route_args or {}))
+        if isinstance(self.experts, nn.ModuleList):
+            out, prob, topi, counts = be.moe_forward(xs, self.gate.weight, self.gate.bias,
+                                                     [ex.buffers6() for ex in self.experts], k, self.tile,
+                                                     routing=(prob, topi, topw))
+        else:
+            out, counts = be.mx4_moe_forward(xs if xs.is_floating_point() else xs.float(), topi, topw,
+                                             self.experts.buffers6(), self.experts.act)
+        return out.view(x.shape), prob.view(*lead, self.num_experts), topi.view(*lead, k), counts
 
     def _forward_train(self, x):
         """The layer with autograd, for training.
@@ -234,13 +336,17 @@ class SwiFFN_MoE(nn.Module):
         d = x.shape[-1]
         lead = x.shape[:-1]
         xs = x.reshape(-1, d)
-        prob = torch.softmax(self.gate(xs.float()), -1)
+        if self.route_args is not None or not isinstance(self.experts, nn.ModuleList):
+            prob, topi, topv = _Route.apply(self._logits(xs), self.balance_bias, self.top_k,
+                                            self.route_args or dict(score="softmax", renorm=True, scale=1.0))
+        else:
+            prob = torch.softmax(self.gate(xs.float()), -1)
+            topv, topi = torch.topk(prob, self.top_k, -1)
+            total = topv.sum(-1, keepdim=True)
+            topv = torch.where(total < 1e-6, torch.full_like(topv, 1.0 / self.top_k), topv / total.clamp_min(1e-9))
         # kept with x's leading dimensions, as the reference's are (model.py:558-565)
         self.last_prob = prob.view(*lead, self.num_experts)
-        topv, topi = torch.topk(prob, self.top_k, -1)
         self.last_topi = topi.detach().view(*lead, self.top_k)
-        total = topv.sum(-1, keepdim=True)
-        topv = torch.where(total < 1e-6, torch.full_like(topv, 1.0 / self.top_k), topv / total.clamp_min(1e-9))
         if xs.is_cuda and 0 < xs.shape[0] * self.top_k < 1 << 31 and self.num_experts <= 64 and self.top_k <= 8 and \
                 hasattr(get_backend(), "moe_dispatch"):
             out, counts = self._experts_dispatched(xs, topi, topv)

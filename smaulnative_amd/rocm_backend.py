@@ -982,15 +982,17 @@ class RocmBackend:
         _lib.check(rc, "wait_timeouts")
         return int(buf.item())
 
-    def moe_forward(self, x, gate_w, gate_b, experts, top_k, tile):
+    def moe_forward(self, x, gate_w, gate_b, experts, top_k, tile, routing=None):
         """SwiFFN_MoE.forward on the device.
 
         x: [..., d] bf16 or fp32; gate_w fp32 [E, d]; gate_b [E] or None;
         experts: E tuples (gate_w8, gate_sc, up_w8, up_sc, down_w8, down_sc).
         Returns (out [..., d] x.dtype, prob [..., E] fp32, topi [..., k] int64,
-        counts [E] int32 on the device).
+        counts [E] int32 on the device).  routing=(prob, topi, topw) [T, ...], as
+        ``moe_route`` gives them: the layer runs no router and returns prob and
+        topi as given; slots with topi outside [0, E) or topw not above 0 add nothing.
         """
-        return self._moe_forward(x, gate_w, gate_b, experts, top_k, tile, None)
+        return self._moe_forward(x, gate_w, gate_b, experts, top_k, tile, None, routing)
 
     def moe_forward_norm(self, x, gate_w, gate_b, experts, top_k, tile, norm_weight=None, eps=1e-6,
                          routing=None, next_router=None):
@@ -1094,7 +1096,9 @@ class RocmBackend:
                     out.data_ptr(), prob.data_ptr(), topi.data_ptr(), topw.data_ptr(),
                     counts.data_ptr(), ws.data_ptr(), ws_bytes, T, d, h, E, top_k, tile, eflags]
             with _device(dev):
-                if norm is None:
+                if norm is None and routing is not None:
+                    rc = lib.smaul_moe_forward_routed(*args, _stream_handle(dev))
+                elif norm is None:
                     rc = lib.smaul_moe_forward(*args, _stream_handle(dev))
                 elif routing is None and nxt is None:
                     rc = lib.smaul_moe_forward_norm(*args, None if nw is None else nw.data_ptr(), norm[1],

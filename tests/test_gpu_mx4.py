@@ -139,6 +139,20 @@ def test_linear_special_rows(act):
         assert (got[1][torch.arange(160) != 7] == 0).all()
 
 
+@pytest.mark.parametrize("K", [32, 128, 160, 384])
+@pytest.mark.parametrize("act", ["keep", "mx4"])
+def test_linear_nan_scales_stay_in_their_row(K, act):
+    """Widths that the products pad: the padding of a row takes nothing from the next one."""
+    gen = torch.Generator().manual_seed(K)
+    x = torch.randn(100, K, generator=gen).bfloat16()
+    w, s = ref.weight(48, K, gen)
+    s[1::2] = 255
+    got = get_backend("rocm").mx4_forward(*_dev(x, w, s), K, 48, act=act).cpu()
+    assert torch.isnan(got[:, 1::2]).all() and torch.isfinite(got[:, 0::2]).all()
+    dx = get_backend("rocm").mx4_backward_input(*_dev(got[:, :48].nan_to_num(), w, torch.where(s == 255, 120, s)), K, 48)
+    assert torch.isfinite(dx).all()
+
+
 def test_linear_wide_range():
     """Scales from one end to the other: the products keep their powers of two."""
     gen = torch.Generator().manual_seed(4)
