@@ -20,23 +20,59 @@ namespace {
 // ---------------------------------------------------------------------------
 // quantisation: 4 lanes a block, 8 values a lane
 // ---------------------------------------------------------------------------
-// 8 consecutive values of a row from column c0, 0 past K
-template <bool BF16, bool VEC>
+// 16 bytes from an address of no more than the values' own alignment
+typedef uint32_t u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+
+__device__ __forceinline__ void mx4_widen(const uint32_t (&u)[4], float* v) {  // 8 bf16
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[2 * j] = __uint_as_float(u[j] << 16);
+    v[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+  }
+}
+
+// 16 bytes that nobody reads again soon, past the caches
+typedef uint32_t u32x4_nt __attribute__((ext_vector_type(4)));
+template <bool NT>
+__device__ __forceinline__ uint4 mx4_ld16(const void* p) {
+  if constexpr (!NT) return *(const uint4*)p;
+  const u32x4_nt v = __builtin_nontemporal_load((const u32x4_nt*)p);
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
+template <bool NT>
+__device__ __forceinline__ void mx4_st16(void* p, uint4 v) {
+  if constexpr (!NT) *(uint4*)p = v;
+  else __builtin_nontemporal_store((u32x4_nt){v.x, v.y, v.z, v.w}, (u32x4_nt*)p);
+}
+
+// 8 consecutive values of a row from column c0, 0 past K.  VEC: whole, 16-byte aligned.
+template <bool BF16, bool VEC, bool NT = false>
 __device__ __forceinline__ void mx4_load8(const void* x, int64_t row, int64_t K, int64_t c0, float (&v)[8]) {
   const int64_t i = row * K + c0;
   if constexpr (VEC) {
     if constexpr (BF16) {
-      const uint4 w = *(const uint4*)((const uint16_t*)x + i);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[2 * j] = __uint_as_float(u[j] << 16);
-        v[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
-      }
+      const uint4 w = mx4_ld16<NT>((const uint16_t*)x + i);
+      mx4_widen({w.x, w.y, w.z, w.w}, v);
     } else {
-      const float4 a = *(const float4*)((const float*)x + i), b = *(const float4*)((const float*)x + i + 4);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 w = mx4_ld16<NT>((const float*)x + i + 4 * h);
+        v[4 * h] = __uint_as_float(w.x); v[4 * h + 1] = __uint_as_float(w.y);
+        v[4 * h + 2] = __uint_as_float(w.z); v[4 * h + 3] = __uint_as_float(w.w);
+      }
+    }
+  } else if (c0 + 8 <= K) {
+    if constexpr (BF16) {
+      const u32x4_at2 w = *(const u32x4_at2*)((const uint16_t*)x + i);
+      mx4_widen({w.x, w.y, w.z, w.w}, v);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const u32x4_at4 w = *(const u32x4_at4*)((const float*)x + i + 4 * h);
+        v[4 * h] = __uint_as_float(w.x); v[4 * h + 1] = __uint_as_float(w.y);
+        v[4 * h + 2] = __uint_as_float(w.z); v[4 * h + 3] = __uint_as_float(w.w);
+      }
     }
   } else {
 #pragma unroll
@@ -59,90 +95,106 @@ __device__ __forceinline__ uint32_t mx4_quad_max(uint32_t m) {
   return max(m, (uint32_t)__shfl_xor((int)m, 2, 4));
 }
 
-// VEC: K is a multiple of 32, so that groups of 8 values, their codes and their
-// blocks are each one run over the whole matrix; a thread takes MX4_U groups, all
-// loaded first.  Otherwise a row's last block is padded and a thread takes one.
+// A thread takes MX4_U groups of 8 values, all loaded first.  VEC: K is a multiple of
+// 32, so that the groups, their codes and their blocks are each one run over the whole
+// matrix; otherwise a row's last block is padded, and a group finds its row by a
+// division (32-bit where the groups' number is).  NT: the values' side goes past the
+// caches, where it is larger than they are anyway (65536 x 2048 bf16 there and back:
+// 143 us through them, 108 past them, 6.3 TB/s; a smaller result is left for its reader).
 constexpr int MX4_U = 4;
+constexpr int64_t MX4_NT_BYTES = 128LL << 20;  // half of the last cache
 
-template <bool BF16, bool VEC>
+// group i of rows of nb blocks: its row, and its first column
+template <bool VEC>
+__device__ __forceinline__ void mx4_place(int64_t i, int64_t nb, bool small, int64_t& row, int64_t& c0) {
+  if constexpr (VEC) {
+    row = 0;
+    c0 = i * 8;
+  } else if (small) {
+    const uint32_t r = (uint32_t)i / (uint32_t)(nb * 4);
+    row = r;
+    c0 = (int64_t)((uint32_t)i - r * (uint32_t)(nb * 4)) * 8;
+  } else {
+    row = i / (nb * 4);
+    c0 = (i - row * nb * 4) * 8;
+  }
+}
+
+template <bool BF16, bool VEC, bool NT>
 __global__ void __launch_bounds__(256)
 mx4_quantize_kernel(const void* __restrict__ x, uint32_t* __restrict__ codes, uint8_t* __restrict__ scales,
                     int64_t rows, int64_t K) {
   const int64_t nb = mx4_blocks(K), groups = rows * nb * 4;
-  if constexpr (VEC) {
-    const int64_t i0 = (int64_t)blockIdx.x * (256 * MX4_U) + threadIdx.x;
-    float v[MX4_U][8];
+  const bool small = groups < (1LL << 31);
+  const int64_t i0 = (int64_t)blockIdx.x * (256 * MX4_U) + threadIdx.x;
+  float v[MX4_U][8];
 #pragma unroll
-    for (int u = 0; u < MX4_U; ++u)
-      if (i0 + u * 256 < groups) mx4_load8<BF16, true>(x, 0, 0, (i0 + u * 256) * 8, v[u]);
+  for (int u = 0; u < MX4_U; ++u)
+    if (i0 + u * 256 < groups) {
+      int64_t row, c0;
+      mx4_place<VEC>(i0 + u * 256, nb, small, row, c0);
+      mx4_load8<BF16, VEC, NT>(x, row, K, c0, v[u]);
+    }
 #pragma unroll
-    for (int u = 0; u < MX4_U; ++u) {
-      const int64_t i = i0 + u * 256;
-      if (i < groups) {  // whole quads
-        const uint32_t byte = mx4_scale_byte(mx4_quad_max(mx4_amax8(v[u])));
-        codes[i] = mx4_encode8(v[u], byte);
-        if ((i & 3) == 0) scales[i >> 2] = (uint8_t)byte;
+  for (int u = 0; u < MX4_U; ++u) {
+    const int64_t i = i0 + u * 256;
+    if (i < groups) {  // whole quads
+      const uint32_t byte = mx4_scale_byte(mx4_quad_max(mx4_amax8(v[u])));
+      codes[i] = mx4_encode8(v[u], byte);
+      if ((i & 3) == 0) scales[i >> 2] = (uint8_t)byte;
+    }
+  }
+}
+
+// 8 decoded values (bf16 pairs) to y[o ..]; whole: all of them are the row's (`left`)
+template <bool BF16, bool VEC, bool NT>
+__device__ __forceinline__ void mx4_store8(void* y, int64_t o, int64_t left, uint4 d) {
+  const uint32_t u[4] = {d.x, d.y, d.z, d.w};
+  if (VEC || left >= 8) {
+    if constexpr (BF16) {
+      const u32x4_at2 w = {d.x, d.y, d.z, d.w};
+      if constexpr (VEC) mx4_st16<NT>((uint16_t*)y + o, d);
+      else *(u32x4_at2*)((uint16_t*)y + o) = w;
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const u32x4_at4 w = {u[2 * h] << 16, u[2 * h] & 0xffff0000u, u[2 * h + 1] << 16, u[2 * h + 1] & 0xffff0000u};
+        if constexpr (VEC) mx4_st16<NT>((float*)y + o + 4 * h, make_uint4(w.x, w.y, w.z, w.w));
+        else *(u32x4_at4*)((float*)y + o + 4 * h) = w;
       }
     }
   } else {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= groups) return;
-    const int64_t blk = i >> 2, row = blk / nb, b = blk - row * nb;
-    float v[8];
-    mx4_load8<BF16, false>(x, row, K, b * MX4_BLOCK + (i & 3) * 8, v);
-    const uint32_t byte = mx4_scale_byte(mx4_quad_max(mx4_amax8(v)));
-    codes[i] = mx4_encode8(v, byte);
-    if ((i & 3) == 0) scales[blk] = (uint8_t)byte;
-  }
-}
-
-// 8 decoded values to a row from its column c0, 16 bytes at a time
-template <bool BF16>
-__device__ __forceinline__ void mx4_store8(void* y, int64_t o, uint4 d) {
-  if constexpr (BF16) {
-    *(uint4*)((uint16_t*)y + o) = d;
-  } else {
-    const uint32_t u[4] = {d.x, d.y, d.z, d.w};
-    float4* p = (float4*)((float*)y + o);
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      p[j] = make_float4(__uint_as_float(u[2 * j] << 16), __uint_as_float(u[2 * j] & 0xffff0000u),
-                         __uint_as_float(u[2 * j + 1] << 16), __uint_as_float(u[2 * j + 1] & 0xffff0000u));
-  }
-}
-
-template <bool BF16, bool VEC>
-__global__ void __launch_bounds__(256)
-mx4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, void* __restrict__ y,
-                      int64_t rows, int64_t K) {
-  const int64_t nb = mx4_blocks(K), groups = rows * nb * 4;
-  if constexpr (VEC) {
-    const int64_t i0 = (int64_t)blockIdx.x * (256 * MX4_U) + threadIdx.x;
-    uint32_t c[MX4_U], s[MX4_U];
-#pragma unroll
-    for (int u = 0; u < MX4_U; ++u)
-      if (i0 + u * 256 < groups) {
-        c[u] = codes[i0 + u * 256];
-        s[u] = scales[(i0 + u * 256) >> 2];
-      }
-#pragma unroll
-    for (int u = 0; u < MX4_U; ++u)
-      if (i0 + u * 256 < groups) mx4_store8<BF16>(y, (i0 + u * 256) * 8, mx4_decode8(c[u], mx4_scale(s[u])));
-  } else {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= groups) return;
-    const int64_t blk = i >> 2, row = blk / nb, c0 = (blk - row * nb) * MX4_BLOCK + (i & 3) * 8;
-    const uint4 d = mx4_decode8(codes[i], mx4_scale(scales[blk]));
-    const uint32_t u[4] = {d.x, d.y, d.z, d.w};
-    const int64_t o = row * K + c0;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (c0 + j < K) {
+      if (j < left) {
         const uint32_t b = j & 1 ? u[j / 2] >> 16 : u[j / 2] & 0xffffu;
         if constexpr (BF16) ((uint16_t*)y)[o + j] = (uint16_t)b;
         else ((float*)y)[o + j] = __uint_as_float(b << 16);
       }
   }
+}
+
+template <bool BF16, bool VEC, bool NT>
+__global__ void __launch_bounds__(256)
+mx4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, void* __restrict__ y,
+                      int64_t rows, int64_t K) {
+  const int64_t nb = mx4_blocks(K), groups = rows * nb * 4;
+  const bool small = groups < (1LL << 31);
+  const int64_t i0 = (int64_t)blockIdx.x * (256 * MX4_U) + threadIdx.x;
+  uint32_t c[MX4_U], s[MX4_U];
+#pragma unroll
+  for (int u = 0; u < MX4_U; ++u)
+    if (i0 + u * 256 < groups) {
+      c[u] = codes[i0 + u * 256];
+      s[u] = scales[(i0 + u * 256) >> 2];
+    }
+#pragma unroll
+  for (int u = 0; u < MX4_U; ++u)
+    if (i0 + u * 256 < groups) {
+      int64_t row, c0;
+      mx4_place<VEC>(i0 + u * 256, nb, small, row, c0);
+      mx4_store8<BF16, VEC, NT>(y, row * K + c0, K - c0, mx4_decode8(c[u], mx4_scale(s[u])));
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -1104,12 +1156,13 @@ int launch_quantize(const void* x, int dtype, uint8_t* codes, uint8_t* scales, i
   const int64_t threads = rows * mx4_blocks(K) * 4;
   if (threads > 256LL * 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_quantize: too many values");
   const bool vec = K % MX4_BLOCK == 0 && aligned(x, 16), bf16 = dtype == SMAUL_DTYPE_BF16;
-  const int64_t per = vec ? 256 * MX4_U : 256;
+  constexpr int64_t per = 256 * MX4_U;
   const dim3 grid((unsigned)((threads + per - 1) / per)), block(256);
-#define SMAUL_Q(B, V) \
-  hipLaunchKernelGGL((mx4_quantize_kernel<B, V>), grid, block, 0, stream, x, (uint32_t*)codes, scales, rows, K)
-  if (bf16) { if (vec) SMAUL_Q(true, true); else SMAUL_Q(true, false); }
-  else { if (vec) SMAUL_Q(false, true); else SMAUL_Q(false, false); }
+  const bool nt = rows * K * (bf16 ? 2 : 4) >= MX4_NT_BYTES;
+#define SMAUL_Q(B, V, N) \
+  hipLaunchKernelGGL((mx4_quantize_kernel<B, V, N>), grid, block, 0, stream, x, (uint32_t*)codes, scales, rows, K)
+  if (bf16) { if (vec && nt) SMAUL_Q(true, true, true); else if (vec) SMAUL_Q(true, true, false); else SMAUL_Q(true, false, false); }
+  else { if (vec && nt) SMAUL_Q(false, true, true); else if (vec) SMAUL_Q(false, true, false); else SMAUL_Q(false, false, false); }
 #undef SMAUL_Q
   return check_launch("mx4_quantize_kernel");
 }
@@ -1237,12 +1290,14 @@ int smaul_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* y, i
   const int64_t threads = rows * mx4_blocks(K) * 4;
   if (threads > 256LL * 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_dequantize: too many values");
   const bool vec = K % MX4_BLOCK == 0 && aligned(y, 16), bf16 = dtype == SMAUL_DTYPE_BF16;
-  const int64_t per = vec ? 256 * MX4_U : 256;
+  constexpr int64_t per = 256 * MX4_U;
   const dim3 grid((unsigned)((threads + per - 1) / per)), block(256);
-#define SMAUL_D(B, V) \
-  hipLaunchKernelGGL((mx4_dequantize_kernel<B, V>), grid, block, 0, stream, (const uint32_t*)codes, scales, y, rows, K)
-  if (bf16) { if (vec) SMAUL_D(true, true); else SMAUL_D(true, false); }
-  else { if (vec) SMAUL_D(false, true); else SMAUL_D(false, false); }
+  const bool nt = rows * K * (bf16 ? 2 : 4) >= MX4_NT_BYTES;
+#define SMAUL_D(B, V, N)                                                                                       \
+  hipLaunchKernelGGL((mx4_dequantize_kernel<B, V, N>), grid, block, 0, stream, (const uint32_t*)codes, scales, \
+                     y, rows, K)
+  if (bf16) { if (vec && nt) SMAUL_D(true, true, true); else if (vec) SMAUL_D(true, true, false); else SMAUL_D(true, false, false); }
+  else { if (vec && nt) SMAUL_D(false, true, true); else if (vec) SMAUL_D(false, true, false); else SMAUL_D(false, false, false); }
 #undef SMAUL_D
   return check_launch("mx4_dequantize_kernel");
 }
