@@ -420,37 +420,33 @@ constexpr int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 bool aligned(const void* p, int to) { return ((uintptr_t)p & (to - 1)) == 0; }
 bool dtype_ok(int d) { return d == SMAUL_DTYPE_F32 || d == SMAUL_DTYPE_BF16; }
 
-// The kernel of larger calls: K in stages of KS, activations, codes and scales brought
-// to LDS by DMA, NSTAGE stages in flight, WM x WN waves over BM rows x BN columns.
+// The two kernels of larger calls: K in stages of KS, activations, codes and scales
+// brought to LDS by DMA, NSTAGE stages in flight, WM x WN waves over BM rows x BN
+// columns.
 //
 // Roles: the weight's rows are the matrix instruction's rows and the activations its
 // columns, and row i of a 32 x 32 tile is given weight row 16 ((i / 4) % 2) + 4 (i / 8)
 // + i % 4, so that the 16 sums of a lane are 16 consecutive outputs of one activation
-// row: they leave as whole 16-byte stores, and a block of the format has its largest
-// value in 8 instructions and one exchange.
-//
-// A_MX4 runs v_mfma_scale_f32_32x32x64_f8f6f4 on the codes as they are: lane i + 32 g
-// has block g of a 64-wide step of its row, one scale byte for the 32 values.  A_BF16
-// and A_F32 decode: a lane's 16 bytes of codes are its block g of the 64-wide step,
-// times their scale (exact), and MFMA q multiplies values 32 g + 8 q and on; fp32
-// activations are three bf16 terms, split after the LDS read.
-//
-// Stages are as wide as make their rows whole cache lines: what bounds the loop is the
-// number of L2 requests, and half a line costs as much as a whole one (16384 rows,
-// K 4096 -> 4096: 190 us with 64-byte rows of codes).
+// row: whole 16-byte pieces, and a block of the format has its largest value in 8
+// instructions and one exchange.
 template <int AT, int WF, int BM, int BN, int WM, int WN, int KS, int NSTAGE>
 struct Mx4Cfg {
   static constexpr int NW = WM * WN;
   static constexpr int XROW = AT == A_MX4 ? KS / 2 : AT == A_BF16 ? KS * 2 : KS * 4;
   static constexpr int WROW = WF == W_BF16 ? KS * 2 : KS / 2;
   static constexpr int XB = BM * XROW, WB = BN * WROW;
-  static constexpr int SROWS = WF == W_BF16 ? 0 : BN + (AT == A_MX4 ? BM : 0), SG = KS < 128 ? 1 : KS / 128;  // scale rows, dwords a row
+  static constexpr int SROWS = WF == W_BF16 ? 0 : BN + (AT == A_MX4 ? BM : 0);  // of scales
+  static constexpr int SG = KS < 128 ? 1 : KS / 128;                            // dwords of each
   static constexpr int STAGE = XB + WB + SROWS * SG * 4;
   // DMA instructions: a wave's of x and W, all of the scales
   static constexpr int X_INS = XB / (1024 * NW), W_INS = WB / (1024 * NW), S_INS = SROWS * SG / 64;
   static constexpr int DMA_MIN = X_INS + W_INS + S_INS / NW;
+  static constexpr int SI = (S_INS + NW - 1) / NW < 1 ? 1 : (S_INS + NW - 1) / NW, SP = SROWS < 64 ? 1 : SROWS / 64;
+  static constexpr int SD = NW % SP == 0 ? 1 : SI;  // different rows of a wave's scale instructions
   static constexpr int TT = BM / WM / 32, WT = BN / WN / 32;  // 32 x 32 tiles of a wave
+  static constexpr int COLS = BN, KW = KS;
   static constexpr int LDS = NSTAGE * STAGE;
+  static constexpr int XS = AT == A_MX4 ? 16 : AT == A_BF16 ? 2 : 4;  // bytes of a unit of ldx
   static_assert(XB % (1024 * NW) == 0 && WB % (1024 * NW) == 0 && SROWS % 64 == 0, "whole DMA instructions");
   static_assert(DMA_MIN * (NSTAGE - 2) < 64 && LDS <= 160 * 1024, "pipeline depth");
 };
@@ -480,6 +476,89 @@ __device__ __forceinline__ i32x8_t mx4_operand(uint4 c) {
   r[0] = (int)c.x; r[1] = (int)c.y; r[2] = (int)c.z; r[3] = (int)c.w;
   r[4] = r[5] = r[6] = r[7] = 0;
   return r;
+}
+
+// Where a lane's DMA instructions of a tile read, and the tile's first rows.
+template <class C, int WF, bool SWIGLU>
+struct Mx4Source {
+  const char* X;
+  const uint8_t *W1, *W2, *S1, *S2;
+  uint32_t x_off[C::X_INS], w_off[C::W_INS], s_off[C::SD];
+};
+
+// 32-bit offsets from the tile's first rows (gathered rows' from x's; the host checks its
+// size).  Rows past the end read the last one: their sums are not stored.  row_of(r):
+// x row of the tile's row r, from row0 where rows are not gathered.
+template <class C, int WF, bool SWIGLU, class RowOf>
+__device__ __forceinline__ void mx4_source(const Mx4Args& p, int e, int64_t row0, int64_t n0, int lane, int wave,
+                                           RowOf row_of, Mx4Source<C, WF, SWIGLU>& q) {
+  constexpr int XL = C::XROW / 16, XR = 64 / XL;  // lanes a row, rows an instruction
+  const int64_t eblocks = (int64_t)e * p.N * p.ldw;  // ldw / 4 groups of N dwords: as many bytes as blocks
+  const int64_t nw = min<int64_t>(n0, p.N - 1);      // first weight row; a tile of padding reads the last
+  const int64_t w0 = (eblocks + nw * p.ldw) * 16, s0 = eblocks + nw * 4;
+  q.W1 = p.w + (WF == W_BF16 ? nw * p.ldw * 2 : w0);
+  q.S1 = p.s + s0;
+  q.W2 = SWIGLU ? p.w2 + w0 : q.W1;
+  q.S2 = SWIGLU ? p.s2 + s0 : q.S1;
+  q.X = (const char*)p.x + (p.row_idx ? 0 : row0 * p.ldx * C::XS);
+#pragma unroll
+  for (int a = 0; a < C::X_INS; ++a) {
+    const int r = (wave * C::X_INS + a) * XR + lane / XL;
+    q.x_off[a] = (uint32_t)(row_of(r) * p.ldx * C::XS + mx4_swz<C::XROW>(r, lane % XL) * 16);
+  }
+  // staged weight row r, from the first: tiles of 32 (gate's, then up's), permuted
+  const int64_t left = p.N - 1 - nw;
+  auto w_row = [&](int r) -> int64_t {
+    int t = r >> 5;
+    if (SWIGLU) t = t >= C::COLS / 64 ? t - C::COLS / 64 : t;
+    return min<int64_t>(t * 32 + mx4_perm(r & 31), left);
+  };
+  constexpr int WL = C::WROW / 16, WR = 64 / WL;
+#pragma unroll
+  for (int b = 0; b < C::W_INS; ++b) {
+    const int r = (wave * C::W_INS + b) * WR + lane / WL;
+    q.w_off[b] = (uint32_t)(w_row(r) * p.ldw * (WF == W_BF16 ? 2 : 16) + mx4_swz<C::WROW>(r, lane % WL) * 16);
+  }
+  // scale instruction i stages 64 rows of one group: of the weight's, then of x's
+#pragma unroll
+  for (int i = 0; i < C::SD; ++i) {
+    const int r = (wave + C::NW * i) % C::SP * 64;
+    q.s_off[i] = (uint32_t)(r < C::COLS ? w_row(r + lane) : (p.row_idx ? 0 : row0) + row_of(r + lane - C::COLS)) * 4;
+  }
+}
+
+// the loads of stage kt into the stage buffer at LDS address l
+template <class C, int WF, bool SWIGLU>
+__device__ __forceinline__ void mx4_dma(const Mx4Args& p, const Mx4Source<C, WF, SWIGLU>& q, int wave, int kt,
+                                        uint32_t l) {
+  constexpr int WR = 64 / (C::WROW / 16);
+#pragma unroll
+  for (int i = 0; i < C::SI; ++i) {
+    const int j = wave + C::NW * i, r = (C::SD == 1 ? wave : j) % C::SP * 64;
+    if (C::S_INS > 0 && (C::S_INS % C::NW == 0 || j < C::S_INS)) {  // uniform
+      const int64_t grp = C::KW < 128 ? kt / (128 / C::KW) : (int64_t)kt * C::SG + j / C::SP;
+      const uint8_t* src =
+          r >= C::COLS ? p.xs + grp * p.xrows * 4 : (SWIGLU && r >= C::COLS / 2 ? q.S2 : q.S1) + grp * p.N * 4;
+      dma4(src, q.s_off[i % C::SD], l + C::XB + C::WB + j * 256);
+    }
+  }
+  const char* xk = q.X + (int64_t)kt * C::XROW;
+#pragma unroll
+  for (int a = 0; a < C::X_INS; ++a) dma16(xk, q.x_off[a], l + (wave * C::X_INS + a) * 1024);
+#pragma unroll
+  for (int b = 0; b < C::W_INS; ++b) {
+    const int r = (wave * C::W_INS + b) * WR;
+    dma16((SWIGLU && r >= C::COLS / 2 ? q.W2 : q.W1) + (int64_t)kt * C::WROW, q.w_off[b],
+          l + C::XB + (wave * C::W_INS + b) * 1024);
+  }
+}
+
+// tile `lin` of m_tiles by n_tiles, in groups of 8 row tiles by all column tiles
+__device__ __forceinline__ void mx4_tile_at(int lin, int m_tiles, int n_tiles, int& mt, int& nt) {
+  constexpr int GM = 8;
+  const int g = lin / (GM * n_tiles), within = lin - g * GM * n_tiles, gm = min(GM, m_tiles - g * GM);
+  mt = g * GM + within % gm;
+  nt = within / gm;
 }
 
 // 16 consecutive sums of row `row` from column n, cast; columns from `ld` on are not
@@ -514,273 +593,15 @@ __device__ __forceinline__ void mx4_store16(void* out, int64_t row, int64_t ld, 
   }
 }
 
-template <int AT, int WF, int OT, bool SWIGLU, int BM, int BN, int WM, int WN, int KS, int NSTAGE>
-__global__ void __launch_bounds__(WM * WN * 64, 2) mx4_gemm_kernel(Mx4Args p) {
-  using C = Mx4Cfg<AT, WF, BM, BN, WM, WN, KS, NSTAGE>;
-  constexpr int TT = C::TT, WT = C::WT, NW = C::NW, BNO = SWIGLU ? BN / 2 : BN, XROW = C::XROW, WROW = C::WROW;
-  __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave / WN, wn = wave % WN;
-
-  // a contiguous band of tiles for each XCD (workgroup b runs on XCD b % 8), in
-  // groups of GM row tiles by all column tiles
-  int mt, nt;
-  {
-    constexpr int GM = 8, NXCD = 8;
-    const int n_tiles = (int)((mx4_cols<OT>(p) + BNO - 1) / BNO), total = gridDim.x, m_tiles = total / n_tiles;
-    int lin = blockIdx.x;
-    const int full = total / NXCD * NXCD;
-    if (lin < full) lin = lin % NXCD * (full / NXCD) + lin / NXCD;
-    const int g = lin / (GM * n_tiles), within = lin - g * GM * n_tiles, gm = min(GM, m_tiles - g * GM);
-    mt = g * GM + within % gm;
-    nt = within / gm;
-  }
-  int e, rows;
-  int64_t row0;
-  if (!mx4_tile<BM>(p, mt, lane, e, row0, rows)) return;
-  const int64_t n0 = (int64_t)nt * BNO;
-  const int64_t eblocks = (int64_t)e * p.N * p.ldw;  // ldw / 4 groups of N dwords: as many bytes as blocks
-  const int64_t nw = min<int64_t>(n0, p.N - 1);  // the tile's first weight row; a tile of padding reads the last
-  const int64_t w0 = (eblocks + nw * p.ldw) * 16, s0 = eblocks + nw * 4;
-  const uint8_t* W1 = p.w + (WF == W_BF16 ? nw * p.ldw * 2 : w0);
-  const uint8_t* S1 = p.s + s0;
-  const uint8_t* W2 = SWIGLU ? p.w2 + w0 : W1;
-  const uint8_t* S2 = SWIGLU ? p.s2 + s0 : S1;
-
-  // ---- DMA sources of this lane: 32-bit offsets from the tile's first rows (gathered
-  // ones from x's; the host checks its size).  Rows past the end read the last one: their
-  // sums are not stored.
-  constexpr int XS = AT == A_MX4 ? 16 : AT == A_BF16 ? 2 : 4;
-  const char* X = (const char*)p.x + (p.row_idx ? 0 : row0 * p.ldx * XS);
-  constexpr int XL = XROW / 16, XR = 64 / XL;  // lanes a row, rows an instruction
-  uint32_t x_off[C::X_INS];
-#pragma unroll
-  for (int a = 0; a < C::X_INS; ++a) {
-    const int r = (wave * C::X_INS + a) * XR + lane / XL;
-    const int lr = min(r, rows - 1);
-    const int64_t xr = p.row_idx ? (int64_t)p.row_idx[row0 + lr] : lr;
-    x_off[a] = (uint32_t)(xr * p.ldx * XS + mx4_swz<XROW>(r, lane % XL) * 16);
-  }
-  // staged weight row q, from the first: tiles of 32 (gate's, then up's), permuted
-  const int64_t left = p.N - 1 - nw;
-  auto w_row = [&](int q) -> int64_t {
-    int t = q >> 5;
-    if (SWIGLU) t = t >= BN / 64 ? t - BN / 64 : t;
-    return min<int64_t>(t * 32 + mx4_perm(q & 31), left);
-  };
-  constexpr int WL = WROW / 16, WR = 64 / WL;
-  uint32_t w_off[C::W_INS];
-#pragma unroll
-  for (int b = 0; b < C::W_INS; ++b) {
-    const int q = (wave * C::W_INS + b) * WR + lane / WL;
-    w_off[b] = (uint32_t)(w_row(q) * p.ldw * (WF == W_BF16 ? 2 : 16) + mx4_swz<WROW>(q, lane % WL) * 16);
-  }
-  // scale instruction i stages 64 rows of one group: of the weight's, then of x's
-  constexpr int SI = (C::S_INS + NW - 1) / NW, SP = C::SROWS < 64 ? 1 : C::SROWS / 64;
-  uint32_t s_off[SI < 1 ? 1 : SI];
-#pragma unroll
-  for (int i = 0; i < SI; ++i) {
-    const int q = (wave + NW * i) % SP * 64 + lane;
-    if (q < BN) {
-      s_off[i] = (uint32_t)(w_row(q) * 4);
-    } else {
-      const int64_t lr = row0 + min(q - BN, rows - 1);
-      s_off[i] = (uint32_t)((p.row_idx ? (int64_t)p.row_idx[lr] : lr) * 4);
-    }
-  }
-
-  const uint32_t lds0 = lds_offset(&smem[0]);
-  auto dma_stage = [&](int kt, int buf) {
-    const uint32_t l = lds0 + (uint32_t)(buf * C::STAGE);
-#pragma unroll
-    for (int i = 0; i < SI; ++i) {
-      const int q = wave + NW * i, r = q % SP * 64;
-      if (C::S_INS % NW == 0 || q < C::S_INS) {
-        const int64_t grp = KS < 128 ? kt / (128 / KS) : (int64_t)kt * C::SG + q / SP;
-        const uint8_t* src = r >= BN ? p.xs + grp * p.xrows * 4 : (SWIGLU && r >= BN / 2 ? S2 : S1) + grp * p.N * 4;
-        dma4(src, s_off[i], l + C::XB + C::WB + q * 256);
-      }
-    }
-    const char* xk = X + (int64_t)kt * XROW;
-#pragma unroll
-    for (int a = 0; a < C::X_INS; ++a) dma16(xk, x_off[a], l + (wave * C::X_INS + a) * 1024);
-#pragma unroll
-    for (int b = 0; b < C::W_INS; ++b) {
-      const int q = (wave * C::W_INS + b) * WR;
-      dma16((SWIGLU && q >= BN / 2 ? W2 : W1) + (int64_t)kt * WROW, w_off[b],
-            l + C::XB + (wave * C::W_INS + b) * 1024);
-    }
-  };
-
+// The sums of a wave's tiles to y.  bf16 rows leave as pieces of 64 bytes, four lanes a
+// row, through 2 KB of LDS of the wave's own: a store of 16 bytes to each of 64 rows is
+// 64 requests (16384 x 4096 x 4096: 203 us so, 191 through LDS; past the caches 187, but
+// 4096 rows 58 us for 52, as half a line is then fetched again).
+template <int OT, bool SWIGLU, int BM, int BN, int WM, int WN>
+__device__ __forceinline__ void mx4_epilogue(const Mx4Args& p, const f32x16_t (&acc)[BN / WN / 32][BM / WM / 32],
+                                             int64_t row0, int rows, int64_t n0, int wm, int wn, int lane, char* own) {
+  constexpr int TT = BM / WM / 32, WT = BN / WN / 32, BNO = SWIGLU ? BN / 2 : BN, OTW = SWIGLU ? WT / 2 : WT;
   const int g = lane >> 5, l32 = lane & 31;
-  // staged row of weight tile j of this wave: with SwiGLU its gate tiles, then its up tiles
-  auto w_tile = [&](int j) -> int {
-    if constexpr (SWIGLU)
-      return j < WT / 2 ? wn * (BN / WN / 2) + j * 32 : BN / 2 + wn * (BN / WN / 2) + (j - WT / 2) * 32;
-    else return wn * (BN / WN) + j * 32;
-  };
-  f32x16_t acc[WT][TT];
-#pragma unroll
-  for (int j = 0; j < WT; ++j)
-#pragma unroll
-    for (int i = 0; i < TT; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[j][i][r] = 0.0f;
-
-  const int nk = (int)(p.K / KS);
-  if constexpr (AT == A_MX4) {
-    // Steps of 64: the operands of a step are read from LDS while the step before is
-    // multiplied, the first of a stage during the last of the stage before.  By then
-    // every wave has the rest of its stage in registers, so that one barrier frees
-    // the buffer for the loads of the stage after the next.  (Left to itself the
-    // compiler reads each operand just before its use: 2.2 times the time of the
-    // instructions' own.)
-    constexpr int STEPS = KS / 64;
-    static_assert(STEPS == 2 || STEPS == 4, "the operands' double buffers repeat every 4 steps");
-    i32x8_t wf[2][WT], xf[2][TT];
-    uint32_t sw[2][WT], sx[2][TT];
-    const char* w_at[WT];  // fixed parts of the addresses
-    const char* x_at[TT];
-#pragma unroll
-    for (int j = 0; j < WT; ++j) w_at[j] = smem + C::XB + (w_tile(j) + l32) * WROW;
-#pragma unroll
-    for (int i = 0; i < TT; ++i) x_at[i] = smem + (wm * (BM / WM) + i * 32 + l32) * XROW;
-    const char* s_at = smem + C::XB + C::WB + l32 * 4;
-    // step u (of 4) is step u % STEPS of a stage
-    auto read = [&](int buf, int u) {
-      const int st = u % STEPS, o = buf * C::STAGE, c = st * 2 + g, to = u & 1;
-      if (u % 2 == 0) {  // the scales of a group of 128
-        const int sb = st / 2;
-#pragma unroll
-        for (int j = 0; j < WT; ++j)
-          sw[u / 2][j] = *(const uint32_t*)(s_at + o + (sb * C::SROWS + w_tile(j)) * 4);
-#pragma unroll
-        for (int i = 0; i < TT; ++i)
-          sx[u / 2][i] = *(const uint32_t*)(s_at + o + (sb * C::SROWS + BN + wm * (BM / WM) + i * 32) * 4);
-      }
-      // tiles are 32 rows apart, which the swizzles do not see
-#pragma unroll
-      for (int i = 0; i < TT; ++i) xf[to][i] = mx4_operand(*(const uint4*)(x_at[i] + o + mx4_swz<XROW>(l32, c) * 16));
-#pragma unroll
-      for (int j = 0; j < WT; ++j) wf[to][j] = mx4_operand(*(const uint4*)(w_at[j] + o + mx4_swz<WROW>(l32, c) * 16));
-    };
-    auto multiply = [&](int u) {
-      if (u % 2 == 0) {  // this lane's blocks, g and g + 2 of the four, to bytes 0 and 2
-#pragma unroll
-        for (int j = 0; j < WT; ++j) sw[u / 2][j] >>= 8 * g;
-#pragma unroll
-        for (int i = 0; i < TT; ++i) sx[u / 2][i] >>= 8 * g;
-      }
-#pragma unroll
-      for (int j = 0; j < WT; ++j)
-#pragma unroll
-        for (int i = 0; i < TT; ++i)
-          acc[j][i] = u % 2 == 0
-              ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[0][j], xf[0][i], acc[j][i], 4, 4, 0,
-                                                                (int)sw[u / 2][j], 0, (int)sx[u / 2][i])
-              : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[1][j], xf[1][i], acc[j][i], 4, 4, 2,
-                                                                (int)sw[u / 2][j], 2, (int)sx[u / 2][i]);
-    };
-#pragma unroll
-    for (int s = 0; s < NSTAGE; ++s) dma_stage(s < nk ? s : nk - 1, s);
-    wait_vm<C::DMA_MIN * (NSTAGE - 1)>();
-    __syncthreads();
-    read(0, 0);
-    int buf = 0;
-    for (int kt = 0; kt < nk; kt += 4 / STEPS) {  // K is a multiple of 256
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if ((u + 1) % STEPS != 0) {
-          read(buf, u + 1);
-        } else {
-          const int next = buf + 1 == NSTAGE ? 0 : buf + 1, ks = kt + u / STEPS + NSTAGE;
-          wait_vm<C::DMA_MIN * (NSTAGE - 2)>();
-          __syncthreads();
-          dma_stage(ks < nk ? ks : nk - 1, buf);
-          read(next, (u + 1) & 3);
-          buf = next;
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(u);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    wait_vm<0>();
-  } else {
-    auto compute = [&](int buf, int kt) {
-      const char* xs_ = smem + buf * C::STAGE;
-      const char* ws_ = xs_ + C::XB;
-      const char* ss_ = ws_ + C::WB;
-#pragma unroll
-      for (int h = 0; h < KS / 64; ++h) {
-        const int sh = 8 * g + 16 * (KS < 128 ? kt & 1 : h & 1);
-        uint4 wc[WT];  // codes of block g of each weight row, and its scale
-        float sc[WT];
-#pragma unroll
-        for (int j = 0; j < WT && WF == W_MX4; ++j) {
-          const int r = w_tile(j) + l32;
-          wc[j] = *(const uint4*)(ws_ + r * WROW + mx4_swz<WROW>(r, h * 2 + g) * 16);
-          sc[j] = mx4_scale((*(const uint32_t*)(ss_ + (h / 2 * C::SROWS + r) * 4) >> sh) & 255u);
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          constexpr int NT = AT == A_F32 ? 3 : 1;
-          bf16x8_t xf[TT][NT];
-#pragma unroll
-          for (int i = 0; i < TT; ++i) {
-            const int r = wm * (BM / WM) + i * 32 + l32;
-            if constexpr (AT == A_BF16) {
-              xf[i][0] = *(const bf16x8_t*)(xs_ + r * XROW + mx4_swz<XROW>(r, h * 8 + g * 4 + q) * 16);
-            } else {
-              const float4 a = *(const float4*)(xs_ + r * XROW + mx4_swz<XROW>(r, h * 16 + g * 8 + q * 2) * 16);
-              const float4 b = *(const float4*)(xs_ + r * XROW + mx4_swz<XROW>(r, h * 16 + g * 8 + q * 2 + 1) * 16);
-              const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-              bf16x8_t t[3];
-              mx4_split3(v, t);
-#pragma unroll
-              for (int k = 0; k < NT; ++k) xf[i][k] = t[k];
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < WT; ++j) {
-            bf16x8_t wf;
-            if constexpr (WF == W_BF16) {
-              const int r = w_tile(j) + l32;
-              wf = *(const bf16x8_t*)(ws_ + r * WROW + mx4_swz<WROW>(r, h * 8 + g * 4 + q) * 16);
-            } else {
-              const uint32_t c = q == 0 ? wc[j].x : q == 1 ? wc[j].y : q == 2 ? wc[j].z : wc[j].w;
-              wf = __builtin_bit_cast(bf16x8_t, mx4_decode8(c, sc[j]));
-            }
-#pragma unroll
-            for (int i = 0; i < TT; ++i)
-#pragma unroll
-              for (int k = 0; k < NT; ++k)
-                acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf, xf[i][k], acc[j][i], 0, 0, 0);
-          }
-        }
-      }
-    };
-    // Stage kt is complete when at most the loads of the later stages are outstanding;
-    // the barrier publishes it and frees the buffer of stage kt - 1.  Stages past the
-    // end load the last one again into a buffer nobody reads.
-#pragma unroll
-    for (int s = 0; s + 1 < NSTAGE; ++s) dma_stage(s < nk ? s : nk - 1, s);
-    int buf = 0, nbuf = NSTAGE - 1;
-    for (int kt = 0; kt < nk; ++kt) {
-      wait_vm<C::DMA_MIN * (NSTAGE - 2)>();
-      __syncthreads();
-      const int ks = kt + NSTAGE - 1;
-      dma_stage(ks < nk ? ks : nk - 1, nbuf);
-      compute(buf, kt);
-      buf = buf + 1 == NSTAGE ? 0 : buf + 1;
-      nbuf = nbuf + 1 == NSTAGE ? 0 : nbuf + 1;
-    }
-    wait_vm<0>();
-  }
-
-  // ---- epilogue: 16 consecutive outputs of one row a lane -------------------------
-  constexpr int OTW = SWIGLU ? WT / 2 : WT;
   const bool inside = n0 + BNO <= p.N;  // of the whole workgroup: no column past N
   const bool whole = OT != O_MX4 && n0 + BNO <= p.ldy && p.ldy % 8 == 0;
 #pragma unroll
@@ -812,11 +633,156 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) mx4_gemm_kernel(Mx4Args p) {
           *(uint2*)((uint8_t*)p.y + b * 16 + g * 8) = make_uint2(lo, hi);
           if (g == 0) p.ys[(nb0 / MX4_GROUP * p.yrows + row) * 4 + nb0 % MX4_GROUP / MX4_BLOCK] = (uint8_t)byte;
         }
-      } else if (live) {
-        mx4_store16<OT == O_BF16>(p.y, row, p.ldy, n, whole, v);
+      } else {
+        if constexpr (OT == O_BF16) {
+          if (whole) {
+            const int m = l32 / 2 & 3;  // 8 lanes' pieces are in different banks, here and below
+            *(uint4*)(own + l32 * 64 + (2 * g ^ m) * 16) =
+                make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+            *(uint4*)(own + l32 * 64 + ((2 * g + 1) ^ m) * 16) = make_uint4(
+                pack_bf16(v[8], v[9]), pack_bf16(v[10], v[11]), pack_bf16(v[12], v[13]), pack_bf16(v[14], v[15]));
+            __builtin_amdgcn_wave_barrier();  // a wave's LDS accesses are done in order
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int r = h * 16 + lane / 4, c = lane % 4, tr = wm * (BM / WM) + i * 32 + r;
+              const uint4 d = *(const uint4*)(own + r * 64 + (c ^ (r / 2 & 3)) * 16);
+              uint16_t* y = (uint16_t*)p.y + (row0 + tr) * p.ldy + nb0 + c * 8;
+              if (tr < rows) *(uint4*)y = d;
+            }
+            __builtin_amdgcn_wave_barrier();
+            continue;
+          }
+        }
+        if (live) mx4_store16<OT == O_BF16>(p.y, row, p.ldy, n, whole, v);
       }
     }
   }
+}
+
+// Activations as they are (A_BF16, A_F32): the weight is decoded.  A lane's 16 bytes of
+// codes are its block g of a 64-wide step, times their scale (exact in bf16), and MFMA
+// q multiplies values 32 g + 8 q and on; fp32 activations are three bf16 terms, split
+// after the LDS read.  W_BF16: the weight's rows are bf16 already.
+template <int AT, int WF, int OT, bool SWIGLU, int BM, int BN, int WM, int WN, int KS, int NSTAGE>
+__global__ void __launch_bounds__(WM * WN * 64, 2) mx4_gemm_kernel(Mx4Args p) {
+  using C = Mx4Cfg<AT, WF, BM, BN, WM, WN, KS, NSTAGE>;
+  static_assert(AT != A_MX4 && OT != O_MX4, "mx4_codes_kernel's");
+  constexpr int TT = C::TT, WT = C::WT, BNO = SWIGLU ? BN / 2 : BN, XROW = C::XROW, WROW = C::WROW;
+  __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+
+  // a contiguous band of tiles for each XCD (workgroup b runs on XCD b % 8)
+  int mt, nt;
+  {
+    constexpr int NXCD = 8;
+    const int n_tiles = (int)((mx4_cols<OT>(p) + BNO - 1) / BNO), total = gridDim.x;
+    int lin = blockIdx.x;
+    const int full = total / NXCD * NXCD;
+    if (lin < full) lin = lin % NXCD * (full / NXCD) + lin / NXCD;
+    mx4_tile_at(lin, total / n_tiles, n_tiles, mt, nt);
+  }
+  int e, rows;
+  int64_t row0;
+  if (!mx4_tile<BM>(p, mt, lane, e, row0, rows)) return;
+  const int64_t n0 = (int64_t)nt * BNO;
+  Mx4Source<C, WF, SWIGLU> src;
+  mx4_source(p, e, row0, n0, lane, wave, [&](int r) -> int64_t {
+    const int lr = min(r, rows - 1);
+    return p.row_idx ? (int64_t)p.row_idx[row0 + lr] : lr;
+  }, src);
+  const uint32_t lds0 = lds_offset(&smem[0]);
+  auto dma_stage = [&](int kt, int buf) { mx4_dma(p, src, wave, kt, lds0 + (uint32_t)(buf * C::STAGE)); };
+
+  const int g = lane >> 5, l32 = lane & 31;
+  // staged row of weight tile j of this wave: with SwiGLU its gate tiles, then its up tiles
+  auto w_tile = [&](int j) -> int {
+    if constexpr (SWIGLU)
+      return j < WT / 2 ? wn * (BN / WN / 2) + j * 32 : BN / 2 + wn * (BN / WN / 2) + (j - WT / 2) * 32;
+    else return wn * (BN / WN) + j * 32;
+  };
+  f32x16_t acc[WT][TT];
+#pragma unroll
+  for (int j = 0; j < WT; ++j)
+#pragma unroll
+    for (int i = 0; i < TT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[j][i][r] = 0.0f;
+
+  const int nk = (int)(p.K / KS);
+  auto compute = [&](int buf, int kt) {
+    const char* xs_ = smem + buf * C::STAGE;
+    const char* ws_ = xs_ + C::XB;
+    const char* ss_ = ws_ + C::WB;
+#pragma unroll
+    for (int h = 0; h < KS / 64; ++h) {
+      const int sh = 8 * g + 16 * (KS < 128 ? kt & 1 : h & 1);
+      uint4 wc[WT];  // codes of block g of each weight row, and its scale
+      float sc[WT];
+#pragma unroll
+      for (int j = 0; j < WT && WF == W_MX4; ++j) {
+        const int r = w_tile(j) + l32;
+        wc[j] = *(const uint4*)(ws_ + r * WROW + mx4_swz<WROW>(r, h * 2 + g) * 16);
+        sc[j] = mx4_scale((*(const uint32_t*)(ss_ + (h / 2 * C::SROWS + r) * 4) >> sh) & 255u);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        constexpr int NT = AT == A_F32 ? 3 : 1;
+        bf16x8_t xf[TT][NT];
+#pragma unroll
+        for (int i = 0; i < TT; ++i) {
+          const int r = wm * (BM / WM) + i * 32 + l32;
+          if constexpr (AT == A_BF16) {
+            xf[i][0] = *(const bf16x8_t*)(xs_ + r * XROW + mx4_swz<XROW>(r, h * 8 + g * 4 + q) * 16);
+          } else {
+            const float4 a = *(const float4*)(xs_ + r * XROW + mx4_swz<XROW>(r, h * 16 + g * 8 + q * 2) * 16);
+            const float4 b = *(const float4*)(xs_ + r * XROW + mx4_swz<XROW>(r, h * 16 + g * 8 + q * 2 + 1) * 16);
+            const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            bf16x8_t t[3];
+            mx4_split3(v, t);
+#pragma unroll
+            for (int k = 0; k < NT; ++k) xf[i][k] = t[k];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < WT; ++j) {
+          bf16x8_t wf;
+          if constexpr (WF == W_BF16) {
+            const int r = w_tile(j) + l32;
+            wf = *(const bf16x8_t*)(ws_ + r * WROW + mx4_swz<WROW>(r, h * 8 + g * 4 + q) * 16);
+          } else {
+            const uint32_t c = q == 0 ? wc[j].x : q == 1 ? wc[j].y : q == 2 ? wc[j].z : wc[j].w;
+            wf = __builtin_bit_cast(bf16x8_t, mx4_decode8(c, sc[j]));
+          }
+#pragma unroll
+          for (int i = 0; i < TT; ++i)
+#pragma unroll
+            for (int k = 0; k < NT; ++k)
+              acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf, xf[i][k], acc[j][i], 0, 0, 0);
+        }
+      }
+    }
+  };
+  // Stage kt is complete when at most the loads of the later stages are outstanding;
+  // the barrier publishes it and frees the buffer of stage kt - 1.  Stages past the
+  // end load the last one again into a buffer nobody reads.
+#pragma unroll
+  for (int s = 0; s + 1 < NSTAGE; ++s) dma_stage(s < nk ? s : nk - 1, s);
+  int buf = 0, nbuf = NSTAGE - 1;
+  for (int kt = 0; kt < nk; ++kt) {
+    wait_vm<C::DMA_MIN * (NSTAGE - 2)>();
+    __syncthreads();
+    const int ks = kt + NSTAGE - 1;
+    dma_stage(ks < nk ? ks : nk - 1, nbuf);
+    compute(buf, kt);
+    buf = buf + 1 == NSTAGE ? 0 : buf + 1;
+    nbuf = nbuf + 1 == NSTAGE ? 0 : nbuf + 1;
+  }
+  wait_vm<0>();
+
+  if constexpr (OT == O_BF16) __syncthreads();  // the stages' LDS is the waves' now
+  mx4_epilogue<OT, SWIGLU, BM, BN, WM, WN>(p, acc, row0, rows, n0, wm, wn, lane, smem + wave * 2048);
 }
 
 template <int AT, int WF, int OT, bool SWIGLU, int BM, int BN, int WM, int WN, int KS, int NSTAGE>
@@ -827,6 +793,204 @@ int launch_gemm_cfg(const Mx4Args& p, int64_t m_tiles, hipStream_t stream) {
   hipLaunchKernelGGL((mx4_gemm_kernel<AT, WF, OT, SWIGLU, BM, BN, WM, WN, KS, NSTAGE>),
                      dim3((unsigned)(m_tiles * n_tiles)), dim3(WM * WN * 64), 0, stream, p);
   return check_launch("mx4_gemm_kernel");
+}
+
+// Activations in the format: v_mfma_scale_f32_32x32x64_f8f6f4 on the codes as they are,
+// lane i + 32 g with block g of a 64-wide step of its row and one scale byte for the 32
+// values.
+//
+// Stages are 256 wide, 128-byte rows: what costs the loop is L2 requests, and half a line
+// is one too.  The operands of a step are read from LDS while the step before is
+// multiplied, the first of a stage during the last of the stage before; by then every
+// wave has the rest of its stage in registers, so that one barrier frees the buffer for
+// the loads of the stage after the next.
+//
+// One workgroup a CU walks a band of tiles as one sequence of stages: the loads of the
+// next tile's first stages leave during the last of this one and its operands are in
+// registers before the epilogue, which they hide behind.  K of 1024 is four stages: a
+// tile's start, its row indices and first loads, took a quarter of its time (16384 tokens
+// to 2 of 8 experts, 1024 by 2560: 274 us with a workgroup a tile, 248 so).
+template <int OT, bool SWIGLU, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(WM * WN * 64, 2) mx4_codes_kernel(Mx4Args p, int m_tiles) {
+  constexpr int KS = 256, NSTAGE = 2, STEPS = KS / 64;
+  using C = Mx4Cfg<A_MX4, W_MX4, BM, BN, WM, WN, KS, NSTAGE>;
+  constexpr int TT = C::TT, WT = C::WT, BNO = SWIGLU ? BN / 2 : BN, XROW = C::XROW, WROW = C::WROW;
+  constexpr int OWN = OT == O_BF16 ? 2048 : 0;  // bytes that a wave's rows leave through
+  __shared__ __attribute__((aligned(1024))) char smem[C::LDS + WM * WN * OWN];
+  __shared__ int index[2][BM];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN, g = lane >> 5, l32 = lane & 31;
+  const uint32_t lds0 = lds_offset(&smem[0]);
+  const int n_tiles = (int)((mx4_cols<OT>(p) + BNO - 1) / BNO);
+
+  // every expert's tiles and segment, a lane an expert
+  int to0 = 0, to1 = 0x7fffffff, so0 = 0, so1 = 0;
+  if (p.seg_off) {
+    if (lane < p.E) {
+      to0 = p.tile_off[lane];
+      to1 = p.tile_off[lane + 1];
+      so0 = p.seg_off[lane];
+      so1 = p.seg_off[lane + 1];
+    }
+    m_tiles = __builtin_amdgcn_readlane(to1, p.E - 1);  // of the bound that the host knows
+  }
+  // XCD x (workgroup b runs on XCD b % 8) takes a contiguous band of the tiles
+  const int wgs = gridDim.x, nx = min(8, wgs), xcd = (int)blockIdx.x % nx, step = (wgs - xcd + nx - 1) / nx;
+  const int total = m_tiles * n_tiles, last = (int)((int64_t)total * (xcd + 1) / nx);
+  int lin = (int)((int64_t)total * xcd / nx) + (int)blockIdx.x / nx;
+  if (lin >= last) return;
+
+  auto place = [&](int at, int& e, int64_t& row0, int& rows, int64_t& n0) {
+    int mt, nt;
+    mx4_tile_at(at, m_tiles, n_tiles, mt, nt);
+    n0 = (int64_t)nt * BNO;
+    if (!p.seg_off) {
+      e = 0;
+      row0 = (int64_t)mt * BM;
+      rows = (int)min<int64_t>(BM, p.R - row0);
+      return;
+    }
+    e = (int)__popcll(__ballot(to1 <= mt));
+    const int r0 = __builtin_amdgcn_readlane(so0, e) + (mt - __builtin_amdgcn_readlane(to0, e)) * BM;
+    row0 = r0;
+    rows = min(BM, __builtin_amdgcn_readlane(so1, e) - r0);
+  };
+  // x rows of tile `at` to LDS (from the tile's first where they are not gathered): two
+  // buffers, one being filled while the other may still be read
+  auto gather = [&](int at, int buf) {
+    int e, rows;
+    int64_t row0, n0;
+    place(at, e, row0, rows, n0);
+    const int r = wave * 64 + lane, lr = min(r, rows - 1);
+    if (wave >= BM / 64) return;
+    if (p.row_idx) dma4(p.row_idx + row0, (uint32_t)lr * 4, lds_offset(&index[buf][wave * 64]));
+    else index[buf][r] = lr;
+  };
+  Mx4Source<C, W_MX4, SWIGLU> src;
+  auto source = [&](int at, int buf) {
+    int e, rows;
+    int64_t row0, n0;
+    place(at, e, row0, rows, n0);
+    mx4_source(p, e, row0, n0, lane, wave, [&](int r) -> int64_t { return index[buf][r]; }, src);
+  };
+  // the loads of the sequence's next stage, of this tile or the one after
+  const int nk = (int)(p.K / KS);
+  int load_at = lin, load_k = nk, turn = 0;
+  auto load = [&](int buf) {
+    if (load_k == nk) {
+      if (load_at >= last) return;
+      source(load_at, turn);
+      turn ^= 1;
+      load_at += step;
+      load_k = 0;
+      if (load_at < last) gather(load_at, turn);  // there at the next stage's barrier
+    }
+    mx4_dma(p, src, wave, load_k, lds0 + (uint32_t)(buf * C::STAGE));
+    ++load_k;
+  };
+  gather(lin, 0);
+  wait_vm<0>();
+  __syncthreads();
+  load(0);
+  wait_vm<0>();
+  __syncthreads();
+  load(1);
+
+  // staged row of weight tile j of this wave: with SwiGLU its gate tiles, then its up tiles
+  auto w_tile = [&](int j) -> int {
+    if constexpr (SWIGLU)
+      return j < WT / 2 ? wn * (BN / WN / 2) + j * 32 : BN / 2 + wn * (BN / WN / 2) + (j - WT / 2) * 32;
+    else return wn * (BN / WN) + j * 32;
+  };
+  i32x8_t wf[2][WT], xf[2][TT];
+  uint32_t sw[2][WT], sx[2][TT];
+  const char* w_at[WT];  // fixed parts of the addresses
+  const char* x_at[TT];
+#pragma unroll
+  for (int j = 0; j < WT; ++j) w_at[j] = smem + C::XB + (w_tile(j) + l32) * WROW;
+#pragma unroll
+  for (int i = 0; i < TT; ++i) x_at[i] = smem + (wm * (BM / WM) + i * 32 + l32) * XROW;
+  const char* s_at = smem + C::XB + C::WB + l32 * 4;
+  auto read = [&](int buf, int u) {
+    const int o = buf * C::STAGE, c = u * 2 + g, to = u & 1;
+    if (u % 2 == 0) {  // the scales of a group of 128
+#pragma unroll
+      for (int j = 0; j < WT; ++j) sw[u / 2][j] = *(const uint32_t*)(s_at + o + (u / 2 * C::SROWS + w_tile(j)) * 4);
+#pragma unroll
+      for (int i = 0; i < TT; ++i)
+        sx[u / 2][i] = *(const uint32_t*)(s_at + o + (u / 2 * C::SROWS + BN + wm * (BM / WM) + i * 32) * 4);
+    }
+    // tiles are 32 rows apart, which the swizzles do not see
+#pragma unroll
+    for (int i = 0; i < TT; ++i) xf[to][i] = mx4_operand(*(const uint4*)(x_at[i] + o + mx4_swz<XROW>(l32, c) * 16));
+#pragma unroll
+    for (int j = 0; j < WT; ++j) wf[to][j] = mx4_operand(*(const uint4*)(w_at[j] + o + mx4_swz<WROW>(l32, c) * 16));
+  };
+  f32x16_t acc[WT][TT];
+  auto multiply = [&](int u) {
+    if (u % 2 == 0) {  // this lane's blocks, g and g + 2 of the four, to bytes 0 and 2
+#pragma unroll
+      for (int j = 0; j < WT; ++j) sw[u / 2][j] >>= 8 * g;
+#pragma unroll
+      for (int i = 0; i < TT; ++i) sx[u / 2][i] >>= 8 * g;
+    }
+#pragma unroll
+    for (int j = 0; j < WT; ++j)
+#pragma unroll
+      for (int i = 0; i < TT; ++i)
+        acc[j][i] = u % 2 == 0
+            ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[0][j], xf[0][i], acc[j][i], 4, 4, 0,
+                                                              (int)sw[u / 2][j], 0, (int)sx[u / 2][i])
+            : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[1][j], xf[1][i], acc[j][i], 4, 4, 2,
+                                                              (int)sw[u / 2][j], 2, (int)sx[u / 2][i]);
+  };
+
+  read(0, 0);
+  int buf = 0;
+  for (; lin < last; lin += step) {
+#pragma unroll
+    for (int j = 0; j < WT; ++j)
+#pragma unroll
+      for (int i = 0; i < TT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[j][i][r] = 0.0f;
+    for (int kt = 0; kt < nk; ++kt, buf ^= 1) {
+#pragma unroll
+      for (int u = 0; u < STEPS; ++u) {
+        if (u + 1 < STEPS) {
+          read(buf, u + 1);
+        } else {
+#pragma unroll
+          for (int j = 0; j < WT; ++j)  // the products so far stay before the branch
+#pragma unroll
+            for (int i = 0; i < TT; ++i) asm volatile("" : "+v"(acc[j][i]));
+          wait_vm<0>();
+          __syncthreads();
+          load(buf);
+          read(buf ^ 1, 0);  // behind the last tile: values that nothing uses
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(u);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    int e, rows;
+    int64_t row0, n0;
+    place(lin, e, row0, rows, n0);
+    mx4_epilogue<OT, SWIGLU, BM, BN, WM, WN>(p, acc, row0, rows, n0, wm, wn, lane, smem + C::LDS + wave * OWN);
+  }
+}
+
+template <int OT, bool SWIGLU, int BM, int BN, int WM, int WN>
+int launch_codes(const Mx4Args& p, int64_t m_tiles, hipStream_t stream) {
+  constexpr int BNO = SWIGLU ? BN / 2 : BN;
+  const int64_t tiles = m_tiles * ((mx4_cols<OT>(p) + BNO - 1) / BNO);
+  if (tiles > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: too many tiles");
+  const int64_t cus = cu_count();
+  hipLaunchKernelGGL((mx4_codes_kernel<OT, SWIGLU, BM, BN, WM, WN>), dim3((unsigned)(tiles < cus ? tiles : cus)),
+                     dim3(WM * WN * 64), 0, stream, p, (int)m_tiles);
+  return check_launch("mx4_codes_kernel");
 }
 
 // The kernel of few rows (up to 64): a workgroup has 32 columns of one expert, its NW
@@ -1175,7 +1339,7 @@ int launch_product(const Mx4Args& p, const Mx4Slots* few, int64_t m_tiles, hipSt
   if (few) return launch_stream<AT, OT, SWIGLU>(p, *few, stream);
   if constexpr (AT == A_F32) return launch_gemm_cfg<AT, W_MX4, OT, SWIGLU, 64, 256, 2, 2, 64, 3>(p, m_tiles, stream);
   else if constexpr (AT == A_BF16) return launch_gemm_cfg<AT, W_MX4, OT, SWIGLU, 128, 256, 2, 2, 64, 3>(p, m_tiles, stream);
-  else return launch_gemm_cfg<AT, W_MX4, OT, SWIGLU, 256, 256, 4, 2, 256, 2>(p, m_tiles, stream);
+  else return launch_codes<OT, SWIGLU, 256, 256, 4, 2>(p, m_tiles, stream);
 }
 
 // activations with a weight: y of `out` type
