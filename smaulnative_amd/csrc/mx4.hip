@@ -219,7 +219,35 @@ struct Mx4Weight {
   int64_t N, K;    // rows of an expert
   int64_t blocks;  // workgroups that the matrix takes
 };
-enum { P_NONE = 0, P_ROUND = 1, P_PAD = 2 };  // activations: as they are, rounded, or copied to padded rows
+// activations: as they are, rounded, or copied to padded rows (fp32: of planes)
+enum { P_NONE = 0, P_ROUND = 1, P_PAD = 2 };
+// v = a + b + c, each the next 8 significant bits: exact in bf16, and all 24 of fp32.
+// An infinity or NaN is a alone.
+__device__ __forceinline__ void mx4_split3(const float* v, uint4 (&t)[3]) {
+  uint32_t h[3][8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float a = __builtin_canonicalizef(v[j]);  // a NaN that keeps its highest bit
+    h[0][j] = __float_as_uint(a) & 0xffff0000u;
+    float r = a - __uint_as_float(h[0][j]);
+    r = r == r ? r : 0.0f;
+    h[1][j] = __float_as_uint(r) & 0xffff0000u;
+    h[2][j] = __float_as_uint(r - __uint_as_float(h[1][j]));
+  }
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    uint32_t u[4];  // the high halves of pairs
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u[j] = __builtin_amdgcn_perm(h[q][2 * j + 1], h[q][2 * j], 0x07060302u);
+    t[q] = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+}
+
+// fp32 rows as the larger products read them: three planes of bf16, 64 values of each in
+// turn, [width / 64][3][64].  Split once here: split after the LDS read, each wave of a
+// tile's columns did it again, 44 instructions beside three products.
+__host__ __device__ __forceinline__ int64_t mx4_plane_at(int64_t c) { return c / 64 * 192 + c % 64; }
+
 struct Mx4Prep {
   Mx4Weight m[3];
   const void* x;
@@ -230,51 +258,56 @@ struct Mx4Prep {
   int xmode, xvec;
 };
 
-// a workgroup: 16 rows by 4 groups, 16 lanes a row
+// a workgroup: 16 rows of one group, 16 lanes a row (16384 x 1024: 10.4 us, 11.7 of four groups)
 template <bool BF16>
 __device__ __forceinline__ void mx4_prep_rows(const Mx4Prep& p, int64_t block) {
-  const int64_t ng = mx4_groups(p.K), cb = (ng + 3) / 4;
-  const int64_t row = block / cb * 16 + (threadIdx.x >> 4), g0 = block % cb * 4;
+  const int64_t ng = mx4_groups(p.K);
+  const uint32_t rb = (uint32_t)block / (uint32_t)ng;  // both from one 32-bit grid
+  const int64_t row = (int64_t)rb * 16 + (threadIdx.x >> 4), g = block - (int64_t)rb * ng;
   const int c = threadIdx.x & 15;
   if (row >= p.T) return;  // whole quads
-  float v[4][8];
+  float v[8];
+  const int64_t c0 = g * MX4_GROUP + c * 8;
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int64_t c0 = (g0 + u) * MX4_GROUP + c * 8;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[u][j] = 0.0f;
-    if (c0 < p.K) {
-      if (p.xvec && c0 + 8 <= p.K) mx4_load8<BF16, true>(p.x, row, p.K, c0, v[u]);
-      else mx4_load8<BF16, false>(p.x, row, p.K, c0, v[u]);
-    }
+  for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+  if (c0 < p.K) {
+    if (p.xvec && c0 + 8 <= p.K) mx4_load8<BF16, true>(p.x, row, p.K, c0, v);
+    else mx4_load8<BF16, false>(p.x, row, p.K, c0, v);
   }
+  const int64_t at = (row * ng + g) * 16 + c;  // groups of 8 values
+  if (p.xmode == P_ROUND) {
+    uint32_t byte = mx4_scale_byte(mx4_quad_max(mx4_amax8(v)));
+    ((uint32_t*)p.xo)[at] = mx4_encode8(v, byte);
+    byte <<= 8 * (c >> 2);  // the group's four blocks to one dword
+    byte |= (uint32_t)__shfl_xor((int)byte, 4, 16);
+    byte |= (uint32_t)__shfl_xor((int)byte, 8, 16);
+    if (c == 0) p.xst[g * p.T + row] = byte;
+  } else if constexpr (BF16) {
+    ((uint4*)p.xo)[at] = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]),
+                                    pack_bf16(v[6], v[7]));
+  } else {
+    uint4 t[3];
+    mx4_split3(v, t);
+    uint16_t* o = (uint16_t*)p.xo + row * ng * (3 * MX4_GROUP) + mx4_plane_at(c0);
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    if (g0 + u >= ng) break;
-    const int64_t at = row * ng * 16 + (g0 + u) * 16 + c;  // groups of 8 values
-    if (p.xmode == P_ROUND) {
-      uint32_t byte = mx4_scale_byte(mx4_quad_max(mx4_amax8(v[u])));
-      ((uint32_t*)p.xo)[at] = mx4_encode8(v[u], byte);
-      byte <<= 8 * (c >> 2);  // the group's four blocks to one dword
-      byte |= (uint32_t)__shfl_xor((int)byte, 4, 16);
-      byte |= (uint32_t)__shfl_xor((int)byte, 8, 16);
-      if (c == 0) p.xst[(g0 + u) * p.T + row] = byte;
-    } else if constexpr (BF16) {
-      ((uint4*)p.xo)[at] = make_uint4(pack_bf16(v[u][0], v[u][1]), pack_bf16(v[u][2], v[u][3]),
-                                      pack_bf16(v[u][4], v[u][5]), pack_bf16(v[u][6], v[u][7]));
-    } else {
-      ((float4*)p.xo)[at * 2] = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
-      ((float4*)p.xo)[at * 2 + 1] = make_float4(v[u][4], v[u][5], v[u][6], v[u][7]);
-    }
+    for (int k = 0; k < 3; ++k) *(uint4*)(o + 64 * k) = t[k];
   }
 }
 
 // a thread: the four blocks of one group of one row, rows fastest
 __device__ __forceinline__ void mx4_prep_weight(const Mx4Weight& m, int64_t E, int64_t block) {
   const int64_t ng = mx4_groups(m.K), nb = mx4_blocks(m.K);
-  const int64_t i = block * 256 + threadIdx.x;
-  if (i >= E * ng * m.N) return;
-  const int64_t q = i / m.N, n = i - q * m.N, e = q / ng, g = q - e * ng, row = e * m.N + n;
+  const int64_t i = block * 256 + threadIdx.x, all = E * ng * m.N;
+  if (i >= all) return;
+  int64_t q, e;
+  if (all < 1LL << 32) {  // 64-bit divisions take as long as the loads
+    q = (uint32_t)i / (uint32_t)m.N;
+    e = (uint32_t)q / (uint32_t)ng;
+  } else {
+    q = i / m.N;
+    e = q / ng;
+  }
+  const int64_t n = i - q * m.N, g = q - e * ng, row = e * m.N + n;
   const uint8_t* s = m.s + row * nb + g * 4;
   uint32_t d = 0;
   if (g * 4 + 4 <= nb && nb % 4 == 0 && ((uintptr_t)m.s & 3) == 0) {
@@ -311,14 +344,22 @@ __global__ void __launch_bounds__(256) mx4_prep_kernel(Mx4Prep p, int64_t E) {
 }
 
 // The weight turned round, for the input gradient: wt[i][o] = W[o][i] in bf16, rows of
-// ldo values (zeros from O on).  A workgroup: 64 o by 64 i, through LDS.
+// ldo values (zeros from O on).  A workgroup: 64 o by 64 i, through LDS.  The first
+// workgroups lay out the gradient's rows where that has to be.
+template <bool BF16>
 __global__ void __launch_bounds__(256)
-mx4_turn_kernel(const uint8_t* __restrict__ w, const uint8_t* __restrict__ s, uint16_t* __restrict__ wt, int64_t O,
-                int64_t I, int64_t ldo) {
+mx4_turn_kernel(Mx4Prep p, const uint8_t* __restrict__ w, const uint8_t* __restrict__ s, uint16_t* __restrict__ wt,
+                int64_t O, int64_t I, int64_t ldo) {
+  if (blockIdx.x < p.xblocks) {
+    mx4_prep_rows<BF16>(p, blockIdx.x);
+    return;
+  }
+  const uint32_t block = blockIdx.x - (uint32_t)p.xblocks;
   constexpr int LD = 72;  // 16-byte rows of 64 o, off the banks' period
   __shared__ __attribute__((aligned(16))) uint16_t sh[64 * LD];
-  const int64_t nb = mx4_blocks(I), ti = (I + 63) / 64;
-  const int64_t i0 = blockIdx.x % ti * 64, o0 = blockIdx.x / ti * 64;
+  const int64_t nb = mx4_blocks(I);
+  const uint32_t ti = (uint32_t)((I + 63) / 64), ot = block / ti;
+  const int64_t i0 = (int64_t)(block - ot * ti) * 64, o0 = (int64_t)ot * 64;
   {
     const int o = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
     const int64_t b = (i0 + c) / MX4_BLOCK;
@@ -349,7 +390,7 @@ enum { A_BF16 = 0, A_F32 = 1, A_MX4 = 2 };
 // The weight: codes and scales, or (mx4_gemm_kernel) rows already decoded to bf16.
 enum { W_MX4 = 0, W_BF16 = 1 };
 // What a tile's sums become: rounded to bf16, fp32, or blocks of the format.
-enum { O_BF16 = 0, O_F32 = 1, O_MX4 = 2 };
+enum { O_BF16 = 0, O_F32 = 1, O_MX4 = 2, O_PLANES = 3 };
 
 struct Mx4Args {
   const void* x;           // rows of K values (A_MX4: codes, 16 bytes a block)
@@ -362,8 +403,9 @@ struct Mx4Args {
   void* y;                 // [rows][N] (O_MX4: codes)
   uint8_t* ys;             // O_MX4: scales
   int64_t R, K, N;
-  // mx4_gemm_kernel: scales are [group][row] dwords (w's of each expert, xs and ys over
-  // xrows and yrows rows); row strides of x and y in values (codes: blocks), of W in blocks
+  // the larger products: scales are [group][row] dwords (w's of each expert, xs and ys over
+  // xrows and yrows rows); row strides of x and y in values (planes: of all three;
+  // codes: blocks), of W in blocks
   int64_t ldx, ldw, ldy, xrows, yrows;
   const int32_t* seg_off;  // null: dense, R rows of one expert
   const int32_t* tile_off;
@@ -397,25 +439,6 @@ __device__ __forceinline__ float mx4_swiglu(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-g * 1.4426950408889634f)) * u;
 }
 
-// v = a + b + c, each the next 8 significant bits: exact in bf16, and all 24 of fp32
-__device__ __forceinline__ void mx4_split3(const float (&v)[8], bf16x8_t (&t)[3]) {
-  uint32_t h[3][8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    h[0][j] = __float_as_uint(v[j]) & 0xffff0000u;
-    const float r = v[j] - __uint_as_float(h[0][j]);
-    h[1][j] = __float_as_uint(r) & 0xffff0000u;
-    h[2][j] = __float_as_uint(r - __uint_as_float(h[1][j]));
-  }
-#pragma unroll
-  for (int q = 0; q < 3; ++q) {
-    uint32_t u[4];  // the high halves of pairs
-#pragma unroll
-    for (int j = 0; j < 4; ++j) u[j] = __builtin_amdgcn_perm(h[q][2 * j + 1], h[q][2 * j], 0x07060302u);
-    t[q] = __builtin_bit_cast(bf16x8_t, make_uint4(u[0], u[1], u[2], u[3]));
-  }
-}
-
 constexpr int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 bool aligned(const void* p, int to) { return ((uintptr_t)p & (to - 1)) == 0; }
 bool dtype_ok(int d) { return d == SMAUL_DTYPE_F32 || d == SMAUL_DTYPE_BF16; }
@@ -432,9 +455,10 @@ bool dtype_ok(int d) { return d == SMAUL_DTYPE_F32 || d == SMAUL_DTYPE_BF16; }
 template <int AT, int WF, int BM, int BN, int WM, int WN, int KS, int NSTAGE>
 struct Mx4Cfg {
   static constexpr int NW = WM * WN;
-  static constexpr int XROW = AT == A_MX4 ? KS / 2 : AT == A_BF16 ? KS * 2 : KS * 4;
+  static constexpr int XP = AT == A_F32 ? 3 : 1;  // planes of x, each BM rows of XROW bytes
+  static constexpr int XROW = AT == A_MX4 ? KS / 2 : KS * 2;
   static constexpr int WROW = WF == W_BF16 ? KS * 2 : KS / 2;
-  static constexpr int XB = BM * XROW, WB = BN * WROW;
+  static constexpr int XB = XP * BM * XROW, WB = BN * WROW;
   static constexpr int SROWS = WF == W_BF16 ? 0 : BN + (AT == A_MX4 ? BM : 0);  // of scales
   static constexpr int SG = KS < 128 ? 1 : KS / 128;                            // dwords of each
   static constexpr int STAGE = XB + WB + SROWS * SG * 4;
@@ -444,9 +468,10 @@ struct Mx4Cfg {
   static constexpr int SI = (S_INS + NW - 1) / NW < 1 ? 1 : (S_INS + NW - 1) / NW, SP = SROWS < 64 ? 1 : SROWS / 64;
   static constexpr int SD = NW % SP == 0 ? 1 : SI;  // different rows of a wave's scale instructions
   static constexpr int TT = BM / WM / 32, WT = BN / WN / 32;  // 32 x 32 tiles of a wave
-  static constexpr int COLS = BN, KW = KS;
+  static constexpr int ROWS = BM, COLS = BN, KW = KS;
   static constexpr int LDS = NSTAGE * STAGE;
-  static constexpr int XS = AT == A_MX4 ? 16 : AT == A_BF16 ? 2 : 4;  // bytes of a unit of ldx
+  static constexpr int XS = AT == A_MX4 ? 16 : 2;  // bytes of a unit of ldx
+  static_assert(AT != A_F32 || KS == 64, "planes take turns every 64 values");
   static_assert(XB % (1024 * NW) == 0 && WB % (1024 * NW) == 0 && SROWS % 64 == 0, "whole DMA instructions");
   static_assert(DMA_MIN * (NSTAGE - 2) < 64 && LDS <= 160 * 1024, "pipeline depth");
 };
@@ -466,7 +491,7 @@ __device__ __forceinline__ int mx4_swz(int r, int c) {
 // columns that a product writes: past N zeros, up to the padded row
 template <int OT>
 __host__ __device__ __forceinline__ int64_t mx4_cols(const Mx4Args& p) {
-  const int64_t c = OT == O_MX4 ? p.ldy * MX4_BLOCK : p.ldy;
+  const int64_t c = OT == O_MX4 ? p.ldy * MX4_BLOCK : OT == O_PLANES ? p.ldy / 3 : p.ldy;
   return c > p.N ? c : p.N;
 }
 
@@ -503,8 +528,9 @@ __device__ __forceinline__ void mx4_source(const Mx4Args& p, int e, int64_t row0
   q.X = (const char*)p.x + (p.row_idx ? 0 : row0 * p.ldx * C::XS);
 #pragma unroll
   for (int a = 0; a < C::X_INS; ++a) {
-    const int r = (wave * C::X_INS + a) * XR + lane / XL;
-    q.x_off[a] = (uint32_t)(row_of(r) * p.ldx * C::XS + mx4_swz<C::XROW>(r, lane % XL) * 16);
+    const int i = (wave * C::X_INS + a) * XR + lane / XL, r = i % C::ROWS;
+    q.x_off[a] =
+        (uint32_t)(row_of(r) * p.ldx * C::XS + i / C::ROWS * C::XROW + mx4_swz<C::XROW>(r, lane % XL) * 16);
   }
   // staged weight row r, from the first: tiles of 32 (gate's, then up's), permuted
   const int64_t left = p.N - 1 - nw;
@@ -542,7 +568,7 @@ __device__ __forceinline__ void mx4_dma(const Mx4Args& p, const Mx4Source<C, WF,
       dma4(src, q.s_off[i % C::SD], l + C::XB + C::WB + j * 256);
     }
   }
-  const char* xk = q.X + (int64_t)kt * C::XROW;
+  const char* xk = q.X + (int64_t)kt * (C::XP * C::XROW);
 #pragma unroll
   for (int a = 0; a < C::X_INS; ++a) dma16(xk, q.x_off[a], l + (wave * C::X_INS + a) * 1024);
 #pragma unroll
@@ -603,7 +629,7 @@ __device__ __forceinline__ void mx4_epilogue(const Mx4Args& p, const f32x16_t (&
   constexpr int TT = BM / WM / 32, WT = BN / WN / 32, BNO = SWIGLU ? BN / 2 : BN, OTW = SWIGLU ? WT / 2 : WT;
   const int g = lane >> 5, l32 = lane & 31;
   const bool inside = n0 + BNO <= p.N;  // of the whole workgroup: no column past N
-  const bool whole = OT != O_MX4 && n0 + BNO <= p.ldy && p.ldy % 8 == 0;
+  const bool whole = (OT == O_BF16 || OT == O_F32) && n0 + BNO <= p.ldy && p.ldy % 8 == 0;
 #pragma unroll
   for (int i = 0; i < TT; ++i) {
     const int lr = wm * (BM / WM) + i * 32 + l32;
@@ -633,6 +659,18 @@ __device__ __forceinline__ void mx4_epilogue(const Mx4Args& p, const f32x16_t (&
           *(uint2*)((uint8_t*)p.y + b * 16 + g * 8) = make_uint2(lo, hi);
           if (g == 0) p.ys[(nb0 / MX4_GROUP * p.yrows + row) * 4 + nb0 % MX4_GROUP / MX4_BLOCK] = (uint8_t)byte;
         }
+      } else if constexpr (OT == O_PLANES) {
+        uint4 lo[3], hi[3];
+        mx4_split3(v, lo);
+        mx4_split3(v + 8, hi);
+        uint16_t* y = (uint16_t*)p.y + row * p.ldy + mx4_plane_at(n);
+        if (live && n < mx4_cols<OT>(p)) {
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            ((uint4*)(y + 64 * k))[0] = lo[k];
+            ((uint4*)(y + 64 * k))[1] = hi[k];
+          }
+        }
       } else {
         if constexpr (OT == O_BF16) {
           if (whole) {
@@ -661,8 +699,8 @@ __device__ __forceinline__ void mx4_epilogue(const Mx4Args& p, const f32x16_t (&
 
 // Activations as they are (A_BF16, A_F32): the weight is decoded.  A lane's 16 bytes of
 // codes are its block g of a 64-wide step, times their scale (exact in bf16), and MFMA
-// q multiplies values 32 g + 8 q and on; fp32 activations are three bf16 terms, split
-// after the LDS read.  W_BF16: the weight's rows are bf16 already.
+// q multiplies values 32 g + 8 q and on; fp32 activations are three planes of bf16.
+// W_BF16: the weight's rows are bf16 already.
 template <int AT, int WF, int OT, bool SWIGLU, int BM, int BN, int WM, int WN, int KS, int NSTAGE>
 __global__ void __launch_bounds__(WM * WN * 64, 2) mx4_gemm_kernel(Mx4Args p) {
   using C = Mx4Cfg<AT, WF, BM, BN, WM, WN, KS, NSTAGE>;
@@ -728,22 +766,13 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) mx4_gemm_kernel(Mx4Args p) {
       }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        constexpr int NT = AT == A_F32 ? 3 : 1;
-        bf16x8_t xf[TT][NT];
+        bf16x8_t xf[TT][C::XP];
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
           const int r = wm * (BM / WM) + i * 32 + l32;
-          if constexpr (AT == A_BF16) {
-            xf[i][0] = *(const bf16x8_t*)(xs_ + r * XROW + mx4_swz<XROW>(r, h * 8 + g * 4 + q) * 16);
-          } else {
-            const float4 a = *(const float4*)(xs_ + r * XROW + mx4_swz<XROW>(r, h * 16 + g * 8 + q * 2) * 16);
-            const float4 b = *(const float4*)(xs_ + r * XROW + mx4_swz<XROW>(r, h * 16 + g * 8 + q * 2 + 1) * 16);
-            const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            bf16x8_t t[3];
-            mx4_split3(v, t);
 #pragma unroll
-            for (int k = 0; k < NT; ++k) xf[i][k] = t[k];
-          }
+          for (int k = 0; k < C::XP; ++k)
+            xf[i][k] = *(const bf16x8_t*)(xs_ + (k * BM + r) * XROW + mx4_swz<XROW>(r, h * 8 + g * 4 + q) * 16);
         }
 #pragma unroll
         for (int j = 0; j < WT; ++j) {
@@ -758,7 +787,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) mx4_gemm_kernel(Mx4Args p) {
 #pragma unroll
           for (int i = 0; i < TT; ++i)
 #pragma unroll
-            for (int k = 0; k < NT; ++k)
+            for (int k = 0; k < C::XP; ++k)
               acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf, xf[i][k], acc[j][i], 0, 0, 0);
         }
       }
@@ -787,7 +816,10 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) mx4_gemm_kernel(Mx4Args p) {
 
 template <int AT, int WF, int OT, bool SWIGLU, int BM, int BN, int WM, int WN, int KS, int NSTAGE>
 int launch_gemm_cfg(const Mx4Args& p, int64_t m_tiles, hipStream_t stream) {
+  using C = Mx4Cfg<AT, WF, BM, BN, WM, WN, KS, NSTAGE>;
   constexpr int BNO = SWIGLU ? BN / 2 : BN;
+  if (BM * p.ldx * C::XS >= 1LL << 32 || BN * p.ldw * (WF == W_BF16 ? 2 : 16) >= 1LL << 32)
+    return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: rows too wide");
   const int64_t n_tiles = (mx4_cols<OT>(p) + BNO - 1) / BNO;
   if (m_tiles * n_tiles > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: too many tiles");
   hipLaunchKernelGGL((mx4_gemm_kernel<AT, WF, OT, SWIGLU, BM, BN, WM, WN, KS, NSTAGE>),
@@ -986,6 +1018,8 @@ template <int OT, bool SWIGLU, int BM, int BN, int WM, int WN>
 int launch_codes(const Mx4Args& p, int64_t m_tiles, hipStream_t stream) {
   constexpr int BNO = SWIGLU ? BN / 2 : BN;
   const int64_t tiles = m_tiles * ((mx4_cols<OT>(p) + BNO - 1) / BNO);
+  if ((BM > BN ? BM : BN) * (p.ldx > p.ldw ? p.ldx : p.ldw) * 16 >= 1LL << 32)
+    return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: rows too wide");
   if (tiles > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: too many tiles");
   const int64_t cus = cu_count();
   hipLaunchKernelGGL((mx4_codes_kernel<OT, SWIGLU, BM, BN, WM, WN>), dim3((unsigned)(tiles < cus ? tiles : cus)),
@@ -1129,7 +1163,10 @@ __global__ void __launch_bounds__(NW * 64) mx4_stream_kernel(Mx4Args p, Mx4Slots
               } else {
                 mx4_load8<AT == A_BF16, false>(p.x, xr, p.K, b * MX4_BLOCK + v * 8, f);
               }
-              mx4_split3(f, t);
+              uint4 u[3];
+              mx4_split3(f, u);
+#pragma unroll
+              for (int k = 0; k < 3; ++k) t[k] = __builtin_bit_cast(bf16x8_t, u[k]);
             }
 #pragma unroll
             for (int j = 0; j < SW; ++j) {
@@ -1332,12 +1369,15 @@ int launch_quantize(const void* x, int dtype, uint8_t* codes, uint8_t* scales, i
 }
 
 // up to this many rows (tokens of a layer) mx4_stream_kernel, past them mx4_gemm_kernel
-int64_t gemm_bm(int at) { return at == A_F32 ? 64 : at == A_MX4 ? 256 : 128; }  // its row tiles
+int64_t gemm_bm(int at) { return at == A_F32 ? 32 : at == A_MX4 ? 256 : 128; }  // its row tiles
 
 template <int AT, int OT, bool SWIGLU>
 int launch_product(const Mx4Args& p, const Mx4Slots* few, int64_t m_tiles, hipStream_t stream) {
   if (few) return launch_stream<AT, OT, SWIGLU>(p, *few, stream);
-  if constexpr (AT == A_F32) return launch_gemm_cfg<AT, W_MX4, OT, SWIGLU, 64, 256, 2, 2, 64, 3>(p, m_tiles, stream);
+  // us, fp32, 4096 x 1024 -> 2560 and 3001 x 1000 -> 777: 77 and 47 of 32 x 256, 84 and 50
+  // of 64 x 256, 87 and 47 of 64 x 128, 91 and 42 of 32 x 128
+  if constexpr (AT == A_F32)
+    return launch_gemm_cfg<AT, W_MX4, SWIGLU ? O_PLANES : OT, SWIGLU, 32, 256, 1, 4, 64, 2>(p, m_tiles, stream);
   else if constexpr (AT == A_BF16) return launch_gemm_cfg<AT, W_MX4, OT, SWIGLU, 128, 256, 2, 2, 64, 3>(p, m_tiles, stream);
   else return launch_codes<OT, SWIGLU, 256, 256, 4, 2>(p, m_tiles, stream);
 }
@@ -1353,13 +1393,15 @@ int launch_linear(const Mx4Args& p, int at, int out, const Mx4Slots* few, int64_
   return launch_product<A_F32, O_F32, false>(p, few, m_tiles, stream);
 }
 
+void prep_rows(Mx4Prep& p, int dtype) {  // the workgroups of x's rows
+  if (p.xmode == P_NONE) return;
+  p.xblocks = (p.T + 15) / 16 * mx4_groups(p.K);
+  p.xvec = aligned(p.x, 16) && p.K % (dtype == SMAUL_DTYPE_BF16 ? 8 : 4) == 0;
+}
+
 int launch_prep(Mx4Prep p, int dtype, int64_t E, hipStream_t stream) {
-  int64_t blocks = 0;
-  if (p.xmode != P_NONE) {
-    p.xblocks = (p.T + 15) / 16 * ((mx4_groups(p.K) + 3) / 4);
-    p.xvec = aligned(p.x, 16) && p.K % (dtype == SMAUL_DTYPE_BF16 ? 8 : 4) == 0;
-    blocks += p.xblocks;
-  }
+  prep_rows(p, dtype);
+  int64_t blocks = p.xblocks;
   for (auto& m : p.m) {
     if (m.w) m.blocks = (E * mx4_groups(m.K) * m.N + 255) / 256;
     blocks += m.blocks;
@@ -1389,8 +1431,8 @@ struct LinearParts {
 };
 LinearParts linear_parts(int64_t rows, int64_t K, int64_t N, int dtype, int act) {
   const bool mx4 = act == SMAUL_ACT_MX4;
-  const int64_t ng = mx4_groups(K), nb = mx4_blocks(K), size = dtype == SMAUL_DTYPE_BF16 ? 2 : 4;
-  const bool pad = K % MX4_STAGE != 0;
+  const int64_t ng = mx4_groups(K), nb = mx4_blocks(K);
+  const bool pad = K % MX4_STAGE != 0, f32 = dtype == SMAUL_DTYPE_F32;
   LinearParts q{};
   Parts w;
   q.gemm = rows > ST_ROWS;
@@ -1398,7 +1440,7 @@ LinearParts linear_parts(int64_t rows, int64_t K, int64_t N, int dtype, int act)
     q.x = w.take(mx4 ? rows * nb * 16 : 0);
     q.xs = w.take(mx4 ? rows * nb : 0);
   } else {
-    q.x = w.take(mx4 ? rows * ng * 64 : pad ? rows * ng * MX4_GROUP * size : 0);
+    q.x = w.take(mx4 ? rows * ng * 64 : f32 || pad ? rows * ng * MX4_GROUP * (f32 ? 6 : 2) : 0);
     q.xs = w.take(mx4 ? rows * ng * 4 : 0);
     q.st = w.take(N * ng * 4);
     q.wp = w.take(pad ? N * ng * 64 : 0);
@@ -1407,19 +1449,20 @@ LinearParts linear_parts(int64_t rows, int64_t K, int64_t N, int dtype, int act)
   return q;
 }
 
-// The input gradient's workspace: the weight turned round and decoded, and g in padded
-// rows where its width is no whole number of stages.
+// The input gradient's workspace: the weight turned round and decoded, and g's planes
+// (fp32), or padded rows where its width is no whole number of stages.
 struct DxParts {
   int64_t ldo, wt, g, total;
-  bool pad;
+  bool lay;
 };
 DxParts dx_parts(int64_t rows, int64_t I, int64_t O, int dtype) {
   DxParts q{};
   Parts w;
   q.ldo = mx4_groups(O) * MX4_GROUP;
-  q.pad = O % 64 != 0;
+  const bool f32 = dtype == SMAUL_DTYPE_F32;
+  q.lay = f32 || O % 64 != 0;
   q.wt = w.take(I * q.ldo * 2);
-  q.g = w.take(q.pad ? rows * q.ldo * (dtype == SMAUL_DTYPE_BF16 ? 2 : 4) : 0);
+  q.g = w.take(q.lay ? rows * q.ldo * (f32 ? 6 : 2) : 0);
   q.total = w.at;
   return q;
 }
@@ -1427,8 +1470,9 @@ DxParts dx_parts(int64_t rows, int64_t I, int64_t O, int dtype) {
 template <int AT, int OT>
 int launch_dx(const Mx4Args& p, hipStream_t stream) {
   // us, 4096 rows 2560 -> 1024 bf16: 33 of 8 waves, 35.5 of 4; 64 rows x 64 columns 44.
-  // fp32, 512 rows: 37 of 64 x 64, 41 of 64 x 128
-  if constexpr (AT == A_F32) return launch_gemm_cfg<AT, W_BF16, OT, false, 64, 64, 2, 2, 64, 3>(p, (p.R + 63) / 64, stream);
+  // fp32, 512 rows and 1001 rows 777 -> 1000: 30 and 22 of 32 x 64, 31 and 25 of 64 x 64,
+  // 41 and 31 of 64 x 128 (half the workgroups of a chip)
+  if constexpr (AT == A_F32) return launch_gemm_cfg<AT, W_BF16, OT, false, 32, 64, 1, 2, 64, 3>(p, (p.R + 31) / 32, stream);
   else return launch_gemm_cfg<AT, W_BF16, OT, false, 128, 128, 4, 2, 64, 4>(p, (p.R + 127) / 128, stream);
 }
 
@@ -1488,7 +1532,7 @@ int smaul_mx4_linear(const void* x, int dtype, const uint8_t* w, const uint8_t* 
   const int at = mx4 ? A_MX4 : bf16 ? A_BF16 : A_F32;
   char* ws = (char*)workspace;
   Mx4Args p{};
-  p.x = mx4 || (q.gemm && pad) ? ws + q.x : x;
+  p.x = mx4 || (q.gemm && (pad || !bf16)) ? ws + q.x : x;
   p.xs = (uint8_t*)ws + q.xs;
   p.w = w;
   p.s = s;
@@ -1508,12 +1552,12 @@ int smaul_mx4_linear(const void* x, int dtype, const uint8_t* w, const uint8_t* 
     f.xst = (uint32_t*)(ws + q.xs);
     f.T = rows;
     f.K = in_f;
-    f.xmode = mx4 ? P_ROUND : pad ? P_PAD : P_NONE;
+    f.xmode = mx4 ? P_ROUND : pad || !bf16 ? P_PAD : P_NONE;
     rc = launch_prep(f, dtype, 1, stream);
     p.s = (uint8_t*)ws + q.st;
     if (pad) p.w = (uint8_t*)ws + q.wp;
     p.K = ng * MX4_GROUP;
-    p.ldx = mx4 ? ng * 4 : p.K;
+    p.ldx = mx4 ? ng * 4 : bf16 ? p.K : 3 * p.K;
     p.ldw = ng * 4;
     p.ldy = out_f;
     p.xrows = rows;
@@ -1547,34 +1591,31 @@ int smaul_mx4_backward_input(const void* g, int dtype, const uint8_t* w, const u
                 (long long)workspace_bytes, (long long)q.total);
   const bool bf16 = dtype == SMAUL_DTYPE_BF16;
   char* ws = (char*)workspace;
-  const int64_t turns = q.ldo / 64 * ((in_f + 63) / 64);
-  if (turns > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_backward_input: too large a weight");
-  hipLaunchKernelGGL(mx4_turn_kernel, dim3((unsigned)turns), dim3(256), 0, stream, w, s, (uint16_t*)(ws + q.wt), out_f,
-                     in_f, q.ldo);
+  Mx4Prep f{};
+  f.x = g;
+  f.xo = ws + q.g;
+  f.T = rows;
+  f.K = out_f;
+  f.xmode = q.lay ? P_PAD : P_NONE;
+  prep_rows(f, dtype);
+  const int64_t blocks = f.xblocks + q.ldo / 64 * ((in_f + 63) / 64);
+  if (blocks > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_backward_input: too large a weight or gradient");
+  auto* kernel = bf16 ? &mx4_turn_kernel<true> : &mx4_turn_kernel<false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, f, w, s, (uint16_t*)(ws + q.wt), out_f, in_f,
+                     q.ldo);
   int rc = check_launch("mx4_turn_kernel");
   if (rc) return rc;
   Mx4Args p{};
-  p.x = g;
+  p.x = q.lay ? ws + q.g : g;
   p.w = (uint8_t*)ws + q.wt;
   p.y = dx;
   p.R = rows;
-  p.K = q.pad ? q.ldo : out_f;
+  p.K = q.lay ? q.ldo : out_f;
   p.N = in_f;
-  p.ldx = p.K;
+  p.ldx = bf16 ? p.K : 3 * p.K;
   p.ldw = q.ldo;
   p.ldy = in_f;
   p.E = 1;
-  if (q.pad) {
-    Mx4Prep f{};
-    f.x = g;
-    f.xo = ws + q.g;
-    f.T = rows;
-    f.K = out_f;
-    f.xmode = P_PAD;
-    rc = launch_prep(f, dtype, 1, stream);
-    if (rc) return rc;
-    p.x = ws + q.g;
-  }
   return bf16 ? launch_dx<A_BF16, O_BF16>(p, stream) : launch_dx<A_F32, O_F32>(p, stream);
 }
 
@@ -1587,8 +1628,9 @@ struct Mx4MoeParts {
 static Mx4MoeParts mx4_moe_parts(int64_t T, int64_t d, int64_t h, int64_t E, int64_t k, int dtype, int act) {
   Mx4MoeParts q{};
   Parts w;
-  const int64_t size = dtype == SMAUL_DTYPE_BF16 ? 2 : 4, R = T * k, gd = mx4_groups(d), gh = mx4_groups(h);
-  const bool mx4 = act == SMAUL_ACT_MX4;
+  const int64_t R = T * k, gd = mx4_groups(d), gh = mx4_groups(h);
+  const bool mx4 = act == SMAUL_ACT_MX4, f32 = dtype == SMAUL_DTYPE_F32;
+  const int64_t size = f32 ? 4 : 2, wide = f32 ? 6 : 2;  // bytes of a value, and of one that the GEMM reads
   q.gemm = T > ST_ROWS;
   if (q.gemm) {
     q.seg_off = w.take((E + 1) * 4);
@@ -1599,9 +1641,9 @@ static Mx4MoeParts mx4_moe_parts(int64_t T, int64_t d, int64_t h, int64_t E, int
     q.scratch_bytes = smaul_moe_dispatch_workspace_size(T, E);
     q.scratch = w.take(q.scratch_bytes);
     const bool pd = d % MX4_STAGE != 0, ph = h % MX4_STAGE != 0;
-    q.xc = w.take(mx4 ? T * gd * 64 : pd ? T * gd * MX4_GROUP * size : 0);
+    q.xc = w.take(mx4 ? T * gd * 64 : pd || f32 ? T * gd * MX4_GROUP * wide : 0);
     q.xs = w.take(mx4 ? T * gd * 4 : 0);
-    q.hc = w.take(mx4 ? R * gh * 64 : R * gh * MX4_GROUP * size);
+    q.hc = w.take(mx4 ? R * gh * 64 : R * gh * MX4_GROUP * wide);
     q.hs = w.take(mx4 ? R * gh * 4 : 0);
     for (int j = 0; j < 3; ++j) {
       q.st[j] = w.take(E * (j < 2 ? h * gd : d * gh) * 4);
@@ -1655,7 +1697,7 @@ int smaul_mx4_moe_forward(const void* x, int dtype, const int64_t* topi, const f
   const int64_t R = T * k, gd = mx4_groups(d), gh = mx4_groups(h);
   const bool pd = d % MX4_STAGE != 0, ph = h % MX4_STAGE != 0;
   const int64_t bm = gemm_bm(at), m_tiles = (R + bm - 1) / bm + E;
-  if (q.gemm && !(mx4 || T * (pd ? gd * MX4_GROUP : d) * (bf16 ? 2 : 4) < (1LL << 32)))
+  if (q.gemm && !(mx4 || T * (pd || !bf16 ? gd * MX4_GROUP : d) * (bf16 ? 2 : 6) < (1LL << 32)))
     return fail(SMAUL_ERR_UNSUPPORTED, "mx4_moe: more than 4 GiB of x");
   if (mx4 && T * gd * 64 >= (1LL << 32)) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_moe: more than 4 GiB of codes of x");
   int rc = SMAUL_OK;
@@ -1665,7 +1707,7 @@ int smaul_mx4_moe_forward(const void* x, int dtype, const int64_t* topi, const f
     if (rc) return rc;
   }
   Mx4Args p{};
-  p.x = mx4 || (q.gemm && pd) ? ws + q.xc : x;
+  p.x = mx4 || (q.gemm && (pd || !bf16)) ? ws + q.xc : x;
   p.xs = (uint8_t*)ws + q.xs;
   p.row_idx = perm_row;
   p.w = gate_w;
@@ -1708,16 +1750,16 @@ int smaul_mx4_moe_forward(const void* x, int dtype, const int64_t* topi, const f
     f.xst = (uint32_t*)(ws + q.xs);
     f.T = T;
     f.K = d;
-    f.xmode = mx4 ? P_ROUND : pd ? P_PAD : P_NONE;
+    f.xmode = mx4 ? P_ROUND : pd || !bf16 ? P_PAD : P_NONE;
     rc = launch_prep(f, dtype, E, stream);
     p.w = at_w[0];
     p.s = at_s[0];
     p.w2 = at_w[1];
     p.s2 = at_s[1];
     p.K = gd * MX4_GROUP;
-    p.ldx = mx4 ? gd * 4 : p.K;
+    p.ldx = mx4 ? gd * 4 : bf16 ? p.K : 3 * p.K;
     p.ldw = gd * 4;
-    p.ldy = mx4 ? gh * 4 : gh * MX4_GROUP;
+    p.ldy = mx4 ? gh * 4 : gh * MX4_GROUP * (bf16 ? 1 : 3);
     p.xrows = T;
     p.yrows = R;
     dn.w = at_w[2];

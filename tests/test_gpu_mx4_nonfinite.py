@@ -1,0 +1,79 @@
+"""The 4-bit products with infinities and NaN among the activations, and values of all of a type's bits."""
+import math
+
+import pytest
+import torch
+
+import _mx4 as ref
+from smaulnative_amd.compute import get_backend
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def _same_kinds(got, want):
+    """Infinities with their signs and NaN where the plain product has them."""
+    got = got.cpu().double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.where(torch.isinf(got), got, torch.zeros_like(got)),
+                       torch.where(torch.isinf(want), want, torch.zeros_like(want)))
+
+
+def _spoil(x):
+    """One value a row is no number; the last payload is in a NaN's lowest bit alone."""
+    x[0, 3], x[1, 40], x[2, 70] = math.inf, -math.inf, math.nan
+    x[3, 0], x[3, 1] = math.inf, -math.inf
+    if x.dtype == F32:
+        x[4].view(torch.int32)[5] = 0x7F800001
+    return x
+
+
+@pytest.mark.parametrize("rows", [9, 70, 300])  # the kernel of few rows, and the larger ones
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_products_of_infinities(rows, dtype):
+    gen = torch.Generator().manual_seed(rows)
+    K, N = 96, 80
+    x = _spoil(torch.randn(rows, K, generator=gen).to(dtype))
+    w, s = ref.weight(N, K, gen)
+    got = get_backend("rocm").mx4_forward(x.to(DEV), w.to(DEV), s.to(DEV), K, N)
+    want = x.double() @ ref.values(w, s, K).t()
+    _same_kinds(got, want)
+    clean = torch.isfinite(x).all(-1)
+    assert clean.sum() == rows - (5 if dtype == F32 else 4) and torch.isfinite(got.cpu()[clean]).all()
+
+    g = _spoil(torch.randn(rows, N, generator=gen).to(dtype))
+    dx = get_backend("rocm").mx4_backward_input(g.to(DEV), w.to(DEV), s.to(DEV), K, N)
+    _same_kinds(dx, g.double() @ ref.values(w, s, K))
+
+
+@pytest.mark.parametrize("T", [9, 150])
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_experts_of_nan_rows(T, dtype):
+    """A token that is no number takes no other with it."""
+    gen = torch.Generator().manual_seed(T)
+    E, d, h, k = 4, 64, 96, 2
+    x = torch.randn(T, d, generator=gen).to(dtype)
+    x[2, 5], x[7, 0] = math.nan, math.inf
+    experts = []
+    for o, i in ((h, d), (h, d), (d, h)):
+        ws = [ref.weight(o, i, gen) for _ in range(E)]
+        experts += [torch.stack([w for w, _ in ws]), torch.stack([s for _, s in ws])]
+    topi = torch.stack([torch.randperm(E, generator=gen)[:k] for _ in range(T)])
+    topw = torch.rand(T, k, generator=gen) + 0.1
+    out, _ = get_backend("rocm").mx4_moe_forward(x.to(DEV), topi.to(DEV), topw.to(DEV), [t.to(DEV) for t in experts])
+    fine = torch.ones(T, dtype=torch.bool)
+    fine[2], fine[7] = False, False
+    out = out.cpu()
+    assert torch.isfinite(out[fine]).all() and torch.isnan(out[2]).all() and not torch.isfinite(out[7]).any()
+
+
+@pytest.mark.parametrize("rows", [9, 150])
+def test_fp32_activations_keep_all_their_bits(rows):
+    """A weight of one code picks single activations: 24 bits come back as they went in."""
+    gen = torch.Generator().manual_seed(rows)
+    K = 64
+    x = torch.randn(rows, K, generator=gen) * torch.pow(2.0, torch.randint(-30, 30, (rows, K), generator=gen).float())
+    w, s = ref.quantize(torch.eye(K))
+    got = get_backend("rocm").mx4_forward(x.to(DEV), w.to(DEV), s.to(DEV), K, K)
+    assert torch.equal(got.cpu(), x)
