@@ -293,7 +293,6 @@ __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
       // each lane from another place on: other banks
       if (per % 4 == 0) {
         int i = 4 * l % per;
-#pragma unroll 2
         for (int j = 0; j < per; j += 4) {
           const float4 c = *(const float4*)(sc + g * per + i);
           i = i + 4 == per ? 0 : i + 4;
@@ -346,45 +345,65 @@ __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
       key[v] &= (uint32_t)__builtin_amdgcn_sbfe((int)word, g & 31, 1);
     }
   }
-  // Lane j gets the j-th highest.  The walk goes on past k while the next one is too
-  // near to the last to be left out.
-  int mine = -1, n = 0;
-  bool near = false, done = false;
-  uint32_t last = 0;
-  for (int j = 0; __ballot(!done); ++j) {
-    uint32_t best = key[0];
+  // Lane j gets the j-th highest, and its key.  A lane's highest goes out of its keys
+  // without a comparison: of key and key - gone the lower is 0 for it alone (~0u: none).
+  int mine = -1;
+  uint32_t val = 0u, best = 0u;
+  auto highest = [&]() {  // the lane's; best: the token's
+    uint32_t own = key[0];
 #pragma unroll
-    for (int v = 1; v < V; ++v) best = max(best, key[v]);
-    const uint32_t own = best;
+    for (int v = 1; v < V; ++v) own = max(own, key[v]);
+    best = own;
     SMAUL_ROW_REDUCE(best, op_umax);
-    bool close = false;
-    if (j > 0 && best != 0u) {
-      const uint32_t ua = last & ~LOW, ub = best & ~LOW;
-      if (p.bias) {
-        const float fa = __uint_as_float(ua >> 31 ? ua ^ 0x80000000u : ~ua);
-        const float fb = __uint_as_float(ub >> 31 ? ub ^ 0x80000000u : ~ub);
-        // each c is off by s_err and half a unit, the second may gain V units by its low bits
-        close = !(fa - fb > 2.0f * s_err + (V + 2) * 0x1p-23f * fmaxf(fabsf(fa), fabsf(fb)));
-      } else {
-        close = !p.bf16 && ua == ub;  // logits that the low bits may tell apart
-      }
-    }
-    if (!done) {
-      done = best == 0u || (j >= p.k && !close);
-      if (!done && j == 16) done = again = true;  // more of them than lanes
-      if (!done) {
-        near |= close;
-        n = j + 1;
-      }
-    }
-    last = best;
+    return own;
+  };
+  auto take = [&](uint32_t own, bool store) {
     // the lowest lane that has it
     const uint32_t has = (uint32_t)(__ballot(own == best) >> (tq * 16)) & 0xffffu;
     const int owner = __builtin_ctz(has);
-    if (!done && l == j) mine = (int)(LOW - (best & LOW)) * 16 + owner;
-    const uint32_t gone = l == owner ? best : 1u;  // 1: no key (a live one is over 2^22)
+    if (store) {
+      val = best;
+      mine = (int)(LOW - (best & LOW)) * 16 + owner;
+    }
+    const uint32_t gone = l == owner ? best : ~0u;
 #pragma unroll
-    for (int v = 0; v < V; ++v) key[v] = key[v] == gone ? 0u : key[v];
+    for (int v = 0; v < V; ++v) key[v] = min(key[v], key[v] - gone);
+  };
+  for (int j = 0; j < p.k; ++j) {
+    const uint32_t own = highest();
+    take(own, l == j);
+  }
+  if (val == 0u) mine = -1;
+  int n = __popc((uint32_t)(__ballot(val != 0u) >> (tq * 16)) & 0xffffu);
+  // is b, which is not above a, too near to be told apart?
+  auto too_near = [&](uint32_t a, uint32_t b) {
+    const uint32_t ua = a & ~LOW, ub = b & ~LOW;
+    if (b == 0u) return false;
+    if (!p.bias) return !p.bf16 && ua == ub;  // logits that the low bits may tell apart
+    const float fa = __uint_as_float(ua >> 31 ? ua ^ 0x80000000u : ~ua);
+    const float fb = __uint_as_float(ub >> 31 ? ub ^ 0x80000000u : ~ub);
+    // each c is off by s_err and half a unit, the second may gain V units by its low bits
+    return !(fa - fb > 2.0f * s_err + (V + 2) * 0x1p-23f * fmaxf(fabsf(fa), fabsf(fb)));
+  };
+  // lane j: the j-th and the one before; lane 0: the last and the next that is left out
+  uint32_t own = highest();
+  const uint32_t before = (uint32_t)__shfl((int)val, l == 0 ? p.k - 1 : l - 1, 16);
+  const bool close = l < p.k && too_near(before, l == 0 ? best : val);
+  const uint32_t closes = (uint32_t)(__ballot(close) >> (tq * 16)) & 0xffffu;
+  bool near = closes != 0u;
+  // the walk goes on past k while the next is too near to the last to be left out
+  bool on_and_on = (closes & 1u) != 0u;
+  uint32_t last = best;
+  for (int j = p.k; __ballot(on_and_on); ++j) {
+    if (on_and_on && j == 16) {  // more of them than lanes
+      again = true;
+      on_and_on = false;
+    }
+    if (on_and_on) n = j + 1;
+    last = best;
+    take(own, on_and_on && l == j);
+    own = highest();
+    on_and_on = on_and_on && too_near(last, best);
   }
   // Neighbours too near for 32 bits: the n found are ordered by what they are in 64
   // (the sum of a softmax with a bias is left to route_row64).
