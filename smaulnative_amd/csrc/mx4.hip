@@ -410,7 +410,8 @@ struct Mx4Args {
   const int32_t* seg_off;  // null: dense, R rows of one expert
   const int32_t* tile_off;
   int E;
-  int xvec;                // mx4_stream_kernel: x rows may be read 16 bytes at a time
+  int xvec;                // mx4_stream_kernel: x rows may be read 16 bytes at a time,
+  int svec;                // and four scales of W
 };
 
 // the rows of m-tile mt: its expert, first logical row and row count (uniform);
@@ -702,7 +703,7 @@ __device__ __forceinline__ void mx4_epilogue(const Mx4Args& p, const f32x16_t (&
 // q multiplies values 32 g + 8 q and on; fp32 activations are three planes of bf16.
 // W_BF16: the weight's rows are bf16 already.
 template <int AT, int WF, int OT, bool SWIGLU, int BM, int BN, int WM, int WN, int KS, int NSTAGE>
-__global__ void __launch_bounds__(WM * WN * 64, 2) mx4_gemm_kernel(Mx4Args p) {
+__global__ void __launch_bounds__(WM * WN * 64, WM * WN < 4 ? 1 : 2) mx4_gemm_kernel(Mx4Args p) {
   using C = Mx4Cfg<AT, WF, BM, BN, WM, WN, KS, NSTAGE>;
   static_assert(AT != A_MX4 && OT != O_MX4, "mx4_codes_kernel's");
   constexpr int TT = C::TT, WT = C::WT, BNO = SWIGLU ? BN / 2 : BN, XROW = C::XROW, WROW = C::WROW;
@@ -1029,8 +1030,13 @@ int launch_codes(const Mx4Args& p, int64_t m_tiles, hipStream_t stream) {
 
 // The kernel of few rows (up to 64): a workgroup has 32 columns of one expert, its NW
 // waves a slice of K each, so that every byte of the weight is read once and all at
-// the same time; rows of x come from the caches, straight into registers.  The
-// waves' sums meet in LDS and are added in the order of the waves.
+// the same time.  A lane's codes lie in a row of their own, but x, which comes from the
+// caches for every 32 columns again, goes through LDS: a load of four rows by 256 bytes
+// asks for 8 lines, one of 32 rows by 32 bytes for 32 (32 x 4096 -> 4096: 10 us, 15.4
+// from registers; 64 tokens to 2 of 8 experts, 1024 by 2560: 14.5 + 9.7 us, 16.4 + 10.8;
+// the weights alone are 5).  The waves' sums meet in LDS too and are added in the order
+// of the waves.  Sending the first weights before the rows are known cost more
+// registers than it won (19.2 us for 14.5).
 //
 // The experts' rows are found here, without a dispatch: a workgroup looks through the
 // T k <= 512 slots for its expert's; the hidden rows and the outputs
@@ -1047,7 +1053,8 @@ constexpr int ST_ROWS = 64, ST_SLOTS = 512;
 
 // whether slot i of (token, expert) is one that the layer runs: an expert of the E, a
 // weight above 0, and the token's first slot with it (as smaul_moe_dispatch)
-__device__ __forceinline__ bool mx4_slot(const int64_t* topi, const float* topw, int64_t t, int j, int k, int E, int e) {
+__device__ __forceinline__ bool mx4_slot(const int64_t* topi, const float* topw, int64_t t, int j, int k, int E,
+                                         int e) {
   if (topi[t * k + j] != e || !(topw[t * k + j] > 0.0f) || e < 0 || e >= E) return false;
   for (int i = 0; i < j; ++i)
     if (topi[t * k + i] == e && topw[t * k + i] > 0.0f) return false;
@@ -1056,9 +1063,13 @@ __device__ __forceinline__ bool mx4_slot(const int64_t* topi, const float* topw,
 
 template <int AT, int OT, bool SWIGLU, bool VEC, int NW>
 __global__ void __launch_bounds__(NW * 64) mx4_stream_kernel(Mx4Args p, Mx4Slots q) {
-  constexpr int SW = SWIGLU ? 2 : 1, U = (AT == A_F32 ? 2 : 4) / (AT == A_MX4 ? 1 : SW);  // steps read at once
+  constexpr int SW = SWIGLU ? 2 : 1, U = AT == A_MX4 ? 4 : 2;  // steps read at once
   constexpr int JS = 1024 + 64;  // bytes between the quarters of a wave's sums: other banks
-  __shared__ __attribute__((aligned(16))) char red[NW * 4 * JS];
+  // x as it is: a wave's U steps of 32 rows, XP pieces of 16 bytes a row, changing places
+  // by the row; the sums meet in the same LDS
+  constexpr bool XL = VEC && AT != A_MX4;
+  constexpr int XSZ = AT == A_BF16 ? 2 : 4, XP = U * 4 * XSZ, XI = XL ? XP / 2 : 1, XW = XL ? 32 * XP * 16 : 0;
+  __shared__ __attribute__((aligned(1024))) char red[NW * (XW > 4 * JS ? XW : 4 * JS)];
   constexpr int NC = ST_SLOTS / (NW * 64);  // slots a thread
   __shared__ int s_row[ST_ROWS], s_cnt[NC * NW];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, l32 = lane & 31;
@@ -1098,9 +1109,30 @@ __global__ void __launch_bounds__(NW * 64) mx4_stream_kernel(Mx4Args p, Mx4Slots
   const int64_t nb = mx4_blocks(p.K);
   const int64_t wrow = n0 + mx4_perm(l32) < p.N ? n0 + mx4_perm(l32) : p.N - 1;
   const int64_t wblk = ((int64_t)e * p.N + wrow) * nb;
-  const int steps = (int)((nb + 1) / 2), per = (steps + NW - 1) / NW;
+  const int steps = (int)((nb + 1) / 2), per = ((steps + NW - 1) / NW + 1) / 2 * 2;
   const int lo = min(wave * per, steps), hi = min(lo + per, steps);
 
+  uint4 wc[U][SW];
+  uint32_t ws[U][SW];
+  auto load_w = [&](int s0) {
+    uint32_t sd[(U + 1) / 2][SW];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t b = (int64_t)(s0 + u) * 2 + g;  // this lane's block of the step
+      const bool in = s0 + u < hi && b < nb;
+#pragma unroll
+      for (int j = 0; j < SW; ++j) {
+        wc[u][j] = in ? *(const uint4*)((j ? p.w2 : p.w) + (wblk + b) * 16) : make_uint4(0, 0, 0, 0);
+        const uint8_t* s = (j ? p.s2 : p.s) + wblk;
+        if (p.svec) {  // the four scales of 128 values at once; slices begin at a multiple
+          if (u % 2 == 0) sd[u / 2][j] = in ? *(const uint32_t*)(s + (b - g)) : 0u;
+          ws[u][j] = sd[u / 2][j] >> (16 * (u & 1) + 8 * g);
+        } else {
+          ws[u][j] = in ? s[b] : 0u;
+        }
+      }
+    }
+  };
   for (int r0 = 0; r0 < rows; r0 += 32) {  // uniform
     const int r = min(r0 + l32, rows - 1);
     const int64_t slot = q.topi ? s_row[r] : r;
@@ -1111,68 +1143,82 @@ __global__ void __launch_bounds__(NW * 64) mx4_stream_kernel(Mx4Args p, Mx4Slots
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[j][i] = 0.0f;
 
+    char* own = red + wave * XW;
+    uint32_t x_at[XI];  // where this lane's piece of DMA instruction a begins, in the row
+    if constexpr (XL) {
+#pragma unroll
+      for (int a = 0; a < XI; ++a) {
+        const int rr = a * (64 / XP) + lane / XP, rc = min(r0 + rr, rows - 1);
+        const int at = q.topi ? s_row[rc] : rc, row = q.topi && q.by_token ? at / q.k : at;
+        x_at[a] = (uint32_t)(row * p.K * XSZ);
+      }
+    }
     for (int s0 = lo; s0 < hi; s0 += U) {
-      uint4 wc[U][SW];
-      uint32_t ws[U][SW];
-      uint4 xv[U][AT == A_MX4 ? 1 : AT == A_BF16 ? 4 : 8];
+      if constexpr (XL) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last pieces are read
+#pragma unroll
+        for (int a = 0; a < XI; ++a) {
+          if (a * (64 / XP) >= rows - r0) break;  // uniform; rows that nobody needs hold anything
+          const int rr = a * (64 / XP) + lane / XP;
+          const int64_t col = (int64_t)s0 * 64 * XSZ + (lane % XP ^ (rr & 15)) * 16, end = p.K * XSZ - 16;
+          dma16(p.x, x_at[a] + (uint32_t)(col < end ? col : end), lds_offset(own + a * 1024));
+        }
+      }
+      load_w(s0);
+      uint4 xv[U];  // A_MX4
       uint32_t xsc[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t b = (int64_t)(s0 + u) * 2 + g;  // this lane's block of the step
+        const int64_t b = (int64_t)(s0 + u) * 2 + g;
         const bool in = s0 + u < hi && b < nb;
-#pragma unroll
-        for (int j = 0; j < SW; ++j) {
-          wc[u][j] = in ? *(const uint4*)((j ? p.w2 : p.w) + (wblk + b) * 16) : make_uint4(0, 0, 0, 0);
-          ws[u][j] = in ? (j ? p.s2 : p.s)[wblk + b] : 0u;
-        }
         if constexpr (AT == A_MX4) {
-          xv[u][0] = in ? *(const uint4*)((const uint8_t*)p.x + (xr * nb + b) * 16) : make_uint4(0, 0, 0, 0);
+          xv[u] = in ? *(const uint4*)((const uint8_t*)p.x + (xr * nb + b) * 16) : make_uint4(0, 0, 0, 0);
           xsc[u] = in ? p.xs[xr * nb + b] : 0u;
-        } else if constexpr (VEC) {
-          constexpr int V16 = AT == A_BF16 ? 4 : 8, EL = AT == A_BF16 ? 8 : 4;
-#pragma unroll
-          for (int v = 0; v < V16; ++v) {
-            const int64_t c = b * MX4_BLOCK + v * EL;  // K is a multiple of EL
-            const char* src = (const char*)p.x + (xr * p.K + c) * (AT == A_BF16 ? 2 : 4);
-            xv[u][v] = s0 + u < hi && c < p.K ? *(const uint4*)src : make_uint4(0, 0, 0, 0);
-          }
         }
       }
+      if constexpr (XL) wait_vm<0>();
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (s0 + u >= hi) break;  // uniform
         if constexpr (AT == A_MX4) {
 #pragma unroll
           for (int j = 0; j < SW; ++j)
-            acc[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx4_operand(wc[u][j]), mx4_operand(xv[u][0]), acc[j],
-                                                                    4, 4, 0, (int)ws[u][j], 0, (int)xsc[u]);
+            acc[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                mx4_operand(wc[u][j]), mx4_operand(xv[u]), acc[j], 4, 4, 0, (int)ws[u][j], 0, (int)xsc[u]);
         } else {
           const int64_t b = (int64_t)(s0 + u) * 2 + g;
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             constexpr int NT = AT == A_F32 ? 3 : 1;
             bf16x8_t t[3];
-            if constexpr (VEC && AT == A_BF16) {
-              t[0] = __builtin_bit_cast(bf16x8_t, xv[u][v]);
+            const bool in = b * MX4_BLOCK + v * 8 < p.K;  // whole pieces
+            auto piece = [&](int i) {
+              const uint4 x = *(const uint4*)(own + (l32 * XP + (i ^ (l32 & 15))) * 16);
+              return in ? x : make_uint4(0, 0, 0, 0);
+            };
+            if constexpr (XL && AT == A_BF16) {
+              t[0] = __builtin_bit_cast(bf16x8_t, piece(u * 8 + g * 4 + v));
             } else {
               float f[8];
-              if constexpr (VEC) {
-                const uint4 a = xv[u][2 * v], c = xv[u][2 * v + 1];
-                f[0] = __uint_as_float(a.x); f[1] = __uint_as_float(a.y); f[2] = __uint_as_float(a.z); f[3] = __uint_as_float(a.w);
-                f[4] = __uint_as_float(c.x); f[5] = __uint_as_float(c.y); f[6] = __uint_as_float(c.z); f[7] = __uint_as_float(c.w);
+              if constexpr (XL) {
+                const uint4 a = piece(u * 16 + g * 8 + 2 * v), c = piece(u * 16 + g * 8 + 2 * v + 1);
+                f[0] = __uint_as_float(a.x); f[1] = __uint_as_float(a.y);
+                f[2] = __uint_as_float(a.z); f[3] = __uint_as_float(a.w);
+                f[4] = __uint_as_float(c.x); f[5] = __uint_as_float(c.y);
+                f[6] = __uint_as_float(c.z); f[7] = __uint_as_float(c.w);
               } else {
                 mx4_load8<AT == A_BF16, false>(p.x, xr, p.K, b * MX4_BLOCK + v * 8, f);
               }
-              uint4 u[3];
-              mx4_split3(f, u);
+              uint4 h[3];
+              mx4_split3(f, h);
 #pragma unroll
-              for (int k = 0; k < 3; ++k) t[k] = __builtin_bit_cast(bf16x8_t, u[k]);
+              for (int k = 0; k < 3; ++k) t[k] = __builtin_bit_cast(bf16x8_t, h[k]);
             }
 #pragma unroll
             for (int j = 0; j < SW; ++j) {
               const uint4 c = wc[u][j];
               const bf16x8_t wf = __builtin_bit_cast(
-                  bf16x8_t, mx4_decode8(v == 0 ? c.x : v == 1 ? c.y : v == 2 ? c.z : c.w, mx4_scale(ws[u][j])));
+                  bf16x8_t, mx4_decode8(v == 0 ? c.x : v == 1 ? c.y : v == 2 ? c.z : c.w, mx4_scale(ws[u][j] & 255u)));
 #pragma unroll
               for (int k = 0; k < NT; ++k)
                 acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf, t[k], acc[j], 0, 0, 0);
@@ -1187,7 +1233,7 @@ __global__ void __launch_bounds__(NW * 64) mx4_stream_kernel(Mx4Args p, Mx4Slots
     float v[SW][4];
 #pragma unroll
     for (int j = 0; j < SW; ++j) {
-      if (j) __syncthreads();
+      if (j || XL) __syncthreads();
 #pragma unroll
       for (int c = 0; c < 4; ++c)
         *(float4*)(red + (wave * 4 + c) * JS + lane * 16) =
@@ -1242,10 +1288,12 @@ __global__ void __launch_bounds__(NW * 64) mx4_stream_kernel(Mx4Args p, Mx4Slots
 }
 
 template <int AT, int OT, bool SWIGLU, int NW>
-int launch_stream_cfg(const Mx4Args& p, const Mx4Slots& q, int64_t groups, hipStream_t stream) {
+int launch_stream_cfg(Mx4Args p, const Mx4Slots& q, int64_t groups, hipStream_t stream) {
+  p.svec = mx4_blocks(p.K) % 4 == 0 && aligned(p.s, 4) && (!SWIGLU || aligned(p.s2, 4));
   const dim3 grid((unsigned)groups), block(NW * 64);
   if constexpr (AT != A_MX4) {
-    if (!p.xvec) {
+    const int64_t x_rows = q.topi ? (q.by_token ? q.T : q.T * q.k) : p.R;
+    if (!p.xvec || x_rows * p.K * 4 >= 1LL << 32) {
       hipLaunchKernelGGL((mx4_stream_kernel<AT, OT, SWIGLU, false, NW>), grid, block, 0, stream, p, q);
       return check_launch("mx4_stream_kernel");
     }
@@ -1362,8 +1410,12 @@ int launch_quantize(const void* x, int dtype, uint8_t* codes, uint8_t* scales, i
   const bool nt = rows * K * (bf16 ? 2 : 4) >= MX4_NT_BYTES;
 #define SMAUL_Q(B, V, N) \
   hipLaunchKernelGGL((mx4_quantize_kernel<B, V, N>), grid, block, 0, stream, x, (uint32_t*)codes, scales, rows, K)
-  if (bf16) { if (vec && nt) SMAUL_Q(true, true, true); else if (vec) SMAUL_Q(true, true, false); else SMAUL_Q(true, false, false); }
-  else { if (vec && nt) SMAUL_Q(false, true, true); else if (vec) SMAUL_Q(false, true, false); else SMAUL_Q(false, false, false); }
+  if (bf16 && vec && nt) SMAUL_Q(true, true, true);
+  else if (bf16 && vec) SMAUL_Q(true, true, false);
+  else if (bf16) SMAUL_Q(true, false, false);
+  else if (vec && nt) SMAUL_Q(false, true, true);
+  else if (vec) SMAUL_Q(false, true, false);
+  else SMAUL_Q(false, false, false);
 #undef SMAUL_Q
   return check_launch("mx4_quantize_kernel");
 }
@@ -1378,7 +1430,8 @@ int launch_product(const Mx4Args& p, const Mx4Slots* few, int64_t m_tiles, hipSt
   // of 64 x 256, 87 and 47 of 64 x 128, 91 and 42 of 32 x 128
   if constexpr (AT == A_F32)
     return launch_gemm_cfg<AT, W_MX4, SWIGLU ? O_PLANES : OT, SWIGLU, 32, 256, 1, 4, 64, 2>(p, m_tiles, stream);
-  else if constexpr (AT == A_BF16) return launch_gemm_cfg<AT, W_MX4, OT, SWIGLU, 128, 256, 2, 2, 64, 3>(p, m_tiles, stream);
+  else if constexpr (AT == A_BF16)
+    return launch_gemm_cfg<AT, W_MX4, OT, SWIGLU, 128, 256, 2, 2, 64, 3>(p, m_tiles, stream);
   else return launch_codes<OT, SWIGLU, 256, 256, 4, 2>(p, m_tiles, stream);
 }
 
@@ -1407,8 +1460,8 @@ int launch_prep(Mx4Prep p, int dtype, int64_t E, hipStream_t stream) {
     blocks += m.blocks;
   }
   if (blocks > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: too many rows");
-  if (dtype == SMAUL_DTYPE_BF16) hipLaunchKernelGGL(mx4_prep_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, stream, p, E);
-  else hipLaunchKernelGGL(mx4_prep_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, stream, p, E);
+  auto* kernel = dtype == SMAUL_DTYPE_BF16 ? &mx4_prep_kernel<true> : &mx4_prep_kernel<false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p, E);
   return check_launch("mx4_prep_kernel");
 }
 
@@ -1504,8 +1557,12 @@ int smaul_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* y, i
 #define SMAUL_D(B, V, N)                                                                                       \
   hipLaunchKernelGGL((mx4_dequantize_kernel<B, V, N>), grid, block, 0, stream, (const uint32_t*)codes, scales, \
                      y, rows, K)
-  if (bf16) { if (vec && nt) SMAUL_D(true, true, true); else if (vec) SMAUL_D(true, true, false); else SMAUL_D(true, false, false); }
-  else { if (vec && nt) SMAUL_D(false, true, true); else if (vec) SMAUL_D(false, true, false); else SMAUL_D(false, false, false); }
+  if (bf16 && vec && nt) SMAUL_D(true, true, true);
+  else if (bf16 && vec) SMAUL_D(true, true, false);
+  else if (bf16) SMAUL_D(true, false, false);
+  else if (vec && nt) SMAUL_D(false, true, true);
+  else if (vec) SMAUL_D(false, true, false);
+  else SMAUL_D(false, false, false);
 #undef SMAUL_D
   return check_launch("mx4_dequantize_kernel");
 }

@@ -115,7 +115,6 @@ __device__ __forceinline__ void route_row64(const RouteArgs& p, int64_t t, int l
       score = p.group_best == 2 && b2 > -inf ? b1 + b2 : b1;
     }
     int ahead = 0;
-#pragma unroll 4
     for (int g = 0; g < p.groups; ++g) {
       const double o = __shfl(score, g, 64);
       ahead += o > score || (o == score && g < lane);

@@ -304,7 +304,8 @@ class SwiFFN_MoE(nn.Module):
         return out
 
     def _logits(self, xs):
-        return F.linear(xs.float(), self.gate.weight.float(), None if self.gate.bias is None else self.gate.bias.float())
+        bias = None if self.gate.bias is None else self.gate.bias.float()
+        return F.linear(xs.float(), self.gate.weight.float(), bias)
 
     def _forward_routed(self, be, x):
         """(out, prob, topi, counts): the router's logits, ``moe_route``, and the experts on

@@ -637,8 +637,8 @@ class RocmBackend:
         lead = x.shape[:-1]
         if topi.dtype != torch.int64 or topw.dtype != torch.float32 or tuple(topi.shape) != (*lead, k) or \
                 tuple(topw.shape) != (*lead, k):
-            raise RuntimeError(f"mx4_moe_forward: topi int64 and topw float32 {[*lead, 'k']} expected, got {topi.dtype} "
-                               f"{list(topi.shape)} / {topw.dtype} {list(topw.shape)}")
+            raise RuntimeError(f"mx4_moe_forward: topi int64 and topw float32 {[*lead, 'k']} expected, got "
+                               f"{topi.dtype} {list(topi.shape)} / {topw.dtype} {list(topw.shape)}")
         if not 1 <= k <= min(E, 8) or E > 64:
             raise ValueError(f"mx4_moe_forward: need 1 <= k <= min(E, 8) and E <= 64, got k={k}, E={E}")
         topi, topw = (t if t.is_contiguous() else t.contiguous() for t in (topi, topw))
