@@ -459,9 +459,8 @@ class RocmBackend:
         if bias is not None:
             if bias.numel() != E:
                 raise RuntimeError(f"moe_route: bias must have {E} elements, got {bias.numel()}")
-            bias = bias.detach()
             if not (bias.dtype == torch.float32 and bias.is_contiguous()):
-                bias = bias.float().contiguous()
+                bias = bias.detach().float().contiguous()
         z = logits if logits.is_contiguous() else logits.contiguous()
         dev = z.device
         prob = torch.empty(T, E, dtype=torch.float32, device=dev) if need_prob else None
@@ -533,9 +532,10 @@ class RocmBackend:
     def _mx4_check(self, name, codes, scales, lead, K):
         """The codes and scales [*lead, 16 n] / [*lead, n] of rows of K values, contiguous."""
         n = (K + 31) // 32
-        for what, t, last in (("codes", codes, n * 16), ("scales", scales, n)):
-            if t.dtype != torch.uint8 or tuple(t.shape) != (*lead, last):
-                raise RuntimeError(f"{name}: {what} must be uint8 {[*lead, last]}, got {t.dtype} {list(t.shape)}")
+        if codes.dtype != torch.uint8 or codes.shape != (*lead, n * 16):
+            raise RuntimeError(f"{name}: codes must be uint8 {[*lead, n * 16]}, got {codes.dtype} {list(codes.shape)}")
+        if scales.dtype != torch.uint8 or scales.shape != (*lead, n):
+            raise RuntimeError(f"{name}: scales must be uint8 {[*lead, n]}, got {scales.dtype} {list(scales.shape)}")
         return self._aligned(codes), self._aligned(scales)
 
     @staticmethod
@@ -635,14 +635,13 @@ class RocmBackend:
         dw, dsc = self._mx4_check("mx4_moe_forward: down", experts[4], experts[5], (E, d), h)
         k = topi.shape[-1]
         lead = x.shape[:-1]
-        if topi.dtype != torch.int64 or topw.dtype != torch.float32 or tuple(topi.shape) != (*lead, k) or \
-                tuple(topw.shape) != (*lead, k):
+        if topi.dtype != torch.int64 or topw.dtype != torch.float32 or topi.shape != (*lead, k) or \
+                topw.shape != topi.shape:
             raise RuntimeError(f"mx4_moe_forward: topi int64 and topw float32 {[*lead, 'k']} expected, got "
                                f"{topi.dtype} {list(topi.shape)} / {topw.dtype} {list(topw.shape)}")
         if not 1 <= k <= min(E, 8) or E > 64:
             raise ValueError(f"mx4_moe_forward: need 1 <= k <= min(E, 8) and E <= 64, got k={k}, E={E}")
-        topi, topw = (t if t.is_contiguous() else t.contiguous() for t in (topi, topw))
-        xc = self._aligned(x)
+        topi, topw, xc = topi.contiguous(), topw.contiguous(), self._aligned(x)
         dev, a, dt = x.device, _lib.ACTS[act], _ACT[x.dtype]
         T = xc.numel() // d
         out = torch.empty(x.shape, dtype=x.dtype, device=dev)
