@@ -247,6 +247,14 @@ class SwiFFN_MoE(nn.Module):
             args["scale"] == 1.0 and not getattr(cfg, "router_bias", False)
         return None if plain and cfg.precision != "mx4" else args
 
+    def _apply(self, fn, *args, **kwargs):
+        kept = self.balance_bias
+        super()._apply(fn, *args, **kwargs)
+        # moves with the layer, but stays fp32: 16 bits would swallow balance_step's steps
+        if kept is not None and self.balance_bias.dtype != kept.dtype and not kept.is_meta:
+            self.balance_bias = kept.to(self.balance_bias.device)
+        return self
+
     @torch.no_grad()
     def balance_step(self, rate: float) -> None:
         """Moves the balance bias by ``rate`` towards the experts that got fewer rows than

@@ -95,3 +95,20 @@ def test_no_fallback_on_host_tensors():
         MX4Linear(64, 8, act="int8")
     with pytest.raises(ValueError):
         mx4.quantize(torch.zeros(3, 4, dtype=torch.int32))
+
+
+def test_balance_bias_stays_fp32():
+    """A cast of the layer leaves the bias' small steps in place; load_state_dict still writes it."""
+    layer = SwiFFN_MoE(MoEConfig(d_model=64, tile=64, num_experts=4, num_experts_per_tok=2, precision="mx4",
+                                 router_bias=True))
+    layer._counts_host = [4, 0, 1, 3]
+    for _ in range(3):
+        layer.balance_step(1e-3)
+    want = torch.tensor([-3e-3, 3e-3, 3e-3, -3e-3])
+    layer.bfloat16()
+    assert layer.gate.weight.dtype == torch.bfloat16 and layer.balance_bias.dtype == torch.float32
+    assert torch.allclose(layer.balance_bias, want, rtol=0, atol=1e-8)  # three sums' half steps
+    other = SwiFFN_MoE(MoEConfig(d_model=64, tile=64, num_experts=4, num_experts_per_tok=2, precision="mx4",
+                                 router_bias=True)).half()
+    other.load_state_dict(layer.state_dict())
+    assert torch.equal(other.balance_bias, layer.balance_bias)
