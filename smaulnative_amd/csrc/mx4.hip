@@ -1520,13 +1520,22 @@ DxParts dx_parts(int64_t rows, int64_t I, int64_t O, int dtype) {
   return q;
 }
 
+// The larger the tile, the less it reads, as long as every CU has one.  us, bf16, by
+// tiles of 128 x 128, 128 x 256 and 256 x 256: 4096 rows 2560 -> 1024 (1, 1/2 and 1/4
+// tiles a CU) 33, 44, 65; 2048 rows 4096 -> 4096 (2, 1, 1/2) 91, 77, 104; 8192 rows (8, 4,
+// 2) 315, 268, 244.  fp32, 512 rows and 1001 rows 777 -> 1000: 30 and 22 of 32 x 64, 31 and
+// 25 of 64 x 64, 41 and 31 of 64 x 128 (half the workgroups of a chip).
 template <int AT, int OT>
 int launch_dx(const Mx4Args& p, hipStream_t stream) {
-  // us, 4096 rows 2560 -> 1024 bf16: 33 of 8 waves, 35.5 of 4; 64 rows x 64 columns 44.
-  // fp32, 512 rows and 1001 rows 777 -> 1000: 30 and 22 of 32 x 64, 31 and 25 of 64 x 64,
-  // 41 and 31 of 64 x 128 (half the workgroups of a chip)
-  if constexpr (AT == A_F32) return launch_gemm_cfg<AT, W_BF16, OT, false, 32, 64, 1, 2, 64, 3>(p, (p.R + 31) / 32, stream);
-  else return launch_gemm_cfg<AT, W_BF16, OT, false, 128, 128, 4, 2, 64, 4>(p, (p.R + 127) / 128, stream);
+  const int64_t cus = cu_count(), mt = (p.R + 127) / 128, nt = (p.N + 255) / 256;
+  if constexpr (AT == A_F32) {
+    return launch_gemm_cfg<AT, W_BF16, OT, false, 32, 64, 1, 2, 64, 3>(p, (p.R + 31) / 32, stream);
+  } else {
+    if ((mt + 1) / 2 * nt >= 2 * cus)
+      return launch_gemm_cfg<AT, W_BF16, OT, false, 256, 256, 4, 2, 64, 2>(p, (mt + 1) / 2, stream);
+    if (mt * nt >= cus) return launch_gemm_cfg<AT, W_BF16, OT, false, 128, 256, 2, 4, 64, 3>(p, mt, stream);
+    return launch_gemm_cfg<AT, W_BF16, OT, false, 128, 128, 4, 2, 64, 4>(p, mt, stream);
+  }
 }
 
 }  // namespace

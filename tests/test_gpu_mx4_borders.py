@@ -1,4 +1,4 @@
-"""The 4-bit products with infinities and NaN among the activations, and values of all of a type's bits."""
+"""The 4-bit products with infinities and NaN among the activations, values of all of a type's bits, and many rows."""
 import math
 
 import pytest
@@ -77,3 +77,17 @@ def test_fp32_activations_keep_all_their_bits(rows):
     w, s = ref.quantize(torch.eye(K))
     got = get_backend("rocm").mx4_forward(x.to(DEV), w.to(DEV), s.to(DEV), K, K)
     assert torch.equal(got.cpu(), x)
+
+
+@pytest.mark.parametrize("rows,K,N", [(4200, 2049, 160), (8230, 4090, 96)])  # both larger tiles of the gradient
+def test_large_gradient(rows, K, N):
+    gen = torch.Generator().manual_seed(rows)
+    w, s = ref.weight(N, K, gen)
+    g = torch.randn(rows, N, generator=gen).to(BF)
+    got = get_backend("rocm").mx4_backward_input(g.to(DEV), w.to(DEV), s.to(DEV), K, N).cpu()
+    some = torch.cat([torch.arange(40), torch.arange(rows - 300, rows)])
+    wv = ref.values(w, s, K)
+    want = g[some].double() @ wv
+    # N products summed in fp32, and half a step of bf16
+    tol = N * 2.0 ** -24 * (g[some].double().abs() @ wv.abs()) + 2.0 ** -8 * want.abs()
+    assert ((got[some].double() - want).abs() <= tol + 1e-37).all()
