@@ -410,6 +410,7 @@ struct Mx4Args {
   const int32_t* seg_off;  // null: dense, R rows of one expert
   const int32_t* tile_off;
   int E;
+  int tile;                // the larger products: which of the kernels' tiles
   int xvec;                // mx4_stream_kernel: x rows may be read 16 bytes at a time,
   int svec;                // and four scales of W
 };
@@ -1420,19 +1421,72 @@ int launch_quantize(const void* x, int dtype, uint8_t* codes, uint8_t* scales, i
   return check_launch("mx4_quantize_kernel");
 }
 
-// up to this many rows (tokens of a layer) mx4_stream_kernel, past them mx4_gemm_kernel
-int64_t gemm_bm(int at) { return at == A_F32 ? 32 : at == A_MX4 ? 256 : 128; }  // its row tiles
+// Up to ST_ROWS rows (tokens of a layer) mx4_stream_kernel runs, past them the larger
+// products, in tiles that fill the chip: what a tile takes (of 256 x 256 = 100, with
+// every CU at work), times the rounds of the CUs.  The last parts of the experts'
+// segments count for half a tile.  us, by tiles of 256 x 256, 128 x 256, 128 x 128 and
+// 64 x 128, rounded activations: 512 x 4096 -> 4096 34, 24, 20, 18; 1500 rows 39, 30, 36,
+// 43; 16384 x 1024 -> 2560 47, 49, -, -; 512 tokens to 2 of 8 experts, 1024 by 2560, 53, 44,
+// 44, 48.  bf16 as it is, 128 x 256 and 64 x 128: 512 rows 58, 31; 1500 rows 65, 65; 16384 x
+// 1024 -> 2560 80, 114.
+struct Mx4Tile {
+  int bm, bn, cost;
+};
+constexpr Mx4Tile CODES_TILES[] = {{256, 256, 100}, {128, 256, 62}, {128, 128, 35}, {64, 128, 27}};
+constexpr Mx4Tile BF16_TILES[] = {{128, 256, 62}, {64, 128, 22}};
+constexpr Mx4Tile F32_TILES[] = {{32, 256, 100}};
+
+struct Mx4Shape {  // of one product
+  int64_t R, K, cols;
+  bool swiglu;
+};
+
+int64_t tile_bm(int at, int tile) {
+  return at == A_F32 ? F32_TILES[tile].bm : at == A_MX4 ? CODES_TILES[tile].bm : BF16_TILES[tile].bm;
+}
+
+// the tile for products that share their row tiles, `parts` experts
+template <int N, int M>
+int pick_tile(const Mx4Tile (&tiles)[N], const Mx4Shape (&products)[M], int64_t parts) {
+  const int64_t cus = cu_count();
+  int best = 0;
+  double least = 0.0;
+  for (int i = 0; i < N; ++i) {
+    double cost = 0.0;
+    for (const Mx4Shape& q : products) {
+      const int64_t bn = q.swiglu ? tiles[i].bn / 2 : tiles[i].bn;
+      const int64_t m = (q.R + tiles[i].bm - 1) / tiles[i].bm + parts / 2, n = (q.cols + bn - 1) / bn;
+      cost += (double)((m * n + cus - 1) / cus) * (double)q.K * tiles[i].cost;
+    }
+    if (i == 0 || cost < least) {
+      best = i;
+      least = cost;
+    }
+  }
+  return best;
+}
+template <int M>
+int pick_tile(int at, const Mx4Shape (&products)[M], int64_t parts) {
+  return at == A_F32 ? 0 : at == A_MX4 ? pick_tile(CODES_TILES, products, parts)
+                                       : pick_tile(BF16_TILES, products, parts);
+}
 
 template <int AT, int OT, bool SWIGLU>
 int launch_product(const Mx4Args& p, const Mx4Slots* few, int64_t m_tiles, hipStream_t stream) {
   if (few) return launch_stream<AT, OT, SWIGLU>(p, *few, stream);
   // us, fp32, 4096 x 1024 -> 2560 and 3001 x 1000 -> 777: 77 and 47 of 32 x 256, 84 and 50
   // of 64 x 256, 87 and 47 of 64 x 128, 91 and 42 of 32 x 128
-  if constexpr (AT == A_F32)
+  if constexpr (AT == A_F32) {
     return launch_gemm_cfg<AT, W_MX4, SWIGLU ? O_PLANES : OT, SWIGLU, 32, 256, 1, 4, 64, 2>(p, m_tiles, stream);
-  else if constexpr (AT == A_BF16)
-    return launch_gemm_cfg<AT, W_MX4, OT, SWIGLU, 128, 256, 2, 2, 64, 3>(p, m_tiles, stream);
-  else return launch_codes<OT, SWIGLU, 256, 256, 4, 2>(p, m_tiles, stream);
+  } else if constexpr (AT == A_BF16) {
+    if (p.tile == 0) return launch_gemm_cfg<AT, W_MX4, OT, SWIGLU, 128, 256, 2, 2, 64, 3>(p, m_tiles, stream);
+    return launch_gemm_cfg<AT, W_MX4, OT, SWIGLU, 64, 128, 2, 2, 64, 3>(p, m_tiles, stream);
+  } else {
+    if (p.tile == 0) return launch_codes<OT, SWIGLU, 256, 256, 4, 2>(p, m_tiles, stream);
+    if (p.tile == 1) return launch_codes<OT, SWIGLU, 128, 256, 2, 4>(p, m_tiles, stream);
+    if (p.tile == 2) return launch_codes<OT, SWIGLU, 128, 128, 2, 2>(p, m_tiles, stream);
+    return launch_codes<OT, SWIGLU, 64, 128, 2, 2>(p, m_tiles, stream);
+  }
 }
 
 // activations with a weight: y of `out` type
@@ -1632,8 +1686,10 @@ int smaul_mx4_linear(const void* x, int dtype, const uint8_t* w, const uint8_t* 
   }
   if (rc) return rc;
   const Mx4Slots few{};
-  return launch_linear(p, at, bf16 ? O_BF16 : O_F32, q.gemm ? nullptr : &few, (rows + gemm_bm(at) - 1) / gemm_bm(at),
-                       stream);
+  const Mx4Shape shape[] = {{rows, in_f, out_f, false}};
+  p.tile = pick_tile(at, shape, 0);
+  const int64_t bm = tile_bm(at, p.tile);
+  return launch_linear(p, at, bf16 ? O_BF16 : O_F32, q.gemm ? nullptr : &few, (rows + bm - 1) / bm, stream);
 }
 
 int64_t smaul_mx4_backward_input_workspace_size(int64_t rows, int64_t in_f, int64_t out_f, int dtype) {
@@ -1762,7 +1818,9 @@ int smaul_mx4_moe_forward(const void* x, int dtype, const int64_t* topi, const f
   const int at = mx4 ? A_MX4 : bf16 ? A_BF16 : A_F32;
   const int64_t R = T * k, gd = mx4_groups(d), gh = mx4_groups(h);
   const bool pd = d % MX4_STAGE != 0, ph = h % MX4_STAGE != 0;
-  const int64_t bm = gemm_bm(at), m_tiles = (R + bm - 1) / bm + E;
+  const Mx4Shape shapes[] = {{R, d, h, true}, {R, h, d, false}};
+  const int tile = pick_tile(at, shapes, E);
+  const int64_t bm = tile_bm(at, tile), m_tiles = (R + bm - 1) / bm + E;
   if (q.gemm && !(mx4 || T * (pd || !bf16 ? gd * MX4_GROUP : d) * (bf16 ? 2 : 6) < (1LL << 32)))
     return fail(SMAUL_ERR_UNSUPPORTED, "mx4_moe: more than 4 GiB of x");
   if (mx4 && T * gd * 64 >= (1LL << 32)) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_moe: more than 4 GiB of codes of x");
@@ -1787,6 +1845,7 @@ int smaul_mx4_moe_forward(const void* x, int dtype, const int64_t* topi, const f
   p.seg_off = seg_off;
   p.tile_off = tile_off;
   p.E = (int)E;
+  p.tile = tile;
   p.xvec = d % 8 == 0;
   Mx4Args dn = p;
   dn.x = p.y;

@@ -91,3 +91,21 @@ def test_large_gradient(rows, K, N):
     # N products summed in fp32, and half a step of bf16
     tol = N * 2.0 ** -24 * (g[some].double().abs() @ wv.abs()) + 2.0 ** -8 * want.abs()
     assert ((got[some].double() - want).abs() <= tol + 1e-37).all()
+
+
+@pytest.mark.parametrize("rows,N", [(100, 500), (1100, 900), (1500, 4090), (4100, 4500)])
+@pytest.mark.parametrize("act", ["keep", "mx4"])
+def test_linear_of_every_tile(rows, N, act):
+    """Rows and columns of the products' different tiles, ending inside one."""
+    gen = torch.Generator().manual_seed(rows + N)
+    K = 200
+    w, s = ref.weight(N, K, gen)
+    x = torch.randn(rows, K, generator=gen).to(BF)
+    got = get_backend("rocm").mx4_forward(x.to(DEV), w.to(DEV), s.to(DEV), K, N, act).cpu()
+    some = torch.cat([torch.arange(40), torch.arange(rows - 60, rows)])
+    xv = ref.rounded(x[some]) if act == "mx4" else x[some].double()
+    wv = ref.values(w, s, K)
+    want = xv @ wv.t()
+    # K products summed in fp32, and half a step of bf16
+    tol = K * 2.0 ** -24 * (xv.abs() @ wv.abs().t()) + 2.0 ** -8 * want.abs()
+    assert ((got[some].double() - want).abs() <= tol + 1e-37).all()
