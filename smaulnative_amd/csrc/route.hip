@@ -344,14 +344,31 @@ __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
       key[v] &= (uint32_t)__builtin_amdgcn_sbfe((int)word, g & 31, 1);
     }
   }
-  // Lane j gets the j-th highest, and its key.  A lane's highest goes out of its keys
-  // without a comparison: of key and key - gone the lower is 0 for it alone (~0u: none).
+  // Lane j gets the j-th highest, and its key.  A lane's keys are lists of four in order,
+  // so that a round looks at their heads alone, and a list whose head is gone moves up.
+  constexpr int L = V < 4 ? V : 4;
+  auto order = [&](int a, int b) {
+    const uint32_t high = max(key[a], key[b]), low = min(key[a], key[b]);
+    key[a] = high;
+    key[b] = low;
+  };
+#pragma unroll
+  for (int v = 0; v < V; v += L) {
+    if constexpr (L == 2) order(v, v + 1);
+    if constexpr (L == 4) {
+      order(v, v + 1);
+      order(v + 2, v + 3);
+      order(v, v + 2);
+      order(v + 1, v + 3);
+      order(v + 1, v + 2);
+    }
+  }
   int mine = -1;
   uint32_t val = 0u, best = 0u;
   auto highest = [&]() {  // the lane's; best: the token's
     uint32_t own = key[0];
 #pragma unroll
-    for (int v = 1; v < V; ++v) own = max(own, key[v]);
+    for (int v = L; v < V; v += L) own = max(own, key[v]);
     best = own;
     SMAUL_ROW_REDUCE(best, op_umax);
     return own;
@@ -364,9 +381,13 @@ __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
       val = best;
       mine = (int)(LOW - (best & LOW)) * 16 + owner;
     }
-    const uint32_t gone = l == owner ? best : ~0u;
+    const uint32_t gone = l == owner ? best : 1u;  // 1: no key (a live one is over 2^22)
 #pragma unroll
-    for (int v = 0; v < V; ++v) key[v] = min(key[v], key[v] - gone);
+    for (int v = 0; v < V; v += L) {
+      const bool up = key[v] == gone;
+#pragma unroll
+      for (int j = 0; j < L; ++j) key[v + j] = up ? (j + 1 < L ? key[v + j + 1] : 0u) : key[v + j];
+    }
   };
   for (int j = 0; j < p.k; ++j) {
     const uint32_t own = highest();
