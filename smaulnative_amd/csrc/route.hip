@@ -218,6 +218,15 @@ __device__ __forceinline__ float route_score(float z, int sigmoid, float m, floa
   return sigmoid ? __builtin_amdgcn_rcpf(1.0f + route_exp(-z)) : route_exp(z - m) * inv;
 }
 
+// floats as integers of the same order
+__device__ __forceinline__ uint32_t route_key(float f) {
+  const uint32_t u = __float_as_uint(f);
+  return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float route_unkey(uint32_t k) {
+  return __uint_as_float(k >> 31 ? k ^ 0x80000000u : ~k);
+}
+
 template <int V>
 __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
   constexpr uint32_t LOW = V - 1;
@@ -225,18 +234,28 @@ __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
   // route_row64's doubles, or the c of the wave's four tokens
   constexpr int SH = 4 * (V * 16 + 8) / 2 > ROUTE_MAX_E ? 4 * (V * 16 + 8) / 2 : ROUTE_MAX_E;
   __shared__ double sh64[ROUTE_WAVES][SH];
-  __shared__ float shg[ROUTE_TOK][ROUTE_MAX_G];
+  __shared__ uint32_t shg[ROUTE_TOK][ROUTE_MAX_G];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, tq = lane >> 4;
   const int64_t t = (int64_t)blockIdx.x * ROUTE_TOK + threadIdx.x / 16;
   const bool on = t < p.T;
   const int64_t row = (on ? t : p.T - 1) * p.E;  // lanes past the end follow along, and store nothing
   float z[V], s[V], b[V];
+  // whole sixteens, known to all lanes, need no comparison in each
+  auto each = [&](auto f, auto past) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = v * 16 + l;
-    z[v] = e < p.E ? route_load(p.z, row + e, p.bf16) + 0.0f : -INF;  // -0 is 0: a tie
-    b[v] = p.bias && e < p.E ? p.bias[e] : 0.0f;
+    for (int v = 0; v < V; ++v) {
+      if ((v + 1) * 16 <= p.E || v * 16 + l < p.E) f(v);
+      else past(v);
+    }
+  };
+  if (p.bf16) {
+    const uint16_t* at = (const uint16_t*)p.z + row + l;
+    each([&](int v) { z[v] = bf2f(at[v * 16]); }, [&](int v) { z[v] = -INF; });
+  } else {
+    const float* at = (const float*)p.z + row + l;
+    each([&](int v) { z[v] = at[v * 16]; }, [&](int v) { z[v] = -INF; });
   }
+  if (p.bias) each([&](int v) { b[v] = p.bias[l + v * 16]; }, [&](int v) { b[v] = 0.0f; });
   float m = -INF, inv = 1.0f;
   if (!p.sigmoid) {
 #pragma unroll
@@ -256,21 +275,24 @@ __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
     for (int v = 0; v < V; ++v) s[v] = route_score(z[v], 1, 0.0f, 0.0f);
   }
   if (p.prob && on) {
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (v * 16 + l < p.E) p.prob[row + v * 16 + l] = s[v];
+    float* at = p.prob + row + l;
+    each([&](int v) { at[v * 16] = s[v]; }, [](int) {});
   }
   // Error of a c: the sum's V + 4 roundings and the exponential's, on scores of at
   // most s_top (the row's highest), and the rounding of c itself.
   const float s_err = (p.sigmoid ? 1.0f : inv) * (V + 16) * 0x1p-24f;
   uint32_t key[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const float c = p.bias ? s[v] + b[v] : s[v];
+  auto judge = [&](int v, float c, float by) {  // by: what the choice goes by
     const bool live = z[v] > -INF && c > -INF;
     s[v] = live ? c : -INF;  // from here on: c
-    const uint32_t u = __float_as_uint(p.bias ? c : z[v]);
-    key[v] = live ? ((u ^ ((uint32_t)((int)u >> 31) | 0x80000000u)) & ~LOW) | (LOW - v) : 0u;
+    key[v] = live ? (route_key(by) & ~LOW) | (LOW - v) : 0u;
+  };
+  if (p.bias) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) judge(v, s[v] + b[v], s[v] + b[v]);
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) judge(v, s[v], z[v] + 0.0f);  // -0 is 0: a tie
   }
   bool again = false;
   if (p.top_groups < p.groups) {
@@ -281,13 +303,13 @@ __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
     for (int v = 0; v < V; ++v) sc[v * 16 + l] = s[v];
     wave_sync();
     const int per = p.E / p.groups;
-    float* sg = shg[wave * 4 + tq];
+    uint32_t* sg = shg[wave * 4 + tq];  // the groups' scores, ordered as integers
     float top = 0.0f;
     for (int g = l; g < p.groups; g += 16) {
       float b1 = -INF, b2 = -INF;
       auto take = [&](float c) {
         b2 = __builtin_amdgcn_fmed3f(b1, b2, c);
-        b1 = fmaxf(b1, c);
+        asm("v_max_f32 %0, %1, %2" : "=v"(b1) : "v"(b1), "v"(c));  // fmaxf makes its operands canonical first
       };
       // each lane from another place on: other banks
       if (per % 4 == 0) {
@@ -308,7 +330,7 @@ __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
         }
       }
       const float score = p.group_best == 2 && b2 > -INF ? b1 + b2 : b1;
-      sg[g] = score;
+      sg[g] = route_key(score + 0.0f);
       if (b1 > -INF) top = fmaxf(top, fmaxf(fabsf(b1), fabsf(score)));
     }
     wave_sync();
@@ -318,12 +340,10 @@ __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
       const int g = g0 + l;
       bool chosen = false;
       if (g < p.groups) {
-        const float mine = sg[g];
+        const uint32_t own = sg[g];
+        const float mine = route_unkey(own);
         int ahead = 0;
-        for (int o = 0; o < p.groups; ++o) {
-          const float other = sg[o];
-          ahead += other > mine || (other == mine && o < g);
-        }
+        for (int o = 0; o < p.groups; ++o) ahead += sg[o] + (o < g ? 1u : 0u) > own;  // ties: the first
         chosen = ahead < p.top_groups;
         if (chosen) lowest = fminf(lowest, mine);
         else highest = fmaxf(highest, mine);
@@ -335,13 +355,18 @@ __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
     top = row_max(top);
     // groups without a live expert may change places
     again = highest > -INF && lowest - highest <= 4.0f * s_err + 8.0f * 0x1p-24f * top;
-    const uint32_t magic = ((1u << 20) + per - 1) / per;  // e / per for e, per <= 512
     const uint32_t in0 = (uint32_t)in, in1 = (uint32_t)(in >> 32);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const uint32_t g = (v * 16 + l) * magic >> 20;
+    auto keep = [&](int v, uint32_t g) {
       const uint32_t word = p.groups > 32 && g >= 32 ? in1 : in0;
       key[v] &= (uint32_t)__builtin_amdgcn_sbfe((int)word, g & 31, 1);
+    };
+    const uint32_t magic = ((1u << 20) + per - 1) / per;  // e / per for e, per <= 512
+    if (per % 16 == 0) {  // a sixteen is of one group
+#pragma unroll
+      for (int v = 0; v < V; ++v) keep(v, v * 16u * magic >> 20);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) keep(v, (v * 16 + l) * magic >> 20);
     }
   }
   // Lane j gets the j-th highest, and its key.  A lane's keys are lists of four in order,
@@ -400,8 +425,7 @@ __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
     const uint32_t ua = a & ~LOW, ub = b & ~LOW;
     if (b == 0u) return false;
     if (!p.bias) return !p.bf16 && ua == ub;  // logits that the low bits may tell apart
-    const float fa = __uint_as_float(ua >> 31 ? ua ^ 0x80000000u : ~ua);
-    const float fb = __uint_as_float(ub >> 31 ? ub ^ 0x80000000u : ~ub);
+    const float fa = route_unkey(ua), fb = route_unkey(ub);
     // each c is off by s_err and half a unit, the second may gain V units by its low bits
     return !(fa - fb > 2.0f * s_err + (V + 2) * 0x1p-23f * fmaxf(fabsf(fa), fabsf(fb)));
   };
