@@ -170,16 +170,17 @@ __device__ __forceinline__ void route_row64(const RouteArgs& p, int64_t t, int l
 // forward: 16 lanes a token, expert 16 v + lane in register v
 // ---------------------------------------------------------------------------
 // The scores are fp32.  An expert's key is one word: its c (or logit) as an ordered
-// integer, the lowest bits replaced by V - 1 - v.  The highest key left is V / 2
-// three-way maxima and four lane exchanges; its low bits say which v, the lowest lane
-// that has it which expert: equal values come out in the order of their index.
+// integer, the lowest bits replaced by V - 1 - v.  The highest key left is a maximum
+// over the heads of a lane's lists and four lane exchanges; its low bits say which v, the
+// lowest lane that has it which expert: equal values come out in the order of their index.
 //
 // What the rounding of the scores or those lost bits could change is not decided in 32
 // bits: experts closer than the error bound are ordered by their c in 64 bits among
 // the few found, and where two groups (the last one in, the first one out) or the
 // scores of a softmax with a bias are that close, the token is done again by
-// route_row64.  In 64 bits throughout, one wave a token, 65536 tokens by 256 experts
-// took 225 us.
+// route_row64.  What bounds it is the vector instructions, about 1300 for four tokens of
+// 256 experts: 65536 tokens take 47 us (their bytes 30), 225 in 64 bits throughout, one
+// wave a token.
 constexpr int ROUTE_WAVES = 4, ROUTE_TOK = ROUTE_WAVES * 4;
 
 template <int CTRL>
@@ -287,14 +288,20 @@ __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
     s[v] = live ? c : -INF;  // from here on: c
     key[v] = live ? (route_key(by) & ~LOW) | (LOW - v) : 0u;
   };
-  if (p.bias) {
+  if constexpr (V > 16) {  // the registers of both loops would cost more waves than they save
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float c = p.bias ? s[v] + b[v] : s[v];
+      judge(v, c, p.bias ? c : z[v] + 0.0f);
+    }
+  } else if (p.bias) {
 #pragma unroll
     for (int v = 0; v < V; ++v) judge(v, s[v] + b[v], s[v] + b[v]);
   } else {
 #pragma unroll
     for (int v = 0; v < V; ++v) judge(v, s[v], z[v] + 0.0f);  // -0 is 0: a tie
   }
-  bool again = false;
+  bool tied = false;  // groups in and out too near
   if (p.top_groups < p.groups) {
     // c to LDS, a group to a lane; the groups' scores to LDS, and each lane counts
     // the groups ahead of its own
@@ -354,7 +361,7 @@ __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
     highest = row_max(highest);
     top = row_max(top);
     // groups without a live expert may change places
-    again = highest > -INF && lowest - highest <= 4.0f * s_err + 8.0f * 0x1p-24f * top;
+    tied = highest > -INF && lowest - highest <= 4.0f * s_err + 8.0f * 0x1p-24f * top;
     const uint32_t in0 = (uint32_t)in, in1 = (uint32_t)(in >> 32);
     auto keep = [&](int v, uint32_t g) {
       const uint32_t word = p.groups > 32 && g >= 32 ? in1 : in0;
@@ -431,12 +438,48 @@ __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
   };
   // lane j: the j-th and the one before; lane 0: the last and the next that is left out
   uint32_t own = highest();
-  const uint32_t before = (uint32_t)__shfl((int)val, l == 0 ? p.k - 1 : l - 1, 16);
+  const int from = l == 0 ? p.k - 1 : l - 1;
+  const uint32_t before = (uint32_t)__shfl((int)val, from, 16);
   const bool close = l < p.k && too_near(before, l == 0 ? best : val);
-  const uint32_t closes = (uint32_t)(__ballot(close) >> (tq * 16)) & 0xffffu;
-  bool near = closes != 0u;
+  bool again = tied, near = false, on_and_on = false;
+  if (__ballot(close || tied)) {
+    // Experts of one logit and one bias are equal in 64 bits too, and stand in the order
+    // of their indices as it is: a batch's padding, whose experts are all the same, needs
+    // no second look (512 rows of it took 20 us of 25).
+    const float zm = mine >= 0 ? route_load(p.z, row + mine, p.bf16) : 0.0f;
+    const float bm = p.bias && mine >= 0 ? p.bias[mine] : 0.0f;
+    const bool differ = !(zm == __shfl(zm, from, 16) && bm == __shfl(bm, from, 16));
+    auto any = [&](bool q) { return ((uint32_t)(__ballot(q) >> (tq * 16)) & 0xffffu) != 0u; };
+    near = any(close && l > 0 && differ);
+    // the last that is chosen, and the next
+    const float zr = __shfl(zm, p.k - 1, 16), br = __shfl(bm, p.k - 1, 16);
+    const bool border = any(close && l == 0);
+    bool even = false;
+    if (border) {  // best is no 0
+      const int next = (int)(LOW - (best & LOW)) * 16 +
+                       __builtin_ctz((uint32_t)(__ballot(own == best) >> (tq * 16)) & 0xffffu);
+      even = route_load(p.z, row + next, p.bf16) == zr && (!p.bias || p.bias[next] == br);
+    }
+    // Where they are equal: is any other expert near them?  And where groups tie: is
+    // any expert other than the chosen, which are all equal?
+    const bool scan = even || (tied && !any(l > 0 && l < p.k && differ));
+    const uint32_t ur = (uint32_t)__shfl((int)val, p.k - 1, 16) & ~LOW;
+    const float fr = route_unkey(ur);
+    bool other = false, uneven = false;
+    for (int e = __ballot(scan) ? l : p.E; e < p.E; e += 16) {
+      const float z = route_load(p.z, row + e, p.bf16) + 0.0f, be = p.bias ? p.bias[e] : 0.0f;
+      if (z == zr && be == br) continue;
+      uneven = true;
+      const float c = p.bias ? route_score(z, p.sigmoid, m, inv) + be : z;
+      // twice too_near's bound, on either side
+      other |= p.bias ? !(fabsf(fr - c) > 4.0f * s_err + (2 * V + 4) * 0x1p-23f * fmaxf(fabsf(fr), fabsf(c)))
+                      : (route_key(c) & ~LOW) == ur;
+    }
+    on_and_on = border && (!even || any(other));
+    near |= on_and_on;
+    again = tied && (!scan || any(uneven));
+  }
   // the walk goes on past k while the next is too near to the last to be left out
-  bool on_and_on = (closes & 1u) != 0u;
   uint32_t last = best;
   for (int j = p.k; __ballot(on_and_on); ++j) {
     if (on_and_on && j == 16) {  // more of them than lanes
