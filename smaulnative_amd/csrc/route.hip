@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
   // most s_top (the row's highest), and the rounding of c itself.
   const float s_err = (p.sigmoid ? 1.0f : inv) * (V + 16) * 0x1p-24f;
   uint32_t key[V];
-  auto judge = [&](int v, float c, float by) {  // by: what the choice goes by
+  auto set_key = [&](int v, float c, float by) {  // by: what the choice goes by
     const bool live = z[v] > -INF && c > -INF;
     s[v] = live ? c : -INF;  // from here on: c
     key[v] = live ? (route_key(by) & ~LOW) | (LOW - v) : 0u;
@@ -292,14 +292,14 @@ __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const float c = p.bias ? s[v] + b[v] : s[v];
-      judge(v, c, p.bias ? c : z[v] + 0.0f);
+      set_key(v, c, p.bias ? c : z[v] + 0.0f);
     }
   } else if (p.bias) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) judge(v, s[v] + b[v], s[v] + b[v]);
+    for (int v = 0; v < V; ++v) set_key(v, s[v] + b[v], s[v] + b[v]);
   } else {
 #pragma unroll
-    for (int v = 0; v < V; ++v) judge(v, s[v], z[v] + 0.0f);  // -0 is 0: a tie
+    for (int v = 0; v < V; ++v) set_key(v, s[v], z[v] + 0.0f);  // -0 is 0: a tie
   }
   bool tied = false;  // groups in and out too near
   if (p.top_groups < p.groups) {
@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(ROUTE_WAVES * 64) route_kernel(RouteArgs p) {
   if (mine >= 0) w = route_score(route_load(p.z, row + mine, p.bf16), p.sigmoid, m, inv);
   const float total = row_sum(w);
   if (p.renorm && mine >= 0) w = total < ROUTE_MIN_SUM ? 1.0f / n : w / total;
-  // a sum next to the guard's border is the 64-bit form's to judge
+  // a sum next to the guard's border is the 64-bit form's to decide
   if (p.renorm) again |= fabsf(total - ROUTE_MIN_SUM) <= 64 * 0x1p-24f * ROUTE_MIN_SUM;
   if (on && l < p.k) {
     p.topi[t * p.k + l] = mine;
