@@ -1288,6 +1288,115 @@ __global__ void __launch_bounds__(NW * 64) mx4_stream_kernel(Mx4Args p, Mx4Slots
   }
 }
 
+// The input gradient of few rows (up to 64), in one launch: a workgroup has one block of
+// columns, its NW waves a slice of the weight's rows each.  A lane reads 32 codes of one
+// weight row, and the wave turns 64 such rows round through LDS of its own.  The blocks
+// of a line of codes are columns of one XCD, which reads the line once.
+template <int AT, bool VEC, int NW>
+__global__ void __launch_bounds__(NW * 64)
+mx4_dx_stream_kernel(const void* __restrict__ g, const uint8_t* __restrict__ w, const uint8_t* __restrict__ s,
+                     void* __restrict__ dx, int64_t R, int64_t I, int64_t O) {
+  constexpr int U = 2, LD = 72;  // steps of 64 rows read at once; rows of 64 bf16, off the banks' period
+  constexpr int JS = 1024 + 64;  // as mx4_stream_kernel's
+  constexpr int NT = AT == A_F32 ? 3 : 1, OWN = 32 * LD * 2 > 4 * JS ? 32 * LD * 2 : 4 * JS;
+  __shared__ __attribute__((aligned(16))) char sh[NW * OWN];
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t nb = mx4_blocks(I);
+  int64_t b0 = blockIdx.x;
+  {
+    const int64_t full = (int64_t)gridDim.x / 8 * 8;
+    if (b0 < full) b0 = b0 % 8 * (full / 8) + b0 / 8;
+  }
+  uint16_t* own = (uint16_t*)(sh + wave * OWN);
+  const int64_t steps = (O + 63) / 64, per = (steps + NW - 1) / NW;
+  const int64_t lo = min((int64_t)wave * per, steps), hi = min(lo + per, steps);
+
+  for (int64_t r0 = 0; r0 < R; r0 += 32) {  // uniform
+    const int64_t r = min(r0 + l32, R - 1);
+    f32x16_t acc;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+    for (int64_t s0 = lo; s0 < hi; s0 += U) {
+      uint4 wc[U];
+      uint32_t ws[U];
+      float v[U][4][8];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t o = (s0 + u) * 64 + lane;
+        const bool in = s0 + u < hi && o < O;
+        wc[u] = in ? *(const uint4*)(w + (o * nb + b0) * 16) : make_uint4(0, 0, 0, 0);
+        ws[u] = in ? s[o * nb + b0] : 0u;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int64_t c = (s0 + u) * 64 + q * 16 + h * 8;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[u][q][j] = 0.0f;
+          if (s0 + u < hi && c < O) mx4_load8<AT == A_BF16, VEC>(g, r, O, c, v[u][q]);  // VEC: O is a multiple of 8
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (s0 + u >= hi) break;  // uniform
+        const float sc = mx4_scale(ws[u]);
+        const uint32_t c[4] = {wc[u].x, wc[u].y, wc[u].z, wc[u].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint4 d = mx4_decode8(c[k], sc);
+          const uint32_t p[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+          for (int j = 0; j < 8; ++j) own[(8 * k + j) * LD + lane] = (uint16_t)(p[j / 2] >> (16 * (j & 1)));
+        }
+        __builtin_amdgcn_wave_barrier();  // a wave's LDS accesses are done in order
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const bf16x8_t a = *(const bf16x8_t*)&own[mx4_perm(l32) * LD + q * 16 + h * 8];
+          uint4 t[3];
+          if constexpr (AT == A_F32) {
+            mx4_split3(v[u][q], t);
+          } else {
+            const float* x = v[u][q];
+            t[0] = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+          }
+#pragma unroll
+          for (int k = 0; k < NT; ++k)
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8_t, t[k]), acc, 0, 0, 0);
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+    // the waves' sums, in the order of the waves: thread by row, half and quarter, as there
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      *(float4*)(sh + (wave * 4 + c) * JS + lane * 16) =
+          make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
+    __syncthreads();
+    if (tid < 256) {
+      const int row = tid >> 3, half = (tid >> 2) & 1, i = tid & 3;
+      float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int q = 0; q < NW; ++q) {
+        const float4 a = *(const float4*)(sh + (q * 4 + i) * JS + (half * 32 + row) * 16);
+        o[0] += a.x;
+        o[1] += a.y;
+        o[2] += a.z;
+        o[3] += a.w;
+      }
+      const int64_t n = b0 * MX4_BLOCK + half * 16 + i * 4;
+      if (r0 + row < R)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (n + c < I) {
+            const int64_t at = (r0 + row) * I + n + c;
+            if constexpr (AT == A_BF16) ((__bf16*)dx)[at] = (__bf16)o[c];
+            else ((float*)dx)[at] = o[c];
+          }
+    }
+    __syncthreads();
+  }
+}
+
 template <int AT, int OT, bool SWIGLU, int NW>
 int launch_stream_cfg(Mx4Args p, const Mx4Slots& q, int64_t groups, hipStream_t stream) {
   p.svec = mx4_blocks(p.K) % 4 == 0 && aligned(p.s, 4) && (!SWIGLU || aligned(p.s2, 4));
@@ -1560,13 +1669,17 @@ LinearParts linear_parts(int64_t rows, int64_t K, int64_t N, int dtype, int act)
 // (fp32), or padded rows where its width is no whole number of stages.
 struct DxParts {
   int64_t ldo, wt, g, total;
-  bool lay;
+  bool gemm, lay;
 };
 DxParts dx_parts(int64_t rows, int64_t I, int64_t O, int dtype) {
   DxParts q{};
   Parts w;
   q.ldo = mx4_groups(O) * MX4_GROUP;
   const bool f32 = dtype == SMAUL_DTYPE_F32;
+  // fp32's second 32 rows cost another pass over the weight: us, 4096 -> 4000, 32 and 33 rows
+  // as few 25 and 41, by tiles 39 and 39; bf16, 33 and 64 rows, 29 and 31, by tiles 44
+  q.gemm = rows > (f32 ? 32 : ST_ROWS);
+  if (!q.gemm) return q;
   q.lay = f32 || O % 64 != 0;
   q.wt = w.take(I * q.ldo * 2);
   q.g = w.take(q.lay ? rows * q.ldo * (f32 ? 6 : 2) : 0);
@@ -1577,7 +1690,8 @@ DxParts dx_parts(int64_t rows, int64_t I, int64_t O, int dtype) {
 // The larger the tile, the less it reads, as long as every CU has one.  us, bf16, by
 // tiles of 128 x 128, 128 x 256 and 256 x 256: 4096 rows 2560 -> 1024 (1, 1/2 and 1/4
 // tiles a CU) 33, 44, 65; 2048 rows 4096 -> 4096 (2, 1, 1/2) 91, 77, 104; 8192 rows (8, 4,
-// 2) 315, 268, 244.  fp32, 512 rows and 1001 rows 777 -> 1000: 30 and 22 of 32 x 64, 31 and
+// 2) 315, 268, 244.  Of 128 x 128 and 64 x 64: 512 rows 4000 -> 4096 (1/2 and 2 tiles a CU)
+// 48, 42, 1024 rows 57, 69; 256 rows 2560 -> 1024 26, 17.6.  fp32, 512 rows and 1001 rows 777 -> 1000: 30 and 22 of 32 x 64, 31 and
 // 25 of 64 x 64, 41 and 31 of 64 x 128 (half the workgroups of a chip).
 template <int AT, int OT>
 int launch_dx(const Mx4Args& p, hipStream_t stream) {
@@ -1588,7 +1702,9 @@ int launch_dx(const Mx4Args& p, hipStream_t stream) {
     if ((mt + 1) / 2 * nt >= 2 * cus)
       return launch_gemm_cfg<AT, W_BF16, OT, false, 256, 256, 4, 2, 64, 2>(p, (mt + 1) / 2, stream);
     if (mt * nt >= cus) return launch_gemm_cfg<AT, W_BF16, OT, false, 128, 256, 2, 4, 64, 3>(p, mt, stream);
-    return launch_gemm_cfg<AT, W_BF16, OT, false, 128, 128, 4, 2, 64, 4>(p, mt, stream);
+    if (mt * ((p.N + 127) / 128) * 2 > cus)
+      return launch_gemm_cfg<AT, W_BF16, OT, false, 128, 128, 4, 2, 64, 4>(p, mt, stream);
+    return launch_gemm_cfg<AT, W_BF16, OT, false, 64, 64, 2, 2, 64, 4>(p, (p.R + 63) / 64, stream);
   }
 }
 
@@ -1708,10 +1824,18 @@ int smaul_mx4_backward_input(const void* g, int dtype, const uint8_t* w, const u
   if (!aligned(g, 16) || !aligned(dx, 16))
     return fail(SMAUL_ERR_INVALID, "mx4_backward_input: g and dx must be 16-byte aligned");
   const DxParts q = dx_parts(rows, in_f, out_f, dtype);
-  if (workspace_bytes < q.total || !workspace || !aligned(workspace, 256))
+  if (workspace_bytes < q.total || (q.total > 0 && (!workspace || !aligned(workspace, 256))))
     return fail(SMAUL_ERR_INVALID, "mx4_backward_input: workspace %lld < %lld bytes, or unaligned",
                 (long long)workspace_bytes, (long long)q.total);
   const bool bf16 = dtype == SMAUL_DTYPE_BF16;
+  if (!q.gemm) {
+    const int64_t blocks = mx4_blocks(in_f);
+    if (blocks > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_backward_input: too wide a weight");
+    auto* kernel = bf16 ? (out_f % 8 == 0 ? &mx4_dx_stream_kernel<A_BF16, true, 8> : &mx4_dx_stream_kernel<A_BF16, false, 8>)
+                        : (out_f % 8 == 0 ? &mx4_dx_stream_kernel<A_F32, true, 8> : &mx4_dx_stream_kernel<A_F32, false, 8>);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(512), 0, stream, g, w, s, dx, rows, in_f, out_f);
+    return check_launch("mx4_dx_stream_kernel");
+  }
   char* ws = (char*)workspace;
   Mx4Prep f{};
   f.x = g;

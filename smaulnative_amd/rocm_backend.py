@@ -592,10 +592,11 @@ class RocmBackend:
         g, w, s = self._mx4_product_check("mx4_backward_input", "g", g, w, s, in_f, out_f, out_f)
         dx = torch.empty(g.shape[0], in_f, dtype=g.dtype, device=g.device)
         nws = lib.smaul_mx4_backward_input_workspace_size(g.shape[0], in_f, out_f, _ACT[g.dtype])
-        ws = torch.empty(nws, dtype=torch.uint8, device=g.device)
+        ws = torch.empty(nws, dtype=torch.uint8, device=g.device) if nws > 0 else None
         with _device(g.device):
             rc = lib.smaul_mx4_backward_input(g.data_ptr(), _ACT[g.dtype], w.data_ptr(), s.data_ptr(), dx.data_ptr(),
-                                              g.shape[0], in_f, out_f, ws.data_ptr(), nws, _stream_handle(g.device))
+                                              g.shape[0], in_f, out_f, None if ws is None else ws.data_ptr(), nws,
+                                              _stream_handle(g.device))
         _lib.check(rc, "mx4_backward_input")
         return dx
 

@@ -61,10 +61,10 @@ def test_mx4_arguments():
     assert lib.smaul_mx4_backward_input(P, 0, P, P, None, 4, 64, 32, P, 1 << 20, None) == bad
     assert lib.smaul_mx4_backward_input(P, 0, P + 8, P, P, 4, 64, 32, P, 1 << 20, None) == bad
     assert lib.smaul_mx4_backward_input(P + 4, 0, P, P, P, 4, 64, 32, P, 1 << 20, None) == bad
-    need = lib.smaul_mx4_backward_input_workspace_size(4, 64, 32, 0)
-    assert need > 0 and lib.smaul_mx4_backward_input_workspace_size(4, 0, 32, 0) == -1
-    assert lib.smaul_mx4_backward_input(P, 0, P, P, P, 4, 64, 32, P, need - 1, None) == bad
-    assert lib.smaul_mx4_backward_input(P, 0, P, P, P, 4, 64, 32, P + 16, need, None) == bad
+    need = lib.smaul_mx4_backward_input_workspace_size(100, 64, 32, 0)
+    assert need > 0 and lib.smaul_mx4_backward_input_workspace_size(100, 0, 32, 0) == -1
+    assert lib.smaul_mx4_backward_input(P, 0, P, P, P, 100, 64, 32, P, need - 1, None) == bad
+    assert lib.smaul_mx4_backward_input(P, 0, P, P, P, 100, 64, 32, P + 16, need, None) == bad
     assert lib.smaul_mx4_linear(P + 4, 1, P, P, P, 10, 64, 32, 0, None, 0, None) == bad
     size = lib.smaul_mx4_moe_workspace_size(64, 128, 256, 8, 2, 1, 1)
     assert size > 0 and lib.smaul_mx4_moe_workspace_size(64, 128, 0, 8, 2, 1, 1) == -1
