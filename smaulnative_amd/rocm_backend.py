@@ -45,11 +45,15 @@ _ACT = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 _HERE = contextlib.nullcontext()
 
 
+# the current device past torch.cuda's check that HIP is up (a device tensor is at hand)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _device(device):
     """``torch.cuda.device(device)``, or nothing to enter where it is the current
     one already (a device switch and back costs a small call 3 us)."""
     index = device.index
-    return _HERE if index is None or index == torch.cuda.current_device() else torch.cuda.device(index)
+    return _HERE if index is None or index == _current_device() else torch.cuda.device(index)
 
 
 # the handle without a Stream object around it (3 us a call); not a public name
@@ -75,12 +79,15 @@ def _drop_entry(backend_ref, key, entry_ref):
 
 
 def _need_device(name: str, *tensors):
+    dev = None
     for t in tensors:
-        if t is not None and not t.is_cuda:
+        if t is None:
+            continue
+        if not t.is_cuda:
             raise RuntimeError(f"{name}: rocm backend needs HIP device tensors, got {t.device}")
-    dev = tensors[0].device
-    for t in tensors[1:]:
-        if t is not None and t.device != dev:
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
             raise RuntimeError(f"{name}: tensors are on different devices ({dev} vs {t.device})")
 
 
