@@ -198,7 +198,7 @@ mx4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restr
 }
 
 // ---------------------------------------------------------------------------
-// operands of the GEMM (mx4_gemm_kernel), one launch for all of a call's
+// operands of the larger products, one launch for all of a call's
 // ---------------------------------------------------------------------------
 // Scales go to [group of 128 values][row] dwords (four blocks' bytes): a stage's
 // scales of consecutive rows are then whole cache lines (a dword from every row of
@@ -839,11 +839,12 @@ int launch_gemm_cfg(const Mx4Args& p, int64_t m_tiles, hipStream_t stream) {
 // wave has the rest of its stage in registers, so that one barrier frees the buffer for
 // the loads of the stage after the next.
 //
-// One workgroup a CU walks a band of tiles as one sequence of stages: the loads of the
-// next tile's first stages leave during the last of this one and its operands are in
-// registers before the epilogue, which they hide behind.  K of 1024 is four stages: a
-// tile's start, its row indices and first loads, took a quarter of its time (16384 tokens
-// to 2 of 8 experts, 1024 by 2560: 274 us with a workgroup a tile, 248 so).
+// A workgroup (one a CU, two of the smaller tiles) walks a band of tiles as one sequence
+// of stages: the loads of the next tile's first stages leave during the last of this one
+// and its operands are in registers before the epilogue, which they hide behind.  K of
+// 1024 is four stages: a tile's start, its row indices and first loads, took a quarter of
+// its time (16384 tokens to 2 of 8 experts, 1024 by 2560: 274 us with a workgroup a tile,
+// 248 so).
 template <int OT, bool SWIGLU, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(WM * WN * 64, 2) mx4_codes_kernel(Mx4Args p, int m_tiles) {
   constexpr int KS = 256, NSTAGE = 2, STEPS = KS / 64;
@@ -1023,8 +1024,9 @@ int launch_codes(const Mx4Args& p, int64_t m_tiles, hipStream_t stream) {
   if ((BM > BN ? BM : BN) * (p.ldx > p.ldw ? p.ldx : p.ldw) * 16 >= 1LL << 32)
     return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: rows too wide");
   if (tiles > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: too many tiles");
-  const int64_t cus = cu_count();
-  hipLaunchKernelGGL((mx4_codes_kernel<OT, SWIGLU, BM, BN, WM, WN>), dim3((unsigned)(tiles < cus ? tiles : cus)),
+  // as many as LDS holds: 512 tokens to 2 of 8 experts 43 us with one a CU, 40 with two
+  const int64_t wgs = cu_count() * (BM * BN <= 128 * 128 ? 2 : 1);
+  hipLaunchKernelGGL((mx4_codes_kernel<OT, SWIGLU, BM, BN, WM, WN>), dim3((unsigned)(tiles < wgs ? tiles : wgs)),
                      dim3(WM * WN * 64), 0, stream, p, (int)m_tiles);
   return check_launch("mx4_codes_kernel");
 }
@@ -1291,7 +1293,9 @@ __global__ void __launch_bounds__(NW * 64) mx4_stream_kernel(Mx4Args p, Mx4Slots
 // The input gradient of few rows (up to 64), in one launch: a workgroup has one block of
 // columns, its NW waves a slice of the weight's rows each.  A lane reads 32 codes of one
 // weight row, and the wave turns 64 such rows round through LDS of its own.  The blocks
-// of a line of codes are columns of one XCD, which reads the line once.
+// of a line of codes are columns of one XCD, which reads the line once.  Two launches are
+// longer than the work: 1 to 32 bf16 rows 2560 -> 1024 10 to 11.5 us, 25 by way of the
+// turned weight (4000 -> 4096: 15 to 17, 43).
 template <int AT, bool VEC, int NW>
 __global__ void __launch_bounds__(NW * 64)
 mx4_dx_stream_kernel(const void* __restrict__ g, const uint8_t* __restrict__ w, const uint8_t* __restrict__ s,
@@ -1356,7 +1360,8 @@ mx4_dx_stream_kernel(const void* __restrict__ g, const uint8_t* __restrict__ w, 
             mx4_split3(v[u][q], t);
           } else {
             const float* x = v[u][q];
-            t[0] = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+            t[0] = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]),
+                              pack_bf16(x[6], x[7]));
           }
 #pragma unroll
           for (int k = 0; k < NT; ++k)
@@ -1691,8 +1696,9 @@ DxParts dx_parts(int64_t rows, int64_t I, int64_t O, int dtype) {
 // tiles of 128 x 128, 128 x 256 and 256 x 256: 4096 rows 2560 -> 1024 (1, 1/2 and 1/4
 // tiles a CU) 33, 44, 65; 2048 rows 4096 -> 4096 (2, 1, 1/2) 91, 77, 104; 8192 rows (8, 4,
 // 2) 315, 268, 244.  Of 128 x 128 and 64 x 64: 512 rows 4000 -> 4096 (1/2 and 2 tiles a CU)
-// 48, 42, 1024 rows 57, 69; 256 rows 2560 -> 1024 26, 17.6.  fp32, 512 rows and 1001 rows 777 -> 1000: 30 and 22 of 32 x 64, 31 and
-// 25 of 64 x 64, 41 and 31 of 64 x 128 (half the workgroups of a chip).
+// 48, 42, 1024 rows 57, 69; 256 rows 2560 -> 1024 26, 17.6.  fp32, 512 rows 2560 -> 1024 and
+// 1001 rows 777 -> 1000: 30 and 22 of 32 x 64, 31 and 25 of 64 x 64, 41 and 31 of 64 x 128
+// (half the workgroups of a chip).
 template <int AT, int OT>
 int launch_dx(const Mx4Args& p, hipStream_t stream) {
   const int64_t cus = cu_count(), mt = (p.R + 127) / 128, nt = (p.N + 255) / 256;
@@ -1831,8 +1837,10 @@ int smaul_mx4_backward_input(const void* g, int dtype, const uint8_t* w, const u
   if (!q.gemm) {
     const int64_t blocks = mx4_blocks(in_f);
     if (blocks > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_backward_input: too wide a weight");
-    auto* kernel = bf16 ? (out_f % 8 == 0 ? &mx4_dx_stream_kernel<A_BF16, true, 8> : &mx4_dx_stream_kernel<A_BF16, false, 8>)
-                        : (out_f % 8 == 0 ? &mx4_dx_stream_kernel<A_F32, true, 8> : &mx4_dx_stream_kernel<A_F32, false, 8>);
+    const bool vec = out_f % 8 == 0;
+    auto* kernel = bf16  ? (vec ? &mx4_dx_stream_kernel<A_BF16, true, 8> : &mx4_dx_stream_kernel<A_BF16, false, 8>)
+                   : vec ? &mx4_dx_stream_kernel<A_F32, true, 8>
+                         : &mx4_dx_stream_kernel<A_F32, false, 8>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(512), 0, stream, g, w, s, dx, rows, in_f, out_f);
     return check_launch("mx4_dx_stream_kernel");
   }
