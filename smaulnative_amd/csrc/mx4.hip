@@ -1194,23 +1194,24 @@ __global__ void __launch_bounds__(NW * 64) mx4_stream_kernel(Mx4Args p, Mx4Slots
           for (int v = 0; v < 4; ++v) {
             constexpr int NT = AT == A_F32 ? 3 : 1;
             bf16x8_t t[3];
-            const bool in = b * MX4_BLOCK + v * 8 < p.K;  // whole pieces
-            auto piece = [&](int i) {
+            const int64_t c0 = b * MX4_BLOCK + v * 8;
+            // piece i, whose first column is c; rows end with whole pieces, past them zeros
+            auto piece = [&](int i, int64_t c) {
               const uint4 x = *(const uint4*)(own + (l32 * XP + (i ^ (l32 & 15))) * 16);
-              return in ? x : make_uint4(0, 0, 0, 0);
+              return c < p.K ? x : make_uint4(0, 0, 0, 0);
             };
             if constexpr (XL && AT == A_BF16) {
-              t[0] = __builtin_bit_cast(bf16x8_t, piece(u * 8 + g * 4 + v));
+              t[0] = __builtin_bit_cast(bf16x8_t, piece(u * 8 + g * 4 + v, c0));
             } else {
               float f[8];
               if constexpr (XL) {
-                const uint4 a = piece(u * 16 + g * 8 + 2 * v), c = piece(u * 16 + g * 8 + 2 * v + 1);
+                const uint4 a = piece(u * 16 + g * 8 + 2 * v, c0), c = piece(u * 16 + g * 8 + 2 * v + 1, c0 + 4);
                 f[0] = __uint_as_float(a.x); f[1] = __uint_as_float(a.y);
                 f[2] = __uint_as_float(a.z); f[3] = __uint_as_float(a.w);
                 f[4] = __uint_as_float(c.x); f[5] = __uint_as_float(c.y);
                 f[6] = __uint_as_float(c.z); f[7] = __uint_as_float(c.w);
               } else {
-                mx4_load8<AT == A_BF16, false>(p.x, xr, p.K, b * MX4_BLOCK + v * 8, f);
+                mx4_load8<AT == A_BF16, false>(p.x, xr, p.K, c0, f);
               }
               uint4 h[3];
               mx4_split3(f, h);

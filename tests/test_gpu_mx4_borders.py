@@ -109,3 +109,39 @@ def test_linear_of_every_tile(rows, N, act):
     # K products summed in fp32, and half a step of bf16
     tol = K * 2.0 ** -24 * (xv.abs() @ wv.abs().t()) + 2.0 ** -8 * want.abs()
     assert ((got[some].double() - want).abs() <= tol + 1e-37).all()
+
+
+@pytest.mark.parametrize("K", [4, 36, 100])
+@pytest.mark.parametrize("rows", [1, 9, 64, 65])
+def test_infinities_at_the_end_of_a_width_off_eight(rows, K):
+    """fp32 rows that end inside a group of 8 values: an infinity among the last four."""
+    gen = torch.Generator().manual_seed(rows + K)
+    N = 70
+    w, s = ref.weight(N, K, gen)
+    for at in range(K - 4, K):
+        x = torch.randn(rows, K, generator=gen)
+        x[rows // 2, at] = -math.inf if at % 2 else math.inf
+        got = get_backend("rocm").mx4_forward(x.to(DEV), w.to(DEV), s.to(DEV), K, N)
+        want = x.double() @ ref.values(w, s, K).t()
+        assert torch.isinf(want).any()
+        _same_kinds(got, want)
+
+
+@pytest.mark.parametrize("T", [9, 150])
+def test_infinite_hidden_values_at_the_end_of_a_width_off_eight(T):
+    """The same of the experts' hidden rows: the last of 36 overflows fp32."""
+    gen = torch.Generator().manual_seed(T)
+    d, h = 64, 36
+    x = torch.rand(T, d, generator=gen) + 0.5
+    gate, up, down = torch.rand(h, d, generator=gen), torch.rand(h, d, generator=gen), torch.randn(d, h, generator=gen)
+    gate[-1] *= 2.0 ** 70
+    up[-1] *= 2.0 ** 70
+    experts = [t[None] for m in (gate, up, down) for t in ref.quantize(m)]
+    g, u = (x.double() @ ref.values(experts[i][0], experts[i + 1][0], d).t() for i in (0, 2))
+    hid = ref.swiglu(g, u).float()
+    assert torch.isinf(hid[:, -1]).all() and torch.isfinite(hid[:, :-1]).all()
+    want = hid.double() @ ref.values(experts[4][0], experts[5][0], h).t()
+    out, _ = get_backend("rocm").mx4_moe_forward(x.to(DEV), torch.zeros(T, 1, dtype=torch.int64, device=DEV),
+                                                 torch.ones(T, 1, device=DEV), [t.to(DEV) for t in experts])
+    assert torch.isinf(want).any()
+    _same_kinds(out, want)
