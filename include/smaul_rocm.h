@@ -504,7 +504,8 @@ int smaul_swiglu_backward(const void* dout, const void* g, const void* u, void* 
  *   topw = s of the chosen (without the bias); renorm: over their sum (1 / n of the
  *   n chosen where the sum is below 1e-6); times scale.
  * An expert with a logit of -inf, or whose c is -inf or NaN, is not chosen; a slot
- * that no expert fills has topi -1 and topw 0 (smaul_moe_dispatch drops it).
+ * that no expert fills has topi -1 and topw 0 (smaul_moe_dispatch drops it).  The
+ * softmax of a row whose logits are all -inf is NaN, and so is its prob.
  * logits: dtype [T, E]; prob fp32 [T, E] (s) or NULL; topi int64 [T, k]; topw fp32
  * [T, k].  E <= 512, k <= 16, groups <= 64 (a divisor of E), and top_groups groups
  * hold at least k experts.  The choice is that of scores in 64 bits.
@@ -517,7 +518,9 @@ int smaul_moe_route(const void* logits, int dtype, const float* bias, float* pro
 /*
  * Gradient of smaul_moe_route in the logits, from those of topw (fp32 [T, k]) and of
  * prob (fp32 [T, E] or NULL), with the choice topi as a constant.  A slot of -1
- * gives nothing, whatever dtopw holds there; a row renormalised to 1 / n neither.
+ * gives nothing, whatever dtopw holds there; a row renormalised to 1 / n neither.  An
+ * expert with a logit of -inf has a gradient of 0, whatever dprob holds there, also in
+ * a row that has no other.
  * dlogits is of the logits' dtype.
  */
 int smaul_moe_route_backward(const float* dtopw, const void* logits, int dtype, const int64_t* topi,

@@ -452,7 +452,8 @@ class RocmBackend:
         is below 1e-6), times ``scale``.  An expert whose logit is -inf is never
         chosen, nor one whose score or bias is NaN; a slot that no expert fills is
         -1 with weight 0, which the dispatch drops.  The choice is that of scores
-        in 64 bits.  ``prob`` is the scores, None unless ``need_prob``."""
+        in 64 bits.  ``prob`` is the scores, None unless ``need_prob``; the softmax of a
+        row whose logits are all -inf is NaN."""
         lib = _lib.load()
         _need_device("moe_route", logits, bias)
         T, E, top_k = self._route_check("moe_route", logits, top_k, score)
@@ -496,7 +497,8 @@ class RocmBackend:
     def moe_route_backward(self, dtopw, logits, topi, score="softmax", renorm=True, scale=1.0, dprob=None):
         """The gradient of ``moe_route`` in its logits (their type), from that of topw
         ([T, k] fp32) and, if given, of prob ([T, E] fp32); the choice ``topi`` is a
-        constant.  A slot of -1 gives none, whatever dtopw holds there."""
+        constant.  A slot of -1 gives none, whatever dtopw holds there, and an expert with
+        a logit of -inf has none, whatever dprob holds there."""
         lib = _lib.load()
         _need_device("moe_route_backward", logits, dtopw, topi, dprob)
         T, E, k = self._route_check("moe_route_backward", logits, topi.shape[-1] if topi.dim() else 0, score)

@@ -278,3 +278,33 @@ def test_route_refusals():
         be.moe_route_backward(torch.zeros(3, 2, device=DEV), z, topi.int())
     with pytest.raises(RuntimeError):
         be.moe_route_backward(torch.zeros(3, 2, device=DEV), z, topi, dprob=torch.zeros(3, 11, device=DEV))
+
+
+@pytest.mark.parametrize("E", [7, 8, 60, 100, 256, 512])
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_route_gradient_of_rows_without_experts(E, dtype):
+    """A row whose logits are all -inf has no gradient, whatever dtopw and dprob hold, nor
+    has a masked expert, whatever dprob holds there; the others have theirs."""
+    be = get_backend("rocm")
+    logits, gen = _logits(9, E, dtype, E)
+    empty = torch.tensor([0, 4, 8])
+    logits[empty] = -math.inf
+    logits[5, 1:] = -math.inf  # one expert left
+    rest = torch.tensor([t for t in range(9) if t not in empty.tolist()])
+    dtopw, dprob = torch.randn(9, 3, generator=gen), torch.randn(9, E, generator=gen)
+    dtopw[4], dprob[8] = math.nan, math.nan
+    plain = dprob.clone()
+    dprob[5, 2], dprob[5, 3] = math.nan, math.inf
+    plain[5, 2:4] = 0.0
+    for score in ("softmax", "sigmoid"):
+        for renorm in (False, True):
+            topi = be.moe_route(logits.to(DEV), 3, score=score, renorm=renorm)[1]
+            assert (topi[empty] == -1).all()
+            for dp in (None, dprob):
+                got = be.moe_route_backward(dtopw.to(DEV), logits.to(DEV), topi, score=score, renorm=renorm,
+                                            dprob=None if dp is None else dp.to(DEV)).cpu()
+                assert (got[empty] == 0).all()
+                alone = be.moe_route_backward(dtopw[rest].to(DEV), logits[rest].to(DEV), topi[rest].contiguous(),
+                                              score=score, renorm=renorm,
+                                              dprob=None if dp is None else plain[rest].to(DEV))
+                assert torch.isfinite(got).all() and torch.equal(got[rest], alone.cpu())
