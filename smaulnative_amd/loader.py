@@ -20,6 +20,10 @@ the rocm backend's repack cache for each layer (the canonical code copies,
 0x7F/0xFF -> 0x7E/0xFE), so the first forward pays nothing.  The stored
 ``w8`` / ``sc`` are kept unchanged: the cache is refreshed whenever a buffer
 is rewritten in place (requant, kernel/fp8_tile.py:252-253).
+
+The layers loaded are the reference's: tiled-E4M3 experts behind a softmax top-k
+router.  A config with another router (``MoEConfig``'s ``router_*`` fields), a balance
+bias among the tensors, and a module of either kind to load into are refused.
 """
 from __future__ import annotations
 
@@ -27,13 +31,18 @@ import json
 import os
 import re
 from dataclasses import dataclass, field
+from types import SimpleNamespace
 from typing import Dict, List, Optional, Tuple
 
 import torch
 
+from smaulnative_amd.moe import is_plain_router
+from smaulnative_amd.mx4 import MX4Experts
+
 PROJ = ("gate", "up", "down")
 _EXPERT_KEY = re.compile(r"^blocks\.(\d+)\.ffn\.experts\.(\d+)\.(gate|up|down)\.(w8|sc)$")
 _ROUTER_KEY = re.compile(r"^blocks\.(\d+)\.ffn\.gate\.(weight|bias)$")
+_BALANCE_KEY = re.compile(r"^blocks\.\d+\.ffn\.balance_bias$")
 
 
 @dataclass
@@ -65,6 +74,9 @@ def read_config(ckpt_dir) -> dict:
         raise ValueError(f"{ckpt_dir}: the rocm MoE path loads precision='fp8' checkpoints only")
     if cfg.get("architecture", "plain") != "plain":
         raise ValueError(f"{ckpt_dir}: the rocm MoE path loads architecture='plain' checkpoints only")
+    if not is_plain_router(SimpleNamespace(**cfg)):
+        fields = {k: v for k, v in cfg.items() if k.startswith("router_")}
+        raise ValueError(f"{ckpt_dir}: the rocm MoE path loads softmax top-k routers only, got {fields}")
     return cfg
 
 
@@ -94,7 +106,7 @@ def load_moe_layers(ckpt_dir, device="cuda", layers=None, prepare=True) -> List[
     with safe_open(path, framework="pt", device=str(dev)) as f:
         keys = set(f.keys())
         moe_keys = {k for k in keys if _EXPERT_KEY.match(k) or _ROUTER_KEY.match(k)}
-        stray = sorted(k for k in keys - moe_keys if ".ffn.experts." in k)
+        stray = sorted(k for k in keys - moe_keys if ".ffn.experts." in k or _BALANCE_KEY.match(k))
         missing = sorted(set(want) - keys)
         unexpected = sorted(k for k in moe_keys if k not in want and not k.endswith(".ffn.gate.bias"))
         if missing or unexpected or stray:
@@ -137,7 +149,13 @@ def load_moe_layers(ckpt_dir, device="cuda", layers=None, prepare=True) -> List[
 
 
 def load_into(module, layer: MoELayer):
-    """Copy a loaded layer into a SwiFFN_MoE module's router and expert buffers (shapes checked)."""
+    """Copy a loaded layer into a SwiFFN_MoE module's router and expert buffers (shapes checked).
+
+    The module has to be of the layer's kind: tiled-E4M3 experts, softmax top-k router."""
+    if isinstance(module.experts, MX4Experts):
+        raise RuntimeError("module has mx4 experts, layer tiled-E4M3 ones")
+    if getattr(module, "route_args", None) is not None:
+        raise RuntimeError(f"module's router is {module.route_args}, layer's the softmax top-k")
     if len(module.experts) != len(layer.experts):
         raise RuntimeError(f"module has {len(module.experts)} experts, layer {len(layer.experts)}")
     with torch.no_grad():

@@ -68,6 +68,23 @@ class MoEConfig:
                              f"num_experts ({self.num_experts})")
 
 
+def _router_fields(cfg) -> dict:
+    """moe_route's arguments from a config's ``router_*`` fields, unchecked."""
+    args = dict(score=getattr(cfg, "router_score", "softmax"), groups=getattr(cfg, "router_groups", 1),
+                top_groups=getattr(cfg, "router_top_groups", None), group_best=getattr(cfg, "router_group_best", 2),
+                renorm=getattr(cfg, "router_renorm", True), scale=getattr(cfg, "router_scale", 1.0))
+    if args["top_groups"] is None:
+        args["top_groups"] = args["groups"]
+    return args
+
+
+def is_plain_router(cfg) -> bool:
+    """Whether a config's router is the reference's: softmax, top-k, renormalised."""
+    args = _router_fields(cfg)
+    return args["score"] == "softmax" and args["top_groups"] == args["groups"] and bool(args["renorm"]) and \
+        args["scale"] == 1.0 and not getattr(cfg, "router_bias", False)
+
+
 def _needs_grad(module: nn.Module, x: torch.Tensor) -> bool:
     """Whether the forward must record autograd: grad mode on and x or a
     parameter of ``module`` requiring grad, in train and eval mode alike (as
@@ -230,11 +247,7 @@ class SwiFFN_MoE(nn.Module):
         """moe_route's arguments from the config's ``router_*`` fields, or None for the
         reference's router (softmax, top-k, renormalised)."""
         E, k = cfg.num_experts, cfg.num_experts_per_tok
-        args = dict(score=getattr(cfg, "router_score", "softmax"), groups=getattr(cfg, "router_groups", 1),
-                    top_groups=getattr(cfg, "router_top_groups", None), group_best=getattr(cfg, "router_group_best", 2),
-                    renorm=getattr(cfg, "router_renorm", True), scale=getattr(cfg, "router_scale", 1.0))
-        if args["top_groups"] is None:
-            args["top_groups"] = args["groups"]
+        args = _router_fields(cfg)
         if args["score"] not in ("softmax", "sigmoid"):
             raise ValueError(f"router_score must be 'softmax' or 'sigmoid', got {args['score']!r}")
         if args["groups"] < 1 or E % args["groups"] or not 1 <= args["top_groups"] <= args["groups"] or \
@@ -243,9 +256,7 @@ class SwiFFN_MoE(nn.Module):
                              f"({args['top_groups']}) of them hold {k}")
         if args["group_best"] not in (1, 2):
             raise ValueError(f"router_group_best must be 1 or 2, got {args['group_best']!r}")
-        plain = args["score"] == "softmax" and args["top_groups"] == args["groups"] and args["renorm"] and \
-            args["scale"] == 1.0 and not getattr(cfg, "router_bias", False)
-        return None if plain and cfg.precision != "mx4" else args
+        return None if is_plain_router(cfg) and cfg.precision != "mx4" else args
 
     def _apply(self, fn, *args, **kwargs):
         kept = self.balance_bias

@@ -127,3 +127,42 @@ def test_loaded_layer_runs_and_tracks_rewrites(tmp_path):
     r2 = oracle.moe_forward(x.cpu(), l0.gate_weight.cpu(), None, experts2, 2)
     assert float((out2.cpu().double() - r2.out.double()).norm() / r2.out.double().norm()) < 2e-3
     assert not torch.equal(out2, out)
+
+
+@pytest.mark.parametrize("field", [dict(router_score="sigmoid"), dict(router_groups=2, router_top_groups=1),
+                                   dict(router_renorm=False), dict(router_scale=2.5), dict(router_bias=True)])
+def test_other_routers_are_refused(tmp_path, field):
+    """A layer that routes otherwise than by softmax top-k does not load as one that does."""
+    write_ckpt(tmp_path, cfg=dict(CFG, **field))
+    with pytest.raises(ValueError, match="router"):
+        read_config(tmp_path)
+    with pytest.raises(ValueError, match="router"):
+        load_moe_layers(tmp_path, device="cpu", prepare=False)
+
+
+def test_a_balance_bias_is_unexpected(tmp_path):
+    write_ckpt(tmp_path, extra="blocks.1.ffn.balance_bias")
+    with pytest.raises(RuntimeError, match="unexpected.*balance_bias"):
+        load_moe_layers(tmp_path, device="cpu", prepare=False)
+    # fields that say the softmax router in other words
+    write_ckpt(tmp_path, cfg=dict(CFG, router_score="softmax", router_groups=2, router_top_groups=2, router_scale=1.0,
+                                  router_renorm=True, router_bias=False, router_group_best=1))
+    assert len(load_moe_layers(tmp_path, device="cpu", prepare=False)) == 2
+    write_ckpt(tmp_path, cfg=dict(CFG, router_groups=2, router_top_groups=None))
+    assert len(load_moe_layers(tmp_path, device="cpu", prepare=False)) == 2
+
+
+@pytest.mark.parametrize("field,err", [(dict(router_score="sigmoid"), "router"), (dict(router_bias=True), "router"),
+                                       (dict(precision="mx4"), "mx4")])
+def test_load_into_other_layers_is_refused(tmp_path, field, err):
+    from smaulnative_amd import MoEConfig, SwiFFN_MoE
+    write_ckpt(tmp_path)
+    layer = load_moe_layers(tmp_path, device="cpu", prepare=False)[0]
+    base = dict(d_model=CFG["d_model"], ffn_mult=CFG["ffn_mult"], num_experts=4, num_experts_per_tok=2)
+    module = SwiFFN_MoE(MoEConfig(**base, **field))
+    before = {k: v.clone() for k, v in module.state_dict().items()}
+    with pytest.raises(RuntimeError, match=err):
+        load_into(module, layer)
+    assert all(torch.equal(v, before[k]) for k, v in module.state_dict().items())
+    plain = load_into(SwiFFN_MoE(MoEConfig(**base)), layer)
+    assert torch.equal(plain.experts[3].down.w8, layer.experts[3][4])
