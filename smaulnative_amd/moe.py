@@ -68,6 +68,10 @@ class MoEConfig:
                              f"num_experts ({self.num_experts})")
 
 
+# of one call of the backend's layer entries and its dispatch
+_CALL_EXPERTS, _CALL_SLOTS = 64, 8
+
+
 def _router_fields(cfg) -> dict:
     """moe_route's arguments from a config's ``router_*`` fields, unchecked."""
     args = dict(score=getattr(cfg, "router_score", "softmax"), groups=getattr(cfg, "router_groups", 1),
@@ -332,14 +336,43 @@ class SwiFFN_MoE(nn.Module):
         lead, k = x.shape[:-1], self.top_k
         xs = x.reshape(-1, x.shape[-1])
         prob, topi, topw = be.moe_route(self._logits(xs), k, bias=self.balance_bias, **(self.route_args or {}))
-        if isinstance(self.experts, nn.ModuleList):
-            out, prob, topi, counts = be.moe_forward(xs, self.gate.weight, self.gate.bias,
-                                                     [ex.buffers6() for ex in self.experts], k, self.tile,
-                                                     routing=(prob, topi, topw))
+        xs = xs if xs.is_floating_point() else xs.float()
+        fp8 = isinstance(self.experts, nn.ModuleList)
+        if k > _CALL_SLOTS or xs.shape[-1] % 8 or xs.dtype not in (torch.float32, torch.bfloat16) or \
+                not (fp8 or self.experts.act == "keep" or xs.dtype == torch.bfloat16):
+            # what the entries do not take runs expert by expert, as in training (with a
+            # host synchronisation each: not to be captured)
+            out, counts = self._experts_by_mask(xs, topi, topw)
+            out, counts = out.to(xs.dtype), torch.tensor(counts, dtype=torch.int32, device=xs.device)
         else:
-            out, counts = be.mx4_moe_forward(xs if xs.is_floating_point() else xs.float(), topi, topw,
-                                             self.experts.buffers6(), self.experts.act)
+            # More experts than one call takes: equal parts, a call each.  The slots of other
+            # parts are outside [0, E) there and add nothing; the parts' sums, each rounded
+            # to x's type, are added in fp32.
+            parts = -(-self.num_experts // _CALL_EXPERTS)
+            step = -(-self.num_experts // parts)
+            calls = [self._part(be, xs, prob, topi, topw, lo, min(lo + step, self.num_experts))
+                     for lo in range(0, self.num_experts, step)]
+            out, counts = calls[0]
+            if parts > 1:
+                out = sum((part.float() for part, _ in calls[1:]), out.float()).to(xs.dtype)
+                counts = torch.cat([c for _, c in calls])
         return out.view(x.shape), prob.view(*lead, self.num_experts), topi.view(*lead, k), counts
+
+    def _part(self, be, xs, prob, topi, topw, lo, hi):
+        """(out, counts) of the experts lo to hi on a routing among all of them."""
+        whole = hi - lo == self.num_experts
+        topi = topi if whole else topi - lo
+        if not isinstance(self.experts, nn.ModuleList):
+            experts = self.experts.buffers6()
+            return be.mx4_moe_forward(xs, topi, topw, experts if whole else tuple([b[lo:hi] for b in experts]),
+                                      self.experts.act)
+        experts = [ex.buffers6() for ex in self.experts]
+        weight, bias = self.gate.weight, self.gate.bias
+        if not whole:  # of the router's arguments only topi and topw are read
+            weight, bias, experts = weight[lo:hi], None, experts[lo:hi]
+            prob = prob.new_empty(prob.shape[0], hi - lo)
+        out, _, _, counts = be.moe_forward(xs, weight, bias, experts, self.top_k, self.tile, routing=(prob, topi, topw))
+        return out, counts
 
     def _forward_train(self, x):
         """The layer with autograd, for training.
@@ -367,8 +400,8 @@ class SwiFFN_MoE(nn.Module):
         # kept with x's leading dimensions, as the reference's are (model.py:558-565)
         self.last_prob = prob.view(*lead, self.num_experts)
         self.last_topi = topi.detach().view(*lead, self.top_k)
-        if xs.is_cuda and 0 < xs.shape[0] * self.top_k < 1 << 31 and self.num_experts <= 64 and self.top_k <= 8 and \
-                hasattr(get_backend(), "moe_dispatch"):
+        if xs.is_cuda and 0 < xs.shape[0] * self.top_k < 1 << 31 and self.num_experts <= _CALL_EXPERTS and \
+                self.top_k <= _CALL_SLOTS and hasattr(get_backend(), "moe_dispatch"):
             out, counts = self._experts_dispatched(xs, topi, topv)
         else:
             out, counts = self._experts_by_mask(xs, topi, topv)

@@ -198,3 +198,52 @@ def test_experts_are_callable():
     for e in (0, 7):
         want = ref.swiglu(x.double().cpu() @ gate[e].t(), x.double().cpu() @ up[e].t()) @ down[e].t()
         assert _rel(m.experts[e](x), want) <= 1e-5
+
+
+def _plain_by_expert(m, x, topi, topw):
+    """``_plain`` with act "mx4" as it runs expert by expert: gate's and up's products and
+    the hidden rows are of x's type (bf16) before they are rounded to the format."""
+    gate, up, down = _weights(m)
+    out = torch.zeros(x.shape, dtype=torch.float64)
+    xv = ref.rounded(x)
+    for e in range(m.num_experts):
+        tok, slot = (topi == e).nonzero(as_tuple=True)
+        if tok.numel():
+            g, u = ((xv[tok] @ w[e].t()).to(x.dtype).double() for w in (gate, up))
+            hid = ref.rounded(ref.swiglu(g, u).to(x.dtype))
+            out = out.index_add(0, tok, (hid @ down[e].t()) * topw[tok, slot].unsqueeze(1))
+    return out
+
+
+@pytest.mark.parametrize("precision,act,dtype,E,k,d", [
+    ("mx4", "keep", F32, 80, 4, 64), ("mx4", "keep", BF, 160, 6, 64), ("mx4", "mx4", BF, 65, 2, 64), ("fp8", "keep", F32, 80, 4, 64),
+    ("fp8", "keep", BF, 130, 8, 64),                                        # more experts than one call takes
+    ("mx4", "keep", F32, 20, 10, 64), ("fp8", "keep", F32, 80, 10, 64),     # more slots
+    ("mx4", "keep", F32, 8, 2, 36), ("mx4", "mx4", F32, 8, 2, 64)])         # widths and types that it does not take
+@pytest.mark.parametrize("T", [7, 90])
+def test_layers_past_one_call(precision, act, dtype, E, k, d, T):
+    """What a layer takes in training it takes without gradients, and means the same."""
+    groups = 5 if E % 5 == 0 else 2 if E % 2 == 0 else 1
+    m = _layer(T + E, precision=precision, expert_act=act, E=E, k=k, d=d, tile=4 if d == 36 else 64, router_score="sigmoid",
+               router_groups=groups, router_top_groups=max(1, groups - 1), router_scale=2.5, router_bias=True)
+    x = torch.randn(T, d, generator=torch.Generator().manual_seed(T)).to(dtype).to(DEV)
+    with torch.no_grad():
+        out = m(x)
+    topi = m.last_topi.cpu()
+    want = ref.route(m._logits(x).detach().cpu(), k, "sigmoid", m.balance_bias.cpu(), groups, max(1, groups - 1), 2, True, 2.5)
+    assert torch.equal(topi, want[1]) and out.dtype == dtype and out.shape == x.shape
+    counts = m.expert_token_counts
+    assert counts == torch.bincount(topi.flatten(), minlength=E).tolist()
+    plain = _plain(m, x.double().cpu(), topi, want[2], act)
+    # as test_layer_with_the_wider_router; rounded rows whose fp32 values differ in their last
+    # bits may round to other codes, a step of 2^-2 of few values
+    bar = 1e-5 if dtype == F32 and act == "keep" else 6e-3
+    assert _rel(out, plain) <= bar
+    trained = m(x.clone().requires_grad_())
+    if act == "mx4" and dtype == BF:
+        plain = _plain_by_expert(m, x.cpu(), topi, want[2])
+    # in training bf16 also rounds gate's and up's products and each expert's output
+    assert _rel(trained.detach(), plain) <= 2 * bar and m.expert_token_counts == counts
+    with torch.no_grad():
+        wide = m(x.view(1, T, d))
+    assert wide.shape == (1, T, d) and torch.equal(wide.view(T, d), out) and m.last_topi.shape == (1, T, k)
