@@ -25,6 +25,7 @@ scores, groups, a balance bias, no renormalisation, a scale; the backend's
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import torch
@@ -260,7 +261,14 @@ class SwiFFN_MoE(nn.Module):
                              f"({args['top_groups']}) of them hold {k}")
         if args["group_best"] not in (1, 2):
             raise ValueError(f"router_group_best must be 1 or 2, got {args['group_best']!r}")
-        return None if is_plain_router(cfg) and cfg.precision != "mx4" else args
+        if is_plain_router(cfg) and cfg.precision != "mx4":
+            return None
+        if not 0.0 < args["scale"] < math.inf:
+            raise ValueError(f"router_scale must be positive and finite, got {args['scale']!r}")
+        if E > 512 or k > 16 or args["groups"] > 64:
+            raise ValueError(f"the router takes up to 512 experts, 16 a token and 64 groups, got {E}, {k} and "
+                             f"{args['groups']}")
+        return args
 
     def _apply(self, fn, *args, **kwargs):
         kept = self.balance_bias

@@ -112,3 +112,25 @@ def test_balance_bias_stays_fp32():
                                  router_bias=True)).half()
     other.load_state_dict(layer.state_dict())
     assert torch.equal(other.balance_bias, layer.balance_bias)
+
+
+def test_router_limits_are_checked_at_construction():
+    """What no forward could run does not construct: moe_route's limits, and a scale that
+    leaves no weight above 0."""
+    def layer(E, k, **kw):
+        return SwiFFN_MoE(MoEConfig(d_model=8, ffn_mult=1.0, tile=8, num_experts=E, num_experts_per_tok=k, **kw))
+
+    for precision in ("fp8", "mx4"):
+        for scale in (0.0, -1.0, math.inf, math.nan):
+            with pytest.raises(ValueError, match="router_scale"):
+                layer(4, 2, precision=precision, router_scale=scale)
+    with pytest.raises(ValueError, match="512"):
+        layer(513, 2, precision="mx4")
+    with pytest.raises(ValueError, match="512"):
+        layer(520, 2, router_score="sigmoid")
+    with pytest.raises(ValueError, match="16"):
+        layer(20, 17, router_score="sigmoid")
+    with pytest.raises(ValueError, match="64"):
+        layer(130, 2, router_groups=65, router_top_groups=3)
+    assert layer(512, 16, precision="mx4", router_groups=64, router_top_groups=9).num_experts == 512
+    assert layer(20, 17).route_args is None  # the softmax router's own limits are its entry's
