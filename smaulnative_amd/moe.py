@@ -270,6 +270,13 @@ class SwiFFN_MoE(nn.Module):
                              f"{args['groups']}")
         return args
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        # a layer pickled before there were other routers
+        self.__dict__.setdefault("route_args", None)
+        if "balance_bias" not in self._buffers:
+            self.__dict__.setdefault("balance_bias", None)
+
     def _apply(self, fn, *args, **kwargs):
         kept = self.balance_bias
         super()._apply(fn, *args, **kwargs)

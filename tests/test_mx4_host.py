@@ -134,3 +134,21 @@ def test_router_limits_are_checked_at_construction():
         layer(130, 2, router_groups=65, router_top_groups=3)
     assert layer(512, 16, precision="mx4", router_groups=64, router_top_groups=9).num_experts == 512
     assert layer(20, 17).route_args is None  # the softmax router's own limits are its entry's
+
+
+def test_layers_pickled_before_the_router_fields():
+    """A whole layer saved when it had no router fields loads, moves and casts as it did."""
+    import copy
+    import pickle
+    layer = SwiFFN_MoE(MoEConfig(d_model=64, num_experts=2, num_experts_per_tok=1))
+    old = copy.copy(layer)
+    old.__dict__ = {k: v for k, v in layer.__dict__.items() if k not in ("route_args", "balance_bias")}
+    again = pickle.loads(pickle.dumps(old))
+    assert again.route_args is None and again.balance_bias is None
+    assert again.to(torch.bfloat16).gate.weight.dtype == torch.bfloat16
+    assert copy.deepcopy(again).route_args is None
+    with pytest.raises(RuntimeError, match="HIP device tensors"):
+        with torch.no_grad():
+            again(torch.zeros(3, 64, dtype=torch.bfloat16))  # as a new one: no host fallback
+    wide = pickle.loads(pickle.dumps(SwiFFN_MoE(MoEConfig(d_model=64, num_experts=2, router_bias=True))))
+    assert wide.route_args["score"] == "softmax" and "balance_bias" in wide.state_dict()
