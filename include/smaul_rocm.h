@@ -507,8 +507,8 @@ int smaul_swiglu_backward(const void* dout, const void* g, const void* u, void* 
  * that no expert fills has topi -1 and topw 0 (smaul_moe_dispatch drops it).  The
  * softmax of a row whose logits are all -inf is NaN, and so is its prob.
  * logits: dtype [T, E]; prob fp32 [T, E] (s) or NULL; topi int64 [T, k]; topw fp32
- * [T, k].  E <= 512, k <= 16, groups <= 64 (a divisor of E), and top_groups groups
- * hold at least k experts.  The choice is that of scores in 64 bits.
+ * [T, k].  T < 2^28, E <= 512, k <= 16, groups <= 64 (a divisor of E), and top_groups
+ * groups hold at least k experts.  The choice is that of scores in 64 bits.
  */
 enum { SMAUL_SCORE_SOFTMAX = 0, SMAUL_SCORE_SIGMOID = 1 };
 int smaul_moe_route(const void* logits, int dtype, const float* bias, float* prob, int64_t* topi, float* topw,
@@ -535,7 +535,9 @@ int smaul_moe_route_backward(const float* dtopw, const void* logits, int dtype, 
  * NaN).  Quantisation: 2^(floor(log2(largest magnitude)) - 2), at least 2^-127; values
  * to nearest, ties to the even code, past 6 to 6; a block that holds an infinity or
  * NaN is all NaN.  Values past K are code 0.  x and y: dtype (f32 or bf16) [rows, K];
- * any K >= 1; codes 4-byte aligned.
+ * any K >= 1; codes 4-byte aligned.  Calls of more work than one launch counts (2^32
+ * work-items; 2^37 values here, 2^35 of an operand of the products below) are
+ * refused.
  */
 int smaul_mx4_quantize(const void* x, int dtype, uint8_t* codes, uint8_t* scales, int64_t rows, int64_t K,
                        hipStream_t stream);

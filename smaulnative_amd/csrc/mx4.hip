@@ -14,6 +14,7 @@
 using smaul::check_launch;
 using smaul::cu_count;
 using smaul::fail;
+using smaul::grid_fits;
 
 namespace {
 
@@ -823,7 +824,7 @@ int launch_gemm_cfg(const Mx4Args& p, int64_t m_tiles, hipStream_t stream) {
   if (BM * p.ldx * C::XS >= 1LL << 32 || BN * p.ldw * (WF == W_BF16 ? 2 : 16) >= 1LL << 32)
     return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: rows too wide");
   const int64_t n_tiles = (mx4_cols<OT>(p) + BNO - 1) / BNO;
-  if (m_tiles * n_tiles > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: too many tiles");
+  if (!grid_fits(m_tiles * n_tiles, WM * WN * 64)) return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: too many tiles");
   hipLaunchKernelGGL((mx4_gemm_kernel<AT, WF, OT, SWIGLU, BM, BN, WM, WN, KS, NSTAGE>),
                      dim3((unsigned)(m_tiles * n_tiles)), dim3(WM * WN * 64), 0, stream, p);
   return check_launch("mx4_gemm_kernel");
@@ -1421,7 +1422,7 @@ int launch_stream_cfg(Mx4Args p, const Mx4Slots& q, int64_t groups, hipStream_t 
 template <int AT, int OT, bool SWIGLU>
 int launch_stream(const Mx4Args& p, const Mx4Slots& q, hipStream_t stream) {
   const int64_t groups = (p.N + 31) / 32 * p.E;
-  if (groups > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: too many columns");
+  if (!grid_fits(groups, 256)) return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: too many columns");
   // 4 waves where there are workgroups enough for that: then all of them run at once
   if (groups > 2 * cu_count()) return launch_stream_cfg<AT, OT, SWIGLU, 4>(p, q, groups, stream);
   return launch_stream_cfg<AT, OT, SWIGLU, 8>(p, q, groups, stream);
@@ -1518,11 +1519,11 @@ int launch_combine(const void* y, const int64_t* topi, const float* topw, const 
 
 int launch_quantize(const void* x, int dtype, uint8_t* codes, uint8_t* scales, int64_t rows, int64_t K,
                     hipStream_t stream) {
-  const int64_t threads = rows * mx4_blocks(K) * 4;
-  if (threads > 256LL * 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_quantize: too many values");
   const bool vec = K % MX4_BLOCK == 0 && aligned(x, 16), bf16 = dtype == SMAUL_DTYPE_BF16;
   constexpr int64_t per = 256 * MX4_U;
-  const dim3 grid((unsigned)((threads + per - 1) / per)), block(256);
+  const int64_t blocks = (rows * mx4_blocks(K) * 4 + per - 1) / per;
+  if (!grid_fits(blocks, 256)) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_quantize: too many values");
+  const dim3 grid((unsigned)blocks), block(256);
   const bool nt = rows * K * (bf16 ? 2 : 4) >= MX4_NT_BYTES;
 #define SMAUL_Q(B, V, N) \
   hipLaunchKernelGGL((mx4_quantize_kernel<B, V, N>), grid, block, 0, stream, x, (uint32_t*)codes, scales, rows, K)
@@ -1628,7 +1629,7 @@ int launch_prep(Mx4Prep p, int dtype, int64_t E, hipStream_t stream) {
     if (m.w) m.blocks = (E * mx4_groups(m.K) * m.N + 255) / 256;
     blocks += m.blocks;
   }
-  if (blocks > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: too many rows");
+  if (!grid_fits(blocks, 256)) return fail(SMAUL_ERR_UNSUPPORTED, "mx4 product: too many rows or weights");
   auto* kernel = dtype == SMAUL_DTYPE_BF16 ? &mx4_prep_kernel<true> : &mx4_prep_kernel<false>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p, E);
   return check_launch("mx4_prep_kernel");
@@ -1734,11 +1735,11 @@ int smaul_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* y, i
   if (rows == 0) return SMAUL_OK;
   if (!codes || !scales || !y) return fail(SMAUL_ERR_INVALID, "mx4_dequantize: null pointer");
   if (!aligned(codes, 4)) return fail(SMAUL_ERR_INVALID, "mx4_dequantize: codes must be 4-byte aligned");
-  const int64_t threads = rows * mx4_blocks(K) * 4;
-  if (threads > 256LL * 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_dequantize: too many values");
   const bool vec = K % MX4_BLOCK == 0 && aligned(y, 16), bf16 = dtype == SMAUL_DTYPE_BF16;
   constexpr int64_t per = 256 * MX4_U;
-  const dim3 grid((unsigned)((threads + per - 1) / per)), block(256);
+  const int64_t blocks = (rows * mx4_blocks(K) * 4 + per - 1) / per;
+  if (!grid_fits(blocks, 256)) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_dequantize: too many values");
+  const dim3 grid((unsigned)blocks), block(256);
   const bool nt = rows * K * (bf16 ? 2 : 4) >= MX4_NT_BYTES;
 #define SMAUL_D(B, V, N)                                                                                       \
   hipLaunchKernelGGL((mx4_dequantize_kernel<B, V, N>), grid, block, 0, stream, (const uint32_t*)codes, scales, \
@@ -1837,7 +1838,7 @@ int smaul_mx4_backward_input(const void* g, int dtype, const uint8_t* w, const u
   const bool bf16 = dtype == SMAUL_DTYPE_BF16;
   if (!q.gemm) {
     const int64_t blocks = mx4_blocks(in_f);
-    if (blocks > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_backward_input: too wide a weight");
+    if (!grid_fits(blocks, 512)) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_backward_input: too wide a weight");
     const bool vec = out_f % 8 == 0;
     auto* kernel = bf16  ? (vec ? &mx4_dx_stream_kernel<A_BF16, true, 8> : &mx4_dx_stream_kernel<A_BF16, false, 8>)
                    : vec ? &mx4_dx_stream_kernel<A_F32, true, 8>
@@ -1854,7 +1855,8 @@ int smaul_mx4_backward_input(const void* g, int dtype, const uint8_t* w, const u
   f.xmode = q.lay ? P_PAD : P_NONE;
   prep_rows(f, dtype);
   const int64_t blocks = f.xblocks + q.ldo / 64 * ((in_f + 63) / 64);
-  if (blocks > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "mx4_backward_input: too large a weight or gradient");
+  if (!grid_fits(blocks, 256))
+    return fail(SMAUL_ERR_UNSUPPORTED, "mx4_backward_input: too large a weight or gradient");
   auto* kernel = bf16 ? &mx4_turn_kernel<true> : &mx4_turn_kernel<false>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, f, w, s, (uint16_t*)(ws + q.wt), out_f, in_f,
                      q.ldo);

@@ -17,6 +17,7 @@
 
 using smaul::check_launch;
 using smaul::fail;
+using smaul::grid_fits;
 
 namespace {
 
@@ -686,7 +687,7 @@ int check_route(const char* what, int dtype, int64_t T, int64_t E, int64_t k, in
     return fail(SMAUL_ERR_UNSUPPORTED, "%s: more than %d experts or top %d", what, ROUTE_MAX_E, ROUTE_MAX_K);
   if (score != SMAUL_SCORE_SOFTMAX && score != SMAUL_SCORE_SIGMOID)
     return fail(SMAUL_ERR_INVALID, "%s: bad score", what);
-  if (T > (1LL << 31)) return fail(SMAUL_ERR_UNSUPPORTED, "%s: more than 2^31 tokens", what);
+  if (!grid_fits((T + 15) / 16, 256)) return fail(SMAUL_ERR_UNSUPPORTED, "%s: 2^28 tokens or more", what);
   return SMAUL_OK;
 }
 

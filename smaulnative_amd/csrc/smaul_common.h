@@ -1,5 +1,5 @@
 // smaul_common.h -- pieces shared by the translation units of libsmaul_rocm.so:
-// the per-thread error channel behind smaul_last_error(), the launch check and the
+// the per-thread error channel behind smaul_last_error(), the launch checks and the
 // device's size.
 #ifndef SMAUL_COMMON_H
 #define SMAUL_COMMON_H
@@ -29,6 +29,10 @@ inline int check_launch(const char* what) {
   if (e != hipSuccess) return fail(SMAUL_ERR_HIP, "%s: launch failed: %s", what, hipGetErrorString(e));
   return SMAUL_OK;
 }
+
+// A launch counts its work-items in 32 bits: of a larger grid it would run what is left
+// of a division by 2^32, without an error.
+inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks < (1LL << 32) / threads; }
 
 // compute units of the current device (cached per device)
 inline int cu_count() {

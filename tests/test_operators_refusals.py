@@ -76,3 +76,24 @@ def test_mx4_arguments():
     assert moe(d=124) == no and moe(dtype=0) == no and moe(T=1 << 40) == no
     assert moe(bytes_=size - 1) == bad and moe(ws=None) == bad and moe(ws=P + 16) == bad and moe(gate=P + 2) == bad
     assert moe(T=0) == _lib.SMAUL_OK
+
+
+def test_calls_past_a_launch_are_refused():
+    """A launch counts its work-items in 32 bits, and runs what is left of a division by
+    2^32 of a larger grid without a word: refused before anything is launched."""
+    lib = _lib.load()
+    bad, no = _lib.SMAUL_ERR_INVALID, _lib.SMAUL_ERR_UNSUPPORTED
+    for T, rc in (((1 << 28) - 16, bad), (1 << 28, no), (1 << 30, no)):  # bad: null pointers are looked at next
+        assert lib.smaul_moe_route(None, 0, None, None, None, None, T, 4, 2, 0, 1, 1, 2, 1, 1.0, None) == rc
+        assert lib.smaul_moe_route_backward(None, None, 0, None, None, None, T, 4, 2, 0, 1, 1.0, None) == rc
+    assert lib.smaul_mx4_quantize(P, 1, P, P, 1 << 32, 32, None) == no
+    assert lib.smaul_mx4_dequantize(P, P, P, 1, 1 << 32, 32, None) == no
+    for rows, K, N in ((1 << 27, 1, 1), (1 << 30, 1, 1), (1 << 22, 8200, 8), (100, 1 << 20, 1 << 20)):
+        for act in (0, 1):
+            need = lib.smaul_mx4_linear_workspace_size(rows, K, N, 1, act)
+            assert lib.smaul_mx4_linear(P, 1, P, P, P, rows, K, N, act, P, need, None) == no
+    for rows, K, N in ((100, 1 << 19, 1 << 17), (1 << 27, 1, 3)):
+        need = lib.smaul_mx4_backward_input_workspace_size(rows, K, N, 1)
+        assert lib.smaul_mx4_backward_input(P, 1, P, P, P, rows, K, N, P, need, None) == no
+    assert lib.smaul_mx4_backward_input(P, 1, P, P, P, 4, 1 << 29, 8, P, 0, None) == no
+    assert lib.smaul_mx4_linear(P, 1, P, P, P, 4, 8, 1 << 29, 0, None, 0, None) == no
