@@ -1538,19 +1538,22 @@ int launch_quantize(const void* x, int dtype, uint8_t* codes, uint8_t* scales, i
 }
 
 // Up to ST_ROWS rows (tokens of a layer) mx4_stream_kernel runs, past them the larger
-// products, in tiles that fill the chip: what a tile takes (of 256 x 256 = 100, with
-// every CU at work), times the rounds of the CUs.  The last parts of the experts'
+// products, in tiles that fill the chip: what a round of the CUs takes (of 256 x 256 =
+// 100), times the rounds.  The smaller tiles of codes run two a CU, in rounds of twice the
+// CUs; a last round of no more than one a CU is `one`.  The last parts of the experts'
 // segments count for half a tile.  us, by tiles of 256 x 256, 128 x 256, 128 x 128 and
-// 64 x 128, rounded activations: 512 x 4096 -> 4096 34, 24, 20, 18; 1500 rows 39, 30, 36,
-// 43; 16384 x 1024 -> 2560 47, 49, -, -; 512 tokens to 2 of 8 experts, 1024 by 2560, 53, 44,
-// 44, 48.  bf16 as it is, 128 x 256 and 64 x 128: 512 rows 58, 31; 1500 rows 65, 65; 16384 x
-// 1024 -> 2560 80, 114.
+// 64 x 128, rounded activations: 512 x 4096 -> 4096 32, 24, 20, 18; 1500 rows 37, 28, 28, 33;
+// 6000 x 4096 -> 1024 (96, 188, 376, 752 tiles) 43, 49, 35, 39; 8192 x 4096 -> 2560 78, 75,
+// 70, 84; 16384 x 1024 -> 2560 45, 47, 46, 57; tokens to 2 of 8 experts, 1024 by 2560: 700
+// 53, 49, 42, 41; 16000 209, 235, 234, 296.  Of 144 products the choice is on average 1.2 % off
+// the best, at most 14.  bf16 as it is, 128 x 256 and 64 x 128: 512 rows 58, 31; 1500 rows
+// 65, 65; 16384 x 1024 -> 2560 80, 114.
 struct Mx4Tile {
-  int bm, bn, cost;
+  int bm, bn, one, two;  // two: 0 where a CU takes them one by one
 };
-constexpr Mx4Tile CODES_TILES[] = {{256, 256, 100}, {128, 256, 62}, {128, 128, 35}, {64, 128, 27}};
-constexpr Mx4Tile BF16_TILES[] = {{128, 256, 62}, {64, 128, 22}};
-constexpr Mx4Tile F32_TILES[] = {{32, 256, 100}};
+constexpr Mx4Tile CODES_TILES[] = {{256, 256, 100, 0}, {128, 256, 63, 0}, {128, 128, 40, 62}, {64, 128, 28, 39}};
+constexpr Mx4Tile BF16_TILES[] = {{128, 256, 62, 0}, {64, 128, 22, 0}};
+constexpr Mx4Tile F32_TILES[] = {{32, 256, 100, 0}};
 
 struct Mx4Shape {  // of one product
   int64_t R, K, cols;
@@ -1572,7 +1575,9 @@ int pick_tile(const Mx4Tile (&tiles)[N], const Mx4Shape (&products)[M], int64_t 
     for (const Mx4Shape& q : products) {
       const int64_t bn = q.swiglu ? tiles[i].bn / 2 : tiles[i].bn;
       const int64_t m = (q.R + tiles[i].bm - 1) / tiles[i].bm + parts / 2, n = (q.cols + bn - 1) / bn;
-      cost += (double)((m * n + cus - 1) / cus) * (double)q.K * tiles[i].cost;
+      const int64_t round = tiles[i].two ? 2 * cus : cus, full = m * n / round, left = m * n % round;
+      const int whole = tiles[i].two ? tiles[i].two : tiles[i].one;
+      cost += (double)q.K * ((double)full * whole + (left == 0 ? 0 : left <= cus ? tiles[i].one : whole));
     }
     if (i == 0 || cost < least) {
       best = i;
