@@ -145,3 +145,32 @@ def test_infinite_hidden_values_at_the_end_of_a_width_off_eight(T):
                                                  torch.ones(T, 1, device=DEV), [t.to(DEV) for t in experts])
     assert torch.isinf(want).any()
     _same_kinds(out, want)
+
+
+@pytest.mark.parametrize("rows", [1, 9, 32, 33, 64, 150, 700])  # few rows, and tiles
+def test_fp32_gradients_keep_all_their_bits(rows):
+    """A weight of one code a row picks single gradients: 24 bits come back as they went in."""
+    gen = torch.Generator().manual_seed(rows)
+    for K in (64, 100):
+        g = torch.randn(rows, K, generator=gen) * torch.pow(2.0, torch.randint(-30, 30, (rows, K), generator=gen).float())
+        w, s = ref.quantize(torch.eye(K))
+        got = get_backend("rocm").mx4_backward_input(g.to(DEV), w.to(DEV), s.to(DEV), K, K)
+        assert torch.equal(got.cpu(), g)
+
+
+@pytest.mark.parametrize("T", [9, 64, 65, 300])
+@pytest.mark.parametrize("d", [64, 104])
+def test_fp32_experts_keep_all_their_bits(T, d):
+    """Gate, up and down weights of one code a row: an output is silu(x) x of its own x.
+
+    The product's arithmetic alone is left: the argument's rounding (|x| 2^-24 of the
+    value), the exponential, sum, reciprocal and two products, a step of 2^-23 each at
+    most: |x| + 10 times 2^-24, below 2^-20 for |x| < 6.  A bf16 term dropped from x or from
+    the hidden rows is 2^-17 and more on most values."""
+    gen = torch.Generator().manual_seed(T + d)
+    x = torch.randn(T, d, generator=gen).clamp(-5.5, 5.5)
+    w, s = ref.quantize(torch.eye(d))
+    out, _ = get_backend("rocm").mx4_moe_forward(x.to(DEV), torch.zeros(T, 1, dtype=torch.int64, device=DEV),
+                                                 torch.ones(T, 1, device=DEV), [t[None].to(DEV) for t in (w, s) * 3])
+    want = ref.swiglu(x.double(), x.double())
+    assert ((out.cpu().double() - want).abs() <= 2.0 ** -20 * want.abs()).all()

@@ -247,3 +247,24 @@ def test_layers_past_one_call(precision, act, dtype, E, k, d, T):
     with torch.no_grad():
         wide = m(x.view(1, T, d))
     assert wide.shape == (1, T, d) and torch.equal(wide.view(T, d), out) and m.last_topi.shape == (1, T, k)
+
+
+@pytest.mark.parametrize("precision", ["mx4", "fp8"])
+def test_router_scores_with_a_gate_bias(precision):
+    """The layer's scores against x . W^T + b formed here in 64 bits."""
+    m = _layer(21, precision=precision, **WIDE)
+    T, d = 70, 128
+    gen = torch.Generator().manual_seed(21)
+    m.gate.bias = torch.nn.Parameter(torch.randn(8, generator=gen).to(DEV))
+    x = torch.randn(T, d, generator=gen)
+    w, b = m.gate.weight.detach().double().cpu(), m.gate.bias.detach().double().cpu()
+    z = x.double() @ w.t() + b
+    want = torch.sigmoid(z)
+    # fp32 sums of d + 1 terms, each rounding at most 2^-24 of their magnitudes; sigmoid's
+    # slope is s (1 - s), and its own arithmetic |z| + 16 steps of 2^-24
+    dz = (x.double().abs() @ w.abs().t() + b.abs()) * (d + 1) * 2.0 ** -24
+    tol = want * ((1 - want) * dz * 1.01 + (z.abs() + 16) * 2.0 ** -24)
+    for train in (False, True):
+        with torch.set_grad_enabled(train):
+            m(x.to(DEV))
+        assert ((m.last_prob.detach().cpu().double() - want).abs() <= tol).all()
