@@ -627,9 +627,10 @@ class RocmBackend:
         ``moe_route`` (or ``moe_router``), distinct experts a token; experts:
         (gate_w, gate_s, up_w, up_s, down_w, down_s), the codes [E, h, 16 n] (gate,
         up) and [E, d, 16 n] (down) and scales of all experts.  ``act`` "mx4" (bf16 x)
-        rounds the rows of x and the hidden rows to the format, "keep" the hidden
-        rows to x's type.  Slots with topi outside [0, E) or topw not above 0 add
-        nothing."""
+        rounds the rows of x and the hidden rows to the format and each slot's
+        output to bf16, "keep" the hidden rows to x's type and no slot's output; the
+        slots are added in fp32 and rounded to x's type once.  Slots with topi outside
+        [0, E) or topw not above 0 add nothing."""
         lib = _lib.load()
         _need_device("mx4_moe_forward", x, topi, topw, *experts)
         if act not in _lib.ACTS:
