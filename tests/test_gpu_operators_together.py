@@ -80,3 +80,47 @@ def test_long_rows_past_32_bit_offsets():
     del x, codes, scales
     dx = be.mx4_backward_input(y, w, s, K, N)
     assert torch.equal(dx[-700:], be.mx4_backward_input(y[-700:].clone(), w, s, K, N))
+
+
+@pytest.mark.parametrize("precision", ["mx4", "fp8"])
+@pytest.mark.parametrize("T", [3, 100])
+def test_layer_of_many_experts_replays(precision, T):
+    """More experts than one call takes: captured, replayed between eager calls on another stream."""
+    E, k, d = 130, 6, 64
+    torch.manual_seed(T)
+    layer = SwiFFN_MoE(MoEConfig(d_model=d, tile=64, num_experts=E, num_experts_per_tok=k, precision=precision,
+                                 router_score="sigmoid", router_groups=10, router_top_groups=4, router_bias=True,
+                                 router_scale=2.5)).to(DEV).eval().requires_grad_(False)
+    gen = torch.Generator().manual_seed(T)
+    x = torch.randn(T, d, generator=gen).bfloat16().to(DEV)
+    layer(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer(x)
+        counts = layer._counts_dev
+    side = torch.cuda.Stream(DEV)
+    for _ in range(3):
+        x.copy_(torch.randn(T, d, generator=gen))
+        graph.replay()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            eager = layer(x)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(out, eager) and torch.equal(counts, layer._counts_dev) and int(counts.sum()) == T * k
+
+
+def test_layer_of_other_types():
+    """fp16 and fp64 rows run through fp32 experts in 4 bits, with and without gradients."""
+    torch.manual_seed(0)
+    layer = SwiFFN_MoE(MoEConfig(d_model=64, tile=64, num_experts=4, num_experts_per_tok=2, precision="mx4")).to(DEV)
+    x = torch.randn(20, 64, generator=torch.Generator().manual_seed(1))
+    with torch.no_grad():
+        want = layer(x.half().float().to(DEV))
+    for dtype in (torch.float16, torch.float64):
+        for train in (False, True):
+            with torch.set_grad_enabled(train):
+                got = layer(x.half().to(dtype).to(DEV))
+            assert got.dtype == dtype and layer.last_topi.shape == (20, 2)
+            # fp16 rounds the expert's products, its hidden rows and outputs, half a step each
+            assert float((got.detach().float() - want).norm() / want.norm()) <= (2e-3 if dtype == torch.float16 else 1e-5)
