@@ -583,6 +583,92 @@ int smaul_mx4_moe_forward(const void* x, int dtype, const int64_t* topi, const f
                           hipStream_t stream);
 
 /*
+ * Rows in blocks of 128 E4M3 codes with a shared power of two (no counterpart in the
+ * reference).  A row of K values is n = ceil(K / 128) blocks: codes uint8 [rows, 128 n]
+ * and scales uint8 [rows, 4 ceil(n / 4)] (four blocks' are one 32-bit word).  A block
+ * stands for its codes' E4M3 values times 2^(scale - 127); the scale is the least power
+ * of two (from 2^-127) over which the block's largest magnitude does not pass 448, codes
+ * are rounded to nearest, ties to even.  A block that holds an infinity or NaN is all NaN
+ * (scale 255, codes 0).  Codes past K and scales past n are 0, and have to be.
+ * x / y: dtype f32 or bf16 (read back in bf16 every value is exact down to its subnormals).
+ */
+int smaul_fp8_block_quantize(const void* x, int dtype, uint8_t* codes, uint8_t* scales, int64_t rows, int64_t K,
+                             hipStream_t stream);
+int smaul_fp8_block_dequantize(const uint8_t* codes, const uint8_t* scales, void* y, int dtype, int64_t rows, int64_t K,
+                               hipStream_t stream);
+
+/*
+ * y[rows, out_f] = Q(x)[rows, in_f] . decode(w, s)^T, w and s [out_f, in_f] in that format,
+ * y of y_dtype (f32 or bf16).  x: rows of x_dtype f32 or bf16, rounded to the format in the
+ * workspace, or with x_dtype SMAUL_DTYPE_FP8_BLOCK codes with scales xs.  Products are
+ * exact, sums fp32.  x, y and w 16-byte aligned, scales 4, the workspace 256.
+ */
+enum { SMAUL_DTYPE_FP8_BLOCK = 2 };
+int64_t smaul_fp8_block_linear_workspace_size(int64_t rows, int64_t in_f, int64_t out_f, int x_dtype);
+int smaul_fp8_block_linear(const void* x, int x_dtype, const uint8_t* xs, const uint8_t* w, const uint8_t* s, void* y,
+                           int y_dtype, int64_t rows, int64_t in_f, int64_t out_f, void* workspace,
+                           int64_t workspace_bytes, hipStream_t stream);
+
+/*
+ * dx[rows, in_f] = g[rows, out_f] . decode(w, s): its input gradient, straight through
+ * the rounding of x; g and dx of dtype (f32 or bf16), g as it is.  g, w and dx 16-byte
+ * aligned, the scales 4, the workspace 256.
+ */
+int64_t smaul_fp8_block_backward_input_workspace_size(int64_t rows, int64_t in_f, int64_t out_f, int dtype);
+int smaul_fp8_block_backward_input(const void* g, int dtype, const uint8_t* w, const uint8_t* s, void* dx, int64_t rows,
+                                   int64_t in_f, int64_t out_f, void* workspace, int64_t workspace_bytes,
+                                   hipStream_t stream);
+
+/*
+ * The gated feed-forward block in that format: hdn = Q(silu(x . Wg^T) * (x . Wu^T)),
+ * y[T, d] (bf16) = hdn . Wd^T; gate_w / up_w [h, d], down_w [d, h].  x: bf16 rows, rounded
+ * first, or codes with xs.  The hidden rows are rounded from fp32.
+ * saved (smaul_fp8_block_ffn_saved_size bytes): what the backward pass takes is kept, in
+ * saved itself, h_codes / h_scales [T, h] and, of an x of rows, x_codes / x_scales [T, d];
+ * NULL: nothing is, and those may be NULL too.  Rows and codes 16-byte aligned, scales 4,
+ * the workspace 256.
+ */
+int64_t smaul_fp8_block_ffn_saved_size(int64_t T, int64_t h);
+int64_t smaul_fp8_block_ffn_workspace_size(int64_t T, int64_t d, int64_t h, int x_dtype, int save);
+int smaul_fp8_block_ffn_forward(const void* x, int x_dtype, const uint8_t* xs, const uint8_t* gate_w,
+                                const uint8_t* gate_s, const uint8_t* up_w, const uint8_t* up_s, const uint8_t* down_w,
+                                const uint8_t* down_s, void* y, uint8_t* x_codes, uint8_t* x_scales, uint8_t* h_codes,
+                                uint8_t* h_scales, void* saved, int64_t T, int64_t d, int64_t h, void* workspace,
+                                int64_t workspace_bytes, hipStream_t stream);
+
+/*
+ * Its gradients, straight through the roundings, all bf16: dx[T, d] (or NULL), dgate and
+ * dup [h, d], ddown [d, h] (or all three NULL) from dy[T, d]; the codes are the forward's.
+ * With T == 0 the weights' gradients are 0.
+ */
+int64_t smaul_fp8_block_ffn_backward_workspace_size(int64_t T, int64_t d, int64_t h);
+int smaul_fp8_block_ffn_backward(const void* dy, const uint8_t* gate_w, const uint8_t* gate_s, const uint8_t* up_w,
+                                 const uint8_t* up_s, const uint8_t* down_w, const uint8_t* down_s,
+                                 const uint8_t* x_codes, const uint8_t* x_scales, const uint8_t* h_codes,
+                                 const uint8_t* h_scales, const void* saved, void* dx, void* dgate, void* dup,
+                                 void* ddown, int64_t T, int64_t d, int64_t h, void* workspace, int64_t workspace_bytes,
+                                 hipStream_t stream);
+
+/*
+ * sum = x + residual (rounded to dtype; residual NULL: sum is x, and not written), and out
+ * = sum / sqrt(mean(sum^2) + eps) * weight (fp32 [d], NULL: ones), computed in fp32:
+ * rounded to dtype, or with scales not NULL to codes and scales of the format above
+ * (out 8-byte aligned).  Outputs do not overlap inputs.
+ */
+int smaul_add_rms_norm(const void* x, const void* residual, int dtype, const float* weight, float eps, void* sum,
+                       void* out, uint8_t* scales, int64_t T, int64_t d, hipStream_t stream);
+
+/*
+ * Its gradients from out's, dy, and sum's, ds (or NULL): dx[T, d] of dtype, which is
+ * residual's too, and dw fp32 [d] (NULL: none).  s is the sum.  Straight through the
+ * rounding of out.  The workspace 256-byte aligned.
+ */
+int64_t smaul_add_rms_norm_backward_workspace_size(int64_t T, int64_t d);
+int smaul_add_rms_norm_backward(const void* dy, const void* s, const void* ds, int dtype, const float* weight,
+                                float eps, void* dx, float* dw, int64_t T, int64_t d, void* workspace,
+                                int64_t workspace_bytes, hipStream_t stream);
+
+/*
  * Measured ceilings for the roofline figures (bench.py --peaks); no
  * counterpart in the reference and not on the MoE path.
  * smaul_peak_mfma: `workgroups` x 4 waves, each issuing `iters` rounds of 8

@@ -19,6 +19,7 @@ SMAUL_ERR_UNSUPPORTED = 2
 SMAUL_ERR_HIP = 3
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_FP8_BLOCK = 2
 FLAG_CANONICAL_CODES = 1
 FLAG_ALIGNED_CODES = 2
 FLAG_TILED_LAYOUT = 4
@@ -86,6 +87,20 @@ SIGNATURES = {
     "smaul_mx4_backward_input": (_I, [_P, _I, _P, _P, _P, _I64, _I64, _I64, _P, _I64, _P]),
     "smaul_mx4_moe_workspace_size": (_I64, [_I64, _I64, _I64, _I64, _I64, _I, _I]),
     "smaul_mx4_moe_forward": (_I, [_P, _I] + [_P] * 10 + [_I64, _I64, _I64, _I64, _I64, _I, _P, _I64, _P]),
+    "smaul_fp8_block_quantize": (_I, [_P, _I, _P, _P, _I64, _I64, _P]),
+    "smaul_fp8_block_dequantize": (_I, [_P, _P, _P, _I, _I64, _I64, _P]),
+    "smaul_fp8_block_linear_workspace_size": (_I64, [_I64, _I64, _I64, _I]),
+    "smaul_fp8_block_linear": (_I, [_P, _I, _P, _P, _P, _P, _I, _I64, _I64, _I64, _P, _I64, _P]),
+    "smaul_fp8_block_backward_input_workspace_size": (_I64, [_I64, _I64, _I64, _I]),
+    "smaul_fp8_block_backward_input": (_I, [_P, _I, _P, _P, _P, _I64, _I64, _I64, _P, _I64, _P]),
+    "smaul_fp8_block_ffn_saved_size": (_I64, [_I64, _I64]),
+    "smaul_fp8_block_ffn_workspace_size": (_I64, [_I64, _I64, _I64, _I, _I]),
+    "smaul_fp8_block_ffn_forward": (_I, [_P, _I] + [_P] * 13 + [_I64, _I64, _I64, _P, _I64, _P]),
+    "smaul_fp8_block_ffn_backward_workspace_size": (_I64, [_I64, _I64, _I64]),
+    "smaul_fp8_block_ffn_backward": (_I, [_P] * 16 + [_I64, _I64, _I64, _P, _I64, _P]),
+    "smaul_add_rms_norm": (_I, [_P, _P, _I, _P, ctypes.c_float, _P, _P, _P, _I64, _I64, _P]),
+    "smaul_add_rms_norm_backward_workspace_size": (_I64, [_I64, _I64]),
+    "smaul_add_rms_norm_backward": (_I, [_P, _P, _P, _I, _P, ctypes.c_float, _P, _P, _I64, _I64, _P, _I64, _P]),
     "smaul_peak_mfma": (_I, [_P, _I, _I, _P]),
     "smaul_peak_stream": (_I, [_P, _I64, _P, _I, _P]),
     "smaul_peak_lds_dma": (_I, [_P, _I64, _P, _I, _I, _P]),

@@ -669,6 +669,191 @@ class RocmBackend:
         _lib.check(rc, "mx4_moe_forward")
         return out, counts
 
+    # ---- rows in blocks of 128 8-bit codes (no counterpart in the reference) ----
+    def fp8_block_quantize(self, x):
+        """(codes uint8 [..., 128 n], scales uint8 [..., 4 ceil(n / 4)]) of x [..., K] fp32 or
+        bf16, n = ceil(K / 128): blocks of 128 E4M3 codes with a shared power of two (E8M0),
+        the least with which no code saturates.  Codes past K and scales past n are 0.  A
+        block that holds an infinity or NaN is all NaN (scale 255)."""
+        lib = _lib.load()
+        _need_device("fp8_block_quantize", x)
+        if x.dtype not in _ACT or x.dim() < 1 or x.shape[-1] < 1:
+            raise RuntimeError(f"fp8_block_quantize: x must be float32 or bfloat16 rows, got {x.dtype} "
+                               f"{tuple(x.shape)}")
+        K = x.shape[-1]
+        n = (K + 127) // 128
+        xc = x if x.is_contiguous() else x.contiguous()
+        codes = torch.empty(*x.shape[:-1], n * 128, dtype=torch.uint8, device=x.device)
+        scales = torch.empty(*x.shape[:-1], (n + 3) // 4 * 4, dtype=torch.uint8, device=x.device)
+        with _device(x.device):
+            rc = lib.smaul_fp8_block_quantize(xc.data_ptr(), _ACT[x.dtype], codes.data_ptr(), scales.data_ptr(),
+                                              xc.numel() // K, K, _stream_handle(x.device))
+        _lib.check(rc, "fp8_block_quantize")
+        return codes, scales
+
+    def _block_check(self, name, codes, scales, lead, K):
+        """The codes and scales [*lead, 128 n] / [*lead, 4 ceil(n / 4)] of rows of K values, contiguous."""
+        n = (K + 127) // 128
+        if codes.dtype != torch.uint8 or codes.shape != (*lead, n * 128):
+            raise RuntimeError(f"{name}: codes must be uint8 {[*lead, n * 128]}, got {codes.dtype} "
+                               f"{list(codes.shape)}")
+        ns = (n + 3) // 4 * 4
+        if scales.dtype != torch.uint8 or scales.shape != (*lead, ns):
+            raise RuntimeError(f"{name}: scales must be uint8 {[*lead, ns]}, got {scales.dtype} {list(scales.shape)}")
+        return self._aligned(codes), self._aligned(scales)
+
+    def fp8_block_dequantize(self, codes, scales, in_f, dtype=torch.float32):
+        """The values [..., in_f] in ``dtype`` (fp32 or bf16, exact in both down to its
+        subnormals) that codes and scales (``fp8_block_quantize``) stand for."""
+        lib = _lib.load()
+        _need_device("fp8_block_dequantize", codes, scales)
+        if dtype not in _ACT:
+            raise RuntimeError(f"fp8_block_dequantize: dtype must be float32 or bfloat16, got {dtype}")
+        if in_f < 1:
+            raise ValueError(f"fp8_block_dequantize: in_f must be positive, got {in_f}")
+        lead = tuple(codes.shape[:-1])
+        codes, scales = self._block_check("fp8_block_dequantize", codes, scales, lead, in_f)
+        y = torch.empty(*lead, in_f, dtype=dtype, device=codes.device)
+        with _device(codes.device):
+            rc = lib.smaul_fp8_block_dequantize(codes.data_ptr(), scales.data_ptr(), y.data_ptr(), _ACT[dtype],
+                                                y.numel() // in_f, in_f, _stream_handle(codes.device))
+        _lib.check(rc, "fp8_block_dequantize")
+        return y
+
+    def _block_rows(self, name, x, xs, width, types):
+        """(x, xs, C type, leading dimensions): rows of ``width`` values of one of ``types``, or
+        with scales xs their codes."""
+        if x.dim() < 1:
+            raise RuntimeError(f"{name}: rows of {width} values expected, got a scalar")
+        lead = tuple(x.shape[:-1])
+        if xs is not None:
+            return (*self._block_check(f"{name}: x", x, xs, lead, width), _lib.DTYPE_FP8_BLOCK, lead)
+        if x.dtype not in types:
+            names = " or ".join(str(t).replace("torch.", "") for t in types)
+            raise RuntimeError(f"{name}: rows must be {names} (or codes with their scales), got {x.dtype}")
+        if x.shape[-1] != width:
+            raise RuntimeError(f"{name}: rows must be [..., {width}], got {tuple(x.shape)}")
+        return self._aligned(x), None, _ACT[x.dtype], lead
+
+    def fp8_block_forward(self, x, w, s, in_f, out_f, xs=None, dtype=None):
+        """y [..., out_f] = Q(x) . W^T, W the weight that codes w [out_f, 128 n] and scales s
+        stand for (``fp8_block_quantize``).  x [..., in_f] fp32 or bf16 is rounded to the
+        format; with scales ``xs`` it is codes already.  ``dtype`` of y: fp32 or bf16, by
+        default x's, of codes bf16.  Products are exact, sums fp32."""
+        lib = _lib.load()
+        _need_device("fp8_block_forward", x, xs, w, s)
+        if in_f < 1 or out_f < 1:
+            raise ValueError(f"fp8_block_forward: in_f/out_f must be positive, got {in_f}/{out_f}")
+        w, s = self._block_check("fp8_block_forward", w, s, (out_f,), in_f)
+        xc, xsc, xt, lead = self._block_rows("fp8_block_forward", x, xs, in_f, (torch.float32, torch.bfloat16))
+        if dtype is None:
+            dtype = x.dtype if xs is None else torch.bfloat16
+        if dtype not in _ACT:
+            raise RuntimeError(f"fp8_block_forward: dtype must be float32 or bfloat16, got {dtype}")
+        y = torch.empty(*lead, out_f, dtype=dtype, device=x.device)
+        rows = y.numel() // out_f
+        nws = lib.smaul_fp8_block_linear_workspace_size(rows, in_f, out_f, xt)
+        ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws > 0 else None
+        with _device(x.device):
+            rc = lib.smaul_fp8_block_linear(xc.data_ptr(), xt, None if xsc is None else xsc.data_ptr(), w.data_ptr(),
+                                            s.data_ptr(), y.data_ptr(), _ACT[dtype], rows, in_f, out_f,
+                                            None if ws is None else ws.data_ptr(), nws, _stream_handle(x.device))
+        _lib.check(rc, "fp8_block_forward")
+        return y
+
+    def fp8_block_backward_input(self, g, w, s, in_f, out_f):
+        """dx [..., in_f] = g [..., out_f] . W in g's type (fp32 or bf16): the input gradient
+        of ``fp8_block_forward``, straight through the rounding of its rows."""
+        lib = _lib.load()
+        _need_device("fp8_block_backward_input", g, w, s)
+        if in_f < 1 or out_f < 1:
+            raise ValueError(f"fp8_block_backward_input: in_f/out_f must be positive, got {in_f}/{out_f}")
+        w, s = self._block_check("fp8_block_backward_input", w, s, (out_f,), in_f)
+        gc, _, gt, lead = self._block_rows("fp8_block_backward_input", g, None, out_f, (torch.float32, torch.bfloat16))
+        dx = torch.empty(*lead, in_f, dtype=g.dtype, device=g.device)
+        rows = dx.numel() // in_f
+        nws = lib.smaul_fp8_block_backward_input_workspace_size(rows, in_f, out_f, gt)
+        ws = torch.empty(nws, dtype=torch.uint8, device=g.device) if nws > 0 else None
+        with _device(g.device):
+            rc = lib.smaul_fp8_block_backward_input(gc.data_ptr(), gt, w.data_ptr(), s.data_ptr(), dx.data_ptr(), rows,
+                                                    in_f, out_f, None if ws is None else ws.data_ptr(), nws,
+                                                    _stream_handle(g.device))
+        _lib.check(rc, "fp8_block_backward_input")
+        return dx
+
+    def _block_weights(self, name, weights, d, h):
+        if d < 1 or h < 1:
+            raise ValueError(f"{name}: d/h must be positive, got {d}/{h}")
+        if len(weights) != 6:
+            raise ValueError(f"{name}: weights is (gate_w, gate_s, up_w, up_s, down_w, down_s)")
+        return [t for i, what, n, k in ((0, "gate", h, d), (2, "up", h, d), (4, "down", d, h))
+                for t in self._block_check(f"{name}: {what}", weights[i], weights[i + 1], (n,), k)]
+
+    def fp8_block_ffn_forward(self, x, weights, d, h, xs=None, save=False):
+        """The gated feed-forward block y [..., d] (bf16) = Q(silu(x Wg^T) * (x Wu^T)) Wd^T.
+
+        x [..., d] bf16, rounded to the format, or with scales ``xs`` codes already; weights:
+        (gate_w, gate_s, up_w, up_s, down_w, down_s) in the format, [h, d], [h, d] and [d, h].
+        Sums are fp32, the hidden rows are rounded to codes from fp32.  With ``save`` returns
+        (y, saved), what ``fp8_block_ffn_backward`` takes."""
+        lib = _lib.load()
+        _need_device("fp8_block_ffn_forward", x, xs, *weights)
+        weights = self._block_weights("fp8_block_ffn_forward", weights, d, h)
+        xc, xsc, xt, lead = self._block_rows("fp8_block_ffn_forward", x, xs, d, (torch.bfloat16,))
+        dev = x.device
+        y = torch.empty(*lead, d, dtype=torch.bfloat16, device=dev)
+        T = y.numel() // d
+
+        def codes(K):
+            n = (K + 127) // 128
+            return (torch.empty(T, n * 128, dtype=torch.uint8, device=dev),
+                    torch.empty(T, (n + 3) // 4 * 4, dtype=torch.uint8, device=dev))
+
+        saved = None
+        if save:
+            saved = (*(codes(d) if xs is None else (xc, xsc)), *codes(h),
+                     torch.empty(lib.smaul_fp8_block_ffn_saved_size(T, h), dtype=torch.uint8, device=dev))
+        nws = lib.smaul_fp8_block_ffn_workspace_size(T, d, h, xt, int(save))
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws > 0 else None
+        with _device(dev):
+            rc = lib.smaul_fp8_block_ffn_forward(xc.data_ptr(), xt, None if xsc is None else xsc.data_ptr(),
+                                                 *[t.data_ptr() for t in weights], y.data_ptr(),
+                                                 *([t.data_ptr() for t in saved] if save else [None] * 5), T, d, h,
+                                                 None if ws is None else ws.data_ptr(), nws, _stream_handle(dev))
+        _lib.check(rc, "fp8_block_ffn_forward")
+        return (y, saved) if save else y
+
+    def fp8_block_ffn_backward(self, dy, weights, saved, d, h, need_dx=True, need_dw=True):
+        """(dx [..., d], dgate [h, d], dup [h, d], ddown [d, h]), bf16, of
+        ``fp8_block_ffn_forward`` from dy [..., d] (bf16), its weights and what it saved,
+        straight through the roundings; None for what is not asked for."""
+        lib = _lib.load()
+        _need_device("fp8_block_ffn_backward", dy, *weights, *saved)
+        weights = self._block_weights("fp8_block_ffn_backward", weights, d, h)
+        dyc, _, _, lead = self._block_rows("fp8_block_ffn_backward", dy, None, d, (torch.bfloat16,))
+        dev = dy.device
+        T = dyc.numel() // d
+        if len(saved) != 5 or saved[4].dtype != torch.uint8 or \
+                saved[4].numel() != lib.smaul_fp8_block_ffn_saved_size(T, h):
+            raise RuntimeError(f"fp8_block_ffn_backward: saved is of another call than one of {T} rows")
+        xc, xs = self._block_check("fp8_block_ffn_backward: x", saved[0], saved[1], tuple(saved[0].shape[:-1]), d)
+        hc, hs = self._block_check("fp8_block_ffn_backward: hidden rows", saved[2], saved[3], (T,), h)
+        if xs.numel() // xs.shape[-1] != T:
+            raise RuntimeError(f"fp8_block_ffn_backward: saved is of another call than one of {T} rows")
+        kept = self._aligned(saved[4])
+        dx = torch.empty(*lead, d, dtype=torch.bfloat16, device=dev) if need_dx else None
+        dw = [torch.empty(n, k, dtype=torch.bfloat16, device=dev) if need_dw else None
+              for n, k in ((h, d), (h, d), (d, h))]
+        nws = lib.smaul_fp8_block_ffn_backward_workspace_size(T, d, h)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws > 0 else None
+        with _device(dev):
+            rc = lib.smaul_fp8_block_ffn_backward(dyc.data_ptr(), *[t.data_ptr() for t in weights], xc.data_ptr(),
+                                                  xs.data_ptr(), hc.data_ptr(), hs.data_ptr(), kept.data_ptr(),
+                                                  *[None if t is None else t.data_ptr() for t in (dx, *dw)], T, d, h,
+                                                  None if ws is None else ws.data_ptr(), nws, _stream_handle(dev))
+        _lib.check(rc, "fp8_block_ffn_backward")
+        return (dx, *dw)
+
     # ---- MoE (model.py:557-585) -------------------------------------------
     def _expert_entry(self, experts: Sequence[Sequence[torch.Tensor]], device, d, h, tile):
         """The repack cache entry of a set of experts: ``table``, a device int64
@@ -973,6 +1158,74 @@ class RocmBackend:
                                     out.data_ptr(), x2.shape[0], d, eps, _stream_handle(x.device))
         _lib.check(rc, "rms_norm")
         return out.reshape(x.shape)
+
+    def _norm_check(self, name, eps, weight, *rows):
+        """The rows contiguous, the weight in fp32; one shape and one type of fp32 and bf16."""
+        first = rows[0]
+        if first.dtype not in _ACT or first.dim() < 1 or first.shape[-1] < 1:
+            raise RuntimeError(f"{name}: float32 or bfloat16 rows expected, got {first.dtype} {tuple(first.shape)}")
+        for t in rows:
+            if t is not None and (t.dtype != first.dtype or t.shape != first.shape):
+                raise RuntimeError(f"{name}: rows of one type and shape expected, got {first.dtype} "
+                                   f"{tuple(first.shape)} and {t.dtype} {tuple(t.shape)}")
+        if not math.isfinite(eps) or eps <= 0:
+            raise ValueError(f"RMSNorm eps must be positive finite, got {eps!r}")
+        if weight is not None:
+            d = first.shape[-1]
+            if weight.numel() != d:
+                raise RuntimeError(f"{name}: weight must have {d} elements, got {weight.numel()}")
+            weight = weight.detach().reshape(d)
+            if weight.dtype != torch.float32 or not weight.is_contiguous():
+                weight = weight.float().contiguous()
+        return weight, [t if t is None or t.is_contiguous() else t.contiguous() for t in rows]
+
+    def add_rms_norm(self, x, residual=None, weight=None, eps=1e-6, quantize=False):
+        """The residual's addition and ``rms_norm`` of the sum in one pass: (s, y), s = x +
+        residual rounded to x's type (x itself without a residual), y the norm of s in x's
+        type.  With ``quantize`` (s, codes, scales): y rounded from fp32 to the format of
+        ``fp8_block_quantize`` instead.
+
+        x and residual [..., d] bf16 or fp32, one type; weight [d] (None: ones)."""
+        lib = _lib.load()
+        _need_device("add_rms_norm", x, residual, weight)
+        w, (xc, rc_) = self._norm_check("add_rms_norm", eps, weight, x, residual)
+        d, dev = x.shape[-1], x.device
+        s = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+        if quantize:
+            n = (d + 127) // 128
+            y = torch.empty(*x.shape[:-1], n * 128, dtype=torch.uint8, device=dev)
+            scales = torch.empty(*x.shape[:-1], (n + 3) // 4 * 4, dtype=torch.uint8, device=dev)
+        else:
+            y, scales = torch.empty(x.shape, dtype=x.dtype, device=dev), None
+        with _device(dev):
+            rc = lib.smaul_add_rms_norm(xc.data_ptr(), None if rc_ is None else rc_.data_ptr(), _ACT[x.dtype],
+                                        None if w is None else w.data_ptr(), eps,
+                                        None if rc_ is None else s.data_ptr(), y.data_ptr(),
+                                        None if scales is None else scales.data_ptr(), xc.numel() // d, d,
+                                        _stream_handle(dev))
+        _lib.check(rc, "add_rms_norm")
+        return (s, y, scales) if quantize else (s, y)
+
+    def add_rms_norm_backward(self, dy, s, weight=None, eps=1e-6, ds=None, need_dw=True):
+        """(dx [..., d] in s's type, dw [d] fp32 or None) of ``add_rms_norm`` from y's gradient
+        dy, the sum s it returned and the sum's own gradient ``ds`` (None: zero).  dx is the
+        residual's gradient too.  Straight through the rounding of y."""
+        lib = _lib.load()
+        _need_device("add_rms_norm_backward", dy, s, weight, ds)
+        w, (dyc, sc, dsc) = self._norm_check("add_rms_norm_backward", eps, weight, dy, s, ds)
+        d, dev = s.shape[-1], s.device
+        T = sc.numel() // d
+        dx = torch.empty(s.shape, dtype=s.dtype, device=dev)
+        dw = torch.empty(d, dtype=torch.float32, device=dev) if need_dw else None
+        nws = lib.smaul_add_rms_norm_backward_workspace_size(T, d) if need_dw else 0
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws > 0 else None
+        with _device(dev):
+            rc = lib.smaul_add_rms_norm_backward(dyc.data_ptr(), sc.data_ptr(), None if dsc is None else dsc.data_ptr(),
+                                                 _ACT[s.dtype], None if w is None else w.data_ptr(), eps, dx.data_ptr(),
+                                                 None if dw is None else dw.data_ptr(), T, d,
+                                                 None if ws is None else ws.data_ptr(), nws, _stream_handle(dev))
+        _lib.check(rc, "add_rms_norm_backward")
+        return dx, dw
 
     def wait_timeouts(self, device=None, reset=False) -> int:
         """Give-ups of the decode combine's bounded wait on ``device`` since the

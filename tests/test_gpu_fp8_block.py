@@ -1,0 +1,152 @@
+"""Rows in blocks of 128 8-bit codes on the device: quantisation, products and input
+gradients against plain 64-bit forms."""
+import math
+
+import pytest
+import torch
+
+import _fp8_block as ref
+from smaulnative_amd.compute import get_backend
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def be():
+    return get_backend("rocm")
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("K", [1, 7, 127, 128, 129, 500, 512, 513, 1000, 1536])
+def test_quantize_is_the_definition(K, dtype):
+    x = (torch.randn(37, K, generator=gen(K)) * torch.exp(4 * torch.randn(37, 1, generator=gen(K + 1)))).to(dtype)
+    codes, scales = be().fp8_block_quantize(x.to(DEV))
+    want = ref.quantize(x)
+    assert torch.equal(codes.cpu(), want[0]) and torch.equal(scales.cpu(), want[1])
+    for out in (F32, BF):
+        y = be().fp8_block_dequantize(codes, scales, K, out)
+        assert y.dtype == out and torch.equal(y.cpu().double(), ref.values(*want, K))
+
+
+def test_quantize_at_the_borders():
+    """Ties, the largest code and the next scale, subnormals, zeros of both signs, the ends of
+    fp32, infinities and NaN."""
+    grid = ref.GRID
+    mids = (grid[1:] + grid[:-1]) / 2
+    rows = []
+    for e in (0, -20, 100, -118, -119, -126):
+        v = torch.cat([mids, mids * (1 + 2.0 ** -12), mids * (1 - 2.0 ** -12)]).float() * 2.0 ** e
+        v = torch.cat([v, -v])
+        v = torch.nn.functional.pad(v, (0, -v.numel() % 127)).view(-1, 127)
+        rows.append(torch.cat([v, torch.full((v.shape[0], 1), 448.0 * 2.0 ** e)], 1))
+    for top in (448.0, 449.0, 447.0, 256.0, 255.0, 480.0, 511.9, 512.0):
+        rows.append(torch.cat([torch.linspace(-top, top, 127), torch.tensor([top])])[None])
+    x = torch.cat(rows)
+    tiny = torch.zeros(9, 128)
+    tiny[0, 5], tiny[1, 0], tiny[1, 1] = 2.0 ** -149, 2.0 ** -126, -(2.0 ** -130)
+    tiny[2, 3], tiny[2, 4] = 2.0 ** -118, 2.0 ** -140
+    tiny[3] = -0.0
+    tiny[4, 7], tiny[4, 8] = torch.finfo(F32).max, 2.0 ** 118
+    tiny[5, 2], tiny[5, 9] = math.inf, 1.0
+    tiny[6, 2], tiny[6, 9] = math.nan, 1.0
+    tiny[7, 127] = -math.inf
+    x = torch.cat([x, tiny])
+    for t in (x, x.to(BF)):
+        codes, scales = be().fp8_block_quantize(t.to(DEV))
+        want = ref.quantize(t)
+        assert torch.equal(scales.cpu(), want[1])
+        assert torch.equal(codes.cpu(), want[0])
+        y = be().fp8_block_dequantize(codes, scales, 128, F32).cpu().double()
+        v = ref.values(*want, 128).float().double()  # fp32's largest value rounds up to 2^128, which is not one
+        assert torch.equal(torch.isnan(y), torch.isnan(v)) and torch.equal(y[~torch.isnan(v)], v[~torch.isnan(v)])
+
+
+def test_quantize_other_layouts():
+    x = torch.randn(6, 5, 200, generator=gen(0)).to(DEV)
+    want = ref.quantize(x.cpu())
+    for t in (x, x.transpose(0, 1).contiguous().transpose(0, 1), torch.randn(6, 5, 203, device=DEV)[..., 1:201].copy_(x)):
+        codes, scales = be().fp8_block_quantize(t)
+        assert torch.equal(codes.cpu(), want[0]) and torch.equal(scales.cpu(), want[1])
+    codes, scales = be().fp8_block_quantize(x[:0])
+    assert codes.shape == (0, 5, 256) and scales.shape == (0, 5, 4)
+    assert be().fp8_block_dequantize(codes, scales, 200).shape == (0, 5, 200)
+
+
+ROWS = [1, 2, 31, 33, 64, 65, 200, 515]
+
+
+@pytest.mark.parametrize("K,N", [(1, 1), (64, 31), (128, 128), (129, 130), (640, 513), (1000, 777), (2048, 260)])
+@pytest.mark.parametrize("rows", ROWS)
+def test_forward(rows, K, N):
+    g = gen(rows * K + N)
+    w, s = ref.weight(N, K, g)
+    wv = ref.values(w, s, K)
+    x = torch.randn(rows, K, generator=g) * torch.exp(torch.randn(rows, 1, generator=g))
+    wd, sd = w.to(DEV), s.to(DEV)
+    for dtype in (BF, F32):
+        t = x.to(dtype)
+        y = be().fp8_block_forward(t.to(DEV), wd, sd, K, N)
+        assert y.dtype == dtype
+        ref.check(y, *ref.product(ref.rounded(t), wv, dtype), (rows, K, N, dtype))
+        c, cs = ref.quantize(t)
+        again = be().fp8_block_forward(c.to(DEV), wd, sd, K, N, xs=cs.to(DEV), dtype=dtype)
+        assert torch.equal(y, again)
+    assert be().fp8_block_forward(c.to(DEV), wd, sd, K, N, xs=cs.to(DEV)).dtype == BF
+
+
+def test_forward_layouts_and_leading_dimensions():
+    K, N = 200, 96
+    g = gen(1)
+    w, s = (t.to(DEV) for t in ref.weight(N, K, g))
+    x = torch.randn(4, 25, K, generator=g).to(BF).to(DEV)
+    want = be().fp8_block_forward(x.view(100, K), w, s, K, N)
+    assert torch.equal(be().fp8_block_forward(x, w, s, K, N), want.view(4, 25, N))
+    wide = torch.zeros(100, K + 3, dtype=BF, device=DEV)
+    wide[:, 1:K + 1] = x.view(100, K)
+    assert torch.equal(be().fp8_block_forward(wide[:, 1:K + 1], w, s, K, N), want)
+    off = torch.zeros(w.numel() + 3, dtype=torch.uint8, device=DEV)
+    off[3:] = w.view(-1)
+    soff = torch.zeros(s.numel() + 1, dtype=torch.uint8, device=DEV)
+    soff[1:] = s.view(-1)
+    assert torch.equal(be().fp8_block_forward(x.view(100, K), off[3:].view(N, -1), soff[1:].view(N, -1), K, N), want)
+    assert be().fp8_block_forward(x[:0], w, s, K, N).shape == (0, 25, N)
+
+
+@pytest.mark.parametrize("rows", [3, 64, 300])
+def test_forward_with_infinities_and_nan(rows):
+    """A block that holds one is all NaN: its row's outputs are, and no other's."""
+    K, N = 300, 140
+    g = gen(rows)
+    w, s = ref.weight(N, K, g)
+    x = torch.randn(rows, K, generator=g)
+    clean = be().fp8_block_forward(x.to(DEV), w.to(DEV), s.to(DEV), K, N).cpu()
+    x[1, 7], x[rows - 1, 299] = math.inf, math.nan
+    y = be().fp8_block_forward(x.to(DEV), w.to(DEV), s.to(DEV), K, N).cpu()
+    bad = torch.zeros(rows, dtype=torch.bool)
+    bad[1] = bad[rows - 1] = True
+    assert torch.isnan(y[bad]).all() and torch.equal(y[~bad], clean[~bad])
+    s[5, 1] = 255
+    y = be().fp8_block_forward(x.to(DEV), w.to(DEV), s.to(DEV), K, N).cpu()
+    assert torch.isnan(y[:, 5]).all()
+    keep = [n for n in range(N) if n != 5]
+    assert torch.equal(y[~bad][:, keep], clean[~bad][:, keep])
+
+
+@pytest.mark.parametrize("K,N", [(1, 1), (64, 31), (128, 128), (129, 130), (513, 640), (777, 1000), (260, 2048)])
+@pytest.mark.parametrize("rows", ROWS)
+def test_backward_input(rows, K, N):
+    g = gen(rows * K + N)
+    w, s = ref.weight(N, K, g)
+    wv = ref.values(w, s, K)
+    dy = torch.randn(rows, N, generator=g) * torch.exp(torch.randn(rows, 1, generator=g))
+    for dtype in (BF, F32):
+        t = dy.to(dtype)
+        dx = be().fp8_block_backward_input(t.to(DEV), w.to(DEV), s.to(DEV), K, N)
+        assert dx.dtype == dtype
+        ref.check(dx, *ref.product(t.double(), wv.t().contiguous(), dtype), (rows, K, N, dtype))
+    assert be().fp8_block_backward_input(t[:0].to(DEV), w.to(DEV), s.to(DEV), K, N).shape == (0, K)
