@@ -33,9 +33,12 @@ HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
     "-ffp-contract=off",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-    "-mllvm", "-amdgpu-mfma-vgpr-form",
     "-I" + os.path.join(REPO, "include"), "-I" + CSRC,
 ]
+
+MFMA_VGPR_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+# sums that stay on the matrix cores until they are stored: in AGPRs, beside 256 other registers
+AGPR_SOURCES = ("fp8_block.hip",)
 
 
 def hipcc() -> str:
@@ -47,7 +50,8 @@ def hipcc() -> str:
 
 def _compile(src: str) -> str:
     obj = os.path.join(OBJDIR, os.path.basename(src) + ".o")
-    res = subprocess.run([hipcc()] + HIPCC_FLAGS + ["-c", src, "-o", obj], capture_output=True, text=True)
+    flags = HIPCC_FLAGS + ([] if os.path.basename(src) in AGPR_SOURCES else MFMA_VGPR_FLAGS)
+    res = subprocess.run([hipcc()] + flags + ["-c", src, "-o", obj], capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"hipcc failed on {src} ({res.returncode}):\n{res.stderr[-4000:]}")
     return obj, res.stderr

@@ -7,7 +7,10 @@
 //   block:   h = Q(silu(x Wg^T) * (x Wu^T)),  y = h Wd^T
 //   its gradients, straight through the roundings: dh = dy Wd, dg = dh u silu'(g),
 //   du = dh silu(g), dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
+#include <utility>
+
 #include "fp8_block.h"
+#include "lds_dma.h"
 
 using smaul::check_launch;
 using smaul::cu_count;
@@ -126,39 +129,558 @@ int launch_product(const FbProduct& p, hipStream_t stream) {
   return check_launch("fb_product_kernel");
 }
 
-// gate's and up's sums [T, h] -> the hidden rows' codes and, to keep, u silu'(g) and
-// silu(g) in their place
-__global__ void __launch_bounds__(256)
-fb_gated_kernel(float* __restrict__ g, float* __restrict__ u, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                int64_t T, int64_t h, int keep) {
-  const int64_t nb = fb_blocks(h), i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = i / (nb * 16), c = i - row * nb * 16;
-  if (row >= T) return;
-  float a[8], b[8], v[8];
-  fb_load8<false>(g, row, h, c * 8, a);
-  fb_load8<false>(u, row, h, c * 8, b);
+// ---------------------------------------------------------------------------
+// products of codes
+// ---------------------------------------------------------------------------
+// What a tile's sums become: bf16 or fp32 rows, or the gated block's hidden rows as codes.
+enum { O_BF16 = 0, O_F32 = 1, O_GATED = 2 };
+
+struct FbArgs {
+  const uint8_t* x;   // R rows of ldx codes
+  const uint8_t* xs;  // their scales, `words` dwords a row
+  const uint8_t* w;   // N rows
+  const uint8_t* s;
+  const uint8_t* w2;  // O_GATED: up's (w, s are gate's)
+  const uint8_t* s2;
+  void* y;            // [R][N] (O_GATED: codes [R][fb_width(N)])
+  uint8_t* ys;        // O_GATED: scales
+  uint8_t* kept;      // O_GATED: what the gradients take, or null
+  int64_t R, N, ldx;  // ldx: of x and w, a multiple of 128
+  int words;
+};
+
+// The kept factors a = u silu'(g) and b = silu(g), 24 bits each: a record of 96 bytes for
+// 16 consecutive hidden values of a row: a's high halves, b's, a's third bytes, b's.
+// (bf16 alone would add its rounding twice to the gradients'.)
+constexpr int FB_RECORD = 96;
+__host__ __device__ __forceinline__ int64_t fb_kept_row(int64_t h) { return fb_width(h) / 16 * FB_RECORD; }
+
+// 16 fp32 to 24 bits, to nearest: high halves and third bytes
+__device__ __forceinline__ void fb_pack24(const float (&v)[16], uint4 (&hi)[2], uint4& lo) {
+  uint32_t u[16];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float sig = 1.0f / (1.0f + expf(-a[j])), si = a[j] * sig;
-    v[j] = si * b[j];
-    a[j] = b[j] * sig * (1.0f + a[j] * (1.0f - sig));
-    b[j] = si;
+  for (int r = 0; r < 16; ++r) {
+    const uint32_t b = __float_as_uint(v[r]);
+    u[r] = (b & 0x7f800000u) == 0x7f800000u ? (b & 0x7fffffu ? b | 0x400000u : b) : b + 0x7fu + ((b >> 8) & 1u);
   }
-  fb_write8(codes, scales, row, nb, c, v);
-  if (keep && c * 8 < h) {
-    fb_store8<false>(g, row, h, c * 8, a);
-    fb_store8<false>(u, row, h, c * 8, b);
+  uint32_t h[8], l[4];
+#pragma unroll
+  for (int r = 0; r < 8; ++r) h[r] = __builtin_amdgcn_perm(u[2 * r + 1], u[2 * r], 0x07060302u);
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    l[r] = (u[4 * r] >> 8 & 255u) | (u[4 * r + 1] & 0xff00u) | (u[4 * r + 2] << 8 & 0xff0000u) |
+           (u[4 * r + 3] << 16 & 0xff000000u);
+  hi[0] = make_uint4(h[0], h[1], h[2], h[3]);
+  hi[1] = make_uint4(h[4], h[5], h[6], h[7]);
+  lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+__device__ __forceinline__ void fb_unpack24(const uint4 (&hi)[2], const uint4& lo, float (&v)[16]) {
+  const uint32_t h[8] = {hi[0].x, hi[0].y, hi[0].z, hi[0].w, hi[1].x, hi[1].y, hi[1].z, hi[1].w};
+  const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    v[r] = __uint_as_float((r & 1 ? h[r / 2] & 0xffff0000u : h[r / 2] << 16) | (l[r / 4] >> (8 * (r & 3)) & 255u) << 8);
+}
+
+// silu(g) u, u silu'(g) and silu(g)
+__device__ __forceinline__ float fb_gated(float g, float u, float& a, float& b) {
+  const float sig = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-g * 1.4426950408889634f));
+  b = g * sig;
+  a = u * (sig * fmaf(g, 1.0f - sig, 1.0f));
+  return b * u;
+}
+
+// f(0), ..., f(N - 1), each with its number as a constant
+template <class F, int... I>
+__device__ __forceinline__ void fb_each(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void fb_each(F&& f) {
+  fb_each(f, std::make_integer_sequence<int, N>{});
+}
+
+// K in stages of 128 (a block, 128-byte rows), codes brought to LDS by DMA, two stages;
+// scales in chunks of 16 stages.  Roles: the weight's rows are the matrix instruction's
+// rows and x's its columns, and row i of a 32 x 32 tile is given weight row 16 ((i / 4) %
+// 2) + 4 (i / 8) + i % 4, so that the 16 sums of a lane are 16 consecutive outputs of one
+// row of x.
+template <int BM, int BN, int WM, int WN>
+struct FbCfg {
+  static constexpr int NW = WM * WN, XB = BM * 128, WB = BN * 128, STAGE = XB + WB;
+  static constexpr int X_INS = XB / (1024 * NW), W_INS = WB / (1024 * NW), S_INS = (BM + BN) / (16 * NW);
+  static constexpr int SC = (BM + BN) * 16;  // a chunk of scales: 4 dwords a row
+  static constexpr int TT = BM / WM / 32, WT = BN / WN / 32;
+  static constexpr int LDS = 2 * STAGE + 2 * SC;
+  static_assert(XB % (1024 * NW) == 0 && WB % (1024 * NW) == 0 && (BM + BN) % (16 * NW) == 0 && BN % 16 == 0,
+                "whole DMA instructions");
+};
+
+__device__ __forceinline__ int fb_perm(int i) { return ((i >> 2) & 1) * 16 + (i >> 3) * 4 + (i & 3); }
+
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ i32x8_t fb_operand(uint4 a, uint4 b) {
+  i32x8_t r;
+  r[0] = (int)a.x; r[1] = (int)a.y; r[2] = (int)a.z; r[3] = (int)a.w;
+  r[4] = (int)b.x; r[5] = (int)b.y; r[6] = (int)b.z; r[7] = (int)b.w;
+  return r;
+}
+
+// 8 codes -> 8 bf16 (exact), times s
+__device__ __forceinline__ bf16x8_t fb_decode8(int lo, int hi, float s) {
+  uint4 r;
+  r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)lo, s, false));
+  r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)lo, s, true));
+  r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)hi, s, false));
+  r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)hi, s, true));
+  return __builtin_bit_cast(bf16x8_t, r);
+}
+
+// sums stay in AGPRs up to here: moved out early they would not fit the other registers
+__device__ __forceinline__ void fb_pin(f32x16_t& v) { asm volatile("" : "+a"(v)); }
+
+// tile `lin` of m_tiles by n_tiles, in groups of 8 row tiles by all column tiles
+__device__ __forceinline__ void fb_tile_at(int lin, int m_tiles, int n_tiles, int& mt, int& nt) {
+  constexpr int GM = 8;
+  const int g = lin / (GM * n_tiles), within = lin - g * GM * n_tiles, gm = min(GM, m_tiles - g * GM);
+  mt = g * GM + within % gm;
+  nt = within / gm;
+}
+
+// v_mfma_scale_f32_32x32x64_f8f6f4: lane i + 32 g has 32 values of row i and one scale
+// byte for them.  It sums 32 bits wide, but 8 neighbouring products are first aligned to
+// the largest of them and lose what is below 2^-13 of it: 1.5e-5 of a sum of normal values
+// in the mean, a hundredth of bf16's own rounding.  fp32 results are not formed so: their
+// codes are decoded (exactly) and multiplied as bf16, at half the rate.  The operands of a step (64 values) are read while the step before is
+// multiplied, the first of a stage during the last of the stage before; by then every
+// wave has the rest of its stage in registers, so that one barrier frees the buffer for
+// the loads of the stage after the next.  A workgroup walks a band of tiles as one
+// sequence of stages.
+template <int OT, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(WM * WN * 64, WM * WN == 4 && BM * BN > 128 * 128 ? 1 : 2)
+fb_codes_kernel(FbArgs p, int m_tiles, int n_tiles) {
+  using C = FbCfg<BM, BN, WM, WN>;
+  constexpr bool GATED = OT == O_GATED;
+  constexpr int TT = C::TT, WT = C::WT, BNO = GATED ? BN / 2 : BN, NW = C::NW;
+  constexpr int OWN = GATED ? 0 : 4096, AMAX = GATED ? BM * WN * 4 : 0;
+  static_assert(!GATED || BNO == FB_BLOCK, "a tile of hidden rows is a block");
+  __shared__ __attribute__((aligned(1024))) char smem[C::LDS + NW * OWN + AMAX];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN, g = lane >> 5, l32 = lane & 31;
+  const uint32_t lds0 = lds_offset(&smem[0]);
+  const int nk = (int)(p.ldx / 128);
+
+  // XCD x (workgroup b runs on XCD b % 8) takes a contiguous band of the tiles
+  const int wgs = gridDim.x, nx = min(8, wgs), xcd = (int)blockIdx.x % nx, step = (wgs - xcd + nx - 1) / nx;
+  const int total = m_tiles * n_tiles, last = (int)((int64_t)total * (xcd + 1) / nx);
+  int lin = (int)((int64_t)total * xcd / nx) + (int)blockIdx.x / nx;
+  if (lin >= last) return;
+
+  // where a lane's loads of a tile read: 32-bit offsets from its first rows; rows past the
+  // end read the last one, their sums are not stored
+  const uint8_t *X, *W, *XS, *WS;  // gate's; up's stand as far from them as the matrices from each other
+  const int64_t to_w2 = GATED ? p.w2 - p.w : 0, to_s2 = GATED ? p.s2 - p.s : 0;
+  uint32_t x_off[C::X_INS], w_off[C::W_INS], s_off[C::S_INS];
+  // staged weight row r, from the tile's first: tiles of 32 (gate's, then up's), permuted
+  auto w_row = [&](int r, int left) __attribute__((always_inline)) -> int {
+    int t = r >> 5;
+    if (GATED) t = t >= BN / 64 ? t - BN / 64 : t;
+    return min(t * 32 + fb_perm(r & 31), left);
+  };
+  const uint32_t ld = (uint32_t)p.ldx, sl = (uint32_t)p.words * 4;
+  bool offsets = true;  // are to be computed
+  auto source = [&](int at) __attribute__((always_inline)) {
+    int mt, nt;
+    fb_tile_at(at, m_tiles, n_tiles, mt, nt);
+    const int64_t row0 = (int64_t)mt * BM, n0 = (int64_t)nt * BNO;
+    const int xleft = (int)min<int64_t>(p.R - 1 - row0, BM - 1), wleft = (int)min<int64_t>(p.N - 1 - n0, BNO - 1);
+    X = p.x + row0 * ld;
+    XS = p.xs + row0 * sl;
+    W = p.w + n0 * ld;
+    WS = p.s + n0 * sl;
+    const bool ragged = xleft < BM - 1 || wleft < BNO - 1;
+    if (!ragged && !offsets) return;  // a whole tile's offsets are there from the one before
+    offsets = ragged;
+    int me = lane;  // nothing of this is kept in registers from tile to tile
+    asm volatile("" : "+v"(me));
+#pragma unroll
+    for (int a = 0; a < C::X_INS; ++a) {
+      const int r = (wave * C::X_INS + a) * 8 + me / 8;
+      x_off[a] = (uint32_t)min(r, xleft) * ld + (uint32_t)((me % 8 ^ swz_a(r)) * 16);
+    }
+#pragma unroll
+    for (int b = 0; b < C::W_INS; ++b) {
+      const int r = (wave * C::W_INS + b) * 8 + me / 8;
+      w_off[b] = (uint32_t)w_row(r, wleft) * ld + (uint32_t)((me % 8 ^ swz_a(r)) * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < C::S_INS; ++i) {
+      const int r = (wave * C::S_INS + i) * 16 + me / 4;
+      s_off[i] = (uint32_t)(r < BN ? w_row(r, wleft) : min(r - BN, xleft)) * sl;
+    }
+  };
+  // the sequence's next stage to load, of this tile or one after (behind the last tile its
+  // stages again, into buffers that nobody reads): its scales where a chunk begins, its
+  // codes one DMA instruction at a time
+  constexpr int INS = C::X_INS + C::W_INS;
+  int load_at = lin, load_k = nk, load_chunk = 0;
+  auto load_begin = [&]() __attribute__((always_inline)) {
+    if (load_k == nk) {
+      if (load_at < last) source(load_at);
+      load_at += step;
+      load_k = 0;
+    }
+    if (load_k % 16 == 0) {
+      const int word = min(load_k / 4 + lane % 4, p.words - 1) * 4;
+#pragma unroll
+      for (int i = 0; i < C::S_INS; ++i) {
+        const int r = (wave * C::S_INS + i) * 16;
+        const uint8_t* from = WS + (GATED && r >= BN / 2 ? to_s2 : 0);
+        if (r >= BN) from = XS;
+        dma4(from, s_off[i] + word, lds0 + 2 * C::STAGE + load_chunk * C::SC + (wave * C::S_INS + i) * 256);
+      }
+      load_chunk ^= 1;
+    }
+  };
+  auto load_one = [&](int buf, int q) __attribute__((always_inline)) {
+    const uint32_t l = lds0 + (uint32_t)(buf * C::STAGE);
+    const int64_t at = (int64_t)load_k * 128;
+    if (q < C::X_INS) {
+      dma16(X + at, x_off[q < C::X_INS ? q : 0], l + (wave * C::X_INS + q) * 1024);
+    } else {
+      const int b = q - C::X_INS, r = (wave * C::W_INS + b) * 8;
+      dma16(W + at + (GATED && r >= BN / 2 ? to_w2 : 0), w_off[b < 0 ? 0 : b], l + C::XB + (wave * C::W_INS + b) * 1024);
+    }
+  };
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    load_begin();
+#pragma unroll
+    for (int q = 0; q < INS; ++q) load_one(b, q);
+    ++load_k;
   }
+  wait_vm<INS>();
+  __syncthreads();
+
+  // staged row of weight tile j of this wave: its gate tiles, then its up tiles
+  auto w_tile = [&](int j) __attribute__((always_inline)) -> int {
+    if constexpr (GATED)
+      return j < WT / 2 ? wn * (BN / WN / 2) + j * 32 : BN / 2 + wn * (BN / WN / 2) + (j - WT / 2) * 32;
+    else return wn * (BN / WN) + j * 32;
+  };
+  i32x8_t wf[2][WT], xf[2][TT];
+  uint32_t sw[WT], sx[TT], nw[WT], nx_[TT];
+  // this lane's 16 bytes of a stage's first step; the others are an XOR away.  Tiles are 32
+  // rows apart, which the swizzle does not see.
+  const uint32_t first = (uint32_t)(l32 * 128 + (2 * g ^ swz_a(l32)) * 16);
+  constexpr int READS = 2 * (TT + WT), S = TT * WT;
+  auto read_one = [&](int buf, int u, int q) __attribute__((always_inline)) {  // half q % 2 of operand q / 2 of step u
+    const char* at = smem + buf * C::STAGE + (first ^ (uint32_t)(u * 64 + q % 2 * 16));
+    const int o = q / 2, j = o - TT;
+    const uint4 v = o < TT ? *(const uint4*)(at + (wm * (BM / WM) + o * 32) * 128)
+                           : *(const uint4*)(at + C::XB + w_tile(j) * 128);
+    i32x8_t& r = o < TT ? xf[u][o < TT ? o : 0] : wf[u][j < 0 ? 0 : j];
+    r[q % 2 * 4] = (int)v.x; r[q % 2 * 4 + 1] = (int)v.y; r[q % 2 * 4 + 2] = (int)v.z; r[q % 2 * 4 + 3] = (int)v.w;
+  };
+  // four stages' scales of this lane's rows, from the chunk
+  auto read_scales = [&](int chunk, int word) __attribute__((always_inline)) {
+    const char* at = smem + 2 * C::STAGE + chunk * C::SC + l32 * 16 + word * 4;
+#pragma unroll
+    for (int j = 0; j < WT; ++j) nw[j] = *(const uint32_t*)(at + w_tile(j) * 16);
+#pragma unroll
+    for (int i = 0; i < TT; ++i) nx_[i] = *(const uint32_t*)(at + (BN + wm * (BM / WM) + i * 32) * 16);
+  };
+  f32x16_t acc[WT][TT];
+  // product s of step u
+  auto multiply = [&](int u, int s, bool fresh) __attribute__((always_inline)) {
+    const f32x16_t zero = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    const int j = s / TT, i = s % TT;
+    const f32x16_t c = fresh && u == 0 ? zero : acc[j][i];
+    if constexpr (OT == O_F32) {
+      acc[j][i] = c;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const bf16x8_t x = fb_decode8(xf[u][i][2 * q], xf[u][i][2 * q + 1], fb_scale(sx[i] & 255u));
+        const bf16x8_t w = fb_decode8(wf[u][j][2 * q], wf[u][j][2 * q + 1], fb_scale(sw[j] & 255u));
+        acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, x, acc[j][i], 0, 0, 0);
+      }
+    } else {
+      acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[u][j], xf[u][i], c, 0, 0, 0, (int)sw[j], 0,
+                                                                 (int)sx[i]);
+    }
+  };
+  auto pin = [&](int n) __attribute__((always_inline)) {  // the first n products stay on their side of a branch or barrier
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      if (s < n) fb_pin(acc[s / TT][s % TT]);
+  };
+  int buf = 0, chunk = 0;
+  // One stage: 2 S products, the rest issued in their shadow.  The second step's operands
+  // are read first; from product B1 on no wave reads this buffer any more, and the loads of
+  // the stage after the next follow, spread out so that they do not queue; from product B2
+  // on the next stage's first operands are read, behind a wait that leaves the loads issued
+  // in this stage (DONE of them by then) in flight.
+  constexpr int B1 = S * 5 / 8, B2 = S + S * 5 / 16, SPAN = 2 * S - 2 - B1;
+  constexpr int STORED = GATED ? TT * WT / 2 : TT * WT * (OT == O_BF16 ? 2 : 4);
+  int stored = 0;
+  constexpr int DONE = ((B2 - 1 - B1) * INS + SPAN - 1) / SPAN;  // of products B1 to B2 - 2
+  auto stage = [&](int kt, bool fresh) __attribute__((always_inline)) {
+    const int sh = kt % 4 * 8, next = kt + 1 == nk ? 0 : kt + 1;
+#pragma unroll
+    for (int j = 0; j < WT; ++j) sw[j] = nw[j] >> sh;
+#pragma unroll
+    for (int i = 0; i < TT; ++i) sx[i] = nx_[i] >> sh;
+    if (next % 16 == 0) chunk ^= 1;
+    fb_each<2 * S>([&](auto number) __attribute__((always_inline)) {
+      constexpr int s = number;
+      if constexpr (s == B1) {
+        pin(fresh ? B1 : S);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        load_begin();
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      multiply(s / S, s % S, fresh);
+      if constexpr (s == B2 - 1) {
+        __builtin_amdgcn_sched_barrier(0);
+        // memory operations are done in order: behind a tile's stores, of which `stored` at
+        // least were issued, the loads before them are waited for alone
+        if (fresh && stored) wait_vm<(DONE + STORED < 63 ? DONE + STORED : 63)>();
+        else wait_vm<DONE>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        read_scales(chunk, next / 4 % 4);
+      }
+      fb_each<READS>([&](auto part) __attribute__((always_inline)) {
+        constexpr int q = part;
+        if constexpr (q * (S / 2) / READS == s) read_one(buf, 1, q);
+        if constexpr (B2 + q * (2 * S - B2) / READS == s) read_one(buf ^ 1, 0, q);  // behind the last tile: unused
+      });
+      fb_each<INS>([&](auto part) __attribute__((always_inline)) {
+        constexpr int q = part;
+        if constexpr (B1 + q * SPAN / INS == s) load_one(buf, q);
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    ++load_k;
+    buf ^= 1;
+  };
+
+#pragma unroll
+  for (int q = 0; q < READS; ++q) read_one(0, 0, q);
+  read_scales(0, 0);
+  for (; lin < last; lin += step) {
+    stage(0, true);
+    for (int kt = 1; kt < nk; ++kt) stage(kt, false);
+    pin(S);
+    int mt, nt;
+    fb_tile_at(lin, m_tiles, n_tiles, mt, nt);
+    const int64_t row0 = (int64_t)mt * BM, n0 = (int64_t)nt * BNO;
+    const int rows = (int)min<int64_t>(BM, p.R - row0);
+    int el = lane;  // the stores' addresses are not kept in registers across the loop
+    asm volatile("" : "+v"(el));
+    const int eg = el >> 5, e32 = el & 31;
+    if constexpr (GATED) {
+      constexpr int HT = WT / 2;
+      float* sh = (float*)(smem + C::LDS);
+      const int64_t nb = fb_blocks(p.N);
+      float top[TT];
+#pragma unroll
+      for (int i = 0; i < TT; ++i) {
+        const int lr = wm * (BM / WM) + i * 32 + e32;
+        float m = 0.0f;
+#pragma unroll
+        for (int j = 0; j < HT; ++j) {
+          const int64_t n = n0 + wn * (BNO / WN) + j * 32 + eg * 16;
+          const int left = (int)min<int64_t>(p.N - n, 16);
+          fb_pin(acc[j][i]);
+          fb_pin(acc[j + HT][i]);
+          float a[16], b[16];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            float v = fb_gated(acc[j][i][r], acc[j + HT][i][r], a[r], b[r]);
+            v = r < left ? v : 0.0f;  // past N: copies of the last row's
+            acc[j][i][r] = v;
+            m = __builtin_elementwise_maximum(m, __builtin_fabsf(v));  // NaN stays NaN
+          }
+          fb_pin(acc[j][i]);
+          if (p.kept && lr < rows) {
+            uint4 hi[2], lo;
+            char* rec = (char*)p.kept + (row0 + lr) * fb_kept_row(p.N) + n / 16 * FB_RECORD;
+            fb_pack24(a, hi, lo);
+            ((uint4*)rec)[0] = hi[0];
+            ((uint4*)rec)[1] = hi[1];
+            ((uint4*)rec)[4] = lo;
+            fb_pack24(b, hi, lo);
+            ((uint4*)rec)[2] = hi[0];
+            ((uint4*)rec)[3] = hi[1];
+            ((uint4*)rec)[5] = lo;
+          }
+        }
+        m = __builtin_elementwise_maximum(m, __shfl_xor(m, 32, 64));
+        top[i] = m;
+        if (WN > 1 && eg == 0) sh[lr * WN + wn] = m;
+      }
+      if constexpr (WN > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TT; ++i)
+#pragma unroll
+          for (int q = 0; q < WN; ++q)
+            top[i] = __builtin_elementwise_maximum(top[i], sh[(wm * (BM / WM) + i * 32 + e32) * WN + q]);
+      }
+#pragma unroll
+      for (int i = 0; i < TT; ++i) {
+        const int lr = wm * (BM / WM) + i * 32 + e32;
+        const uint32_t byte = fb_scale_byte(__float_as_uint(top[i]) & 0x7fffffffu);
+        if (lr < rows) {
+#pragma unroll
+          for (int j = 0; j < HT; ++j) {
+            fb_pin(acc[j][i]);
+            float v[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) v[r] = acc[j][i][r];
+            const uint2 lo = fb_encode8(v, byte), hi = fb_encode8(v + 8, byte);
+            *(uint4*)((uint8_t*)p.y + (row0 + lr) * nb * FB_BLOCK + n0 + wn * (BNO / WN) + j * 32 + eg * 16) =
+                make_uint4(lo.x, lo.y, hi.x, hi.y);
+          }
+          if (wn == 0 && eg == 0) {
+            uint8_t* s = p.ys + (row0 + lr) * ((nb + 3) / 4 * 4);
+            s[nt] = (uint8_t)byte;
+            if (nt + 1 == nb)
+              for (int64_t q = nb; q < (nb + 3) / 4 * 4; ++q) s[q] = 0;
+          }
+        }
+      }
+      if constexpr (WN > 1) __syncthreads();  // the maxima's LDS is free for the next tile
+      stored = rows == BM ? TT * HT : 0;
+    } else {
+      // rows leave as whole lines, 32 at a time, through 4 KB of LDS of the wave's own,
+      // 16-byte chunks changing places by the row; a wave's LDS accesses are done in order
+      constexpr int ES = OT == O_BF16 ? 2 : 4, UJ = 4 / ES, UNITS = TT * WT / UJ;
+      const bool whole = rows == BM && n0 + BN <= p.N && p.N % (16 / ES) == 0;  // of the whole workgroup
+      char* own = smem + C::LDS + wave * OWN;
+      char* out = (char*)p.y + ((row0 + wm * (BM / WM)) * p.N + n0 + wn * (BN / WN)) * ES;
+      uint4 d0, d1, d2, d3;
+      auto to_lds = [&](int i, int j) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < UJ; ++h) {
+          fb_pin(acc[j + h][i]);
+          const f32x16_t v = acc[j + h][i];
+#pragma unroll
+          for (int q = 0; q < ES; ++q) {
+            const int c = h * 4 + ES * eg + q, r = q * (16 / ES);
+            uint4 u;
+            if constexpr (OT == O_BF16)
+              u = make_uint4(pack_bf16(v[r], v[r + 1]), pack_bf16(v[r + 2], v[r + 3]), pack_bf16(v[r + 4], v[r + 5]),
+                             pack_bf16(v[r + 6], v[r + 7]));
+            else
+              u = make_uint4(__float_as_uint(v[r]), __float_as_uint(v[r + 1]), __float_as_uint(v[r + 2]),
+                             __float_as_uint(v[r + 3]));
+            *(uint4*)(own + e32 * 128 + (c ^ (e32 & 7)) * 16) = u;
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
+      };
+      if (whole) {
+        const uint32_t ldy = (uint32_t)p.N * ES;
+        auto store = [&](int u) __attribute__((always_inline)) {
+          char* at = out + (int64_t)(u / (WT / UJ) * 32) * ldy + u % (WT / UJ) * 128;
+          const uint32_t o = (uint32_t)(el / 8) * ldy + el % 8 * 16;
+          *(uint4*)(at + o) = d0;
+          *(uint4*)(at + o + 8 * ldy) = d1;
+          *(uint4*)(at + o + 16 * ldy) = d2;
+          *(uint4*)(at + o + 24 * ldy) = d3;
+        };
+        fb_each<UNITS + 1>([&](auto unit) __attribute__((always_inline)) {  // stored while the next is read
+          constexpr int u = unit;
+          if constexpr (u < UNITS) to_lds(u / (WT / UJ), u % (WT / UJ) * UJ);
+          if constexpr (u > 0) store(u - 1);
+          if constexpr (u < UNITS) {
+            const char* at = own + (el / 8) * 128 + (el % 8 ^ el / 8) * 16;
+            d0 = *(const uint4*)at;
+            d1 = *(const uint4*)(at + 1024);
+            d2 = *(const uint4*)(at + 2048);
+            d3 = *(const uint4*)(at + 3072);
+            __builtin_amdgcn_wave_barrier();
+          }
+        });
+      } else {
+        fb_each<UNITS>([&](auto unit) __attribute__((always_inline)) {
+          constexpr int u = unit;
+          const int i = u / (WT / UJ), j = u % (WT / UJ) * UJ, tr = wm * (BM / WM) + i * 32;
+          to_lds(i, j);
+          const int64_t n = n0 + wn * (BN / WN) + j * 32;
+#pragma nounroll
+          for (int e = el; e < 32 * (128 / ES); e += 64) {
+            const int r = e / (128 / ES), c = e % (128 / ES), b = c * ES;
+            const char* v = own + r * 128 + (b / 16 ^ (r & 7)) * 16 + b % 16;
+            const int64_t at = (row0 + tr + r) * p.N + n + c;
+            if (tr + r < rows && n + c < p.N) {
+              if constexpr (OT == O_BF16) ((uint16_t*)p.y)[at] = *(const uint16_t*)v;
+              else ((float*)p.y)[at] = *(const float*)v;
+            }
+          }
+          __builtin_amdgcn_wave_barrier();
+        });
+      }
+      stored = whole ? UNITS * 4 : 0;
+    }
+  }
+  wait_vm<0>();
+}
+
+template <int OT, int BM, int BN, int WM, int WN>
+int launch_codes_cfg(const FbArgs& p, hipStream_t stream) {
+  constexpr int BNO = OT == O_GATED ? BN / 2 : BN;
+  const int64_t mt = (p.R + BM - 1) / BM, nt = (p.N + BNO - 1) / BNO;
+  if ((BM > BN ? BM : BN) * p.ldx >= 1LL << 32) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block product: rows too wide");
+  if (mt * nt > 2147483647LL || mt > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block product: too many tiles");
+  const int64_t wgs = cu_count() * (BM * BN <= 128 * 128 ? 2 : 1);
+  hipLaunchKernelGGL((fb_codes_kernel<OT, BM, BN, WM, WN>), dim3((unsigned)(mt * nt < wgs ? mt * nt : wgs)),
+                     dim3(WM * WN * 64), 0, stream, p, (int)mt, (int)nt);
+  return check_launch("fb_codes_kernel");
+}
+
+template <int OT>
+int launch_codes(const FbArgs& p, hipStream_t stream) {
+  return launch_codes_cfg<OT, 256, 256, 2, 2>(p, stream);
+}
+
+FbArgs codes_args(const void* x, const uint8_t* xs, const uint8_t* w, const uint8_t* s, void* y, int64_t R, int64_t K,
+                  int64_t N) {
+  FbArgs p{};
+  p.x = (const uint8_t*)x;
+  p.xs = xs;
+  p.w = w;
+  p.s = s;
+  p.y = y;
+  p.R = R;
+  p.N = N;
+  p.ldx = fb_width(K);
+  p.words = (int)fb_words(K);
+  return p;
 }
 
 // dh -> dg and du, by the factors that the forward pass kept
 __global__ void __launch_bounds__(256)
-fb_gated_backward_kernel(const float* __restrict__ dh, const float* __restrict__ a, const float* __restrict__ b,
-                         float* __restrict__ dg, float* __restrict__ du, int64_t n) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  dg[i] = dh[i] * a[i];
-  du[i] = dh[i] * b[i];
+fb_gated_backward_kernel(const float* __restrict__ dh, const uint8_t* __restrict__ kept, float* __restrict__ dg,
+                         float* __restrict__ du, int64_t T, int64_t h) {
+  const int64_t nr = fb_width(h) / 16, i = (int64_t)blockIdx.x * 256 + threadIdx.x, t = i / nr, c = (i - t * nr) * 16;
+  if (t >= T || c >= h) return;
+  const uint4* rec = (const uint4*)(kept + i * FB_RECORD);
+  float a[16], b[16];
+  fb_unpack24({rec[0], rec[1]}, rec[4], a);
+  fb_unpack24({rec[2], rec[3]}, rec[5], b);
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    if (c + r < h) {
+      const float v = dh[t * h + c + r];
+      dg[t * h + c + r] = v * a[r];
+      du[t * h + c + r] = v * b[r];
+    }
 }
 
 // a workspace laid out part by part
@@ -183,7 +705,7 @@ int launch_quantize(const void* x, int dtype, uint8_t* codes, uint8_t* scales, i
 }
 
 struct FfnParts {
-  int64_t xc, xs, hc, hs, keep, total;
+  int64_t xc, xs, hc, hs, total;
 };
 // what the caller keeps for the gradients stands in `saved` (save), the rest in the workspace
 FfnParts ffn_parts(int64_t T, int64_t d, int64_t h, int x_dtype, bool save) {
@@ -194,7 +716,6 @@ FfnParts ffn_parts(int64_t T, int64_t d, int64_t h, int x_dtype, bool save) {
   q.xs = w.take(rows ? T * fb_words(d) * 4 : 0);
   q.hc = w.take(save ? 0 : T * fb_width(h));
   q.hs = w.take(save ? 0 : T * fb_words(h) * 4);
-  q.keep = w.take(save ? 0 : T * h * 8);
   q.total = w.at;
   return q;
 }
@@ -276,17 +797,8 @@ int smaul_fp8_block_linear(const void* x, int x_dtype, const uint8_t* xs, const 
     x = c;
     xs = cs;
   }
-  FbProduct p{};
-  p.a[0] = codes_mat(x, xs, in_f);
-  p.b[0] = codes_mat(w, s, in_f);
-  p.pairs = 1;
-  p.bf16 = y_dtype == SMAUL_DTYPE_BF16;
-  p.c = y;
-  p.M = rows;
-  p.N = out_f;
-  p.K = in_f;
-  p.ldc = out_f;
-  return launch_product(p, stream);
+  const FbArgs p = codes_args(x, xs, w, s, y, rows, in_f, out_f);
+  return y_dtype == SMAUL_DTYPE_BF16 ? launch_codes<O_BF16>(p, stream) : launch_codes<O_F32>(p, stream);
 }
 
 int64_t smaul_fp8_block_backward_input_workspace_size(int64_t rows, int64_t in_f, int64_t out_f, int dtype) {
@@ -323,7 +835,7 @@ int smaul_fp8_block_backward_input(const void* g, int dtype, const uint8_t* w, c
 
 int64_t smaul_fp8_block_ffn_saved_size(int64_t T, int64_t h) {
   if (T < 0 || h <= 0) return -1;
-  return T * h * 8;
+  return T * fb_kept_row(h);
 }
 
 int64_t smaul_fp8_block_ffn_workspace_size(int64_t T, int64_t d, int64_t h, int x_dtype, int save) {
@@ -363,33 +875,13 @@ int smaul_fp8_block_ffn_forward(const void* x, int x_dtype, const uint8_t* xs, c
   }
   uint8_t* hc = save ? h_codes : ws + q.hc;
   uint8_t* hs = save ? h_scales : ws + q.hs;
-  float* g = save ? (float*)saved : (float*)(ws + q.keep);
-  float* u = g + T * h;
-  FbProduct p{};
-  p.pairs = 1;
-  p.a[0] = codes_mat(x, xs, d);
-  p.b[0] = codes_mat(gate_w, gate_s, d);
-  p.c = g;
-  p.M = T;
-  p.N = h;
-  p.K = d;
-  p.ldc = h;
-  if (int rc = launch_product(p, stream)) return rc;
-  p.b[0] = codes_mat(up_w, up_s, d);
-  p.c = u;
-  if (int rc = launch_product(p, stream)) return rc;
-  const int64_t blocks = (T * fb_blocks(h) * 16 + 255) / 256;
-  if (!grid_fits(blocks, 256)) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block_ffn: too many values");
-  hipLaunchKernelGGL(fb_gated_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, g, u, hc, hs, T, h, (int)save);
-  if (int rc = check_launch("fb_gated_kernel")) return rc;
-  p.a[0] = codes_mat(hc, hs, h);
-  p.b[0] = codes_mat(down_w, down_s, h);
-  p.c = y;
-  p.bf16 = 1;
-  p.N = d;
-  p.K = h;
-  p.ldc = d;
-  return launch_product(p, stream);
+  FbArgs p = codes_args(x, xs, gate_w, gate_s, hc, T, d, h);
+  p.w2 = up_w;
+  p.s2 = up_s;
+  p.ys = hs;
+  p.kept = (uint8_t*)saved;
+  if (int rc = launch_codes<O_GATED>(p, stream)) return rc;
+  return launch_codes<O_BF16>(codes_args(hc, hs, down_w, down_s, y, T, h, d), stream);
 }
 
 int64_t smaul_fp8_block_ffn_backward_workspace_size(int64_t T, int64_t d, int64_t h) {
@@ -422,7 +914,6 @@ int smaul_fp8_block_ffn_backward(const void* dy, const uint8_t* gate_w, const ui
                 (long long)workspace_bytes, (long long)q.total);
   char* ws = (char*)workspace;
   float *dh = (float*)(ws + q.dh), *dg = (float*)(ws + q.dg), *du = (float*)(ws + q.du);
-  const float* a = (const float*)saved;
   FbProduct p{};
   p.pairs = 1;
   p.a[0] = float_mat(dy, d, F_BF16);
@@ -434,10 +925,10 @@ int smaul_fp8_block_ffn_backward(const void* dy, const uint8_t* gate_w, const ui
   p.ldc = h;
   if (T > 0) {
     if (int rc = launch_product(p, stream)) return rc;
-    const int64_t blocks = (T * h + 255) / 256;
+    const int64_t blocks = (T * (fb_width(h) / 16) + 255) / 256;
     if (!grid_fits(blocks, 256)) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block_ffn_backward: too many values");
-    hipLaunchKernelGGL(fb_gated_backward_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, dh, a, a + T * h, dg, du,
-                       T * h);
+    hipLaunchKernelGGL(fb_gated_backward_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, dh,
+                       (const uint8_t*)saved, dg, du, T, h);
     if (int rc = check_launch("fb_gated_backward_kernel")) return rc;
   }
   p.bf16 = 1;

@@ -64,10 +64,27 @@ def weight(out_f, in_f, gen, std=0.05):
     return quantize(torch.randn(out_f, in_f, generator=gen) * std)
 
 
-def product(x, w, dtype):
-    """(y, bound) of x w^T: products exact, sums fp32 over whole blocks, y rounded once."""
+def _tops(x):
+    """The largest magnitude of each 8 neighbouring values of a row, [..., K / 8]."""
+    x = torch.nn.functional.pad(x.abs(), (0, -x.shape[-1] % 8))
+    return x.view(*x.shape[:-1], -1, 8).amax(-1)
+
+
+def aligned(x, w):
+    """What an 8-bit matrix instruction may lose of x w^T: 8 neighbouring products are summed
+    with the last bit 2^-13 of the largest's power of two (measured on the device: a product
+    2^-13 of its neighbour counts, one of 2^-14 does not), so up to 7 of them lose less than
+    2^-13 of the largest each."""
+    return 7 * 2.0 ** -13 * (_tops(x) @ _tops(w).t())
+
+
+def product(x, w, dtype, codes=False):
+    """(y, bound) of x w^T: products exact, sums fp32 over whole blocks, y rounded once;
+    ``codes``: bf16 results of the 8-bit instructions."""
     y = x @ w.t()
     err = 128 * blocks(x.shape[-1]) * U * (x.abs() @ w.abs().t())
+    if codes and dtype == torch.bfloat16:
+        err = err + aligned(x, w)
     return y, err + HALF[dtype] * (y.abs() + err) + 1e-44
 
 
@@ -103,13 +120,13 @@ def ffn(x, gate, up, down):
     """(y, bound, g, u, h, bound of h's values): hidden rows rounded from fp32, y to bf16."""
     g, u = x @ gate.t(), x @ up.t()
     rel = 128 * blocks(x.shape[-1]) * U
-    ge, ue = x.abs() @ gate.abs().t() * rel, x.abs() @ up.abs().t() * rel
+    ge, ue = (x.abs() @ w.abs().t() * rel + aligned(x, w) for w in (gate, up))
     v = silu(g) * u
     # |silu'| <= 1.1, |silu(g)| <= |g|; 2^-19 for the product's own arithmetic
     ve = 1.1 * ge * (u.abs() + ue) + g.abs() * ue + 2.0 ** -19 * v.abs()
     h, he = rounded(v), moved(v, ve)
     y = h @ down.t()
-    ye = he @ down.abs().t() + 128 * blocks(h.shape[-1]) * U * ((h.abs() + he) @ down.abs().t())
+    ye = he @ down.abs().t() + 128 * blocks(h.shape[-1]) * U * ((h.abs() + he) @ down.abs().t()) + aligned(h.abs() + he, down)
     return y, ye + HALF[torch.bfloat16] * (y.abs() + ye), g, u, h, he, ge, ue
 
 

@@ -114,6 +114,8 @@ def test_linear_layer():
         assert y.shape == (3, 70, N)
         xv = ref.rounded(x.detach().cpu().float().view(-1, K))
         want, bound = ref.product(xv, w, F32)
+        if dtype == BF:
+            bound = bound + ref.aligned(xv, w)
         half = {F32: ref.U, BF: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype]
         bound = bound + half * (want.abs() + bound)  # the product is rounded to x's type, then the bias added in fp32
         want = want + lin.bias.detach().cpu().double()
