@@ -262,7 +262,8 @@ fb_codes_kernel(FbArgs p, int m_tiles, int n_tiles) {
   using C = FbCfg<BM, BN, WM, WN>;
   constexpr bool GATED = OT == O_GATED;
   constexpr int TT = C::TT, WT = C::WT, BNO = GATED ? BN / 2 : BN, NW = C::NW;
-  constexpr int OWN = GATED ? 0 : 4096, AMAX = GATED ? BM * WN * 4 : 0;
+  // a wave's part of LDS for the rows that leave: 2 KB where two workgroups share a CU
+  constexpr int OWN = GATED ? 0 : OT == O_BF16 && BM * BN <= 128 * 128 ? 2048 : 4096, AMAX = GATED ? BM * WN * 4 : 0;
   static_assert(!GATED || BNO == FB_BLOCK, "a tile of hidden rows is a block");
   __shared__ __attribute__((aligned(1024))) char smem[C::LDS + NW * OWN + AMAX];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -422,7 +423,7 @@ fb_codes_kernel(FbArgs p, int m_tiles, int n_tiles) {
   // on the next stage's first operands are read, behind a wait that leaves the loads issued
   // in this stage (DONE of them by then) in flight.
   constexpr int B1 = S * 5 / 8, B2 = S + S * 5 / 16, SPAN = 2 * S - 2 - B1;
-  constexpr int STORED = GATED ? TT * WT / 2 : TT * WT * (OT == O_BF16 ? 2 : 4);
+  constexpr int STORED = GATED ? TT * WT / 2 : TT * WT * (OT == O_BF16 ? 2 : 4);  // instructions of a whole tile
   int stored = 0;
   constexpr int DONE = ((B2 - 1 - B1) * INS + SPAN - 1) / SPAN;  // of products B1 to B2 - 2
   auto stage = [&](int kt, bool fresh) __attribute__((always_inline)) {
@@ -555,13 +556,18 @@ fb_codes_kernel(FbArgs p, int m_tiles, int n_tiles) {
         }
       }
       if constexpr (WN > 1) __syncthreads();  // the maxima's LDS is free for the next tile
-      stored = rows == BM ? TT * HT : 0;
+      stored = rows == BM ? STORED : 0;
     } else {
-      // rows leave as whole lines, 32 at a time, through 4 KB of LDS of the wave's own,
-      // 16-byte chunks changing places by the row; a wave's LDS accesses are done in order
-      constexpr int ES = OT == O_BF16 ? 2 : 4, UJ = 4 / ES, UNITS = TT * WT / UJ;
-      const bool whole = rows == BM && n0 + BN <= p.N && p.N % (16 / ES) == 0;  // of the whole workgroup
+      // rows leave 32 at a time, as whole lines (halves from 2 KB), through LDS of the wave's
+      // own, 16-byte chunks changing places by the row; its LDS accesses are done in order
       char* own = smem + C::LDS + wave * OWN;
+      constexpr int ES = OT == O_BF16 ? 2 : 4, RB = OWN / 32, CH = RB / 16, UJ = RB / 32 / ES, UNITS = TT * WT / UJ;
+      auto place = [&](int r, int c) __attribute__((always_inline)) -> char* {
+        return own + r * RB + (c ^ (CH == 8 ? r & 7 : r / 2 & 3)) * 16;
+      };
+      const bool whole = n0 + BN <= p.N && p.N % (16 / ES) == 0;  // of the whole workgroup
+      const uint32_t ldy = (uint32_t)p.N * ES;
+      const int left = rows - wm * (BM / WM);  // rows of this wave's
       char* out = (char*)p.y + ((row0 + wm * (BM / WM)) * p.N + n0 + wn * (BN / WN)) * ES;
       uint4 d0, d1, d2, d3;
       auto to_lds = [&](int i, int j) __attribute__((always_inline)) {
@@ -579,54 +585,65 @@ fb_codes_kernel(FbArgs p, int m_tiles, int n_tiles) {
             else
               u = make_uint4(__float_as_uint(v[r]), __float_as_uint(v[r + 1]), __float_as_uint(v[r + 2]),
                              __float_as_uint(v[r + 3]));
-            *(uint4*)(own + e32 * 128 + (c ^ (e32 & 7)) * 16) = u;
+            *(uint4*)place(e32, c) = u;
           }
         }
         __builtin_amdgcn_wave_barrier();
       };
       if (whole) {
-        const uint32_t ldy = (uint32_t)p.N * ES;
         auto store = [&](int u) __attribute__((always_inline)) {
-          char* at = out + (int64_t)(u / (WT / UJ) * 32) * ldy + u % (WT / UJ) * 128;
-          const uint32_t o = (uint32_t)(el / 8) * ldy + el % 8 * 16;
-          *(uint4*)(at + o) = d0;
-          *(uint4*)(at + o + 8 * ldy) = d1;
-          *(uint4*)(at + o + 16 * ldy) = d2;
-          *(uint4*)(at + o + 24 * ldy) = d3;
+          const int r = u / (WT / UJ) * 32 + el / CH;
+          char* at = out + (int64_t)(u / (WT / UJ) * 32) * ldy + u % (WT / UJ) * RB;
+          const uint32_t o = (uint32_t)(el / CH) * ldy + el % CH * 16;
+          if (r < left) *(uint4*)(at + o) = d0;
+          if (r + 64 / CH < left) *(uint4*)(at + o + 64 / CH * ldy) = d1;
+          if constexpr (CH == 8) {
+            if (r + 16 < left) *(uint4*)(at + o + 16 * ldy) = d2;
+            if (r + 24 < left) *(uint4*)(at + o + 24 * ldy) = d3;
+          }
         };
         fb_each<UNITS + 1>([&](auto unit) __attribute__((always_inline)) {  // stored while the next is read
           constexpr int u = unit;
           if constexpr (u < UNITS) to_lds(u / (WT / UJ), u % (WT / UJ) * UJ);
           if constexpr (u > 0) store(u - 1);
           if constexpr (u < UNITS) {
-            const char* at = own + (el / 8) * 128 + (el % 8 ^ el / 8) * 16;
+            const char* at = place(el / CH, el % CH);  // 8 rows and more apart, which the places do not see
             d0 = *(const uint4*)at;
             d1 = *(const uint4*)(at + 1024);
-            d2 = *(const uint4*)(at + 2048);
-            d3 = *(const uint4*)(at + 3072);
+            if constexpr (CH == 8) {
+              d2 = *(const uint4*)(at + 2048);
+              d3 = *(const uint4*)(at + 3072);
+            }
             __builtin_amdgcn_wave_barrier();
           }
         });
-      } else {
+      } else {  // rows of any alignment, the last columns one by one
         fb_each<UNITS>([&](auto unit) __attribute__((always_inline)) {
-          constexpr int u = unit;
-          const int i = u / (WT / UJ), j = u % (WT / UJ) * UJ, tr = wm * (BM / WM) + i * 32;
-          to_lds(i, j);
-          const int64_t n = n0 + wn * (BN / WN) + j * 32;
+          constexpr int u = unit, c0 = u % (WT / UJ) * (RB / ES);
+          to_lds(u / (WT / UJ), u % (WT / UJ) * UJ);
+          const int n = (int)min<int64_t>(p.N - n0 - wn * (BN / WN) - c0, RB / ES) - el % CH * (16 / ES);
 #pragma nounroll
-          for (int e = el; e < 32 * (128 / ES); e += 64) {
-            const int r = e / (128 / ES), c = e % (128 / ES), b = c * ES;
-            const char* v = own + r * 128 + (b / 16 ^ (r & 7)) * 16 + b % 16;
-            const int64_t at = (row0 + tr + r) * p.N + n + c;
-            if (tr + r < rows && n + c < p.N) {
-              if constexpr (OT == O_BF16) ((uint16_t*)p.y)[at] = *(const uint16_t*)v;
-              else ((float*)p.y)[at] = *(const float*)v;
+          for (int h = 0; h < CH / 2; ++h) {
+            const int tr = h * (64 / CH) + el / CH, r = u / (WT / UJ) * 32 + tr;
+            const char* v = place(tr, el % CH);
+            char* at = out + (int64_t)r * ldy + (c0 + el % CH * (16 / ES)) * ES;
+            if (r >= left) continue;
+            if (n >= 16 / ES) {
+              const uint4 w = *(const uint4*)v;
+              if constexpr (OT == O_BF16) *(fb_u32x4_at2*)at = (fb_u32x4_at2){w.x, w.y, w.z, w.w};
+              else *(fb_u32x4_at4*)at = (fb_u32x4_at4){w.x, w.y, w.z, w.w};
+            } else {
+#pragma nounroll
+              for (int e = 0; e < n; ++e) {
+                if constexpr (OT == O_BF16) ((uint16_t*)at)[e] = ((const uint16_t*)v)[e];
+                else ((float*)at)[e] = ((const float*)v)[e];
+              }
             }
           }
           __builtin_amdgcn_wave_barrier();
         });
       }
-      stored = whole ? UNITS * 4 : 0;
+      stored = whole && rows == BM ? STORED : 0;
     }
   }
   wait_vm<0>();
@@ -644,9 +661,53 @@ int launch_codes_cfg(const FbArgs& p, hipStream_t stream) {
   return check_launch("fb_codes_kernel");
 }
 
+// Tiles that fill the chip, by the rounds they take: what a stage of a round of the CUs
+// takes and what the rest of its tiles does (10 ns), times the rounds.  The smaller tiles
+// run two a CU, in rounds of twice the CUs, a last round of no more than one a CU in `one`;
+// a last round that leaves CUs idle has a higher clock, up to 1.7 times.
+struct FbTile {
+  int bm, bn, one, two, rest;  // two: 0 where a CU takes them one by one
+};
+constexpr FbTile ROW_TILES[] = {{256, 256, 153, 0, 490}, {128, 256, 85, 0, 300}, {128, 128, 52, 105, 160}, {64, 128, 45, 76, 100}};
+constexpr FbTile GATED_TILES[] = {{256, 256, 153, 0, 900}, {128, 256, 85, 0, 500}, {64, 256, 60, 0, 300}};
+
+template <int N>
+int pick_tile(const FbTile (&tiles)[N], const FbArgs& p, bool gated) {
+  const int64_t cus = cu_count(), nk = p.ldx / 128;
+  int best = 0;
+  double least = 0.0;
+  for (int i = 0; i < N; ++i) {
+    const FbTile& t = tiles[i];
+    const int64_t bn = gated ? t.bn / 2 : t.bn, n = (p.R + t.bm - 1) / t.bm * ((p.N + bn - 1) / bn);
+    const int64_t round = t.two ? 2 * cus : cus, full = n / round, left = n % round;
+    const double whole = (double)(nk * (t.two ? t.two : t.one) + t.rest);
+    double last = whole * (0.6 + 0.4 * (double)left / (double)round);
+    if (t.two && left <= cus) last = (double)(nk * t.one + t.rest);
+    const double cost = (double)full * whole + (left ? last : 0.0);
+    if (i == 0 || cost < least) {
+      best = i;
+      least = cost;
+    }
+  }
+  return best;
+}
+
 template <int OT>
 int launch_codes(const FbArgs& p, hipStream_t stream) {
-  return launch_codes_cfg<OT, 256, 256, 2, 2>(p, stream);
+  if constexpr (OT == O_GATED) {
+    switch (pick_tile(GATED_TILES, p, true)) {
+      case 0: return launch_codes_cfg<OT, 256, 256, 2, 2>(p, stream);
+      case 1: return launch_codes_cfg<OT, 128, 256, 2, 2>(p, stream);
+      default: return launch_codes_cfg<OT, 64, 256, 1, 4>(p, stream);
+    }
+  } else {
+    switch (pick_tile(ROW_TILES, p, false)) {
+      case 0: return launch_codes_cfg<OT, 256, 256, 2, 2>(p, stream);
+      case 1: return launch_codes_cfg<OT, 128, 256, 2, 2>(p, stream);
+      case 2: return launch_codes_cfg<OT, 128, 128, 2, 2>(p, stream);
+      default: return launch_codes_cfg<OT, 64, 128, 2, 2>(p, stream);
+    }
+  }
 }
 
 FbArgs codes_args(const void* x, const uint8_t* xs, const uint8_t* w, const uint8_t* s, void* y, int64_t R, int64_t K,
