@@ -7,6 +7,7 @@
 //   block:   h = Q(silu(x Wg^T) * (x Wu^T)),  y = h Wd^T
 //   its gradients, straight through the roundings: dh = dy Wd, dg = dh u silu'(g),
 //   du = dh silu(g), dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
+#include <algorithm>
 #include <utility>
 
 #include "fp8_block.h"
@@ -54,98 +55,24 @@ fb_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restric
 // ---------------------------------------------------------------------------
 // products
 // ---------------------------------------------------------------------------
-enum { F_F32 = 0, F_BF16 = 1, F_CODES = 2 };
-
-// a matrix of rows of ld values (codes: with scales of ld / 128 blocks), or with
-// `turned` its transpose
-struct FbMat {
-  const void* p;
-  const uint8_t* s;
-  int64_t ld;
-  int fmt, turned;
-};
-
-__device__ __forceinline__ float fb_at(const FbMat& m, int64_t r, int64_t c) {
-  if (m.turned) {
-    const int64_t t = r;
-    r = c;
-    c = t;
-  }
-  const int64_t i = r * m.ld + c;
-  if (m.fmt == F_F32) return ((const float*)m.p)[i];
-  if (m.fmt == F_BF16) return bf2f(((const uint16_t*)m.p)[i]);
-  const uint32_t code = ((const uint8_t*)m.p)[i];
-  float v[4];
-  fb_decode4(code, fb_scale(m.s[r * ((m.ld / FB_BLOCK + 3) / 4 * 4) + c / FB_BLOCK]), v);
-  return v[0];
-}
-
-struct FbProduct {
-  FbMat a[2], b[2];  // c = a[0] b[0]^T + a[1] b[1]^T (pairs of them)
-  int pairs, bf16;   // c's type
-  void* c;
-  int64_t M, N, K, ldc;
-};
-
-// 64 x 64 outputs a workgroup, in fp32
-__global__ void __launch_bounds__(256) fb_product_kernel(FbProduct p) {
-  __shared__ float sa[16][66], sb[16][66];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 5, l32 = lane & 31;
-  const int64_t nt = (p.N + 63) / 64, m0 = (int64_t)blockIdx.x / nt * 64, n0 = (int64_t)blockIdx.x % nt * 64;
-  const int wm = wave >> 1, wn = wave & 1;
-  f32x16_t acc;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
-  for (int q = 0; q < p.pairs; ++q)
-    for (int64_t k0 = 0; k0 < p.K; k0 += 16) {
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = j * 256 + tid, r = i >> 4, k = i & 15;
-        const bool in = k0 + k < p.K;
-        sa[k][r] = in && m0 + r < p.M ? fb_at(p.a[q], m0 + r, k0 + k) : 0.0f;
-        sb[k][r] = in && n0 + r < p.N ? fb_at(p.b[q], n0 + r, k0 + k) : 0.0f;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < 16; k += 2)
-        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(sa[k + g][wm * 32 + l32], sb[k + g][wn * 32 + l32], acc, 0, 0, 0);
-    }
-  const int64_t n = n0 + wn * 32 + l32;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int64_t m = m0 + wm * 32 + (r & 3) + 8 * (r >> 2) + 4 * g;
-    if (m < p.M && n < p.N) {
-      if (p.bf16) ((__bf16*)p.c)[m * p.ldc + n] = (__bf16)acc[r];
-      else ((float*)p.c)[m * p.ldc + n] = acc[r];
-    }
-  }
-}
-
-int launch_product(const FbProduct& p, hipStream_t stream) {
-  const int64_t blocks = (p.M + 63) / 64 * ((p.N + 63) / 64);
-  if (!grid_fits(blocks, 256)) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block product: too many tiles");
-  hipLaunchKernelGGL(fb_product_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p);
-  return check_launch("fb_product_kernel");
-}
-
-// ---------------------------------------------------------------------------
-// products of codes
-// ---------------------------------------------------------------------------
-// What a tile's sums become: bf16 or fp32 rows, or the gated block's hidden rows as codes.
-enum { O_BF16 = 0, O_F32 = 1, O_GATED = 2 };
+// Both sides' rows: codes with their scales, or bf16 (a row's bytes a multiple of 128).
+enum { F_CODES = 0, F_BF16 = 1 };
+// What a tile's sums become: bf16 or fp32 rows, the gated block's hidden rows as codes, or
+// (sums dh) its dg and du by the factors that the forward pass kept.
+enum { O_BF16 = 0, O_F32 = 1, O_GATED = 2, O_DGATED = 3 };
 
 struct FbArgs {
-  const uint8_t* x;   // R rows of ldx codes
-  const uint8_t* xs;  // their scales, `words` dwords a row
+  const uint8_t* x;   // R rows of ldx bytes
+  const uint8_t* xs;  // F_CODES: their scales, `words` dwords a row
   const uint8_t* w;   // N rows
   const uint8_t* s;
   const uint8_t* w2;  // O_GATED: up's (w, s are gate's)
   const uint8_t* s2;
-  void* y;            // [R][N] (O_GATED: codes [R][fb_width(N)])
+  void* y;            // [R][N] (O_GATED: codes [R][fb_width(N)], O_DGATED: bf16 [R][2][ldh])
   uint8_t* ys;        // O_GATED: scales
-  uint8_t* kept;      // O_GATED: what the gradients take, or null
+  uint8_t* kept;      // O_GATED: what the gradients take, or null; O_DGATED: that
   int64_t R, N, ldx;  // ldx: of x and w, a multiple of 128
+  int64_t ldh;        // O_DGATED: N to whole stages, zeros from N on
   int words;
 };
 
@@ -205,11 +132,11 @@ __device__ __forceinline__ void fb_each(F&& f) {
 // rows and x's its columns, and row i of a 32 x 32 tile is given weight row 16 ((i / 4) %
 // 2) + 4 (i / 8) + i % 4, so that the 16 sums of a lane are 16 consecutive outputs of one
 // row of x.
-template <int BM, int BN, int WM, int WN>
+template <int FMT, int BM, int BN, int WM, int WN>
 struct FbCfg {
   static constexpr int NW = WM * WN, XB = BM * 128, WB = BN * 128, STAGE = XB + WB;
   static constexpr int X_INS = XB / (1024 * NW), W_INS = WB / (1024 * NW), S_INS = (BM + BN) / (16 * NW);
-  static constexpr int SC = (BM + BN) * 16;  // a chunk of scales: 4 dwords a row
+  static constexpr int SC = FMT == F_CODES ? (BM + BN) * 16 : 0;  // a chunk of scales: 4 dwords a row
   static constexpr int TT = BM / WM / 32, WT = BN / WN / 32;
   static constexpr int LDS = 2 * STAGE + 2 * SC;
   static_assert(XB % (1024 * NW) == 0 && WB % (1024 * NW) == 0 && (BM + BN) % (16 * NW) == 0 && BN % 16 == 0,
@@ -239,6 +166,12 @@ __device__ __forceinline__ bf16x8_t fb_decode8(int lo, int hi, float s) {
 // sums stay in AGPRs up to here: moved out early they would not fit the other registers
 __device__ __forceinline__ void fb_pin(f32x16_t& v) { asm volatile("" : "+a"(v)); }
 
+// half q of an operand's 32 bytes, as bf16
+__device__ __forceinline__ bf16x8_t fb_half(const i32x8_t& v, int q) {
+  return __builtin_bit_cast(bf16x8_t, make_uint4((uint32_t)v[4 * q], (uint32_t)v[4 * q + 1], (uint32_t)v[4 * q + 2],
+                                                 (uint32_t)v[4 * q + 3]));
+}
+
 // tile `lin` of m_tiles by n_tiles, in groups of 8 row tiles by all column tiles
 __device__ __forceinline__ void fb_tile_at(int lin, int m_tiles, int n_tiles, int& mt, int& nt) {
   constexpr int GM = 8;
@@ -256,10 +189,10 @@ __device__ __forceinline__ void fb_tile_at(int lin, int m_tiles, int n_tiles, in
 // wave has the rest of its stage in registers, so that one barrier frees the buffer for
 // the loads of the stage after the next.  A workgroup walks a band of tiles as one
 // sequence of stages.
-template <int OT, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(WM * WN * 64, WM * WN == 4 && BM * BN > 128 * 128 ? 1 : 2)
-fb_codes_kernel(FbArgs p, int m_tiles, int n_tiles) {
-  using C = FbCfg<BM, BN, WM, WN>;
+template <int FMT, int OT, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(WM * WN * 64, BM * BN > 128 * 128 || BN > 128 || OT == O_F32 ? 1 : 2)
+fb_product_kernel(FbArgs p, int m_tiles, int n_tiles) {
+  using C = FbCfg<FMT, BM, BN, WM, WN>;
   constexpr bool GATED = OT == O_GATED;
   constexpr int TT = C::TT, WT = C::WT, BNO = GATED ? BN / 2 : BN, NW = C::NW;
   // a wave's part of LDS for the rows that leave: 2 KB where two workgroups share a CU
@@ -297,9 +230,9 @@ fb_codes_kernel(FbArgs p, int m_tiles, int n_tiles) {
     const int64_t row0 = (int64_t)mt * BM, n0 = (int64_t)nt * BNO;
     const int xleft = (int)min<int64_t>(p.R - 1 - row0, BM - 1), wleft = (int)min<int64_t>(p.N - 1 - n0, BNO - 1);
     X = p.x + row0 * ld;
-    XS = p.xs + row0 * sl;
+    if (FMT == F_CODES) XS = p.xs + row0 * sl;
     W = p.w + n0 * ld;
-    WS = p.s + n0 * sl;
+    if (FMT == F_CODES) WS = p.s + n0 * sl;
     const bool ragged = xleft < BM - 1 || wleft < BNO - 1;
     if (!ragged && !offsets) return;  // a whole tile's offsets are there from the one before
     offsets = ragged;
@@ -332,7 +265,7 @@ fb_codes_kernel(FbArgs p, int m_tiles, int n_tiles) {
       load_at += step;
       load_k = 0;
     }
-    if (load_k % 16 == 0) {
+    if (FMT == F_CODES && load_k % 16 == 0) {
       const int word = min(load_k / 4 + lane % 4, p.words - 1) * 4;
 #pragma unroll
       for (int i = 0; i < C::S_INS; ++i) {
@@ -398,7 +331,12 @@ fb_codes_kernel(FbArgs p, int m_tiles, int n_tiles) {
     const f32x16_t zero = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     const int j = s / TT, i = s % TT;
     const f32x16_t c = fresh && u == 0 ? zero : acc[j][i];
-    if constexpr (OT == O_F32) {
+    if constexpr (FMT == F_BF16) {
+      acc[j][i] = c;
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb_half(wf[u][j], q), fb_half(xf[u][i], q), acc[j][i], 0, 0, 0);
+    } else if constexpr (OT == O_F32) {
       acc[j][i] = c;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -429,9 +367,9 @@ fb_codes_kernel(FbArgs p, int m_tiles, int n_tiles) {
   auto stage = [&](int kt, bool fresh) __attribute__((always_inline)) {
     const int sh = kt % 4 * 8, next = kt + 1 == nk ? 0 : kt + 1;
 #pragma unroll
-    for (int j = 0; j < WT; ++j) sw[j] = nw[j] >> sh;
+    for (int j = 0; j < WT && FMT == F_CODES; ++j) sw[j] = nw[j] >> sh;
 #pragma unroll
-    for (int i = 0; i < TT; ++i) sx[i] = nx_[i] >> sh;
+    for (int i = 0; i < TT && FMT == F_CODES; ++i) sx[i] = nx_[i] >> sh;
     if (next % 16 == 0) chunk ^= 1;
     fb_each<2 * S>([&](auto number) __attribute__((always_inline)) {
       constexpr int s = number;
@@ -452,7 +390,7 @@ fb_codes_kernel(FbArgs p, int m_tiles, int n_tiles) {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
-        read_scales(chunk, next / 4 % 4);
+        if constexpr (FMT == F_CODES) read_scales(chunk, next / 4 % 4);
       }
       fb_each<READS>([&](auto part) __attribute__((always_inline)) {
         constexpr int q = part;
@@ -471,7 +409,7 @@ fb_codes_kernel(FbArgs p, int m_tiles, int n_tiles) {
 
 #pragma unroll
   for (int q = 0; q < READS; ++q) read_one(0, 0, q);
-  read_scales(0, 0);
+  if constexpr (FMT == F_CODES) read_scales(0, 0);
   for (; lin < last; lin += step) {
     stage(0, true);
     for (int kt = 1; kt < nk; ++kt) stage(kt, false);
@@ -557,6 +495,63 @@ fb_codes_kernel(FbArgs p, int m_tiles, int n_tiles) {
       }
       if constexpr (WN > 1) __syncthreads();  // the maxima's LDS is free for the next tile
       stored = rows == BM ? STORED : 0;
+    } else if constexpr (OT == O_DGATED) {
+      // 64-byte pieces of dg and of du, each through 2 KB of LDS of the wave's own; the next
+      // 16 values' factors are on their way while these are multiplied
+      char* own = smem + C::LDS + wave * OWN;
+      auto place = [&](int m, int r, int c) __attribute__((always_inline)) -> char* {
+        return own + m * 2048 + r * 64 + (c ^ (r / 2 & 3)) * 16;
+      };
+      const int left = rows - wm * (BM / WM);
+      const int64_t nrec = fb_width(p.N) / 16, w0 = n0 + wn * (BN / WN), r0 = row0 + wm * (BM / WM);
+      uint4 rec[6];
+      auto factors = [&](int u) __attribute__((always_inline)) {
+        const int r = min(u / WT * 32 + e32, left - 1);
+        const int64_t c = min<int64_t>((w0 + u % WT * 32) / 16 + eg, nrec - 1);
+        const uint4* at = (const uint4*)(p.kept + ((r0 + (r < 0 ? 0 : r)) * nrec + c) * FB_RECORD);
+        rec[0] = at[0]; rec[1] = at[1]; rec[2] = at[2]; rec[3] = at[3]; rec[4] = at[4]; rec[5] = at[5];
+      };
+      if (left > 0) {
+        factors(0);
+        fb_each<TT * WT>([&](auto unit) __attribute__((always_inline)) {
+          constexpr int u = unit, i = u / WT, j = u % WT;
+          const uint4 ah[2] = {rec[0], rec[1]}, bh[2] = {rec[2], rec[3]}, al = rec[4], bl = rec[5];
+          if constexpr (u + 1 < TT * WT) factors(u + 1);
+          float a[16], b[16];
+          fb_unpack24(ah, al, a);
+          fb_unpack24(bh, bl, b);
+          fb_pin(acc[j][i]);
+          const f32x16_t v = acc[j][i];
+          const int in = (int)min<int64_t>(p.N - (w0 + j * 32 + eg * 16), 16);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            a[r] = r < in ? v[r] * a[r] : 0.0f;
+            b[r] = r < in ? v[r] * b[r] : 0.0f;
+          }
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const int k = 8 * q;
+            *(uint4*)place(0, e32, 2 * eg + q) = make_uint4(pack_bf16(a[k], a[k + 1]), pack_bf16(a[k + 2], a[k + 3]),
+                                                            pack_bf16(a[k + 4], a[k + 5]), pack_bf16(a[k + 6], a[k + 7]));
+            *(uint4*)place(1, e32, 2 * eg + q) = make_uint4(pack_bf16(b[k], b[k + 1]), pack_bf16(b[k + 2], b[k + 3]),
+                                                            pack_bf16(b[k + 4], b[k + 5]), pack_bf16(b[k + 6], b[k + 7]));
+          }
+          __builtin_amdgcn_wave_barrier();
+          const int64_t n = w0 + j * 32 + el % 4 * 8;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int tr = h * 16 + el / 4;
+            const uint4 g = *(const uint4*)place(0, tr, el % 4), t = *(const uint4*)place(1, tr, el % 4);
+            if (i * 32 + tr < left && n < p.ldh) {
+              uint16_t* at = (uint16_t*)p.y + (r0 + i * 32 + tr) * 2 * p.ldh + n;
+              *(uint4*)at = g;
+              *(uint4*)(at + p.ldh) = t;
+            }
+          }
+          __builtin_amdgcn_wave_barrier();
+        });
+      }
+      stored = 0;
     } else {
       // rows leave 32 at a time, as whole lines (halves from 2 KB), through LDS of the wave's
       // own, 16-byte chunks changing places by the row; its LDS accesses are done in order
@@ -649,16 +644,16 @@ fb_codes_kernel(FbArgs p, int m_tiles, int n_tiles) {
   wait_vm<0>();
 }
 
-template <int OT, int BM, int BN, int WM, int WN>
-int launch_codes_cfg(const FbArgs& p, hipStream_t stream) {
+template <int FMT, int OT, int BM, int BN, int WM, int WN>
+int launch_product_cfg(const FbArgs& p, hipStream_t stream) {
   constexpr int BNO = OT == O_GATED ? BN / 2 : BN;
   const int64_t mt = (p.R + BM - 1) / BM, nt = (p.N + BNO - 1) / BNO;
   if ((BM > BN ? BM : BN) * p.ldx >= 1LL << 32) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block product: rows too wide");
   if (mt * nt > 2147483647LL || mt > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block product: too many tiles");
   const int64_t wgs = cu_count() * (BM * BN <= 128 * 128 ? 2 : 1);
-  hipLaunchKernelGGL((fb_codes_kernel<OT, BM, BN, WM, WN>), dim3((unsigned)(mt * nt < wgs ? mt * nt : wgs)),
+  hipLaunchKernelGGL((fb_product_kernel<FMT, OT, BM, BN, WM, WN>), dim3((unsigned)(mt * nt < wgs ? mt * nt : wgs)),
                      dim3(WM * WN * 64), 0, stream, p, (int)mt, (int)nt);
-  return check_launch("fb_codes_kernel");
+  return check_launch("fb_product_kernel");
 }
 
 // Tiles that fill the chip, by the rounds they take: what a stage of a round of the CUs
@@ -692,20 +687,20 @@ int pick_tile(const FbTile (&tiles)[N], const FbArgs& p, bool gated) {
   return best;
 }
 
-template <int OT>
-int launch_codes(const FbArgs& p, hipStream_t stream) {
+template <int FMT, int OT>
+int launch_product(const FbArgs& p, hipStream_t stream) {
   if constexpr (OT == O_GATED) {
     switch (pick_tile(GATED_TILES, p, true)) {
-      case 0: return launch_codes_cfg<OT, 256, 256, 2, 2>(p, stream);
-      case 1: return launch_codes_cfg<OT, 128, 256, 2, 2>(p, stream);
-      default: return launch_codes_cfg<OT, 64, 256, 1, 4>(p, stream);
+      case 0: return launch_product_cfg<FMT, OT, 256, 256, 2, 2>(p, stream);
+      case 1: return launch_product_cfg<FMT, OT, 128, 256, 2, 2>(p, stream);
+      default: return launch_product_cfg<FMT, OT, 64, 256, 1, 4>(p, stream);
     }
   } else {
     switch (pick_tile(ROW_TILES, p, false)) {
-      case 0: return launch_codes_cfg<OT, 256, 256, 2, 2>(p, stream);
-      case 1: return launch_codes_cfg<OT, 128, 256, 2, 2>(p, stream);
-      case 2: return launch_codes_cfg<OT, 128, 128, 2, 2>(p, stream);
-      default: return launch_codes_cfg<OT, 64, 128, 2, 2>(p, stream);
+      case 0: return launch_product_cfg<FMT, OT, 256, 256, 2, 2>(p, stream);
+      case 1: return launch_product_cfg<FMT, OT, 128, 256, 2, 2>(p, stream);
+      case 2: return launch_product_cfg<FMT, OT, 128, 128, 2, 2>(p, stream);
+      default: return launch_product_cfg<FMT, OT, 64, 128, 2, 2>(p, stream);
     }
   }
 }
@@ -725,23 +720,130 @@ FbArgs codes_args(const void* x, const uint8_t* xs, const uint8_t* w, const uint
   return p;
 }
 
-// dh -> dg and du, by the factors that the forward pass kept
-__global__ void __launch_bounds__(256)
-fb_gated_backward_kernel(const float* __restrict__ dh, const uint8_t* __restrict__ kept, float* __restrict__ dg,
-                         float* __restrict__ du, int64_t T, int64_t h) {
-  const int64_t nr = fb_width(h) / 16, i = (int64_t)blockIdx.x * 256 + threadIdx.x, t = i / nr, c = (i - t * nr) * 16;
-  if (t >= T || c >= h) return;
-  const uint4* rec = (const uint4*)(kept + i * FB_RECORD);
-  float a[16], b[16];
-  fb_unpack24({rec[0], rec[1]}, rec[4], a);
-  fb_unpack24({rec[2], rec[3]}, rec[5], b);
+// ---------------------------------------------------------------------------
+// operands of the gradients' products: bf16 rows of whole stages (64 values)
+// ---------------------------------------------------------------------------
+// Several matrices a launch, each R rows of C values: bf16 rows, fp32 rows or codes
+// (decoded: exact in bf16), turned round (dst [C][ld]) or as they lie (dst [R][ld]), zeros
+// up to whole stages.  fp32 rows are three bf16 planes, each the next 8 bits (exact), 64
+// values of each in turn; the other side's rows are then there three times.
+enum { S_BF16 = 0, S_F32 = 1, S_CODES = 2 };
+struct FbTurn {
+  const void* src;
+  const uint8_t* scales;
+  uint16_t* dst;
+  int64_t R, C, lds, ld;  // lds: the source's row, in values
+  int64_t blocks;
+  int fmt, turned, copies;
+};
+constexpr int FB_TURNS = 6;
+struct FbTurns {
+  FbTurn t[FB_TURNS];
+};
+__host__ __device__ __forceinline__ int64_t fb_stages(int64_t K) { return (K + 63) / 64; }
+
+// a workgroup: 64 by 64 values, 16 of a row a thread, through LDS
+__global__ void __launch_bounds__(256) fb_turn_kernel(FbTurns a) {
+  constexpr int LD = 72;  // 16-byte rows off the banks' period
+  __shared__ __attribute__((aligned(16))) uint16_t sh[64 * LD];
+  int64_t b = blockIdx.x;
+  int k = 0;
 #pragma unroll
-  for (int r = 0; r < 16; ++r)
-    if (c + r < h) {
-      const float v = dh[t * h + c + r];
-      dg[t * h + c + r] = v * a[r];
-      du[t * h + c + r] = v * b[r];
+  for (int j = 0; j + 1 < FB_TURNS; ++j)
+    if (k == j && b >= a.t[j].blocks) {
+      b -= a.t[j].blocks;
+      k = j + 1;
     }
+  const FbTurn& t = a.t[k];
+  const int64_t across = fb_stages(t.C), r0 = b / across * 64, c0 = b % across * 64;
+  const int tid = threadIdx.x, lr = tid >> 2, lc = (tid & 3) * 16;
+  const int64_t r = r0 + lr, c = c0 + lc;
+  float v[16];
+  const bool in = r < t.R && c < t.C;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float* o = v + 8 * h;
+    float u[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) u[q] = 0.0f;
+    if (in && c + 8 * h < t.C) {
+      if (t.fmt == S_CODES) {
+        const uint2 w = *(const uint2*)((const uint8_t*)t.src + r * t.lds + c + 8 * h);
+        const float s = fb_scale(t.scales[r * ((t.lds / FB_BLOCK + 3) / 4 * 4) + c / FB_BLOCK]);
+        fb_decode4(w.x, s, u);
+        fb_decode4(w.y, s, u + 4);
+      } else if (t.fmt == S_BF16) {
+        fb_load8<true>(t.src, r, t.C, c + 8 * h, u);
+      } else {
+        fb_load8<false>(t.src, r, t.C, c + 8 * h, u);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) o[q] = c + 8 * h + q < t.C ? u[q] : 0.0f;
+  }
+  const int planes = t.fmt == S_F32 ? 3 : 1;
+  for (int p = 0; p < planes; ++p) {
+    uint32_t w[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      uint32_t part[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float& f = v[2 * q + e];
+        if (t.fmt == S_F32) {  // the next 8 significant bits; an infinity or NaN is in the first plane alone
+          const float x = __builtin_canonicalizef(f);
+          const uint32_t top = __float_as_uint(x) & 0xffff0000u;
+          const float rest = x - __uint_as_float(top);
+          f = rest == rest ? rest : 0.0f;
+          part[e] = top >> 16;
+        } else {
+          part[e] = __float_as_uint(f) >> 16;  // exact
+        }
+      }
+      w[q] = part[0] | part[1] << 16;
+    }
+    if (t.turned) {
+#pragma unroll
+      for (int q = 0; q < 16; ++q) sh[(lc + q) * LD + lr] = (uint16_t)(w[q / 2] >> (16 * (q & 1)));
+    } else if (r < t.R) {
+      uint4* o = (uint4*)(t.dst + r * t.ld + c0 * planes + p * 64 + lc);
+      o[0] = make_uint4(w[0], w[1], w[2], w[3]);
+      o[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+  }
+  if (!t.turned) return;  // the whole workgroup
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int at = tid + q * 256, i = at >> 3, j = (at & 7) * 8;
+    if (c0 + i < t.C)
+      for (int e = 0; e < t.copies; ++e)
+        *(uint4*)(t.dst + (c0 + i) * t.ld + r0 * t.copies + e * 64 + j) = *(const uint4*)&sh[i * LD + j];
+  }
+}
+
+__global__ void __launch_bounds__(256) fb_clear_kernel(uint16_t* p, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
+}
+
+int launch_turns(FbTurns& a, int n, hipStream_t stream) {
+  int64_t blocks = 0;
+  for (int i = 0; i < n; ++i) {
+    a.t[i].blocks = fb_stages(a.t[i].R) * fb_stages(a.t[i].C);
+    blocks += a.t[i].blocks;
+  }
+  if (!grid_fits(blocks, 256)) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block gradient: too many values");
+  if (n == 0 || blocks == 0) return SMAUL_OK;
+  hipLaunchKernelGGL(fb_turn_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  return check_launch("fb_turn_kernel");
+}
+
+FbTurn turn_codes(const void* codes, const uint8_t* scales, int64_t R, int64_t C, uint16_t* dst, int64_t ld,
+                  int copies = 1) {
+  return FbTurn{codes, scales, dst, R, C, fb_width(C), ld, 0, S_CODES, 1, copies};
+}
+FbTurn turn_rows(const void* rows, int fmt, int64_t R, int64_t C, uint16_t* dst, int64_t ld, int turned) {
+  return FbTurn{rows, nullptr, dst, R, C, C, ld, 0, fmt, turned, 1};
 }
 
 // a workspace laid out part by part
@@ -782,22 +884,54 @@ FfnParts ffn_parts(int64_t T, int64_t d, int64_t h, int x_dtype, bool save) {
 }
 
 struct FfnBackParts {
-  int64_t dh, dg, du, total;
+  int64_t dy, wd, wgu, dgu, dgut, xt, dyt, ht, total;
+  int64_t lt, ld, lh;  // T, d and h to whole stages
 };
-FfnBackParts ffn_back_parts(int64_t T, int64_t h) {
+FfnBackParts ffn_back_parts(int64_t T, int64_t d, int64_t h, bool dx, bool dw) {
   FfnBackParts q{};
   Parts w;
-  q.dh = w.take(T * h * 4);
-  q.dg = w.take(T * h * 4);
-  q.du = w.take(T * h * 4);
+  q.lt = fb_stages(T) * 64;
+  q.ld = fb_stages(d) * 64;
+  q.lh = fb_stages(h) * 64;
+  q.dy = w.take(d % 64 ? T * q.ld * 2 : 0);
+  q.wd = w.take(h * q.ld * 2);
+  q.wgu = w.take(dx ? d * q.lh * 4 : 0);
+  q.dgu = w.take(T * q.lh * 4);
+  q.dgut = w.take(dw ? q.lh * q.lt * 4 : 0);
+  q.xt = w.take(dw ? d * q.lt * 2 : 0);
+  q.dyt = w.take(dw ? d * q.lt * 2 : 0);
+  q.ht = w.take(dw ? h * q.lt * 2 : 0);
   q.total = w.at;
   return q;
 }
 
-FbMat codes_mat(const void* p, const uint8_t* s, int64_t K, int turned = 0) {
-  return FbMat{p, s, fb_width(K), F_CODES, turned};
+struct DxParts {
+  int64_t g, wt, total, ld;
+  int copies;
+};
+DxParts dx_parts(int64_t rows, int64_t in_f, int64_t out_f, int dtype) {
+  DxParts q{};
+  Parts w;
+  const bool f32 = dtype == SMAUL_DTYPE_F32;
+  q.copies = f32 ? 3 : 1;
+  q.ld = fb_stages(out_f) * 64 * q.copies;
+  q.g = w.take(f32 || out_f % 64 ? rows * q.ld * 2 : 0);
+  q.wt = w.take(in_f * q.ld * 2);
+  q.total = w.at;
+  return q;
 }
-FbMat float_mat(const void* p, int64_t ld, int fmt, int turned = 0) { return FbMat{p, nullptr, ld, fmt, turned}; }
+
+// x [R][ld] . w [N][ld]^T, bf16 rows of whole stages
+FbArgs rows_args(const void* x, const void* w, void* y, int64_t R, int64_t ld, int64_t N) {
+  FbArgs p{};
+  p.x = (const uint8_t*)x;
+  p.w = (const uint8_t*)w;
+  p.y = y;
+  p.R = R;
+  p.N = N;
+  p.ldx = ld * 2;
+  return p;
+}
 
 }  // namespace
 
@@ -859,12 +993,12 @@ int smaul_fp8_block_linear(const void* x, int x_dtype, const uint8_t* xs, const 
     xs = cs;
   }
   const FbArgs p = codes_args(x, xs, w, s, y, rows, in_f, out_f);
-  return y_dtype == SMAUL_DTYPE_BF16 ? launch_codes<O_BF16>(p, stream) : launch_codes<O_F32>(p, stream);
+  return y_dtype == SMAUL_DTYPE_BF16 ? launch_product<F_CODES, O_BF16>(p, stream) : launch_product<F_CODES, O_F32>(p, stream);
 }
 
 int64_t smaul_fp8_block_backward_input_workspace_size(int64_t rows, int64_t in_f, int64_t out_f, int dtype) {
   if (rows < 0 || in_f <= 0 || out_f <= 0 || !fb_dtype_ok(dtype)) return -1;
-  return 0;
+  return dx_parts(rows, in_f, out_f, dtype).total;
 }
 
 int smaul_fp8_block_backward_input(const void* g, int dtype, const uint8_t* w, const uint8_t* s, void* dx, int64_t rows,
@@ -880,18 +1014,20 @@ int smaul_fp8_block_backward_input(const void* g, int dtype, const uint8_t* w, c
   if (workspace_bytes < need || (need > 0 && (!workspace || !fb_aligned(workspace, 256))))
     return fail(SMAUL_ERR_INVALID, "fp8_block_backward_input: workspace %lld < %lld bytes, or unaligned",
                 (long long)workspace_bytes, (long long)need);
+  const DxParts q = dx_parts(rows, in_f, out_f, dtype);
+  char* ws = (char*)workspace;
   const bool bf16 = dtype == SMAUL_DTYPE_BF16;
-  FbProduct p{};
-  p.a[0] = float_mat(g, out_f, bf16 ? F_BF16 : F_F32);
-  p.b[0] = codes_mat(w, s, in_f, 1);
-  p.pairs = 1;
-  p.bf16 = bf16;
-  p.c = dx;
-  p.M = rows;
-  p.N = in_f;
-  p.K = out_f;
-  p.ldc = in_f;
-  return launch_product(p, stream);
+  uint16_t* wt = (uint16_t*)(ws + q.wt);
+  FbTurns a{};
+  int n = 0;
+  a.t[n++] = turn_codes(w, s, out_f, in_f, wt, q.ld, q.copies);
+  if (!bf16 || out_f % 64) {
+    a.t[n++] = turn_rows(g, bf16 ? S_BF16 : S_F32, rows, out_f, (uint16_t*)(ws + q.g), q.ld, 0);
+    g = ws + q.g;
+  }
+  if (int rc = launch_turns(a, n, stream)) return rc;
+  const FbArgs p = rows_args(g, wt, dx, rows, q.ld, in_f);
+  return bf16 ? launch_product<F_BF16, O_BF16>(p, stream) : launch_product<F_BF16, O_F32>(p, stream);
 }
 
 int64_t smaul_fp8_block_ffn_saved_size(int64_t T, int64_t h) {
@@ -941,13 +1077,13 @@ int smaul_fp8_block_ffn_forward(const void* x, int x_dtype, const uint8_t* xs, c
   p.s2 = up_s;
   p.ys = hs;
   p.kept = (uint8_t*)saved;
-  if (int rc = launch_codes<O_GATED>(p, stream)) return rc;
-  return launch_codes<O_BF16>(codes_args(hc, hs, down_w, down_s, y, T, h, d), stream);
+  if (int rc = launch_product<F_CODES, O_GATED>(p, stream)) return rc;
+  return launch_product<F_CODES, O_BF16>(codes_args(hc, hs, down_w, down_s, y, T, h, d), stream);
 }
 
 int64_t smaul_fp8_block_ffn_backward_workspace_size(int64_t T, int64_t d, int64_t h) {
   if (T < 0 || d <= 0 || h <= 0) return -1;
-  return ffn_back_parts(T, h).total;
+  return ffn_back_parts(T, d, h, true, true).total;
 }
 
 int smaul_fp8_block_ffn_backward(const void* dy, const uint8_t* gate_w, const uint8_t* gate_s, const uint8_t* up_w,
@@ -969,62 +1105,52 @@ int smaul_fp8_block_ffn_backward(const void* dy, const uint8_t* gate_w, const ui
                         (const void*)ddown})
     if (!fb_aligned(p, 16))
       return fail(SMAUL_ERR_INVALID, "fp8_block_ffn_backward: rows and codes must be 16-byte aligned");
-  const FfnBackParts q = ffn_back_parts(T, h);
+  const FfnBackParts q = ffn_back_parts(T, d, h, dx != nullptr, weights);
   if (workspace_bytes < q.total || (q.total > 0 && (!workspace || !fb_aligned(workspace, 256))))
     return fail(SMAUL_ERR_INVALID, "fp8_block_ffn_backward: workspace %lld < %lld bytes, or unaligned",
                 (long long)workspace_bytes, (long long)q.total);
   char* ws = (char*)workspace;
-  float *dh = (float*)(ws + q.dh), *dg = (float*)(ws + q.dg), *du = (float*)(ws + q.du);
-  FbProduct p{};
-  p.pairs = 1;
-  p.a[0] = float_mat(dy, d, F_BF16);
-  p.b[0] = codes_mat(down_w, down_s, h, 1);
-  p.c = dh;
-  p.M = T;
-  p.N = h;
-  p.K = d;
-  p.ldc = h;
-  if (T > 0) {
-    if (int rc = launch_product(p, stream)) return rc;
-    const int64_t blocks = (T * (fb_width(h) / 16) + 255) / 256;
-    if (!grid_fits(blocks, 256)) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block_ffn_backward: too many values");
-    hipLaunchKernelGGL(fb_gated_backward_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, dh,
-                       (const uint8_t*)saved, dg, du, T, h);
-    if (int rc = check_launch("fb_gated_backward_kernel")) return rc;
+  if (T == 0) {
+    const int64_t n = d * h * 2;  // bytes, cleared by a kernel: a captured call may not record a fill of memory
+    for (void* p : {dgate, dup, ddown}) {
+      hipLaunchKernelGGL(fb_clear_kernel, dim3((unsigned)std::min<int64_t>((n / 2 + 255) / 256, 4096)), dim3(256), 0,
+                         stream, (uint16_t*)p, n / 2);
+      if (int rc = check_launch("fb_clear_kernel")) return rc;
+    }
+    return SMAUL_OK;
   }
-  p.bf16 = 1;
-  if (dx && T > 0) {
-    p.pairs = 2;
-    p.a[0] = float_mat(dg, h, F_F32);
-    p.b[0] = codes_mat(gate_w, gate_s, d, 1);
-    p.a[1] = float_mat(du, h, F_F32);
-    p.b[1] = codes_mat(up_w, up_s, d, 1);
-    p.c = dx;
-    p.N = d;
-    p.K = h;
-    p.ldc = d;
-    if (int rc = launch_product(p, stream)) return rc;
+  uint16_t *wd = (uint16_t*)(ws + q.wd), *wgu = (uint16_t*)(ws + q.wgu), *dgu = (uint16_t*)(ws + q.dgu);
+  uint16_t *dgut = (uint16_t*)(ws + q.dgut), *xt = (uint16_t*)(ws + q.xt), *dyt = (uint16_t*)(ws + q.dyt);
+  uint16_t* ht = (uint16_t*)(ws + q.ht);
+  FbTurns a{};
+  int n = 0;
+  const void* rows = dy;
+  a.t[n++] = turn_codes(down_w, down_s, d, h, wd, q.ld);
+  if (d % 64) {
+    a.t[n++] = turn_rows(dy, S_BF16, T, d, (uint16_t*)(ws + q.dy), q.ld, 0);
+    rows = ws + q.dy;
   }
+  if (dx) {
+    a.t[n++] = turn_codes(gate_w, gate_s, h, d, wgu, 2 * q.lh);
+    a.t[n++] = turn_codes(up_w, up_s, h, d, wgu + q.lh, 2 * q.lh);
+  }
+  if (int rc = launch_turns(a, n, stream)) return rc;
+  FbArgs p = rows_args(rows, wd, dgu, T, q.ld, h);
+  p.kept = (uint8_t*)saved;
+  p.ldh = q.lh;
+  if (int rc = launch_product<F_BF16, O_DGATED>(p, stream)) return rc;
+  if (dx)
+    if (int rc = launch_product<F_BF16, O_BF16>(rows_args(dgu, wgu, dx, T, 2 * q.lh, d), stream)) return rc;
   if (!weights) return SMAUL_OK;
-  p.pairs = 1;
-  p.K = T;
-  p.M = h;
-  p.N = d;
-  p.ldc = d;
-  p.a[0] = float_mat(dg, h, F_F32, 1);
-  p.b[0] = codes_mat(x_codes, x_scales, d, 1);
-  p.c = dgate;
-  if (int rc = launch_product(p, stream)) return rc;
-  p.a[0] = float_mat(du, h, F_F32, 1);
-  p.c = dup;
-  if (int rc = launch_product(p, stream)) return rc;
-  p.a[0] = float_mat(dy, d, F_BF16, 1);
-  p.b[0] = codes_mat(h_codes, h_scales, h, 1);
-  p.c = ddown;
-  p.M = d;
-  p.N = h;
-  p.ldc = h;
-  return launch_product(p, stream);
+  FbTurns b{};
+  b.t[0] = turn_rows(dgu, S_BF16, T, 2 * q.lh, dgut, q.lt, 1);
+  b.t[1] = turn_codes(x_codes, x_scales, T, d, xt, q.lt);
+  b.t[2] = turn_rows(dy, S_BF16, T, d, dyt, q.lt, 1);
+  b.t[3] = turn_codes(h_codes, h_scales, T, h, ht, q.lt);
+  if (int rc = launch_turns(b, 4, stream)) return rc;
+  if (int rc = launch_product<F_BF16, O_BF16>(rows_args(dgut, xt, dgate, h, q.lt, d), stream)) return rc;
+  if (int rc = launch_product<F_BF16, O_BF16>(rows_args(dgut + q.lh * q.lt, xt, dup, h, q.lt, d), stream)) return rc;
+  return launch_product<F_BF16, O_BF16>(rows_args(dyt, ht, ddown, d, q.lt, h), stream);
 }
 
 }  // extern "C"
