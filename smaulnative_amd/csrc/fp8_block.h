@@ -57,13 +57,33 @@ __device__ __forceinline__ void fb_decode4(uint32_t w, float s, float* v) {
 typedef uint32_t fb_u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t fb_u32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
 
+// NT: past the caches, for rows that are larger than they are
+constexpr int64_t FB_NT_BYTES = 128LL << 20;  // half of the last cache
+struct FbAt2 { typedef fb_u32x4_at2 T; };  // (a template argument would lose the alignment)
+struct FbAt4 { typedef fb_u32x4_at4 T; };
+template <class At, bool NT>
+__device__ __forceinline__ uint4 fb_ld16(const void* p) {
+  typedef typename At::T T;
+  T v;
+  if constexpr (NT) v = __builtin_nontemporal_load((const T*)p);
+  else v = *(const T*)p;
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
+template <class At, bool NT>
+__device__ __forceinline__ void fb_st16(void* p, uint4 v) {
+  typedef typename At::T T;
+  const T w = {v.x, v.y, v.z, v.w};
+  if constexpr (NT) __builtin_nontemporal_store(w, (T*)p);
+  else *(T*)p = w;
+}
 // 8 consecutive values of a row of K from column c0, 0 past K
-template <bool BF16>
+template <bool BF16, bool NT = false>
 __device__ __forceinline__ void fb_load8(const void* x, int64_t row, int64_t K, int64_t c0, float (&v)[8]) {
   const int64_t i = row * K + c0;
   if (c0 + 8 <= K) {
     if constexpr (BF16) {
-      const fb_u32x4_at2 w = *(const fb_u32x4_at2*)((const uint16_t*)x + i);
+      const uint4 q = fb_ld16<FbAt2, NT>((const uint16_t*)x + i);
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         v[2 * j] = __uint_as_float(w[j] << 16);
@@ -72,9 +92,9 @@ __device__ __forceinline__ void fb_load8(const void* x, int64_t row, int64_t K, 
     } else {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const fb_u32x4_at4 w = *(const fb_u32x4_at4*)((const float*)x + i + 4 * h);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[4 * h + j] = __uint_as_float(w[j]);
+        const uint4 q = fb_ld16<FbAt4, NT>((const float*)x + i + 4 * h);
+        v[4 * h] = __uint_as_float(q.x); v[4 * h + 1] = __uint_as_float(q.y);
+        v[4 * h + 2] = __uint_as_float(q.z); v[4 * h + 3] = __uint_as_float(q.w);
       }
     }
   } else {
@@ -85,7 +105,7 @@ __device__ __forceinline__ void fb_load8(const void* x, int64_t row, int64_t K, 
 }
 
 // ... and to it, nothing past K
-template <bool BF16>
+template <bool BF16, bool NT = false>
 __device__ __forceinline__ void fb_store8(void* y, int64_t row, int64_t K, int64_t c0, const float (&v)[8]) {
   const int64_t i = row * K + c0;
   if constexpr (BF16) {
@@ -93,7 +113,7 @@ __device__ __forceinline__ void fb_store8(void* y, int64_t row, int64_t K, int64
 #pragma unroll
     for (int j = 0; j < 4; ++j) u[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
     if (c0 + 8 <= K) {
-      *(fb_u32x4_at2*)((uint16_t*)y + i) = (fb_u32x4_at2){u[0], u[1], u[2], u[3]};
+      fb_st16<FbAt2, NT>((uint16_t*)y + i, make_uint4(u[0], u[1], u[2], u[3]));
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -103,9 +123,9 @@ __device__ __forceinline__ void fb_store8(void* y, int64_t row, int64_t K, int64
     if (c0 + 8 <= K) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        *(fb_u32x4_at4*)((float*)y + i + 4 * h) =
-            (fb_u32x4_at4){__float_as_uint(v[4 * h]), __float_as_uint(v[4 * h + 1]), __float_as_uint(v[4 * h + 2]),
-                           __float_as_uint(v[4 * h + 3])};
+        fb_st16<FbAt4, NT>((float*)y + i + 4 * h,
+                           make_uint4(__float_as_uint(v[4 * h]), __float_as_uint(v[4 * h + 1]),
+                                      __float_as_uint(v[4 * h + 2]), __float_as_uint(v[4 * h + 3])));
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)

@@ -25,12 +25,19 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 // ---------------------------------------------------------------------------
 // quantisation: 16 lanes a block, 8 values a lane
 // ---------------------------------------------------------------------------
+// chunk i of rows of n: its row and place in it (a 64-bit division takes as long as the loads)
+__device__ __forceinline__ void fb_place(int64_t i, int64_t n, int64_t rows, int64_t& row, int64_t& c) {
+  row = rows * n < 1LL << 32 ? (int64_t)((uint32_t)i / (uint32_t)n) : i / n;
+  c = i - row * n;
+}
+
 template <bool BF16>
 __global__ void __launch_bounds__(256)
 fb_quantize_kernel(const void* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t rows,
                    int64_t K) {
   const int64_t nb = fb_blocks(K), i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = i / (nb * 16), c = i - row * nb * 16;
+  int64_t row, c;
+  fb_place(i, nb * 16, rows, row, c);
   if (row >= rows) return;  // whole blocks
   float v[8];
   fb_load8<BF16>(x, row, K, c * 8, v);
@@ -42,7 +49,8 @@ __global__ void __launch_bounds__(256)
 fb_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, void* __restrict__ y,
                      int64_t rows, int64_t K) {
   const int64_t nb = fb_blocks(K), i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = i / (nb * 16), c = i - row * nb * 16;
+  int64_t row, c;
+  fb_place(i, nb * 16, rows, row, c);
   if (row >= rows || c * 8 >= K) return;
   const uint2 w = *(const uint2*)(codes + row * nb * FB_BLOCK + c * 8);
   const float s = fb_scale(scales[row * ((nb + 3) / 4 * 4) + c / 16]);
@@ -82,23 +90,27 @@ struct FbArgs {
 constexpr int FB_RECORD = 96;
 __host__ __device__ __forceinline__ int64_t fb_kept_row(int64_t h) { return fb_width(h) / 16 * FB_RECORD; }
 
-// 16 fp32 to 24 bits, to nearest: high halves and third bytes
+// a float's bits, its third byte to nearest
+__device__ __forceinline__ uint32_t fb_bits24(float v) {
+  const uint32_t b = __float_as_uint(v);
+  return (b & 0x7f800000u) == 0x7f800000u ? (b & 0x7fffffu ? b | 0x400000u : b) : b + 0x7fu + ((b >> 8) & 1u);
+}
+// 4 or 16 values: high halves and third bytes
+__device__ __forceinline__ void fb_pack24(const float (&v)[4], uint2& hi, uint32_t& lo) {
+  const uint32_t u[4] = {fb_bits24(v[0]), fb_bits24(v[1]), fb_bits24(v[2]), fb_bits24(v[3])};
+  hi = make_uint2(__builtin_amdgcn_perm(u[1], u[0], 0x07060302u), __builtin_amdgcn_perm(u[3], u[2], 0x07060302u));
+  lo = (u[0] >> 8 & 255u) | (u[1] & 0xff00u) | (u[2] << 8 & 0xff0000u) | (u[3] << 16 & 0xff000000u);
+}
 __device__ __forceinline__ void fb_pack24(const float (&v)[16], uint4 (&hi)[2], uint4& lo) {
-  uint32_t u[16];
+  uint2 h[4];
+  uint32_t l[4];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const uint32_t b = __float_as_uint(v[r]);
-    u[r] = (b & 0x7f800000u) == 0x7f800000u ? (b & 0x7fffffu ? b | 0x400000u : b) : b + 0x7fu + ((b >> 8) & 1u);
+  for (int q = 0; q < 4; ++q) {
+    const float f[4] = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+    fb_pack24(f, h[q], l[q]);
   }
-  uint32_t h[8], l[4];
-#pragma unroll
-  for (int r = 0; r < 8; ++r) h[r] = __builtin_amdgcn_perm(u[2 * r + 1], u[2 * r], 0x07060302u);
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-    l[r] = (u[4 * r] >> 8 & 255u) | (u[4 * r + 1] & 0xff00u) | (u[4 * r + 2] << 8 & 0xff0000u) |
-           (u[4 * r + 3] << 16 & 0xff000000u);
-  hi[0] = make_uint4(h[0], h[1], h[2], h[3]);
-  hi[1] = make_uint4(h[4], h[5], h[6], h[7]);
+  hi[0] = make_uint4(h[0].x, h[0].y, h[1].x, h[1].y);
+  hi[1] = make_uint4(h[2].x, h[2].y, h[3].x, h[3].y);
   lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 __device__ __forceinline__ void fb_unpack24(const uint4 (&hi)[2], const uint4& lo, float (&v)[16]) {
@@ -721,6 +733,217 @@ FbArgs codes_args(const void* x, const uint8_t* xs, const uint8_t* w, const uint
 }
 
 // ---------------------------------------------------------------------------
+// few rows (up to FB_FEW)
+// ---------------------------------------------------------------------------
+// Launches, latency and the weight's bytes are all there is: every load of a wave leaves
+// at once, straight to registers, and rows that are not codes yet are rounded on the way.
+constexpr int FB_FEW = 64;
+enum { X_F32 = 0, X_BF16 = 1, X_CODES = 2 };  // as the C types
+
+// 64 values of one block of a row (32 of each of its two steps, from c0 and c0 + 64) ->
+// their codes, the row's other 64 in lane + 32
+template <int XT>
+__device__ __forceinline__ void fb_round64(const void* x, int64_t row, int64_t K, int64_t c0, i32x8_t (&op)[2],
+                                           uint32_t& byte) {
+  float v[8][8];
+  uint32_t top = 0;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    fb_load8<XT == X_BF16>(x, row, K, c0 + q / 4 * 64 + q % 4 * 8, v[q]);
+    top = max(top, fb_amax8(v[q]));
+  }
+  byte = fb_scale_byte(max(top, (uint32_t)__shfl_xor((int)top, 32, 64)));
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const uint2 c = fb_encode8(v[q], byte);
+    op[q / 4][q % 4 * 2] = (int)c.x;
+    op[q / 4][q % 4 * 2 + 1] = (int)c.y;
+  }
+}
+
+// A workgroup has 32 rows of the weight (of the gated block 16 of gate's and 16 of up's),
+// its 8 waves a slice of K each; the waves' sums meet in LDS and are added in the order of
+// the waves.  A lane's codes of the weight lie in a row of their own; x's, which every
+// workgroup reads, do too up to 32 rows, past them they come through LDS in whole lines,
+// 16-byte chunks changing places by the row (us, direct and by LDS: 1 x 1024 -> 2560 4.1 and
+// 5.2, 64 x 2560 -> 1024 10.3 and 8.7).  RT: tiles of 32 rows of x.  Hidden values leave in fp32 (O_GATED): a block of their
+// codes would take 256 rows of weights a workgroup, whose bytes one CU waits for longer than
+// another launch takes (1 token, 1024 by 2560: 11 us for 4.5 and 2).
+template <int XT, int OT, int RT>
+__global__ void __launch_bounds__(512) fb_stream_kernel(FbArgs p, int64_t K) {
+  constexpr int NW = 8, U = 2;  // blocks read at once
+  constexpr bool GATED = OT == O_GATED, XL = XT == X_CODES && RT > 1;
+  constexpr int OWN = XL ? U * RT * 32 * FB_BLOCK : RT * 4096;  // a wave's x, and its sums
+  __shared__ __attribute__((aligned(1024))) char smem[NW * OWN];
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t n0 = (int64_t)blockIdx.x * (GATED ? 16 : 32), nb = p.ldx / FB_BLOCK, ns = (int64_t)p.words * 4;
+  const int tr = fb_perm(l32);  // row of the tile: the first 16 are lane group 0's sums
+  const int64_t wrow = min<int64_t>(n0 + (GATED ? tr & 15 : tr), p.N - 1);
+  const uint8_t* w = (GATED && tr >= 16 ? p.w2 : p.w) + wrow * p.ldx + g * 32;
+  const uint8_t* ws = (GATED && tr >= 16 ? p.s2 : p.s) + wrow * ns;
+  const int rows = (int)p.R, per = (int)((nb + NW - 1) / NW);
+  const int lo = (int)min<int64_t>((int64_t)wave * per, nb), hi = (int)min<int64_t>(lo + per, nb);
+  f32x16_t acc[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[t][r] = 0.0f;
+  char* own = smem + wave * OWN;
+  for (int b0 = lo; b0 < hi; b0 += U) {
+    i32x8_t wf[U][2], xf[U][RT][2];
+    uint32_t sw[U], sx[U][RT];
+    if constexpr (XL) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last pieces are read
+#pragma unroll
+      for (int a = 0; a < U * RT * 4; ++a) {  // 8 rows of a block
+        const int u = a / (RT * 4), r0 = a % (RT * 4) * 8, r = r0 + lane / 8;
+        if (r0 >= rows) continue;  // uniform; rows that nobody needs hold anything
+        dma16(p.x + (int64_t)min(b0 + u, hi - 1) * FB_BLOCK,
+              (uint32_t)(min(r, rows - 1) * (int)p.ldx + (lane % 8 ^ (r & 7)) * 16), lds_offset(own + a * 1024));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int b = min(b0 + u, hi - 1);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4* at = (const uint4*)(w + (int64_t)b * FB_BLOCK + h * 64);
+        wf[u][h] = fb_operand(at[0], at[1]);
+      }
+      sw[u] = ws[b];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const int64_t row = min(t * 32 + l32, rows - 1);
+        if constexpr (XT == X_CODES) {
+          sx[u][t] = p.xs[row * ns + b];
+#pragma unroll
+          for (int h = 0; h < 2 && !XL; ++h) {
+            const uint4* at = (const uint4*)(p.x + row * p.ldx + (int64_t)b * FB_BLOCK + h * 64 + g * 32);
+            xf[u][t][h] = fb_operand(at[0], at[1]);
+          }
+        } else fb_round64<XT>(p.x, row, K, (int64_t)b * FB_BLOCK + g * 32, xf[u][t], sx[u][t]);
+      }
+    }
+    if constexpr (XL) {
+      wait_vm<0>();
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const char* at = own + ((u * RT + t) * 32 + l32) * FB_BLOCK;
+            const int c = h * 4 + g * 2;
+            xf[u][t][h] = fb_operand(*(const uint4*)(at + (c ^ (l32 & 7)) * 16), *(const uint4*)(at + (c + 1 ^ (l32 & 7)) * 16));
+          }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (b0 + u >= hi) break;  // uniform
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          if constexpr (OT == O_F32) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                  fb_decode8(wf[u][h][2 * q], wf[u][h][2 * q + 1], fb_scale(sw[u])),
+                  fb_decode8(xf[u][t][h][2 * q], xf[u][t][h][2 * q + 1], fb_scale(sx[u][t])), acc[t], 0, 0, 0);
+          } else {
+            acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[u][h], xf[u][t][h], acc[t], 0, 0, 0, (int)sw[u],
+                                                                    0, (int)sx[u][t]);
+          }
+        }
+    }
+  }
+  __syncthreads();
+  float4* red = (float4*)smem;
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      red[((wave * RT + t) * 4 + i) * 64 + lane] =
+          make_float4(acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]);
+  __syncthreads();
+  auto sum = [&](int t, int i, int l, float (&f)[4]) {  // of the waves: four columns of a row
+    float4 v = red[(t * 4 + i) * 64 + l];
+#pragma unroll
+    for (int q = 1; q < NW; ++q) {
+      const float4 a = red[((q * RT + t) * 4 + i) * 64 + l];
+      v.x += a.x;
+      v.y += a.y;
+      v.z += a.z;
+      v.w += a.w;
+    }
+    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+  };
+  if constexpr (GATED) {
+    if (tid >= RT * 128) return;
+    const int l = tid & 31, i = tid >> 5 & 3, t = tid >> 7;
+    float f[4], v[4], a[4], b[4];
+    sum(t, i, l, f);
+    sum(t, i, l + 32, v);
+    const int64_t row = t * 32 + l, n = n0 + i * 4;
+    if (row >= rows) return;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      v[q] = fb_gated(f[q], v[q], a[q], b[q]);
+      if (n + q < p.N) ((float*)p.y)[row * p.N + n + q] = v[q];
+    }
+    if (p.kept) {
+      uint8_t* rec = p.kept + row * fb_kept_row(p.N) + (int64_t)blockIdx.x * FB_RECORD;
+      uint2 hi2;
+      uint32_t lo2;
+      fb_pack24(a, hi2, lo2);
+      *(uint2*)(rec + i * 8) = hi2;
+      *(uint32_t*)(rec + 64 + i * 4) = lo2;
+      fb_pack24(b, hi2, lo2);
+      *(uint2*)(rec + 32 + i * 8) = hi2;
+      *(uint32_t*)(rec + 80 + i * 4) = lo2;
+    }
+  } else {
+    for (int e = tid; e < RT * 256; e += 512) {
+      const int l = e & 63, i = e >> 6 & 3, t = e >> 8;
+      float f[4];
+      sum(t, i, l, f);
+      const int64_t row = t * 32 + (l & 31), n = n0 + (l >> 5) * 16 + i * 4;
+      if (row < rows) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (n + q < p.N) {
+            if constexpr (OT == O_BF16) ((__bf16*)p.y)[row * p.N + n + q] = (__bf16)f[q];
+            else ((float*)p.y)[row * p.N + n + q] = f[q];
+          }
+      }
+    }
+  }
+}
+
+template <int XT, int OT>
+int launch_stream_of(const FbArgs& p, int64_t K, hipStream_t stream) {
+  const int64_t blocks = OT == O_GATED ? (p.N + 15) / 16 : (p.N + 31) / 32;
+  if (!grid_fits(blocks, 512)) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block product: too many columns");
+  if (FB_FEW * p.ldx >= 1LL << 31) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block product: rows too wide");
+  auto* kernel = p.R <= 32 ? &fb_stream_kernel<XT, OT, 1> : &fb_stream_kernel<XT, OT, 2>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(512), 0, stream, p, K);
+  return check_launch("fb_stream_kernel");
+}
+// Whether fb_stream_kernel rounds rows itself: as long as a wave has one block of few of
+// them, whose rounding is then less than a launch (1 x 1024 -> 2560: 7.8 us on the device for
+// 4.1 and 2, but 9.7 for 12 as a call by itself; 16 x 2560 -> 1024: 11.8 for 6.3 and 2).
+bool rounds_itself(int64_t rows, int64_t K) { return rows <= 16 && fb_blocks(K) <= 8; }
+
+template <int OT>
+int launch_stream(const FbArgs& p, int x_dtype, int64_t K, hipStream_t stream) {
+  if (x_dtype == SMAUL_DTYPE_FP8_BLOCK) return launch_stream_of<X_CODES, OT>(p, K, stream);
+  if (x_dtype == SMAUL_DTYPE_BF16) return launch_stream_of<X_BF16, OT>(p, K, stream);
+  if constexpr (OT != O_GATED) return launch_stream_of<X_F32, OT>(p, K, stream);
+  return fail(SMAUL_ERR_INVALID, "fp8_block_ffn: bad dtype");
+}
+
+// ---------------------------------------------------------------------------
 // operands of the gradients' products: bf16 rows of whole stages (64 values)
 // ---------------------------------------------------------------------------
 // Several matrices a launch, each R rows of C values: bf16 rows, fp32 rows or codes
@@ -868,17 +1091,18 @@ int launch_quantize(const void* x, int dtype, uint8_t* codes, uint8_t* scales, i
 }
 
 struct FfnParts {
-  int64_t xc, xs, hc, hs, total;
+  int64_t xc, xs, hc, hs, hf, total;
 };
 // what the caller keeps for the gradients stands in `saved` (save), the rest in the workspace
 FfnParts ffn_parts(int64_t T, int64_t d, int64_t h, int x_dtype, bool save) {
   FfnParts q{};
   Parts w;
-  const bool rows = x_dtype != SMAUL_DTYPE_FP8_BLOCK && !save;
+  const bool rows = x_dtype != SMAUL_DTYPE_FP8_BLOCK && !save && !rounds_itself(T, d);
   q.xc = w.take(rows ? T * fb_width(d) : 0);
   q.xs = w.take(rows ? T * fb_words(d) * 4 : 0);
   q.hc = w.take(save ? 0 : T * fb_width(h));
   q.hs = w.take(save ? 0 : T * fb_words(h) * 4);
+  q.hf = w.take(T <= FB_FEW ? T * h * 4 : 0);
   q.total = w.at;
   return q;
 }
@@ -964,7 +1188,7 @@ int smaul_fp8_block_dequantize(const uint8_t* codes, const uint8_t* scales, void
 int64_t smaul_fp8_block_linear_workspace_size(int64_t rows, int64_t in_f, int64_t out_f, int x_dtype) {
   if (rows < 0 || in_f <= 0 || out_f <= 0 || !x_ok(x_dtype)) return -1;
   Parts w;
-  if (x_dtype != SMAUL_DTYPE_FP8_BLOCK) {
+  if (x_dtype != SMAUL_DTYPE_FP8_BLOCK && !rounds_itself(rows, in_f)) {
     w.take(rows * fb_width(in_f));
     w.take(rows * fb_words(in_f) * 4);
   }
@@ -985,14 +1209,18 @@ int smaul_fp8_block_linear(const void* x, int x_dtype, const uint8_t* xs, const 
   if (workspace_bytes < need || (need > 0 && (!workspace || !fb_aligned(workspace, 256))))
     return fail(SMAUL_ERR_INVALID, "fp8_block_linear: workspace %lld < %lld bytes, or unaligned",
                 (long long)workspace_bytes, (long long)need);
-  if (!given) {
+  if (!given && !rounds_itself(rows, in_f)) {
     uint8_t* c = (uint8_t*)workspace;
     uint8_t* cs = c + fb_align256(rows * fb_width(in_f));
     if (int rc = launch_quantize(x, x_dtype, c, cs, rows, in_f, stream)) return rc;
     x = c;
     xs = cs;
+    x_dtype = SMAUL_DTYPE_FP8_BLOCK;
   }
   const FbArgs p = codes_args(x, xs, w, s, y, rows, in_f, out_f);
+  if (rows <= FB_FEW)
+    return y_dtype == SMAUL_DTYPE_BF16 ? launch_stream<O_BF16>(p, x_dtype, in_f, stream)
+                                       : launch_stream<O_F32>(p, x_dtype, in_f, stream);
   return y_dtype == SMAUL_DTYPE_BF16 ? launch_product<F_CODES, O_BF16>(p, stream) : launch_product<F_CODES, O_F32>(p, stream);
 }
 
@@ -1063,7 +1291,10 @@ int smaul_fp8_block_ffn_forward(const void* x, int x_dtype, const uint8_t* xs, c
     return fail(SMAUL_ERR_INVALID, "fp8_block_ffn: workspace %lld < %lld bytes, or unaligned",
                 (long long)workspace_bytes, (long long)q.total);
   uint8_t* ws = (uint8_t*)workspace;
-  if (!given) {
+  const bool few = T <= FB_FEW;
+  int xt = x_dtype;
+  if (!given && (save || !rounds_itself(T, d))) {
+    xt = SMAUL_DTYPE_FP8_BLOCK;
     uint8_t* xc = save ? x_codes : ws + q.xc;
     uint8_t* xcs = save ? x_scales : ws + q.xs;
     if (int rc = launch_quantize(x, x_dtype, xc, xcs, T, d, stream)) return rc;
@@ -1077,8 +1308,15 @@ int smaul_fp8_block_ffn_forward(const void* x, int x_dtype, const uint8_t* xs, c
   p.s2 = up_s;
   p.ys = hs;
   p.kept = (uint8_t*)saved;
-  if (int rc = launch_product<F_CODES, O_GATED>(p, stream)) return rc;
-  return launch_product<F_CODES, O_BF16>(codes_args(hc, hs, down_w, down_s, y, T, h, d), stream);
+  const FbArgs down = codes_args(hc, hs, down_w, down_s, y, T, h, d);
+  if (!few) {
+    if (int rc = launch_product<F_CODES, O_GATED>(p, stream)) return rc;
+    return launch_product<F_CODES, O_BF16>(down, stream);
+  }
+  p.y = ws + q.hf;
+  if (int rc = launch_stream<O_GATED>(p, xt, d, stream)) return rc;
+  if (int rc = launch_quantize(ws + q.hf, SMAUL_DTYPE_F32, hc, hs, T, h, stream)) return rc;
+  return launch_stream<O_BF16>(down, SMAUL_DTYPE_FP8_BLOCK, h, stream);
 }
 
 int64_t smaul_fp8_block_ffn_backward_workspace_size(int64_t T, int64_t d, int64_t h) {

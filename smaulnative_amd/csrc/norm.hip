@@ -8,102 +8,241 @@
 #include "fp8_block.h"
 
 using smaul::check_launch;
+using smaul::cu_count;
 using smaul::fail;
 using smaul::grid_fits;
 
 namespace {
 
-// the sum over a row's NW waves, in each of their lanes (red: NW floats of the row's own)
+// The sum over a row's NW waves, in each of their lanes (red: NW values of the row's own).
 template <int NW>
-__device__ __forceinline__ float row_sum(float v, float* red, int wave) {
+__device__ __forceinline__ double row_sum(double v, double* red, int wave) {
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
   if constexpr (NW > 1) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[wave] = v;
     __syncthreads();
-    v = 0.0f;
+    v = 0.0;
 #pragma unroll
     for (int w = 0; w < NW; ++w) v += red[w];
   }
   return v;
 }
 
-__device__ __forceinline__ float inv_rms(float ss, int64_t d, float eps) {
-  return 1.0f / __fsqrt_rn(ss / (float)d + eps);
+// 1 / sqrt(m): the 32-bit root with one step of Newton in 64
+__device__ __forceinline__ double inv_root(double m) {
+  if (!(m > 1e-30 && m < 1e30)) return 1.0 / sqrt(m);
+  const double r = (double)__builtin_amdgcn_rsqf((float)m);
+  return r * (1.5 - 0.5 * m * r * r);
+}
+
+__device__ __forceinline__ float sum_squares(const float (&v)[8]) {
+  float a = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a = fmaf(v[j], v[j], a);
+  return a;
 }
 
 // A row is NW waves', a lane has 8 values of every NW * 512, the first CH of them kept in
-// registers (the rest are read again).
-template <bool BF16, bool CODES, int NW, int CH>
+// registers (the rest are read again).  Memory bounds it.
+//
+// 8 values' squares are summed in 32 bits, the rest of the sum and the root in 64, and the
+// two products with 1 / rms and the weight carry their errors along (1 / rms as two
+// floats): y is off by little more than its own rounding, so that a code is seldom the
+// neighbouring one of what 64 bits give (in 32 bits throughout about one in 250000).
+template <bool BF16, bool CODES, bool NT, int NW, int CH>
 __global__ void __launch_bounds__(256)
 add_rms_norm_kernel(const void* __restrict__ x, const void* __restrict__ r, const float* __restrict__ weight,
                     void* __restrict__ sum, void* __restrict__ out, uint8_t* __restrict__ scales, int64_t T, int64_t d,
                     float eps) {
   constexpr int ROWS = 4 / NW;
-  __shared__ float red[4];
+  __shared__ double red[4];
   const int lane = threadIdx.x & 63, w4 = threadIdx.x >> 6, wave = w4 % NW;
   const int64_t t = (int64_t)blockIdx.x * ROWS + w4 / NW;
   if (NW == 1 && t >= T) return;  // a workgroup of more waves has one row
   const int64_t nb = fb_blocks(d), chunks = nb * 16;
-  float keep[CH][8];
-  // s of the chunk that begins at column c, and what is stored of it
-  auto load = [&](int64_t c, float (&v)[8]) {
-    fb_load8<BF16>(x, t, d, c, v);
+  float keep[CH][8], extra[CH][8];
+  auto chunk = [&](int i) -> int64_t { return (int64_t)i * (NW * 64) + wave * 64 + lane; };
+  double ss = 0.0;
+  // s of the chunk that begins at column c
+  auto add = [&](int64_t c, float (&v)[8], const float (&q)[8]) {
     if (r) {
-      float q[8];
-      fb_load8<BF16>(r, t, d, c, q);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = BF16 ? (float)(__bf16)(v[j] + q[j]) : v[j] + q[j];
     }
   };
-  float ss = 0.0f;
-  auto add = [&](int64_t c, const float (&v)[8]) {
-    if (r && c < d) fb_store8<BF16>(sum, t, d, c, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
-  };
-  auto chunk = [&](int i) -> int64_t { return (int64_t)i * (NW * 64) + wave * 64 + lane; };
-#pragma unroll
-  for (int i = 0; i < CH; ++i) load(chunk(i) * 8, keep[i]);
-#pragma unroll
-  for (int i = 0; i < CH; ++i) add(chunk(i) * 8, keep[i]);
-  for (int i = CH; chunk(i) - lane < chunks; ++i) {
-    float v[8];
-    load(chunk(i) * 8, v);
-    add(chunk(i) * 8, v);
+  for (int i = 0; i < CH; ++i) {
+    fb_load8<BF16, NT>(x, t, d, chunk(i) * 8, keep[i]);
+    if (r) fb_load8<BF16, NT>(r, t, d, chunk(i) * 8, extra[i]);
   }
-  const float rstd = inv_rms(row_sum<NW>(ss, red, wave), d, eps);
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    add(chunk(i) * 8, keep[i], extra[i]);
+    if (r && chunk(i) * 8 < d) fb_store8<BF16, NT>(sum, t, d, chunk(i) * 8, keep[i]);
+    ss += (double)sum_squares(keep[i]);
+  }
+  for (int i = CH; chunk(i) - lane < chunks; ++i) {
+    float v[8], q[8];
+    fb_load8<BF16, NT>(x, t, d, chunk(i) * 8, v);
+    if (r) fb_load8<BF16, NT>(r, t, d, chunk(i) * 8, q);
+    add(chunk(i) * 8, v, q);
+    if (r && chunk(i) * 8 < d) fb_store8<BF16, NT>(sum, t, d, chunk(i) * 8, v);
+    ss += (double)sum_squares(v);
+  }
+  const double root = inv_root(row_sum<NW>(ss, red, wave) / (double)d + (double)eps);
+  const float rh = (float)root, rl = (float)(root - (double)rh);
   auto put = [&](int64_t c, float (&v)[8]) {  // whole blocks of lanes
     if (c >= chunks * 8) return;
-    float wv[8];
+    float w[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) wv[j] = 1.0f;
-    if (weight) fb_load8<false>(weight, 0, d, c, wv);
+    for (int j = 0; j < 8; ++j) w[j] = 1.0f;
+    if (weight) fb_load8<false>(weight, 0, d, c, w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = v[j] * rstd * wv[j];
+    for (int j = 0; j < 8; ++j) {
+      const float a = v[j] * rh, ae = fmaf(v[j], rl, fmaf(v[j], rh, -a));
+      const float y = a * w[j], ye = fmaf(ae, w[j], fmaf(a, w[j], -y)), z = y + ye;
+      v[j] = z == z ? z : y;  // an infinity has no error to carry
+    }
     if constexpr (CODES) fb_write8((uint8_t*)out, scales, t, nb, c / 8, v);
-    else if (c < d) fb_store8<BF16>(out, t, d, c, v);
+    else if (c < d) fb_store8<BF16, NT>(out, t, d, c, v);
   };
 #pragma unroll
   for (int i = 0; i < CH; ++i) put(chunk(i) * 8, keep[i]);
   for (int i = CH; chunk(i) - lane < chunks; ++i) {
-    float v[8];
-    load(chunk(i) * 8, v);
+    float v[8], q[8];
+    fb_load8<BF16, NT>(x, t, d, chunk(i) * 8, v);
+    if (r) fb_load8<BF16, NT>(r, t, d, chunk(i) * 8, q);
+    add(chunk(i) * 8, v, q);
     put(chunk(i) * 8, v);
   }
 }
 
-// Rows blockIdx.x, + gridDim.x, ...: a workgroup's share of dw stays in registers until
-// its rows are done.  Columns from CH * 2048 on take another pass of the kernel's loop
-// for their part of dw (col0).
-template <bool BF16, int CH>
+// One pass over the rows: a row's values and gradients stay in registers between its two
+// sums and dx, the next row's are on their way meanwhile, and a workgroup's share of dw
+// stays until its rows (blockIdx.x * ROWS, + gridDim.x * ROWS, ...) are done;
+// norm_weight_sum_kernel adds the shares in their order.  d is no more than NW * CH * 512.
+template <bool BF16, bool NT, int NW, int CH>
 __global__ void __launch_bounds__(256)
 add_rms_norm_backward_kernel(const void* __restrict__ dy, const void* __restrict__ s, const void* __restrict__ ds,
                              const float* __restrict__ weight, void* __restrict__ dx, float* __restrict__ part,
                              int64_t T, int64_t d, float eps) {
-  __shared__ float red[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int ROWS = 4 / NW;
+  __shared__ double red[2][8];
+  __shared__ float share[NW < 4 ? 4 * 512 : 1];
+  const int lane = threadIdx.x & 63, w4 = threadIdx.x >> 6, wave = w4 % NW, first = w4 - wave;
+  auto col = [&](int i) -> int64_t { return ((int64_t)i * (NW * 64) + wave * 64 + lane) * 8; };
+  float w[CH][8], acc[CH][8], v[CH][8], g[CH][8], o[CH][8];
+#pragma unroll
+  for (int i = 0; i < CH; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      w[i][j] = 1.0f;
+      acc[i][j] = 0.0f;
+      o[i][j] = 0.0f;
+    }
+  if (weight) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) fb_load8<false>(weight, 0, d, col(i), w[i]);
+  }
+  auto load = [&](int64_t t, float (&a)[CH][8], float (&b)[CH][8], float (&c)[CH][8]) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      fb_load8<BF16, NT>(s, t, d, col(i), a[i]);
+      fb_load8<BF16, NT>(dy, t, d, col(i), b[i]);
+      if (ds) fb_load8<BF16, NT>(ds, t, d, col(i), c[i]);
+    }
+  };
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  int64_t t = (int64_t)blockIdx.x * ROWS + w4 / NW;
+  if (t < T) load(t, v, g, o);
+  int turn = 0;
+  for (int64_t t0 = (int64_t)blockIdx.x * ROWS; t0 < T; t0 += step, t += step, turn ^= 1) {  // of the whole workgroup
+    float v2[CH][8], g2[CH][8], o2[CH][8];
+    if (t + step < T) load(t + step, v2, g2, o2);
+    double ss = 0.0, sd = 0.0;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      float a = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a = fmaf(w[i][j] * g[i][j], v[i][j], a);
+      ss += (double)sum_squares(v[i]);
+      sd += (double)a;
+    }
+#pragma unroll
+    for (int q = 32; q >= 1; q >>= 1) {
+      ss += __shfl_xor(ss, q, 64);
+      sd += __shfl_xor(sd, q, 64);
+    }
+    if constexpr (NW > 1) {  // two places by turns: one barrier a row
+      if (lane == 0) {
+        red[turn][w4] = ss;
+        red[turn][4 + w4] = sd;
+      }
+      __syncthreads();
+      ss = sd = 0.0;
+#pragma unroll
+      for (int q = 0; q < NW; ++q) {
+        ss += red[turn][first + q];
+        sd += red[turn][4 + first + q];
+      }
+    }
+    if (t >= T) continue;  // a last row that is not there
+    const double root = inv_root(ss / (double)d + (double)eps);
+    const float rstd = (float)root, dot = (float)(sd / (double)d * root * root);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        acc[i][j] = fmaf(g[i][j], v[i][j] * rstd, acc[i][j]);
+        o[i][j] += (w[i][j] * g[i][j] - v[i][j] * dot) * rstd;
+      }
+      if (col(i) < d) fb_store8<BF16, NT>(dx, t, d, col(i), o[i]);
+    }
+    if (t + step < T) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          v[i][j] = v2[i][j];
+          g[i][j] = g2[i][j];
+          o[i][j] = ds ? o2[i][j] : 0.0f;
+        }
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    if constexpr (NW < 4) {  // its rows' waves
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) share[w4 * 512 + j * 64 + lane] = acc[i][j];
+      __syncthreads();
+      if (first == 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float a = 0.0f;
+#pragma unroll
+          for (int q = 0; q < ROWS; ++q) a += share[(q * NW + wave) * 512 + j * 64 + lane];
+          acc[i][j] = a;
+        }
+        if (col(i) < d) fb_store8<false>(part, blockIdx.x, d, col(i), acc[i]);
+      }
+    } else if (col(i) < d) {
+      fb_store8<false>(part, blockIdx.x, d, col(i), acc[i]);
+    }
+  }
+}
+
+// Rows of any width: read again for dx, and for every CH * 2048 columns of dw.
+template <bool BF16, int CH>
+__global__ void __launch_bounds__(256)
+add_rms_norm_backward_wide_kernel(const void* __restrict__ dy, const void* __restrict__ s, const void* __restrict__ ds,
+                                  const float* __restrict__ weight, void* __restrict__ dx, float* __restrict__ part,
+                                  int64_t T, int64_t d, float eps) {
+  __shared__ double red[4];
+  const int wave = threadIdx.x >> 6;
   const int64_t chunks = (d + 7) / 8;
   for (int64_t c0 = 0; c0 < chunks; c0 += CH * 256) {  // of dw's columns
     float acc[CH][8];
@@ -112,22 +251,21 @@ add_rms_norm_backward_kernel(const void* __restrict__ dy, const void* __restrict
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[i][j] = 0.0f;
     for (int64_t t = blockIdx.x; t < T; t += gridDim.x) {
-      float ss = 0.0f, sd = 0.0f;
+      double ss = 0.0, sd = 0.0;
       for (int64_t c = threadIdx.x; c < chunks; c += 256) {
-        float v[8], g[8], w[8];
+        float v[8], g[8], w[8], a = 0.0f;
         fb_load8<BF16>(s, t, d, c * 8, v);
         fb_load8<BF16>(dy, t, d, c * 8, g);
 #pragma unroll
         for (int j = 0; j < 8; ++j) w[j] = 1.0f;
         if (weight) fb_load8<false>(weight, 0, d, c * 8, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          ss = fmaf(v[j], v[j], ss);
-          sd = fmaf(w[j] * g[j], v[j], sd);
-        }
+        for (int j = 0; j < 8; ++j) a = fmaf(w[j] * g[j], v[j], a);
+        ss += (double)sum_squares(v);
+        sd += (double)a;
       }
-      const float rstd = inv_rms(row_sum<4>(ss, red, wave), d, eps);
-      const float dot = row_sum<4>(sd, red, wave) / (float)d * rstd * rstd;
+      const double root = inv_root(row_sum<4>(ss, red, wave) / (double)d + (double)eps);
+      const float rstd = (float)root, dot = (float)(row_sum<4>(sd, red, wave) / (double)d * root * root);
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int64_t c = c0 + i * 256 + threadIdx.x;
@@ -163,21 +301,32 @@ add_rms_norm_backward_kernel(const void* __restrict__ dy, const void* __restrict
   }
 }
 
-// dw: the workgroups' parts, in their order
-__global__ void __launch_bounds__(256)
+// dw: the workgroups' parts, 32 of them at a time, in their order
+__global__ void __launch_bounds__(1024)
 norm_weight_sum_kernel(const float* __restrict__ part, float* __restrict__ dw, int parts, int64_t d) {
-  __shared__ float sh[4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  __shared__ float sh[32][33];
+  const int col = threadIdx.x & 31, row = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + col;
   float a = 0.0f;
-  if (c < d)
-    for (int p = wave; p < parts; p += 4) a += part[p * d + c];
-  sh[wave][lane] = a;
+  if (c < d) {
+#pragma unroll 8
+    for (int p = row; p < parts; p += 32) a += part[p * d + c];
+  }
+  sh[row][col] = a;
   __syncthreads();
-  if (wave == 0 && c < d) dw[c] = sh[0][lane] + sh[1][lane] + sh[2][lane] + sh[3][lane];
+  if (row == 0 && c < d) {
+    float t = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) t += sh[r][col];
+    dw[c] = t;
+  }
 }
 
-int norm_parts(int64_t T) { return (int)(T < 512 ? T : 512); }
+// workgroups of the backward pass, each with a part of dw: four a CU
+int64_t norm_parts(int64_t T, int64_t d) {
+  const int64_t rows = d <= 512 ? (T + 3) / 4 : d <= 1024 ? (T + 1) / 2 : T, most = 4 * cu_count();
+  return rows < most ? rows : most;
+}
 
 }  // namespace
 
@@ -191,30 +340,38 @@ int smaul_add_rms_norm(const void* x, const void* residual, int dtype, const flo
   if (!x || !out || (residual && !sum)) return fail(SMAUL_ERR_INVALID, "add_rms_norm: null pointer");
   if (scales && !fb_aligned(out, 8)) return fail(SMAUL_ERR_INVALID, "add_rms_norm: codes must be 8-byte aligned");
   const bool bf16 = dtype == SMAUL_DTYPE_BF16;
-  const int64_t blocks = d <= 2048 ? (T + 3) / 4 : T;
+  const bool nt = T * d * (bf16 ? 2 : 4) >= FB_NT_BYTES;
+  // a workgroup a row from 2048 columns on, and for so few rows that a wave a row would
+  // leave most of the chip idle
+  const bool wide = d > 2048 || T <= cu_count();
+  const int64_t blocks = wide ? T : (T + 3) / 4;
   if (!grid_fits(blocks, 256)) return fail(SMAUL_ERR_UNSUPPORTED, "add_rms_norm: too many rows");
-  const dim3 grid((unsigned)blocks), block(256);
-#define SMAUL_N(B, C, NW) \
-  hipLaunchKernelGGL((add_rms_norm_kernel<B, C, NW, 4>), grid, block, 0, stream, x, residual, weight, sum, out, scales, \
-                     T, d, eps)
-  if (d <= 2048) {
-    if (bf16 && scales) SMAUL_N(true, true, 1);
-    else if (bf16) SMAUL_N(true, false, 1);
-    else if (scales) SMAUL_N(false, true, 1);
-    else SMAUL_N(false, false, 1);
-  } else {
-    if (bf16 && scales) SMAUL_N(true, true, 4);
-    else if (bf16) SMAUL_N(true, false, 4);
-    else if (scales) SMAUL_N(false, true, 4);
-    else SMAUL_N(false, false, 4);
-  }
+#define SMAUL_N(B, C, N)                                                                                             \
+  do {                                                                                                               \
+    auto* kernel = wide ? (d <= 2048 ? &add_rms_norm_kernel<B, C, false, 4, 1> : &add_rms_norm_kernel<B, C, N, 4, 4>) \
+                   : d <= 512  ? &add_rms_norm_kernel<B, C, N, 1, 1>                                                  \
+                   : d <= 1024 ? &add_rms_norm_kernel<B, C, N, 1, 2>                                                  \
+                               : &add_rms_norm_kernel<B, C, N, 1, 4>;                                                 \
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, x, residual, weight, sum, out, scales,  \
+                       T, d, eps);                                                                                   \
+  } while (0)
+#define SMAUL_NT(B, C)           \
+  do {                           \
+    if (nt) SMAUL_N(B, C, true); \
+    else SMAUL_N(B, C, false);   \
+  } while (0)
+  if (bf16 && scales) SMAUL_NT(true, true);
+  else if (bf16) SMAUL_NT(true, false);
+  else if (scales) SMAUL_NT(false, true);
+  else SMAUL_NT(false, false);
+#undef SMAUL_NT
 #undef SMAUL_N
   return check_launch("add_rms_norm_kernel");
 }
 
 int64_t smaul_add_rms_norm_backward_workspace_size(int64_t T, int64_t d) {
   if (T < 0 || d <= 0) return -1;
-  return norm_parts(T) * d * 4;
+  return norm_parts(T, d) * d * 4;
 }
 
 int smaul_add_rms_norm_backward(const void* dy, const void* s, const void* ds, int dtype, const float* weight,
@@ -230,17 +387,28 @@ int smaul_add_rms_norm_backward(const void* dy, const void* s, const void* ds, i
   if (workspace_bytes < need || (need > 0 && (!workspace || !fb_aligned(workspace, 256))))
     return fail(SMAUL_ERR_INVALID, "add_rms_norm_backward: workspace %lld < %lld bytes, or unaligned",
                 (long long)workspace_bytes, (long long)need);
-  if (!grid_fits((d + 63) / 64, 256)) return fail(SMAUL_ERR_UNSUPPORTED, "add_rms_norm_backward: rows too wide");
-  const int parts = norm_parts(T);
+  if (!grid_fits((d + 31) / 32, 1024)) return fail(SMAUL_ERR_UNSUPPORTED, "add_rms_norm_backward: rows too wide");
+  const int parts = (int)norm_parts(T, d);
   float* part = dw ? (float*)workspace : nullptr;
   if (T > 0) {
-    auto* kernel = dtype == SMAUL_DTYPE_BF16 ? &add_rms_norm_backward_kernel<true, 4>
-                                             : &add_rms_norm_backward_kernel<false, 4>;
+    const bool bf16 = dtype == SMAUL_DTYPE_BF16;
+    const bool nt = T * d * (bf16 ? 2 : 4) >= FB_NT_BYTES;
+    auto* kernel = bf16 ? &add_rms_norm_backward_wide_kernel<true, 4> : &add_rms_norm_backward_wide_kernel<false, 4>;
+#define SMAUL_B(NW, CH)                                                                         \
+  kernel = bf16 ? (nt ? &add_rms_norm_backward_kernel<true, true, NW, CH>                       \
+                      : &add_rms_norm_backward_kernel<true, false, NW, CH>)                     \
+                : (nt ? &add_rms_norm_backward_kernel<false, true, NW, CH>                      \
+                      : &add_rms_norm_backward_kernel<false, false, NW, CH>)
+    if (d <= 512) SMAUL_B(1, 1);
+    else if (d <= 1024) SMAUL_B(2, 1);
+    else if (d <= 2048) SMAUL_B(4, 1);
+    else if (d <= 4096) SMAUL_B(4, 2);
+#undef SMAUL_B
     hipLaunchKernelGGL(kernel, dim3((unsigned)parts), dim3(256), 0, stream, dy, s, ds, weight, dx, part, T, d, eps);
     if (int rc = check_launch("add_rms_norm_backward_kernel")) return rc;
   }
   if (!dw) return SMAUL_OK;
-  hipLaunchKernelGGL(norm_weight_sum_kernel, dim3((unsigned)((d + 63) / 64)), dim3(256), 0, stream, part, dw, parts, d);
+  hipLaunchKernelGGL(norm_weight_sum_kernel, dim3((unsigned)((d + 31) / 32)), dim3(1024), 0, stream, part, dw, parts, d);
   return check_launch("norm_weight_sum_kernel");
 }
 

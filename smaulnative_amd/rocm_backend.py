@@ -91,6 +91,13 @@ def _need_device(name: str, *tensors):
             raise RuntimeError(f"{name}: tensors are on different devices ({dev} vs {t.device})")
 
 
+def _need_one_device(name: str, first, *more):
+    """``_need_device`` of tensors that are mostly there: one look at each."""
+    index = first.get_device()
+    if index < 0 or any(t is not None and t.get_device() != index for t in more):
+        _need_device(name, first, *more)
+
+
 class RocmBackend:
     """MI355X backend over libsmaul_rocm.so (hand-written HIP for gfx950)."""
 
@@ -676,7 +683,7 @@ class RocmBackend:
         the least with which no code saturates.  Codes past K and scales past n are 0.  A
         block that holds an infinity or NaN is all NaN (scale 255)."""
         lib = _lib.load()
-        _need_device("fp8_block_quantize", x)
+        _need_one_device("fp8_block_quantize", x)
         if x.dtype not in _ACT or x.dim() < 1 or x.shape[-1] < 1:
             raise RuntimeError(f"fp8_block_quantize: x must be float32 or bfloat16 rows, got {x.dtype} "
                                f"{tuple(x.shape)}")
@@ -694,11 +701,11 @@ class RocmBackend:
     def _block_check(self, name, codes, scales, lead, K):
         """The codes and scales [*lead, 128 n] / [*lead, 4 ceil(n / 4)] of rows of K values, contiguous."""
         n = (K + 127) // 128
-        if codes.dtype != torch.uint8 or codes.shape != (*lead, n * 128):
+        ns = (n + 3) // 4 * 4
+        if codes.dtype is not torch.uint8 or codes.shape != (*lead, n * 128):
             raise RuntimeError(f"{name}: codes must be uint8 {[*lead, n * 128]}, got {codes.dtype} "
                                f"{list(codes.shape)}")
-        ns = (n + 3) // 4 * 4
-        if scales.dtype != torch.uint8 or scales.shape != (*lead, ns):
+        if scales.dtype is not torch.uint8 or scales.shape != (*lead, ns):
             raise RuntimeError(f"{name}: scales must be uint8 {[*lead, ns]}, got {scales.dtype} {list(scales.shape)}")
         return self._aligned(codes), self._aligned(scales)
 
@@ -706,7 +713,7 @@ class RocmBackend:
         """The values [..., in_f] in ``dtype`` (fp32 or bf16, exact in both down to its
         subnormals) that codes and scales (``fp8_block_quantize``) stand for."""
         lib = _lib.load()
-        _need_device("fp8_block_dequantize", codes, scales)
+        _need_one_device("fp8_block_dequantize", codes, scales)
         if dtype not in _ACT:
             raise RuntimeError(f"fp8_block_dequantize: dtype must be float32 or bfloat16, got {dtype}")
         if in_f < 1:
@@ -727,7 +734,7 @@ class RocmBackend:
             raise RuntimeError(f"{name}: rows of {width} values expected, got a scalar")
         lead = tuple(x.shape[:-1])
         if xs is not None:
-            return (*self._block_check(f"{name}: x", x, xs, lead, width), _lib.DTYPE_FP8_BLOCK, lead)
+            return (*self._block_check(name, x, xs, lead, width), _lib.DTYPE_FP8_BLOCK, lead)
         if x.dtype not in types:
             names = " or ".join(str(t).replace("torch.", "") for t in types)
             raise RuntimeError(f"{name}: rows must be {names} (or codes with their scales), got {x.dtype}")
@@ -741,7 +748,7 @@ class RocmBackend:
         format; with scales ``xs`` it is codes already.  ``dtype`` of y: fp32 or bf16, by
         default x's, of codes bf16.  Products are exact, sums fp32."""
         lib = _lib.load()
-        _need_device("fp8_block_forward", x, xs, w, s)
+        _need_one_device("fp8_block_forward", x, xs, w, s)
         if in_f < 1 or out_f < 1:
             raise ValueError(f"fp8_block_forward: in_f/out_f must be positive, got {in_f}/{out_f}")
         w, s = self._block_check("fp8_block_forward", w, s, (out_f,), in_f)
@@ -765,7 +772,7 @@ class RocmBackend:
         """dx [..., in_f] = g [..., out_f] . W in g's type (fp32 or bf16): the input gradient
         of ``fp8_block_forward``, straight through the rounding of its rows."""
         lib = _lib.load()
-        _need_device("fp8_block_backward_input", g, w, s)
+        _need_one_device("fp8_block_backward_input", g, w, s)
         if in_f < 1 or out_f < 1:
             raise ValueError(f"fp8_block_backward_input: in_f/out_f must be positive, got {in_f}/{out_f}")
         w, s = self._block_check("fp8_block_backward_input", w, s, (out_f,), in_f)
@@ -786,8 +793,9 @@ class RocmBackend:
             raise ValueError(f"{name}: d/h must be positive, got {d}/{h}")
         if len(weights) != 6:
             raise ValueError(f"{name}: weights is (gate_w, gate_s, up_w, up_s, down_w, down_s)")
-        return [t for i, what, n, k in ((0, "gate", h, d), (2, "up", h, d), (4, "down", d, h))
-                for t in self._block_check(f"{name}: {what}", weights[i], weights[i + 1], (n,), k)]
+        return (*self._block_check(name, weights[0], weights[1], (h,), d),
+                *self._block_check(name, weights[2], weights[3], (h,), d),
+                *self._block_check(name, weights[4], weights[5], (d,), h))
 
     def fp8_block_ffn_forward(self, x, weights, d, h, xs=None, save=False):
         """The gated feed-forward block y [..., d] (bf16) = Q(silu(x Wg^T) * (x Wu^T)) Wd^T.
@@ -797,7 +805,7 @@ class RocmBackend:
         Sums are fp32, the hidden rows are rounded to codes from fp32.  With ``save`` returns
         (y, saved), what ``fp8_block_ffn_backward`` takes."""
         lib = _lib.load()
-        _need_device("fp8_block_ffn_forward", x, xs, *weights)
+        _need_one_device("fp8_block_ffn_forward", x, xs, *weights)
         weights = self._block_weights("fp8_block_ffn_forward", weights, d, h)
         xc, xsc, xt, lead = self._block_rows("fp8_block_ffn_forward", x, xs, d, (torch.bfloat16,))
         dev = x.device
@@ -828,7 +836,7 @@ class RocmBackend:
         ``fp8_block_ffn_forward`` from dy [..., d] (bf16), its weights and what it saved,
         straight through the roundings; None for what is not asked for."""
         lib = _lib.load()
-        _need_device("fp8_block_ffn_backward", dy, *weights, *saved)
+        _need_one_device("fp8_block_ffn_backward", dy, *weights, *saved)
         weights = self._block_weights("fp8_block_ffn_backward", weights, d, h)
         dyc, _, _, lead = self._block_rows("fp8_block_ffn_backward", dy, None, d, (torch.bfloat16,))
         dev = dy.device
@@ -836,8 +844,8 @@ class RocmBackend:
         if len(saved) != 5 or saved[4].dtype != torch.uint8 or \
                 saved[4].numel() != lib.smaul_fp8_block_ffn_saved_size(T, h):
             raise RuntimeError(f"fp8_block_ffn_backward: saved is of another call than one of {T} rows")
-        xc, xs = self._block_check("fp8_block_ffn_backward: x", saved[0], saved[1], tuple(saved[0].shape[:-1]), d)
-        hc, hs = self._block_check("fp8_block_ffn_backward: hidden rows", saved[2], saved[3], (T,), h)
+        xc, xs = self._block_check("fp8_block_ffn_backward", saved[0], saved[1], tuple(saved[0].shape[:-1]), d)
+        hc, hs = self._block_check("fp8_block_ffn_backward", saved[2], saved[3], (T,), h)
         if xs.numel() // xs.shape[-1] != T:
             raise RuntimeError(f"fp8_block_ffn_backward: saved is of another call than one of {T} rows")
         kept = self._aligned(saved[4])
@@ -1187,7 +1195,7 @@ class RocmBackend:
 
         x and residual [..., d] bf16 or fp32, one type; weight [d] (None: ones)."""
         lib = _lib.load()
-        _need_device("add_rms_norm", x, residual, weight)
+        _need_one_device("add_rms_norm", x, residual, weight)
         w, (xc, rc_) = self._norm_check("add_rms_norm", eps, weight, x, residual)
         d, dev = x.shape[-1], x.device
         s = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
@@ -1211,7 +1219,7 @@ class RocmBackend:
         dy, the sum s it returned and the sum's own gradient ``ds`` (None: zero).  dx is the
         residual's gradient too.  Straight through the rounding of y."""
         lib = _lib.load()
-        _need_device("add_rms_norm_backward", dy, s, weight, ds)
+        _need_one_device("add_rms_norm_backward", dy, s, weight, ds)
         w, (dyc, sc, dsc) = self._norm_check("add_rms_norm_backward", eps, weight, dy, s, ds)
         d, dev = s.shape[-1], s.device
         T = sc.numel() // d
