@@ -201,9 +201,14 @@ __device__ __forceinline__ void fb_tile_at(int lin, int m_tiles, int n_tiles, in
 // wave has the rest of its stage in registers, so that one barrier frees the buffer for
 // the loads of the stage after the next.  A workgroup walks a band of tiles as one
 // sequence of stages.
-template <int FMT, int OT, int BM, int BN, int WM, int WN>
+// Several products of one K (G of them) share the launch, one after the other in the band.
+template <int G>
+struct FbBatch {
+  FbArgs p[G];
+};
+template <int FMT, int OT, int BM, int BN, int WM, int WN, int G>
 __global__ void __launch_bounds__(WM * WN * 64, BM * BN > 128 * 128 || BN > 128 || OT == O_F32 ? 1 : 2)
-fb_product_kernel(FbArgs p, int m_tiles, int n_tiles) {
+fb_product_kernel(FbBatch<G> batch) {
   using C = FbCfg<FMT, BM, BN, WM, WN>;
   constexpr bool GATED = OT == O_GATED;
   constexpr int TT = C::TT, WT = C::WT, BNO = GATED ? BN / 2 : BN, NW = C::NW;
@@ -215,18 +220,36 @@ fb_product_kernel(FbArgs p, int m_tiles, int n_tiles) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN, g = lane >> 5, l32 = lane & 31;
   const uint32_t lds0 = lds_offset(&smem[0]);
-  const int nk = (int)(p.ldx / 128);
+  const int nk = (int)(batch.p[0].ldx / 128);
+  auto tiles = [&](int q) __attribute__((always_inline)) -> int {
+    return (int)((batch.p[q].R + BM - 1) / BM * ((batch.p[q].N + BNO - 1) / BNO));
+  };
+  // tile `at` of all: its product, and its place there
+  auto locate = [&](int at, int& mt, int& nt) __attribute__((always_inline)) -> int {
+    int q = 0;
+#pragma unroll
+    for (int j = 0; j + 1 < G; ++j)
+      if (q == j && at >= tiles(j)) {
+        at -= tiles(j);
+        q = j + 1;
+      }
+    fb_tile_at(at, (int)((batch.p[q].R + BM - 1) / BM), (int)((batch.p[q].N + BNO - 1) / BNO), mt, nt);
+    return q;
+  };
 
   // XCD x (workgroup b runs on XCD b % 8) takes a contiguous band of the tiles
   const int wgs = gridDim.x, nx = min(8, wgs), xcd = (int)blockIdx.x % nx, step = (wgs - xcd + nx - 1) / nx;
-  const int total = m_tiles * n_tiles, last = (int)((int64_t)total * (xcd + 1) / nx);
+  int total = 0;
+#pragma unroll
+  for (int j = 0; j < G; ++j) total += tiles(j);
+  const int last = (int)((int64_t)total * (xcd + 1) / nx);
   int lin = (int)((int64_t)total * xcd / nx) + (int)blockIdx.x / nx;
   if (lin >= last) return;
 
   // where a lane's loads of a tile read: 32-bit offsets from its first rows; rows past the
   // end read the last one, their sums are not stored
   const uint8_t *X, *W, *XS, *WS;  // gate's; up's stand as far from them as the matrices from each other
-  const int64_t to_w2 = GATED ? p.w2 - p.w : 0, to_s2 = GATED ? p.s2 - p.s : 0;
+  const int64_t to_w2 = GATED ? batch.p[0].w2 - batch.p[0].w : 0, to_s2 = GATED ? batch.p[0].s2 - batch.p[0].s : 0;
   uint32_t x_off[C::X_INS], w_off[C::W_INS], s_off[C::S_INS];
   // staged weight row r, from the tile's first: tiles of 32 (gate's, then up's), permuted
   auto w_row = [&](int r, int left) __attribute__((always_inline)) -> int {
@@ -234,11 +257,11 @@ fb_product_kernel(FbArgs p, int m_tiles, int n_tiles) {
     if (GATED) t = t >= BN / 64 ? t - BN / 64 : t;
     return min(t * 32 + fb_perm(r & 31), left);
   };
-  const uint32_t ld = (uint32_t)p.ldx, sl = (uint32_t)p.words * 4;
+  const uint32_t ld = (uint32_t)batch.p[0].ldx, sl = (uint32_t)batch.p[0].words * 4;
   bool offsets = true;  // are to be computed
   auto source = [&](int at) __attribute__((always_inline)) {
     int mt, nt;
-    fb_tile_at(at, m_tiles, n_tiles, mt, nt);
+    const FbArgs& p = batch.p[locate(at, mt, nt)];
     const int64_t row0 = (int64_t)mt * BM, n0 = (int64_t)nt * BNO;
     const int xleft = (int)min<int64_t>(p.R - 1 - row0, BM - 1), wleft = (int)min<int64_t>(p.N - 1 - n0, BNO - 1);
     X = p.x + row0 * ld;
@@ -278,7 +301,7 @@ fb_product_kernel(FbArgs p, int m_tiles, int n_tiles) {
       load_k = 0;
     }
     if (FMT == F_CODES && load_k % 16 == 0) {
-      const int word = min(load_k / 4 + lane % 4, p.words - 1) * 4;
+      const int word = min(load_k / 4 + lane % 4, batch.p[0].words - 1) * 4;
 #pragma unroll
       for (int i = 0; i < C::S_INS; ++i) {
         const int r = (wave * C::S_INS + i) * 16;
@@ -427,7 +450,7 @@ fb_product_kernel(FbArgs p, int m_tiles, int n_tiles) {
     for (int kt = 1; kt < nk; ++kt) stage(kt, false);
     pin(S);
     int mt, nt;
-    fb_tile_at(lin, m_tiles, n_tiles, mt, nt);
+    const FbArgs& p = batch.p[locate(lin, mt, nt)];
     const int64_t row0 = (int64_t)mt * BM, n0 = (int64_t)nt * BNO;
     const int rows = (int)min<int64_t>(BM, p.R - row0);
     int el = lane;  // the stores' addresses are not kept in registers across the loop
@@ -656,15 +679,22 @@ fb_product_kernel(FbArgs p, int m_tiles, int n_tiles) {
   wait_vm<0>();
 }
 
-template <int FMT, int OT, int BM, int BN, int WM, int WN>
-int launch_product_cfg(const FbArgs& p, hipStream_t stream) {
+template <int FMT, int OT, int BM, int BN, int WM, int WN, int G>
+int launch_product_cfg(const FbBatch<G>& b, hipStream_t stream) {
   constexpr int BNO = OT == O_GATED ? BN / 2 : BN;
-  const int64_t mt = (p.R + BM - 1) / BM, nt = (p.N + BNO - 1) / BNO;
-  if ((BM > BN ? BM : BN) * p.ldx >= 1LL << 32) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block product: rows too wide");
-  if (mt * nt > 2147483647LL || mt > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block product: too many tiles");
+  int64_t tiles = 0;
+  for (const FbArgs& p : b.p) {
+    const int64_t mt = (p.R + BM - 1) / BM, nt = (p.N + BNO - 1) / BNO;
+    if (mt > 2147483647LL || nt > 2147483647LL || mt * nt > 2147483647LL)
+      return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block product: too many tiles");
+    tiles += mt * nt;
+  }
+  if ((BM > BN ? BM : BN) * b.p[0].ldx >= 1LL << 32)
+    return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block product: rows too wide");
+  if (tiles > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block product: too many tiles");
   const int64_t wgs = cu_count() * (BM * BN <= 128 * 128 ? 2 : 1);
-  hipLaunchKernelGGL((fb_product_kernel<FMT, OT, BM, BN, WM, WN>), dim3((unsigned)(mt * nt < wgs ? mt * nt : wgs)),
-                     dim3(WM * WN * 64), 0, stream, p, (int)mt, (int)nt);
+  hipLaunchKernelGGL((fb_product_kernel<FMT, OT, BM, BN, WM, WN, G>), dim3((unsigned)(tiles < wgs ? tiles : wgs)),
+                     dim3(WM * WN * 64), 0, stream, b);
   return check_launch("fb_product_kernel");
 }
 
@@ -678,14 +708,16 @@ struct FbTile {
 constexpr FbTile ROW_TILES[] = {{256, 256, 153, 0, 490}, {128, 256, 85, 0, 300}, {128, 128, 52, 105, 160}, {64, 128, 45, 76, 100}};
 constexpr FbTile GATED_TILES[] = {{256, 256, 153, 0, 900}, {128, 256, 85, 0, 500}, {64, 256, 60, 0, 300}};
 
-template <int N>
-int pick_tile(const FbTile (&tiles)[N], const FbArgs& p, bool gated) {
-  const int64_t cus = cu_count(), nk = p.ldx / 128;
+template <int N, int G>
+int pick_tile(const FbTile (&tiles)[N], const FbBatch<G>& batch, bool gated) {
+  const int64_t cus = cu_count(), nk = batch.p[0].ldx / 128;
   int best = 0;
   double least = 0.0;
   for (int i = 0; i < N; ++i) {
     const FbTile& t = tiles[i];
-    const int64_t bn = gated ? t.bn / 2 : t.bn, n = (p.R + t.bm - 1) / t.bm * ((p.N + bn - 1) / bn);
+    const int64_t bn = gated ? t.bn / 2 : t.bn;
+    int64_t n = 0;
+    for (const FbArgs& p : batch.p) n += (p.R + t.bm - 1) / t.bm * ((p.N + bn - 1) / bn);
     const int64_t round = t.two ? 2 * cus : cus, full = n / round, left = n % round;
     const double whole = (double)(nk * (t.two ? t.two : t.one) + t.rest);
     double last = whole * (0.6 + 0.4 * (double)left / (double)round);
@@ -699,22 +731,26 @@ int pick_tile(const FbTile (&tiles)[N], const FbArgs& p, bool gated) {
   return best;
 }
 
-template <int FMT, int OT>
-int launch_product(const FbArgs& p, hipStream_t stream) {
+template <int FMT, int OT, int G>
+int launch_products(const FbBatch<G>& b, hipStream_t stream) {
   if constexpr (OT == O_GATED) {
-    switch (pick_tile(GATED_TILES, p, true)) {
-      case 0: return launch_product_cfg<FMT, OT, 256, 256, 2, 2>(p, stream);
-      case 1: return launch_product_cfg<FMT, OT, 128, 256, 2, 2>(p, stream);
-      default: return launch_product_cfg<FMT, OT, 64, 256, 1, 4>(p, stream);
+    switch (pick_tile(GATED_TILES, b, true)) {
+      case 0: return launch_product_cfg<FMT, OT, 256, 256, 2, 2>(b, stream);
+      case 1: return launch_product_cfg<FMT, OT, 128, 256, 2, 2>(b, stream);
+      default: return launch_product_cfg<FMT, OT, 64, 256, 1, 4>(b, stream);
     }
   } else {
-    switch (pick_tile(ROW_TILES, p, false)) {
-      case 0: return launch_product_cfg<FMT, OT, 256, 256, 2, 2>(p, stream);
-      case 1: return launch_product_cfg<FMT, OT, 128, 256, 2, 2>(p, stream);
-      case 2: return launch_product_cfg<FMT, OT, 128, 128, 2, 2>(p, stream);
-      default: return launch_product_cfg<FMT, OT, 64, 128, 2, 2>(p, stream);
+    switch (pick_tile(ROW_TILES, b, false)) {
+      case 0: return launch_product_cfg<FMT, OT, 256, 256, 2, 2>(b, stream);
+      case 1: return launch_product_cfg<FMT, OT, 128, 256, 2, 2>(b, stream);
+      case 2: return launch_product_cfg<FMT, OT, 128, 128, 2, 2>(b, stream);
+      default: return launch_product_cfg<FMT, OT, 64, 128, 2, 2>(b, stream);
     }
   }
+}
+template <int FMT, int OT>
+int launch_product(const FbArgs& p, hipStream_t stream) {
+  return launch_products<FMT, OT>(FbBatch<1>{{p}}, stream);
 }
 
 FbArgs codes_args(const void* x, const uint8_t* xs, const uint8_t* w, const uint8_t* s, void* y, int64_t R, int64_t K,
@@ -1386,9 +1422,9 @@ int smaul_fp8_block_ffn_backward(const void* dy, const uint8_t* gate_w, const ui
   b.t[2] = turn_rows(dy, S_BF16, T, d, dyt, q.lt, 1);
   b.t[3] = turn_codes(h_codes, h_scales, T, h, ht, q.lt);
   if (int rc = launch_turns(b, 4, stream)) return rc;
-  if (int rc = launch_product<F_BF16, O_BF16>(rows_args(dgut, xt, dgate, h, q.lt, d), stream)) return rc;
-  if (int rc = launch_product<F_BF16, O_BF16>(rows_args(dgut + q.lh * q.lt, xt, dup, h, q.lt, d), stream)) return rc;
-  return launch_product<F_BF16, O_BF16>(rows_args(dyt, ht, ddown, d, q.lt, h), stream);
+  const FbBatch<3> grads{{rows_args(dgut, xt, dgate, h, q.lt, d),
+                          rows_args(dgut + q.lh * q.lt, xt, dup, h, q.lt, d), rows_args(dyt, ht, ddown, d, q.lt, h)}};
+  return launch_products<F_BF16, O_BF16>(grads, stream);
 }
 
 }  // extern "C"
