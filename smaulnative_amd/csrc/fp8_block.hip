@@ -139,18 +139,18 @@ __device__ __forceinline__ void fb_each(F&& f) {
   fb_each(f, std::make_integer_sequence<int, N>{});
 }
 
-// K in stages of 128 (a block, 128-byte rows), codes brought to LDS by DMA, two stages;
-// scales in chunks of 16 stages.  Roles: the weight's rows are the matrix instruction's
+// K in stages of 128 (a block, 128-byte rows), codes brought to LDS by DMA, NS stages;
+// scales in chunks of 16 stages, as many.  Roles: the weight's rows are the matrix instruction's
 // rows and x's its columns, and row i of a 32 x 32 tile is given weight row 16 ((i / 4) %
 // 2) + 4 (i / 8) + i % 4, so that the 16 sums of a lane are 16 consecutive outputs of one
 // row of x.
-template <int FMT, int BM, int BN, int WM, int WN>
+template <int FMT, int BM, int BN, int WM, int WN, int NS>
 struct FbCfg {
   static constexpr int NW = WM * WN, XB = BM * 128, WB = BN * 128, STAGE = XB + WB;
   static constexpr int X_INS = XB / (1024 * NW), W_INS = WB / (1024 * NW), S_INS = (BM + BN) / (16 * NW);
   static constexpr int SC = FMT == F_CODES ? (BM + BN) * 16 : 0;  // a chunk of scales: 4 dwords a row
   static constexpr int TT = BM / WM / 32, WT = BN / WN / 32;
-  static constexpr int LDS = 2 * STAGE + 2 * SC;
+  static constexpr int LDS = NS * (STAGE + SC);
   static_assert(XB % (1024 * NW) == 0 && WB % (1024 * NW) == 0 && (BM + BN) % (16 * NW) == 0 && BN % 16 == 0,
                 "whole DMA instructions");
 };
@@ -206,14 +206,14 @@ template <int G>
 struct FbBatch {
   FbArgs p[G];
 };
-template <int FMT, int OT, int BM, int BN, int WM, int WN, int G>
-__global__ void __launch_bounds__(WM * WN * 64, BM * BN > 128 * 128 || BN > 128 || OT == O_F32 ? 1 : 2)
+template <int FMT, int OT, int BM, int BN, int WM, int WN, int NS, int G>
+__global__ void __launch_bounds__(WM * WN * 64, NS > 2 || BM * BN > 128 * 128 || BN > 128 || OT == O_F32 ? 1 : 2)
 fb_product_kernel(FbBatch<G> batch) {
-  using C = FbCfg<FMT, BM, BN, WM, WN>;
+  using C = FbCfg<FMT, BM, BN, WM, WN, NS>;
   constexpr bool GATED = OT == O_GATED;
   constexpr int TT = C::TT, WT = C::WT, BNO = GATED ? BN / 2 : BN, NW = C::NW;
   // a wave's part of LDS for the rows that leave: 2 KB where two workgroups share a CU
-  constexpr int OWN = GATED ? 0 : OT == O_BF16 && BM * BN <= 128 * 128 ? 2048 : 4096, AMAX = GATED ? BM * WN * 4 : 0;
+  constexpr int OWN = GATED ? 0 : OT == O_BF16 && NS == 2 && BM * BN <= 128 * 128 ? 2048 : 4096, AMAX = GATED ? BM * WN * 4 : 0;
   static_assert(!GATED || BNO == FB_BLOCK, "a tile of hidden rows is a block");
   __shared__ __attribute__((aligned(1024))) char smem[C::LDS + NW * OWN + AMAX];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -237,13 +237,15 @@ fb_product_kernel(FbBatch<G> batch) {
     return q;
   };
 
-  // XCD x (workgroup b runs on XCD b % 8) takes a contiguous band of the tiles
-  const int wgs = gridDim.x, nx = min(8, wgs), xcd = (int)blockIdx.x % nx, step = (wgs - xcd + nx - 1) / nx;
+  // XCD x (workgroup b runs on XCD b % 8) takes a contiguous band of the tiles, as long as
+  // its share of the workgroups
   int total = 0;
 #pragma unroll
   for (int j = 0; j < G; ++j) total += tiles(j);
-  const int last = (int)((int64_t)total * (xcd + 1) / nx);
-  int lin = (int)((int64_t)total * xcd / nx) + (int)blockIdx.x / nx;
+  const int wgs = gridDim.x, xcd = (int)blockIdx.x % 8, step = (wgs - xcd + 7) / 8;
+  const int before = xcd * (wgs / 8) + min(xcd, wgs % 8);  // workgroups of the XCDs before
+  const int last = (int)((int64_t)total * (before + step) / wgs);
+  int lin = (int)((int64_t)total * before / wgs) + (int)blockIdx.x / 8;
   if (lin >= last) return;
 
   // where a lane's loads of a tile read: 32-bit offsets from its first rows; rows past the
@@ -307,9 +309,9 @@ fb_product_kernel(FbBatch<G> batch) {
         const int r = (wave * C::S_INS + i) * 16;
         const uint8_t* from = WS + (GATED && r >= BN / 2 ? to_s2 : 0);
         if (r >= BN) from = XS;
-        dma4(from, s_off[i] + word, lds0 + 2 * C::STAGE + load_chunk * C::SC + (wave * C::S_INS + i) * 256);
+        dma4(from, s_off[i] + word, lds0 + NS * C::STAGE + load_chunk * C::SC + (wave * C::S_INS + i) * 256);
       }
-      load_chunk ^= 1;
+      load_chunk = load_chunk + 1 == NS ? 0 : load_chunk + 1;
     }
   };
   auto load_one = [&](int buf, int q) __attribute__((always_inline)) {
@@ -323,13 +325,14 @@ fb_product_kernel(FbBatch<G> batch) {
     }
   };
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
+  for (int b = 0; b < NS; ++b) {
     load_begin();
 #pragma unroll
     for (int q = 0; q < INS; ++q) load_one(b, q);
     ++load_k;
   }
-  wait_vm<INS>();
+  // (a chunk of scales stands before its stage's codes)
+  wait_vm<INS * (NS - 1)>();
   __syncthreads();
 
   // staged row of weight tile j of this wave: its gate tiles, then its up tiles
@@ -354,7 +357,7 @@ fb_product_kernel(FbBatch<G> batch) {
   };
   // four stages' scales of this lane's rows, from the chunk
   auto read_scales = [&](int chunk, int word) __attribute__((always_inline)) {
-    const char* at = smem + 2 * C::STAGE + chunk * C::SC + l32 * 16 + word * 4;
+    const char* at = smem + NS * C::STAGE + chunk * C::SC + l32 * 16 + word * 4;
 #pragma unroll
     for (int j = 0; j < WT; ++j) nw[j] = *(const uint32_t*)(at + w_tile(j) * 16);
 #pragma unroll
@@ -392,20 +395,23 @@ fb_product_kernel(FbBatch<G> batch) {
   int buf = 0, chunk = 0;
   // One stage: 2 S products, the rest issued in their shadow.  The second step's operands
   // are read first; from product B1 on no wave reads this buffer any more, and the loads of
-  // the stage after the next follow, spread out so that they do not queue; from product B2
-  // on the next stage's first operands are read, behind a wait that leaves the loads issued
-  // in this stage (DONE of them by then) in flight.
+  // the stage that takes its place follow, spread out so that they do not queue; from product
+  // B2 on the next stage's first operands are read, behind a wait that leaves the loads of
+  // later stages (of this stage's DONE by then) in flight.
   constexpr int B1 = S * 5 / 8, B2 = S + S * 5 / 16, SPAN = 2 * S - 2 - B1;
   constexpr int STORED = GATED ? TT * WT / 2 : TT * WT * (OT == O_BF16 ? 2 : 4);  // instructions of a whole tile
   int stored = 0;
   constexpr int DONE = ((B2 - 1 - B1) * INS + SPAN - 1) / SPAN;  // of products B1 to B2 - 2
+  constexpr int FLIGHT = DONE + (NS - 2) * INS;  // loads behind those of the next stage
+  static_assert(FLIGHT < 64, "vmcnt range");
   auto stage = [&](int kt, bool fresh) __attribute__((always_inline)) {
     const int sh = kt % 4 * 8, next = kt + 1 == nk ? 0 : kt + 1;
 #pragma unroll
     for (int j = 0; j < WT && FMT == F_CODES; ++j) sw[j] = nw[j] >> sh;
 #pragma unroll
     for (int i = 0; i < TT && FMT == F_CODES; ++i) sx[i] = nx_[i] >> sh;
-    if (next % 16 == 0) chunk ^= 1;
+    if (next % 16 == 0) chunk = chunk + 1 == NS ? 0 : chunk + 1;
+    const int after = buf + 1 == NS ? 0 : buf + 1;
     fb_each<2 * S>([&](auto number) __attribute__((always_inline)) {
       constexpr int s = number;
       if constexpr (s == B1) {
@@ -420,8 +426,8 @@ fb_product_kernel(FbBatch<G> batch) {
         __builtin_amdgcn_sched_barrier(0);
         // memory operations are done in order: behind a tile's stores, of which `stored` at
         // least were issued, the loads before them are waited for alone
-        if (fresh && stored) wait_vm<(DONE + STORED < 63 ? DONE + STORED : 63)>();
-        else wait_vm<DONE>();
+        if (fresh && stored) wait_vm<(FLIGHT + STORED < 63 ? FLIGHT + STORED : 63)>();
+        else wait_vm<FLIGHT>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
@@ -430,7 +436,7 @@ fb_product_kernel(FbBatch<G> batch) {
       fb_each<READS>([&](auto part) __attribute__((always_inline)) {
         constexpr int q = part;
         if constexpr (q * (S / 2) / READS == s) read_one(buf, 1, q);
-        if constexpr (B2 + q * (2 * S - B2) / READS == s) read_one(buf ^ 1, 0, q);  // behind the last tile: unused
+        if constexpr (B2 + q * (2 * S - B2) / READS == s) read_one(after, 0, q);  // behind the last tile: unused
       });
       fb_each<INS>([&](auto part) __attribute__((always_inline)) {
         constexpr int q = part;
@@ -439,7 +445,7 @@ fb_product_kernel(FbBatch<G> batch) {
       __builtin_amdgcn_sched_barrier(0);
     });
     ++load_k;
-    buf ^= 1;
+    buf = after;
   };
 
 #pragma unroll
@@ -679,7 +685,7 @@ fb_product_kernel(FbBatch<G> batch) {
   wait_vm<0>();
 }
 
-template <int FMT, int OT, int BM, int BN, int WM, int WN, int G>
+template <int FMT, int OT, int BM, int BN, int WM, int WN, int NS, int G>
 int launch_product_cfg(const FbBatch<G>& b, hipStream_t stream) {
   constexpr int BNO = OT == O_GATED ? BN / 2 : BN;
   int64_t tiles = 0;
@@ -692,8 +698,8 @@ int launch_product_cfg(const FbBatch<G>& b, hipStream_t stream) {
   if ((BM > BN ? BM : BN) * b.p[0].ldx >= 1LL << 32)
     return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block product: rows too wide");
   if (tiles > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block product: too many tiles");
-  const int64_t wgs = cu_count() * (BM * BN <= 128 * 128 ? 2 : 1);
-  hipLaunchKernelGGL((fb_product_kernel<FMT, OT, BM, BN, WM, WN, G>), dim3((unsigned)(tiles < wgs ? tiles : wgs)),
+  const int64_t wgs = cu_count() * (NS == 2 && BM * BN <= 128 * 128 ? 2 : 1);
+  hipLaunchKernelGGL((fb_product_kernel<FMT, OT, BM, BN, WM, WN, NS, G>), dim3((unsigned)(tiles < wgs ? tiles : wgs)),
                      dim3(WM * WN * 64), 0, stream, b);
   return check_launch("fb_product_kernel");
 }
@@ -705,7 +711,7 @@ int launch_product_cfg(const FbBatch<G>& b, hipStream_t stream) {
 struct FbTile {
   int bm, bn, one, two, rest;  // two: 0 where a CU takes them one by one
 };
-constexpr FbTile ROW_TILES[] = {{256, 256, 153, 0, 490}, {128, 256, 85, 0, 300}, {128, 128, 52, 105, 160}, {64, 128, 45, 76, 100}};
+constexpr FbTile ROW_TILES[] = {{256, 256, 153, 0, 490}, {128, 256, 85, 0, 300}, {128, 128, 52, 105, 160}, {64, 128, 37, 0, 150}};
 constexpr FbTile GATED_TILES[] = {{256, 256, 153, 0, 900}, {128, 256, 85, 0, 500}, {64, 256, 60, 0, 300}};
 
 template <int N, int G>
@@ -735,16 +741,16 @@ template <int FMT, int OT, int G>
 int launch_products(const FbBatch<G>& b, hipStream_t stream) {
   if constexpr (OT == O_GATED) {
     switch (pick_tile(GATED_TILES, b, true)) {
-      case 0: return launch_product_cfg<FMT, OT, 256, 256, 2, 2>(b, stream);
-      case 1: return launch_product_cfg<FMT, OT, 128, 256, 2, 2>(b, stream);
-      default: return launch_product_cfg<FMT, OT, 64, 256, 1, 4>(b, stream);
+      case 0: return launch_product_cfg<FMT, OT, 256, 256, 2, 2, 2>(b, stream);
+      case 1: return launch_product_cfg<FMT, OT, 128, 256, 2, 2, 2>(b, stream);
+      default: return launch_product_cfg<FMT, OT, 64, 256, 1, 4, 3>(b, stream);
     }
   } else {
     switch (pick_tile(ROW_TILES, b, false)) {
-      case 0: return launch_product_cfg<FMT, OT, 256, 256, 2, 2>(b, stream);
-      case 1: return launch_product_cfg<FMT, OT, 128, 256, 2, 2>(b, stream);
-      case 2: return launch_product_cfg<FMT, OT, 128, 128, 2, 2>(b, stream);
-      default: return launch_product_cfg<FMT, OT, 64, 128, 2, 2>(b, stream);
+      case 0: return launch_product_cfg<FMT, OT, 256, 256, 2, 2, 2>(b, stream);
+      case 1: return launch_product_cfg<FMT, OT, 128, 256, 2, 2, 2>(b, stream);
+      case 2: return launch_product_cfg<FMT, OT, 128, 128, 2, 2, 2>(b, stream);
+      default: return launch_product_cfg<FMT, OT, 64, 128, 2, 2, 4>(b, stream);
     }
   }
 }
