@@ -84,11 +84,19 @@ struct FbArgs {
   int words;
 };
 
-// The kept factors a = u silu'(g) and b = silu(g), 24 bits each: a record of 96 bytes for
-// 16 consecutive hidden values of a row: a's high halves, b's, a's third bytes, b's.
-// (bf16 alone would add its rounding twice to the gradients'.)
-constexpr int FB_RECORD = 96;
-__host__ __device__ __forceinline__ int64_t fb_kept_row(int64_t h) { return fb_width(h) / 16 * FB_RECORD; }
+// The kept factors a = u silu'(g) and b = silu(g), 24 bits each (bf16 alone would add its
+// rounding twice to the gradients').  Both passes have them in tiles of 32 rows by 32
+// columns, 16 consecutive columns of row i in lane i or i + 32, so that is how they lie: a
+// tile is 6 pieces of 16 bytes a lane (a's high halves, b's, a's third bytes, b's), each
+// piece a whole KB of the 64 lanes.
+constexpr int FB_KEPT = 6 * 1024;
+__host__ __device__ __forceinline__ int64_t fb_kept_size(int64_t T, int64_t h) {
+  return (T + 31) / 32 * (fb_width(h) / 32) * FB_KEPT;
+}
+// piece 0 of row `row`, columns n to n + 15, of h hidden columns
+__device__ __forceinline__ int64_t fb_kept_at(int64_t row, int64_t n, int64_t h) {
+  return (row / 32 * (fb_width(h) / 32) + n / 32) * FB_KEPT + (row % 32 + n / 16 % 2 * 32) * 16;
+}
 
 // a float's bits, its third byte to nearest
 __device__ __forceinline__ uint32_t fb_bits24(float v) {
@@ -488,15 +496,15 @@ fb_product_kernel(FbBatch<G> batch) {
           fb_pin(acc[j][i]);
           if (p.kept && lr < rows) {
             uint4 hi[2], lo;
-            char* rec = (char*)p.kept + (row0 + lr) * fb_kept_row(p.N) + n / 16 * FB_RECORD;
+            uint4* to = (uint4*)(p.kept + fb_kept_at(row0 + lr, n, p.N));  // pieces are 64 of these apart
             fb_pack24(a, hi, lo);
-            ((uint4*)rec)[0] = hi[0];
-            ((uint4*)rec)[1] = hi[1];
-            ((uint4*)rec)[4] = lo;
+            to[0] = hi[0];
+            to[64] = hi[1];
+            to[256] = lo;
             fb_pack24(b, hi, lo);
-            ((uint4*)rec)[2] = hi[0];
-            ((uint4*)rec)[3] = hi[1];
-            ((uint4*)rec)[5] = lo;
+            to[128] = hi[0];
+            to[192] = hi[1];
+            to[320] = lo;
           }
         }
         m = __builtin_elementwise_maximum(m, __shfl_xor(m, 32, 64));
@@ -537,27 +545,31 @@ fb_product_kernel(FbBatch<G> batch) {
       if constexpr (WN > 1) __syncthreads();  // the maxima's LDS is free for the next tile
       stored = rows == BM ? STORED : 0;
     } else if constexpr (OT == O_DGATED) {
-      // 64-byte pieces of dg and of du, each through 2 KB of LDS of the wave's own; the next
-      // 16 values' factors are on their way while these are multiplied
+      // 64-byte pieces of dg and of du, each through 2 KB of LDS of the wave's own; the factors
+      // of the next AHEAD units of 16 values are on their way while these are multiplied (8192
+      // tokens, 1024 by 2560, one unit ahead 100 us)
+      constexpr int AHEAD = TT * WT > 8 ? 2 : 3, UNITS = TT * WT;
       char* own = smem + C::LDS + wave * OWN;
       auto place = [&](int m, int r, int c) __attribute__((always_inline)) -> char* {
         return own + m * 2048 + r * 64 + (c ^ (r / 2 & 3)) * 16;
       };
       const int left = rows - wm * (BM / WM);
-      const int64_t nrec = fb_width(p.N) / 16, w0 = n0 + wn * (BN / WN), r0 = row0 + wm * (BM / WM);
-      uint4 rec[6];
-      auto factors = [&](int u) __attribute__((always_inline)) {
-        const int r = min(u / WT * 32 + e32, left - 1);
-        const int64_t c = min<int64_t>((w0 + u % WT * 32) / 16 + eg, nrec - 1);
-        const uint4* at = (const uint4*)(p.kept + ((r0 + (r < 0 ? 0 : r)) * nrec + c) * FB_RECORD);
-        rec[0] = at[0]; rec[1] = at[1]; rec[2] = at[2]; rec[3] = at[3]; rec[4] = at[4]; rec[5] = at[5];
+      const int64_t w0 = n0 + wn * (BN / WN), r0 = row0 + wm * (BM / WM);
+      const int64_t last_row = (p.R - 1) / 32 * 32, last_col = fb_width(p.N) - 32;  // tiles there are
+      uint4 rec[AHEAD + 1][6];
+      auto factors = [&](int u, uint4 (&to)[6]) __attribute__((always_inline)) {
+        const uint4* at = (const uint4*)(p.kept + fb_kept_at(min(r0 + u / WT * 32, last_row), min(w0 + u % WT * 32, last_col),
+                                                             p.N)) + el;
+        to[0] = at[0]; to[1] = at[64]; to[2] = at[128]; to[3] = at[192]; to[4] = at[256]; to[5] = at[320];
       };
       if (left > 0) {
-        factors(0);
-        fb_each<TT * WT>([&](auto unit) __attribute__((always_inline)) {
-          constexpr int u = unit, i = u / WT, j = u % WT;
-          const uint4 ah[2] = {rec[0], rec[1]}, bh[2] = {rec[2], rec[3]}, al = rec[4], bl = rec[5];
-          if constexpr (u + 1 < TT * WT) factors(u + 1);
+        fb_each<(AHEAD < UNITS ? AHEAD : UNITS)>([&](auto unit) __attribute__((always_inline)) {
+          factors(unit, rec[unit]);
+        });
+        fb_each<UNITS>([&](auto unit) __attribute__((always_inline)) {
+          constexpr int u = unit, i = u / WT, j = u % WT, at = u % (AHEAD + 1);
+          if constexpr (u + AHEAD < UNITS) factors(u + AHEAD, rec[(u + AHEAD) % (AHEAD + 1)]);
+          const uint4 ah[2] = {rec[at][0], rec[at][1]}, bh[2] = {rec[at][2], rec[at][3]}, al = rec[at][4], bl = rec[at][5];
           float a[16], b[16];
           fb_unpack24(ah, al, a);
           fb_unpack24(bh, bl, b);
@@ -712,6 +724,7 @@ struct FbTile {
   int bm, bn, one, two, rest;  // two: 0 where a CU takes them one by one
 };
 constexpr FbTile ROW_TILES[] = {{256, 256, 153, 0, 490}, {128, 256, 85, 0, 300}, {128, 128, 52, 105, 160}, {64, 128, 37, 0, 150}};
+constexpr FbTile DGATED_TILES[] = {{256, 256, 153, 0, 1400}, {128, 256, 85, 0, 800}, {128, 128, 52, 105, 500}, {64, 128, 37, 0, 300}};
 constexpr FbTile GATED_TILES[] = {{256, 256, 153, 0, 900}, {128, 256, 85, 0, 500}, {64, 256, 60, 0, 300}};
 
 template <int N, int G>
@@ -746,7 +759,7 @@ int launch_products(const FbBatch<G>& b, hipStream_t stream) {
       default: return launch_product_cfg<FMT, OT, 64, 256, 1, 4, 3>(b, stream);
     }
   } else {
-    switch (pick_tile(ROW_TILES, b, false)) {
+    switch (OT == O_DGATED ? pick_tile(DGATED_TILES, b, false) : pick_tile(ROW_TILES, b, false)) {
       case 0: return launch_product_cfg<FMT, OT, 256, 256, 2, 2, 2>(b, stream);
       case 1: return launch_product_cfg<FMT, OT, 128, 256, 2, 2, 2>(b, stream);
       case 2: return launch_product_cfg<FMT, OT, 128, 128, 2, 2, 2>(b, stream);
@@ -935,15 +948,15 @@ __global__ void __launch_bounds__(512) fb_stream_kernel(FbArgs p, int64_t K) {
       if (n + q < p.N) ((float*)p.y)[row * p.N + n + q] = v[q];
     }
     if (p.kept) {
-      uint8_t* rec = p.kept + row * fb_kept_row(p.N) + (int64_t)blockIdx.x * FB_RECORD;
+      uint8_t* to = p.kept + fb_kept_at(row, n0, p.N);
       uint2 hi2;
       uint32_t lo2;
       fb_pack24(a, hi2, lo2);
-      *(uint2*)(rec + i * 8) = hi2;
-      *(uint32_t*)(rec + 64 + i * 4) = lo2;
+      *(uint2*)(to + i / 2 * 1024 + i % 2 * 8) = hi2;
+      *(uint32_t*)(to + 4096 + i * 4) = lo2;
       fb_pack24(b, hi2, lo2);
-      *(uint2*)(rec + 32 + i * 8) = hi2;
-      *(uint32_t*)(rec + 80 + i * 4) = lo2;
+      *(uint2*)(to + 2048 + i / 2 * 1024 + i % 2 * 8) = hi2;
+      *(uint32_t*)(to + 5120 + i * 4) = lo2;
     }
   } else {
     for (int e = tid; e < RT * 256; e += 512) {
@@ -1302,7 +1315,7 @@ int smaul_fp8_block_backward_input(const void* g, int dtype, const uint8_t* w, c
 
 int64_t smaul_fp8_block_ffn_saved_size(int64_t T, int64_t h) {
   if (T < 0 || h <= 0) return -1;
-  return T * fb_kept_row(h);
+  return fb_kept_size(T, h);
 }
 
 int64_t smaul_fp8_block_ffn_workspace_size(int64_t T, int64_t d, int64_t h, int x_dtype, int save) {

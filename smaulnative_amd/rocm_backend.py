@@ -1172,19 +1172,17 @@ class RocmBackend:
         first = rows[0]
         if first.dtype not in _ACT or first.dim() < 1 or first.shape[-1] < 1:
             raise RuntimeError(f"{name}: float32 or bfloat16 rows expected, got {first.dtype} {tuple(first.shape)}")
-        for t in rows:
-            if t is not None and (t.dtype != first.dtype or t.shape != first.shape):
+        for t in rows[1:]:
+            if t is not None and (t.dtype is not first.dtype or t.shape != first.shape):
                 raise RuntimeError(f"{name}: rows of one type and shape expected, got {first.dtype} "
                                    f"{tuple(first.shape)} and {t.dtype} {tuple(t.shape)}")
         if not math.isfinite(eps) or eps <= 0:
             raise ValueError(f"RMSNorm eps must be positive finite, got {eps!r}")
         if weight is not None:
-            d = first.shape[-1]
-            if weight.numel() != d:
-                raise RuntimeError(f"{name}: weight must have {d} elements, got {weight.numel()}")
-            weight = weight.detach().reshape(d)
-            if weight.dtype != torch.float32 or not weight.is_contiguous():
-                weight = weight.float().contiguous()
+            if weight.numel() != first.shape[-1]:
+                raise RuntimeError(f"{name}: weight must have {first.shape[-1]} elements, got {weight.numel()}")
+            if weight.dtype is not torch.float32 or not weight.is_contiguous():
+                weight = weight.detach().float().contiguous()
         return weight, [t if t is None or t.is_contiguous() else t.contiguous() for t in rows]
 
     def add_rms_norm(self, x, residual=None, weight=None, eps=1e-6, quantize=False):
@@ -1198,11 +1196,11 @@ class RocmBackend:
         _need_one_device("add_rms_norm", x, residual, weight)
         w, (xc, rc_) = self._norm_check("add_rms_norm", eps, weight, x, residual)
         d, dev = x.shape[-1], x.device
-        s = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+        s = x if residual is None else torch.empty_like(xc)
         if quantize:
-            n = (d + 127) // 128
-            y = torch.empty(*x.shape[:-1], n * 128, dtype=torch.uint8, device=dev)
-            scales = torch.empty(*x.shape[:-1], (n + 3) // 4 * 4, dtype=torch.uint8, device=dev)
+            n, lead = (d + 127) // 128, x.shape[:-1]
+            y = torch.empty((*lead, n * 128), dtype=torch.uint8, device=dev)
+            scales = torch.empty((*lead, (n + 3) // 4 * 4), dtype=torch.uint8, device=dev)
         else:
             y, scales = torch.empty(x.shape, dtype=x.dtype, device=dev), None
         with _device(dev):
