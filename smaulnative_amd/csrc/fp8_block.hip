@@ -1020,47 +1020,38 @@ struct FbTurns {
 };
 __host__ __device__ __forceinline__ int64_t fb_stages(int64_t K) { return (K + 63) / 64; }
 
-// a workgroup: 64 by 64 values, 16 of a row a thread, through LDS
-__global__ void __launch_bounds__(256) fb_turn_kernel(FbTurns a) {
-  constexpr int LD = 72;  // 16-byte rows off the banks' period
-  __shared__ __attribute__((aligned(16))) uint16_t sh[64 * LD];
-  int64_t b = blockIdx.x;
-  int k = 0;
-#pragma unroll
-  for (int j = 0; j + 1 < FB_TURNS; ++j)
-    if (k == j && b >= a.t[j].blocks) {
-      b -= a.t[j].blocks;
-      k = j + 1;
-    }
-  const FbTurn& t = a.t[k];
-  const int64_t across = fb_stages(t.C), r0 = b / across * 64, c0 = b % across * 64;
+// a workgroup: 64 by 64 values, 16 of a row a thread, through LDS where they are turned
+template <int FMT, bool TURNED>
+__device__ __forceinline__ void fb_turn(const FbTurn& t, int64_t b, uint16_t* sh) {
+  constexpr int LD = 72, PLANES = FMT == S_F32 ? 3 : 1;  // 16-byte rows off the banks' period
+  const uint32_t across = (uint32_t)fb_stages(t.C), rb = (uint32_t)b / across;  // both from one 32-bit grid
+  const int64_t r0 = (int64_t)rb * 64, c0 = (b - (int64_t)rb * across) * 64;
   const int tid = threadIdx.x, lr = tid >> 2, lc = (tid & 3) * 16;
   const int64_t r = r0 + lr, c = c0 + lc;
   float v[16];
-  const bool in = r < t.R && c < t.C;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float* o = v + 8 * h;
-    float u[8];
+  for (int q = 0; q < 16; ++q) v[q] = 0.0f;
+  if (r < t.R && c < t.C) {
+    if constexpr (FMT == S_CODES) {  // rows end with zero codes
+      const uint4 w = *(const uint4*)((const uint8_t*)t.src + r * t.lds + c);
+      const float s = fb_scale(t.scales[r * ((t.lds / FB_BLOCK + 3) / 4 * 4) + c / FB_BLOCK]);
+      fb_decode4(w.x, s, v);
+      fb_decode4(w.y, s, v + 4);
+      fb_decode4(w.z, s, v + 8);
+      fb_decode4(w.w, s, v + 12);
+    } else {
+      float lo[8], hi[8];
+      fb_load8<FMT == S_BF16>(t.src, r, t.C, c, lo);
+      fb_load8<FMT == S_BF16>(t.src, r, t.C, c + 8, hi);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) u[q] = 0.0f;
-    if (in && c + 8 * h < t.C) {
-      if (t.fmt == S_CODES) {
-        const uint2 w = *(const uint2*)((const uint8_t*)t.src + r * t.lds + c + 8 * h);
-        const float s = fb_scale(t.scales[r * ((t.lds / FB_BLOCK + 3) / 4 * 4) + c / FB_BLOCK]);
-        fb_decode4(w.x, s, u);
-        fb_decode4(w.y, s, u + 4);
-      } else if (t.fmt == S_BF16) {
-        fb_load8<true>(t.src, r, t.C, c + 8 * h, u);
-      } else {
-        fb_load8<false>(t.src, r, t.C, c + 8 * h, u);
+      for (int q = 0; q < 8; ++q) {
+        v[q] = lo[q];
+        v[q + 8] = hi[q];
       }
     }
-#pragma unroll
-    for (int q = 0; q < 8; ++q) o[q] = c + 8 * h + q < t.C ? u[q] : 0.0f;
   }
-  const int planes = t.fmt == S_F32 ? 3 : 1;
-  for (int p = 0; p < planes; ++p) {
+#pragma unroll
+  for (int p = 0; p < PLANES; ++p) {
     uint32_t w[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
@@ -1068,7 +1059,7 @@ __global__ void __launch_bounds__(256) fb_turn_kernel(FbTurns a) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float& f = v[2 * q + e];
-        if (t.fmt == S_F32) {  // the next 8 significant bits; an infinity or NaN is in the first plane alone
+        if constexpr (FMT == S_F32) {  // the next 8 significant bits; an infinity or NaN is in the first plane alone
           const float x = __builtin_canonicalizef(f);
           const uint32_t top = __float_as_uint(x) & 0xffff0000u;
           const float rest = x - __uint_as_float(top);
@@ -1080,24 +1071,44 @@ __global__ void __launch_bounds__(256) fb_turn_kernel(FbTurns a) {
       }
       w[q] = part[0] | part[1] << 16;
     }
-    if (t.turned) {
+    if constexpr (TURNED) {
 #pragma unroll
       for (int q = 0; q < 16; ++q) sh[(lc + q) * LD + lr] = (uint16_t)(w[q / 2] >> (16 * (q & 1)));
     } else if (r < t.R) {
-      uint4* o = (uint4*)(t.dst + r * t.ld + c0 * planes + p * 64 + lc);
+      uint4* o = (uint4*)(t.dst + r * t.ld + c0 * PLANES + p * 64 + lc);
       o[0] = make_uint4(w[0], w[1], w[2], w[3]);
       o[1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
   }
-  if (!t.turned) return;  // the whole workgroup
-  __syncthreads();
+  if constexpr (TURNED) {
+    __syncthreads();
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int at = tid + q * 256, i = at >> 3, j = (at & 7) * 8;
-    if (c0 + i < t.C)
-      for (int e = 0; e < t.copies; ++e)
-        *(uint4*)(t.dst + (c0 + i) * t.ld + r0 * t.copies + e * 64 + j) = *(const uint4*)&sh[i * LD + j];
+    for (int q = 0; q < 2; ++q) {
+      const int at = tid + q * 256, i = at >> 3, j = (at & 7) * 8;
+      if (c0 + i < t.C) {
+        const uint4 d = *(const uint4*)&sh[i * LD + j];
+        uint16_t* o = t.dst + (c0 + i) * t.ld + r0 * t.copies + j;
+        for (int e = 0; e < t.copies; ++e) *(uint4*)(o + e * 64) = d;
+      }
+    }
   }
+}
+
+__global__ void __launch_bounds__(256) fb_turn_kernel(FbTurns a) {
+  __shared__ __attribute__((aligned(16))) uint16_t sh[64 * 72];
+  int64_t b = blockIdx.x;
+  int k = 0;
+#pragma unroll
+  for (int j = 0; j + 1 < FB_TURNS; ++j)
+    if (k == j && b >= a.t[j].blocks) {
+      b -= a.t[j].blocks;
+      k = j + 1;
+    }
+  const FbTurn& t = a.t[k];
+  if (t.fmt == S_CODES) fb_turn<S_CODES, true>(t, b, sh);
+  else if (t.fmt == S_F32) fb_turn<S_F32, false>(t, b, sh);
+  else if (t.turned) fb_turn<S_BF16, true>(t, b, sh);
+  else fb_turn<S_BF16, false>(t, b, sh);
 }
 
 __global__ void __launch_bounds__(256) fb_clear_kernel(uint16_t* p, int64_t n) {
