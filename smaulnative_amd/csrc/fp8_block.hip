@@ -976,6 +976,137 @@ __global__ void __launch_bounds__(512) fb_stream_kernel(FbArgs p, int64_t K) {
   }
 }
 
+// v = a + b + c, each the next 8 significant bits: exact in bf16, and all 24 of fp32.  An
+// infinity or NaN is a alone.
+__device__ __forceinline__ void fb_split3(float (&v)[8], bf16x8_t (&t)[3]) {
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    uint32_t w[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t part[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float x = __builtin_canonicalizef(v[2 * q + e]);
+        part[e] = __float_as_uint(x) >> 16;
+        const float rest = x - __uint_as_float(part[e] << 16);
+        v[2 * q + e] = rest == rest ? rest : 0.0f;
+      }
+      w[q] = part[0] | part[1] << 16;
+    }
+    t[k] = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+  }
+}
+
+// The input gradient of few rows, in one launch: a workgroup has 32 columns, its 8 waves a
+// slice of the weight's rows each.  A lane reads 32 codes of one row, and the wave turns 64
+// such rows round through LDS of its own, decoded to bf16.  The four workgroups that share
+// a line of codes are neighbours in one XCD's band.  (1 row 2560 -> 1024: 21 us by way of
+// the turned weight.)
+template <bool BF16, int RT>
+__global__ void __launch_bounds__(512)
+fb_dx_stream_kernel(const void* __restrict__ grad, const uint8_t* __restrict__ w, const uint8_t* __restrict__ s,
+                    void* __restrict__ dx, int R, int64_t I, int64_t O) {
+  constexpr int NW = 8, LD = 72, OWN = RT * 4096 > 32 * LD * 2 ? RT * 4096 : 32 * LD * 2, NT = BF16 ? 1 : 3;
+  __shared__ __attribute__((aligned(16))) char smem[NW * OWN];
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int64_t b0 = blockIdx.x;
+  {
+    const int64_t full = (int64_t)gridDim.x / 8 * 8;
+    if (b0 < full) b0 = b0 % 8 * (full / 8) + b0 / 8;
+  }
+  const int64_t k0 = b0 * 32, nb = fb_blocks(I), ns = (nb + 3) / 4 * 4;
+  const int64_t steps = (O + 63) / 64, per = (steps + NW - 1) / NW;
+  const int64_t lo = min((int64_t)wave * per, steps), hi = min(lo + per, steps);
+  uint16_t* own = (uint16_t*)(smem + wave * OWN);
+  f32x16_t acc[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[t][r] = 0.0f;
+  uint4 c0, c1;
+  float sc;
+  auto codes = [&](int64_t step) {  // rows past the last: zeros
+    const int64_t o = step * 64 + lane;
+    c0 = c1 = make_uint4(0, 0, 0, 0);
+    sc = 1.0f;
+    if (o < O) {
+      const uint4* at = (const uint4*)(w + o * nb * FB_BLOCK + k0);
+      c0 = at[0];
+      c1 = at[1];
+      sc = fb_scale(s[o * ns + k0 / FB_BLOCK]);
+    }
+  };
+  if (lo < hi) codes(lo);
+  for (int64_t step = lo; step < hi; ++step) {
+    float v[RT][4][8];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) fb_load8<BF16>(grad, min(t * 32 + l32, R - 1), O, step * 64 + q * 16 + g * 8, v[t][q]);
+    const uint32_t c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float f[4];
+      fb_decode4(c[j], sc, f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) own[(4 * j + e) * LD + lane] = (uint16_t)(__float_as_uint(f[e]) >> 16);
+    }
+    if (step + 1 < hi) codes(step + 1);
+    __builtin_amdgcn_wave_barrier();  // a wave's LDS accesses are done in order
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const bf16x8_t a = *(const bf16x8_t*)&own[fb_perm(l32) * LD + q * 16 + g * 8];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        bf16x8_t x[3];
+        if constexpr (BF16) {
+          const float* f = v[t][q];
+          x[0] = __builtin_bit_cast(bf16x8_t, make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]),
+                                                         pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])));
+        } else {
+          fb_split3(v[t][q], x);
+        }
+#pragma unroll
+        for (int k = 0; k < NT; ++k) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, x[k], acc[t], 0, 0, 0);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  float4* red = (float4*)smem;
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      red[((wave * RT + t) * 4 + i) * 64 + lane] =
+          make_float4(acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]);
+  __syncthreads();
+  for (int e = tid; e < RT * 256; e += 512) {
+    const int l = e & 63, i = e >> 6 & 3, t = e >> 8;
+    float4 a = red[(t * 4 + i) * 64 + l];
+#pragma unroll
+    for (int q = 1; q < NW; ++q) {
+      const float4 b = red[((q * RT + t) * 4 + i) * 64 + l];
+      a.x += b.x;
+      a.y += b.y;
+      a.z += b.z;
+      a.w += b.w;
+    }
+    const int64_t row = t * 32 + (l & 31), n = k0 + (l >> 5) * 16 + i * 4;
+    const float f[4] = {a.x, a.y, a.z, a.w};
+    if (row < R) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (n + q < I) {
+          if constexpr (BF16) ((__bf16*)dx)[row * I + n + q] = (__bf16)f[q];
+          else ((float*)dx)[row * I + n + q] = f[q];
+        }
+    }
+  }
+}
+
 template <int XT, int OT>
 int launch_stream_of(const FbArgs& p, int64_t K, hipStream_t stream) {
   const int64_t blocks = OT == O_GATED ? (p.N + 15) / 16 : (p.N + 31) / 32;
@@ -1203,6 +1334,7 @@ DxParts dx_parts(int64_t rows, int64_t in_f, int64_t out_f, int dtype) {
   DxParts q{};
   Parts w;
   const bool f32 = dtype == SMAUL_DTYPE_F32;
+  if (rows <= FB_FEW) return q;
   q.copies = f32 ? 3 : 1;
   q.ld = fb_stages(out_f) * 64 * q.copies;
   q.g = w.take(f32 || out_f % 64 ? rows * q.ld * 2 : 0);
@@ -1311,6 +1443,14 @@ int smaul_fp8_block_backward_input(const void* g, int dtype, const uint8_t* w, c
   const DxParts q = dx_parts(rows, in_f, out_f, dtype);
   char* ws = (char*)workspace;
   const bool bf16 = dtype == SMAUL_DTYPE_BF16;
+  if (rows <= FB_FEW) {
+    const int64_t blocks = (in_f + 31) / 32;
+    if (!grid_fits(blocks, 512)) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block_backward_input: too wide a weight");
+    auto* kernel = bf16 ? (rows <= 32 ? &fb_dx_stream_kernel<true, 1> : &fb_dx_stream_kernel<true, 2>)
+                        : (rows <= 32 ? &fb_dx_stream_kernel<false, 1> : &fb_dx_stream_kernel<false, 2>);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(512), 0, stream, g, w, s, dx, (int)rows, in_f, out_f);
+    return check_launch("fb_dx_stream_kernel");
+  }
   uint16_t* wt = (uint16_t*)(ws + q.wt);
   FbTurns a{};
   int n = 0;
