@@ -66,8 +66,9 @@ fb_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restric
 // Both sides' rows: codes with their scales, or bf16 (a row's bytes a multiple of 128).
 enum { F_CODES = 0, F_BF16 = 1 };
 // What a tile's sums become: bf16 or fp32 rows, the gated block's hidden rows as codes, or
-// (sums dh) its dg and du by the factors that the forward pass kept.
-enum { O_BF16 = 0, O_F32 = 1, O_GATED = 2, O_DGATED = 3 };
+// (sums dh) its dg and du by the factors that the forward pass kept, or a part of them
+// (fp32, one of several slices of K).
+enum { O_BF16 = 0, O_F32 = 1, O_GATED = 2, O_DGATED = 3, O_PART = 4 };
 
 struct FbArgs {
   const uint8_t* x;   // R rows of ldx bytes
@@ -81,6 +82,7 @@ struct FbArgs {
   uint8_t* kept;      // O_GATED: what the gradients take, or null; O_DGATED: that
   int64_t R, N, ldx;  // ldx: of x and w, a multiple of 128
   int64_t ldh;        // O_DGATED: N to whole stages, zeros from N on
+  int splits, per;    // slices of K, each of `per` stages and a y of its own (0: one)
   int words;
 };
 
@@ -228,13 +230,18 @@ fb_product_kernel(FbBatch<G> batch) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN, g = lane >> 5, l32 = lane & 31;
   const uint32_t lds0 = lds_offset(&smem[0]);
-  const int nk = (int)(batch.p[0].ldx / 128);
+  // slices of K: only where every workgroup has one tile
+  constexpr bool SPLITS = NS == 4 && G == 1 && (OT == O_F32 || OT == O_PART);
+  const bool split = SPLITS && batch.p[0].per > 0;
+  int nk = (int)(batch.p[0].ldx / 128), k0 = 0;
+  int64_t part = 0;
   auto tiles = [&](int q) __attribute__((always_inline)) -> int {
     return (int)((batch.p[q].R + BM - 1) / BM * ((batch.p[q].N + BNO - 1) / BNO));
   };
   // tile `at` of all: its product, and its place there
   auto locate = [&](int at, int& mt, int& nt) __attribute__((always_inline)) -> int {
     int q = 0;
+    if (split) at %= tiles(0);
 #pragma unroll
     for (int j = 0; j + 1 < G; ++j)
       if (q == j && at >= tiles(j)) {
@@ -250,10 +257,17 @@ fb_product_kernel(FbBatch<G> batch) {
   int total = 0;
 #pragma unroll
   for (int j = 0; j < G; ++j) total += tiles(j);
+  if (split) total *= batch.p[0].splits;
   const int wgs = gridDim.x, xcd = (int)blockIdx.x % 8, step = (wgs - xcd + 7) / 8;
   const int before = xcd * (wgs / 8) + min(xcd, wgs % 8);  // workgroups of the XCDs before
   const int last = (int)((int64_t)total * (before + step) / wgs);
   int lin = (int)((int64_t)total * before / wgs) + (int)blockIdx.x / 8;
+  if (split && lin < last) {
+    const int t = tiles(0), slice = lin / t;
+    k0 = slice * batch.p[0].per;
+    nk = min(nk - k0, batch.p[0].per);
+    part = slice * batch.p[0].R * batch.p[0].N;
+  }
   if (lin >= last) return;
 
   // where a lane's loads of a tile read: 32-bit offsets from its first rows; rows past the
@@ -274,10 +288,10 @@ fb_product_kernel(FbBatch<G> batch) {
     const FbArgs& p = batch.p[locate(at, mt, nt)];
     const int64_t row0 = (int64_t)mt * BM, n0 = (int64_t)nt * BNO;
     const int xleft = (int)min<int64_t>(p.R - 1 - row0, BM - 1), wleft = (int)min<int64_t>(p.N - 1 - n0, BNO - 1);
-    X = p.x + row0 * ld;
-    if (FMT == F_CODES) XS = p.xs + row0 * sl;
-    W = p.w + n0 * ld;
-    if (FMT == F_CODES) WS = p.s + n0 * sl;
+    X = p.x + row0 * ld + (int64_t)k0 * 128;
+    if (FMT == F_CODES) XS = p.xs + row0 * sl + k0;
+    W = p.w + n0 * ld + (int64_t)k0 * 128;
+    if (FMT == F_CODES) WS = p.s + n0 * sl + k0;
     const bool ragged = xleft < BM - 1 || wleft < BNO - 1;
     if (!ragged && !offsets) return;  // a whole tile's offsets are there from the one before
     offsets = ragged;
@@ -311,7 +325,7 @@ fb_product_kernel(FbBatch<G> batch) {
       load_k = 0;
     }
     if (FMT == F_CODES && load_k % 16 == 0) {
-      const int word = min(load_k / 4 + lane % 4, batch.p[0].words - 1) * 4;
+      const int word = min(load_k / 4 + lane % 4, batch.p[0].words - 1 - k0 / 4) * 4;
 #pragma unroll
       for (int i = 0; i < C::S_INS; ++i) {
         const int r = (wave * C::S_INS + i) * 16;
@@ -616,7 +630,7 @@ fb_product_kernel(FbBatch<G> batch) {
       const bool whole = n0 + BN <= p.N && p.N % (16 / ES) == 0;  // of the whole workgroup
       const uint32_t ldy = (uint32_t)p.N * ES;
       const int left = rows - wm * (BM / WM);  // rows of this wave's
-      char* out = (char*)p.y + ((row0 + wm * (BM / WM)) * p.N + n0 + wn * (BN / WN)) * ES;
+      char* out = (char*)p.y + (part + (row0 + wm * (BM / WM)) * p.N + n0 + wn * (BN / WN)) * ES;
       uint4 d0, d1, d2, d3;
       auto to_lds = [&](int i, int j) __attribute__((always_inline)) {
 #pragma unroll
@@ -705,7 +719,7 @@ int launch_product_cfg(const FbBatch<G>& b, hipStream_t stream) {
     const int64_t mt = (p.R + BM - 1) / BM, nt = (p.N + BNO - 1) / BNO;
     if (mt > 2147483647LL || nt > 2147483647LL || mt * nt > 2147483647LL)
       return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block product: too many tiles");
-    tiles += mt * nt;
+    tiles += mt * nt * (p.per ? p.splits : 1);
   }
   if ((BM > BN ? BM : BN) * b.p[0].ldx >= 1LL << 32)
     return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block product: rows too wide");
@@ -767,8 +781,74 @@ int launch_products(const FbBatch<G>& b, hipStream_t stream) {
     }
   }
 }
+// y = the slices' parts, in their order
+template <bool BF16>
+__global__ void __launch_bounds__(256) fb_join_kernel(const float* __restrict__ part, void* __restrict__ y, int splits,
+                                                      int64_t n) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s = 0; s < splits; ++s) {
+    const float* at = part + s * n + i;
+    if (i + 4 <= n) {
+      const fb_u32x4_at4 u = *(const fb_u32x4_at4*)at;
+      v[0] += __uint_as_float(u.x);
+      v[1] += __uint_as_float(u.y);
+      v[2] += __uint_as_float(u.z);
+      v[3] += __uint_as_float(u.w);
+    } else {
+      for (int j = 0; i + j < n; ++j) v[j] += at[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (i + j < n) {
+      if constexpr (BF16) ((__bf16*)y)[i + j] = (__bf16)v[j];
+      else ((float*)y)[i + j] = v[j];
+    }
+}
+
+// Few tiles of a long K leave most CUs idle: K in slices, as many as CUs have a tile each,
+// of 8 stages and more, and another launch that joins them (3 us): 65 x 2560 -> 1024 fp32 52
+// to 20 us, 509 x 2560 -> 500 18 to 9.
+struct Slices {
+  int splits, per;  // 0: not worth it
+  int64_t bytes;
+};
+Slices slices(int64_t R, int64_t N, int64_t nk) {
+  const int64_t tiles = (R + 63) / 64 * ((N + 127) / 128);
+  Slices q{};
+  int64_t most = cu_count() / std::max<int64_t>(tiles, 1);
+  most = std::min(most, nk / 8);
+  if (most < 2) return q;
+  const int64_t per = ((nk + most - 1) / most + 3) / 4 * 4;  // whole words of scales
+  q.splits = (int)((nk + per - 1) / per);
+  q.per = (int)per;
+  // what is saved, a stage 0.37 us, is to be more than the join
+  if (q.splits < 2 || (nk - per) * 37 < 400) return Slices{};
+  q.bytes = q.splits * R * N * 4;
+  return q;
+}
+int64_t slices_bytes(int64_t R, int64_t N, int64_t nk) { return slices(R, N, nk).bytes; }
+
+// room: slices_bytes of workspace (256-byte aligned), or null where there are none
 template <int FMT, int OT>
-int launch_product(const FbArgs& p, hipStream_t stream) {
+int launch_product(const FbArgs& p, void* room, hipStream_t stream) {
+  if constexpr (OT == O_BF16 || OT == O_F32) {
+    const Slices q = slices(p.R, p.N, p.ldx / 128);
+    if (q.splits) {
+      FbArgs a = p;
+      a.splits = q.splits;
+      a.per = q.per;
+      a.y = room;
+      constexpr int PART = FMT == F_CODES && OT == O_BF16 ? O_PART : O_F32;
+      if (int rc = launch_product_cfg<FMT, PART, 64, 128, 2, 2, 4>(FbBatch<1>{{a}}, stream)) return rc;
+      const int64_t n = p.R * p.N;
+      hipLaunchKernelGGL((fb_join_kernel<OT == O_BF16>), dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, stream,
+                         (const float*)room, p.y, q.splits, n);
+      return check_launch("fb_join_kernel");
+    }
+  }
   return launch_products<FMT, OT>(FbBatch<1>{{p}}, stream);
 }
 
@@ -1287,8 +1367,22 @@ int launch_quantize(const void* x, int dtype, uint8_t* codes, uint8_t* scales, i
   return check_launch("fb_quantize_kernel");
 }
 
+struct LinearParts {
+  int64_t xc, xs, room, total;
+};
+LinearParts linear_parts(int64_t rows, int64_t in_f, int64_t out_f, int x_dtype) {
+  LinearParts q{};
+  Parts w;
+  const bool round = x_dtype != SMAUL_DTYPE_FP8_BLOCK && !rounds_itself(rows, in_f);
+  q.xc = w.take(round ? rows * fb_width(in_f) : 0);
+  q.xs = w.take(round ? rows * fb_words(in_f) * 4 : 0);
+  q.room = w.take(rows > FB_FEW ? slices_bytes(rows, out_f, fb_blocks(in_f)) : 0);
+  q.total = w.at;
+  return q;
+}
+
 struct FfnParts {
-  int64_t xc, xs, hc, hs, hf, total;
+  int64_t xc, xs, hc, hs, hf, room, total;
 };
 // what the caller keeps for the gradients stands in `saved` (save), the rest in the workspace
 FfnParts ffn_parts(int64_t T, int64_t d, int64_t h, int x_dtype, bool save) {
@@ -1300,12 +1394,13 @@ FfnParts ffn_parts(int64_t T, int64_t d, int64_t h, int x_dtype, bool save) {
   q.hc = w.take(save ? 0 : T * fb_width(h));
   q.hs = w.take(save ? 0 : T * fb_words(h) * 4);
   q.hf = w.take(T <= FB_FEW ? T * h * 4 : 0);
+  q.room = w.take(T > FB_FEW ? slices_bytes(T, d, fb_blocks(h)) : 0);
   q.total = w.at;
   return q;
 }
 
 struct FfnBackParts {
-  int64_t dy, wd, wgu, dgu, dgut, xt, dyt, ht, total;
+  int64_t dy, wd, wgu, dgu, dgut, xt, dyt, ht, room, total;
   int64_t lt, ld, lh;  // T, d and h to whole stages
 };
 FfnBackParts ffn_back_parts(int64_t T, int64_t d, int64_t h, bool dx, bool dw) {
@@ -1322,12 +1417,13 @@ FfnBackParts ffn_back_parts(int64_t T, int64_t d, int64_t h, bool dx, bool dw) {
   q.xt = w.take(dw ? d * q.lt * 2 : 0);
   q.dyt = w.take(dw ? d * q.lt * 2 : 0);
   q.ht = w.take(dw ? h * q.lt * 2 : 0);
+  q.room = w.take(dx ? slices_bytes(T, d, q.lh / 32) : 0);
   q.total = w.at;
   return q;
 }
 
 struct DxParts {
-  int64_t g, wt, total, ld;
+  int64_t g, wt, room, total, ld;
   int copies;
 };
 DxParts dx_parts(int64_t rows, int64_t in_f, int64_t out_f, int dtype) {
@@ -1339,6 +1435,7 @@ DxParts dx_parts(int64_t rows, int64_t in_f, int64_t out_f, int dtype) {
   q.ld = fb_stages(out_f) * 64 * q.copies;
   q.g = w.take(f32 || out_f % 64 ? rows * q.ld * 2 : 0);
   q.wt = w.take(in_f * q.ld * 2);
+  q.room = w.take(slices_bytes(rows, in_f, q.ld / 64));
   q.total = w.at;
   return q;
 }
@@ -1385,12 +1482,7 @@ int smaul_fp8_block_dequantize(const uint8_t* codes, const uint8_t* scales, void
 
 int64_t smaul_fp8_block_linear_workspace_size(int64_t rows, int64_t in_f, int64_t out_f, int x_dtype) {
   if (rows < 0 || in_f <= 0 || out_f <= 0 || !x_ok(x_dtype)) return -1;
-  Parts w;
-  if (x_dtype != SMAUL_DTYPE_FP8_BLOCK && !rounds_itself(rows, in_f)) {
-    w.take(rows * fb_width(in_f));
-    w.take(rows * fb_words(in_f) * 4);
-  }
-  return w.at;
+  return linear_parts(rows, in_f, out_f, x_dtype).total;
 }
 
 int smaul_fp8_block_linear(const void* x, int x_dtype, const uint8_t* xs, const uint8_t* w, const uint8_t* s, void* y,
@@ -1403,13 +1495,14 @@ int smaul_fp8_block_linear(const void* x, int x_dtype, const uint8_t* xs, const 
   if (!x || !w || !s || !y || (given && !xs)) return fail(SMAUL_ERR_INVALID, "fp8_block_linear: null pointer");
   if (!fb_aligned(x, 16) || !fb_aligned(w, 16) || !fb_aligned(y, 16) || !fb_aligned(s, 4) || (given && !fb_aligned(xs, 4)))
     return fail(SMAUL_ERR_INVALID, "fp8_block_linear: x, y and the codes must be 16-byte aligned, the scales 4-byte");
-  const int64_t need = smaul_fp8_block_linear_workspace_size(rows, in_f, out_f, x_dtype);
+  const LinearParts q = linear_parts(rows, in_f, out_f, x_dtype);
+  const int64_t need = q.total;
   if (workspace_bytes < need || (need > 0 && (!workspace || !fb_aligned(workspace, 256))))
     return fail(SMAUL_ERR_INVALID, "fp8_block_linear: workspace %lld < %lld bytes, or unaligned",
                 (long long)workspace_bytes, (long long)need);
   if (!given && !rounds_itself(rows, in_f)) {
-    uint8_t* c = (uint8_t*)workspace;
-    uint8_t* cs = c + fb_align256(rows * fb_width(in_f));
+    uint8_t* c = (uint8_t*)workspace + q.xc;
+    uint8_t* cs = (uint8_t*)workspace + q.xs;
     if (int rc = launch_quantize(x, x_dtype, c, cs, rows, in_f, stream)) return rc;
     x = c;
     xs = cs;
@@ -1419,7 +1512,9 @@ int smaul_fp8_block_linear(const void* x, int x_dtype, const uint8_t* xs, const 
   if (rows <= FB_FEW)
     return y_dtype == SMAUL_DTYPE_BF16 ? launch_stream<O_BF16>(p, x_dtype, in_f, stream)
                                        : launch_stream<O_F32>(p, x_dtype, in_f, stream);
-  return y_dtype == SMAUL_DTYPE_BF16 ? launch_product<F_CODES, O_BF16>(p, stream) : launch_product<F_CODES, O_F32>(p, stream);
+  void* room = (char*)workspace + q.room;
+  return y_dtype == SMAUL_DTYPE_BF16 ? launch_product<F_CODES, O_BF16>(p, room, stream)
+                                     : launch_product<F_CODES, O_F32>(p, room, stream);
 }
 
 int64_t smaul_fp8_block_backward_input_workspace_size(int64_t rows, int64_t in_f, int64_t out_f, int dtype) {
@@ -1461,7 +1556,8 @@ int smaul_fp8_block_backward_input(const void* g, int dtype, const uint8_t* w, c
   }
   if (int rc = launch_turns(a, n, stream)) return rc;
   const FbArgs p = rows_args(g, wt, dx, rows, q.ld, in_f);
-  return bf16 ? launch_product<F_BF16, O_BF16>(p, stream) : launch_product<F_BF16, O_F32>(p, stream);
+  void* room = ws + q.room;
+  return bf16 ? launch_product<F_BF16, O_BF16>(p, room, stream) : launch_product<F_BF16, O_F32>(p, room, stream);
 }
 
 int64_t smaul_fp8_block_ffn_saved_size(int64_t T, int64_t h) {
@@ -1516,8 +1612,8 @@ int smaul_fp8_block_ffn_forward(const void* x, int x_dtype, const uint8_t* xs, c
   p.kept = (uint8_t*)saved;
   const FbArgs down = codes_args(hc, hs, down_w, down_s, y, T, h, d);
   if (!few) {
-    if (int rc = launch_product<F_CODES, O_GATED>(p, stream)) return rc;
-    return launch_product<F_CODES, O_BF16>(down, stream);
+    if (int rc = launch_product<F_CODES, O_GATED>(p, nullptr, stream)) return rc;
+    return launch_product<F_CODES, O_BF16>(down, ws + q.room, stream);
   }
   p.y = ws + q.hf;
   if (int rc = launch_stream<O_GATED>(p, xt, d, stream)) return rc;
@@ -1582,9 +1678,9 @@ int smaul_fp8_block_ffn_backward(const void* dy, const uint8_t* gate_w, const ui
   FbArgs p = rows_args(rows, wd, dgu, T, q.ld, h);
   p.kept = (uint8_t*)saved;
   p.ldh = q.lh;
-  if (int rc = launch_product<F_BF16, O_DGATED>(p, stream)) return rc;
+  if (int rc = launch_product<F_BF16, O_DGATED>(p, nullptr, stream)) return rc;
   if (dx)
-    if (int rc = launch_product<F_BF16, O_BF16>(rows_args(dgu, wgu, dx, T, 2 * q.lh, d), stream)) return rc;
+    if (int rc = launch_product<F_BF16, O_BF16>(rows_args(dgu, wgu, dx, T, 2 * q.lh, d), ws + q.room, stream)) return rc;
   if (!weights) return SMAUL_OK;
   FbTurns b{};
   b.t[0] = turn_rows(dgu, S_BF16, T, 2 * q.lh, dgut, q.lt, 1);

@@ -150,3 +150,20 @@ def test_backward_input(rows, K, N):
         assert dx.dtype == dtype
         ref.check(dx, *ref.product(t.double(), wv.t().contiguous(), dtype), (rows, K, N, dtype))
     assert be().fp8_block_backward_input(t[:0].to(DEV), w.to(DEV), s.to(DEV), K, N).shape == (0, K)
+
+
+@pytest.mark.parametrize("rows,K,N", [(70, 8192, 140), (130, 6000, 300), (65, 5001, 70), (200, 16384, 96)])
+def test_few_tiles_of_a_long_axis(rows, K, N):
+    """K in slices that are joined: forward, and the input gradient over as many outputs."""
+    g = gen(rows)
+    w, s = ref.weight(N, K, g)
+    wv = ref.values(w, s, K)
+    x = torch.randn(rows, K, generator=g)
+    for dtype in (BF, F32):
+        y = be().fp8_block_forward(x.to(dtype).to(DEV), w.to(DEV), s.to(DEV), K, N)
+        ref.check(y, *ref.product(ref.rounded(x.to(dtype)), wv, dtype, codes=True), (rows, K, N, dtype))
+    w, s = ref.weight(K, N, g)
+    wv = ref.values(w, s, N)
+    for dtype in (BF, F32):
+        dx = be().fp8_block_backward_input(x.to(dtype).to(DEV), w.to(DEV), s.to(DEV), N, K)
+        ref.check(dx, *ref.product(x.to(dtype).double(), wv.t().contiguous(), dtype), (rows, K, N, dtype))

@@ -28,7 +28,7 @@ def block(T, d, h, seed=0):
 
 
 SHAPES = [(1, 1, 1), (1, 128, 128), (2, 64, 200), (3, 300, 129), (33, 128, 384), (64, 200, 640), (65, 130, 257),
-          (130, 256, 512), (300, 500, 1251), (257, 129, 130)]
+          (130, 256, 512), (300, 500, 1251), (257, 129, 130), (70, 130, 4200)]
 
 
 @pytest.mark.parametrize("T,d,h", SHAPES)
