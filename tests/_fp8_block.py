@@ -116,11 +116,12 @@ def silu(g):
     return g * torch.sigmoid(g)
 
 
-def ffn(x, gate, up, down):
-    """(y, bound, g, u, h, bound of h's values): hidden rows rounded from fp32, y to bf16."""
+def ffn(x, gate, up, down, exact=False):
+    """(y, bound, g, u, h, bound of h's values): hidden rows rounded from fp32, y to bf16.
+    ``exact``: hidden rows of exact products (few of them), else of the 8-bit instructions."""
     g, u = x @ gate.t(), x @ up.t()
     rel = 128 * blocks(x.shape[-1]) * U
-    ge, ue = (x.abs() @ w.abs().t() * rel + aligned(x, w) for w in (gate, up))
+    ge, ue = (x.abs() @ w.abs().t() * rel + (0 if exact else aligned(x, w)) for w in (gate, up))
     v = silu(g) * u
     # |silu'| <= 1.1, |silu(g)| <= |g|; 2^-19 for the product's own arithmetic
     ve = 1.1 * ge * (u.abs() + ue) + g.abs() * ue + 2.0 ** -19 * v.abs()
@@ -130,10 +131,10 @@ def ffn(x, gate, up, down):
     return y, ye + HALF[torch.bfloat16] * (y.abs() + ye), g, u, h, he, ge, ue
 
 
-def ffn_grad(x, dy, gate, up, down, kept):
+def ffn_grad(x, dy, gate, up, down, kept, exact=False):
     """{name: (gradient, bound)} of the block; ``kept``: how far what the forward pass keeps of
     u silu'(g) and silu(g) is rounded, relative.  dg and du are rounded to bf16."""
-    y, ye, g, u, h, he, ge, ue = ffn(x, gate, up, down)
+    y, ye, g, u, h, he, ge, ue = ffn(x, gate, up, down, exact)
     d, n, T = x.shape[-1], gate.shape[0], x.shape[0]
     half = HALF[torch.bfloat16]
     sig = torch.sigmoid(g)
