@@ -65,6 +65,24 @@ def _rows(x):
     return x if x.dtype in (torch.float32, torch.bfloat16) else x.float()
 
 
+def _check_leaves(*leaves):
+    """Refuses to record a pass under capture while a pass recorded outside holds one of its
+    leaves: autograd orders the leaf's accumulation by the stream of the pass that first
+    recorded it, and a captured backward pass that meets a stream outside its capture ends
+    the process.  Returns what the caller holds until its pass is recorded: the leaves'
+    nodes, which carry the mark."""
+    leaves = [t for t in leaves if t is not None and t.requires_grad and t.is_leaf and t.is_cuda]
+    if not leaves or not torch.is_grad_enabled():
+        return []
+    capturing = torch.cuda.is_current_stream_capturing()
+    nodes = [torch.autograd.graph.get_gradient_edge(t).node for t in leaves]
+    for node in nodes:
+        if node.metadata.setdefault("smaul_captured", capturing) is False and capturing:
+            raise RuntimeError("a pass recorded outside of this capture still holds a leaf of this one: free its "
+                               "outputs before the capture")
+    return nodes
+
+
 class _Matmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, codes, scales, in_f, out_f):
@@ -121,8 +139,12 @@ class FP8BlockLinear(nn.Module):
             self.bias.copy_(bias.detach())
 
     def forward(self, x):
+        nodes = _check_leaves(x, self.bias)
         y = _Matmul.apply(x, self.w8, self.ws, self.in_f, self.out_f)
-        return y if self.bias is None else y + self.bias
+        if self.bias is not None:
+            y = y + self.bias
+        del nodes
+        return y
 
     def extra_repr(self):
         return f"in_f={self.in_f}, out_f={self.out_f}, bias={self.bias is not None}"
@@ -160,7 +182,10 @@ class AddRMSNorm(nn.Module):
         self.weight = nn.Parameter(torch.ones(d))
 
     def forward(self, x, residual=None):
-        return _AddRMSNorm.apply(x, residual, self.weight, self.eps)
+        nodes = _check_leaves(x, residual, self.weight)
+        y = _AddRMSNorm.apply(x, residual, self.weight, self.eps)
+        del nodes
+        return y
 
     def extra_repr(self):
         return f"d={self.weight.numel()}, eps={self.eps}"
@@ -257,10 +282,13 @@ class FP8BlockFFN(nn.Module):
 
     def _apply_block(self, x, residual, norm_weight, eps):
         weights = self._weights()
+        nodes = _check_leaves(x, residual, norm_weight, *weights)
         # a recorded pass keeps what its gradients need
         need = torch.is_grad_enabled() and any(t is not None and t.requires_grad
                                                for t in (x, residual, norm_weight, *weights))
-        return _FFN.apply(x, residual, norm_weight, eps, self.d, self.h, self.trainable, need, *weights)
+        y = _FFN.apply(x, residual, norm_weight, eps, self.d, self.h, self.trainable, need, *weights)
+        del nodes
+        return y
 
     def forward(self, x):
         return self._apply_block(x, None, None, None)
