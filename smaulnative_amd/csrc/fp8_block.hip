@@ -100,16 +100,14 @@ __device__ __forceinline__ int64_t fb_kept_at(int64_t row, int64_t n, int64_t h)
   return (row / 32 * (fb_width(h) / 32) + n / 32) * FB_KEPT + (row % 32 + n / 16 % 2 * 32) * 16;
 }
 
-// a float's bits, its third byte to nearest
-__device__ __forceinline__ uint32_t fb_bits24(float v) {
-  const uint32_t b = __float_as_uint(v);
-  return (b & 0x7f800000u) == 0x7f800000u ? (b & 0x7fffffu ? b | 0x400000u : b) : b + 0x7fu + ((b >> 8) & 1u);
-}
+// a float's bits, its third byte to nearest (halves up); an infinity's sum keeps its other bytes
+__device__ __forceinline__ uint32_t fb_bits24(float v) { return v == v ? __float_as_uint(v) + 0x80u : 0x7fc00000u; }
 // 4 or 16 values: high halves and third bytes
 __device__ __forceinline__ void fb_pack24(const float (&v)[4], uint2& hi, uint32_t& lo) {
   const uint32_t u[4] = {fb_bits24(v[0]), fb_bits24(v[1]), fb_bits24(v[2]), fb_bits24(v[3])};
   hi = make_uint2(__builtin_amdgcn_perm(u[1], u[0], 0x07060302u), __builtin_amdgcn_perm(u[3], u[2], 0x07060302u));
-  lo = (u[0] >> 8 & 255u) | (u[1] & 0xff00u) | (u[2] << 8 & 0xff0000u) | (u[3] << 16 & 0xff000000u);
+  lo = __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[3], u[2], 0x0c0c0501u), __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0501u),
+                             0x05040100u);
 }
 __device__ __forceinline__ void fb_pack24(const float (&v)[16], uint4 (&hi)[2], uint4& lo) {
   uint2 h[4];
@@ -128,7 +126,7 @@ __device__ __forceinline__ void fb_unpack24(const uint4 (&hi)[2], const uint4& l
   const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w};
 #pragma unroll
   for (int r = 0; r < 16; ++r)
-    v[r] = __uint_as_float((r & 1 ? h[r / 2] & 0xffff0000u : h[r / 2] << 16) | (l[r / 4] >> (8 * (r & 3)) & 255u) << 8);
+    v[r] = __uint_as_float(__builtin_amdgcn_perm(h[r / 2], l[r / 4], (r & 1 ? 0x0706000cu : 0x0504000cu) | (r & 3) << 8));
 }
 
 // silu(g) u, u silu'(g) and silu(g)
@@ -501,13 +499,17 @@ fb_product_kernel(FbBatch<G> batch) {
           const int left = (int)min<int64_t>(p.N - n, 16);
           fb_pin(acc[j][i]);
           fb_pin(acc[j + HT][i]);
-          float a[16], b[16];
+          float v[16], a[16], b[16];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) v[r] = fb_gated(acc[j][i][r], acc[j + HT][i][r], a[r], b[r]);
+          if (n0 + BNO > p.N) {  // past N: copies of the last row's
+#pragma unroll
+            for (int r = 0; r < 16; ++r) v[r] = r < left ? v[r] : 0.0f;
+          }
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            float v = fb_gated(acc[j][i][r], acc[j + HT][i][r], a[r], b[r]);
-            v = r < left ? v : 0.0f;  // past N: copies of the last row's
-            acc[j][i][r] = v;
-            m = __builtin_elementwise_maximum(m, __builtin_fabsf(v));  // NaN stays NaN
+            acc[j][i][r] = v[r];
+            m = __builtin_elementwise_maximum(m, __builtin_fabsf(v[r]));  // NaN stays NaN
           }
           fb_pin(acc[j][i]);
           if (p.kept && lr < rows) {
