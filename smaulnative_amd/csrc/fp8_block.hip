@@ -1062,37 +1062,38 @@ __global__ void __launch_bounds__(512) fb_stream_kernel(FbArgs p, int64_t K) {
   }
 }
 
-// v = a + b + c, each the next 8 significant bits: exact in bf16, and all 24 of fp32.  An
-// infinity or NaN is a alone.
-__device__ __forceinline__ void fb_split3(float (&v)[8], bf16x8_t (&t)[3]) {
+// v = a + b + c, each the next 8 significant bits: exact in bf16 (their upper halves), and all
+// 24 of fp32.  An infinity or NaN is a alone.
+__device__ __forceinline__ void fb_thirds(float v, uint32_t (&t)[3]) {
+  const float x = __builtin_canonicalizef(v);
+  t[0] = __float_as_uint(x) & 0xffff0000u;
+  const float rest = x - __uint_as_float(t[0]), y = rest == rest ? rest : 0.0f;
+  t[1] = __float_as_uint(y) & 0xffff0000u;
+  t[2] = __float_as_uint(y - __uint_as_float(t[1]));
+}
+__device__ __forceinline__ void fb_split3(const float (&v)[8], bf16x8_t (&t)[3]) {
+  uint32_t w[3][4];
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    uint32_t w[4];
+  for (int q = 0; q < 4; ++q) {
+    uint32_t a[3], b[3];
+    fb_thirds(v[2 * q], a);
+    fb_thirds(v[2 * q + 1], b);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      uint32_t part[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float x = __builtin_canonicalizef(v[2 * q + e]);
-        part[e] = __float_as_uint(x) >> 16;
-        const float rest = x - __uint_as_float(part[e] << 16);
-        v[2 * q + e] = rest == rest ? rest : 0.0f;
-      }
-      w[q] = part[0] | part[1] << 16;
-    }
-    t[k] = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+    for (int k = 0; k < 3; ++k) w[k][q] = __builtin_amdgcn_perm(b[k], a[k], 0x07060302u);
   }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) t[k] = __builtin_bit_cast(bf16x8_t, make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]));
 }
 
-// The input gradient of few rows, in one launch: a workgroup has 32 columns, its 8 waves a
-// slice of the weight's rows each.  A lane reads 32 codes of one row, and the wave turns 64
-// such rows round through LDS of its own, decoded to bf16.  The four workgroups that share
-// a line of codes are neighbours in one XCD's band.  (1 row 2560 -> 1024: 21 us by way of
-// the turned weight.)
+// The input gradient of few rows, in one launch: a workgroup has 32 columns of up to 64 rows,
+// its 8 waves a slice of the weight's rows each.  A lane reads 32 codes of one row, and the
+// wave turns 64 such rows round through LDS of its own, decoded to bf16.  The groups of rows
+// and the four workgroups that share a line of codes are neighbours in one XCD's band.  (1 row
+// 2560 -> 1024: 9 us, 21 by way of the turned weight.)
 template <bool BF16, int RT>
 __global__ void __launch_bounds__(512)
 fb_dx_stream_kernel(const void* __restrict__ grad, const uint8_t* __restrict__ w, const uint8_t* __restrict__ s,
-                    void* __restrict__ dx, int R, int64_t I, int64_t O) {
+                    void* __restrict__ dx, int64_t rows, int64_t I, int64_t O) {
   constexpr int NW = 8, LD = 72, OWN = RT * 4096 > 32 * LD * 2 ? RT * 4096 : 32 * LD * 2, NT = BF16 ? 1 : 3;
   __shared__ __attribute__((aligned(16))) char smem[NW * OWN];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, l32 = lane & 31;
@@ -1102,7 +1103,9 @@ fb_dx_stream_kernel(const void* __restrict__ grad, const uint8_t* __restrict__ w
     const int64_t full = (int64_t)gridDim.x / 8 * 8;
     if (b0 < full) b0 = b0 % 8 * (full / 8) + b0 / 8;
   }
-  const int64_t k0 = b0 * 32, nb = fb_blocks(I), ns = (nb + 3) / 4 * 4;
+  const int64_t groups = (rows + RT * 32 - 1) / (RT * 32), row0 = b0 % groups * (RT * 32);
+  const int64_t k0 = b0 / groups * 32, nb = fb_blocks(I), ns = (nb + 3) / 4 * 4;
+  const int R = (int)min<int64_t>(rows - row0, RT * 32);
   const int64_t steps = (O + 63) / 64, per = (steps + NW - 1) / NW;
   const int64_t lo = min((int64_t)wave * per, steps), hi = min(lo + per, steps);
   uint16_t* own = (uint16_t*)(smem + wave * OWN);
@@ -1130,7 +1133,7 @@ fb_dx_stream_kernel(const void* __restrict__ grad, const uint8_t* __restrict__ w
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) fb_load8<BF16>(grad, min(t * 32 + l32, R - 1), O, step * 64 + q * 16 + g * 8, v[t][q]);
+      for (int q = 0; q < 4; ++q) fb_load8<BF16>(grad, row0 + min(t * 32 + l32, R - 1), O, step * 64 + q * 16 + g * 8, v[t][q]);
     const uint32_t c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -1180,14 +1183,15 @@ fb_dx_stream_kernel(const void* __restrict__ grad, const uint8_t* __restrict__ w
       a.z += b.z;
       a.w += b.w;
     }
-    const int64_t row = t * 32 + (l & 31), n = k0 + (l >> 5) * 16 + i * 4;
+    const int row = t * 32 + (l & 31);
+    const int64_t n = k0 + (l >> 5) * 16 + i * 4;
     const float f[4] = {a.x, a.y, a.z, a.w};
     if (row < R) {
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         if (n + q < I) {
-          if constexpr (BF16) ((__bf16*)dx)[row * I + n + q] = (__bf16)f[q];
-          else ((float*)dx)[row * I + n + q] = f[q];
+          if constexpr (BF16) ((__bf16*)dx)[(row0 + row) * I + n + q] = (__bf16)f[q];
+          else ((float*)dx)[(row0 + row) * I + n + q] = f[q];
         }
     }
   }
@@ -1267,34 +1271,26 @@ __device__ __forceinline__ void fb_turn(const FbTurn& t, int64_t b, uint16_t* sh
       }
     }
   }
+  uint32_t w[PLANES][8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    uint32_t x[3] = {__float_as_uint(v[2 * q])}, y[3] = {__float_as_uint(v[2 * q + 1])};  // exact in bf16
+    if constexpr (FMT == S_F32) {
+      fb_thirds(v[2 * q], x);
+      fb_thirds(v[2 * q + 1], y);
+    }
+#pragma unroll
+    for (int p = 0; p < PLANES; ++p) w[p][q] = __builtin_amdgcn_perm(y[p], x[p], 0x07060302u);
+  }
 #pragma unroll
   for (int p = 0; p < PLANES; ++p) {
-    uint32_t w[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      uint32_t part[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float& f = v[2 * q + e];
-        if constexpr (FMT == S_F32) {  // the next 8 significant bits; an infinity or NaN is in the first plane alone
-          const float x = __builtin_canonicalizef(f);
-          const uint32_t top = __float_as_uint(x) & 0xffff0000u;
-          const float rest = x - __uint_as_float(top);
-          f = rest == rest ? rest : 0.0f;
-          part[e] = top >> 16;
-        } else {
-          part[e] = __float_as_uint(f) >> 16;  // exact
-        }
-      }
-      w[q] = part[0] | part[1] << 16;
-    }
     if constexpr (TURNED) {
 #pragma unroll
-      for (int q = 0; q < 16; ++q) sh[(lc + q) * LD + lr] = (uint16_t)(w[q / 2] >> (16 * (q & 1)));
+      for (int q = 0; q < 16; ++q) sh[(lc + q) * LD + lr] = (uint16_t)(w[p][q / 2] >> (16 * (q & 1)));
     } else if (r < t.R) {
       uint4* o = (uint4*)(t.dst + r * t.ld + c0 * PLANES + p * 64 + lc);
-      o[0] = make_uint4(w[0], w[1], w[2], w[3]);
-      o[1] = make_uint4(w[4], w[5], w[6], w[7]);
+      o[0] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+      o[1] = make_uint4(w[p][4], w[p][5], w[p][6], w[p][7]);
     }
   }
   if constexpr (TURNED) {
@@ -1428,6 +1424,18 @@ FfnBackParts ffn_back_parts(int64_t T, int64_t d, int64_t h, bool dx, bool dw) {
   return q;
 }
 
+// Whether fb_dx_stream_kernel has the call: of few rows, and of as many as one round of the
+// CUs takes in two steps a wave.  There the two launches (or three, in slices) wait for one
+// another longer than the weight's being turned by each group of rows takes (us, by way of
+// the turned weight and so: 512 x 777 -> 1000 fp32 22.5 and 13.4, 2048 x 256 -> 256 13.1 and
+// 8.7, 128 x 1024 -> 2560 bf16 13.4 and 9.5; past it 1001 x 777 -> 1000 fp32 26.3 and 24.2, bf16
+// 13.7 and 22.6).
+bool dx_streams(int64_t rows, int64_t in_f, int64_t out_f) {
+  if (rows <= FB_FEW) return true;
+  const int64_t wgs = (in_f + 31) / 32 * ((rows + 63) / 64);
+  return (wgs + cu_count() - 1) / cu_count() * (((out_f + 63) / 64 + 7) / 8) <= 2;
+}
+
 struct DxParts {
   int64_t g, wt, room, total, ld;
   int copies;
@@ -1436,7 +1444,7 @@ DxParts dx_parts(int64_t rows, int64_t in_f, int64_t out_f, int dtype) {
   DxParts q{};
   Parts w;
   const bool f32 = dtype == SMAUL_DTYPE_F32;
-  if (rows <= FB_FEW) return q;
+  if (dx_streams(rows, in_f, out_f)) return q;
   q.copies = f32 ? 3 : 1;
   q.ld = fb_stages(out_f) * 64 * q.copies;
   q.g = w.take(f32 || out_f % 64 ? rows * q.ld * 2 : 0);
@@ -1544,12 +1552,12 @@ int smaul_fp8_block_backward_input(const void* g, int dtype, const uint8_t* w, c
   const DxParts q = dx_parts(rows, in_f, out_f, dtype);
   char* ws = (char*)workspace;
   const bool bf16 = dtype == SMAUL_DTYPE_BF16;
-  if (rows <= FB_FEW) {
-    const int64_t blocks = (in_f + 31) / 32;
+  if (dx_streams(rows, in_f, out_f)) {
+    const int64_t blocks = (in_f + 31) / 32 * ((rows + 63) / 64);
     if (!grid_fits(blocks, 512)) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block_backward_input: too wide a weight");
     auto* kernel = bf16 ? (rows <= 32 ? &fb_dx_stream_kernel<true, 1> : &fb_dx_stream_kernel<true, 2>)
                         : (rows <= 32 ? &fb_dx_stream_kernel<false, 1> : &fb_dx_stream_kernel<false, 2>);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(512), 0, stream, g, w, s, dx, (int)rows, in_f, out_f);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(512), 0, stream, g, w, s, dx, rows, in_f, out_f);
     return check_launch("fb_dx_stream_kernel");
   }
   uint16_t* wt = (uint16_t*)(ws + q.wt);

@@ -167,3 +167,24 @@ def test_few_tiles_of_a_long_axis(rows, K, N):
     for dtype in (BF, F32):
         dx = be().fp8_block_backward_input(x.to(dtype).to(DEV), w.to(DEV), s.to(DEV), N, K)
         ref.check(dx, *ref.product(x.to(dtype).double(), wv.t().contiguous(), dtype), (rows, K, N, dtype))
+
+
+# a wave's steps and the rounds of workgroups on either side of what one launch has
+@pytest.mark.parametrize("rows,K,N", [(65, 513, 1024), (65, 513, 1025), (300, 131, 1101), (257, 64, 777), (1001, 1000, 777),
+                                      (520, 1000, 1000), (2100, 250, 500), (2100, 260, 520)])
+def test_backward_input_by_either_way(rows, K, N):
+    g = gen(rows * K + N)
+    w, s = ref.weight(N, K, g)
+    wv = ref.values(w, s, K).t().contiguous()
+    dy = torch.randn(rows, N, generator=g)
+    for dtype in (BF, F32):
+        t = dy.to(dtype)
+        dx = be().fp8_block_backward_input(t.to(DEV), w.to(DEV), s.to(DEV), K, N)
+        ref.check(dx, *ref.product(t.double(), wv, dtype), (rows, K, N, dtype))
+        t[1, N - 1], t[rows - 1, 0], t[rows // 2, 5] = float("nan"), float("inf"), float("-inf")
+        bad = dx.clone()
+        bad[[1, rows - 1, rows // 2]] = 0
+        dx = be().fp8_block_backward_input(t.to(DEV), w.to(DEV), s.to(DEV), K, N)
+        assert not torch.isfinite(dx[[1, rows - 1, rows // 2]]).any()
+        dx[[1, rows - 1, rows // 2]] = 0
+        assert torch.equal(dx, bad)
