@@ -601,7 +601,9 @@ int smaul_fp8_block_dequantize(const uint8_t* codes, const uint8_t* scales, void
  * y[rows, out_f] = Q(x)[rows, in_f] . decode(w, s)^T, w and s [out_f, in_f] in that format,
  * y of y_dtype (f32 or bf16).  x: rows of x_dtype f32 or bf16, rounded to the format in the
  * workspace, or with x_dtype SMAUL_DTYPE_FP8_BLOCK codes with scales xs.  Products are
- * exact, sums fp32.  x, y and w 16-byte aligned, scales 4, the workspace 256.
+ * exact, sums fp32; towards a y of bf16, 8 neighbouring products may be summed with the last
+ * bit 2^-13 of the largest's power of two.  x, y and w 16-byte aligned, scales 4, the
+ * workspace 256.
  */
 enum { SMAUL_DTYPE_FP8_BLOCK = 2 };
 int64_t smaul_fp8_block_linear_workspace_size(int64_t rows, int64_t in_f, int64_t out_f, int x_dtype);
@@ -622,7 +624,9 @@ int smaul_fp8_block_backward_input(const void* g, int dtype, const uint8_t* w, c
 /*
  * The gated feed-forward block in that format: hdn = Q(silu(x . Wg^T) * (x . Wu^T)),
  * y[T, d] (bf16) = hdn . Wd^T; gate_w / up_w [h, d], down_w [d, h].  x: bf16 rows, rounded
- * first, or codes with xs.  The hidden rows are rounded from fp32.
+ * first, or codes with xs.  The hidden rows are rounded from fp32, whose sums are as those
+ * towards bf16 above where T and h are large (more than a tile of 64 by 128 for each CU),
+ * fp32 throughout below.
  * saved (smaul_fp8_block_ffn_saved_size bytes): what the backward pass takes is kept, in
  * saved itself, h_codes / h_scales [T, h] and, of an x of rows, x_codes / x_scales [T, d];
  * NULL: nothing is, and those may be NULL too.  Rows and codes 16-byte aligned, scales 4,

@@ -11,7 +11,8 @@ Flags:
   instructions in generated code.
 - ``-mllvm -amdgpu-mfma-vgpr-form``: MFMA results in ordinary VGPRs.  The
   GEMM scales every MFMA partial with a VALU fma; with the results in AGPRs
-  each of those would need two extra v_accvgpr moves.
+  each of those would need two extra v_accvgpr moves.  Not for ``AGPR_SOURCES``,
+  whose sums stay on the matrix cores until they are stored.
 """
 from __future__ import annotations
 

@@ -512,7 +512,7 @@ fb_product_kernel(FbBatch<G> batch) {
             m = __builtin_elementwise_maximum(m, __builtin_fabsf(v[r]));  // NaN stays NaN
           }
           fb_pin(acc[j][i]);
-          if (p.kept && lr < rows) {
+          if (p.kept && lr < rows) {  // 8192 tokens, 1024 by 2560: 91 us with down for 74 without
             uint4 hi[2], lo;
             uint4* to = (uint4*)(p.kept + fb_kept_at(row0 + lr, n, p.N));  // pieces are 64 of these apart
             fb_pack24(a, hi, lo);
@@ -565,7 +565,7 @@ fb_product_kernel(FbBatch<G> batch) {
     } else if constexpr (OT == O_DGATED) {
       // 64-byte pieces of dg and of du, each through 2 KB of LDS of the wave's own; the factors
       // of the next AHEAD units of 16 values are on their way while these are multiplied (8192
-      // tokens, 1024 by 2560, one unit ahead 100 us)
+      // tokens, 1024 by 2560: 82 us, one unit ahead 100; the product alone 35, the bytes 45)
       constexpr int AHEAD = TT * WT > 8 ? 2 : 3, UNITS = TT * WT;
       char* own = smem + C::LDS + wave * OWN;
       auto place = [&](int m, int r, int c) __attribute__((always_inline)) -> char* {

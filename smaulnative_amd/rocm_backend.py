@@ -746,7 +746,8 @@ class RocmBackend:
         """y [..., out_f] = Q(x) . W^T, W the weight that codes w [out_f, 128 n] and scales s
         stand for (``fp8_block_quantize``).  x [..., in_f] fp32 or bf16 is rounded to the
         format; with scales ``xs`` it is codes already.  ``dtype`` of y: fp32 or bf16, by
-        default x's, of codes bf16.  Products are exact, sums fp32."""
+        default x's, of codes bf16.  Products are exact, sums fp32; towards bf16, 8
+        neighbouring products may be summed with the last bit 2^-13 of the largest's."""
         lib = _lib.load()
         _need_one_device("fp8_block_forward", x, xs, w, s)
         if in_f < 1 or out_f < 1:
@@ -802,8 +803,9 @@ class RocmBackend:
 
         x [..., d] bf16, rounded to the format, or with scales ``xs`` codes already; weights:
         (gate_w, gate_s, up_w, up_s, down_w, down_s) in the format, [h, d], [h, d] and [d, h].
-        Sums are fp32, the hidden rows are rounded to codes from fp32.  With ``save`` returns
-        (y, saved), what ``fp8_block_ffn_backward`` takes."""
+        Sums are as ``fp8_block_forward``'s (gate's and up's of few rows fp32 throughout), the
+        hidden rows are rounded to codes from fp32.  With ``save`` returns (y, saved), what
+        ``fp8_block_ffn_backward`` takes; given codes are held there as they are."""
         lib = _lib.load()
         _need_one_device("fp8_block_ffn_forward", x, xs, *weights)
         weights = self._block_weights("fp8_block_ffn_forward", weights, d, h)
