@@ -1085,16 +1085,16 @@ __device__ __forceinline__ void fb_split3(const float (&v)[8], bf16x8_t (&t)[3])
   for (int k = 0; k < 3; ++k) t[k] = __builtin_bit_cast(bf16x8_t, make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]));
 }
 
-// The input gradient of few rows, in one launch: a workgroup has 32 columns of up to 64 rows,
+// The input gradient of few rows, in one launch: a workgroup has 32 CT columns of up to 64 rows,
 // its 8 waves a slice of the weight's rows each.  A lane reads 32 codes of one row, and the
 // wave turns 64 such rows round through LDS of its own, decoded to bf16.  The groups of rows
 // and the four workgroups that share a line of codes are neighbours in one XCD's band.  (1 row
 // 2560 -> 1024: 9 us, 21 by way of the turned weight.)
-template <bool BF16, int RT>
+template <bool BF16, int RT, int CT>
 __global__ void __launch_bounds__(512)
 fb_dx_stream_kernel(const void* __restrict__ grad, const uint8_t* __restrict__ w, const uint8_t* __restrict__ s,
                     void* __restrict__ dx, int64_t rows, int64_t I, int64_t O) {
-  constexpr int NW = 8, LD = 72, OWN = RT * 4096 > 32 * LD * 2 ? RT * 4096 : 32 * LD * 2, NT = BF16 ? 1 : 3;
+  constexpr int NW = 8, LD = 72, OWN = RT * 4096 > 32 * LD * 2 ? CT * RT * 4096 : CT * 32 * LD * 2, NT = BF16 ? 1 : 3;
   __shared__ __attribute__((aligned(16))) char smem[NW * OWN];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1104,26 +1104,32 @@ fb_dx_stream_kernel(const void* __restrict__ grad, const uint8_t* __restrict__ w
     if (b0 < full) b0 = b0 % 8 * (full / 8) + b0 / 8;
   }
   const int64_t groups = (rows + RT * 32 - 1) / (RT * 32), row0 = b0 % groups * (RT * 32);
-  const int64_t k0 = b0 / groups * 32, nb = fb_blocks(I), ns = (nb + 3) / 4 * 4;
+  const int64_t k0 = b0 / groups * (CT * 32), nb = fb_blocks(I), ns = (nb + 3) / 4 * 4;
   const int R = (int)min<int64_t>(rows - row0, RT * 32);
   const int64_t steps = (O + 63) / 64, per = (steps + NW - 1) / NW;
   const int64_t lo = min((int64_t)wave * per, steps), hi = min(lo + per, steps);
   uint16_t* own = (uint16_t*)(smem + wave * OWN);
-  f32x16_t acc[RT];
+  f32x16_t acc[CT][RT];
 #pragma unroll
-  for (int t = 0; t < RT; ++t)
+  for (int c = 0; c < CT; ++c)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) acc[t][r] = 0.0f;
-  uint4 c0, c1;
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[c][t][r] = 0.0f;
+  uint4 c0[CT], c1[CT];
   float sc;
   auto codes = [&](int64_t step) {  // rows past the last: zeros
     const int64_t o = step * 64 + lane;
-    c0 = c1 = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int c = 0; c < CT; ++c) c0[c] = c1[c] = make_uint4(0, 0, 0, 0);
     sc = 1.0f;
     if (o < O) {
       const uint4* at = (const uint4*)(w + o * nb * FB_BLOCK + k0);
-      c0 = at[0];
-      c1 = at[1];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        c0[c] = at[2 * c];
+        c1[c] = at[2 * c + 1];
+      }
       sc = fb_scale(s[o * ns + k0 / FB_BLOCK]);
     }
   };
@@ -1134,19 +1140,24 @@ fb_dx_stream_kernel(const void* __restrict__ grad, const uint8_t* __restrict__ w
     for (int t = 0; t < RT; ++t)
 #pragma unroll
       for (int q = 0; q < 4; ++q) fb_load8<BF16>(grad, row0 + min(t * 32 + l32, R - 1), O, step * 64 + q * 16 + g * 8, v[t][q]);
-    const uint32_t c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float f[4];
-      fb_decode4(c[j], sc, f);
+    for (int c = 0; c < CT; ++c) {
+      const uint32_t w8[8] = {c0[c].x, c0[c].y, c0[c].z, c0[c].w, c1[c].x, c1[c].y, c1[c].z, c1[c].w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) own[(4 * j + e) * LD + lane] = (uint16_t)(__float_as_uint(f[e]) >> 16);
+      for (int j = 0; j < 8; ++j) {
+        float f[4];
+        fb_decode4(w8[j], sc, f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) own[(c * 32 + 4 * j + e) * LD + lane] = (uint16_t)(__float_as_uint(f[e]) >> 16);
+      }
     }
     if (step + 1 < hi) codes(step + 1);
     __builtin_amdgcn_wave_barrier();  // a wave's LDS accesses are done in order
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const bf16x8_t a = *(const bf16x8_t*)&own[fb_perm(l32) * LD + q * 16 + g * 8];
+      bf16x8_t a[CT];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) a[c] = *(const bf16x8_t*)&own[(c * 32 + fb_perm(l32)) * LD + q * 16 + g * 8];
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
         bf16x8_t x[3];
@@ -1158,7 +1169,9 @@ fb_dx_stream_kernel(const void* __restrict__ grad, const uint8_t* __restrict__ w
           fb_split3(v[t][q], x);
         }
 #pragma unroll
-        for (int k = 0; k < NT; ++k) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, x[k], acc[t], 0, 0, 0);
+        for (int k = 0; k < NT; ++k)
+#pragma unroll
+          for (int c = 0; c < CT; ++c) acc[c][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[c], x[k], acc[c][t], 0, 0, 0);
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -1166,25 +1179,26 @@ fb_dx_stream_kernel(const void* __restrict__ grad, const uint8_t* __restrict__ w
   __syncthreads();
   float4* red = (float4*)smem;
 #pragma unroll
-  for (int t = 0; t < RT; ++t)
+  for (int t = 0; t < CT * RT; ++t)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      red[((wave * RT + t) * 4 + i) * 64 + lane] =
-          make_float4(acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]);
+    for (int i = 0; i < 4; ++i) {
+      const f32x16_t& v = acc[t / RT][t % RT];
+      red[((wave * CT * RT + t) * 4 + i) * 64 + lane] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    }
   __syncthreads();
-  for (int e = tid; e < RT * 256; e += 512) {
-    const int l = e & 63, i = e >> 6 & 3, t = e >> 8;
-    float4 a = red[(t * 4 + i) * 64 + l];
+  for (int e = tid; e < CT * RT * 256; e += 512) {
+    const int l = e & 63, i = e >> 6 & 3, ct = e >> 8, t = ct % RT;
+    float4 a = red[(ct * 4 + i) * 64 + l];
 #pragma unroll
     for (int q = 1; q < NW; ++q) {
-      const float4 b = red[((q * RT + t) * 4 + i) * 64 + l];
+      const float4 b = red[((q * CT * RT + ct) * 4 + i) * 64 + l];
       a.x += b.x;
       a.y += b.y;
       a.z += b.z;
       a.w += b.w;
     }
     const int row = t * 32 + (l & 31);
-    const int64_t n = k0 + (l >> 5) * 16 + i * 4;
+    const int64_t n = k0 + ct / RT * 32 + (l >> 5) * 16 + i * 4;
     const float f[4] = {a.x, a.y, a.z, a.w};
     if (row < R) {
 #pragma unroll
@@ -1427,13 +1441,20 @@ FfnBackParts ffn_back_parts(int64_t T, int64_t d, int64_t h, bool dx, bool dw) {
 // Whether fb_dx_stream_kernel has the call: of few rows, and of as many as one round of the
 // CUs takes in two steps a wave.  There the two launches (or three, in slices) wait for one
 // another longer than the weight's being turned by each group of rows takes (us, by way of
-// the turned weight and so: 512 x 777 -> 1000 fp32 22.5 and 13.4, 2048 x 256 -> 256 13.1 and
-// 8.7, 128 x 1024 -> 2560 bf16 13.4 and 9.5; past it 1001 x 777 -> 1000 fp32 26.3 and 24.2, bf16
-// 13.7 and 22.6).
-bool dx_streams(int64_t rows, int64_t in_f, int64_t out_f) {
-  if (rows <= FB_FEW) return true;
-  const int64_t wgs = (in_f + 31) / 32 * ((rows + 63) / 64);
-  return (wgs + cu_count() - 1) / cu_count() * (((out_f + 63) / 64 + 7) / 8) <= 2;
+// the turned weight and so: 512 x 777 -> 1000 fp32 22.5 and 13.5, 2048 x 256 -> 256 13.1 and
+// 8.8, 128 x 1024 -> 2560 bf16 13.4 and 9.5; past it 500 x 1024 -> 2560 bf16 14 and 25).  fp32
+// rows, whose thirds take longer than the weight, have 64 columns a workgroup where that makes
+// one round of two (1001 x 777 -> 1000 26.3, so 18.6, of 32 columns 24.2; bf16 13.7 and 15.8),
+// but 32 where these are one (512 rows 13.5 for 15.7).
+int64_t dx_groups(int64_t rows, int64_t in_f, int columns) { return (in_f + columns - 1) / columns * ((rows + 63) / 64); }
+bool dx_fits(int64_t rows, int64_t in_f, int64_t out_f, int columns) {
+  return (dx_groups(rows, in_f, columns) + cu_count() - 1) / cu_count() * (((out_f + 63) / 64 + 7) / 8) <= 2;
+}
+bool dx_wide(int64_t rows, int64_t in_f, int64_t out_f, bool f32) {
+  return f32 && rows > FB_FEW && !dx_fits(rows, in_f, out_f, 32) && dx_fits(rows, in_f, out_f, 64);
+}
+bool dx_streams(int64_t rows, int64_t in_f, int64_t out_f, bool f32) {
+  return rows <= FB_FEW || dx_fits(rows, in_f, out_f, 32) || dx_wide(rows, in_f, out_f, f32);
 }
 
 struct DxParts {
@@ -1444,7 +1465,7 @@ DxParts dx_parts(int64_t rows, int64_t in_f, int64_t out_f, int dtype) {
   DxParts q{};
   Parts w;
   const bool f32 = dtype == SMAUL_DTYPE_F32;
-  if (dx_streams(rows, in_f, out_f)) return q;
+  if (dx_streams(rows, in_f, out_f, f32)) return q;
   q.copies = f32 ? 3 : 1;
   q.ld = fb_stages(out_f) * 64 * q.copies;
   q.g = w.take(f32 || out_f % 64 ? rows * q.ld * 2 : 0);
@@ -1552,11 +1573,13 @@ int smaul_fp8_block_backward_input(const void* g, int dtype, const uint8_t* w, c
   const DxParts q = dx_parts(rows, in_f, out_f, dtype);
   char* ws = (char*)workspace;
   const bool bf16 = dtype == SMAUL_DTYPE_BF16;
-  if (dx_streams(rows, in_f, out_f)) {
-    const int64_t blocks = (in_f + 31) / 32 * ((rows + 63) / 64);
+  if (dx_streams(rows, in_f, out_f, !bf16)) {
+    const bool wide = dx_wide(rows, in_f, out_f, !bf16);
+    const int64_t blocks = dx_groups(rows, in_f, wide ? 64 : 32);
     if (!grid_fits(blocks, 512)) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block_backward_input: too wide a weight");
-    auto* kernel = bf16 ? (rows <= 32 ? &fb_dx_stream_kernel<true, 1> : &fb_dx_stream_kernel<true, 2>)
-                        : (rows <= 32 ? &fb_dx_stream_kernel<false, 1> : &fb_dx_stream_kernel<false, 2>);
+    auto* kernel = wide   ? &fb_dx_stream_kernel<false, 2, 2>
+                   : bf16 ? (rows <= 32 ? &fb_dx_stream_kernel<true, 1, 1> : &fb_dx_stream_kernel<true, 2, 1>)
+                          : (rows <= 32 ? &fb_dx_stream_kernel<false, 1, 1> : &fb_dx_stream_kernel<false, 2, 1>);
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(512), 0, stream, g, w, s, dx, rows, in_f, out_f);
     return check_launch("fb_dx_stream_kernel");
   }

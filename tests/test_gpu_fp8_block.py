@@ -171,7 +171,7 @@ def test_few_tiles_of_a_long_axis(rows, K, N):
 
 # a wave's steps and the rounds of workgroups on either side of what one launch has
 @pytest.mark.parametrize("rows,K,N", [(65, 513, 1024), (65, 513, 1025), (300, 131, 1101), (257, 64, 777), (1001, 1000, 777),
-                                      (520, 1000, 1000), (2100, 250, 500), (2100, 260, 520)])
+                                      (520, 1000, 1000), (2100, 250, 500), (2100, 260, 520), (900, 1090, 520), (1024, 1025, 512)])
 def test_backward_input_by_either_way(rows, K, N):
     g = gen(rows * K + N)
     w, s = ref.weight(N, K, g)
