@@ -634,8 +634,10 @@ fb_product_kernel(FbBatch<G> batch) {
       auto place = [&](int r, int c) __attribute__((always_inline)) -> char* {
         return own + r * RB + (c ^ (CH == 8 ? r & 7 : r / 2 & 3)) * 16;
       };
-      const bool whole = n0 + BN <= p.N && p.N % (16 / ES) == 0;  // of the whole workgroup
-      const uint32_t ldy = (uint32_t)p.N * ES;
+      // of the whole workgroup: its offsets are 32 bits, up to 31 rows and a piece of one
+      const int64_t row_bytes = p.N * ES;
+      const bool whole = n0 + BN <= p.N && p.N % (16 / ES) == 0 && row_bytes < 1LL << 27;
+      const uint32_t ldy = (uint32_t)row_bytes;
       const int left = rows - wm * (BM / WM);  // rows of this wave's
       char* out = (char*)p.y + (part + (row0 + wm * (BM / WM)) * p.N + n0 + wn * (BN / WN)) * ES;
       uint4 d0, d1, d2, d3;
@@ -686,7 +688,7 @@ fb_product_kernel(FbBatch<G> batch) {
             __builtin_amdgcn_wave_barrier();
           }
         });
-      } else {  // rows of any alignment, the last columns one by one
+      } else {  // rows of any alignment and width, the last columns one by one
         fb_each<UNITS>([&](auto unit) __attribute__((always_inline)) {
           constexpr int u = unit, c0 = u % (WT / UJ) * (RB / ES);
           to_lds(u / (WT / UJ), u % (WT / UJ) * UJ);
@@ -695,7 +697,7 @@ fb_product_kernel(FbBatch<G> batch) {
           for (int h = 0; h < CH / 2; ++h) {
             const int tr = h * (64 / CH) + el / CH, r = u / (WT / UJ) * 32 + tr;
             const char* v = place(tr, el % CH);
-            char* at = out + (int64_t)r * ldy + (c0 + el % CH * (16 / ES)) * ES;
+            char* at = out + r * row_bytes + (c0 + el % CH * (16 / ES)) * ES;
             if (r >= left) continue;
             if (n >= 16 / ES) {
               const uint4 w = *(const uint4*)v;

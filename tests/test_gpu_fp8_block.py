@@ -188,3 +188,48 @@ def test_backward_input_by_either_way(rows, K, N):
         assert not torch.isfinite(dx[[1, rows - 1, rows // 2]]).any()
         dx[[1, rows - 1, rows // 2]] = 0
         assert torch.equal(dx, bad)
+
+
+def room(bytes_):
+    free = torch.cuda.mem_get_info()[0]
+    if free < bytes_:
+        pytest.skip(f"needs {bytes_ >> 30} GiB of device memory, {free >> 30} are free")
+
+
+def repeats(y, y0):
+    """Whether y's columns are y0's, over and over."""
+    P = y0.shape[1]
+    return all(torch.equal(y[:, k:k + P], y0[:, :y.shape[1] - k]) for k in range(0, y.shape[1], P))
+
+
+# 31 rows of the result pass 32 bits of bytes, whole vectors a row
+@pytest.mark.parametrize("dtype,N", [(F32, 44739248), (BF, 89478488)])
+def test_forward_of_very_wide_results(dtype, N):
+    """Columns repeat with a period that no tile has, and are the narrow product's."""
+    room(40 << 30)
+    K, P, rows = 100, 60011, 70
+    w0, s0 = ref.weight(P, K, gen(3))
+    w0, s0 = w0.to(DEV), s0.to(DEV)
+    x = torch.randn(rows, K, generator=gen(4)).to(dtype).to(DEV)
+    y0 = be().fp8_block_forward(x, w0, s0, K, P)
+    at = torch.randint(0, P, (50,), generator=gen(5))
+    wv = ref.values(w0[at.to(DEV)].cpu(), s0[at.to(DEV)].cpu(), K)
+    ref.check(y0[:, at.to(DEV)], *ref.product(ref.rounded(x.cpu()), wv, dtype, codes=True), (dtype, N))
+    w, s = (t.repeat(-(-N // P), 1)[:N] for t in (w0, s0))
+    assert repeats(be().fp8_block_forward(x, w, s, K, N), y0)
+
+
+@pytest.mark.parametrize("dtype,K", [(F32, 44739248), (BF, 89478488)])
+def test_backward_input_of_very_wide_results(dtype, K):
+    room(80 << 30)
+    N, P, rows = 20, 60416, 70  # the scales repeat with the codes: a period of whole words of them
+    w0, s0 = ref.weight(N, P, gen(6))
+    w, s = w0.to(DEV).repeat(1, -(-K // P)), s0.to(DEV).repeat(1, -(-K // P))
+    n = ref.blocks(K)
+    w, s = w[:, :128 * n].contiguous(), s[:, :(n + 3) // 4 * 4].contiguous()
+    w[:, K:], s[:, n:] = 0, 0
+    g = torch.randn(rows, N, generator=gen(7)).to(dtype)
+    dx0 = be().fp8_block_backward_input(g.to(DEV), w0.to(DEV), s0.to(DEV), P, N)
+    wv = ref.values(w0, s0, P)[:, :1000].t().contiguous()
+    ref.check(dx0[:, :1000], *ref.product(g.double(), wv, dtype), (dtype, K))
+    assert repeats(be().fp8_block_backward_input(g.to(DEV), w, s, K, N), dx0)
