@@ -65,6 +65,15 @@ def _rows(x):
     return x if x.dtype in (torch.float32, torch.bfloat16) else x.float()
 
 
+def _addends(x, residual):
+    """x and residual in one type that the norm reads, and the type of their sum."""
+    total = x.dtype if residual is None else torch.promote_types(x.dtype, residual.dtype)
+    if not total.is_floating_point:
+        total = torch.float32
+    kind = total if total in (torch.float32, torch.bfloat16) else torch.float32
+    return x.to(kind), None if residual is None else residual.to(kind), total
+
+
 def _check_leaves(*leaves):
     """Refuses to record a pass under capture while a pass recorded outside holds one of its
     leaves: autograd orders the leaf's accumulation by the stream of the pass that first
@@ -170,7 +179,10 @@ class _AddRMSNorm(torch.autograd.Function):
 
 
 class AddRMSNorm(nn.Module):
-    """(y, s): s = x + residual (x without one), y = RMSNorm(s) in x's type, one device pass."""
+    """(y, s): s = x + residual (x without one), y = RMSNorm(s) in x's type, one device pass.
+
+    Rows of another type than fp32 or bf16 and addends of two types are cast first, s is in the
+    type of their sum (which y is formed from in fp32 then, not rounded) and gradients in their own."""
 
     def __init__(self, d, eps=1e-6):
         super().__init__()
@@ -183,9 +195,10 @@ class AddRMSNorm(nn.Module):
 
     def forward(self, x, residual=None):
         nodes = _check_leaves(x, residual, self.weight)
-        y = _AddRMSNorm.apply(x, residual, self.weight, self.eps)
+        a, b, total = _addends(x, residual)
+        y, s = _AddRMSNorm.apply(a, b, self.weight, self.eps)
         del nodes
-        return y
+        return y.to(x.dtype if x.is_floating_point() else total), s.to(total)
 
     def extra_repr(self):
         return f"d={self.weight.numel()}, eps={self.eps}"
@@ -286,9 +299,12 @@ class FP8BlockFFN(nn.Module):
         # a recorded pass keeps what its gradients need
         need = torch.is_grad_enabled() and any(t is not None and t.requires_grad
                                                for t in (x, residual, norm_weight, *weights))
-        y = _FFN.apply(x, residual, norm_weight, eps, self.d, self.h, self.trainable, need, *weights)
+        a, b, total = (x, None, None) if eps is None else _addends(x, residual)
+        y = _FFN.apply(a, b, norm_weight, eps, self.d, self.h, self.trainable, need, *weights)
         del nodes
-        return y
+        if eps is None:
+            return y
+        return y[0].to(x.dtype if x.is_floating_point() else total), y[1].to(total)
 
     def forward(self, x):
         return self._apply_block(x, None, None, None)
@@ -299,7 +315,7 @@ class FP8BlockFFN(nn.Module):
 
 class FP8BlockNormFFN(FP8BlockFFN):
     """(y, s): s = x + residual (x without one), y = the block on RMSNorm(s), whose codes
-    the norm writes itself (rounded once, from fp32)."""
+    the norm writes itself (rounded once, from fp32).  Types as ``AddRMSNorm``'s."""
 
     def __init__(self, d, h, trainable=False, eps=1e-6):
         super().__init__(d, h, trainable)

@@ -191,6 +191,72 @@ def test_norm_layer(dtype, residual):
         assert torch.equal(r.grad, x.grad)
 
 
+F16 = torch.float16
+STEP = {F32: (ref.U, 2.0 ** -149), BF: (2.0 ** -8, 2.0 ** -133), F16: (2.0 ** -11, 2.0 ** -25), torch.float64: (0.0, 0.0)}
+# x's type, the residual's, the sum's
+TYPES = [(F16, None, F16), (F16, F16, F16), (BF, F32, F32), (F32, BF, F32), (F16, BF, F32), (BF, F16, F32),
+         (torch.float64, torch.float64, torch.float64)]
+
+
+def typed(T, d, xt, rt, seed):
+    """x, the residual (or None) as leaves, and gradients of the outputs, which the sum's type holds."""
+    torch.manual_seed(seed)
+    x = torch.randn(T, d).to(xt).to(DEV).requires_grad_()
+    r = None if rt is None else torch.randn(T, d).to(rt).to(DEV).requires_grad_()
+    return x, r, torch.randn(T, d).to(xt).to(DEV), torch.randn(T, d).to(BF).to(DEV)
+
+
+@pytest.mark.parametrize("xt,rt,total", TYPES)
+def test_norm_layer_of_other_types(xt, rt, total):
+    """Computed in fp32 on fp32 addends, each output and gradient rounded to its own type once more."""
+    T, d = 50, 300
+    m = AddRMSNorm(d, 1e-5).to(DEV)
+    x, r, dy, ds = typed(T, d, xt, rt, 4)
+    y, s = m(x, r)
+    assert y.dtype == xt and s.dtype == total
+    torch.autograd.backward([y, s], [dy, ds.to(total)])
+    sv = x.detach().cpu().float()
+    if r is not None:
+        sv = sv + r.detach().cpu().float()
+    assert torch.equal(s.detach().cpu(), sv.to(total))
+
+    def again(v, e, dtype):  # rounded to fp32, then to dtype
+        half, least = STEP[dtype]
+        e = e + ref.U * (v.abs() + e)
+        return v, e + half * (v.abs() + e) + least
+
+    w = torch.ones(d).double()
+    ref.check(y, *again(*ref.norm(sv.double(), w, 1e-5), xt))
+    (dx, dxe), (dw, dwe) = ref.norm_grad(dy.cpu().double(), sv.double(), w, 1e-5, ds.cpu().double(), F32)
+    ref.check(m.weight.grad, dw, dwe)
+    for leaf, dtype in ((x, xt), (r, rt)):
+        if leaf is not None:
+            assert leaf.grad.dtype == dtype
+            ref.check(leaf.grad, *again(dx, dxe, dtype))
+
+
+@pytest.mark.parametrize("xt,rt,total", TYPES)
+@pytest.mark.parametrize("T", [7, 130])
+def test_norm_block_layer_of_other_types(T, xt, rt, total):
+    """As the layer on fp32 addends."""
+    torch.manual_seed(T)
+    d, h = 136, 300
+    m = FP8BlockNormFFN(d, h, True).to(DEV)
+    x, r, dy, ds = typed(T, d, xt, rt, T)
+    y, s = m(x, r)
+    assert y.dtype == xt and s.dtype == total
+    torch.autograd.backward([y, s], [dy, ds.to(total)])
+    grads = [p.grad for p in m.parameters()]
+    m.zero_grad(set_to_none=True)
+    x2, r2 = (t if t is None else t.detach().float().requires_grad_() for t in (x, r))
+    y2, s2 = m(x2, r2)
+    torch.autograd.backward([y2, s2], [dy.float(), ds.float()])
+    assert torch.equal(y, y2.to(xt)) and torch.equal(s, s2.to(total))
+    assert all(torch.equal(a, p.grad) for a, p in zip(grads, m.parameters()))
+    for a, b in ((x, x2), (r, r2)):
+        assert a is None or (a.grad.dtype == a.dtype and torch.equal(a.grad, b.grad.to(a.dtype)))
+
+
 def _module_weights(m):
     if m.trainable:
         return [ref.rounded(t.detach().cpu().float()) for t in (m.gate, m.up, m.down)]
