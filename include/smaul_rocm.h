@@ -655,8 +655,8 @@ int smaul_fp8_block_ffn_backward(const void* dy, const uint8_t* gate_w, const ui
 
 /*
  * sum = x + residual (rounded to dtype; residual NULL: sum is x, and not written), and out
- * = sum / sqrt(mean(sum^2) + eps) * weight (fp32 [d], NULL: ones), computed in fp32:
- * rounded to dtype, or with scales not NULL to codes and scales of the format above
+ * = sum / sqrt(mean(sum^2) + eps) * weight (fp32 [d], NULL: ones), the mean and the root
+ * in fp64, the rest in fp32: rounded to dtype, or with scales not NULL to codes and scales of the format above
  * (out 8-byte aligned).  Outputs do not overlap inputs.
  */
 int smaul_add_rms_norm(const void* x, const void* residual, int dtype, const float* weight, float eps, void* sum,
@@ -664,8 +664,8 @@ int smaul_add_rms_norm(const void* x, const void* residual, int dtype, const flo
 
 /*
  * Its gradients from out's, dy, and sum's, ds (or NULL): dx[T, d] of dtype, which is
- * residual's too, and dw fp32 [d] (NULL: none).  s is the sum.  Straight through the
- * rounding of out.  The workspace 256-byte aligned.
+ * residual's too, and dw fp32 [d] (NULL: none).  s is the sum.  A row's two sums are in
+ * fp64, dw's in fp32.  Straight through the rounding of out.  The workspace 256-byte aligned.
  */
 int64_t smaul_add_rms_norm_backward_workspace_size(int64_t T, int64_t d);
 int smaul_add_rms_norm_backward(const void* dy, const void* s, const void* ds, int dtype, const float* weight,

@@ -37,10 +37,28 @@ __device__ __forceinline__ double inv_root(double m) {
   return r * (1.5 - 0.5 * m * r * r);
 }
 
-__device__ __forceinline__ float sum_squares(const float (&v)[8]) {
-  float a = 0.0f;
+// A row's 1 / rms as r k, k the power of two with which values of the largest rows stay in
+// the middle of fp32: k v r is v / rms, and neither k v nor r is subnormal or overflows.
+struct Root {
+  double r;
+  float k;
+};
+__device__ __forceinline__ Root row_root(double ss, int64_t d, float eps) {
+  const double r = inv_root(ss / (double)d + (double)eps);
+  return r < 1e-30 ? Root{r * 0x1p64, 0x1p-64f} : Root{r, 1.0f};
+}
+
+// of 8 values, in 64 bits
+__device__ __forceinline__ double sum_squares(const float (&v)[8]) {
+  double a = 0.0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) a = fmaf(v[j], v[j], a);
+  for (int j = 0; j < 8; ++j) a = fma((double)v[j], (double)v[j], a);
+  return a;
+}
+__device__ __forceinline__ double sum_products(const float (&w)[8], const float (&g)[8], const float (&v)[8]) {
+  double a = 0.0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a = fma((double)(w[j] * g[j]), (double)v[j], a);
   return a;
 }
 
@@ -48,10 +66,10 @@ __device__ __forceinline__ float sum_squares(const float (&v)[8]) {
 // registers (the rest are read again).  Memory bounds it: 32768 x 2048 bf16 to codes 93 us, 5.1
 // TB/s.
 //
-// 8 values' squares are summed in 32 bits, the rest of the sum and the root in 64, and the
-// two products with 1 / rms and the weight carry their errors along (1 / rms as two
-// floats): y is off by little more than its own rounding, so that a code is seldom the
-// neighbouring one of what 64 bits give (in 32 bits throughout about one in 250000).
+// The squares, their sum and the root are in 64 bits (in 32, rows past 1.8e19 would overflow;
+// 2 us of the 93), and the two products with 1 / rms and the weight carry their errors along
+// (1 / rms as two floats): y is off by little more than its own rounding, so that a code is
+// seldom the neighbouring one of what 64 bits give (in 32 bits throughout about one in 250000).
 template <bool BF16, bool CODES, bool NT, int NW, int CH>
 __global__ void __launch_bounds__(256)
 add_rms_norm_kernel(const void* __restrict__ x, const void* __restrict__ r, const float* __restrict__ weight,
@@ -82,7 +100,7 @@ add_rms_norm_kernel(const void* __restrict__ x, const void* __restrict__ r, cons
   for (int i = 0; i < CH; ++i) {
     add(chunk(i) * 8, keep[i], extra[i]);
     if (r && chunk(i) * 8 < d) fb_store8<BF16, NT>(sum, t, d, chunk(i) * 8, keep[i]);
-    ss += (double)sum_squares(keep[i]);
+    ss += sum_squares(keep[i]);
   }
   for (int i = CH; chunk(i) - lane < chunks; ++i) {
     float v[8], q[8];
@@ -90,10 +108,10 @@ add_rms_norm_kernel(const void* __restrict__ x, const void* __restrict__ r, cons
     if (r) fb_load8<BF16, NT>(r, t, d, chunk(i) * 8, q);
     add(chunk(i) * 8, v, q);
     if (r && chunk(i) * 8 < d) fb_store8<BF16, NT>(sum, t, d, chunk(i) * 8, v);
-    ss += (double)sum_squares(v);
+    ss += sum_squares(v);
   }
-  const double root = inv_root(row_sum<NW>(ss, red, wave) / (double)d + (double)eps);
-  const float rh = (float)root, rl = (float)(root - (double)rh);
+  const Root root = row_root(row_sum<NW>(ss, red, wave), d, eps);
+  const float rh = (float)root.r, rl = (float)(root.r - (double)rh);
   auto put = [&](int64_t c, float (&v)[8]) {  // whole blocks of lanes
     if (c >= chunks * 8) return;
     float w[8];
@@ -102,7 +120,7 @@ add_rms_norm_kernel(const void* __restrict__ x, const void* __restrict__ r, cons
     if (weight) fb_load8<false>(weight, 0, d, c, w);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float a = v[j] * rh, ae = fmaf(v[j], rl, fmaf(v[j], rh, -a));
+      const float u = v[j] * root.k, a = u * rh, ae = fmaf(u, rl, fmaf(u, rh, -a));
       const float y = a * w[j], ye = fmaf(ae, w[j], fmaf(a, w[j], -y)), z = y + ye;
       v[j] = z == z ? z : y;  // an infinity has no error to carry
     }
@@ -166,11 +184,8 @@ add_rms_norm_backward_kernel(const void* __restrict__ dy, const void* __restrict
     double ss = 0.0, sd = 0.0;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      float a = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) a = fmaf(w[i][j] * g[i][j], v[i][j], a);
-      ss += (double)sum_squares(v[i]);
-      sd += (double)a;
+      ss += sum_squares(v[i]);
+      sd += sum_products(w[i], g[i], v[i]);
     }
 #pragma unroll
     for (int q = 32; q >= 1; q >>= 1) {
@@ -191,14 +206,15 @@ add_rms_norm_backward_kernel(const void* __restrict__ dy, const void* __restrict
       }
     }
     if (t >= T) continue;  // a last row that is not there
-    const double root = inv_root(ss / (double)d + (double)eps);
-    const float rstd = (float)root, dot = (float)(sd / (double)d * root * root);
+    const Root root = row_root(ss, d, eps);
+    const float rstd = (float)root.r, dot = (float)(sd / (double)d * root.r * root.r * (double)root.k);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        acc[i][j] = fmaf(g[i][j], v[i][j] * rstd, acc[i][j]);
-        o[i][j] += (w[i][j] * g[i][j] - v[i][j] * dot) * rstd;
+        const float u = v[i][j] * root.k;
+        acc[i][j] = fmaf(g[i][j], u * rstd, acc[i][j]);
+        o[i][j] += (w[i][j] * g[i][j] - u * dot) * rstd * root.k;
       }
       if (col(i) < d) fb_store8<BF16>(dx, t, d, col(i), o[i]);
     }
@@ -255,19 +271,18 @@ add_rms_norm_backward_wide_kernel(const void* __restrict__ dy, const void* __res
     for (int64_t t = blockIdx.x; t < T; t += gridDim.x) {
       double ss = 0.0, sd = 0.0;
       for (int64_t c = threadIdx.x; c < chunks; c += 256) {
-        float v[8], g[8], w[8], a = 0.0f;
+        float v[8], g[8], w[8];
         fb_load8<BF16>(s, t, d, c * 8, v);
         fb_load8<BF16>(dy, t, d, c * 8, g);
 #pragma unroll
         for (int j = 0; j < 8; ++j) w[j] = 1.0f;
         if (weight) fb_load8<false>(weight, 0, d, c * 8, w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) a = fmaf(w[j] * g[j], v[j], a);
-        ss += (double)sum_squares(v);
-        sd += (double)a;
+        ss += sum_squares(v);
+        sd += sum_products(w, g, v);
       }
-      const double root = inv_root(row_sum<4>(ss, red, wave) / (double)d + (double)eps);
-      const float rstd = (float)root, dot = (float)(row_sum<4>(sd, red, wave) / (double)d * root * root);
+      const Root root = row_root(row_sum<4>(ss, red, wave), d, eps);
+      const float rstd = (float)root.r;
+      const float dot = (float)(row_sum<4>(sd, red, wave) / (double)d * root.r * root.r * (double)root.k);
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int64_t c = c0 + i * 256 + threadIdx.x;
@@ -276,7 +291,7 @@ add_rms_norm_backward_wide_kernel(const void* __restrict__ dy, const void* __res
           fb_load8<BF16>(s, t, d, c * 8, v);
           fb_load8<BF16>(dy, t, d, c * 8, g);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(g[j], v[j] * rstd, acc[i][j]);
+          for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(g[j], v[j] * root.k * rstd, acc[i][j]);
         }
       }
       for (int64_t c = threadIdx.x; c0 == 0 && c < chunks; c += 256) {
@@ -291,7 +306,7 @@ add_rms_norm_backward_wide_kernel(const void* __restrict__ dy, const void* __res
         if (weight) fb_load8<false>(weight, 0, d, c * 8, w);
         if (ds) fb_load8<BF16>(ds, t, d, c * 8, o);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] += (w[j] * g[j] - v[j] * dot) * rstd;
+        for (int j = 0; j < 8; ++j) o[j] += (w[j] * g[j] - v[j] * root.k * dot) * rstd * root.k;
         fb_store8<BF16>(dx, t, d, c * 8, o);
       }
     }

@@ -120,3 +120,36 @@ def test_layouts_and_empty_calls():
     assert dx.shape == (0, 200) and dw.shape == (200,) and not dw.any()
     same, z = be().add_rms_norm(dev[0])
     assert same is dev[0] and torch.equal(z, be().add_rms_norm(dev[0], None, torch.ones(200, device=DEV), 1e-6)[1])
+
+
+# each width's form; few rows and more than the chip has CUs
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T,d", [(20, 64), (300, 300), (20, 900), (300, 1500), (20, 3000), (20, 5000), (20, 9001)])
+def test_very_large_and_small_rows(T, d, dtype):
+    """Finite rows whose squares, or products with a gradient, fp32 does not hold; and ordinary rows
+    with one such value.  The bounds of ordinary rows, and two steps of the type's least value where
+    results are that small (a product and its scaling back)."""
+    g = torch.Generator().manual_seed(d)
+    scales = (2e37, 1e36, 1e34, 1e30, 1e25, 1e20, 3e19, 1e18, 1.0, 1e-18, 1e-20, 1e-25)
+    rows = torch.tensor(scales, dtype=torch.float64).repeat(-(-T // 12))[:T, None]
+    x, r, dy, ds = ((torch.randn(T, d, generator=g).double() * rows).to(dtype) if i < 2 else
+                    torch.randn(T, d, generator=g).to(dtype) for i in range(4))
+    x[8, d // 2], x[9, d - 1], x[10, 0] = 1e25, -3e38, 1e20
+    dy = (dy.double() * torch.where(rows > 1e15, 1e15, 1.0)).to(dtype)
+    w = 1 + 0.3 * torch.randn(d, generator=g)
+    wd = w.double()
+    s = (x.float() + r.float()).to(dtype)
+    least = {BF: 2.0 ** -133, F32: 2.0 ** -149}[dtype]
+    assert torch.isfinite(s).all()
+    dev = [t.to(DEV) for t in (x, r, w, dy, ds)]
+    y, e = ref.norm(s.double(), wd, EPS)
+    got_s, got = be().add_rms_norm(*dev[:3], EPS)
+    assert torch.equal(got_s.cpu(), s)
+    ref.check(got, y, e + ref.HALF[dtype] * (y.abs() + e) + 2 * least, (T, d, dtype))
+    _, c, cs = be().add_rms_norm(*dev[:3], EPS, quantize=True)
+    ref.check(ref.values(c.cpu(), cs.cpu(), d), ref.rounded(y), ref.moved(y, e + 2.0 ** -148), (T, d, dtype))
+    for extra in (ds, None):
+        (dx, dxe), (dw, dwe) = ref.norm_grad(dy.double(), s.double(), wd, EPS, None if extra is None else extra.double(), dtype)
+        got, gw = be().add_rms_norm_backward(dev[3], got_s, dev[2], EPS, ds=None if extra is None else dev[4])
+        ref.check(got, dx, dxe + 2 * least, (T, d, dtype))
+        ref.check(gw, dw, dwe, (T, d, dtype))
