@@ -164,6 +164,18 @@ struct FbCfg {
                 "whole DMA instructions");
 };
 
+// ... and its kernel: a wave's part of LDS for the rows that leave (2 KB where two workgroups
+// share a CU for it), the hidden rows' maxima.  PAIRED: two workgroups a CU.
+template <int FMT, int OT, int BM, int BN, int WM, int WN, int NS>
+struct FbProduct : FbCfg<FMT, BM, BN, WM, WN, NS> {
+  using C = FbCfg<FMT, BM, BN, WM, WN, NS>;
+  static constexpr bool GATED = OT == O_GATED || OT == O_GATED_EXACT, EXACT = OT == O_F32 || OT == O_GATED_EXACT;
+  static constexpr bool SMALL = NS == 2 && BM * BN <= 128 * 128;
+  static constexpr int OWN = GATED ? 0 : OT == O_BF16 && SMALL ? 2048 : 4096, AMAX = GATED ? BM * WN * 4 : 0;
+  static constexpr int SMEM = C::LDS + C::NW * OWN + AMAX;
+  static constexpr bool PAIRED = SMALL && 2 * SMEM <= 160 * 1024;
+};
+
 __device__ __forceinline__ int fb_perm(int i) { return ((i >> 2) & 1) * 16 + (i >> 3) * 4 + (i & 3); }
 
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
@@ -220,15 +232,13 @@ struct FbBatch {
   FbArgs p[G];
 };
 template <int FMT, int OT, int BM, int BN, int WM, int WN, int NS, int G>
-__global__ void __launch_bounds__(WM * WN * 64, NS > 2 || BM * BN > 128 * 128 || BN > 128 || OT == O_F32 ? 1 : 2)
+__global__ void __launch_bounds__(WM * WN * 64, (FbProduct<FMT, OT, BM, BN, WM, WN, NS>::PAIRED ? 2 : 1))
 fb_product_kernel(FbBatch<G> batch) {
-  using C = FbCfg<FMT, BM, BN, WM, WN, NS>;
-  constexpr bool GATED = OT == O_GATED || OT == O_GATED_EXACT, EXACT = OT == O_F32 || OT == O_GATED_EXACT;
-  constexpr int TT = C::TT, WT = C::WT, BNO = GATED ? BN / 2 : BN, NW = C::NW;
-  // a wave's part of LDS for the rows that leave: 2 KB where two workgroups share a CU
-  constexpr int OWN = GATED ? 0 : OT == O_BF16 && NS == 2 && BM * BN <= 128 * 128 ? 2048 : 4096, AMAX = GATED ? BM * WN * 4 : 0;
+  using C = FbProduct<FMT, OT, BM, BN, WM, WN, NS>;
+  constexpr bool GATED = C::GATED, EXACT = C::EXACT;
+  constexpr int TT = C::TT, WT = C::WT, BNO = GATED ? BN / 2 : BN, NW = C::NW, OWN = C::OWN;
   static_assert(!GATED || BNO == FB_BLOCK, "a tile of hidden rows is a block");
-  __shared__ __attribute__((aligned(1024))) char smem[C::LDS + NW * OWN + AMAX];
+  __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN, g = lane >> 5, l32 = lane & 31;
@@ -733,20 +743,23 @@ int launch_product_cfg(const FbBatch<G>& b, hipStream_t stream) {
   if ((BM > BN ? BM : BN) * b.p[0].ldx >= 1LL << 32)
     return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block product: rows too wide");
   if (tiles > 2147483647LL) return fail(SMAUL_ERR_UNSUPPORTED, "fp8_block product: too many tiles");
-  const int64_t wgs = cu_count() * (NS == 2 && BM * BN <= 128 * 128 ? 2 : 1);
+  const int64_t wgs = cu_count() * (FbProduct<FMT, OT, BM, BN, WM, WN, NS>::PAIRED ? 2 : 1);
   hipLaunchKernelGGL((fb_product_kernel<FMT, OT, BM, BN, WM, WN, NS, G>), dim3((unsigned)(tiles < wgs ? tiles : wgs)),
                      dim3(WM * WN * 64), 0, stream, b);
   return check_launch("fb_product_kernel");
 }
 
 // Tiles that fill the chip, by the rounds they take: what a stage of a round of the CUs
-// takes and what the rest of its tiles does (10 ns), times the rounds.  The smaller tiles
-// run two a CU, in rounds of twice the CUs, a last round of no more than one a CU in `one`;
-// a last round that leaves CUs idle has a higher clock, up to 1.7 times.
+// takes and what the rest of its tiles does (10 ns), times the rounds.  The 128 x 128 tile
+// mostly runs two a CU, in rounds of twice the CUs, a last round of no more than one a CU in
+// `one`; a last round that leaves CUs idle has a higher clock, up to 1.7 times.
 struct FbTile {
   int bm, bn, one, two, rest;  // two: 0 where a CU takes them one by one
 };
 constexpr FbTile ROW_TILES[] = {{256, 256, 153, 0, 490}, {128, 256, 85, 0, 300}, {128, 128, 52, 105, 160}, {64, 128, 37, 0, 150}};
+// decoded codes (fp32 results): 128 values a stage at the bf16 rate, and scales and fp32 rows
+// together leave LDS for one workgroup only
+constexpr FbTile EXACT_TILES[] = {{256, 256, 275, 0, 650}, {128, 256, 160, 0, 300}, {128, 128, 101, 0, 200}, {64, 128, 70, 0, 100}};
 constexpr FbTile DGATED_TILES[] = {{256, 256, 153, 0, 1400}, {128, 256, 85, 0, 800}, {128, 128, 52, 105, 500}, {64, 128, 37, 0, 300}};
 constexpr FbTile GATED_TILES[] = {{256, 256, 153, 0, 900}, {128, 256, 85, 0, 500}, {64, 256, 60, 0, 300}};
 
@@ -784,7 +797,9 @@ int launch_products(const FbBatch<G>& b, hipStream_t stream) {
       default: return launch_product_cfg<FMT, OT, 64, 256, 1, 4, 3>(b, stream);
     }
   } else {
-    switch (OT == O_DGATED ? pick_tile(DGATED_TILES, b, false) : pick_tile(ROW_TILES, b, false)) {
+    constexpr auto& tiles = OT == O_DGATED ? DGATED_TILES : FMT == F_CODES && OT == O_F32 ? EXACT_TILES : ROW_TILES;
+    static_assert(FbProduct<FMT, OT, 128, 128, 2, 2, 2>::PAIRED == (tiles[2].two > 0), "rounds as the CUs take them");
+    switch (pick_tile(tiles, b, false)) {
       case 0: return launch_product_cfg<FMT, OT, 256, 256, 2, 2, 2>(b, stream);
       case 1: return launch_product_cfg<FMT, OT, 128, 256, 2, 2, 2>(b, stream);
       case 2: return launch_product_cfg<FMT, OT, 128, 128, 2, 2, 2>(b, stream);

@@ -99,6 +99,20 @@ def test_forward(rows, K, N):
     assert be().fp8_block_forward(c.to(DEV), wd, sd, K, N, xs=cs.to(DEV)).dtype == BF
 
 
+# a size for each tile of products with fp32 results, ragged in rows, columns and K
+@pytest.mark.parametrize("rows,K,N", [(600, 130, 1000), (3001, 300, 2602), (1473, 233, 4821), (7108, 290, 1843)])
+def test_forward_of_many_rows_in_fp32(rows, K, N):
+    g = gen(rows)
+    w, s = ref.weight(N, K, g)
+    x = torch.randn(rows, K, generator=g)
+    y = be().fp8_block_forward(x.to(DEV), w.to(DEV), s.to(DEV), K, N).cpu()
+    at = torch.cat([torch.tensor([0, 63, 64, 255, 256, rows - 1]), torch.randperm(rows, generator=g)[:300]])
+    ref.check(y[at], *ref.product(ref.rounded(x[at]), ref.values(w, s, K), F32), (rows, K, N))
+    few = be().fp8_block_forward(x[:50].to(DEV), w.to(DEV), s.to(DEV), K, N).cpu()
+    bound = 2 * ref.product(ref.rounded(x[:50]), ref.values(w, s, K), F32)[1]
+    assert bool(((y[:50].double() - few.double()).abs() <= bound).all())
+
+
 def test_forward_layouts_and_leading_dimensions():
     K, N = 200, 96
     g = gen(1)
