@@ -601,9 +601,9 @@ int smaul_fp8_block_dequantize(const uint8_t* codes, const uint8_t* scales, void
  * y[rows, out_f] = Q(x)[rows, in_f] . decode(w, s)^T, w and s [out_f, in_f] in that format,
  * y of y_dtype (f32 or bf16).  x: rows of x_dtype f32 or bf16, rounded to the format in the
  * workspace, or with x_dtype SMAUL_DTYPE_FP8_BLOCK codes with scales xs.  Products are
- * exact, sums fp32; towards a y of bf16, 8 neighbouring products may be summed with the last
- * bit 2^-13 of the largest's power of two.  x, y and w 16-byte aligned, scales 4, the
- * workspace 256.
+ * exact, sums fp32; towards a y of bf16, from 33 rows on, 8 neighbouring products may be
+ * summed with the last bit 2^-13 of the largest's power of two.  x, y and w 16-byte
+ * aligned, scales 4, the workspace 256.
  */
 enum { SMAUL_DTYPE_FP8_BLOCK = 2 };
 int64_t smaul_fp8_block_linear_workspace_size(int64_t rows, int64_t in_f, int64_t out_f, int x_dtype);
@@ -656,8 +656,8 @@ int smaul_fp8_block_ffn_backward(const void* dy, const uint8_t* gate_w, const ui
 /*
  * sum = x + residual (rounded to dtype; residual NULL: sum is x, and not written), and out
  * = sum / sqrt(mean(sum^2) + eps) * weight (fp32 [d], NULL: ones), the mean and the root
- * in fp64, the rest in fp32: rounded to dtype, or with scales not NULL to codes and scales of the format above
- * (out 8-byte aligned).  Outputs do not overlap inputs.
+ * in fp64, the rest in fp32: rounded to dtype, or with scales not NULL to codes and scales
+ * of the format above (out 8-byte aligned).  Outputs do not overlap inputs.
  */
 int smaul_add_rms_norm(const void* x, const void* residual, int dtype, const float* weight, float eps, void* sum,
                        void* out, uint8_t* scales, int64_t T, int64_t d, hipStream_t stream);

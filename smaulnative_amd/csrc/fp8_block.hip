@@ -930,6 +930,10 @@ __device__ __forceinline__ void fb_round64(const void* x, int64_t row, int64_t K
 // 5.2, 64 x 2560 -> 1024 10.3 and 8.7).  RT: tiles of 32 rows of x.  Hidden values leave in fp32 (O_GATED): a block of their
 // codes would take 256 rows of weights a workgroup, whose bytes one CU waits for longer than
 // another launch takes (1 token, 1024 by 2560: 11 us for 4.5 and 2).
+// Codes are decoded and multiplied as bf16 (exact) but for bf16 results of 33 to 64 rows, where the
+// 8-bit instruction gains what it loses bits for: 64 x 8192 -> 8192 23.1 us for 25.3, 64 x 1024 -> 2560
+// 7.4 for 7.7; of fewer rows it gains nothing (16 x 2560 -> 1024 6.3 both, 1 x 4096 -> 4096 8.6 for 8.3)
+// to 4 % (1 x 8192 -> 28672 48.4 for 49.4, one row of bf16, 1024 -> 2560, 7.7 for 8.0).
 template <int XT, int OT, int RT>
 __global__ void __launch_bounds__(512) fb_stream_kernel(FbArgs p, int64_t K) {
   constexpr int NW = 8, U = 2;  // blocks read at once
@@ -1006,7 +1010,7 @@ __global__ void __launch_bounds__(512) fb_stream_kernel(FbArgs p, int64_t K) {
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-          if constexpr (OT == O_F32 || GATED) {  // exact
+          if constexpr (OT == O_F32 || GATED || RT == 1) {  // exact
 #pragma unroll
             for (int q = 0; q < 4; ++q)
               acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(

@@ -746,8 +746,9 @@ class RocmBackend:
         """y [..., out_f] = Q(x) . W^T, W the weight that codes w [out_f, 128 n] and scales s
         stand for (``fp8_block_quantize``).  x [..., in_f] fp32 or bf16 is rounded to the
         format; with scales ``xs`` it is codes already.  ``dtype`` of y: fp32 or bf16, by
-        default x's, of codes bf16.  Products are exact, sums fp32; towards bf16, 8
-        neighbouring products may be summed with the last bit 2^-13 of the largest's."""
+        default x's, of codes bf16.  Products are exact, sums fp32; towards bf16, from
+        33 rows on, 8 neighbouring products may be summed with the last bit 2^-13 of the
+        largest's."""
         lib = _lib.load()
         _need_one_device("fp8_block_forward", x, xs, w, s)
         if in_f < 1 or out_f < 1:

@@ -113,6 +113,23 @@ def test_forward_of_many_rows_in_fp32(rows, K, N):
     assert bool(((y[:50].double() - few.double()).abs() <= bound).all())
 
 
+@pytest.mark.parametrize("rows,K", [(1, 300), (8, 300), (16, 1000), (17, 300), (32, 2000)])
+def test_products_of_few_rows_are_exact(rows, K):
+    """Two large products that cancel, each among seven of 2^-15 of it: the sum of the small ones is
+    left, whatever the result's type (their sum is short enough for fp32 and bf16)."""
+    x = torch.zeros(rows, K)
+    x[:, :16] = 2.0 ** -7
+    x[:, 0], x[:, 8] = 256.0, -256.0
+    x *= (2.0 ** torch.arange(rows).remainder(5))[:, None]
+    want = x[:, :16].double().sum(-1, keepdim=True).expand(-1, 40)
+    w = torch.zeros(40, K)
+    w[:, :16] = 1.0
+    w, s = ref.quantize(w)
+    for dtype in (BF, F32):
+        y = be().fp8_block_forward(x.to(dtype).to(DEV), w.to(DEV), s.to(DEV), K, 40)
+        assert torch.equal(y.cpu().double(), want)
+
+
 def test_forward_layouts_and_leading_dimensions():
     K, N = 200, 96
     g = gen(1)
