@@ -643,9 +643,11 @@ int smaul_fp8_block_ffn_forward(const void* x, int x_dtype, const uint8_t* xs, c
 /*
  * Its gradients, straight through the roundings, all bf16: dx[T, d] (or NULL), dgate and
  * dup [h, d], ddown [d, h] (or all three NULL) from dy[T, d]; the codes are the forward's.
- * With T == 0 the weights' gradients are 0.
+ * With T == 0 the weights' gradients are 0.  The workspace: for all gradients, or for dx
+ * and the weights' (dw) as asked for, each 0 or 1.  The codes may be NULL without dw.
  */
 int64_t smaul_fp8_block_ffn_backward_workspace_size(int64_t T, int64_t d, int64_t h);
+int64_t smaul_fp8_block_ffn_backward_part_workspace_size(int64_t T, int64_t d, int64_t h, int dx, int dw);
 int smaul_fp8_block_ffn_backward(const void* dy, const uint8_t* gate_w, const uint8_t* gate_s, const uint8_t* up_w,
                                  const uint8_t* up_s, const uint8_t* down_w, const uint8_t* down_s,
                                  const uint8_t* x_codes, const uint8_t* x_scales, const uint8_t* h_codes,

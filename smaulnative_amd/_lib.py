@@ -97,6 +97,7 @@ SIGNATURES = {
     "smaul_fp8_block_ffn_workspace_size": (_I64, [_I64, _I64, _I64, _I, _I]),
     "smaul_fp8_block_ffn_forward": (_I, [_P, _I] + [_P] * 13 + [_I64, _I64, _I64, _P, _I64, _P]),
     "smaul_fp8_block_ffn_backward_workspace_size": (_I64, [_I64, _I64, _I64]),
+    "smaul_fp8_block_ffn_backward_part_workspace_size": (_I64, [_I64, _I64, _I64, _I, _I]),
     "smaul_fp8_block_ffn_backward": (_I, [_P] * 16 + [_I64, _I64, _I64, _P, _I64, _P]),
     "smaul_add_rms_norm": (_I, [_P, _P, _I, _P, ctypes.c_float, _P, _P, _P, _I64, _I64, _P]),
     "smaul_add_rms_norm_backward_workspace_size": (_I64, [_I64, _I64]),

@@ -1697,6 +1697,11 @@ int64_t smaul_fp8_block_ffn_backward_workspace_size(int64_t T, int64_t d, int64_
   return ffn_back_parts(T, d, h, true, true).total;
 }
 
+int64_t smaul_fp8_block_ffn_backward_part_workspace_size(int64_t T, int64_t d, int64_t h, int dx, int dw) {
+  if (T < 0 || d <= 0 || h <= 0) return -1;
+  return ffn_back_parts(T, d, h, dx != 0, dw != 0).total;
+}
+
 int smaul_fp8_block_ffn_backward(const void* dy, const uint8_t* gate_w, const uint8_t* gate_s, const uint8_t* up_w,
                                  const uint8_t* up_s, const uint8_t* down_w, const uint8_t* down_s,
                                  const uint8_t* x_codes, const uint8_t* x_scales, const uint8_t* h_codes,

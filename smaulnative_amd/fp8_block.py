@@ -221,6 +221,8 @@ class _FFN(torch.autograd.Function):
         y = be.fp8_block_ffn_forward(rows, codes, d, h, xs=xs, save=need)
         if need:
             y, saved = y
+            if not trainable:  # only the weights' gradients read the codes
+                saved = (None, None, None, None, saved[4])
             ctx.dims, ctx.xtype, ctx.wtype = (d, h, eps), x.dtype, None if norm_weight is None else norm_weight.dtype
             ctx.save_for_backward(s, norm_weight, *codes, *saved)
         y = y.to(x.dtype if x.is_floating_point() else torch.float32)

@@ -837,7 +837,8 @@ class RocmBackend:
     def fp8_block_ffn_backward(self, dy, weights, saved, d, h, need_dx=True, need_dw=True):
         """(dx [..., d], dgate [h, d], dup [h, d], ddown [d, h]), bf16, of
         ``fp8_block_ffn_forward`` from dy [..., d] (bf16), its weights and what it saved,
-        straight through the roundings; None for what is not asked for."""
+        straight through the roundings; None for what is not asked for.  Without ``need_dw``
+        the codes in saved may be None: only the weights' gradients read them."""
         lib = _lib.load()
         _need_one_device("fp8_block_ffn_backward", dy, *weights, *saved)
         weights = self._block_weights("fp8_block_ffn_backward", weights, d, h)
@@ -847,19 +848,23 @@ class RocmBackend:
         if len(saved) != 5 or saved[4].dtype != torch.uint8 or \
                 saved[4].numel() != lib.smaul_fp8_block_ffn_saved_size(T, h):
             raise RuntimeError(f"fp8_block_ffn_backward: saved is of another call than one of {T} rows")
-        xc, xs = self._block_check("fp8_block_ffn_backward", saved[0], saved[1], tuple(saved[0].shape[:-1]), d)
-        hc, hs = self._block_check("fp8_block_ffn_backward", saved[2], saved[3], (T,), h)
-        if xs.numel() // xs.shape[-1] != T:
-            raise RuntimeError(f"fp8_block_ffn_backward: saved is of another call than one of {T} rows")
+        held = [None] * 4
+        if need_dw or all(t is not None for t in saved[:4]):
+            if any(t is None for t in saved[:4]):
+                raise RuntimeError("fp8_block_ffn_backward: the weights' gradients need the codes in saved")
+            held = [*self._block_check("fp8_block_ffn_backward", saved[0], saved[1], tuple(saved[0].shape[:-1]), d),
+                    *self._block_check("fp8_block_ffn_backward", saved[2], saved[3], (T,), h)]
+            if held[1].numel() // held[1].shape[-1] != T:
+                raise RuntimeError(f"fp8_block_ffn_backward: saved is of another call than one of {T} rows")
         kept = self._aligned(saved[4])
         dx = torch.empty(*lead, d, dtype=torch.bfloat16, device=dev) if need_dx else None
         dw = [torch.empty(n, k, dtype=torch.bfloat16, device=dev) if need_dw else None
               for n, k in ((h, d), (h, d), (d, h))]
-        nws = lib.smaul_fp8_block_ffn_backward_workspace_size(T, d, h)
+        nws = lib.smaul_fp8_block_ffn_backward_part_workspace_size(T, d, h, need_dx, need_dw)
         ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws > 0 else None
         with _device(dev):
-            rc = lib.smaul_fp8_block_ffn_backward(dyc.data_ptr(), *[t.data_ptr() for t in weights], xc.data_ptr(),
-                                                  xs.data_ptr(), hc.data_ptr(), hs.data_ptr(), kept.data_ptr(),
+            rc = lib.smaul_fp8_block_ffn_backward(dyc.data_ptr(), *[t.data_ptr() for t in weights],
+                                                  *[None if t is None else t.data_ptr() for t in held], kept.data_ptr(),
                                                   *[None if t is None else t.data_ptr() for t in (dx, *dw)], T, d, h,
                                                   None if ws is None else ws.data_ptr(), nws, _stream_handle(dev))
         _lib.check(rc, "fp8_block_ffn_backward")

@@ -102,6 +102,22 @@ def test_block_arguments():
     assert bwd(nb=need - 1) == BAD and bwd(ws=P + 64) == BAD
 
 
+def test_block_backward_workspace_of_what_is_asked_for():
+    lib = _lib.load()
+    size = lib.smaul_fp8_block_ffn_backward_part_workspace_size
+    assert size(-1, 64, 96, 1, 1) == size(70, 0, 96, 1, 1) == size(70, 64, 0, 1, 1) == -1
+    for T, d, h in ((70, 64, 96), (300, 130, 1000)):
+        every = lib.smaul_fp8_block_ffn_backward_workspace_size(T, d, h)
+        need = {(dx, dw): size(T, d, h, dx, dw) for dx in (0, 1) for dw in (0, 1)}
+        assert need[1, 1] == every and need[1, 0] < every and need[0, 1] < every
+        # dx alone: no copy of x's, dy's, h's rows, dg or du turned round
+        assert need[1, 0] <= every - 2 * T * (2 * d + 3 * h)
+        for dx, dw in ((1, 0), (0, 1), (1, 1)):
+            w = P if dw else None
+            assert lib.smaul_fp8_block_ffn_backward(P, P, P, P, P, P, P, *[w] * 4, P, P if dx else None, w, w, w, T, d, h, P,
+                                                    need[dx, dw] - 1, None) == BAD
+
+
 def test_norm_arguments():
     lib = _lib.load()
 

@@ -6,7 +6,7 @@ import torch.nn as nn
 
 import _fp8_block as ref
 from smaulnative_amd import AddRMSNorm, FP8BlockFFN, FP8BlockLinear, FP8BlockNormFFN, FP8Linear, SwiFFN, MoEConfig
-from smaulnative_amd import fp8_block
+from smaulnative_amd import _lib, fp8_block
 from smaulnative_amd.compute import get_backend
 
 pytestmark = pytest.mark.gpu
@@ -284,6 +284,34 @@ def test_block_layer(T, trainable):
             ref.check(g, *want["d" + name])
     with torch.no_grad():
         assert torch.equal(m(x), y)
+
+
+def test_memory_of_a_frozen_block():
+    """Its pass keeps the factors (6 bytes a hidden value) beside its input and output, and its
+    gradient makes room for dx alone."""
+    T, d, h, slack = 2048, 256, 2048, 1 << 21
+    m = FP8BlockFFN(d, h).to(DEV)
+    x = torch.randn(T, d, device=DEV).to(BF).requires_grad_()
+    dy = torch.randn(T, d, device=DEV).to(BF)
+    want = torch.autograd.grad(m(x), x, dy)[0]
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y = m(x)
+    held = torch.cuda.memory_allocated() - before
+    assert 6 * T * h <= held <= 6 * T * h + 2 * T * d + slack
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    assert torch.equal(torch.autograd.grad(y, x, dy)[0], want)
+    # dg and du, the three weights turned round, dx in slices and itself
+    need = _lib.load().smaul_fp8_block_ffn_backward_part_workspace_size(T, d, h, 1, 0)
+    assert torch.cuda.max_memory_allocated() - before <= need + 2 * T * d + slack
+    # and the codes are asked for where weights' gradients are
+    w = [getattr(m, n) for n in m._NAMES]
+    _, saved = be().fp8_block_ffn_forward(x.detach(), w, d, h, save=True)
+    bare = (None, None, None, None, saved[4])
+    assert torch.equal(be().fp8_block_ffn_backward(dy, w, bare, d, h, need_dw=False)[0], want)
+    with pytest.raises(RuntimeError, match="need the codes"):
+        be().fp8_block_ffn_backward(dy, w, bare, d, h)
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
