@@ -165,6 +165,7 @@ class _AddRMSNorm(torch.autograd.Function):
         s, y = get_backend().add_rms_norm(x, residual, weight, eps)
         ctx.eps, ctx.wtype = eps, None if weight is None else weight.dtype
         ctx.save_for_backward(s, weight)
+        ctx.set_materialize_grads(False)  # a sum that nothing uses has no gradient to read
         if residual is None:
             s = s.view_as(s)  # an output of its own
         return y, s
@@ -174,7 +175,9 @@ class _AddRMSNorm(torch.autograd.Function):
     def backward(ctx, dy, ds):
         s, weight = ctx.saved_tensors
         need_dw = weight is not None and ctx.needs_input_grad[2]
-        dx, dw = get_backend().add_rms_norm_backward(dy.to(s.dtype), s, weight, ctx.eps, ds.to(s.dtype), need_dw)
+        dy = torch.zeros_like(s) if dy is None else dy.to(s.dtype)
+        ds = None if ds is None else ds.to(s.dtype)
+        dx, dw = get_backend().add_rms_norm_backward(dy, s, weight, ctx.eps, ds, need_dw)
         return dx, dx if ctx.needs_input_grad[1] else None, dw.to(ctx.wtype) if need_dw else None, None
 
 
@@ -225,6 +228,7 @@ class _FFN(torch.autograd.Function):
                 saved = (None, None, None, None, saved[4])
             ctx.dims, ctx.xtype, ctx.wtype = (d, h, eps), x.dtype, None if norm_weight is None else norm_weight.dtype
             ctx.save_for_backward(s, norm_weight, *codes, *saved)
+            ctx.set_materialize_grads(False)
         y = y.to(x.dtype if x.is_floating_point() else torch.float32)
         if eps is None:
             return y
@@ -239,12 +243,14 @@ class _FFN(torch.autograd.Function):
         need_dw = ctx.wtypes is not None and any(ctx.needs_input_grad[8:])
         need_norm = norm_weight is not None and ctx.needs_input_grad[2]
         need_dx = ctx.needs_input_grad[0] or ctx.needs_input_grad[1] or need_norm
-        dx, *dw = be.fp8_block_ffn_backward(dy.to(torch.bfloat16), codes, saved, d, h, need_dx, need_dw)
+        dy = torch.zeros_like(s, dtype=torch.bfloat16) if dy is None else dy.to(torch.bfloat16)
+        dx, *dw = be.fp8_block_ffn_backward(dy, codes, saved, d, h, need_dx, need_dw)
         dn = None
         if need_dx:
             dx = dx.to(ctx.xtype)
             if eps is not None:
-                dx, dn = be.add_rms_norm_backward(dx, s, norm_weight, eps, ds.to(s.dtype), need_norm)
+                ds = None if ds is None else ds.to(s.dtype)
+                dx, dn = be.add_rms_norm_backward(dx, s, norm_weight, eps, ds, need_norm)
         dw = [g.to(t) for g, t in zip(dw, ctx.wtypes)] if need_dw else [None] * (3 if ctx.wtypes is not None else 6)
         return (dx if ctx.needs_input_grad[0] else None, dx if ctx.needs_input_grad[1] else None,
                 dn.to(ctx.wtype) if need_norm else None, None, None, None, None, None, *dw)

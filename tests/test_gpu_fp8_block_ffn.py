@@ -286,6 +286,33 @@ def test_block_layer(T, trainable):
         assert torch.equal(m(x), y)
 
 
+@pytest.mark.parametrize("residual", [True, False])
+@pytest.mark.parametrize("layer", [lambda: AddRMSNorm(136), lambda: FP8BlockNormFFN(136, 200, True), lambda: FP8BlockNormFFN(136, 200)])
+def test_an_output_that_nothing_uses(layer, residual, monkeypatch):
+    """Its gradient is zeros, which for the sum are neither filled in nor read."""
+    torch.manual_seed(0)
+    m = layer().to(DEV)
+    x, r = (torch.randn(20, 136, device=DEV).to(BF).requires_grad_() for _ in range(2))
+    inputs = [x, *([r] if residual else []), *m.parameters()]
+    dy, ds = (torch.randn(20, 136, device=DEV).to(BF) for _ in range(2))
+    seen, entry = [], type(be()).add_rms_norm_backward
+
+    def look(self, dy, s, weight=None, eps=1e-6, ds=None, need_dw=True):
+        seen.append(ds)
+        return entry(self, dy, s, weight, eps, ds, need_dw)
+
+    monkeypatch.setattr(type(be()), "add_rms_norm_backward", look)
+    y, s = m(x, r if residual else None)
+    got = torch.autograd.grad(y, inputs, dy)
+    assert seen == [None]
+    y, s = m(x, r if residual else None)
+    want = torch.autograd.grad([y, s], inputs, [dy, torch.zeros_like(s)])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    y, s = m(x, r if residual else None)
+    got = torch.autograd.grad(s, inputs, ds)
+    assert torch.equal(got[0], ds) and not any(t.any() for t in got[1 + residual:])
+
+
 def test_memory_of_a_frozen_block():
     """Its pass keeps the factors (6 bytes a hidden value) beside its input and output, and its
     gradient makes room for dx alone."""
