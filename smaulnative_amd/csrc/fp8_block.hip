@@ -1467,13 +1467,16 @@ FfnBackParts ffn_back_parts(int64_t T, int64_t d, int64_t h, bool dx, bool dw) {
 // CUs takes in two steps a wave.  There the two launches (or three, in slices) wait for one
 // another longer than the weight's being turned by each group of rows takes (us, by way of
 // the turned weight and so: 512 x 777 -> 1000 fp32 22.5 and 13.5, 2048 x 256 -> 256 13.1 and
-// 8.8, 128 x 1024 -> 2560 bf16 13.4 and 9.5; past it 500 x 1024 -> 2560 bf16 14 and 25).  fp32
-// rows, whose thirds take longer than the weight, have 64 columns a workgroup where that makes
-// one round of two (1001 x 777 -> 1000 26.3, so 18.6, of 32 columns 24.2; bf16 13.7 and 15.8),
-// but 32 where these are one (512 rows 13.5 for 15.7).
+// 8.8, 128 x 1024 -> 2560 bf16 13.4 and 9.5; past it 500 x 1024 -> 2560 bf16 14 and 25, in two rounds
+// 3816 x 383 -> 159 bf16 11.3 and 19.7, 1078 x 205 -> 1019 fp32 15.3 and 22.8).  fp32 rows, whose
+// thirds take longer than the weight, have 64 columns a workgroup where 32 take two rounds
+// (2934 x 318 -> 293 17.4 by way of the turned weight, so 13.1, of 32 columns 17.4; 653 x 470 -> 1135
+// 21.4, 14.0 and 18.2; at the edge, 256 workgroups, 1001 x 777 -> 1000 26.3, 18.6 and 24.2; past it
+// 2804 x 315 -> 379 18.1 and 21.1; of as few outputs as 64, 205 x 64 -> 2738, 9.3 and 10.3), but 32
+// where these are one round (512 rows 13.5 for 15.7).
 int64_t dx_groups(int64_t rows, int64_t in_f, int columns) { return (in_f + columns - 1) / columns * ((rows + 63) / 64); }
 bool dx_fits(int64_t rows, int64_t in_f, int64_t out_f, int columns) {
-  return (dx_groups(rows, in_f, columns) + cu_count() - 1) / cu_count() * (((out_f + 63) / 64 + 7) / 8) <= 2;
+  return dx_groups(rows, in_f, columns) <= cu_count() && ((out_f + 63) / 64 + 7) / 8 <= 2;
 }
 bool dx_wide(int64_t rows, int64_t in_f, int64_t out_f, bool f32) {
   return f32 && rows > FB_FEW && !dx_fits(rows, in_f, out_f, 32) && dx_fits(rows, in_f, out_f, 64);

@@ -221,6 +221,20 @@ def test_backward_input_by_either_way(rows, K, N):
         assert torch.equal(dx, bad)
 
 
+# one workgroup a CU and one more, of 32 and of 64 columns (256 CUs), and two rounds of them
+@pytest.mark.parametrize("rows,K,N", [(1024, 510, 300), (1024, 520, 300), (1000, 1024, 600), (1030, 1010, 600), (2200, 140, 470),
+                                      (1790, 70, 880), (3800, 380, 150), (70, 8192, 65), (200, 4090, 1024)])
+def test_backward_input_about_one_round(rows, K, N):
+    g = gen(rows)
+    w, s = ref.weight(N, K, g)
+    wv = ref.values(w, s, K).t().contiguous()
+    dy = torch.randn(rows, N, generator=g)
+    for dtype in (BF, F32):
+        t = dy.to(dtype)
+        dx = be().fp8_block_backward_input(t.to(DEV), w.to(DEV), s.to(DEV), K, N)
+        ref.check(dx, *ref.product(t.double(), wv, dtype), (rows, K, N, dtype))
+
+
 def room(bytes_):
     free = torch.cuda.mem_get_info()[0]
     if free < bytes_:
