@@ -262,7 +262,7 @@ add_rms_norm_backward_wide_kernel(const void* __restrict__ dy, const void* __res
   __shared__ double red[4];
   const int wave = threadIdx.x >> 6;
   const int64_t chunks = (d + 7) / 8;
-  for (int64_t c0 = 0; c0 < chunks; c0 += CH * 256) {  // of dw's columns
+  for (int64_t c0 = 0; c0 < (part ? chunks : 1); c0 += CH * 256) {  // of dw's columns, the first with dx
     float acc[CH][8];
 #pragma unroll
     for (int i = 0; i < CH; ++i)
