@@ -37,16 +37,9 @@ __device__ __forceinline__ double inv_root(double m) {
   return r * (1.5 - 0.5 * m * r * r);
 }
 
-// A row's 1 / rms as r k, k the power of two with which values of the largest rows stay in
-// the middle of fp32: k v r is v / rms, and neither k v nor r is subnormal or overflows.
-struct Root {
-  double r;
-  float k;
-};
-__device__ __forceinline__ Root row_root(double ss, int64_t d, float eps) {
-  const double r = inv_root(ss / (double)d + (double)eps);
-  return r < 1e-30 ? Root{r * 0x1p64, 0x1p-64f} : Root{r, 1.0f};
-}
+// (as fp32 it keeps 22 bits for the largest rms there is, 3.4e38: no scaling, which would cost
+// the forward pass 2 us of 92 by a product a value, 13 by a branch)
+__device__ __forceinline__ double row_root(double ss, int64_t d, float eps) { return inv_root(ss / (double)d + (double)eps); }
 
 // of 8 values, in 64 bits
 __device__ __forceinline__ double sum_squares(const float (&v)[8]) {
@@ -67,7 +60,7 @@ __device__ __forceinline__ double sum_products(const float (&w)[8], const float 
 // TB/s.
 //
 // The squares, their sum and the root are in 64 bits (in 32, rows past 1.8e19 would overflow;
-// 2 us of the 93), and the two products with 1 / rms and the weight carry their errors along
+// 1 % of the time, 4 of the gradients'), and the two products with 1 / rms and the weight carry their errors along
 // (1 / rms as two floats): y is off by little more than its own rounding, so that a code is
 // seldom the neighbouring one of what 64 bits give (in 32 bits throughout about one in 250000).
 template <bool BF16, bool CODES, bool NT, int NW, int CH>
@@ -110,8 +103,8 @@ add_rms_norm_kernel(const void* __restrict__ x, const void* __restrict__ r, cons
     if (r && chunk(i) * 8 < d) fb_store8<BF16, NT>(sum, t, d, chunk(i) * 8, v);
     ss += sum_squares(v);
   }
-  const Root root = row_root(row_sum<NW>(ss, red, wave), d, eps);
-  const float rh = (float)root.r, rl = (float)(root.r - (double)rh);
+  const double root = row_root(row_sum<NW>(ss, red, wave), d, eps);
+  const float rh = (float)root, rl = (float)(root - (double)rh);
   auto put = [&](int64_t c, float (&v)[8]) {  // whole blocks of lanes
     if (c >= chunks * 8) return;
     float w[8];
@@ -120,7 +113,7 @@ add_rms_norm_kernel(const void* __restrict__ x, const void* __restrict__ r, cons
     if (weight) fb_load8<false>(weight, 0, d, c, w);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float u = v[j] * root.k, a = u * rh, ae = fmaf(u, rl, fmaf(u, rh, -a));
+      const float a = v[j] * rh, ae = fmaf(v[j], rl, fmaf(v[j], rh, -a));
       const float y = a * w[j], ye = fmaf(ae, w[j], fmaf(a, w[j], -y)), z = y + ye;
       v[j] = z == z ? z : y;  // an infinity has no error to carry
     }
@@ -206,15 +199,14 @@ add_rms_norm_backward_kernel(const void* __restrict__ dy, const void* __restrict
       }
     }
     if (t >= T) continue;  // a last row that is not there
-    const Root root = row_root(ss, d, eps);
-    const float rstd = (float)root.r, dot = (float)(sd / (double)d * root.r * root.r * (double)root.k);
+    const double root = row_root(ss, d, eps);
+    const float rstd = (float)root, dot = (float)(sd / (double)d * root * root);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float u = v[i][j] * root.k;
-        acc[i][j] = fmaf(g[i][j], u * rstd, acc[i][j]);
-        o[i][j] += (w[i][j] * g[i][j] - u * dot) * rstd * root.k;
+        acc[i][j] = fmaf(g[i][j], v[i][j] * rstd, acc[i][j]);
+        o[i][j] += (w[i][j] * g[i][j] - v[i][j] * dot) * rstd;
       }
       if (col(i) < d) fb_store8<BF16>(dx, t, d, col(i), o[i]);
     }
@@ -280,9 +272,8 @@ add_rms_norm_backward_wide_kernel(const void* __restrict__ dy, const void* __res
         ss += sum_squares(v);
         sd += sum_products(w, g, v);
       }
-      const Root root = row_root(row_sum<4>(ss, red, wave), d, eps);
-      const float rstd = (float)root.r;
-      const float dot = (float)(row_sum<4>(sd, red, wave) / (double)d * root.r * root.r * (double)root.k);
+      const double root = row_root(row_sum<4>(ss, red, wave), d, eps);
+      const float rstd = (float)root, dot = (float)(row_sum<4>(sd, red, wave) / (double)d * root * root);
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int64_t c = c0 + i * 256 + threadIdx.x;
@@ -291,7 +282,7 @@ add_rms_norm_backward_wide_kernel(const void* __restrict__ dy, const void* __res
           fb_load8<BF16>(s, t, d, c * 8, v);
           fb_load8<BF16>(dy, t, d, c * 8, g);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(g[j], v[j] * root.k * rstd, acc[i][j]);
+          for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(g[j], v[j] * rstd, acc[i][j]);
         }
       }
       for (int64_t c = threadIdx.x; c0 == 0 && c < chunks; c += 256) {
@@ -306,7 +297,7 @@ add_rms_norm_backward_wide_kernel(const void* __restrict__ dy, const void* __res
         if (weight) fb_load8<false>(weight, 0, d, c * 8, w);
         if (ds) fb_load8<BF16>(ds, t, d, c * 8, o);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] += (w[j] * g[j] - v[j] * root.k * dot) * rstd * root.k;
+        for (int j = 0; j < 8; ++j) o[j] += (w[j] * g[j] - v[j] * dot) * rstd;
         fb_store8<BF16>(dx, t, d, c * 8, o);
       }
     }
