@@ -56,8 +56,8 @@ __device__ __forceinline__ double sum_products(const float (&w)[8], const float 
 }
 
 // A row is NW waves', a lane has 8 values of every NW * 512, the first CH of them kept in
-// registers (the rest are read again).  Memory bounds it: 32768 x 2048 bf16 to codes 93 us, 5.1
-// TB/s.
+// registers (the rest are read again).  Memory bounds it: 32768 x 2048 bf16 to codes 97 us, 4.9
+// TB/s, to rows 94.
 //
 // The squares, their sum and the root are in 64 bits (in 32, rows past 1.8e19 would overflow;
 // 1 % of the time, 4 of the gradients'), and the two products with 1 / rms and the weight carry their errors along
@@ -135,7 +135,7 @@ add_rms_norm_kernel(const void* __restrict__ x, const void* __restrict__ r, cons
 // sums and dx, the next row's are on their way meanwhile, and a workgroup's share of dw
 // stays until its rows (blockIdx.x * ROWS, + gridDim.x * ROWS, ...) are done;
 // norm_weight_sum_kernel adds the shares in their order.  d is no more than NW * CH * 512.
-// Memory bounds it: 16384 x 2048 bf16 49 us, 5.5 TB/s (178 with the rows read again).
+// Memory bounds it: 16384 x 2048 bf16 57 us, 4.7 TB/s (50 without dw; 178 with the rows read again).
 template <bool BF16, int NW, int CH>
 __global__ void __launch_bounds__(256)
 add_rms_norm_backward_kernel(const void* __restrict__ dy, const void* __restrict__ s, const void* __restrict__ ds,
@@ -330,10 +330,11 @@ norm_weight_sum_kernel(const float* __restrict__ part, float* __restrict__ dw, i
   }
 }
 
-// workgroups of the backward pass, each with a part of dw: four a CU (16384 x 2048 49 us, of
-// two a CU 66, of eight 52)
+// workgroups of the backward pass, each with a part of dw: as many as run, four a CU, of 2049
+// to 4096 columns two (16384 x 2048 62 us, of two a CU 82, of eight 68; 8192 x 4096 78, of four 90)
 int64_t norm_parts(int64_t T, int64_t d) {
-  const int64_t rows = d <= 512 ? (T + 3) / 4 : d <= 1024 ? (T + 1) / 2 : T, most = 4 * cu_count();
+  const int64_t rows = d <= 512 ? (T + 3) / 4 : d <= 1024 ? (T + 1) / 2 : T;
+  const int64_t most = (d > 2048 && d <= 4096 ? 2 : 4) * (int64_t)cu_count();
   return rows < most ? rows : most;
 }
 

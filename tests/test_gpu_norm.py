@@ -67,6 +67,17 @@ def test_backward(T, d, dtype):
             assert none is None and torch.equal(only, got)
 
 
+@pytest.mark.parametrize("T,d", [(700, 2049), (1100, 4096), (530, 4097)])
+def test_backward_of_more_rows_than_workgroups(T, d):
+    """Wide rows in several turns of a workgroup, their shares of the weight's gradient joined."""
+    x, _, w, g = inputs(T, d, BF, 5)
+    dy = torch.randn(T, d, generator=g).to(BF)
+    (dx, dxe), (dw, dwe) = ref.norm_grad(dy.double(), x.double(), w.double(), EPS, None, BF)
+    got, gw = be().add_rms_norm_backward(dy.to(DEV), x.to(DEV), w.to(DEV), EPS)
+    ref.check(got, dx, dxe, (T, d))
+    ref.check(gw, dw, dwe, (T, d))
+
+
 def test_gradient_against_differences():
     """Central differences of the norm in 64 bits: truncation h^2 times the third derivative
     (of a function of values near 1, order 1) and rounding 2^-53 / h, h = 1e-5; fp32's own
