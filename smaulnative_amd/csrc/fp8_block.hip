@@ -23,8 +23,10 @@ namespace {
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 // ---------------------------------------------------------------------------
-// quantisation: 16 lanes a block, 8 values a lane.  Memory bounds both ways: 32768 x 2048
-// codes read back to bf16 31 us, 6.4 TB/s (the codes from the last cache)
+// quantisation: 16 lanes a block, 8 values a lane.  Memory bounds it both ways: 32768 x 2048
+// bf16 to codes 34 us, 5.9 TB/s, of fp32 55, 6.1; codes read back to bf16 31 us, 6.4 TB/s (the
+// codes from the last cache).  8192 x 1024 bf16 5.8 us, 4.4 TB/s: a launch and two rounds of
+// the workgroups that run at once, one chain of loads each.
 // ---------------------------------------------------------------------------
 // chunk i of rows of n: its row and place in it (a 64-bit division takes as long as the loads)
 __device__ __forceinline__ void fb_place(int64_t i, int64_t n, int64_t rows, int64_t& row, int64_t& c) {
@@ -219,14 +221,19 @@ __device__ __forceinline__ void fb_tile_at(int lin, int m_tiles, int n_tiles, in
 // in the mean, a hundredth of bf16's own rounding.  fp32 results are not formed so, nor
 // hidden rows as long as they are few, of which a value or a block's scale that is rounded
 // to its other neighbour is seen in the block's output: their codes are decoded (exactly)
-// and multiplied as bf16, at half the rate.  The operands of a step (64 values) are read while the step before is
-// multiplied, the first of a stage during the last of the stage before; by then every
-// wave has the rest of its stage in registers, so that one barrier frees the buffer for
-// the loads of the stage after the next.  A workgroup walks a band of tiles as one
-// sequence of stages.
+// and multiplied as bf16, at half the rate (16384 x 2048 -> 5120 to fp32 275 us, 1.25 PFLOP/s).
+//
+// The operands of a step (64 values) are read while the step before is multiplied, the first
+// of a stage during the last of the stage before; by then every wave has the rest of its
+// stage in registers, so that one barrier frees the buffer for the loads of the stage after
+// the next.  A workgroup walks a band of tiles as one sequence of stages.
 // Several products of one K (G of them) share the launch, one after the other in the band.
-// 16384 x 2048 -> 5120 codes to bf16: 134 us, 2.6 PFLOP/s, where the instruction alone reaches 4.0 on
-// such values (and 4.9 on zeros: power bounds it).  bf16, 8192 x 5120 -> 1024: 90 us, 950 TFLOP/s.
+//
+// 16384 x 2048 -> 5120 codes to bf16: 134 us, 2.6 PFLOP/s (many in a row 160: power).  Of a 256 x
+// 256 tile's 29 us the 16 stages are 24.5, 2.8 PFLOP/s, where the instruction alone reaches 4.0 on
+// such values (and 4.9 on zeros): one wave a SIMD, to which a stage's two barriers and waits are
+// exposed; the epilogue is the rest.  bf16, 8192 x 5120 -> 1024: 73 us, 1.2 PFLOP/s of 1.95, in a
+// training step, warm, 86.
 template <int G>
 struct FbBatch {
   FbArgs p[G];

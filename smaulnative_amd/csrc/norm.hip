@@ -60,9 +60,11 @@ __device__ __forceinline__ double sum_products(const float (&w)[8], const float 
 // TB/s, to rows 94.
 //
 // The squares, their sum and the root are in 64 bits (in 32, rows past 1.8e19 would overflow;
-// 1 % of the time, 4 of the gradients'), and the two products with 1 / rms and the weight carry their errors along
-// (1 / rms as two floats): y is off by little more than its own rounding, so that a code is
-// seldom the neighbouring one of what 64 bits give (in 32 bits throughout about one in 250000).
+// 1 % of the time, 4 of the gradients'), and the two products with 1 / rms and the weight carry
+// their errors along (1 / rms as two floats): y is off by little more than its own rounding, so that a code is
+// seldom the neighbouring one of what 64 bits give: one in 2 million, where y as fp32 lands on
+// the middle of two codes (in 32 bits throughout about one in 250000; y rounded to odd instead
+// leaves one in 30 million, but takes 5 % of the time, and either code is as near).
 template <bool BF16, bool CODES, bool NT, int NW, int CH>
 __global__ void __launch_bounds__(256)
 add_rms_norm_kernel(const void* __restrict__ x, const void* __restrict__ r, const float* __restrict__ weight,
