@@ -26,9 +26,10 @@ __device__ __forceinline__ float fb_scale(uint32_t byte) {
 }
 
 // From the bits of the largest magnitude: its exponent less 8 (448 = 1.75 * 2^8), one
-// more where its mantissa is past 1.75.  Infinities and NaN have the largest bits: 255.
-__device__ __forceinline__ uint32_t fb_scale_byte(uint32_t amax_bits) {
-  if (amax_bits >= 0x7f800000u) return 255u;
+// more where its mantissa is past 1.75.  Infinities and NaN have the largest bits, from
+// `infinity` on: 255.
+__device__ __forceinline__ uint32_t fb_scale_byte(uint32_t amax_bits, uint32_t infinity = 0x7f800000u) {
+  if (amax_bits >= infinity) return 255u;
   return (uint32_t)max((int)((amax_bits + 0x1fffffu) >> 23) - 8, 0);
 }
 
@@ -152,8 +153,8 @@ __device__ __forceinline__ uint32_t fb_block_max(uint32_t m) {
 // Chunk `chunk` (8 values) of row `row` as codes, called by the 16 lanes of a block at
 // once; the first writes the block's scale, and the last block's the scales past it.
 __device__ __forceinline__ void fb_write8(uint8_t* codes, uint8_t* scales, int64_t row, int64_t nb, int64_t chunk,
-                                          const float (&v)[8]) {
-  const uint32_t byte = fb_scale_byte(fb_block_max(fb_amax8(v)));
+                                          const float (&v)[8], uint32_t infinity = 0x7f800000u) {
+  const uint32_t byte = fb_scale_byte(fb_block_max(fb_amax8(v)), infinity);
   *(uint2*)(codes + row * nb * FB_BLOCK + chunk * 8) = fb_encode8(v, byte);
   if ((chunk & 15) == 0) {
     const int64_t b = chunk / 16, ns = (nb + 3) / 4 * 4;

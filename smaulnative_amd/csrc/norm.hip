@@ -61,10 +61,10 @@ __device__ __forceinline__ double sum_products(const float (&w)[8], const float 
 //
 // The squares, their sum and the root are in 64 bits (in 32, rows past 1.8e19 would overflow;
 // 1 % of the time, 4 of the gradients'), and the two products with 1 / rms and the weight carry
-// their errors along (1 / rms as two floats): y is off by little more than its own rounding, so that a code is
-// seldom the neighbouring one of what 64 bits give: one in 2 million, where y as fp32 lands on
-// the middle of two codes (in 32 bits throughout about one in 250000; y rounded to odd instead
-// leaves one in 30 million, but takes 5 % of the time, and either code is as near).
+// their errors along (1 / rms as two floats).  Towards codes y is rounded to odd, so that one
+// that fp32 would round to the middle of two codes goes to its own side of it: a code is the
+// neighbouring one of what 64 bits give once in 30 million (2 % of the time; y to nearest once
+// in 2 million, in 32 bits throughout in 250000).
 template <bool BF16, bool CODES, bool NT, int NW, int CH>
 __global__ void __launch_bounds__(256)
 add_rms_norm_kernel(const void* __restrict__ x, const void* __restrict__ r, const float* __restrict__ weight,
@@ -116,10 +116,17 @@ add_rms_norm_kernel(const void* __restrict__ x, const void* __restrict__ r, cons
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float a = v[j] * rh, ae = fmaf(v[j], rl, fmaf(v[j], rh, -a));
-      const float y = a * w[j], ye = fmaf(ae, w[j], fmaf(a, w[j], -y)), z = y + ye;
-      v[j] = z == z ? z : y;  // an infinity has no error to carry
+      const float y = a * w[j], ye = fmaf(ae, w[j], fmaf(a, w[j], -y));
+      if constexpr (CODES) {
+        const int less = (int)__float_as_uint(fmaf(ye, y, 0.0f)) >> 31;  // -1: |y + ye| < |y| (never of 0)
+        v[j] = __uint_as_float((__float_as_uint(y) + (uint32_t)less) | 1u);
+      } else {
+        const float z = y + ye;
+        v[j] = z == z ? z : y;  // an infinity has no error to carry
+      }
     }
-    if constexpr (CODES) fb_write8((uint8_t*)out, scales, t, nb, c / 8, v);
+    // (an infinity less one is fp32's largest)
+    if constexpr (CODES) fb_write8((uint8_t*)out, scales, t, nb, c / 8, v, 0x7f7fffffu);
     else if (c < d) fb_store8<BF16, NT>(out, t, d, c, v);
   };
 #pragma unroll

@@ -133,6 +133,28 @@ def test_layouts_and_empty_calls():
     assert same is dev[0] and torch.equal(z, be().add_rms_norm(dev[0], None, torch.ones(200, device=DEV), 1e-6)[1])
 
 
+def test_codes_where_fp32_lands_between_two():
+    """Values whose nearest fp32 number is the middle of two codes: rounded twice, to nearest, half of
+    them would go to the code on the other side.  y + ye, the value to 2^-47, may lie more than a step
+    of fp32 from y (1.5 at most, seldom), and only then the other code is left: less than a quarter."""
+    T, d = 4096, 2048
+    w = (1 + 0.3 * torch.randn(d, generator=torch.Generator().manual_seed(1))).to(DEV)
+    found, other = 0, 0
+    for seed in range(8):
+        x = torch.randn(T, d, generator=torch.Generator(DEV).manual_seed(seed), device=DEV)
+        y = ref.norm(x.double(), w.double(), EPS)[0]
+        middle = (y.float().view(torch.int32) & 0xfffff) == 0x80000
+        middle &= y.abs() > 1e-2  # no subnormal codes
+        rows = middle.any(1).nonzero()[:, 0]
+        codes = be().add_rms_norm(x, None, w, EPS, quantize=True)[1][rows].cpu()
+        want = ref.quantize(y[rows].cpu())[0]
+        at = middle[rows].cpu()
+        found += int(at.sum())
+        other += int((codes[at] != want[at]).sum())
+        assert torch.equal(codes[~at], want[~at])
+    assert found >= 20 and other < found / 4, (other, found)
+
+
 # each width's form; few rows and more than the chip has CUs
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("T,d", [(20, 64), (300, 300), (20, 900), (300, 1500), (20, 3000), (20, 5000), (20, 9001)])
