@@ -56,7 +56,7 @@ __device__ __forceinline__ double sum_products(const float (&w)[8], const float 
 }
 
 // A row is NW waves', a lane has 8 values of every NW * 512, the first CH of them kept in
-// registers (the rest are read again).  Memory bounds it: 32768 x 2048 bf16 to codes 97 us, 4.9
+// registers (the rest are read again).  Memory bounds it: 32768 x 2048 bf16 to codes 99 us, 4.8
 // TB/s, to rows 94.
 //
 // The squares, their sum and the root are in 64 bits (in 32, rows past 1.8e19 would overflow;
